@@ -461,6 +461,91 @@ kvb_status kvb_operational_rd(const float* A, int64_t rows, int64_t n, int64_t l
                               const float* mults, int n_mults, double* D, float* C, void* workspace,
                               size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------ *
+ * The paged path: many sequences of different lengths in one pool.  The reference keeps one dense buffer
+ * per state object (LayerState, STRATA_KV.py:682-720) and attends over it with chunked_attention
+ * (STRATA_KV.py:641-675); these entry points serve the same computations for a batch of growing
+ * sequences.
+ *
+ * Causal attention of packed prompts (or of chunks after their prefixes) with grouped heads: sequence s
+ * has the query rows [cu_q[s], cu_q[s + 1]) and the key rows [cu_k[s], cu_k[s + 1]); its query i sees the
+ * keys j <= i + (key rows - query rows), so a query sees all keys before it when the queries are the last
+ * positions.  A row that sees no key gives zeros and -inf.  q (nq, Hq, d), k and v (nk, Hkv, d) of one dtype
+ * (f16 / bf16) with d in {64, 128} contiguous, the element strides below multiples of 8 and 16-byte aligned
+ * bases; cu_q, cu_k (n + 1) int32 on the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype;
+ * lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written. */
+kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq,
+                                 int Hkv, int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
+                                 int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, int n,
+                                 float scaling, void* out, float* lse, void* stream);
+
+/* A pool of pages of `page` (16, 32, 64 or 128) tokens, device tensors, dense: codes kc, vc (n_pages, Hkv,
+ * page, d) uint8 (16-byte aligned) and scales ks, vs (n_pages, Hkv) float32, a stored value being
+ * (code - 128) * scale; table (n_slots, max_blocks) int32, the pages of each sequence (slot), -1 past its
+ * last; lens (n_slots) int32, its tokens; refs (n_pages) int32, how many sequences hold a page (0: free).
+ * d in {64, 128}.  The page of a token is table[slot][position / page].  Slot numbers, page numbers and row
+ * ranges that do not fit raise status bit 1 and that part of the call is left out. */
+typedef struct kvb_pages {
+    uint8_t* kc;
+    uint8_t* vc;
+    float* ks;
+    float* vs;
+    int32_t* table;
+    int32_t* lens;
+    int32_t* refs;
+    int64_t n_pages;
+    int Hkv, d, page, n_slots, max_blocks;
+} kvb_pages;
+
+/* Room for add[i] more tokens in sequence slots[i] (distinct slots): fresh pages are the lowest free ones in
+ * the order of the list; lens grow; start[i] = the length before.  When a slot is out of range, a row of the
+ * table too short or the pool has too few free pages, nothing changes and every start[i] is -1 (status bit 1
+ * or 4).  slots, add, start: n int32 on the device. */
+kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32_t* add, int n, int32_t* start, void* stream);
+
+/* Codes of packed rows: the rows [cu[i], cu[i + 1]) of k and v (rows, Hkv, d) go to the positions start[i],
+ * start[i] + 1, ... of sequence slots[i] (start[i] < 0: left out).  Per (page, head) and side, s = max |x| / 127 over
+ * the page's rows so far (non-finite values left out; 0 where the maximum is below 2^-100), code = clamp(rint(x *
+ * (1 / s)), -127, 127) + 128, NaN as 128.  Rows before the first one written keep the page's scale as long as it
+ * suffices (s = max(old s, new rows)) and are recoded from their codes where it grows, code' = rint((code - 128) *
+ * (old s / s)) + 128.  A page that several sequences hold is not written (status bit 1).  dtype f32 / f16 / bf16,
+ * d contiguous, element strides as given. */
+kvb_status kvb_page_write(const kvb_pages* p, const int32_t* slots, const int32_t* start, const int32_t* cu, int n,
+                          const void* k, const void* v, int dtype, int64_t rows, int64_t k_row, int64_t k_head,
+                          int64_t v_row, int64_t v_head, void* stream);
+
+/* The stored values of the same ranges, rounded to dtype: k and v (rows, Hkv, d) dense. */
+kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t* start, const int32_t* cu, int n, void* k,
+                         void* v, int dtype, int64_t rows, void* stream);
+
+/* Attention of the last Tq positions of each sequence over its pages: q (n, Hq, Tq, d) dense (f16 / bf16), query
+ * t of sequence slots[i] sees the keys j <= lens - Tq + t.  out (n, Tq, Hq, d) in q's dtype; lse (n, Tq, Hq)
+ * float32 or null.  A row that sees no key gives zeros and -inf.  workspace: 256-byte aligned, zero-filled once
+ * before its first use and then reused (every call leaves its counters at zero), one per stream that runs
+ * calls concurrently. */
+size_t kvb_page_attend_workspace(const kvb_pages* p, int n, int Hq, int Tq);
+kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
+                           float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Sequence dst[i] becomes a copy of src[i], all from the state before the call (distinct dst; a dst may be a src):
+ * full pages are shared, a partial last page is copied to a fresh page (the lowest ones free before the call, in
+ * the order of the list), what dst held before is released.  src[i] == dst[i] keeps the sequence as it is.  With
+ * too few free pages nothing changes (status bit 4).  workspace 256-byte aligned. */
+size_t kvb_page_fork_workspace(const kvb_pages* p, int n);
+kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
+/* Drops the sequences: references down, rows -1, lens 0. */
+kvb_status kvb_page_free(const kvb_pages* p, const int32_t* slots, int n, void* stream);
+
+/* Moves the live pages with id >= *n_live, in ascending order, into the free pages below, in ascending order, and
+ * renames them in the table; *n_live (device int32) = the number of live pages, which are then the first ones. */
+size_t kvb_page_compact_workspace(const kvb_pages* p);
+kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+
+/* Whole pages, codes and scales: page src[i] over page dst[i] (distinct dst, none of them a src). */
+kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* stream);
+
 /* Build the split-K plan (pure host computation, no CUDA calls) for n_ctas CTAs.  plan_out receives
  * [n_ctas, n_pieces, n_heads, cta_begin[n_ctas + 1], n_pieces x (head, stratum, first chunk, end
  * chunk, slot), head_begin[n_heads + 1]]: pieces in CTA order, each with the slot of its partial;

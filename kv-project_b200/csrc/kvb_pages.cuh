@@ -1,0 +1,473 @@
+// kvb_pages.cuh - the 8-bit paged KV cache: what fills it, reads it back and moves its pages.
+//
+// A page holds `page` consecutive tokens of one sequence for every KV head: codes (Hkv, page, d) uint8 for
+// keys and for values, and one float32 scale per (page, head) and side.  A stored value is
+// (code - 128) * scale; codes lie in [1, 255], so 128 is zero and -127 .. 127 are symmetric.
+//
+//   write    s = max |x| / 127 over the page's rows so far (non-finite x left out; 0 where that maximum is
+//            below 2^-100), code = clamp(rint(x * (1 / s)), -127, 127) + 128, NaN -> 128.  Rows that are
+//            already in the page keep it as long as it suffices: s = max(s_old, s_new rows); where it grows
+//            they are recoded from their codes, code' = rint((code - 128) * (s_old / s)) + 128.  Each
+//            operation is one float32 rounding, so the codes are a function of the writes alone.
+//   extend   pages for sequences that grow; a fresh page is the lowest id whose reference count is zero
+//   fork     a sequence becomes a copy of another: full pages are shared (reference counts), the last
+//            partial page is copied, because it will be written
+//   free     drops a sequence's references
+//   compact  live pages with id >= n_live move, in ascending order, into the holes below, in ascending
+//            order, so that the pool's first n_live pages are the live ones
+//   copy     whole pages, codes and scales
+//
+// All of it moves bytes: the floor is the bytes read and written at the measured copy bandwidth, and for
+// small calls the launches.
+#pragma once
+
+#include "kvb_pages_view.cuh"
+
+namespace kvb {
+
+// The sequence whose packed rows hold virtual page slot x: sequence i owns the slots from
+// cu[i] / page + 2 i on, which are enough for every page that its rows touch (cu[i + 1] - cu[i] rows touch at
+// most that difference / page + 2 pages).  Whole warp; 32-way search, so one round trip for n <= 32.
+__device__ __forceinline__ int touch_sequence(const int32_t* cu, int n, int page, int64_t x, int64_t& slot0) {
+    const int lane = threadIdx.x & 31;
+    int lo = 0, len = n;
+    while (true) {
+        const int step = (len + 31) / 32;
+        const int i = lo + lane * step;
+        const bool le = i < lo + len && int64_t(cu[i] / page) + 2 * int64_t(i) <= x;
+        const int k = 31 - __clz(int(__ballot_sync(0xffffffffu, le) | 1u));
+        lo += k * step;
+        len = min(step, n - lo);
+        if (step == 1) break;
+    }
+    slot0 = int64_t(cu[lo] / page) + 2 * int64_t(lo);
+    return lo;
+}
+
+// One page's part of a packed write or read.
+struct Touch {
+    int64_t page_id;      // < 0: nothing to do
+    int row0, rows;       // rows of the page
+    int64_t token0;       // first packed row
+};
+
+__device__ __forceinline__ Touch find_touch(const PagesView& P, const int32_t* slots, const int32_t* start,
+                                            const int32_t* cu, int n, int64_t rows, int64_t x) {
+    Touch t{-1, 0, 0, 0};
+    int64_t slot0;
+    const int i = touch_sequence(cu, n, P.page, x, slot0);
+    const int a = cu[i], b = cu[i + 1], st = start[i], slot = slots[i];
+    if (st < 0 || b <= a) return t;
+    const int64_t block = st / P.page + (x - slot0);
+    const int64_t lo = imax64(st, block * P.page), hi = imin64(int64_t(st) + (b - a), (block + 1) * P.page);
+    if (lo >= hi) return t;
+    if (a < 0 || b > rows || slot < 0 || slot >= P.n_slots || block >= P.max_blocks) {
+        raise_status(KVB_DEV_BOUNDS);
+        return t;
+    }
+    const int id = P.table[int64_t(slot) * P.max_blocks + block];
+    if (id < 0 || id >= P.n_pages) {
+        raise_status(KVB_DEV_BOUNDS);
+        return t;
+    }
+    t.page_id = id;
+    t.row0 = int(lo - block * P.page);
+    t.rows = int(hi - lo);
+    t.token0 = a + (lo - st);
+    return t;
+}
+
+// max over the block of non-negative floats
+__device__ __forceinline__ float block_max(float v, float* sh) {
+    v = warp_max(v);
+    if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+    __syncthreads();
+    float m = 0.f;
+    for (int w = 0; w < int(blockDim.x >> 5); ++w) m = fmaxf(m, sh[w]);
+    return m;
+}
+
+__device__ __forceinline__ uint8_t code8(float x, float inv) {
+    const float c = x * inv;
+    return uint8_t(int(c != c ? 0.f : fminf(fmaxf(rintf(c), -127.f), 127.f)) + 128);
+}
+
+struct PageRowsParams {
+    PagesView P;
+    const int32_t* slots;
+    const int32_t* start;
+    const int32_t* cu;
+    int n;
+    int64_t rows;
+    const void* x[2];              // k, v
+    int64_t row_stride[2], head_stride[2];
+    void* out[2];                  // read: dense (rows, Hkv, d)
+};
+
+// grid (touch slots, Hkv, 2)
+template <typename T>
+__global__ void page_write_kernel(const __grid_constant__ PageRowsParams A) {
+    __shared__ float sh[32];
+    const PagesView& P = A.P;
+    const int h = blockIdx.y, side = blockIdx.z;
+    const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
+    if (t.page_id < 0) return;
+    if (P.refs[t.page_id] > 1) {               // a page that several sequences hold is not written
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return;
+    }
+    const T* x = static_cast<const T*>(A.x[side]) + t.token0 * A.row_stride[side] + h * A.head_stride[side];
+    uint8_t* codes = (side ? P.vc : P.kc) + (t.page_id * P.Hkv + h) * int64_t(P.page) * P.d;
+    float* scale = (side ? P.vs : P.ks) + t.page_id * P.Hkv + h;
+    const float old = t.row0 > 0 ? *scale : 0.f;
+    const int total = t.rows * P.d;
+    float a = 0.f;
+    for (int e = threadIdx.x; e < total; e += blockDim.x) {
+        const float v = to_f32(x[(e / P.d) * A.row_stride[side] + e % P.d]);
+        a = fmaxf(a, fabsf(v) < INFINITY ? fabsf(v) : 0.f);
+    }
+    a = block_max(a, sh);
+    const float s = fmaxf(old, a < 0x1p-100f ? 0.f : __fdiv_rn(a, 127.f));
+    if (s > old && old > 0.f) {
+        const float ratio = __fdiv_rn(old, s);
+        for (int e = threadIdx.x; e < t.row0 * P.d; e += blockDim.x)
+            codes[e] = uint8_t(int(rintf(float(int(codes[e]) - 128) * ratio)) + 128);
+    }
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+    for (int e = threadIdx.x; e < total; e += blockDim.x)
+        codes[t.row0 * P.d + e] = code8(to_f32(x[(e / P.d) * A.row_stride[side] + e % P.d]), inv);
+    if (threadIdx.x == 0) *scale = s;          // every thread has read the old one before block_max's barrier
+}
+
+template <typename T>
+__global__ void page_read_kernel(const __grid_constant__ PageRowsParams A) {
+    const PagesView& P = A.P;
+    const int h = blockIdx.y, side = blockIdx.z;
+    const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
+    if (t.page_id < 0) return;
+    const uint8_t* codes = (side ? P.vc : P.kc) + (t.page_id * P.Hkv + h) * int64_t(P.page) * P.d + t.row0 * P.d;
+    const float s = (side ? P.vs : P.ks)[t.page_id * P.Hkv + h];
+    T* out = static_cast<T*>(A.out[side]) + (t.token0 * P.Hkv + h) * P.d;
+    for (int e = threadIdx.x; e < t.rows * P.d; e += blockDim.x)
+        out[int64_t(e / P.d) * P.Hkv * P.d + e % P.d] = from_f32<T>(float(int(codes[e]) - 128) * s);
+}
+
+// ------------------------------------------------------------------------------------------------
+// Page tables.  One block of 1024 threads plans (which pages are free, who gets which), blocks of the
+// following launch move the data.
+// ------------------------------------------------------------------------------------------------
+constexpr int PG_THREADS = 1024;
+constexpr int PG_TILE = 32 * PG_THREADS;       // pages whose state the planning block holds in registers
+
+// Exclusive scan of one int per thread of a PG_THREADS block; total in `sum`.
+__device__ __forceinline__ int block_scan(int v, int* sh, int& sum) {
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) sh[w] = x;
+    __syncthreads();
+    int t = sh[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, t, o);
+        if (lane >= o) t += y;
+    }
+    sum = __shfl_sync(0xffffffffu, t, 31);
+    const int before = w ? __shfl_sync(0xffffffffu, t, w - 1) : 0;
+    return before + x - v;
+}
+
+// Bit mask over the 32 pages tile0 + 1024 warp + 32 lane + 0..31: set where the page is free.  The loads are
+// coalesced (each covers 32 consecutive pages of the warp's 1024) and all in flight together.
+__device__ __forceinline__ uint32_t free_mask(const int32_t* refs, int64_t n_pages, int64_t tile0) {
+    const int lane = threadIdx.x & 31;
+    const int64_t base = tile0 + (threadIdx.x >> 5) * 1024;
+    int r[32];
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const int64_t p = base + i * 32 + lane;
+        r[i] = p < n_pages ? refs[p] : -1;
+    }
+    uint32_t mine = 0;
+#pragma unroll
+    for (int i = 0; i < 32; ++i) {
+        const uint32_t m = __ballot_sync(0xffffffffu, r[i] == 0);
+        if (lane == i) mine = m;
+    }
+    return mine;
+}
+
+// The `total` lowest free pages, in ascending order, to give(rank, page).  False (and nothing given) when the
+// pool has fewer.
+template <typename F>
+__device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh, F give) {
+    if (total == 0) return true;
+    int found = 0, sum = 0, at0 = 0;
+    uint32_t first = 0;
+    for (int64_t t0 = 0; t0 < P.n_pages && found < total; t0 += PG_TILE) {
+        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
+        const int at = block_scan(__popc(m), sh, sum);
+        if (t0 == 0) { first = m; at0 = at; }
+        found += sum;
+    }
+    if (found < total) return false;
+    int before = 0;
+    for (int64_t t0 = 0; t0 < P.n_pages && before < total; t0 += PG_TILE) {
+        uint32_t m = first;
+        int at = at0;
+        if (t0 > 0) {
+            m = free_mask(P.refs, P.n_pages, t0);
+            at = block_scan(__popc(m), sh, sum);
+        } else if (P.n_pages > PG_TILE) {
+            at = block_scan(__popc(m), sh, sum);          // sum of this tile again
+        }
+        int rank = before + at;
+        const int64_t base = t0 + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 32;
+        for (; m && rank < total; m &= m - 1, ++rank) give(rank, int(base + __ffs(m) - 1));
+        before += sum;
+    }
+    return true;
+}
+
+// largest i with off[i] <= r (off ascending, off[0] = 0)
+__device__ __forceinline__ int owner_of(const int* off, int n, int r) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (off[mid] <= r) lo = mid;
+        else hi = mid;
+    }
+    return lo;
+}
+
+// One block.  start[i] = the tokens that sequence slots[i] had, or -1 where the call was refused (a slot out of
+// range, a row too short, not enough free pages): then nothing is changed.
+__global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, const int32_t* slots, const int32_t* add, int n,
+                                                                 int32_t* start) {
+    extern __shared__ int off[];               // off[i]: pages of the sequences before i
+    __shared__ int sh[32];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    int total = 0;
+    for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int need = 0;
+        if (i < n) {
+            const int s = slots[i], a = add[i];
+            const int have = s >= 0 && s < P.n_slots ? P.lens[s] : 0;
+            if (s < 0 || s >= P.n_slots || a < 0 || int64_t(have) + a > int64_t(P.max_blocks) * P.page) bad = 1;
+            else need = blocks_of(have + a, P.page) - blocks_of(have, P.page);
+        }
+        int sum;
+        const int at = block_scan(need, sh, sum);
+        if (i < n) off[i] = total + at;
+        total += sum;
+    }
+    __syncthreads();
+    if (bad) {
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+    } else if (!take_free(P, total, sh, [&](int rank, int id) {
+                   const int i = owner_of(off, n, rank);
+                   const int s = slots[i];
+                   P.table[int64_t(s) * P.max_blocks + blocks_of(P.lens[s], P.page) + rank - off[i]] = id;
+                   P.refs[id] = 1;
+               })) {
+        if (threadIdx.x == 0) { raise_status(KVB_DEV_POOL); bad = 1; }
+    }
+    __syncthreads();                           // the lengths were read by every thread's give()
+    for (int i = threadIdx.x; i < n; i += PG_THREADS) {
+        start[i] = bad ? -1 : P.lens[slots[i]];
+        if (!bad) P.lens[slots[i]] += add[i];
+    }
+}
+
+// One block per sequence.
+__global__ void page_free_kernel(PagesView P, const int32_t* slots) {
+    __shared__ int len;
+    const int s = slots[blockIdx.x];
+    if (s < 0 || s >= P.n_slots) {
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return;
+    }
+    if (threadIdx.x == 0) len = atomicExch(&P.lens[s], 0);          // a slot named twice is freed once
+    __syncthreads();
+    int32_t* row = P.table + int64_t(s) * P.max_blocks;
+    for (int b = threadIdx.x; b < min(blocks_of(len, P.page), P.max_blocks); b += blockDim.x) {
+        const int id = row[b];
+        if (id >= 0 && id < P.n_pages) atomicSub(&P.refs[id], 1);
+        row[b] = -1;
+    }
+}
+
+// Copy one page's codes and scales; whole block.
+__device__ __forceinline__ void copy_page(const PagesView& P, int64_t from, int64_t to, int part, int parts) {
+    const int64_t n16 = int64_t(P.Hkv) * P.page * P.d / 16;
+    const uint4* a[2] = {reinterpret_cast<const uint4*>(P.kc) + from * n16, reinterpret_cast<const uint4*>(P.vc) + from * n16};
+    uint4* b[2] = {reinterpret_cast<uint4*>(P.kc) + to * n16, reinterpret_cast<uint4*>(P.vc) + to * n16};
+    for (int side = 0; side < 2; ++side)
+        for (int64_t i = int64_t(part) * blockDim.x + threadIdx.x; i < n16; i += int64_t(parts) * blockDim.x) b[side][i] = a[side][i];
+    if (part == 0)
+        for (int h = threadIdx.x; h < P.Hkv; h += blockDim.x) {
+            P.ks[to * P.Hkv + h] = P.ks[from * P.Hkv + h];
+            P.vs[to * P.Hkv + h] = P.vs[from * P.Hkv + h];
+        }
+}
+
+// grid (pages, parts)
+__global__ void page_copy_kernel(PagesView P, const int32_t* src, const int32_t* dst) {
+    const int a = src[blockIdx.x], b = dst[blockIdx.x];
+    if (a < 0 || b < 0 || a >= P.n_pages || b >= P.n_pages) {
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return;
+    }
+    if (a != b) copy_page(P, a, b, blockIdx.y, gridDim.y);
+}
+
+// Workspace of a fork: [ok, pad, ...] then per fork: length, fresh page (or -1); then the source rows.
+struct ForkWork {
+    int32_t* head;      // [0]: 1 when the call goes ahead
+    int32_t* len;       // (n)
+    int32_t* fresh;     // (n)
+    int32_t* rows;      // (n, max_blocks)
+};
+
+// One block: lengths and fresh pages of all forks, from the state before any of them.
+__global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, const int32_t* src, const int32_t* dst, int n,
+                                                               ForkWork W) {
+    extern __shared__ int off[];
+    __shared__ int sh[32];
+    __shared__ int bad;
+    if (threadIdx.x == 0) bad = 0;
+    __syncthreads();
+    int total = 0;
+    for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int part = 0;
+        if (i < n) {
+            const int s = src[i], t = dst[i];
+            if (s < 0 || s >= P.n_slots || t < 0 || t >= P.n_slots) bad = 1;
+            else {
+                const int len = P.lens[s];
+                W.len[i] = len;
+                part = s != t && len % P.page != 0;
+            }
+            W.fresh[i] = -1;
+        }
+        int sum;
+        const int at = block_scan(part, sh, sum);
+        if (i < n) off[i] = total + at;
+        total += sum;
+    }
+    if (threadIdx.x == 0) off[n] = total;
+    __syncthreads();
+    // rank r belongs to the last i with off[i] <= r: that i has a partial page, those sharing its offset before it none
+    if (bad) {
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+    } else if (!take_free(P, total, sh, [&](int rank, int id) { W.fresh[owner_of(off, n, rank)] = id; })) {
+        if (threadIdx.x == 0) { raise_status(KVB_DEV_POOL); bad = 1; }
+    }
+    __syncthreads();
+    if (threadIdx.x == 0) W.head[0] = !bad;
+}
+
+// grid (forks, 1 + parts): part 0 snapshots the source's row, the others copy its partial page
+__global__ void fork_copy_kernel(PagesView P, const int32_t* src, ForkWork W) {
+    if (!W.head[0]) return;
+    const int i = blockIdx.x;
+    const int32_t* row = P.table + int64_t(src[i]) * P.max_blocks;
+    const int nb = blocks_of(W.len[i], P.page), fresh = W.fresh[i];
+    if (blockIdx.y == 0) {
+        for (int b = threadIdx.x; b < nb; b += blockDim.x)
+            W.rows[int64_t(i) * P.max_blocks + b] = b == nb - 1 && fresh >= 0 ? fresh : row[b];
+    } else if (fresh >= 0) {
+        const int from = row[nb - 1];
+        if (from >= 0 && from < P.n_pages) copy_page(P, from, fresh, blockIdx.y - 1, gridDim.y - 1);
+    }
+}
+
+// grid (forks): references and rows
+__global__ void fork_commit_kernel(PagesView P, const int32_t* src, const int32_t* dst, ForkWork W) {
+    if (!W.head[0]) return;
+    const int i = blockIdx.x, t = dst[i];
+    if (src[i] == t) return;
+    __shared__ int old;
+    if (threadIdx.x == 0) old = P.lens[t];
+    __syncthreads();
+    int32_t* row = P.table + int64_t(t) * P.max_blocks;
+    const int nb = blocks_of(W.len[i], P.page), ob = blocks_of(old, P.page);
+    for (int b = threadIdx.x; b < max(nb, ob); b += blockDim.x) {
+        if (b < ob && row[b] >= 0 && row[b] < P.n_pages) atomicSub(&P.refs[row[b]], 1);
+        const int id = b < nb ? W.rows[int64_t(i) * P.max_blocks + b] : -1;
+        if (id >= 0 && id < P.n_pages) atomicAdd(&P.refs[id], 1);
+        row[b] = id;
+    }
+    if (threadIdx.x == 0) P.lens[t] = W.len[i];
+}
+
+// Workspace of a compaction: [n_live, moves], then move r: from[r] -> to[r], and new_id (by old page)
+struct CompactWork {
+    int32_t* head;
+    int32_t* from;
+    int32_t* to;
+    int32_t* new_id;
+};
+
+// One block.
+__global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, CompactWork W) {
+    __shared__ int sh[32];
+    int live = 0, sum;
+    for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
+        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
+        block_scan(__popc(m), sh, sum);
+        live += int(imin64(PG_TILE, P.n_pages - t0)) - sum;
+    }
+    // holes and movers in ascending order: as many of the one as of the other
+    int holes = 0, movers = 0;
+    for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
+        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
+        const int64_t base = t0 + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 32;
+        const int64_t below = imin64(imax64(live - base, 0), 32), valid = imin64(imax64(P.n_pages - base, 0), 32);
+        const uint32_t lo = below == 32 ? 0xffffffffu : (1u << below) - 1, in = valid == 32 ? 0xffffffffu : (1u << valid) - 1;
+        uint32_t hole = m & lo, mover = ~m & in & ~lo;
+        int nh, nm;
+        int rh = holes + block_scan(__popc(hole), sh, nh);
+        int rm = movers + block_scan(__popc(mover), sh, nm);
+        for (; hole; hole &= hole - 1) W.to[rh++] = int(base + __ffs(hole) - 1);
+        for (; mover; mover &= mover - 1) W.from[rm++] = int(base + __ffs(mover) - 1);
+        holes += nh;
+        movers += nm;
+    }
+    __syncthreads();
+    for (int r = threadIdx.x; r < movers; r += PG_THREADS) W.new_id[W.from[r]] = W.to[r];
+    if (threadIdx.x == 0) {
+        W.head[0] = live;
+        W.head[1] = movers;
+    }
+}
+
+__global__ void compact_move_kernel(PagesView P, CompactWork W, int32_t* n_live) {
+    const int live = W.head[0], moves = W.head[1];
+    if (blockIdx.x == 0 && threadIdx.x == 0) *n_live = live;
+    constexpr int PARTS = 4;
+    for (int w = blockIdx.x; w < moves * PARTS; w += gridDim.x) {
+        const int r = w / PARTS;
+        copy_page(P, W.from[r], W.to[r], w % PARTS, PARTS);
+        if (w % PARTS == 0 && threadIdx.x == 0) {
+            P.refs[W.to[r]] = P.refs[W.from[r]];
+            P.refs[W.from[r]] = 0;
+        }
+    }
+    const int64_t entries = int64_t(P.n_slots) * P.max_blocks;
+    for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < entries; e += int64_t(gridDim.x) * blockDim.x) {
+        const int id = P.table[e];
+        if (id >= live && id < P.n_pages) P.table[e] = W.new_id[id];
+    }
+}
+
+}  // namespace kvb

@@ -55,6 +55,12 @@ class Coverage(C.Structure):
                 ("local", C.c_int), ("score_cap", C.c_int64)]
 
 
+class Pages(C.Structure):
+    """kvb_pages of include/kvb.h: the 8-bit paged cache's device tensors and sizes."""
+    _fields_ = [(n, C.c_void_p) for n in ("kc", "vc", "ks", "vs", "table", "lens", "refs")] + \
+               [("n_pages", C.c_int64)] + [(n, C.c_int) for n in ("Hkv", "d", "page", "n_slots", "max_blocks")]
+
+
 SIGNATURES = {
     "kvb_last_error": (C.c_char_p, []),
     "kvb_version": (C.c_int, []),
@@ -98,6 +104,19 @@ SIGNATURES = {
     "kvb_uq_values": (_i32, [_p, _i64, _i64, _i64, _p, _p, _p, _p]),
     "kvb_operational_rd_workspace": (C.c_size_t, [_i64, _i32, _i32]),
     "kvb_operational_rd": (_i32, [_p, _i64, _i64, _i64, _p, _i32, _p, _i32, _p, _p, _p, C.c_size_t, _p]),
+    "kvb_prefill_attention": (_i32, [_p, _p, _p, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
+                                     _p, _p, _i32, _f32, _p, _p, _p]),
+    "kvb_page_extend": (_i32, [_p, _p, _p, _i32, _p, _p]),
+    "kvb_page_write": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p]),
+    "kvb_page_read": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _i32, _i64, _p]),
+    "kvb_page_attend_workspace": (C.c_size_t, [_p, _i32, _i32, _i32]),
+    "kvb_page_attend": (_i32, [_p, _p, _i32, _i32, _i32, _p, _i32, _f32, _p, _p, _p, C.c_size_t, _p]),
+    "kvb_page_fork_workspace": (C.c_size_t, [_p, _i32]),
+    "kvb_page_fork": (_i32, [_p, _p, _p, _i32, _p, C.c_size_t, _p]),
+    "kvb_page_free": (_i32, [_p, _p, _i32, _p]),
+    "kvb_page_compact_workspace": (C.c_size_t, [_p]),
+    "kvb_page_compact": (_i32, [_p, _p, _p, C.c_size_t, _p]),
+    "kvb_page_copy": (_i32, [_p, _p, _p, _i32, _p]),
     "kvb_quasar_scores": (_i32, [_p, _i32, _i32, _i32, _p, C.c_size_t, _p, _i32, _p, _i32, _i64, _p, _p]),
     "kvb_quasar_values_workspace": (C.c_size_t, [_i32, _i32, _i64, _i32]),
     "kvb_quasar_values": (_i32, [_p, _i32, _i32, _i64, _p, C.c_size_t, _p, _i32, _p, _i32, _i32, _p, _p, C.c_size_t, _p]),

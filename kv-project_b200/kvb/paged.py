@@ -1,0 +1,214 @@
+"""The paged path: causal attention of packed prompts, and a pool of 8-bit pages that many sequences share.
+
+  prefill_attention   attention of whole prompts packed without padding, or of chunks after their prefixes
+                      (chunked_attention over a prompt, STRATA_KV.py:641-675)
+  PagePool            keys and values of growing sequences in 8-bit pages (one scale per page, KV head and
+                      side): extend, write, attend, read, fork, free, compact, copy_pages.  It stands where
+                      the reference's per-sequence buffers do (LayerState, STRATA_KV.py:682-720), for a batch.
+
+Every call enqueues on the current stream and never synchronises.  Whole numbers (slots, lengths, page
+numbers) are int32 tensors on the device, so a captured graph serves any lengths; ranges that do not fit are
+left out and raise the device status word (``kvb.device_status``: bit 1 a range, bit 4 a pool without enough
+free pages).
+"""
+
+from __future__ import annotations
+
+import ctypes as C
+
+import torch
+
+from . import _lib as L
+from .ops import _DT, _stream
+
+_I32 = torch.int32
+
+
+def _device_ints(who: str, n, **ts):
+    """int32, contiguous, one-dimensional CUDA tensors of n entries (None: any number)."""
+    for name, t in ts.items():
+        if not t.is_cuda or t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
+            raise ValueError(f"{who}: {name} must be a contiguous int32 CUDA tensor of {'n' if n is None else n} entries")
+
+
+def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor = None,
+                      scaling: float = None, out: torch.Tensor = None, return_lse: bool = False):
+    """Causal attention of packed sequences: q (Nq, Hq, d), k and v (Nk, Hkv, d) float16 / bfloat16, any row and head
+    strides (d contiguous); sequence s has the query rows cu_q[s] .. cu_q[s + 1] - 1 and the key rows of cu_k (default:
+    cu_q).  Query i of a sequence sees its keys j <= i + (keys - queries): with as many keys as queries the usual causal
+    mask, with more the queries are the last positions.  Query head a reads KV head a // (Hq // Hkv).  scaling defaults
+    to d ** -0.5.  Returns out (Nq, Hq, d), with return_lse also the log-sum-exp (Nq, Hq) float32; a row that sees no
+    key gives zeros and -inf."""
+    if cu_k is None:
+        cu_k = cu_q
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError("prefill_attention: q (Nq, Hq, d), k and v (Nk, Hkv, d)")
+    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+        raise ValueError("kvb: tensors must live on a CUDA device")
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError("prefill_attention: q, k and v of one dtype")
+    nq, hq, d = q.shape
+    nk, hkv, _ = k.shape
+    _device_ints("prefill_attention", None, cu_q=cu_q, cu_k=cu_k)
+    n = cu_q.shape[0] - 1
+    if n < 0 or cu_k.shape[0] != n + 1:
+        raise ValueError("prefill_attention: cu_q and cu_k hold n + 1 offsets each")
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if d and not qs[2] == ks[2] == vs[2] == 1:
+        raise ValueError("prefill_attention: d must be contiguous")
+    if out is None:
+        out = torch.empty((nq, hq, d), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
+        raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype")
+    lse = torch.empty((nq, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    st = L.lib().kvb_prefill_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
+        vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
+        lse.data_ptr() if return_lse else None, _stream(q.device))
+    if st:
+        L.check(st, "kvb_prefill_attention")
+    return (out, lse) if return_lse else out
+
+
+class PagePool:
+    """Pages of ``page`` tokens for Hkv KV heads: codes kc, vc (n_pages, Hkv, page, d) uint8 and scales ks, vs (n_pages,
+    Hkv) float32 (a stored value is (code - 128) * scale), table (n_slots, max_blocks) int32 with each sequence's pages,
+    lens (n_slots) int32, refs (n_pages) int32.  The pool works on the tensors it is given; layers that share table,
+    lens and refs call extend / free once and write / attend per layer."""
+
+    def __init__(self, kc, vc, ks, vs, table, lens, refs):
+        ts = (kc, vc, ks, vs, table, lens, refs)
+        if kc.dim() != 4 or not all(t.is_cuda and t.is_contiguous() and t.device == kc.device for t in ts):
+            raise ValueError("PagePool: contiguous CUDA tensors of one device, kc (n_pages, Hkv, page, d)")
+        n_pages, hkv, page, d = kc.shape
+        if vc.shape != kc.shape or kc.dtype != torch.uint8 or vc.dtype != torch.uint8:
+            raise ValueError("PagePool: kc and vc uint8 (n_pages, Hkv, page, d)")
+        if ks.shape != (n_pages, hkv) or vs.shape != ks.shape or ks.dtype != torch.float32 or vs.dtype != torch.float32:
+            raise ValueError("PagePool: ks and vs float32 (n_pages, Hkv)")
+        if table.dim() != 2 or lens.shape != (table.shape[0],) or refs.shape != (n_pages,) or \
+                any(t.dtype != _I32 for t in (table, lens, refs)):
+            raise ValueError("PagePool: table (n_slots, max_blocks), lens (n_slots), refs (n_pages) int32")
+        self.kc, self.vc, self.ks, self.vs, self.table, self.lens, self.refs = ts
+        self.n_pages, self.Hkv, self.page, self.d = n_pages, hkv, page, d
+        self.device = kc.device
+        self._c = L.Pages(*[t.data_ptr() for t in ts], n_pages, hkv, d, page, *table.shape)
+        self._p = C.byref(self._c)
+        self._ws = {}
+
+    @classmethod
+    def create(cls, n_pages: int, Hkv: int, d: int, page: int = 64, n_slots: int = 64, max_blocks: int = None, device="cuda"):
+        """An empty pool (max_blocks: pages of the longest sequence; all of the pool by default)."""
+        z = dict(device=device)
+        return cls(torch.full((n_pages, Hkv, page, d), 128, dtype=torch.uint8, **z),
+                   torch.full((n_pages, Hkv, page, d), 128, dtype=torch.uint8, **z),
+                   torch.zeros((n_pages, Hkv), **z), torch.zeros((n_pages, Hkv), **z),
+                   torch.full((n_slots, n_pages if max_blocks is None else max_blocks), -1, dtype=_I32, **z),
+                   torch.zeros(n_slots, dtype=_I32, **z), torch.zeros(n_pages, dtype=_I32, **z))
+
+    def _workspace(self, kind: str, stream: int, size: int) -> torch.Tensor:
+        """A zero-filled buffer for one kind of call on one stream, kept while it is large enough."""
+        ws = self._ws.get((kind, stream))
+        if ws is None or ws.numel() < size:
+            ws = self._ws[(kind, stream)] = torch.zeros(max(size, 256), dtype=torch.uint8, device=self.device)
+        return ws
+
+    def extend(self, slots: torch.Tensor, add: torch.Tensor) -> torch.Tensor:
+        """Pages for add[i] more tokens of sequence slots[i]; returns the positions (n,) int32 where they go (-1: the call
+        was refused, nothing changed)."""
+        n = slots.shape[0]
+        _device_ints("extend", n, slots=slots, add=add)
+        start = torch.empty_like(slots)
+        st = L.lib().kvb_page_extend(self._p, slots.data_ptr(), add.data_ptr(), n, start.data_ptr(), _stream(self.device))
+        if st:
+            L.check(st, "kvb_page_extend")
+        return start
+
+    def write(self, slots, start, cu, k, v) -> None:
+        """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
+        sequence slots[i] (as extend returned them)."""
+        n = slots.shape[0]
+        _device_ints("write", n, slots=slots, start=start)
+        _device_ints("write", n + 1, cu=cu)
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (self.Hkv, self.d) or k.dtype != v.dtype or not (k.is_cuda and v.is_cuda):
+            raise ValueError("write: k and v (N, Hkv, d) CUDA tensors of one dtype")
+        a, b = k.stride(), v.stride()
+        if a[2] != 1 or b[2] != 1:
+            raise ValueError("write: d must be contiguous")
+        st = L.lib().kvb_page_write(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                                    _DT.get(k.dtype, -1), k.shape[0], a[0], a[1], b[0], b[1], _stream(self.device))
+        if st:
+            L.check(st, "kvb_page_write")
+
+    def read(self, slots, start, cu, rows: int, dtype=torch.bfloat16):
+        """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
+        write (rows = cu[-1])."""
+        n = slots.shape[0]
+        _device_ints("read", n, slots=slots, start=start)
+        _device_ints("read", n + 1, cu=cu)
+        k, v = (torch.empty((rows, self.Hkv, self.d), dtype=dtype, device=self.device) for _ in range(2))
+        st = L.lib().kvb_page_read(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                                   _DT.get(dtype, -1), rows, _stream(self.device))
+        if st:
+            L.check(st, "kvb_page_read")
+        return k, v
+
+    def attend(self, q, slots, scaling: float = None, out=None, return_lse: bool = False):
+        """Attention of q (n, Hq, Tq, d), the last Tq positions of each sequence, over its pages -> (n, Tq, Hq, d) in q's
+        dtype (float16 / bfloat16); with return_lse also the log-sum-exp (n, Tq, Hq) float32."""
+        if q.dim() != 4 or q.shape[3] != self.d or not q.is_cuda:
+            raise ValueError("attend: q (n, Hq, Tq, d) on the pool's device")
+        n, hq, tq, d = q.shape
+        _device_ints("attend", n, slots=slots)
+        if not q.is_contiguous():
+            q = q.contiguous()
+        if out is None:
+            out = torch.empty((n, tq, hq, d), dtype=q.dtype, device=q.device)
+        elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
+            raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype")
+        lse = torch.empty((n, tq, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        lib, stream = L.lib(), _stream(self.device)
+        ws = self._ws.get((stream, n, hq, tq))
+        if ws is None:
+            ws = self._ws[(stream, n, hq, tq)] = self._workspace("attend", stream, lib.kvb_page_attend_workspace(self._p, n, hq, tq))
+        st = lib.kvb_page_attend(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, slots.data_ptr(), n,
+                                 d ** -0.5 if scaling is None else scaling, out.data_ptr(), lse.data_ptr() if return_lse else None,
+                                 ws.data_ptr(), ws.numel(), stream)
+        if st:
+            L.check(st, "kvb_page_attend")
+        return (out, lse) if return_lse else out
+
+    def fork(self, src, dst) -> None:
+        """Sequence dst[i] becomes a copy of src[i] (full pages shared, a partial last page copied); what it held is
+        released.  All sources are taken as they were before the call."""
+        n = src.shape[0]
+        _device_ints("fork", n, src=src, dst=dst)
+        lib, stream = L.lib(), _stream(self.device)
+        ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
+        st = lib.kvb_page_fork(self._p, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
+        if st:
+            L.check(st, "kvb_page_fork")
+
+    def free(self, slots) -> None:
+        """Drops the sequences and their references to pages."""
+        _device_ints("free", None, slots=slots)
+        st = L.lib().kvb_page_free(self._p, slots.data_ptr(), slots.shape[0], _stream(self.device))
+        if st:
+            L.check(st, "kvb_page_free")
+
+    def compact(self) -> torch.Tensor:
+        """Moves the live pages to the pool's start; returns their number (one int32 on the device)."""
+        lib, stream = L.lib(), _stream(self.device)
+        ws = self._workspace("compact", stream, lib.kvb_page_compact_workspace(self._p))
+        live = torch.empty((), dtype=_I32, device=self.device)
+        st = lib.kvb_page_compact(self._p, live.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        if st:
+            L.check(st, "kvb_page_compact")
+        return live
+
+    def copy_pages(self, src, dst) -> None:
+        """Page src[i] over page dst[i], codes and scales."""
+        n = src.shape[0]
+        _device_ints("copy_pages", n, src=src, dst=dst)
+        st = L.lib().kvb_page_copy(self._p, src.data_ptr(), dst.data_ptr(), n, _stream(self.device))
+        if st:
+            L.check(st, "kvb_page_copy")
