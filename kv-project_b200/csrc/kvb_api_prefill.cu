@@ -1,18 +1,44 @@
-// kvb_api_prefill.cu - kvb_prefill_attention (include/kvb.h): validation and launch of the causal attention of
-// packed prompts.
+// kvb_api_prefill.cu - kvb_prefill_attention (include/kvb.h): validation, tensor maps and launch of the causal
+// attention of packed prompts (kvb_prefill.cuh).
 #include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "kvb_host.h"
 #include "kvb_common.cuh"
-#include "kvb_rowattn.cuh"
+#include "kvb_prefill.cuh"
 
 namespace {
 
-template <typename T>
-void launch(const kvb::PrefillParams& a, int d, cudaStream_t s) {
-    const dim3 grid(unsigned((a.nq + kvb::RA_WARPS - 1) / kvb::RA_WARPS), unsigned(a.Hq));
-    if (d == 64) kvb::prefill_rows_kernel<T, 64><<<grid, kvb::RA_WARPS * 32, 0, s>>>(a);
-    else kvb::prefill_rows_kernel<T, 128><<<grid, kvb::RA_WARPS * 32, 0, s>>>(a);
+// Rows of `heads` heads of d 16-bit channels as a 3D tensor (d, heads, rows): box 64 x box_heads x box_rows, 128-byte
+// swizzle.
+kvb_status make_map(CUtensorMap* m, const char* name, const void* base, int bf16, int d, int heads, int64_t rows,
+                    int64_t head_stride, int64_t row_stride, int box_heads, int box_rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return fail(KVB_ECUDA, "prefill_attention: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(rows)};
+    // the stride of a dimension of one entry is never used, but has to be a valid one
+    const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head_stride : d) * 2, cuuint64_t(rows > 1 ? row_stride : d) * 2};
+    const cuuint32_t box[3] = {64, cuuint32_t(box_heads), cuuint32_t(box_rows)};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 3, const_cast<void*>(base),
+                          dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(KVB_EINVAL, "prefill_attention: no tensor map for %s (strides %lld, %lld)", name,
+                                       static_cast<long long>(head_stride), static_cast<long long>(row_stride));
+    return KVB_OK;
+}
+
+template <typename T, int D>
+kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
+    constexpr int SM = kvb::PfShape<D>::SMEM;
+    const auto kern = kvb::prefill_kernel<T, D>;
+    if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "prefill_attention"))
+        return st;
+    const int64_t items = a.Hkv * (a.nq / (2 * a.tt) + a.n);         // at least as many as there are
+    kern<<<unsigned(std::min<int64_t>(items, resolve_ctas(0))), kvb::PF_THREADS, SM, s>>>(a);
+    return launch_check("prefill_attention");
 }
 
 }  // namespace
@@ -29,17 +55,43 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
         return fail(KVB_EINVAL, "prefill_attention: Hq a multiple of Hkv, at most 65535");
     if (dtype != KVB_F16 && dtype != KVB_BF16) return fail(KVB_EUNSUPPORTED, "prefill_attention: float16 or bfloat16");
     if (d != 64 && d != 128) return fail(KVB_EUNSUPPORTED, "prefill_attention: d 64 or 128");
+    if (Hq / Hkv > 128) return fail(KVB_EUNSUPPORTED, "prefill_attention: at most 128 query heads per KV head");
     if (n == 0 || nq == 0) return KVB_OK;
     if (!q || (!k && nk) || (!v && nk) || !cu_q || !cu_k || !out) return fail(KVB_EINVAL, "prefill_attention: null argument");
     for (int64_t st : {q_row, q_head, k_row, k_head, v_row, v_head})
         if (st < 0 || st % 8 != 0) return fail(KVB_EINVAL, "prefill_attention: row and head strides multiples of 8 elements");
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
         return fail(KVB_EINVAL, "prefill_attention: q, k, v and out need 16-byte alignment");
-    const kvb::PrefillParams a{q, k, v, q_row, q_head, k_row, k_head, v_row, v_head, cu_q, cu_k, nq, nk, n, Hq, Hkv,
-                               scaling * 1.44269504088896340736f, out, lse};
-    if (dtype == KVB_F16) launch<__half>(a, d, static_cast<cudaStream_t>(stream));
-    else launch<__nv_bfloat16>(a, d, static_cast<cudaStream_t>(stream));
-    return launch_check("prefill_attention");
+    if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "prefill_attention: scaling must be finite");
+    kvb::PrefillParams a{};
+    a.rep = Hq / Hkv;
+    a.tt = 128 / a.rep;
+    const int bf16 = dtype == KVB_BF16;
+    // without keys nothing is loaded from k and v: their maps then describe q
+    const bool none = nk == 0;
+    if (kvb_status st = make_map(&a.tm_q, "q", q, bf16, d, Hq, nq, q_head, q_row, a.rep, a.tt)) return st;
+    if (kvb_status st = none ? make_map(&a.tm_k, "k", q, bf16, d, Hq, nq, q_head, q_row, 1, 128)
+                             : make_map(&a.tm_k, "k", k, bf16, d, Hkv, nk, k_head, k_row, 1, 128)) return st;
+    if (kvb_status st = none ? make_map(&a.tm_v, "v", q, bf16, d, Hq, nq, q_head, q_row, 1, 128)
+                             : make_map(&a.tm_v, "v", v, bf16, d, Hkv, nk, v_head, v_row, 1, 128)) return st;
+    a.v = v;
+    a.v_row = v_row;
+    a.v_head = v_head;
+    a.cu_q = cu_q;
+    a.cu_k = cu_k;
+    a.nq = nq;
+    a.nk = nk;
+    a.n = n;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    // a scaling of zero becomes one too small to matter, so that -inf stays -inf
+    a.lam = std::max(std::fabs(scaling) * 1.44269504088896340736f, 1e-37f);
+    a.negate = scaling < 0;
+    a.out = out;
+    a.lse = lse;
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (bf16) return d == 128 ? launch<__nv_bfloat16, 128>(a, s) : launch<__nv_bfloat16, 64>(a, s);
+    return d == 128 ? launch<__half, 128>(a, s) : launch<__half, 64>(a, s);
 }
 
 }  // extern "C"

@@ -1,0 +1,602 @@
+// kvb_prefill.cuh - causal attention of packed prompts on the 5th-generation tensor cores.
+//
+//   S = Q K^T,  x = scaling log2(e) S,  m = running row maximum of x,  P = 2^(x - m),  l = sum P,  O = P V,
+//   out = O / l,  lse = ln 2 m + ln l, over the keys j <= i + (keys - queries) that a query sees.
+//
+// One pass over the keys with the running maximum and sum of a softmax.  The `rep` query heads of a KV head are
+// packed into the tile's rows (row = token * rep + head in the group), so a tile of 128 rows is 128 / rep tokens
+// of one KV head and a short chunk still fills it.  A work item is two such tiles, A and B, of one sequence and KV
+// head; both read the same key and value tiles of 128 tokens.  While the softmax of one tile runs on the CUDA cores
+// (a warpgroup of its own, thread = row) the tensor cores work for the other:
+//   warp 8    schedules the items and issues the TMA loads (128-byte swizzle; Q once per item, K and V through a ring)
+//   warp 9    allocates tensor memory and issues the MMAs: S = Q K^T (both operands from shared memory) and
+//             O += P V with P read from tensor memory and V as the MN-major operand
+//   warps 0-3, 4-7   the softmax of tile A, B: S from tensor memory, P (rounded to the inputs' type: it is the
+//             MMA's operand) back over it, the division by l and the stores
+// Tensor memory (512 columns): S / P of A and B (128 + 128), O of A and B (d + d).  O is rescaled only when a
+// row's maximum grew by more than 2^8 (P then reaches 256 at most, well inside float16's range; the sums stay in
+// float32), which is seldom after the first tiles.
+//
+// Masks: logits of keys past a row's limit become -inf by selection, so what lies there does not matter; values
+// there would still meet a weight of zero in the MMA (0 * NaN), so in tiles that some row of the item does not see
+// whole, value rows past the sequence become zeros in shared memory, and non-finite entries of the sequence's own
+// later tokens too, which the rows that do see them get added back at the end.
+//
+// Work items are dealt in descending order of their key tiles, forth and back over the CTAs: every CTA finds its
+// next item by bisection on the tile count (a warp reduction over the sequences per step), so no plan is built
+// before the launch and no counter is kept.
+//
+// Every wait is bounded; after a timeout all roles stop, copies in flight are waited for and tensor memory is freed.
+#pragma once
+#include <cuda.h>
+
+#include <climits>
+#include <type_traits>
+
+#include "kvb_common.cuh"
+#include "kvb_pages_view.cuh"
+#include "kvb_spectral.cuh"
+
+namespace kvb {
+
+constexpr int PF_KT = 128;                    // keys per tile
+constexpr int PF_THREADS = 384;               // warps 10 and 11 only give up their registers
+// registers of a thread in the softmax warpgroups and in the third: 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's
+constexpr int PF_REGS_SOFTMAX = 208, PF_REGS_REST = 88;
+constexpr int PF_TMEM_COLS = 512;
+constexpr float PF_LAZY = 8.f;                // log2 of how far a maximum may grow before O is rescaled
+
+struct PrefillParams {
+    CUtensorMap tm_q;                         // (d, Hq, nq), box 64 x rep x (128 / rep)
+    CUtensorMap tm_k, tm_v;                   // (d, Hkv, nk), box 64 x 1 x 128
+    const void* v;                            // values again, for the non-finite entries that are added back
+    int64_t v_row, v_head;
+    const int32_t* cu_q;
+    const int32_t* cu_k;
+    int64_t nq, nk;
+    int n, Hq, Hkv, rep, tt;                  // tt = 128 / rep tokens per tile
+    float lam;                                // |scaling| log2(e), > 0
+    int negate;                               // scaling < 0
+    void* out;                                // (nq, Hq, d)
+    float* lse;                               // (nq, Hq) or null
+};
+
+template <int D>
+struct PfShape {
+    static constexpr int HALVES = D / 64;
+    static constexpr int TILE_BYTES = 128 * D * 2;
+    static constexpr int STAGES = D == 128 ? 5 : 8;
+    static constexpr int Q_BYTES = 2 * TILE_BYTES;
+    static constexpr int SMEM = 1024 + Q_BYTES + STAGES * TILE_BYTES + 1024;
+};
+
+struct PfItem {
+    int q0, ql, k0, kl;                       // the sequence's rows
+    int t0;                                   // first token of tile A within it
+    int head;                                 // KV head; < 0: no more work
+    int n[2];                                 // key tiles of A and B
+    int jm;                                   // first key tile that some row does not see whole
+    uint32_t bad[4][4];                       // non-finite value rows of the tiles jm ..
+};
+
+struct PfShared {
+    uint64_t q_full, q_empty;
+    uint64_t kv_full[8], kv_empty[8];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t item_full[2], item_empty[2];
+    uint32_t tmem;
+    int abort;
+    uint32_t kv_issued, q_issued;
+    PfItem item[2];
+};
+static_assert(sizeof(PfShared) <= 1024, "the barrier block");
+
+// K-major and MN-major (128-byte swizzle) shared-memory matrix descriptors: 8-row (8-k) groups 1024 B apart; for the
+// MN-major one `lead` bytes from one 64-element block of the contiguous dimension to the next.
+__device__ __forceinline__ uint64_t pf_desc_mn(uint32_t saddr, uint32_t lead) {
+    return uint64_t((saddr >> 4) & 0x3FFF) | (uint64_t(lead >> 4) << 16) | (uint64_t(1024 >> 4) << 32) | (uint64_t(1) << 46) |
+           (uint64_t(2) << 61);
+}
+
+__host__ __device__ constexpr uint32_t pf_idesc(int N, int bf16, int b_mn) {
+    return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) |
+           (uint32_t(128 >> 4) << 24);
+}
+
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\t"
+        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
+        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        : "memory");
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
+}
+
+#define PF_R8(r, o) "=r"(r[o]), "=r"(r[o + 1]), "=r"(r[o + 2]), "=r"(r[o + 3]), "=r"(r[o + 4]), "=r"(r[o + 5]), "=r"(r[o + 6]), "=r"(r[o + 7])
+#define PF_W8(r, o) "r"(r[o]), "r"(r[o + 1]), "r"(r[o + 2]), "r"(r[o + 3]), "r"(r[o + 4]), "r"(r[o + 5]), "r"(r[o + 6]), "r"(r[o + 7])
+
+// 32 columns of this thread's tensor-memory lane: valid after pf_wait_ld()
+__device__ __forceinline__ void pf_ld32(uint32_t addr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : PF_R8(r, 0), PF_R8(r, 8), PF_R8(r, 16), PF_R8(r, 24)
+        : "r"(addr));
+}
+__device__ __forceinline__ void pf_st32(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%32], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,"
+        "%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31};" ::PF_W8(r, 0),
+        PF_W8(r, 8), PF_W8(r, 16), PF_W8(r, 24), "r"(addr)
+        : "memory");
+}
+__device__ __forceinline__ void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pf_pack(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pf_pack<__half>(float lo, float hi) { return pack_half2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pf_pack<__nv_bfloat16>(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Whether one of the two packed values is not finite: x * 0 is NaN for NaN and infinities only.
+template <typename T>
+__device__ __forceinline__ bool pf_not_finite(const uint4& w) {
+    using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
+    const T2 z = *reinterpret_cast<const T2*>("\0\0\0");
+    const uint32_t a[4] = {w.x, w.y, w.z, w.w};
+    T2 s = z;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) s = __hfma2(*reinterpret_cast<const T2*>(&a[i]), z, s);
+    return __hisnan(s.x) || __hisnan(s.y);
+}
+
+// ---------------------------------------------------------------------------------------------
+// Work items in descending order of key tiles.
+// ---------------------------------------------------------------------------------------------
+struct PfSeq {
+    int q0, ql, k0, kl, pairs;
+};
+
+__device__ __forceinline__ PfSeq pf_seq(const PrefillParams& A, int s) {
+    PfSeq q{0, 0, 0, 0, 0};
+    if (s < A.n) {
+        q.q0 = A.cu_q[s];
+        q.ql = A.cu_q[s + 1] - q.q0;
+        q.k0 = A.cu_k[s];
+        q.kl = A.cu_k[s + 1] - q.k0;
+        if (q.ql <= 0) q.ql = 0;
+        else if (q.q0 < 0 || q.k0 < 0 || q.kl < 0 || int64_t(q.q0) + q.ql > A.nq || int64_t(q.k0) + q.kl > A.nk) {
+            raise_status(KVB_DEV_BOUNDS);
+            q.ql = q.kl = 0;
+        }
+        q.pairs = (q.ql + 2 * A.tt - 1) / (2 * A.tt);
+    }
+    return q;
+}
+
+// How many of a sequence's tile pairs have t key tiles or more: pair p ends at the query min(2 tt (p + 1), ql), which
+// sees kl - ql + that many keys.
+__device__ __forceinline__ int pf_count(const PfSeq& q, int t, int tt) {
+    if (t <= 0) return q.pairs;
+    const int need = PF_KT * (t - 1) + 1;
+    if (q.kl < need) return 0;
+    const int first = max(need - q.kl + q.ql + 2 * tt - 1, 0) / (2 * tt) - 1;      // ceil(..) - 1
+    return q.pairs - min(max(first, 0), q.pairs - 1);
+}
+
+__device__ __forceinline__ int pf_warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
+
+// Item `idx`; `t` the last item's key tiles (a bound for the search), or < 0 at first.  Whole warp; false when there
+// are no more.
+__device__ __forceinline__ bool pf_item(const PrefillParams& A, int64_t idx, int& t, PfItem& out) {
+    const int lane = threadIdx.x & 31;
+    PfSeq mine = pf_seq(A, lane);
+    auto total = [&](int tiles) {
+        int64_t c = 0;
+        for (int s0 = 0; s0 < A.n; s0 += 32) {
+            const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
+            c += pf_warp_sum(q.pairs ? pf_count(q, tiles, A.tt) : 0);
+        }
+        return c * A.Hkv;
+    };
+    int hi = t;
+    if (t < 0) {
+        int most = 0;
+        for (int s0 = 0; s0 < A.n; s0 += 32) {
+            const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
+            most = max(most, __reduce_max_sync(0xffffffffu, (q.kl + PF_KT - 1) / PF_KT));
+        }
+        hi = most;
+    }
+    if (idx >= total(0)) return false;
+    int lo = 0;                                   // the largest t with total(t) > idx
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) / 2;
+        if (total(mid) > idx) lo = mid;
+        else hi = mid - 1;
+    }
+    t = lo;
+    int64_t r = idx - total(t + 1);               // rank among the items of t tiles
+    for (int s0 = 0; s0 < A.n; s0 += 32) {
+        const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
+        const int above = q.pairs ? pf_count(q, t + 1, A.tt) : 0;
+        const int c = (q.pairs ? pf_count(q, t, A.tt) : 0) - above;
+        int x = c;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const int64_t sum = int64_t(__shfl_sync(0xffffffffu, x, 31)) * A.Hkv;
+        if (r >= sum) { r -= sum; continue; }
+        const uint32_t b = __ballot_sync(0xffffffffu, int64_t(x) * A.Hkv > r);
+        const int src = __ffs(int(b)) - 1;
+        const int64_t before = int64_t(x - c) * A.Hkv;
+        const int pair = q.pairs - above - c + int((r - before) / A.Hkv), head = int((r - before) % A.Hkv);
+        out.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+        out.ql = __shfl_sync(0xffffffffu, q.ql, src);
+        out.k0 = __shfl_sync(0xffffffffu, q.k0, src);
+        out.kl = __shfl_sync(0xffffffffu, q.kl, src);
+        out.t0 = __shfl_sync(0xffffffffu, pair, src) * 2 * A.tt;
+        out.head = __shfl_sync(0xffffffffu, head, src);
+        for (int w = 0; w < 2; ++w) {
+            const int last = min(out.t0 + (w + 1) * A.tt, out.ql);          // tokens before it
+            const int keys = last > out.t0 + w * A.tt ? min(max(out.kl - out.ql + last, 0), out.kl) : 0;
+            out.n[w] = (keys + PF_KT - 1) / PF_KT;
+        }
+        out.jm = max(out.kl - out.ql + out.t0 + 1, 0) / PF_KT;
+        return true;
+    }
+    return false;
+}
+
+template <typename T, int D>
+__global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_constant__ PrefillParams A) {
+    using S = PfShape<D>;
+    constexpr int BF16 = std::is_same<T, __nv_bfloat16>::value ? 1 : 0;
+    extern __shared__ uint8_t pf_raw[];
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pf_raw) + 1023) & ~uintptr_t(1023));
+    uint8_t* sq = base;                                          // [tile][half][128 rows][64 ch]
+    uint8_t* skv = base + S::Q_BYTES;                            // [stage][half][128 tokens][64 ch]: K, V, K, V, ...
+    PfShared& sh = *reinterpret_cast<PfShared*>(skv + S::STAGES * S::TILE_BYTES);
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+    if (threadIdx.x == 0) {
+        mbar_init(&sh.q_full, 1);
+        mbar_init(&sh.q_empty, 1);
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&sh.kv_full[i], 1);
+            mbar_init(&sh.kv_empty[i], 1);
+        }
+        for (int w = 0; w < 2; ++w) {
+            mbar_init(&sh.s_full[w], 1);
+            mbar_init(&sh.p_full[w], 4);
+            mbar_init(&sh.o_full[w], 1);
+            mbar_init(&sh.item_full[w], 1);
+            mbar_init(&sh.item_empty[w], 9);
+        }
+        sh.abort = 0;
+        sh.kv_issued = sh.q_issued = 0;
+        fence_mbar_init();
+    }
+    if (warp == 9) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&sh.tmem)),
+                     "r"(PF_TMEM_COLS));
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh.tmem;
+    volatile int* abort = &sh.abort;
+    // a wait that gave up stops every role
+    auto wait = [&](uint64_t* bar, uint32_t count) {
+        if (*abort) return false;
+        if (mbar_wait(bar, count & 1)) return true;
+        *abort = 1;
+        return false;
+    };
+
+    if (warp >= 8) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_REST));
+    if (warp == 8) {
+        // ---------------- schedule and loads ----------------
+        uint32_t it = 0, items = 0;
+        int t = -1;
+        bool ok = true;
+        for (int64_t round = 0; ok; ++round) {
+            const int64_t idx = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            PfItem x;
+            const bool more = pf_item(A, idx, t, x);
+            PfItem& slot = sh.item[round & 1];
+            if (round >= 2) ok = __all_sync(0xffffffffu, wait(&sh.item_empty[round & 1], uint32_t(round / 2 - 1)));
+            if (!ok) break;
+            if (lane == 0) {
+                slot = x;
+                if (!more) slot.head = -1;
+                for (int i = 0; i < 16; ++i) slot.bad[i / 4][i % 4] = 0;
+                mbar_arrive(&sh.item_full[round & 1]);
+            }
+            if (!more) break;
+            const int nt = max(x.n[0], x.n[1]);
+            if (lane == 0 && nt > 0) {
+                ok = items == 0 || wait(&sh.q_empty, items - 1);
+                if (ok) {
+                    const uint32_t bytes = uint32_t(A.tt * A.rep) * D * 2;
+                    mbar_arrive_expect_tx(&sh.q_full, 2 * bytes);
+                    for (int w = 0; w < 2; ++w)
+                        for (int h = 0; h < S::HALVES; ++h)
+                            tma_load_3d(sq + w * S::TILE_BYTES + h * (128 * 128), &A.tm_q, h * 64, x.head * A.rep,
+                                        x.q0 + x.t0 + w * A.tt, &sh.q_full);
+                    sh.q_issued = ++items;
+                }
+                for (int j = 0; ok && j < 2 * nt; ++j, ++it) {
+                    const int st = it % S::STAGES;
+                    if (it >= S::STAGES && !wait(&sh.kv_empty[st], it / S::STAGES - 1)) { ok = false; break; }
+                    mbar_arrive_expect_tx(&sh.kv_full[st], S::TILE_BYTES);
+                    for (int h = 0; h < S::HALVES; ++h)
+                        tma_load_3d(skv + st * S::TILE_BYTES + h * (128 * 128), j & 1 ? &A.tm_v : &A.tm_k, h * 64, x.head,
+                                    x.k0 + (j >> 1) * PF_KT, &sh.kv_full[st]);
+                    sh.kv_issued = it + 1;
+                }
+            }
+            ok = __shfl_sync(0xffffffffu, int(ok), 0);
+        }
+    } else if (warp == 9) {
+        // ---------------- MMA issue ----------------
+        if (lane == 0) {
+            constexpr uint32_t IDESC_S = pf_idesc(PF_KT, BF16, 0), IDESC_O = pf_idesc(D, BF16, 1);
+            uint32_t kv = 0, items = 0, pv[2] = {0, 0};
+            bool ok = true;
+            auto stage = [&](uint32_t c) { return smem_u32(skv + (c % S::STAGES) * S::TILE_BYTES); };
+            auto scores = [&](int w, uint32_t kst) {             // S_w = Q_w K^T
+                const uint32_t a = smem_u32(sq + w * S::TILE_BYTES), b = stage(kst);
+#pragma unroll
+                for (int k = 0; k < D / 16; ++k) {
+                    const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
+                    umma_f16(tmem + uint32_t(w * PF_KT), umma_desc_sw128(a + off), umma_desc_sw128(b + off), IDESC_S, k != 0);
+                }
+                umma_commit(&sh.s_full[w]);
+            };
+            for (int64_t round = 0; ok; ++round) {
+                if (!wait(&sh.item_full[round & 1], uint32_t(round / 2))) break;
+                const PfItem& x = sh.item[round & 1];
+                const int n0 = x.n[0], n1 = x.n[1], head = x.head;
+                mbar_arrive(&sh.item_empty[round & 1]);
+                if (head < 0) break;
+                const int nt = max(n0, n1);
+                if (nt == 0) continue;
+                const uint32_t k0 = kv;                          // K(j) is load k0 + 2 j, V(j) the one after
+                kv += 2 * nt;
+                ok = wait(&sh.q_full, items) && wait(&sh.kv_full[k0 % S::STAGES], k0 / S::STAGES);
+                ++items;
+                if (!ok) break;
+                tc_fence_after();
+                for (int w = 0; w < 2; ++w)
+                    if ((w ? n1 : n0) > 0) scores(w, k0);
+                umma_commit(&sh.kv_empty[k0 % S::STAGES]);
+                if (nt == 1) umma_commit(&sh.q_empty);
+                for (int j = 0; ok && j < nt; ++j) {
+                    const uint32_t vj = k0 + 2 * j + 1, kn = vj + 1;
+                    ok = wait(&sh.kv_full[vj % S::STAGES], vj / S::STAGES);
+                    if (ok && j + 1 < nt) ok = wait(&sh.kv_full[kn % S::STAGES], kn / S::STAGES);
+                    for (int w = 0; ok && w < 2; ++w) {
+                        const int n = w ? n1 : n0;
+                        if (j >= n) continue;
+                        if (!(ok = wait(&sh.p_full[w], pv[w]++))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int k = 0; k < PF_KT / 16; ++k)     // O_w += P_w V
+                            umma_f16_ts(tmem + 256 + uint32_t(w * D), tmem + uint32_t(w * PF_KT + k * 8),
+                                        pf_desc_mn(stage(vj) + k * 2048, 128 * 128), IDESC_O, j != 0 || k != 0);
+                        umma_commit(&sh.o_full[w]);
+                        if (j + 1 < n) scores(w, kn);
+                    }
+                    if (!ok) break;
+                    umma_commit(&sh.kv_empty[vj % S::STAGES]);
+                    if (j + 1 < nt) umma_commit(&sh.kv_empty[kn % S::STAGES]);
+                    if (j + 2 == nt) umma_commit(&sh.q_empty);   // the last scores are issued
+                }
+            }
+            // after a timeout the MMAs already issued finish before tensor memory is released
+            if (*abort)
+                for (int w = 0; w < 2; ++w)
+                    if (pv[w] > 0) mbar_wait(&sh.o_full[w], (pv[w] - 1) & 1, 10000000ull);
+        }
+    }
+    } else {
+        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFTMAX));
+        // ---------------- softmax: warpgroup w, thread = row ----------------
+        const int w = warp >> 2, row = threadIdx.x & 127;
+        const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
+        const uint32_t s_col = lanes + uint32_t(w * PF_KT), o_col = lanes + 256 + uint32_t(w * D);
+        uint32_t steps = 0, kv = 0;                              // this tile's MMA rounds; loads of the items so far
+        auto all = [&](bool b) { return __all_sync(0xffffffffu, b) != 0; };
+        for (int64_t round = 0;; ++round) {
+            if (!all(wait(&sh.item_full[round & 1], uint32_t(round / 2)))) break;
+            PfItem& x = sh.item[round & 1];
+            const int head = x.head;
+            if (head < 0) break;
+            const int n = x.n[w], nt = max(x.n[0], x.n[1]), jm = x.jm, kl = x.kl;
+            const int tok = x.t0 + w * A.tt + row / A.rep;       // token of the sequence
+            const bool valid = row < A.tt * A.rep && tok < x.ql;
+            const int limit = valid ? min(max(kl - x.ql + tok + 1, 0), kl) : INT_MAX;    // rows of no token mask nothing
+            float m = -INFINITY, l = 0.f;
+            bool ok = true;
+            for (int j = 0; j < n; ++j, ++steps) {
+                if (!(ok = all(wait(&sh.s_full[w], steps)))) break;
+                tc_fence_after();
+                uint32_t r[PF_KT];
+#pragma unroll
+                for (int c = 0; c < PF_KT; c += 32) pf_ld32(s_col + c, r + c);
+                pf_wait_ld();
+                float* v = reinterpret_cast<float*>(r);
+                if (A.negate) {
+#pragma unroll
+                    for (int i = 0; i < PF_KT; ++i) v[i] = -v[i];
+                }
+                const int lim = limit - j * PF_KT;
+                if (__any_sync(0xffffffffu, lim < PF_KT)) {
+#pragma unroll
+                    for (int i = 0; i < PF_KT; ++i) v[i] = i < lim ? v[i] : -INFINITY;
+                }
+                float mx[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                for (int i = 4; i < PF_KT; i += 8) {
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mx[k] = i + 4 + k < PF_KT ? fmaxf(fmaxf(mx[k], v[i + k]), v[i + 4 + k]) : fmaxf(mx[k], v[i + k]);
+                }
+                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.lam;
+                // a row that has seen nothing takes its first maximum as it is; O is zero until then
+                if (m == -INFINITY) m = top;
+                const bool grow = valid && top > m + PF_LAZY;
+                if (__any_sync(0xffffffffu, grow)) {
+                    // O holds the sums of the tiles before: wait for them, and scale the rows that grew
+                    const float f = grow ? ex2(m - top) : 1.f;
+                    m = grow ? top : m;
+                    l *= f;
+                    if (j > 0) {
+                        if (!(ok = all(wait(&sh.o_full[w], steps - 1)))) break;
+                        tc_fence_after();
+#pragma unroll
+                        for (int c = 0; c < D; c += 32) {
+                            uint32_t o[32];
+                            pf_ld32(o_col + c, o);
+                            pf_wait_ld();
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                            pf_st32(o_col + c, o);
+                        }
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+                for (int c = 0; c < PF_KT; c += 64) {
+                    uint32_t p[32];
+#pragma unroll
+                    for (int i = 0; i < 64; i += 2) {
+                        const float a = ex2(__fmaf_rn(v[c + i], A.lam, -ref)), b = ex2(__fmaf_rn(v[c + i + 1], A.lam, -ref));
+                        sum[i & 2] += a;
+                        sum[(i & 2) + 1] += b;
+                        p[i / 2] = pf_pack<T>(a, b);
+                    }
+                    pf_st32(s_col + c / 2, p);
+                }
+                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                if (j >= jm) {
+                    // value rows that some row of the item does not see: see the head of this file
+                    const uint32_t vj = kv + 2 * j + 1;
+                    if (!(ok = all(wait(&sh.kv_full[vj % S::STAGES], vj / S::STAGES)))) break;
+                    uint8_t* vt = skv + (vj % S::STAGES) * S::TILE_BYTES + row * 128;
+                    const bool past = j * PF_KT + row >= kl;
+                    bool bad = false;
+                    if (!past) {
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c)
+                            bad |= pf_not_finite<T>(*reinterpret_cast<const uint4*>(vt + (c >> 3) * (128 * 128) + ((c & 7) ^ (row & 7)) * 16));
+                    }
+                    const uint32_t mask = __ballot_sync(0xffffffffu, bad);
+                    if (mask && lane == 0) atomicOr(&x.bad[j - jm][warp & 3], mask);
+                    __threadfence_block();
+                    if (past) {
+#pragma unroll
+                        for (int c = 0; c < D / 8; ++c) *reinterpret_cast<uint4*>(vt + (c >> 3) * (128 * 128) + c % 8 * 16) = uint4{0, 0, 0, 0};
+                    } else if (bad) {
+                        for (int c = 0; c < D; ++c) {
+                            T* e = reinterpret_cast<T*>(vt + (c >> 6) * (128 * 128) + (((c >> 3) & 7) ^ (row & 7)) * 16) + (c & 7);
+                            if (!(fabsf(to_f32(*e)) < INFINITY)) *e = from_f32<T>(0.f);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                }
+                pf_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_full[w]);
+            }
+            if (!ok) break;
+            if (n > 0) {
+                if (!all(wait(&sh.o_full[w], steps - 1))) break;
+                tc_fence_after();
+            }
+            // records of non-finite values, complete: the last MMA waited for all four warps' P, made after them
+            bool any_bad = false;
+            if (jm < nt)
+                for (int i = 0; i < 16; ++i) any_bad |= reinterpret_cast<volatile uint32_t*>(x.bad)[i] != 0;
+            const int64_t out_row = int64_t(x.q0) + tok;
+            const int hq = head * A.rep + row % A.rep;
+            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
+            T* dst = static_cast<T*>(A.out) + (out_row * A.Hq + hq) * D;
+#pragma unroll 1
+            for (int c = 0; c < D; c += 32) {
+                uint32_t o[32];
+                if (n > 0) {
+                    pf_ld32(o_col + c, o);
+                    pf_wait_ld();
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 32; ++i) o[i] = 0;
+                }
+                if (any_bad && valid && l != 0.f) {
+                    const T* vp = static_cast<const T*>(A.v) + int64_t(x.k0) * A.v_row + head * A.v_head + c;
+                    for (int b = 0; b < 4 * PF_KT; ++b) {
+                        const int key = jm * PF_KT + b;
+                        if (key < limit && (x.bad[b >> 7][(b >> 5) & 3] >> (b & 31) & 1)) {
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) {
+                                const float e = to_f32(vp[key * A.v_row + i]);
+                                if (!(fabsf(e) < INFINITY)) o[i] = __float_as_uint(__uint_as_float(o[i]) + e);
+                            }
+                        }
+                    }
+                }
+                if (valid) {
+                    uint32_t h[16];
+#pragma unroll
+                    for (int i = 0; i < 16; ++i)
+                        h[i] = pf_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
+#pragma unroll
+                    for (int i = 0; i < 4; ++i)
+                        *reinterpret_cast<uint4*>(dst + c + 8 * i) = uint4{h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]};
+                }
+            }
+            if (valid && A.lse)
+                A.lse[out_row * A.Hq + hq] = l == 0.f ? -INFINITY : m * 0.693147180559945309f + logf(l);
+            tc_fence_before();
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[round & 1]);
+            kv += 2 * nt;
+        }
+    }
+
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort) {
+        raise_status(KVB_DEV_TIMEOUT);
+        const uint32_t n = sh.kv_issued;
+        for (uint32_t k = n > uint32_t(S::STAGES) ? n - S::STAGES : 0; k < n; ++k)
+            mbar_wait(&sh.kv_full[k % S::STAGES], (k / S::STAGES) & 1, 10000000ull);
+        if (sh.q_issued > 0) mbar_wait(&sh.q_full, (sh.q_issued - 1) & 1, 10000000ull);
+    }
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    if (warp == 9) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(PF_TMEM_COLS));
+}
+
+}  // namespace kvb

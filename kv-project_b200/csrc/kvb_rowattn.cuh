@@ -1,5 +1,4 @@
-// kvb_rowattn.cuh - attention one query row at a time, in float32: the packed prompts' causal attention and
-// the attention over 8-bit pages.
+// kvb_rowattn.cuh - attention over 8-bit pages one query row at a time, in float32.
 //
 //   s_j = scaling q . k_j,  m = max s_j,  l = sum e^(s_j - m),  o = sum e^(s_j - m) v_j / l,  lse = m + ln l
 //
@@ -49,40 +48,6 @@ __device__ __forceinline__ void row_attention(const float* q, const Keys& keys, 
     }
 }
 
-// The sequence whose packed rows hold row r (cu ascending, cu[0] = 0); whole warp or single thread alike.
-__device__ __forceinline__ int row_sequence(const int32_t* cu, int n, int64_t r) {
-    int lo = 0, hi = n;
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (cu[mid] <= r) lo = mid;
-        else hi = mid;
-    }
-    return lo;
-}
-
-struct PrefillParams {
-    const void* q;
-    const void* k;
-    const void* v;
-    int64_t q_row, q_head, k_row, k_head, v_row, v_head;     // element strides
-    const int32_t* cu_q;
-    const int32_t* cu_k;
-    int64_t nq, nk;
-    int n, Hq, Hkv;
-    float lam;                 // scaling * log2(e)
-    void* out;                 // (nq, Hq, d)
-    float* lse;                // (nq, Hq) or null
-};
-
-template <typename T>
-struct DenseKeys {
-    const T* kp;
-    const T* vp;
-    int64_t ks, vs;
-    __device__ __forceinline__ float k(int j, int c) const { return to_f32(kp[j * ks + c]); }
-    __device__ __forceinline__ float v(int j, int c) const { return to_f32(vp[j * vs + c]); }
-};
-
 constexpr float RA_LN2 = 0.693147180559945309f;
 
 template <typename T, int D>
@@ -92,31 +57,6 @@ __device__ __forceinline__ void store_row(const float (&o)[D / 32], float m, flo
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) out[lane * (D / 32) + c] = from_f32<T>(o[c] * inv);
     if (lse && lane == 0) *lse = l == 0.f ? -INFINITY : m * RA_LN2 + logf(l);
-}
-
-// grid (ceil(nq / RA_WARPS), Hq)
-template <typename T, int D>
-__global__ void __launch_bounds__(RA_WARPS * 32) prefill_rows_kernel(const __grid_constant__ PrefillParams A) {
-    __shared__ float sq[RA_WARPS][D];
-    const int w = threadIdx.x >> 5, lane = threadIdx.x & 31, hq = blockIdx.y;
-    const int64_t r = int64_t(blockIdx.x) * RA_WARPS + w;
-    if (r >= A.nq || r >= A.cu_q[A.n]) return;             // rows of no sequence stay as they are
-    const int s = row_sequence(A.cu_q, A.n, r);
-    const int q0 = A.cu_q[s], ql = A.cu_q[s + 1] - q0, k0 = A.cu_k[s], kl = A.cu_k[s + 1] - k0;
-    if (q0 < 0 || k0 < 0 || kl < 0 || r >= int64_t(q0) + ql || int64_t(k0) + kl > A.nk) {
-        if (lane == 0) raise_status(KVB_DEV_BOUNDS);
-        return;
-    }
-    const int seen = max(0, min(kl, kl - ql + int(r - q0) + 1));
-    const T* q = static_cast<const T*>(A.q) + r * A.q_row + hq * A.q_head;
-    for (int c = lane; c < D; c += 32) sq[w][c] = to_f32(q[c]);
-    __syncwarp();
-    const int h = hq / (A.Hq / A.Hkv);
-    const DenseKeys<T> keys{static_cast<const T*>(A.k) + k0 * A.k_row + h * A.k_head,
-                            static_cast<const T*>(A.v) + k0 * A.v_row + h * A.v_head, A.k_row, A.v_row};
-    float o[D / 32], m, l;
-    row_attention<D>(sq[w], keys, seen, A.lam, o, m, l);
-    store_row<T, D>(o, m, l, static_cast<T*>(A.out) + (r * A.Hq + hq) * D, A.lse ? A.lse + r * A.Hq + hq : nullptr);
 }
 
 struct PagedAttendParams {
