@@ -1,18 +1,65 @@
-// kvb_api_paged.cu - kvb_page_attend (include/kvb.h): validation and launch of the attention over the 8-bit
-// paged cache.
+// kvb_api_paged.cu - kvb_page_attend (include/kvb.h): validation, tensor maps and launch of the attention over the
+// 8-bit paged cache (kvb_paged_decode.cuh).
 #include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
 
 #include "kvb_host.h"
 #include "kvb_pages_host.h"
-#include "kvb_rowattn.cuh"
+#include "kvb_paged_decode.cuh"
 
 namespace {
 
-template <typename T>
-void launch(const kvb::PagedAttendParams& a, cudaStream_t s) {
-    const dim3 grid(unsigned((int64_t(a.n) * a.Tq + kvb::RA_WARPS - 1) / kvb::RA_WARPS), unsigned(a.Hq));
-    if (a.P.d == 64) kvb::paged_rows_kernel<T, 64><<<grid, kvb::RA_WARPS * 32, 0, s>>>(a);
-    else kvb::paged_rows_kernel<T, 128><<<grid, kvb::RA_WARPS * 32, 0, s>>>(a);
+constexpr int64_t kCountBytes = kvb::PD_MAX_CTAS * 4;
+
+// floats of one partial: up to 16 query rows
+int64_t part_floats(int d) { return 16 * (int64_t(d) + 2); }
+
+// Codes as (d, page, n_pages * Hkv) bytes: box d x min(page, 32) x 1, swizzled over the d bytes of a row.
+kvb_status make_map(CUtensorMap* m, const kvb_pages* p, const void* codes) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return fail(KVB_ECUDA, "page_attend: cuTensorMapEncodeTiled unavailable");
+    const cuuint64_t dims[3] = {cuuint64_t(p->d), cuuint64_t(p->page), cuuint64_t(p->n_pages * p->Hkv)};
+    const cuuint64_t strides[2] = {cuuint64_t(p->d), cuuint64_t(p->d) * p->page};
+    const cuuint32_t box[3] = {cuuint32_t(p->d), cuuint32_t(std::min(p->page, kvb::PD_UNIT)), 1};
+    const cuuint32_t estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, estr,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, p->d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KVB_OK : fail(KVB_ECUDA, "page_attend: no tensor map for the codes");
+}
+
+template <typename T, int D, int NT>
+kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
+    constexpr int SM = kvb::PdShape<D, NT>::SMEM;
+    const auto kern = kvb::paged_decode_kernel<T, D, NT>;
+    if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "page_attend"))
+        return st;
+    a.groups = (a.rep * a.Tq + 8 * NT - 1) / (8 * NT);
+    const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
+    const int n = a.n;
+    const char* q = static_cast<const char*>(a.q);
+    char* out = static_cast<char*>(a.out);
+    const int64_t per = int64_t(a.Hq) * a.Tq;
+    const int32_t* slots = a.slots;
+    float* lse = a.lse;
+    for (int i = 0; i < n; i += kvb::PD_MAX_SEQS) {
+        a.n = std::min(n - i, kvb::PD_MAX_SEQS);
+        a.q = q + i * per * D * 2;
+        a.out = out + i * per * D * 2;
+        a.lse = lse ? lse + i * per : nullptr;
+        a.slots = slots + i;
+        kern<<<grid, kvb::PD_THREADS, SM, s>>>(a);
+        if (kvb_status st = launch_check("page_attend")) return st;
+    }
+    return KVB_OK;
+}
+
+// One column group of 8 query rows where they fit, two (the codes' conversion shared by 16 rows) where they do not.
+template <typename T, int D>
+kvb_status launch_rows(const kvb::PagedDecodeParams& a, cudaStream_t s) {
+    return a.rep * a.Tq <= 8 ? launch<T, D, 1>(a, s) : launch<T, D, 2>(a, s);
 }
 
 }  // namespace
@@ -21,7 +68,7 @@ extern "C" {
 
 size_t kvb_page_attend_workspace(const kvb_pages* p, int n, int Hq, int Tq) {
     if (kvbh::check_pages("page_attend", p) || n < 0 || Hq <= 0 || Tq <= 0) return 0;
-    return 256;
+    return size_t(kCountBytes + 2 * kvb::PD_MAX_CTAS * part_floats(p->d) * 4);
 }
 
 kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
@@ -29,15 +76,32 @@ kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq,
     if (kvb_status st = kvbh::check_pages("page_attend", p)) return st;
     if (n > 0 && (!q || !slots || !out || !workspace)) return fail(KVB_EINVAL, "page_attend: null argument");
     if (Hq <= 0 || Hq % p->Hkv != 0 || Hq > 65535) return fail(KVB_EINVAL, "page_attend: Hq a multiple of Hkv, at most 65535");
-    if (n < 0 || Tq <= 0) return fail(KVB_EINVAL, "page_attend: n >= 0, Tq >= 1");
+    if (n < 0 || Tq <= 0 || Tq > (1 << 20)) return fail(KVB_EINVAL, "page_attend: n >= 0, 1 <= Tq <= 2^20");
     if (dtype != KVB_F16 && dtype != KVB_BF16) return fail(KVB_EUNSUPPORTED, "page_attend: q of float16 or bfloat16");
+    if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "page_attend: scaling must be finite");
+    if (p->n_pages * p->Hkv > INT32_MAX) return fail(KVB_EINVAL, "page_attend: n_pages * Hkv < 2^31");
+    if (n == 0) return KVB_OK;
+    if (!aligned(q, 16)) return fail(KVB_EINVAL, "page_attend: q needs 16-byte alignment");
     if (workspace_bytes < kvb_page_attend_workspace(p, n, Hq, Tq) || !aligned(workspace, 256))
         return fail(KVB_EINVAL, "page_attend: workspace of %zu bytes, 256-byte aligned", kvb_page_attend_workspace(p, n, Hq, Tq));
-    if (n == 0) return KVB_OK;
-    const kvb::PagedAttendParams a{kvbh::view_of(p), q, slots, n, Hq, Tq, scaling * 1.44269504088896340736f, out, lse};
-    if (dtype == KVB_F16) launch<__half>(a, static_cast<cudaStream_t>(stream));
-    else launch<__nv_bfloat16>(a, static_cast<cudaStream_t>(stream));
-    return launch_check("page_attend");
+    kvb::PagedDecodeParams a{};
+    if (kvb_status st = make_map(&a.tm_k, p, p->kc)) return st;
+    if (kvb_status st = make_map(&a.tm_v, p, p->vc)) return st;
+    a.P = kvbh::view_of(p);
+    a.q = q;
+    a.slots = slots;
+    a.n = n;
+    a.Hq = Hq;
+    a.Tq = Tq;
+    a.rep = Hq / p->Hkv;
+    a.lam = scaling * 1.44269504088896340736f;
+    a.out = out;
+    a.lse = lse;
+    a.count = static_cast<uint32_t*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == KVB_F16) return p->d == 128 ? launch_rows<__half, 128>(a, s) : launch_rows<__half, 64>(a, s);
+    return p->d == 128 ? launch_rows<__nv_bfloat16, 128>(a, s) : launch_rows<__nv_bfloat16, 64>(a, s);
 }
 
 }  // extern "C"

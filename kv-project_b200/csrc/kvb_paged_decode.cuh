@@ -1,0 +1,548 @@
+// kvb_paged_decode.cuh - attention of a few queries per sequence over the 8-bit paged cache.
+//
+//   s_j = lam q . (kc_j - 128) ks,  o = sum_j 2^(s_j - m) (vc_j - 128) vs / l,  l = sum_j 2^(s_j - m)
+//
+// with lam = scaling log2(e), over the keys that the query sees (query t of Tq: j <= len - Tq + t).
+//
+// The floor is the codes read once: 2 d bytes per token and KV head.  One persistent CTA per SM; a unit of work is
+// 32 tokens of one (sequence, KV head, row group), and every CTA takes an equal run of units in (sequence, head,
+// group, token) order, found from the lengths inside the kernel: any mixture of lengths is balanced, nothing is
+// planned before the launch.  Warp 8 copies the units' codes with TMA through a ring in shared memory (192 KB in flight
+// at d = 128: about 4 us of the SM's share of the bandwidth); units go to the eight computing warps in turn, each of which
+// keeps its own running softmax.  At the end of a run the warps' states are joined in shared memory; a run that is
+// only a part of a (sequence, head, group) leaves a partial, and the CTA that completes the last part joins the
+// partials in the order of the tokens, so the result does not depend on timing.
+//
+// Per 16 tokens, with the query rows (rep heads x Tq queries, 8 per MMA column group) as the N operand:
+//   S (tokens x rows) = K Q^T: a code byte becomes the fp16 pattern 0x6400 | byte = 1024 + code (one byte permute per
+//     two codes), less 1152: exact.  The channels are dealt to the lanes so that a lane reads 16-byte pieces of a row;
+//     with the 128-byte (64-byte for d = 64) swizzle these reads meet no bank twice.
+//   w = 2^(s + log2 vs - m): the value scale goes into the exponent, l takes w / vs.  m is a reference that is only
+//     raised when a logit passes it by 2^8.
+//   O^T (channels x rows) += V^T W^T: the tokens of a lane's codes are interleaved by byte permutes, W goes through
+//     movmatrix and is rounded to fp16 (2^-11; it is the MMA's operand type).
+// Queries are scaled by a power of two per row before they become fp16, so bfloat16 queries are exact too.
+#pragma once
+#include <cuda.h>
+
+#include "kvb_common.cuh"
+#include "kvb_pages_view.cuh"
+#include "kvb_prefill.cuh"
+
+namespace kvb {
+
+constexpr int PD_WARPS = 8;
+constexpr int PD_THREADS = 32 * (PD_WARPS + 1);
+constexpr int PD_UNIT = 32;                   // tokens
+constexpr int PD_MAX_SEQS = 1024;             // sequences of one launch (their offsets are in shared memory)
+constexpr int PD_MAX_CTAS = 256;
+constexpr int PD_MIN_UNITS = 2;               // a CTA's least share of the work
+constexpr float PD_LAZY = 8.f;
+
+struct PagedDecodeParams {
+    CUtensorMap tm_k, tm_v;                   // codes as (d, page, n_pages * Hkv), box d x min(page, 32) x 1
+    PagesView P;
+    const void* q;                            // (n, Hq, Tq, d)
+    const int32_t* slots;
+    int n, Hq, Tq, rep, groups;               // groups of 8 NT query rows per (sequence, KV head)
+    float lam;
+    void* out;                                // (n, Tq, Hq, d)
+    float* lse;                               // (n, Tq, Hq) or null
+    float* part;                              // [2 grid][8 NT x (2 + d)]: m, l, then O
+    uint32_t* count;                          // [grid]
+};
+
+template <int D, int NT>
+struct PdShape {
+    static constexpr int ROWS = 8 * NT;
+    static constexpr int SIDE = PD_UNIT * D;                    // bytes of one side of a unit
+    static constexpr int STAGE = 2 * SIDE;
+    static constexpr int JOIN = PD_WARPS * 8 * (D + 4) * 4;     // the warps' O rows, 8 query rows at a time
+    static constexpr int STAGES = D == 128 ? 23 : 40;
+    static constexpr int PART = ROWS * (D + 2);
+    static constexpr int SMEM = 1024 + STAGES * STAGE + JOIN;
+};
+
+struct PdPiece {
+    int seq, vh, a, b, units;                 // sequence, head * groups + group, unit range, units of the sequence
+};
+
+// The piece that begins at unit `cur` of all work (pre: units before each sequence, per head and group).
+__device__ __forceinline__ PdPiece pd_piece(const int* pre, int n, int hg, int64_t cur, int64_t end) {
+    int lo = 0, hi = n;
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (int64_t(pre[mid]) * hg <= cur) lo = mid;
+        else hi = mid;
+    }
+    PdPiece p;
+    p.seq = lo;
+    p.units = pre[lo + 1] - pre[lo];
+    const int64_t local = cur - int64_t(pre[lo]) * hg;
+    p.vh = int(local / p.units);
+    p.a = int(local - int64_t(p.vh) * p.units);
+    p.b = int(imin64(p.units, p.a + (end - cur)));
+    return p;
+}
+
+__device__ __forceinline__ uint32_t pd_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
+
+// bytes -> two fp16 values code - 128 (exact)
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t pd_half2(uint32_t w) {
+    const uint32_t x = pd_prmt(w, 0x64646464u, SEL);
+    uint32_t y;
+    asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));      // 1152
+    return y;
+}
+
+template <typename T>
+__device__ __forceinline__ float2 pd_pair(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pd_pair<__half>(uint32_t w) { return unpack_half2(w); }
+template <>
+__device__ __forceinline__ float2 pd_pair<__nv_bfloat16>(uint32_t w) {
+    return float2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+
+// log2 of a float32 power of two scale that brings |x| <= amax into [8, 16); 0 for 0
+__device__ __forceinline__ int pd_exponent(float amax) {
+    const int e = int(__float_as_uint(amax) >> 23) & 255;
+    return amax > 0.f ? min(3 - (e - 127), 126) : 0;
+}
+
+template <typename T, int D, int NT>
+__global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __grid_constant__ PagedDecodeParams A) {
+    using S = PdShape<D, NT>;
+    constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
+    extern __shared__ uint8_t pd_raw[];
+    __shared__ int pre[PD_MAX_SEQS + 1];
+    __shared__ uint64_t full[S::STAGES], empty[S::STAGES];
+    __shared__ float4 scales[S::STAGES];                         // ks, ks of tokens 16 .., vs, vs
+    __shared__ float s_m[PD_WARPS][S::ROWS], s_l[PD_WARPS][S::ROWS];
+    __shared__ int warp_sum[PD_WARPS + 1];
+    __shared__ int s_abort, s_last;
+    __shared__ uint32_t issued;
+    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
+    float* join = reinterpret_cast<float*>(ring + S::STAGES * S::STAGE);       // [warp][8 rows][D + 4]
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const PagesView& P = A.P;
+
+    if (threadIdx.x == 0) {
+        for (int i = 0; i < S::STAGES; ++i) {
+            mbar_init(&full[i], 1);
+            mbar_init(&empty[i], 1);
+        }
+        s_abort = 0;
+        issued = 0;
+        fence_mbar_init();
+        pre[0] = 0;
+    }
+    // units before each sequence: an inclusive scan, PD_THREADS sequences at a time; an empty sequence is one unit
+    // without keys, whose rows still have to be written
+    int before = 0;
+    for (int i0 = 0; i0 < A.n; i0 += PD_THREADS) {
+        const int i = i0 + threadIdx.x;
+        int u = 0;
+        if (i < A.n) {
+            const int slot = A.slots[i];
+            int len = 0;
+            if (slot >= 0 && slot < P.n_slots) len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
+            else raise_status(KVB_DEV_BOUNDS);
+            u = max(1, (len + PD_UNIT - 1) / PD_UNIT);
+        }
+        int x = u;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        __syncthreads();
+        if (lane == 31) warp_sum[warp] = x;
+        __syncthreads();
+        int sum = 0;
+        for (int w = 0; w <= PD_WARPS; ++w) {
+            if (w == warp) x += sum;
+            sum += warp_sum[w];
+        }
+        if (i < A.n) pre[i + 1] = before + x;
+        before += sum;
+    }
+    __syncthreads();
+    const int hg = P.Hkv * A.groups;
+    const int64_t work = int64_t(pre[A.n]) * hg;
+    // CTAs that take part (every one of them has work) and this one's run
+    const int64_t ctas = imax64(1, imin64(gridDim.x, work / PD_MIN_UNITS)), cta = blockIdx.x;
+    const int64_t u0 = cta < ctas ? work * cta / ctas : 0, u1 = cta < ctas ? work * (cta + 1) / ctas : 0;
+    volatile int* abort = &s_abort;
+    auto wait = [&](uint64_t* bar, uint32_t count) {
+        if (*abort) return false;
+        if (mbar_wait(bar, count & 1)) return true;
+        *abort = 1;
+        return false;
+    };
+
+    if (warp == PD_WARPS) {
+        // ---------------- copies: every lane prepares one of the next 32 units, then they are issued in order ----------------
+        struct Unit {
+            int page[2], row[2], off, bytes;
+            float4 sc;
+        };
+        const int box = min(P.page, PD_UNIT);
+        auto prepare = [&](int64_t cur) {
+            Unit u{};
+            u.sc = float4{0.f, 0.f, 0.f, 0.f};
+            if (cur >= u1) return u;
+            const PdPiece p = pd_piece(pre, A.n, hg, cur, u1);
+            const int slot = A.slots[p.seq], h = p.vh / A.groups, t0 = p.a * PD_UNIT;
+            u.off = t0 % P.page;
+            if (slot < 0 || slot >= P.n_slots) return u;
+            const int len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
+            for (int i = 0; i < 2; ++i) {
+                if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
+                const int id = P.table[int64_t(slot) * P.max_blocks + (t0 + i * box) / P.page];
+                if (id < 0 || id >= P.n_pages) {
+                    raise_status(KVB_DEV_BOUNDS);
+                    continue;
+                }
+                u.row[i] = id * P.Hkv + h;
+                u.bytes += 2 * box * D;
+                u.page[i] = 1;
+                const float k = P.ks[int64_t(id) * P.Hkv + h], v = P.vs[int64_t(id) * P.Hkv + h];
+                if (i == 0) { u.sc.x = u.sc.y = k; u.sc.z = u.sc.w = v; }
+                else { u.sc.y = k; u.sc.w = v; }
+            }
+            return u;
+        };
+        Unit u = prepare(u0 + lane);
+        bool ok = true;
+        for (int64_t b = u0; b < u1 && ok; b += 32) {
+            const Unit next = prepare(b + 32 + lane);
+            for (int k = 0; k < 32 && b + k < u1 && ok; ++k) {
+                if (lane == k) {
+                    const uint32_t it = uint32_t(b + k - u0);
+                    const int st = it % S::STAGES;
+                    ok = it < S::STAGES || wait(&empty[st], it / S::STAGES - 1);
+                    if (ok) {
+                        scales[st] = u.sc;
+                        mbar_arrive_expect_tx(&full[st], u.bytes);
+                        uint8_t* dst = ring + st * S::STAGE;
+                        for (int i = 0; i < 2; ++i)
+                            if (u.page[i]) {
+                                tma_load_3d(dst + i * box * D, &A.tm_k, 0, u.off, u.row[i], &full[st]);
+                                tma_load_3d(dst + S::SIDE + i * box * D, &A.tm_v, 0, u.off, u.row[i], &full[st]);
+                            }
+                        issued = it + 1;
+                    }
+                }
+                ok = __shfl_sync(0xffffffffu, int(ok), k);
+            }
+            u = next;
+        }
+    } else {
+        // ---------------- computing warps ----------------
+        const int g = lane >> 2, t = lane & 3;
+        int first = 1;
+        for (int64_t cur = u0; cur < u1;) {
+            const PdPiece p = pd_piece(pre, A.n, hg, cur, u1);
+            const int slot = A.slots[p.seq], h = p.vh / A.groups, row0 = (p.vh % A.groups) * S::ROWS;
+            const int len = slot >= 0 && slot < P.n_slots ? min(max(P.lens[slot], 0), P.max_blocks * P.page) : 0;
+            const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
+            // ---- the group's query rows as B operands: lane (g, t) holds row g, channels (D / 4) t ..
+            uint32_t qf[NT][KS][2];
+            float lam[NT][2];
+            int lim[NT][2];                                      // keys that the rows 2t, 2t + 1 see
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                const int r = row0 + 8 * x + g;
+                float amax = 0.f;
+                uint4 raw[KS / 2];
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) raw[i] = uint4{0, 0, 0, 0};
+                if (r < A.rep * A.Tq) {
+                    const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r % A.rep) * A.Tq + r / A.rep) * D + (D / 4) * t;
+#pragma unroll
+                    for (int i = 0; i < KS / 2; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 8 * i);
+                }
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) {
+                    const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = pd_pair<T>(ws[k]);
+                        amax = fmaxf(amax, fmaxf(fabsf(f.x), fabsf(f.y)));
+                    }
+                }
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+                amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+                const int e = pd_exponent(amax);
+                const float up = __uint_as_float(uint32_t(127 + e) << 23);
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) {
+                    const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) {
+                        const float2 f = pd_pair<T>(ws[k]);
+                        qf[x][2 * i + (k >> 1)][k & 1] = pack_half2(f.x * up, f.y * up);
+                    }
+                }
+                const float down = A.lam * __uint_as_float(uint32_t(127 - e) << 23);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    lam[x][k] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + k));
+                    lim[x][k] = len - A.Tq + (row0 + 8 * x + 2 * t + k) / A.rep + 1;
+                }
+            }
+            float o[NT][KS][4], m[NT][2], l[NT][2];
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                m[x][0] = m[x][1] = -INFINITY;
+                l[x][0] = l[x][1] = 0.f;
+#pragma unroll
+                for (int c = 0; c < KS; ++c) o[x][c][0] = o[x][c][1] = o[x][c][2] = o[x][c][3] = 0.f;
+            }
+            // the first unit of the piece that is this warp's (units go to the warps in turn over the CTA's whole run)
+            const uint32_t it0 = uint32_t(cur - u0);
+            for (uint32_t k = (warp - it0) & (PD_WARPS - 1); k < uint32_t(p.b - p.a); k += PD_WARPS) {
+                const uint32_t it = it0 + k;
+                const int st = it % S::STAGES;
+                if (!__all_sync(0xffffffffu, wait(&full[st], it / S::STAGES))) continue;
+                const float4 sc = scales[st];
+                const int t0 = (p.a + int(k)) * PD_UNIT;
+                const uint8_t* kt = ring + st * S::STAGE;
+                const bool edge = t0 + PD_UNIT > len - A.Tq + 1;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    if (t0 + 16 * half >= len) break;
+                    // ---- S = K Q^T
+                    float s[NT][4];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+#pragma unroll
+                    for (int c = 0; c < D / 64; ++c) {
+                        uint4 a, b;
+                        if (D == 128) {
+                            const int ch = ((2 * t + c) ^ g) * 16;
+                            a = *reinterpret_cast<const uint4*>(kt + (16 * half + g) * 128 + ch);
+                            b = *reinterpret_cast<const uint4*>(kt + (16 * half + g + 8) * 128 + ch);
+                        } else {
+                            const int ch = (t ^ ((g >> 1) & 3)) * 16;
+                            a = *reinterpret_cast<const uint4*>(kt + (16 * half + g) * 64 + ch);
+                            b = *reinterpret_cast<const uint4*>(kt + (16 * half + g + 8) * 64 + ch);
+                        }
+                        const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) {
+                            const uint32_t f[4] = {pd_half2<0x4140>(wa[i]), pd_half2<0x4140>(wb[i]), pd_half2<0x4342>(wa[i]),
+                                                   pd_half2<0x4342>(wb[i])};
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) mma16816(s[x], f, qf[x][4 * c + i][0], qf[x][4 * c + i][1]);
+                        }
+                    }
+                    // ---- weights: y = s + log2 vs; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1
+                    const float ks = half ? sc.y : sc.x, vraw = half ? sc.w : sc.z;
+                    const float vs = vraw > 0.f ? vraw : 1.f;    // a page of zeros: any scale does
+                    const float lv = __log2f(vs), rv = __frcp_rn(vs);
+                    bool grow = false;
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        const float l0 = lam[x][0] * ks, l1 = lam[x][1] * ks;
+                        s[x][0] = __fmaf_rn(s[x][0], l0, lv);
+                        s[x][1] = __fmaf_rn(s[x][1], l1, lv);
+                        s[x][2] = __fmaf_rn(s[x][2], l0, lv);
+                        s[x][3] = __fmaf_rn(s[x][3], l1, lv);
+                        if (edge) {
+                            const int j = t0 + 16 * half + g;
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; ++k2) {
+                                if (j >= lim[x][k2]) s[x][k2] = -INFINITY;
+                                if (j + 8 >= lim[x][k2]) s[x][2 + k2] = -INFINITY;
+                            }
+                        }
+                        grow |= fmaxf(s[x][0], s[x][2]) > m[x][0] + PD_LAZY || fmaxf(s[x][1], s[x][3]) > m[x][1] + PD_LAZY;
+                    }
+                    if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                        for (int x = 0; x < NT; ++x)
+#pragma unroll
+                            for (int k2 = 0; k2 < 2; ++k2) {
+                                float top = fmaxf(s[x][k2], s[x][2 + k2]);
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
+                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
+                                if (top > m[x][k2] + PD_LAZY) {
+                                    const float f = ex2(m[x][k2] - top);
+                                    m[x][k2] = top;
+                                    l[x][k2] *= f;
+#pragma unroll
+                                    for (int c = 0; c < KS; ++c) {
+                                        o[x][c][k2] *= f;
+                                        o[x][c][2 + k2] *= f;
+                                    }
+                                }
+                            }
+                    }
+                    uint32_t wf[NT][2];
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
+                        const float w0 = ex2(s[x][0] - r0), w1 = ex2(s[x][1] - r1), w2 = ex2(s[x][2] - r0), w3 = ex2(s[x][3] - r1);
+                        l[x][0] = __fmaf_rn(w0 + w2, rv, l[x][0]);
+                        l[x][1] = __fmaf_rn(w1 + w3, rv, l[x][1]);
+                        wf[x][0] = movmatrix_trans(pack_half2(w0, w1));
+                        wf[x][1] = movmatrix_trans(pack_half2(w2, w3));
+                    }
+                    // ---- O^T += V^T W^T: lane (g, t) holds channels (D / 8) g .. of the tokens 2t, 2t + 1, 2t + 8, 2t + 9
+                    const uint8_t* vt = kt + S::SIDE + half * 16 * D;
+                    uint32_t wv[4][D / 32];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const int tok = 2 * t + (i & 1) + 8 * (i >> 1);
+                        if (D == 128) {
+                            const uint4 x = *reinterpret_cast<const uint4*>(vt + tok * 128 + ((g ^ (tok & 7)) * 16));
+                            wv[i][0] = x.x, wv[i][1] = x.y, wv[i][D / 32 - 2] = x.z, wv[i][D / 32 - 1] = x.w;
+                        } else {
+                            const uint2 x = *reinterpret_cast<const uint2*>(vt + tok * 64 + (((g >> 1) ^ ((tok >> 1) & 3)) * 16) + (g & 1) * 8);
+                            wv[i][0] = x.x, wv[i][1] = x.y;
+                        }
+                    }
+#pragma unroll
+                    for (int i = 0; i < D / 32; ++i) {
+#pragma unroll
+                        for (int b = 0; b < 2; ++b) {
+                            const uint32_t sel = b ? 0x7362u : 0x5140u;
+                            const uint32_t lo = pd_prmt(wv[0][i], wv[1][i], sel), hi = pd_prmt(wv[2][i], wv[3][i], sel);
+                            const uint32_t f[4] = {pd_half2<0x4140>(lo), pd_half2<0x4342>(lo), pd_half2<0x4140>(hi), pd_half2<0x4342>(hi)};
+#pragma unroll
+                            for (int x = 0; x < NT; ++x) mma16816(o[x][2 * i + b], f, wf[x][0], wf[x][1]);
+                        }
+                    }
+                }
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&empty[st]);
+            }
+            // ---- join the warps: row sums, then O, 8 rows at a time
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");           // the last join's reads are done
+#pragma unroll
+            for (int x = 0; x < NT; ++x)
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    float v = l[x][k];
+                    v += __shfl_xor_sync(0xffffffffu, v, 4);
+                    v += __shfl_xor_sync(0xffffffffu, v, 8);
+                    v += __shfl_xor_sync(0xffffffffu, v, 16);
+                    if (g == 0) {
+                        s_m[warp][8 * x + 2 * t + k] = m[x][k];
+                        s_l[warp][8 * x + 2 * t + k] = v;
+                    }
+                }
+            const bool whole = p.a == 0 && p.b == p.units;
+            float* part = A.part + int64_t(2 * blockIdx.x + (first ? 0 : 1)) * S::PART;
+            T* out = static_cast<T*>(A.out);
+#pragma unroll
+            for (int x = 0; x < NT; ++x) {
+                if (x > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                float* mine = join + warp * 8 * (D + 4);
+#pragma unroll
+                for (int c = 0; c < KS; ++c)
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        mine[(2 * t + (k & 1)) * (D + 4) + (D / 8) * g + 2 * c + (k >> 1)] = o[x][c][k];
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                // warp w joins query row 8 x + w; a lane D / 32 channels
+                const int r = 8 * x + warp;
+                float top = -INFINITY;
+#pragma unroll
+                for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+                const float ref = top == -INFINITY ? 0.f : top;
+                float sum = 0.f, acc[D / 32];
+#pragma unroll
+                for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+#pragma unroll
+                for (int w = 0; w < PD_WARPS; ++w) {
+                    const float f = ex2(s_m[w][r] - ref);
+                    sum = __fmaf_rn(s_l[w][r], f, sum);
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) acc[c] = __fmaf_rn(join[(w * 8 + warp) * (D + 4) + lane + 32 * c], f, acc[c]);
+                }
+                if (whole) {
+                    if (r < nrows) {
+                        const int rr = row0 + r;
+                        const int64_t at = (int64_t(p.seq) * A.Tq + rr / A.rep) * A.Hq + h * A.rep + rr % A.rep;
+                        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) out[at * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
+                        if (A.lse && lane == 0) A.lse[at] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+                    }
+                } else {
+                    if (lane == 0) {
+                        part[r] = top;
+                        part[S::ROWS + r] = sum;
+                    }
+#pragma unroll
+                    for (int c = 0; c < D / 32; ++c) part[2 * S::ROWS + r * D + lane + 32 * c] = acc[c];
+                }
+            }
+            if (!whole) {
+                // the units of this (sequence, head, group) belong to the CTAs c0 .. c1; the last of them to arrive joins
+                const int64_t v0 = cur - p.a, v1 = v0 + p.units;
+                auto owner = [&](int64_t u) {                    // the CTA whose run holds unit u
+                    int c = int(u * ctas / work);
+                    while (work * (c + 1) / ctas <= u) ++c;
+                    while (work * c / ctas > u) --c;
+                    return c;
+                };
+                const int c0 = owner(v0), c1 = owner(v1 - 1);
+                __threadfence();
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                if (threadIdx.x == 0) {
+                    const uint32_t seen = atomicAdd(&A.count[c0], 1u);
+                    s_last = seen == uint32_t(c1 - c0);
+                    if (s_last) A.count[c0] = 0;
+                    else if (seen > uint32_t(c1 - c0)) raise_status(KVB_DEV_WORKSPACE);
+                }
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                if (s_last) {
+                    __threadfence();
+                    auto slot_of = [&](int c) { return A.part + int64_t(2 * c + (work * c / ctas >= v0 ? 0 : 1)) * S::PART; };
+                    for (int r = warp; r < nrows; r += PD_WARPS) {
+                        float top = -INFINITY;
+                        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot_of(c) + r));
+                        top = warp_max(top);
+                        const float ref = top == -INFINITY ? 0.f : top;
+                        float sum = 0.f, acc[D / 32];
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+#pragma unroll 4
+                        for (int c = c0; c <= c1; ++c) {
+                            const float* q = slot_of(c);
+                            const float f = ex2(__ldcg(q + r) - ref);
+                            sum = __fmaf_rn(__ldcg(q + S::ROWS + r), f, sum);
+#pragma unroll
+                            for (int i = 0; i < D / 32; ++i) acc[i] = __fmaf_rn(__ldcg(q + 2 * S::ROWS + r * D + lane + 32 * i), f, acc[i]);
+                        }
+                        const int rr = row0 + r;
+                        const int64_t at = (int64_t(p.seq) * A.Tq + rr / A.rep) * A.Hq + h * A.rep + rr % A.rep;
+                        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+#pragma unroll
+                        for (int c = 0; c < D / 32; ++c) out[at * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
+                        if (A.lse && lane == 0) A.lse[at] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+                    }
+                }
+            }
+            cur += p.b - p.a;
+            first = 0;
+        }
+    }
+
+    __syncthreads();
+    if (threadIdx.x == 0 && *abort) {
+        raise_status(KVB_DEV_TIMEOUT);
+        const uint32_t n = issued;
+        for (uint32_t k = n > uint32_t(S::STAGES) ? n - S::STAGES : 0; k < n; ++k)
+            mbar_wait(&full[k % S::STAGES], (k / S::STAGES) & 1, 10000000ull);
+    }
+    __syncthreads();
+}
+
+}  // namespace kvb
