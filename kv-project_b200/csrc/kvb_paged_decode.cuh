@@ -7,9 +7,10 @@
 // The floor is the codes read once: 2 d bytes per token and KV head.  One persistent CTA per SM; a unit of work is
 // 32 tokens of one (sequence, KV head, row group), and every CTA takes an equal run of units in (sequence, head,
 // group, token) order, found from the lengths inside the kernel: any mixture of lengths is balanced, nothing is
-// planned before the launch.  Warp 8 copies the units' codes with TMA through a ring in shared memory (192 KB in flight
-// at d = 128: about 4 us of the SM's share of the bandwidth); units go to the eight computing warps in turn, each of which
-// keeps its own running softmax.  At the end of a run the warps' states are joined in shared memory; a run that is
+// planned before the launch.  Units go to the eight warps in turn; each warp copies its own units' codes with TMA through
+// its own ring (192 KB in flight per SM at d = 128, about 4 us of its share of the bandwidth; one warp copying for all
+// was slower than the copies: 178 us for 537 MB without any arithmetic) and keeps its own running softmax.  Page numbers
+// and scales are fetched 32 units ahead, a lane a unit.  At the end of a run the warps' states are joined in shared memory; a run that is
 // only a part of a (sequence, head, group) leaves a partial, and the CTA that completes the last part joins the
 // partials in the order of the tokens, so the result does not depend on timing.
 //
@@ -32,7 +33,7 @@
 namespace kvb {
 
 constexpr int PD_WARPS = 8;
-constexpr int PD_THREADS = 32 * (PD_WARPS + 1);
+constexpr int PD_THREADS = 32 * PD_WARPS;
 constexpr int PD_UNIT = 32;                   // tokens
 constexpr int PD_MAX_SEQS = 1024;             // sequences of one launch (their offsets are in shared memory)
 constexpr int PD_MAX_CTAS = 256;
@@ -57,10 +58,10 @@ struct PdShape {
     static constexpr int ROWS = 8 * NT;
     static constexpr int SIDE = PD_UNIT * D;                    // bytes of one side of a unit
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int JOIN = PD_WARPS * 8 * (D + 4) * 4;     // the warps' O rows, 8 query rows at a time
-    static constexpr int STAGES = D == 128 ? 23 : 40;
+    static constexpr int STAGES = D == 128 ? 3 : 6;             // per warp
+    static constexpr int JOIN = PD_WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
     static constexpr int PART = ROWS * (D + 2);
-    static constexpr int SMEM = 1024 + STAGES * STAGE + JOIN;
+    static constexpr int SMEM = 1024 + PD_WARPS * STAGES * STAGE + JOIN;
 };
 
 struct PdPiece {
@@ -116,25 +117,20 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
     using S = PdShape<D, NT>;
     constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
     extern __shared__ uint8_t pd_raw[];
-    __shared__ int pre[PD_MAX_SEQS + 1];
-    __shared__ uint64_t full[S::STAGES], empty[S::STAGES];
-    __shared__ float4 scales[S::STAGES];                         // ks, ks of tokens 16 .., vs, vs
+    __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS];
+    __shared__ uint64_t full[PD_WARPS][S::STAGES];
     __shared__ float s_m[PD_WARPS][S::ROWS], s_l[PD_WARPS][S::ROWS];
-    __shared__ int warp_sum[PD_WARPS + 1];
+    __shared__ int warp_sum[PD_WARPS];
     __shared__ int s_abort, s_last;
-    __shared__ uint32_t issued;
-    uint8_t* ring = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
-    float* join = reinterpret_cast<float*>(ring + S::STAGES * S::STAGE);       // [warp][8 rows][D + 4]
+    uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
+    float* join = reinterpret_cast<float*>(base + PD_WARPS * S::STAGES * S::STAGE);      // [warp][8 rows][64 + 4]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    uint8_t* ring = base + warp * S::STAGES * S::STAGE;
     const PagesView& P = A.P;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < S::STAGES; ++i) {
-            mbar_init(&full[i], 1);
-            mbar_init(&empty[i], 1);
-        }
+        for (int i = 0; i < PD_WARPS * S::STAGES; ++i) mbar_init(&full[0][i], 1);
         s_abort = 0;
-        issued = 0;
         fence_mbar_init();
         pre[0] = 0;
     }
@@ -149,6 +145,8 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
             int len = 0;
             if (slot >= 0 && slot < P.n_slots) len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
             else raise_status(KVB_DEV_BOUNDS);
+            s_slot[i] = slot;
+            s_len[i] = len;
             u = max(1, (len + PD_UNIT - 1) / PD_UNIT);
         }
         int x = u;
@@ -161,7 +159,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w <= PD_WARPS; ++w) {
+        for (int w = 0; w < PD_WARPS; ++w) {
             if (w == warp) x += sum;
             sum += warp_sum[w];
         }
@@ -182,71 +180,73 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         return false;
     };
 
-    if (warp == PD_WARPS) {
-        // ---------------- copies: every lane prepares one of the next 32 units, then they are issued in order ----------------
-        struct Unit {
-            int page[2], row[2], off, bytes;
-            float4 sc;
-        };
-        const int box = min(P.page, PD_UNIT);
-        auto prepare = [&](int64_t cur) {
-            Unit u{};
-            u.sc = float4{0.f, 0.f, 0.f, 0.f};
-            if (cur >= u1) return u;
-            const PdPiece p = pd_piece(pre, A.n, hg, cur, u1);
-            const int slot = A.slots[p.seq], h = p.vh / A.groups, t0 = p.a * PD_UNIT;
-            u.off = t0 % P.page;
-            if (slot < 0 || slot >= P.n_slots) return u;
-            const int len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
-            for (int i = 0; i < 2; ++i) {
-                if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
-                const int id = P.table[int64_t(slot) * P.max_blocks + (t0 + i * box) / P.page];
-                if (id < 0 || id >= P.n_pages) {
-                    raise_status(KVB_DEV_BOUNDS);
-                    continue;
-                }
-                u.row[i] = id * P.Hkv + h;
-                u.bytes += 2 * box * D;
-                u.page[i] = 1;
-                const float k = P.ks[int64_t(id) * P.Hkv + h], v = P.vs[int64_t(id) * P.Hkv + h];
-                if (i == 0) { u.sc.x = u.sc.y = k; u.sc.z = u.sc.w = v; }
-                else { u.sc.y = k; u.sc.w = v; }
-            }
-            return u;
-        };
-        Unit u = prepare(u0 + lane);
-        bool ok = true;
-        for (int64_t b = u0; b < u1 && ok; b += 32) {
-            const Unit next = prepare(b + 32 + lane);
-            for (int k = 0; k < 32 && b + k < u1 && ok; ++k) {
-                if (lane == k) {
-                    const uint32_t it = uint32_t(b + k - u0);
-                    const int st = it % S::STAGES;
-                    ok = it < S::STAGES || wait(&empty[st], it / S::STAGES - 1);
-                    if (ok) {
-                        scales[st] = u.sc;
-                        mbar_arrive_expect_tx(&full[st], u.bytes);
-                        uint8_t* dst = ring + st * S::STAGE;
-                        for (int i = 0; i < 2; ++i)
-                            if (u.page[i]) {
-                                tma_load_3d(dst + i * box * D, &A.tm_k, 0, u.off, u.row[i], &full[st]);
-                                tma_load_3d(dst + S::SIDE + i * box * D, &A.tm_v, 0, u.off, u.row[i], &full[st]);
-                            }
-                        issued = it + 1;
-                    }
-                }
-                ok = __shfl_sync(0xffffffffu, int(ok), k);
-            }
-            u = next;
+    auto row_at = [&](int seq, int h, int r) { return (int64_t(seq) * A.Tq + r / A.rep) * A.Hq + h * A.rep + r % A.rep; };
+    auto store_pair = [&](int seq, int h, int r, int ch, float a, float b, float sum) {
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row_at(seq, h, r) * D + ch) = pf_pack<T>(a * inv, b * inv);
+    };
+    auto store_lse = [&](int seq, int h, int r, float top, float sum) {
+        if (A.lse) A.lse[row_at(seq, h, r)] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+    };
+
+    // ---------------- copies: the warp's unit k is the CTA's unit warp + 8 k; lane i looks after the units k = i mod 32 ----------------
+    struct Place {
+        int row[2], off;                                         // rows of the tensor maps (< 0: nothing there), token in the page
+    };
+    const int box = min(P.page, PD_UNIT);
+    const int mine = int(imax64(0, (u1 - u0 - warp + PD_WARPS - 1) / PD_WARPS));         // units of this warp
+    auto place = [&](int k) {
+        Place x{{-1, -1}, 0};
+        if (k >= mine) return x;
+        const PdPiece p = pd_piece(pre, A.n, hg, u0 + warp + int64_t(k) * PD_WARPS, u1);
+        const int h = p.vh / A.groups, t0 = p.a * PD_UNIT, len = s_len[p.seq];
+        x.off = t0 % P.page;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
+            const int id = P.table[int64_t(s_slot[p.seq]) * P.max_blocks + (t0 + i * box) / P.page];
+            if (id >= 0 && id < P.n_pages) x.row[i] = id * P.Hkv + h;
+            else raise_status(KVB_DEV_BOUNDS);
         }
-    } else {
-        // ---------------- computing warps ----------------
+        return x;
+    };
+    auto scales_of = [&](const Place& x) {                       // ks, ks of the tokens 16 .., vs, vs
+        float4 f{0.f, 0.f, 0.f, 0.f};
+        if (x.row[0] >= 0) f.x = f.y = P.ks[x.row[0]], f.z = f.w = P.vs[x.row[0]];
+        if (x.row[1] >= 0) f.y = P.ks[x.row[1]], f.w = P.vs[x.row[1]];
+        return f;
+    };
+    Place at = place(lane), ahead{};                             // of the units being copied, and of the 32 after
+    float4 sc_now{0.f, 0.f, 0.f, 0.f}, sc_next{0.f, 0.f, 0.f, 0.f};      // scales of the units being computed, and of the next
+    int copied = 0;
+    auto copy = [&]() {                                          // the warp's next unit
+        if (copied >= mine) return;
+        if ((copied & 31) == 0) {
+            if (copied > 0) at = ahead;
+            sc_next = scales_of(at);
+            ahead = place(copied + 32 + lane);
+        }
+        if (lane == (copied & 31)) {
+            const int st = copied % S::STAGES;
+            uint64_t* bar = &full[warp][st];
+            mbar_arrive_expect_tx(bar, uint32_t((at.row[0] >= 0) + (at.row[1] >= 0)) * 2 * box * D);
+            uint8_t* dst = ring + st * S::STAGE;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+                if (at.row[i] >= 0) {
+                    tma_load_3d(dst + i * box * D, &A.tm_k, 0, at.off, at.row[i], bar);
+                    tma_load_3d(dst + S::SIDE + i * box * D, &A.tm_v, 0, at.off, at.row[i], bar);
+                }
+        }
+        ++copied;
+    };
+    for (int i = 0; i < S::STAGES; ++i) copy();
+    {
         const int g = lane >> 2, t = lane & 3;
-        int first = 1;
+        int first = 1, unit = 0;
         for (int64_t cur = u0; cur < u1;) {
             const PdPiece p = pd_piece(pre, A.n, hg, cur, u1);
-            const int slot = A.slots[p.seq], h = p.vh / A.groups, row0 = (p.vh % A.groups) * S::ROWS;
-            const int len = slot >= 0 && slot < P.n_slots ? min(max(P.lens[slot], 0), P.max_blocks * P.page) : 0;
+            const int h = p.vh / A.groups, row0 = (p.vh % A.groups) * S::ROWS, len = s_len[p.seq];
             const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
             // ---- the group's query rows as B operands: lane (g, t) holds row g, channels (D / 4) t ..
             uint32_t qf[NT][KS][2];
@@ -303,11 +303,13 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
             }
             // the first unit of the piece that is this warp's (units go to the warps in turn over the CTA's whole run)
             const uint32_t it0 = uint32_t(cur - u0);
-            for (uint32_t k = (warp - it0) & (PD_WARPS - 1); k < uint32_t(p.b - p.a); k += PD_WARPS) {
-                const uint32_t it = it0 + k;
-                const int st = it % S::STAGES;
-                if (!__all_sync(0xffffffffu, wait(&full[st], it / S::STAGES))) continue;
-                const float4 sc = scales[st];
+            for (uint32_t k = (warp - it0) & (PD_WARPS - 1); k < uint32_t(p.b - p.a); k += PD_WARPS, ++unit) {
+                const int st = unit % S::STAGES;
+                if (!__all_sync(0xffffffffu, wait(&full[warp][st], unit / S::STAGES))) continue;
+                if ((unit & 31) == 0) sc_now = sc_next;
+                const int src = unit & 31;
+                const float4 sc{__shfl_sync(0xffffffffu, sc_now.x, src), __shfl_sync(0xffffffffu, sc_now.y, src),
+                                __shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
                 const int t0 = (p.a + int(k)) * PD_UNIT;
                 const uint8_t* kt = ring + st * S::STAGE;
                 const bool edge = t0 + PD_UNIT > len - A.Tq + 1;
@@ -418,8 +420,8 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                         }
                     }
                 }
-                __syncwarp();
-                if (lane == 0) mbar_arrive(&empty[st]);
+                __syncwarp();                                    // every lane has read the stage: refill it
+                copy();
             }
             // ---- join the warps: row sums, then O, 8 rows at a time
             asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");           // the last join's reads are done
@@ -438,49 +440,50 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 }
             const bool whole = p.a == 0 && p.b == p.units;
             float* part = A.part + int64_t(2 * blockIdx.x + (first ? 0 : 1)) * S::PART;
-            T* out = static_cast<T*>(A.out);
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                if (x > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
-                float* mine = join + warp * 8 * (D + 4);
-#pragma unroll
-                for (int c = 0; c < KS; ++c)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mine[(2 * t + (k & 1)) * (D + 4) + (D / 8) * g + 2 * c + (k >> 1)] = o[x][c][k];
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
-                // warp w joins query row 8 x + w; a lane D / 32 channels
+                // warp w joins query row 8 x + w; column c of the buffer is channel (D / 8) (c / 8) + 8 y + c % 8
                 const int r = 8 * x + warp;
-                float top = -INFINITY;
+                float top = -INFINITY, sum = 0.f, f[PD_WARPS];
 #pragma unroll
-                for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
-                const float ref = top == -INFINITY ? 0.f : top;
-                float sum = 0.f, acc[D / 32];
+                for (int y = 0; y < D / 64; ++y) {
+                    if (x + y > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                    float* to = join + warp * 8 * 68 + 2 * t * 68 + 8 * g;
 #pragma unroll
-                for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+                    for (int c = 0; c < 4; ++c) {
+                        *reinterpret_cast<float2*>(to + 2 * c) = float2{o[x][4 * y + c][0], o[x][4 * y + c][2]};
+                        *reinterpret_cast<float2*>(to + 68 + 2 * c) = float2{o[x][4 * y + c][1], o[x][4 * y + c][3]};
+                    }
+                    asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                    if (y == 0) {
 #pragma unroll
-                for (int w = 0; w < PD_WARPS; ++w) {
-                    const float f = ex2(s_m[w][r] - ref);
-                    sum = __fmaf_rn(s_l[w][r], f, sum);
+                        for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+                        const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                    for (int c = 0; c < D / 32; ++c) acc[c] = __fmaf_rn(join[(w * 8 + warp) * (D + 4) + lane + 32 * c], f, acc[c]);
+                        for (int w = 0; w < PD_WARPS; ++w) {
+                            f[w] = ex2(s_m[w][r] - ref);
+                            sum = __fmaf_rn(s_l[w][r], f[w], sum);
+                        }
+                    }
+                    float2 acc{0.f, 0.f};
+#pragma unroll
+                    for (int w = 0; w < PD_WARPS; ++w) {
+                        const float2 v = *reinterpret_cast<const float2*>(join + (w * 8 + warp) * 68 + 2 * lane);
+                        acc.x = __fmaf_rn(v.x, f[w], acc.x);
+                        acc.y = __fmaf_rn(v.y, f[w], acc.y);
+                    }
+                    const int ch = (D / 8) * (lane >> 2) + 8 * y + 2 * (lane & 3);
+                    if (whole) {
+                        if (r < nrows) store_pair(p.seq, h, row0 + r, ch, acc.x, acc.y, sum);
+                    } else {
+                        *reinterpret_cast<float2*>(part + 2 * S::ROWS + r * D + ch) = acc;
+                    }
                 }
                 if (whole) {
-                    if (r < nrows) {
-                        const int rr = row0 + r;
-                        const int64_t at = (int64_t(p.seq) * A.Tq + rr / A.rep) * A.Hq + h * A.rep + rr % A.rep;
-                        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-#pragma unroll
-                        for (int c = 0; c < D / 32; ++c) out[at * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
-                        if (A.lse && lane == 0) A.lse[at] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
-                    }
-                } else {
-                    if (lane == 0) {
-                        part[r] = top;
-                        part[S::ROWS + r] = sum;
-                    }
-#pragma unroll
-                    for (int c = 0; c < D / 32; ++c) part[2 * S::ROWS + r * D + lane + 32 * c] = acc[c];
+                    if (r < nrows && lane == 0) store_lse(p.seq, h, row0 + r, top, sum);
+                } else if (lane == 0) {
+                    part[r] = top;
+                    part[S::ROWS + r] = sum;
                 }
             }
             if (!whole) {
@@ -510,23 +513,25 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                         for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot_of(c) + r));
                         top = warp_max(top);
                         const float ref = top == -INFINITY ? 0.f : top;
-                        float sum = 0.f, acc[D / 32];
+                        float sum = 0.f;
+                        float2 acc[D / 64];
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) acc[c] = 0.f;
+                        for (int i = 0; i < D / 64; ++i) acc[i] = float2{0.f, 0.f};
 #pragma unroll 4
                         for (int c = c0; c <= c1; ++c) {
                             const float* q = slot_of(c);
                             const float f = ex2(__ldcg(q + r) - ref);
                             sum = __fmaf_rn(__ldcg(q + S::ROWS + r), f, sum);
 #pragma unroll
-                            for (int i = 0; i < D / 32; ++i) acc[i] = __fmaf_rn(__ldcg(q + 2 * S::ROWS + r * D + lane + 32 * i), f, acc[i]);
+                            for (int i = 0; i < D / 64; ++i) {
+                                const float2 v = __ldcg(reinterpret_cast<const float2*>(q + 2 * S::ROWS + r * D + 2 * lane + 64 * i));
+                                acc[i].x = __fmaf_rn(v.x, f, acc[i].x);
+                                acc[i].y = __fmaf_rn(v.y, f, acc[i].y);
+                            }
                         }
-                        const int rr = row0 + r;
-                        const int64_t at = (int64_t(p.seq) * A.Tq + rr / A.rep) * A.Hq + h * A.rep + rr % A.rep;
-                        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
 #pragma unroll
-                        for (int c = 0; c < D / 32; ++c) out[at * D + lane + 32 * c] = from_f32<T>(acc[c] * inv);
-                        if (A.lse && lane == 0) A.lse[at] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+                        for (int i = 0; i < D / 64; ++i) store_pair(p.seq, h, row0 + r, 2 * lane + 64 * i, acc[i].x, acc[i].y, sum);
+                        if (lane == 0) store_lse(p.seq, h, row0 + r, top, sum);
                     }
                 }
             }
@@ -535,12 +540,11 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         }
     }
 
-    __syncthreads();
-    if (threadIdx.x == 0 && *abort) {
-        raise_status(KVB_DEV_TIMEOUT);
-        const uint32_t n = issued;
-        for (uint32_t k = n > uint32_t(S::STAGES) ? n - S::STAGES : 0; k < n; ++k)
-            mbar_wait(&full[k % S::STAGES], (k / S::STAGES) & 1, 10000000ull);
+    if (*abort) {                                                // copies in flight land before shared memory is released
+        if (lane == 0) {
+            raise_status(KVB_DEV_TIMEOUT);
+            for (int k = max(0, copied - S::STAGES); k < copied; ++k) mbar_wait(&full[warp][k % S::STAGES], (k / S::STAGES) & 1, 10000000ull);
+        }
     }
     __syncthreads();
 }
