@@ -26,6 +26,8 @@
 #pragma once
 #include <cuda.h>
 
+#include <climits>
+
 #include "kvb_common.cuh"
 #include "kvb_pages_view.cuh"
 #include "kvb_prefill.cuh"
@@ -37,7 +39,8 @@ constexpr int PD_THREADS = 32 * PD_WARPS;
 constexpr int PD_UNIT = 32;                   // tokens
 constexpr int PD_MAX_SEQS = 1024;             // sequences of one launch (their offsets are in shared memory)
 constexpr int PD_MAX_CTAS = 256;
-constexpr int PD_MIN_UNITS = 2;               // a CTA's least share of the work
+constexpr int PD_FIXED = 12;                  // what a (sequence, head, group) costs beside its units, in units
+constexpr int PD_LEAST = 4;                   // a CTA's least share
 constexpr float PD_LAZY = 8.f;
 
 struct PagedDecodeParams {
@@ -64,25 +67,52 @@ struct PdShape {
     static constexpr int SMEM = 1024 + PD_WARPS * STAGES * STAGE + JOIN;
 };
 
-struct PdPiece {
-    int seq, vh, a, b, units;                 // sequence, head * groups + group, unit range, units of the sequence
+// The work of a call: per (sequence, KV head, row group) its units, and PD_FIXED more in the shares that the CTAs get
+// (preparing the queries and joining the warps costs about as much time as that many units).
+struct PdPlan {
+    const int* pre;                           // [n + 1] units before each sequence, for one head and group
+    int n, hg;                                // sequences; KV heads x groups
+    int quota, extra, ctas;                   // shares: the first `extra` CTAs get quota + 1
+
+    __device__ __forceinline__ int share(int c) const { return c * quota + min(c, extra); }
+    __device__ __forceinline__ int holder(int v) const {
+        const int big = extra * (quota + 1);
+        return v < big ? v / (quota + 1) : extra + (v - big) / quota;
+    }
+    // units before the place `v` of the shares
+    __device__ __forceinline__ int units_before(int v) const {
+        int lo = 0, hi = n;
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) >> 1;
+            if ((pre[mid] + mid * PD_FIXED) * hg <= v) lo = mid;
+            else hi = mid;
+        }
+        const int u = pre[lo + 1] - pre[lo], local = v - (pre[lo] + lo * PD_FIXED) * hg, vh = min(local / (u + PD_FIXED), hg);
+        return pre[lo] * hg + vh * u + max(local - vh * (u + PD_FIXED) - PD_FIXED, 0);
+    }
 };
 
-// The piece that begins at unit `cur` of all work (pre: units before each sequence, per head and group).
-__device__ __forceinline__ PdPiece pd_piece(const int* pre, int n, int hg, int64_t cur, int64_t end) {
-    int lo = 0, hi = n;
+struct PdPiece {
+    int seq, vh, a, b, units;                 // sequence, head * groups + group, unit range, units of the sequence
+    int v0;                                   // where the (sequence, head, group) begins in the shares
+};
+
+// The piece that begins at unit `cur` of all work.
+__device__ __forceinline__ PdPiece pd_piece(const PdPlan& W, int cur, int end) {
+    int lo = 0, hi = W.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (int64_t(pre[mid]) * hg <= cur) lo = mid;
+        if (W.pre[mid] * W.hg <= cur) lo = mid;
         else hi = mid;
     }
     PdPiece p;
     p.seq = lo;
-    p.units = pre[lo + 1] - pre[lo];
-    const int64_t local = cur - int64_t(pre[lo]) * hg;
-    p.vh = int(local / p.units);
-    p.a = int(local - int64_t(p.vh) * p.units);
-    p.b = int(imin64(p.units, p.a + (end - cur)));
+    p.units = W.pre[lo + 1] - W.pre[lo];
+    const int local = cur - W.pre[lo] * W.hg;
+    p.vh = local / p.units;
+    p.a = local - p.vh * p.units;
+    p.b = min(p.units, p.a + (end - cur));
+    p.v0 = (W.pre[lo] + lo * PD_FIXED) * W.hg + p.vh * (p.units + PD_FIXED);
     return p;
 }
 
@@ -167,11 +197,21 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         before += sum;
     }
     __syncthreads();
-    const int hg = P.Hkv * A.groups;
-    const int64_t work = int64_t(pre[A.n]) * hg;
-    // CTAs that take part (every one of them has work) and this one's run
-    const int64_t ctas = imax64(1, imin64(gridDim.x, work / PD_MIN_UNITS)), cta = blockIdx.x;
-    const int64_t u0 = cta < ctas ? work * cta / ctas : 0, u1 = cta < ctas ? work * (cta + 1) / ctas : 0;
+    PdPlan W;
+    W.pre = pre;
+    W.n = A.n;
+    W.hg = P.Hkv * A.groups;
+    const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
+    if (work > INT_MAX) {                                        // 2^36 token-heads: more than the memory holds
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return;
+    }
+    W.ctas = max(1, min(int(gridDim.x), int(work) / PD_LEAST));
+    W.quota = int(work) / W.ctas;
+    W.extra = int(work) - W.quota * W.ctas;
+    const int cta = blockIdx.x;
+    if (cta >= W.ctas) return;
+    const int u0 = W.units_before(W.share(cta)), u1 = W.units_before(W.share(cta + 1));
     volatile int* abort = &s_abort;
     auto wait = [&](uint64_t* bar, uint32_t count) {
         if (*abort) return false;
@@ -189,16 +229,39 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         if (A.lse) A.lse[row_at(seq, h, r)] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
     };
 
+    // the query rows of a piece: lane (g, t) holds row g of 8, channels (D / 4) t ..
+    const int g = lane >> 2, t = lane & 3;
+    uint4 raw[NT][KS / 2];
+    auto load_q = [&](const PdPiece& p) {
+        const int h = p.vh / A.groups, row0 = (p.vh - h * A.groups) * S::ROWS;
+#pragma unroll
+        for (int x = 0; x < NT; ++x) {
+            const int r = row0 + 8 * x + g;
+#pragma unroll
+            for (int i = 0; i < KS / 2; ++i) raw[x][i] = uint4{0, 0, 0, 0};
+            if (r < A.rep * A.Tq) {
+                const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r % A.rep) * A.Tq + r / A.rep) * D + (D / 4) * t;
+#pragma unroll
+                for (int i = 0; i < KS / 2; ++i) raw[x][i] = __ldg(reinterpret_cast<const uint4*>(q + 8 * i));
+            }
+        }
+    };
+    PdPiece p{};
+    if (u0 < u1) {
+        p = pd_piece(W, u0, u1);
+        load_q(p);
+    }
+
     // ---------------- copies: the warp's unit k is the CTA's unit warp + 8 k; lane i looks after the units k = i mod 32 ----------------
     struct Place {
         int row[2], off;                                         // rows of the tensor maps (< 0: nothing there), token in the page
     };
     const int box = min(P.page, PD_UNIT);
-    const int mine = int(imax64(0, (u1 - u0 - warp + PD_WARPS - 1) / PD_WARPS));         // units of this warp
+    const int mine = max(0, (u1 - u0 - warp + PD_WARPS - 1) / PD_WARPS);                 // units of this warp
     auto place = [&](int k) {
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
-        const PdPiece p = pd_piece(pre, A.n, hg, u0 + warp + int64_t(k) * PD_WARPS, u1);
+        const PdPiece p = pd_piece(W, u0 + warp + k * PD_WARPS, u1);
         const int h = p.vh / A.groups, t0 = p.a * PD_UNIT, len = s_len[p.seq];
         x.off = t0 % P.page;
 #pragma unroll
@@ -242,31 +305,20 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
     };
     for (int i = 0; i < S::STAGES; ++i) copy();
     {
-        const int g = lane >> 2, t = lane & 3;
         int first = 1, unit = 0;
-        for (int64_t cur = u0; cur < u1;) {
-            const PdPiece p = pd_piece(pre, A.n, hg, cur, u1);
-            const int h = p.vh / A.groups, row0 = (p.vh % A.groups) * S::ROWS, len = s_len[p.seq];
+        for (int cur = u0; cur < u1;) {
+            const int h = p.vh / A.groups, row0 = (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
             const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
-            // ---- the group's query rows as B operands: lane (g, t) holds row g, channels (D / 4) t ..
+            // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
             float lam[NT][2];
             int lim[NT][2];                                      // keys that the rows 2t, 2t + 1 see
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                const int r = row0 + 8 * x + g;
                 float amax = 0.f;
-                uint4 raw[KS / 2];
-#pragma unroll
-                for (int i = 0; i < KS / 2; ++i) raw[i] = uint4{0, 0, 0, 0};
-                if (r < A.rep * A.Tq) {
-                    const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r % A.rep) * A.Tq + r / A.rep) * D + (D / 4) * t;
-#pragma unroll
-                    for (int i = 0; i < KS / 2; ++i) raw[i] = *reinterpret_cast<const uint4*>(q + 8 * i);
-                }
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) {
-                    const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    const uint32_t ws[4] = {raw[x][i].x, raw[x][i].y, raw[x][i].z, raw[x][i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float2 f = pd_pair<T>(ws[k]);
@@ -279,7 +331,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 const float up = __uint_as_float(uint32_t(127 + e) << 23);
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) {
-                    const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+                    const uint32_t ws[4] = {raw[x][i].x, raw[x][i].y, raw[x][i].z, raw[x][i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float2 f = pd_pair<T>(ws[k]);
@@ -302,24 +354,26 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 for (int c = 0; c < KS; ++c) o[x][c][0] = o[x][c][1] = o[x][c][2] = o[x][c][3] = 0.f;
             }
             // the first unit of the piece that is this warp's (units go to the warps in turn over the CTA's whole run)
-            const uint32_t it0 = uint32_t(cur - u0);
-            for (uint32_t k = (warp - it0) & (PD_WARPS - 1); k < uint32_t(p.b - p.a); k += PD_WARPS, ++unit) {
+            for (int k = (warp - (cur - u0)) & (PD_WARPS - 1); k < p.b - p.a; k += PD_WARPS, ++unit) {
                 const int st = unit % S::STAGES;
                 if (!__all_sync(0xffffffffu, wait(&full[warp][st], unit / S::STAGES))) continue;
                 if ((unit & 31) == 0) sc_now = sc_next;
                 const int src = unit & 31;
-                const float4 sc{__shfl_sync(0xffffffffu, sc_now.x, src), __shfl_sync(0xffffffffu, sc_now.y, src),
-                                __shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
-                const int t0 = (p.a + int(k)) * PD_UNIT;
+                const float ks[2] = {__shfl_sync(0xffffffffu, sc_now.x, src), __shfl_sync(0xffffffffu, sc_now.y, src)};
+                float vs[2] = {__shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
+                const int t0 = (p.a + k) * PD_UNIT;
                 const uint8_t* kt = ring + st * S::STAGE;
                 const bool edge = t0 + PD_UNIT > len - A.Tq + 1;
+                // ---- S = K Q^T for the two halves of 16 tokens; past the sequence's end the codes are whatever the page
+                // holds (any byte is a finite value) and are masked below
+                float s[2][NT][4];
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    if (t0 + 16 * half >= len) break;
-                    // ---- S = K Q^T
-                    float s[NT][4];
+                    float s2[2][NT][4];                          // two chains of MMAs
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) s[x][0] = s[x][1] = s[x][2] = s[x][3] = 0.f;
+                    for (int c = 0; c < 2; ++c)
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) s2[c][x][0] = s2[c][x][1] = s2[c][x][2] = s2[c][x][3] = 0.f;
 #pragma unroll
                     for (int c = 0; c < D / 64; ++c) {
                         uint4 a, b;
@@ -338,63 +392,83 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                             const uint32_t f[4] = {pd_half2<0x4140>(wa[i]), pd_half2<0x4140>(wb[i]), pd_half2<0x4342>(wa[i]),
                                                    pd_half2<0x4342>(wb[i])};
 #pragma unroll
-                            for (int x = 0; x < NT; ++x) mma16816(s[x], f, qf[x][4 * c + i][0], qf[x][4 * c + i][1]);
+                            for (int x = 0; x < NT; ++x) mma16816(s2[i & 1][x], f, qf[x][4 * c + i][0], qf[x][4 * c + i][1]);
                         }
                     }
-                    // ---- weights: y = s + log2 vs; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1
-                    const float ks = half ? sc.y : sc.x, vraw = half ? sc.w : sc.z;
-                    const float vs = vraw > 0.f ? vraw : 1.f;    // a page of zeros: any scale does
-                    const float lv = __log2f(vs), rv = __frcp_rn(vs);
-                    bool grow = false;
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        const float l0 = lam[x][0] * ks, l1 = lam[x][1] * ks;
-                        s[x][0] = __fmaf_rn(s[x][0], l0, lv);
-                        s[x][1] = __fmaf_rn(s[x][1], l1, lv);
-                        s[x][2] = __fmaf_rn(s[x][2], l0, lv);
-                        s[x][3] = __fmaf_rn(s[x][3], l1, lv);
-                        if (edge) {
-                            const int j = t0 + 16 * half + g;
+                    for (int x = 0; x < NT; ++x)
 #pragma unroll
-                            for (int k2 = 0; k2 < 2; ++k2) {
-                                if (j >= lim[x][k2]) s[x][k2] = -INFINITY;
-                                if (j + 8 >= lim[x][k2]) s[x][2 + k2] = -INFINITY;
-                            }
-                        }
-                        grow |= fmaxf(s[x][0], s[x][2]) > m[x][0] + PD_LAZY || fmaxf(s[x][1], s[x][3]) > m[x][1] + PD_LAZY;
-                    }
-                    if (__any_sync(0xffffffffu, grow)) {
+                        for (int i = 0; i < 4; ++i) s[half][x][i] = s2[0][x][i] + s2[1][x][i];
+                }
+                // ---- weights: y = s + log2 vs; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1 of either half
+                float rv[2];
+                bool grow = false;
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
+                    vs[half] = vs[half] > 0.f ? vs[half] : 1.f;  // a page of zeros: any scale does
+                    rv[half] = __frcp_rn(vs[half]);
+                    const float lv = __log2f(vs[half]);
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) s[half][x][i] = __fmaf_rn(s[half][x][i], lam[x][i & 1] * ks[half], lv);
+                }
+                if (edge) {
+#pragma unroll
+                    for (int half = 0; half < 2; ++half)
 #pragma unroll
                         for (int x = 0; x < NT; ++x)
 #pragma unroll
-                            for (int k2 = 0; k2 < 2; ++k2) {
-                                float top = fmaxf(s[x][k2], s[x][2 + k2]);
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 4));
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 8));
-                                top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 16));
-                                if (top > m[x][k2] + PD_LAZY) {
-                                    const float f = ex2(m[x][k2] - top);
-                                    m[x][k2] = top;
-                                    l[x][k2] *= f;
+                            for (int i = 0; i < 4; ++i)
+                                if (t0 + 16 * half + g + 8 * (i >> 1) >= lim[x][i & 1]) s[half][x][i] = -INFINITY;
+                }
+                float top[NT][2];
 #pragma unroll
-                                    for (int c = 0; c < KS; ++c) {
-                                        o[x][c][k2] *= f;
-                                        o[x][c][2 + k2] *= f;
-                                    }
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        top[x][i] = fmaxf(fmaxf(s[0][x][i], s[0][x][i + 2]), fmaxf(s[1][x][i], s[1][x][i + 2]));
+                        grow |= top[x][i] > m[x][i] + PD_LAZY;
+                    }
+                if (__any_sync(0xffffffffu, grow)) {
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {
+                            float y = top[x][i];
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                            if (y > m[x][i] + PD_LAZY) {
+                                const float f = ex2(m[x][i] - y);
+                                m[x][i] = y;
+                                l[x][i] *= f;
+#pragma unroll
+                                for (int c = 0; c < KS; ++c) {
+                                    o[x][c][i] *= f;
+                                    o[x][c][2 + i] *= f;
                                 }
                             }
-                    }
-                    uint32_t wf[NT][2];
+                        }
+                }
+                uint32_t wf[2][NT][2];
 #pragma unroll
-                    for (int x = 0; x < NT; ++x) {
-                        const float r0 = m[x][0] == -INFINITY ? 0.f : m[x][0], r1 = m[x][1] == -INFINITY ? 0.f : m[x][1];
-                        const float w0 = ex2(s[x][0] - r0), w1 = ex2(s[x][1] - r1), w2 = ex2(s[x][2] - r0), w3 = ex2(s[x][3] - r1);
-                        l[x][0] = __fmaf_rn(w0 + w2, rv, l[x][0]);
-                        l[x][1] = __fmaf_rn(w1 + w3, rv, l[x][1]);
-                        wf[x][0] = movmatrix_trans(pack_half2(w0, w1));
-                        wf[x][1] = movmatrix_trans(pack_half2(w2, w3));
+                for (int x = 0; x < NT; ++x) {
+                    const float r[2] = {m[x][0] == -INFINITY ? 0.f : m[x][0], m[x][1] == -INFINITY ? 0.f : m[x][1]};
+#pragma unroll
+                    for (int half = 0; half < 2; ++half) {
+                        float w[4];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) w[i] = ex2(s[half][x][i] - r[i & 1]);
+                        l[x][0] = __fmaf_rn(w[0] + w[2], rv[half], l[x][0]);
+                        l[x][1] = __fmaf_rn(w[1] + w[3], rv[half], l[x][1]);
+                        wf[half][x][0] = movmatrix_trans(pack_half2(w[0], w[1]));
+                        wf[half][x][1] = movmatrix_trans(pack_half2(w[2], w[3]));
                     }
-                    // ---- O^T += V^T W^T: lane (g, t) holds channels (D / 8) g .. of the tokens 2t, 2t + 1, 2t + 8, 2t + 9
+                }
+                // ---- O^T += V^T W^T: lane (g, t) holds channels (D / 8) g .. of the tokens 2t, 2t + 1, 2t + 8, 2t + 9
+#pragma unroll
+                for (int half = 0; half < 2; ++half) {
                     const uint8_t* vt = kt + S::SIDE + half * 16 * D;
                     uint32_t wv[4][D / 32];
 #pragma unroll
@@ -416,12 +490,18 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                             const uint32_t lo = pd_prmt(wv[0][i], wv[1][i], sel), hi = pd_prmt(wv[2][i], wv[3][i], sel);
                             const uint32_t f[4] = {pd_half2<0x4140>(lo), pd_half2<0x4342>(lo), pd_half2<0x4140>(hi), pd_half2<0x4342>(hi)};
 #pragma unroll
-                            for (int x = 0; x < NT; ++x) mma16816(o[x][2 * i + b], f, wf[x][0], wf[x][1]);
+                            for (int x = 0; x < NT; ++x) mma16816(o[x][2 * i + b], f, wf[half][x][0], wf[half][x][1]);
                         }
                     }
                 }
                 __syncwarp();                                    // every lane has read the stage: refill it
                 copy();
+            }
+            const int next = cur + p.b - p.a;
+            PdPiece pn{};
+            if (next < u1) {                                     // the next piece's queries arrive during the joining
+                pn = pd_piece(W, next, u1);
+                load_q(pn);
             }
             // ---- join the warps: row sums, then O, 8 rows at a time
             asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");           // the last join's reads are done
@@ -487,27 +567,22 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 }
             }
             if (!whole) {
-                // the units of this (sequence, head, group) belong to the CTAs c0 .. c1; the last of them to arrive joins
-                const int64_t v0 = cur - p.a, v1 = v0 + p.units;
-                auto owner = [&](int64_t u) {                    // the CTA whose run holds unit u
-                    int c = int(u * ctas / work);
-                    while (work * (c + 1) / ctas <= u) ++c;
-                    while (work * c / ctas > u) --c;
-                    return c;
-                };
-                const int c0 = owner(v0), c1 = owner(v1 - 1);
-                __threadfence();
+                // its units belong to the CTAs c0 .. c1; the last of them to arrive joins
+                const int c0 = W.holder(p.v0 + PD_FIXED), c1 = W.holder(p.v0 + PD_FIXED + p.units - 1);
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
                 if (threadIdx.x == 0) {
+                    __threadfence();
                     const uint32_t seen = atomicAdd(&A.count[c0], 1u);
                     s_last = seen == uint32_t(c1 - c0);
                     if (s_last) A.count[c0] = 0;
                     else if (seen > uint32_t(c1 - c0)) raise_status(KVB_DEV_WORKSPACE);
+                    __threadfence();
                 }
                 asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
                 if (s_last) {
-                    __threadfence();
-                    auto slot_of = [&](int c) { return A.part + int64_t(2 * c + (work * c / ctas >= v0 ? 0 : 1)) * S::PART; };
+                    // the partial of c is its first one, unless the (sequence, head, group) begins inside c's run
+                    const float* slot0 = A.part + int64_t(2 * c0 + (W.share(c0) < p.v0 ? 1 : 0)) * S::PART;
+                    auto slot_of = [&](int c) { return c == c0 ? slot0 : A.part + int64_t(2 * c) * S::PART; };
                     for (int r = warp; r < nrows; r += PD_WARPS) {
                         float top = -INFINITY;
                         for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot_of(c) + r));
@@ -517,16 +592,20 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                         float2 acc[D / 64];
 #pragma unroll
                         for (int i = 0; i < D / 64; ++i) acc[i] = float2{0.f, 0.f};
-#pragma unroll 4
-                        for (int c = c0; c <= c1; ++c) {
-                            const float* q = slot_of(c);
-                            const float f = ex2(__ldcg(q + r) - ref);
-                            sum = __fmaf_rn(__ldcg(q + S::ROWS + r), f, sum);
+                        for (int cc = c0; cc <= c1; cc += 32) {
+                            const int mine_c = min(cc + lane, c1);
+                            const float f_mine = ex2(__ldcg(slot_of(mine_c) + r) - ref), l_mine = __ldcg(slot_of(mine_c) + S::ROWS + r);
+#pragma unroll 8
+                            for (int k = 0; k < min(32, c1 - cc + 1); ++k) {
+                                const float f = __shfl_sync(0xffffffffu, f_mine, k);
+                                sum = __fmaf_rn(__shfl_sync(0xffffffffu, l_mine, k), f, sum);
+                                const float* q = slot_of(cc + k) + 2 * S::ROWS + r * D + 2 * lane;
 #pragma unroll
-                            for (int i = 0; i < D / 64; ++i) {
-                                const float2 v = __ldcg(reinterpret_cast<const float2*>(q + 2 * S::ROWS + r * D + 2 * lane + 64 * i));
-                                acc[i].x = __fmaf_rn(v.x, f, acc[i].x);
-                                acc[i].y = __fmaf_rn(v.y, f, acc[i].y);
+                                for (int i = 0; i < D / 64; ++i) {
+                                    const float2 v = __ldcg(reinterpret_cast<const float2*>(q + 64 * i));
+                                    acc[i].x = __fmaf_rn(v.x, f, acc[i].x);
+                                    acc[i].y = __fmaf_rn(v.y, f, acc[i].y);
+                                }
                             }
                         }
 #pragma unroll
@@ -535,11 +614,11 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                     }
                 }
             }
-            cur += p.b - p.a;
+            cur = next;
+            p = pn;
             first = 0;
         }
     }
-
     if (*abort) {                                                // copies in flight land before shared memory is released
         if (lane == 0) {
             raise_status(KVB_DEV_TIMEOUT);
