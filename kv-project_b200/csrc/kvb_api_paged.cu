@@ -50,7 +50,7 @@ kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
         a.out = out + i * per * D * 2;
         a.lse = lse ? lse + i * per : nullptr;
         a.slots = slots + i;
-        kern<<<grid, kvb::PD_THREADS, SM, s>>>(a);
+        kern<<<grid, kvb::PdShape<D, NT>::THREADS, SM, s>>>(a);
         if (kvb_status st = launch_check("page_attend")) return st;
     }
     return KVB_OK;

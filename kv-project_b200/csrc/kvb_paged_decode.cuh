@@ -34,10 +34,8 @@
 
 namespace kvb {
 
-constexpr int PD_WARPS = 8;
-constexpr int PD_THREADS = 32 * PD_WARPS;
 constexpr int PD_UNIT = 32;                   // tokens
-constexpr int PD_MAX_SEQS = 1024;             // sequences of one launch (their offsets are in shared memory)
+constexpr int PD_MAX_SEQS = 512;              // sequences of one launch (their offsets are in shared memory)
 constexpr int PD_MAX_CTAS = 256;
 constexpr int PD_FIXED = 12;                  // what a (sequence, head, group) costs beside its units, in units
 constexpr int PD_LEAST = 4;                   // a CTA's least share
@@ -58,13 +56,15 @@ struct PagedDecodeParams {
 
 template <int D, int NT>
 struct PdShape {
+    static constexpr int WARPS = 8;                             // 12 with two stages each: 104 against 103 us (8 x 32768), 109 against 89 (ragged)
+    static constexpr int THREADS = 32 * WARPS;
     static constexpr int ROWS = 8 * NT;
     static constexpr int SIDE = PD_UNIT * D;                    // bytes of one side of a unit
     static constexpr int STAGE = 2 * SIDE;
-    static constexpr int STAGES = D == 128 ? 3 : 6;             // per warp
-    static constexpr int JOIN = PD_WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
+    static constexpr int STAGES = 3 * (128 / D);             // per warp
+    static constexpr int JOIN = WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
     static constexpr int PART = ROWS * (D + 2);
-    static constexpr int SMEM = 1024 + PD_WARPS * STAGES * STAGE + JOIN;
+    static constexpr int SMEM = 1024 + WARPS * STAGES * STAGE + JOIN;
 };
 
 // The work of a call: per (sequence, KV head, row group) its units, and PD_FIXED more in the shares that the CTAs get
@@ -118,10 +118,14 @@ __device__ __forceinline__ PdPiece pd_piece(const PdPlan& W, int cur, int end) {
 
 __device__ __forceinline__ uint32_t pd_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
 
+// bytes -> two fp16 values 1024 + code
+template <uint32_t SEL>
+__device__ __forceinline__ uint32_t pd_raw2(uint32_t w) { return pd_prmt(w, 0x64646464u, SEL); }
+
 // bytes -> two fp16 values code - 128 (exact)
 template <uint32_t SEL>
 __device__ __forceinline__ uint32_t pd_half2(uint32_t w) {
-    const uint32_t x = pd_prmt(w, 0x64646464u, SEL);
+    const uint32_t x = pd_raw2<SEL>(w);
     uint32_t y;
     asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(y) : "r"(x), "r"(0x64806480u));      // 1152
     return y;
@@ -143,31 +147,31 @@ __device__ __forceinline__ int pd_exponent(float amax) {
 }
 
 template <typename T, int D, int NT>
-__global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __grid_constant__ PagedDecodeParams A) {
+__global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kernel(const __grid_constant__ PagedDecodeParams A) {
     using S = PdShape<D, NT>;
     constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
     extern __shared__ uint8_t pd_raw[];
     __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS];
-    __shared__ uint64_t full[PD_WARPS][S::STAGES];
-    __shared__ float s_m[PD_WARPS][S::ROWS], s_l[PD_WARPS][S::ROWS];
-    __shared__ int warp_sum[PD_WARPS];
+    __shared__ uint64_t full[S::WARPS][S::STAGES];
+    __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS];
+    __shared__ int warp_sum[S::WARPS];
     __shared__ int s_abort, s_last;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
-    float* join = reinterpret_cast<float*>(base + PD_WARPS * S::STAGES * S::STAGE);      // [warp][8 rows][64 + 4]
+    float* join = reinterpret_cast<float*>(base + S::WARPS * S::STAGES * S::STAGE);      // [warp][8 rows][64 + 4]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     uint8_t* ring = base + warp * S::STAGES * S::STAGE;
     const PagesView& P = A.P;
 
     if (threadIdx.x == 0) {
-        for (int i = 0; i < PD_WARPS * S::STAGES; ++i) mbar_init(&full[0][i], 1);
+        for (int i = 0; i < S::WARPS * S::STAGES; ++i) mbar_init(&full[0][i], 1);
         s_abort = 0;
         fence_mbar_init();
         pre[0] = 0;
     }
-    // units before each sequence: an inclusive scan, PD_THREADS sequences at a time; an empty sequence is one unit
+    // units before each sequence: an inclusive scan, S::THREADS sequences at a time; an empty sequence is one unit
     // without keys, whose rows still have to be written
     int before = 0;
-    for (int i0 = 0; i0 < A.n; i0 += PD_THREADS) {
+    for (int i0 = 0; i0 < A.n; i0 += S::THREADS) {
         const int i = i0 + threadIdx.x;
         int u = 0;
         if (i < A.n) {
@@ -189,7 +193,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         if (lane == 31) warp_sum[warp] = x;
         __syncthreads();
         int sum = 0;
-        for (int w = 0; w < PD_WARPS; ++w) {
+        for (int w = 0; w < S::WARPS; ++w) {
             if (w == warp) x += sum;
             sum += warp_sum[w];
         }
@@ -252,16 +256,16 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         load_q(p);
     }
 
-    // ---------------- copies: the warp's unit k is the CTA's unit warp + 8 k; lane i looks after the units k = i mod 32 ----------------
+    // ---------------- copies: the warp's unit k is the CTA's unit warp + S::WARPS k; lane i looks after the units k = i mod 32 ----------------
     struct Place {
         int row[2], off;                                         // rows of the tensor maps (< 0: nothing there), token in the page
     };
     const int box = min(P.page, PD_UNIT);
-    const int mine = max(0, (u1 - u0 - warp + PD_WARPS - 1) / PD_WARPS);                 // units of this warp
+    const int mine = max(0, (u1 - u0 - warp + S::WARPS - 1) / S::WARPS);                 // units of this warp
     auto place = [&](int k) {
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
-        const PdPiece p = pd_piece(W, u0 + warp + k * PD_WARPS, u1);
+        const PdPiece p = pd_piece(W, u0 + warp + k * S::WARPS, u1);
         const int h = p.vh / A.groups, t0 = p.a * PD_UNIT, len = s_len[p.seq];
         x.off = t0 % P.page;
 #pragma unroll
@@ -273,14 +277,15 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
         }
         return x;
     };
-    auto scales_of = [&](const Place& x) {                       // ks, ks of the tokens 16 .., vs, vs
+    auto scales_of = [&](const Place& x) {                       // ks and vs of the tokens 0 .. and 16 ..
         float4 f{0.f, 0.f, 0.f, 0.f};
         if (x.row[0] >= 0) f.x = f.y = P.ks[x.row[0]], f.z = f.w = P.vs[x.row[0]];
         if (x.row[1] >= 0) f.y = P.ks[x.row[1]], f.w = P.vs[x.row[1]];
         return f;
     };
+    auto log_scale = [](float v) { return v > 0.f ? __log2f(v) : 0.f; };      // a page of zeros: any scale does
     Place at = place(lane), ahead{};                             // of the units being copied, and of the 32 after
-    float4 sc_now{0.f, 0.f, 0.f, 0.f}, sc_next{0.f, 0.f, 0.f, 0.f};      // scales of the units being computed, and of the next
+    float4 sc_now{0.f, 0.f, 0.f, 0.f}, sc_next{0.f, 0.f, 0.f, 0.f};      // ks, log2 vs of the units being computed; scales of the next
     int copied = 0;
     auto copy = [&]() {                                          // the warp's next unit
         if (copied >= mine) return;
@@ -311,7 +316,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
             const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
-            float lam[NT][2];
+            float lam[NT][2], bias[NT][2];                       // bias: -1152 sum q, what the codes' pattern adds
             int lim[NT][2];                                      // keys that the rows 2t, 2t + 1 see
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
@@ -329,19 +334,26 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
                 const int e = pd_exponent(amax);
                 const float up = __uint_as_float(uint32_t(127 + e) << 23);
+                float sum = 0.f;
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) {
                     const uint32_t ws[4] = {raw[x][i].x, raw[x][i].y, raw[x][i].z, raw[x][i].w};
 #pragma unroll
                     for (int k = 0; k < 4; ++k) {
                         const float2 f = pd_pair<T>(ws[k]);
-                        qf[x][2 * i + (k >> 1)][k & 1] = pack_half2(f.x * up, f.y * up);
+                        const uint32_t qh = pack_half2(f.x * up, f.y * up);
+                        qf[x][2 * i + (k >> 1)][k & 1] = qh;
+                        const float2 r = unpack_half2(qh);
+                        sum += r.x + r.y;
                     }
                 }
+                sum += __shfl_xor_sync(0xffffffffu, sum, 1);
+                sum += __shfl_xor_sync(0xffffffffu, sum, 2);
                 const float down = A.lam * __uint_as_float(uint32_t(127 - e) << 23);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     lam[x][k] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + k));
+                    bias[x][k] = -1152.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + k));
                     lim[x][k] = len - A.Tq + (row0 + 8 * x + 2 * t + k) / A.rep + 1;
                 }
             }
@@ -354,13 +366,14 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 for (int c = 0; c < KS; ++c) o[x][c][0] = o[x][c][1] = o[x][c][2] = o[x][c][3] = 0.f;
             }
             // the first unit of the piece that is this warp's (units go to the warps in turn over the CTA's whole run)
-            for (int k = (warp - (cur - u0)) & (PD_WARPS - 1); k < p.b - p.a; k += PD_WARPS, ++unit) {
+            const int lead = (cur - u0) % S::WARPS;
+            for (int k = warp < lead ? warp - lead + S::WARPS : warp - lead; k < p.b - p.a; k += S::WARPS, ++unit) {
                 const int st = unit % S::STAGES;
                 if (!__all_sync(0xffffffffu, wait(&full[warp][st], unit / S::STAGES))) continue;
-                if ((unit & 31) == 0) sc_now = sc_next;
+                if ((unit & 31) == 0) sc_now = float4{sc_next.x, sc_next.y, log_scale(sc_next.z), log_scale(sc_next.w)};
                 const int src = unit & 31;
                 const float ks[2] = {__shfl_sync(0xffffffffu, sc_now.x, src), __shfl_sync(0xffffffffu, sc_now.y, src)};
-                float vs[2] = {__shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
+                const float lv[2] = {__shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
                 const int t0 = (p.a + k) * PD_UNIT;
                 const uint8_t* kt = ring + st * S::STAGE;
                 const bool edge = t0 + PD_UNIT > len - A.Tq + 1;
@@ -373,7 +386,9 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
 #pragma unroll
                     for (int c = 0; c < 2; ++c)
 #pragma unroll
-                        for (int x = 0; x < NT; ++x) s2[c][x][0] = s2[c][x][1] = s2[c][x][2] = s2[c][x][3] = 0.f;
+                        for (int x = 0; x < NT; ++x)
+#pragma unroll
+                            for (int i = 0; i < 4; ++i) s2[c][x][i] = c ? 0.f : bias[x][i & 1];
 #pragma unroll
                     for (int c = 0; c < D / 64; ++c) {
                         uint4 a, b;
@@ -389,8 +404,8 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                         const uint32_t wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
                         for (int i = 0; i < 4; ++i) {
-                            const uint32_t f[4] = {pd_half2<0x4140>(wa[i]), pd_half2<0x4140>(wb[i]), pd_half2<0x4342>(wa[i]),
-                                                   pd_half2<0x4342>(wb[i])};
+                            const uint32_t f[4] = {pd_raw2<0x4140>(wa[i]), pd_raw2<0x4140>(wb[i]), pd_raw2<0x4342>(wa[i]),
+                                                   pd_raw2<0x4342>(wb[i])};
 #pragma unroll
                             for (int x = 0; x < NT; ++x) mma16816(s2[i & 1][x], f, qf[x][4 * c + i][0], qf[x][4 * c + i][1]);
                         }
@@ -401,17 +416,14 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                         for (int i = 0; i < 4; ++i) s[half][x][i] = s2[0][x][i] + s2[1][x][i];
                 }
                 // ---- weights: y = s + log2 vs; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1 of either half
-                float rv[2];
+                const float rv[2] = {ex2(-lv[0]), ex2(-lv[1])};
                 bool grow = false;
 #pragma unroll
                 for (int half = 0; half < 2; ++half) {
-                    vs[half] = vs[half] > 0.f ? vs[half] : 1.f;  // a page of zeros: any scale does
-                    rv[half] = __frcp_rn(vs[half]);
-                    const float lv = __log2f(vs[half]);
 #pragma unroll
                     for (int x = 0; x < NT; ++x)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[half][x][i] = __fmaf_rn(s[half][x][i], lam[x][i & 1] * ks[half], lv);
+                        for (int i = 0; i < 4; ++i) s[half][x][i] = __fmaf_rn(s[half][x][i], lam[x][i & 1] * ks[half], lv[half]);
                 }
                 if (edge) {
 #pragma unroll
@@ -504,7 +516,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                 load_q(pn);
             }
             // ---- join the warps: row sums, then O, 8 rows at a time
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");           // the last join's reads are done
+            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");           // the last join's reads are done
 #pragma unroll
             for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -524,30 +536,30 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
             for (int x = 0; x < NT; ++x) {
                 // warp w joins query row 8 x + w; column c of the buffer is channel (D / 8) (c / 8) + 8 y + c % 8
                 const int r = 8 * x + warp;
-                float top = -INFINITY, sum = 0.f, f[PD_WARPS];
+                float top = -INFINITY, sum = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
-                    if (x + y > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                    if (x + y > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                     float* to = join + warp * 8 * 68 + 2 * t * 68 + 8 * g;
 #pragma unroll
                     for (int c = 0; c < 4; ++c) {
                         *reinterpret_cast<float2*>(to + 2 * c) = float2{o[x][4 * y + c][0], o[x][4 * y + c][2]};
                         *reinterpret_cast<float2*>(to + 68 + 2 * c) = float2{o[x][4 * y + c][1], o[x][4 * y + c][3]};
                     }
-                    asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                    asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                     if (y == 0) {
 #pragma unroll
-                        for (int w = 0; w < PD_WARPS; ++w) top = fmaxf(top, s_m[w][r]);
+                        for (int w = 0; w < S::WARPS; ++w) top = fmaxf(top, s_m[w][r]);
                         const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
-                        for (int w = 0; w < PD_WARPS; ++w) {
+                        for (int w = 0; w < S::WARPS; ++w) {
                             f[w] = ex2(s_m[w][r] - ref);
                             sum = __fmaf_rn(s_l[w][r], f[w], sum);
                         }
                     }
                     float2 acc{0.f, 0.f};
 #pragma unroll
-                    for (int w = 0; w < PD_WARPS; ++w) {
+                    for (int w = 0; w < S::WARPS; ++w) {
                         const float2 v = *reinterpret_cast<const float2*>(join + (w * 8 + warp) * 68 + 2 * lane);
                         acc.x = __fmaf_rn(v.x, f[w], acc.x);
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
@@ -569,7 +581,7 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
             if (!whole) {
                 // its units belong to the CTAs c0 .. c1; the last of them to arrive joins
                 const int c0 = W.holder(p.v0 + PD_FIXED), c1 = W.holder(p.v0 + PD_FIXED + p.units - 1);
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                 if (threadIdx.x == 0) {
                     __threadfence();
                     const uint32_t seen = atomicAdd(&A.count[c0], 1u);
@@ -578,12 +590,12 @@ __global__ void __launch_bounds__(PD_THREADS, 1) paged_decode_kernel(const __gri
                     else if (seen > uint32_t(c1 - c0)) raise_status(KVB_DEV_WORKSPACE);
                     __threadfence();
                 }
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * PD_WARPS) : "memory");
+                asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                 if (s_last) {
                     // the partial of c is its first one, unless the (sequence, head, group) begins inside c's run
                     const float* slot0 = A.part + int64_t(2 * c0 + (W.share(c0) < p.v0 ? 1 : 0)) * S::PART;
                     auto slot_of = [&](int c) { return c == c0 ? slot0 : A.part + int64_t(2 * c) * S::PART; };
-                    for (int r = warp; r < nrows; r += PD_WARPS) {
+                    for (int r = warp; r < nrows; r += S::WARPS) {
                         float top = -INFINITY;
                         for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot_of(c) + r));
                         top = warp_max(top);
