@@ -103,13 +103,36 @@ __host__ __device__ constexpr uint32_t pf_idesc(int N, int bf16, int b_mn) {
            (uint32_t(128 >> 4) << 24);
 }
 
-// D[tmem] (+)= A[tmem] B[smem]
-__device__ __forceinline__ void umma_f16_ts(uint32_t tmem_d, uint32_t tmem_a, uint64_t b, uint32_t idesc, int acc) {
+// The MMA warp runs converged, so that descriptors stay in uniform registers (issued from a divergent branch of one lane an
+// MMA took 91 cycles, 64 is its time on the tensor core); `lead` is set in the one lane that issues.
+__device__ __forceinline__ uint32_t pf_elect() {
+    uint32_t lead;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(lead));
+    return lead;
+}
+// D[tmem] (+)= A[smem] B[smem]
+__device__ __forceinline__ void pf_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "setp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(tmem_d),
-        "r"(tmem_a), "l"(b), "r"(idesc), "r"(acc)
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+// D[tmem] (+)= A[tmem] B[smem]
+__device__ __forceinline__ void pf_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+    asm volatile(
+        "{\n\t.reg .pred p, q;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
+        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        : "memory");
+}
+__device__ __forceinline__ void pf_commit(uint32_t lead, uint64_t* bar) {
+    asm volatile(
+        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
+        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
+        "r"(lead)
         : "memory");
 }
 
@@ -305,6 +328,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
     volatile int* abort = &sh.abort;
     // a wait that gave up stops every role
     auto wait = [&](uint64_t* bar, uint32_t count) {
+        if (mbar_try_wait(bar, count & 1)) return true;
         if (*abort) return false;
         if (mbar_wait(bar, count & 1)) return true;
         *abort = 1;
@@ -358,65 +382,78 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         }
     } else if (warp == 9) {
         // ---------------- MMA issue ----------------
-        if (lane == 0) {
-            constexpr uint32_t IDESC_S = pf_idesc(PF_KT, BF16, 0), IDESC_O = pf_idesc(D, BF16, 1);
-            uint32_t kv = 0, items = 0, pv[2] = {0, 0};
-            bool ok = true;
-            auto stage = [&](uint32_t c) { return smem_u32(skv + (c % S::STAGES) * S::TILE_BYTES); };
-            auto scores = [&](int w, uint32_t kst) {             // S_w = Q_w K^T
-                const uint32_t a = smem_u32(sq + w * S::TILE_BYTES), b = stage(kst);
+        constexpr uint32_t IDESC_S = pf_idesc(PF_KT, BF16, 0), IDESC_O = pf_idesc(D, BF16, 1);
+        const uint32_t lead = pf_elect(), tm = __shfl_sync(0xffffffffu, tmem, 0);
+        const uint64_t q_desc = umma_desc_sw128(smem_u32(sq)), k_desc = umma_desc_sw128(smem_u32(skv)),
+                       v_desc = pf_desc_mn(smem_u32(skv), 128 * 128);
+        auto all = [&](bool b) { return __all_sync(0xffffffffu, b) != 0; };
+        uint32_t items = 0, pv[2] = {0, 0};
+        uint32_t st = 0, ph = 0;                                 // stage and phase of the next load to be used
+        auto next = [&]() {
+            if (++st == S::STAGES) { st = 0; ph ^= 1; }
+        };
+        // descriptor addresses count 16 bytes
+        auto scores = [&](int w, uint32_t kst) {                 // S_w = Q_w K^T
+            const uint64_t a = q_desc + uint32_t(w * (S::TILE_BYTES >> 4)), b = k_desc + kst * uint32_t(S::TILE_BYTES >> 4);
 #pragma unroll
-                for (int k = 0; k < D / 16; ++k) {
-                    const uint32_t off = (k >> 2) * (128 * 128) + (k & 3) * 32;
-                    umma_f16(tmem + uint32_t(w * PF_KT), umma_desc_sw128(a + off), umma_desc_sw128(b + off), IDESC_S, k != 0);
-                }
-                umma_commit(&sh.s_full[w]);
-            };
-            for (int64_t round = 0; ok; ++round) {
-                if (!wait(&sh.item_full[round & 1], uint32_t(round / 2))) break;
-                const PfItem& x = sh.item[round & 1];
-                const int n0 = x.n[0], n1 = x.n[1], head = x.head;
-                mbar_arrive(&sh.item_empty[round & 1]);
-                if (head < 0) break;
-                const int nt = max(n0, n1);
-                if (nt == 0) continue;
-                const uint32_t k0 = kv;                          // K(j) is load k0 + 2 j, V(j) the one after
-                kv += 2 * nt;
-                ok = wait(&sh.q_full, items) && wait(&sh.kv_full[k0 % S::STAGES], k0 / S::STAGES);
-                ++items;
-                if (!ok) break;
-                tc_fence_after();
-                for (int w = 0; w < 2; ++w)
-                    if ((w ? n1 : n0) > 0) scores(w, k0);
-                umma_commit(&sh.kv_empty[k0 % S::STAGES]);
-                if (nt == 1) umma_commit(&sh.q_empty);
-                for (int j = 0; ok && j < nt; ++j) {
-                    const uint32_t vj = k0 + 2 * j + 1, kn = vj + 1;
-                    ok = wait(&sh.kv_full[vj % S::STAGES], vj / S::STAGES);
-                    if (ok && j + 1 < nt) ok = wait(&sh.kv_full[kn % S::STAGES], kn / S::STAGES);
-                    for (int w = 0; ok && w < 2; ++w) {
-                        const int n = w ? n1 : n0;
-                        if (j >= n) continue;
-                        if (!(ok = wait(&sh.p_full[w], pv[w]++))) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int k = 0; k < PF_KT / 16; ++k)     // O_w += P_w V
-                            umma_f16_ts(tmem + 256 + uint32_t(w * D), tmem + uint32_t(w * PF_KT + k * 8),
-                                        pf_desc_mn(stage(vj) + k * 2048, 128 * 128), IDESC_O, j != 0 || k != 0);
-                        umma_commit(&sh.o_full[w]);
-                        if (j + 1 < n) scores(w, kn);
-                    }
-                    if (!ok) break;
-                    umma_commit(&sh.kv_empty[vj % S::STAGES]);
-                    if (j + 1 < nt) umma_commit(&sh.kv_empty[kn % S::STAGES]);
-                    if (j + 2 == nt) umma_commit(&sh.q_empty);   // the last scores are issued
-                }
+            for (int k = 0; k < D / 16; ++k) {
+                const uint32_t off = ((k >> 2) * (128 * 128) + (k & 3) * 32) >> 4;
+                pf_mma_ss(lead, tm + uint32_t(w * PF_KT), a + off, b + off, IDESC_S, k != 0);
             }
-            // after a timeout the MMAs already issued finish before tensor memory is released
-            if (*abort)
-                for (int w = 0; w < 2; ++w)
-                    if (pv[w] > 0) mbar_wait(&sh.o_full[w], (pv[w] - 1) & 1, 10000000ull);
+            pf_commit(lead, &sh.s_full[w]);
+        };
+        bool ok = true;
+        for (int64_t round = 0; ok; ++round) {
+            if (!all(wait(&sh.item_full[round & 1], uint32_t(round / 2)))) break;
+            const PfItem& x = sh.item[round & 1];
+            const int n0 = __shfl_sync(0xffffffffu, x.n[0], 0), n1 = __shfl_sync(0xffffffffu, x.n[1], 0);
+            const int head = __shfl_sync(0xffffffffu, x.head, 0);
+            __syncwarp();
+            if (lane == 0) mbar_arrive(&sh.item_empty[round & 1]);
+            if (head < 0) break;
+            const int nt = max(n0, n1);
+            if (nt == 0) continue;
+            ok = all(wait(&sh.q_full, items) && wait(&sh.kv_full[st], ph));
+            ++items;
+            if (!ok) break;
+            tc_fence_after();
+            for (int w = 0; w < 2; ++w)
+                if ((w ? n1 : n0) > 0) scores(w, st);
+            pf_commit(lead, &sh.kv_empty[st]);
+            if (nt == 1) pf_commit(lead, &sh.q_empty);
+            next();
+            for (int j = 0; ok && j < nt; ++j) {
+                const uint32_t vst = st;                         // V(j), then K(j + 1)
+                ok = all(wait(&sh.kv_full[st], ph));
+                next();
+                const uint32_t kst = st;
+                const bool more = j + 1 < nt;
+                if (ok && more) ok = all(wait(&sh.kv_full[st], ph));
+                if (more) next();
+                for (int w = 0; ok && w < 2; ++w) {
+                    const int n = w ? n1 : n0;
+                    if (j >= n) continue;
+                    ok = all(wait(&sh.p_full[w], pv[w]++));
+                    if (!ok) break;
+                    tc_fence_after();
+                    const uint64_t v = v_desc + vst * uint32_t(S::TILE_BYTES >> 4);
+#pragma unroll
+                    for (int k = 0; k < PF_KT / 16; ++k)         // O_w += P_w V
+                        pf_mma_ts(lead, tm + 256 + uint32_t(w * D), tm + uint32_t(w * PF_KT + k * 8), v + uint32_t(k * (2048 >> 4)), IDESC_O,
+                                  j != 0 || k != 0);
+                    pf_commit(lead, &sh.o_full[w]);
+                    if (j + 1 < n) scores(w, kst);
+                }
+                if (!ok) break;
+                pf_commit(lead, &sh.kv_empty[vst]);
+                if (more) pf_commit(lead, &sh.kv_empty[kst]);
+                if (j + 2 == nt) pf_commit(lead, &sh.q_empty);   // the last scores are issued
+            }
         }
+        // after a timeout the MMAs already issued finish before tensor memory is released
+        if (*abort)
+            for (int w = 0; w < 2; ++w)
+                if (pv[w] > 0) mbar_wait(&sh.o_full[w], (pv[w] - 1) & 1, 10000000ull);
     }
     } else {
         asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFTMAX));
