@@ -17,6 +17,15 @@
 // row's maximum grew by more than 2^8 (P then reaches 256 at most, well inside float16's range; the sums stay in
 // float32), which is seldom after the first tiles.
 //
+// A tile's step is a chain (logits from the tensor cores, weights, the two products), the other tile's fills its gaps, and
+// what the chain costs beside the products bounds the kernel.  So: the weights are computed with the reference maximum
+// so far while the new maximum is taken (the tile is redone in the rare case that it grew too far); P is handed over
+// in two parts, 96 columns and 32, and the first part's product runs while the second is computed; and the MMA warp
+// runs converged.  16384 tokens, 32 heads over 8, d 128: 2102 us without these three, 1885 with the converged warp, 1799
+// with the early weights and P in halves, 1728 with the masked tiles known ahead, 1649 with P in 96 + 32 and 224
+// registers (1334 TFLOP/s).  Measured and left: two threads a row (1971), steps of 64 keys with two score buffers (1894), an MMA warp
+// per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906).
+//
 // Masks: logits of keys past a row's limit become -inf by selection, so what lies there does not matter; values
 // there would still meet a weight of zero in the MMA (0 * NaN), so in tiles that some row of the item does not see
 // whole, value rows past the sequence become zeros in shared memory, and non-finite entries of the sequence's own
@@ -41,8 +50,8 @@ namespace kvb {
 
 constexpr int PF_KT = 128;                    // keys per tile
 constexpr int PF_THREADS = 384;               // warps 10 and 11 only give up their registers
-// registers of a thread in the softmax warpgroups and in the third: 2 x 128 x 208 + 128 x 88 = 384 x 168, the launch's
-constexpr int PF_REGS_SOFTMAX = 208, PF_REGS_REST = 88;
+// registers of a thread in the softmax warpgroups and in the third: 2 x 128 x 224 + 128 x 56 = 384 x 168, the launch's
+constexpr int PF_REGS_SOFTMAX = 224, PF_REGS_REST = 56;
 constexpr int PF_TMEM_COLS = 512;
 constexpr float PF_LAZY = 8.f;                // log2 of how far a maximum may grow before O is rescaled
 
@@ -82,7 +91,7 @@ struct PfItem {
 struct PfShared {
     uint64_t q_full, q_empty;
     uint64_t kv_full[8], kv_empty[8];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_most[2], p_full[2], o_full[2];        // p_most: the first 96 columns of P
     uint64_t item_full[2], item_empty[2];
     uint32_t tmem;
     int abort;
@@ -162,6 +171,12 @@ __device__ __forceinline__ void pf_st32(uint32_t addr, const uint32_t* r) {
         PF_W8(r, 8), PF_W8(r, 16), PF_W8(r, 24), "r"(addr)
         : "memory");
 }
+__device__ __forceinline__ void pf_st16(uint32_t addr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%16], {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15};" ::PF_W8(r, 0),
+        PF_W8(r, 8), "r"(addr)
+        : "memory");
+}
 __device__ __forceinline__ void pf_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void pf_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
@@ -173,6 +188,45 @@ template <>
 __device__ __forceinline__ uint32_t pf_pack<__nv_bfloat16>(float lo, float hi) {
     __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
     return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Two float32 operations in one instruction.
+__device__ __forceinline__ uint64_t pf_two(float a, float b) {
+    uint64_t d;
+    asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float2 pf_split(uint64_t a) {
+    float2 d;
+    asm("mov.b64 {%0, %1}, %2;" : "=f"(d.x), "=f"(d.y) : "l"(a));
+    return d;
+}
+__device__ __forceinline__ uint64_t pf_fma2(uint64_t a, uint64_t b, uint64_t c) {
+    uint64_t d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+    return d;
+}
+__device__ __forceinline__ uint64_t pf_add2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
+__device__ __forceinline__ float pf_max3_nan(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+
+// P of 32 columns: 2^(v lam - ref), packed, and their sums added.
+template <typename T>
+__device__ __forceinline__ void pf_weights(const uint32_t* v, uint64_t lam, uint64_t nref, uint32_t* p, uint64_t (&sum)[2]) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const float2 y = pf_split(pf_fma2(pf_two(__uint_as_float(v[2 * i]), __uint_as_float(v[2 * i + 1])), lam, nref));
+        const float a = ex2(y.x), b = ex2(y.y);
+        sum[i & 1] = pf_add2(sum[i & 1], pf_two(a, b));
+        p[i] = pf_pack<T>(a, b);
+    }
 }
 
 // Whether one of the two packed values is not finite: x * 0 is NaN for NaN and infinities only.
@@ -307,6 +361,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         }
         for (int w = 0; w < 2; ++w) {
             mbar_init(&sh.s_full[w], 1);
+            mbar_init(&sh.p_most[w], 4);
             mbar_init(&sh.p_full[w], 4);
             mbar_init(&sh.o_full[w], 1);
             mbar_init(&sh.item_full[w], 1);
@@ -424,23 +479,30 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             next();
             for (int j = 0; ok && j < nt; ++j) {
                 const uint32_t vst = st;                         // V(j), then K(j + 1)
-                ok = all(wait(&sh.kv_full[st], ph));
+                const uint32_t vph = ph;
                 next();
                 const uint32_t kst = st;
                 const bool more = j + 1 < nt;
-                if (ok && more) ok = all(wait(&sh.kv_full[st], ph));
+                ok = all(lane & 1 && more ? wait(&sh.kv_full[kst], ph) : wait(&sh.kv_full[vst], vph));
                 if (more) next();
                 for (int w = 0; ok && w < 2; ++w) {
                     const int n = w ? n1 : n0;
                     if (j >= n) continue;
+                    const uint64_t v = v_desc + vst * uint32_t(S::TILE_BYTES >> 4);
+                    auto values = [&](int k) {                   // O_w += P_w V, 16 tokens
+                        pf_mma_ts(lead, tm + 256 + uint32_t(w * D), tm + uint32_t(w * PF_KT + k * 8), v + uint32_t(k * (2048 >> 4)), IDESC_O,
+                                  j != 0 || k != 0);
+                    };
+                    ok = all(wait(&sh.p_most[w], pv[w]));
+                    if (!ok) break;
+                    tc_fence_after();
+#pragma unroll
+                    for (int k = 0; k < 6; ++k) values(k);
                     ok = all(wait(&sh.p_full[w], pv[w]++));
                     if (!ok) break;
                     tc_fence_after();
-                    const uint64_t v = v_desc + vst * uint32_t(S::TILE_BYTES >> 4);
 #pragma unroll
-                    for (int k = 0; k < PF_KT / 16; ++k)         // O_w += P_w V
-                        pf_mma_ts(lead, tm + 256 + uint32_t(w * D), tm + uint32_t(w * PF_KT + k * 8), v + uint32_t(k * (2048 >> 4)), IDESC_O,
-                                  j != 0 || k != 0);
+                    for (int k = 6; k < PF_KT / 16; ++k) values(k);
                     pf_commit(lead, &sh.o_full[w]);
                     if (j + 1 < n) scores(w, kst);
                 }
@@ -472,6 +534,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             const int tok = x.t0 + w * A.tt + row / A.rep;       // token of the sequence
             const bool valid = row < A.tt * A.rep && tok < x.ql;
             const int limit = valid ? min(max(kl - x.ql + tok + 1, 0), kl) : INT_MAX;    // rows of no token mask nothing
+            const int jmask = __reduce_min_sync(0xffffffffu, limit) / PF_KT;     // first tile that a row of the warp does not see whole
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int j = 0; j < n; ++j, ++steps) {
@@ -486,56 +549,68 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
 #pragma unroll
                     for (int i = 0; i < PF_KT; ++i) v[i] = -v[i];
                 }
+                // The first 64 weights are computed with the reference so far while the maximum is taken: it serves unless
+                // a row's maximum grew by 2^8, has not begun, or is not finite.
                 const int lim = limit - j * PF_KT;
-                if (__any_sync(0xffffffffu, lim < PF_KT)) {
+                const bool masked = j >= jmask;
+                uint32_t p[32];
+                uint64_t sum[2] = {0, 0};
+                auto weights = [&](int c) {                      // of the columns c .. c + 31, into half of p
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    pf_weights<T>(r + c, pf_two(A.lam, A.lam), pf_two(-ref, -ref), p + (c & 32) / 2, sum);
+                };
+                auto maximum = [&]() {
+                    float mx[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 0; i < PF_KT; ++i) v[i] = i < lim ? v[i] : -INFINITY;
+                    for (int i = 4; i < PF_KT - 4; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) mx[k] = pf_max3_nan(mx[k], v[i + k], v[i + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) mx[k] = pf_max3_nan(mx[k], mx[k], v[PF_KT - 4 + k]);
+                    return pf_max3_nan(pf_max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * A.lam;
+                };
+                bool fast = j > 0 && !masked;
+                if (fast) {
+                    weights(0);
+                    weights(32);
+                    const float top = maximum();
+                    fast = !__any_sync(0xffffffffu, valid && !(top <= m + PF_LAZY && m > -INFINITY));
                 }
-                float mx[4] = {v[0], v[1], v[2], v[3]};
+                if (!fast) {
+                    if (masked) {
 #pragma unroll
-                for (int i = 4; i < PF_KT; i += 8) {
+                        for (int i = 0; i < PF_KT; ++i) v[i] = i < lim ? v[i] : -INFINITY;
+                    }
+                    const float top = maximum();
+                    // a row that has seen nothing takes its first maximum as it is; O is zero until then.  NaN and +inf
+                    // make the row NaN, as they do in the formula.
+                    const bool odd = !(top < INFINITY), grow = valid && (top > m + PF_LAZY || odd) && m > -INFINITY;
+                    const float to = odd ? NAN : top;
+                    if (m == -INFINITY) m = to;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        // O holds the sums of the tiles before: wait for them, and scale the rows that grew
+                        const float f = grow ? ex2(m - to) : 1.f;
+                        m = grow ? to : m;
+                        l *= f;
+                        if (j > 0) {
+                            if (!(ok = all(wait(&sh.o_full[w], steps - 1)))) break;
+                            tc_fence_after();
+#pragma unroll 1
+                            for (int c = 0; c < D; c += 32) {
+                                uint32_t o[32];
+                                pf_ld32(o_col + c, o);
+                                pf_wait_ld();
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        mx[k] = i + 4 + k < PF_KT ? fmaxf(fmaxf(mx[k], v[i + k]), v[i + 4 + k]) : fmaxf(mx[k], v[i + k]);
-                }
-                const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3])) * A.lam;
-                // a row that has seen nothing takes its first maximum as it is; O is zero until then
-                if (m == -INFINITY) m = top;
-                const bool grow = valid && top > m + PF_LAZY;
-                if (__any_sync(0xffffffffu, grow)) {
-                    // O holds the sums of the tiles before: wait for them, and scale the rows that grew
-                    const float f = grow ? ex2(m - top) : 1.f;
-                    m = grow ? top : m;
-                    l *= f;
-                    if (j > 0) {
-                        if (!(ok = all(wait(&sh.o_full[w], steps - 1)))) break;
-                        tc_fence_after();
-#pragma unroll
-                        for (int c = 0; c < D; c += 32) {
-                            uint32_t o[32];
-                            pf_ld32(o_col + c, o);
-                            pf_wait_ld();
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                            pf_st32(o_col + c, o);
+                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
+                                pf_st32(o_col + c, o);
+                            }
                         }
                     }
+                    sum[0] = sum[1] = 0;
+                    weights(0);
+                    weights(32);
                 }
-                const float ref = m == -INFINITY ? 0.f : m;
-                float sum[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-                for (int c = 0; c < PF_KT; c += 64) {
-                    uint32_t p[32];
-#pragma unroll
-                    for (int i = 0; i < 64; i += 2) {
-                        const float a = ex2(__fmaf_rn(v[c + i], A.lam, -ref)), b = ex2(__fmaf_rn(v[c + i + 1], A.lam, -ref));
-                        sum[i & 2] += a;
-                        sum[(i & 2) + 1] += b;
-                        p[i / 2] = pf_pack<T>(a, b);
-                    }
-                    pf_st32(s_col + c / 2, p);
-                }
-                l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                pf_st32(s_col, p);
                 if (j >= jm) {
                     // value rows that some row of the item does not see: see the head of this file
                     const uint32_t vj = kv + 2 * j + 1;
@@ -562,6 +637,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                     }
                     fence_proxy_async_smem();
                 }
+                weights(64);
+                pf_st16(s_col + 32, p);
+                pf_wait_st();
+                tc_fence_before();
+                __syncwarp();
+                if (lane == 0) mbar_arrive(&sh.p_most[w]);
+                weights(96);
+                pf_st16(s_col + 48, p + 16);
+                const float2 s0 = pf_split(sum[0]), s1 = pf_split(sum[1]);
+                l += (s0.x + s0.y) + (s1.x + s1.y);
                 pf_wait_st();
                 tc_fence_before();
                 __syncwarp();
