@@ -23,6 +23,17 @@ kvb_status check_rows(const char* who, const kvb_pages* p, const int32_t* slots,
     return KVB_OK;
 }
 
+// Rounds of 8 values a thread that hold a whole page of rows.
+template <typename T>
+void launch_write(const kvb::PageRowsParams& a, dim3 grid, cudaStream_t s) {
+    const int rounds = a.P.page * a.P.d / (8 * kvb::PW_THREADS);
+    if (rounds <= 1) kvb::page_write_kernel<T, 1><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else if (rounds == 2) kvb::page_write_kernel<T, 2><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else if (rounds == 4) kvb::page_write_kernel<T, 4><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else if (rounds == 8) kvb::page_write_kernel<T, 8><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else kvb::page_write_kernel<T, 16><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+}
+
 size_t fork_rows_offset(int n) { return (size_t(64 + 2 * size_t(n)) * 4 + 255) / 256 * 256; }
 
 kvb::ForkWork fork_work(void* ws, int n) {
@@ -63,9 +74,13 @@ kvb_status kvb_page_write(const kvb_pages* p, const int32_t* slots, const int32_
     kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {k, v}, {k_row, v_row}, {k_head, v_head}, {}};
     const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)), unsigned(p->Hkv), 2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == KVB_F32) kvb::page_write_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (dtype == KVB_F16) kvb::page_write_kernel<__half><<<grid, 256, 0, s>>>(a);
-    else kvb::page_write_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    const bool vectors = dtype != KVB_F32 && aligned(k, 16) && aligned(v, 16) && (k_row | k_head | v_row | v_head) % 8 == 0;
+    if (vectors) {
+        if (dtype == KVB_F16) launch_write<__half>(a, grid, s);
+        else launch_write<__nv_bfloat16>(a, grid, s);
+    } else if (dtype == KVB_F32) kvb::page_write_any_kernel<float><<<grid, 256, 0, s>>>(a);
+    else if (dtype == KVB_F16) kvb::page_write_any_kernel<__half><<<grid, 256, 0, s>>>(a);
+    else kvb::page_write_any_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
     return launch_check("page_write");
 }
 
@@ -73,12 +88,13 @@ kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t
                          void* v, int dtype, int64_t rows, void* stream) {
     if (kvb_status st = check_rows("page_read", p, slots, start, cu, n, k, v, dtype, rows)) return st;
     if (n == 0 || rows == 0) return KVB_OK;
+    if (!aligned(k, 16) || !aligned(v, 16)) return fail(KVB_EINVAL, "page_read: k and v need 16-byte alignment");
     kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {}, {}, {}, {k, v}};
     const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)), unsigned(p->Hkv), 2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == KVB_F32) kvb::page_read_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (dtype == KVB_F16) kvb::page_read_kernel<__half><<<grid, 256, 0, s>>>(a);
-    else kvb::page_read_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
+    if (dtype == KVB_F32) kvb::page_read_kernel<float><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else if (dtype == KVB_F16) kvb::page_read_kernel<__half><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    else kvb::page_read_kernel<__nv_bfloat16><<<grid, kvb::PW_THREADS, 0, s>>>(a);
     return launch_check("page_read");
 }
 
@@ -106,7 +122,7 @@ kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* 
     if (n > 0 && (!src || !dst)) return fail(KVB_EINVAL, "page_copy: null argument");
     if (n < 0) return fail(KVB_EINVAL, "page_copy: n >= 0");
     if (n == 0) return KVB_OK;
-    kvb::page_copy_kernel<<<dim3(unsigned(n), 4), 256, 0, static_cast<cudaStream_t>(stream)>>>(kvbh::view_of(p), src, dst);
+    kvb::page_copy_kernel<<<dim3(unsigned(n), 4), kvb::PG_COPY_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(kvbh::view_of(p), src, dst);
     return launch_check("page_copy");
 }
 
@@ -129,7 +145,7 @@ kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     kvb::fork_plan_kernel<<<1, kvb::PG_THREADS, size_t(n + 1) * 4, s>>>(v, src, dst, n, w);
     if (kvb_status st = launch_check("page_fork plan")) return st;
-    kvb::fork_copy_kernel<<<dim3(unsigned(n), 1 + 4), 256, 0, s>>>(v, src, w);
+    kvb::fork_copy_kernel<<<dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s>>>(v, src, w);
     if (kvb_status st = launch_check("page_fork copy")) return st;
     kvb::fork_commit_kernel<<<unsigned(n), 128, 0, s>>>(v, src, dst, w);
     return launch_check("page_fork commit");
@@ -152,7 +168,7 @@ kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     kvb::compact_plan_kernel<<<1, kvb::PG_THREADS, 0, s>>>(v, w);
     if (kvb_status st = launch_check("page_compact plan")) return st;
-    kvb::compact_move_kernel<<<148 * 4, 256, 0, s>>>(v, w, n_live);
+    kvb::compact_move_kernel<<<148 * 4, kvb::PG_COPY_THREADS, 0, s>>>(v, w, n_live);
     return launch_check("page_compact move");
 }
 

@@ -21,6 +21,8 @@
 // small calls the launches.
 #pragma once
 
+#include <type_traits>
+
 #include "kvb_pages_view.cuh"
 
 namespace kvb {
@@ -46,14 +48,14 @@ __device__ __forceinline__ int touch_sequence(const int32_t* cu, int n, int page
 
 // One page's part of a packed write or read.
 struct Touch {
-    int64_t page_id;      // < 0: nothing to do
+    int slot, block;      // the page is table[slot][block]; slot < 0: nothing to do
     int row0, rows;       // rows of the page
     int64_t token0;       // first packed row
 };
 
 __device__ __forceinline__ Touch find_touch(const PagesView& P, const int32_t* slots, const int32_t* start,
                                             const int32_t* cu, int n, int64_t rows, int64_t x) {
-    Touch t{-1, 0, 0, 0};
+    Touch t{-1, 0, 0, 0, 0};
     int64_t slot0;
     const int i = touch_sequence(cu, n, P.page, x, slot0);
     const int a = cu[i], b = cu[i + 1], st = start[i], slot = slots[i];
@@ -65,16 +67,20 @@ __device__ __forceinline__ Touch find_touch(const PagesView& P, const int32_t* s
         raise_status(KVB_DEV_BOUNDS);
         return t;
     }
-    const int id = P.table[int64_t(slot) * P.max_blocks + block];
-    if (id < 0 || id >= P.n_pages) {
-        raise_status(KVB_DEV_BOUNDS);
-        return t;
-    }
-    t.page_id = id;
+    t.slot = slot;
+    t.block = int(block);
     t.row0 = int(lo - block * P.page);
     t.rows = int(hi - lo);
     t.token0 = a + (lo - st);
     return t;
+}
+
+// The page of a touch, or -1 (with the status bit).
+__device__ __forceinline__ int64_t touch_page(const PagesView& P, const Touch& t) {
+    const int id = P.table[int64_t(t.slot) * P.max_blocks + t.block];
+    if (id >= 0 && id < P.n_pages) return id;
+    raise_status(KVB_DEV_BOUNDS);
+    return -1;
 }
 
 // max over the block of non-negative floats
@@ -104,21 +110,37 @@ struct PageRowsParams {
     void* out[2];                  // read: dense (rows, Hkv, d)
 };
 
-// grid (touch slots, Hkv, 2)
+// scale of a page that has `old` and takes rows of magnitude up to a
+__device__ __forceinline__ float page_scale(float old, float a) { return fmaxf(old, a < 0x1p-100f ? 0.f : __fdiv_rn(a, 127.f)); }
+
+// Recode the rows before the first new one for a scale that grew; whole block, 16 codes a thread and round.
+__device__ __forceinline__ void recode_rows(uint8_t* codes, int n, float ratio) {
+    for (int e = threadIdx.x * 16; e < n; e += blockDim.x * 16) {
+        uint4 w = *reinterpret_cast<uint4*>(codes + e);
+        uint8_t* c = reinterpret_cast<uint8_t*>(&w);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) c[i] = uint8_t(int(rintf(float(int(c[i]) - 128) * ratio)) + 128);
+        *reinterpret_cast<uint4*>(codes + e) = w;
+    }
+}
+
+// Any type, strides and alignment, the rows read twice.  grid (touch slots, Hkv, 2)
 template <typename T>
-__global__ void page_write_kernel(const __grid_constant__ PageRowsParams A) {
+__global__ void page_write_any_kernel(const __grid_constant__ PageRowsParams A) {
     __shared__ float sh[32];
     const PagesView& P = A.P;
     const int h = blockIdx.y, side = blockIdx.z;
     const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
-    if (t.page_id < 0) return;
-    if (P.refs[t.page_id] > 1) {               // a page that several sequences hold is not written
+    if (t.slot < 0) return;
+    const int64_t page = touch_page(P, t);
+    if (page < 0) return;
+    if (P.refs[page] > 1) {                    // a page that several sequences hold is not written
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return;
     }
     const T* x = static_cast<const T*>(A.x[side]) + t.token0 * A.row_stride[side] + h * A.head_stride[side];
-    uint8_t* codes = (side ? P.vc : P.kc) + (t.page_id * P.Hkv + h) * int64_t(P.page) * P.d;
-    float* scale = (side ? P.vs : P.ks) + t.page_id * P.Hkv + h;
+    uint8_t* codes = (side ? P.vc : P.kc) + (page * P.Hkv + h) * int64_t(P.page) * P.d;
+    float* scale = (side ? P.vs : P.ks) + page * P.Hkv + h;
     const float old = t.row0 > 0 ? *scale : 0.f;
     const int total = t.rows * P.d;
     float a = 0.f;
@@ -126,30 +148,149 @@ __global__ void page_write_kernel(const __grid_constant__ PageRowsParams A) {
         const float v = to_f32(x[(e / P.d) * A.row_stride[side] + e % P.d]);
         a = fmaxf(a, fabsf(v) < INFINITY ? fabsf(v) : 0.f);
     }
-    a = block_max(a, sh);
-    const float s = fmaxf(old, a < 0x1p-100f ? 0.f : __fdiv_rn(a, 127.f));
-    if (s > old && old > 0.f) {
-        const float ratio = __fdiv_rn(old, s);
-        for (int e = threadIdx.x; e < t.row0 * P.d; e += blockDim.x)
-            codes[e] = uint8_t(int(rintf(float(int(codes[e]) - 128) * ratio)) + 128);
-    }
+    const float s = page_scale(old, block_max(a, sh));
+    if (s > old && old > 0.f) recode_rows(codes, t.row0 * P.d, __fdiv_rn(old, s));
     const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
     for (int e = threadIdx.x; e < total; e += blockDim.x)
         codes[t.row0 * P.d + e] = code8(to_f32(x[(e / P.d) * A.row_stride[side] + e % P.d]), inv);
     if (threadIdx.x == 0) *scale = s;          // every thread has read the old one before block_max's barrier
 }
 
+constexpr int PW_THREADS = 128;
+
 template <typename T>
-__global__ void page_read_kernel(const __grid_constant__ PageRowsParams A) {
+__device__ __forceinline__ float2 pair_f32(uint32_t w);
+template <>
+__device__ __forceinline__ float2 pair_f32<__half>(uint32_t w) { return unpack_half2(w); }
+template <>
+__device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
+    return float2{__uint_as_float(w << 16), __uint_as_float(w & 0xffff0000u)};
+}
+
+// 16-bit rows on 16-byte strides: a thread holds 8 values of up to ROUNDS rounds in registers, so the rows are read
+// once.  The maximum is taken on the magnitudes' bits, two a word (they order like the values), which also shows whether
+// a value is not finite; without one, rint(x inv) + 128 is the low byte of x inv + (1.5 2^23 + 128), as |x inv| <= 127 up to
+// the roundings of s and 1 / s.  Bound by the bytes; many small blocks keep enough loads in flight.  16384 tokens, 8 heads,
+// d 128: 67 MB read and 34 MB written.
+template <typename T, int ROUNDS>
+__global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_constant__ PageRowsParams A) {
+    __shared__ uint32_t sh[PW_THREADS / 32];
     const PagesView& P = A.P;
     const int h = blockIdx.y, side = blockIdx.z;
     const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
-    if (t.page_id < 0) return;
-    const uint8_t* codes = (side ? P.vc : P.kc) + (t.page_id * P.Hkv + h) * int64_t(P.page) * P.d + t.row0 * P.d;
-    const float s = (side ? P.vs : P.ks)[t.page_id * P.Hkv + h];
+    if (t.slot < 0) return;
+    // threads of a row, rows of a round
+    const int shift = P.d == 128 ? 4 : 3, r0 = threadIdx.x >> shift, step = PW_THREADS >> shift;
+    const int c = (threadIdx.x & ((1 << shift) - 1)) * 8;
+    const T* x = static_cast<const T*>(A.x[side]) + t.token0 * A.row_stride[side] + h * A.head_stride[side] + c;
+    uint4 raw[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int r = r0 + i * step;
+        raw[i] = r < t.rows ? __ldg(reinterpret_cast<const uint4*>(x + r * A.row_stride[side])) : uint4{0, 0, 0, 0};
+    }
+    const int64_t page = touch_page(P, t);
+    if (page < 0) return;
+    if (P.refs[page] > 1) {                    // a page that several sequences hold is not written
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return;
+    }
+    uint8_t* codes = (side ? P.vc : P.kc) + (page * P.Hkv + h) * int64_t(P.page) * P.d;
+    float* scale = (side ? P.vs : P.ks) + page * P.Hkv + h;
+    const float old = t.row0 > 0 ? *scale : 0.f;
+    uint32_t top = 0;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        top = __vmaxu2(top, raw[i].x & 0x7fff7fffu);
+        top = __vmaxu2(top, raw[i].y & 0x7fff7fffu);
+        top = __vmaxu2(top, raw[i].z & 0x7fff7fffu);
+        top = __vmaxu2(top, raw[i].w & 0x7fff7fffu);
+    }
+    auto block_top = [&](uint32_t v) {
+        v = __reduce_max_sync(0xffffffffu, max(v & 0xffffu, v >> 16));
+        if ((threadIdx.x & 31) == 0) sh[threadIdx.x >> 5] = v;
+        __syncthreads();
+        uint32_t m = sh[0];
+#pragma unroll
+        for (int w = 1; w < PW_THREADS / 32; ++w) m = max(m, sh[w]);
+        return m;
+    };
+    constexpr uint32_t INF_BITS = std::is_same<T, __half>::value ? 0x7c00u : 0x7f80u;
+    uint32_t m = block_top(top);
+    const bool finite = m < INF_BITS;
+    if (!finite) {                             // the largest of the finite ones
+        top = 0;
+#pragma unroll
+        for (int i = 0; i < ROUNDS; ++i) {
+            const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                const uint32_t lo = ws[k] & 0x7fffu, hi = (ws[k] >> 16) & 0x7fffu;
+                top = max(top, max(lo < INF_BITS ? lo : 0u, hi < INF_BITS ? hi : 0u));
+            }
+        }
+        __syncthreads();
+        m = block_top(top);
+    }
+    const float s = page_scale(old, pair_f32<T>(m).x);
+    if (s > old && old > 0.f) recode_rows(codes, t.row0 * P.d, __fdiv_rn(old, s));
+    const float inv = s > 0.f ? __fdiv_rn(1.f, s) : 0.f;
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int r = r0 + i * step;
+        if (r >= t.rows) break;
+        const uint32_t ws[4] = {raw[i].x, raw[i].y, raw[i].z, raw[i].w};
+        uint32_t out[2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+            const float2 a = pair_f32<T>(ws[2 * k]), b = pair_f32<T>(ws[2 * k + 1]);
+            if (finite) {
+                constexpr float MAGIC = 12582912.f + 128.f;
+                const uint32_t u0 = __float_as_uint(__fadd_rn(__fmul_rn(a.x, inv), MAGIC)), u1 = __float_as_uint(__fadd_rn(__fmul_rn(a.y, inv), MAGIC));
+                const uint32_t u2 = __float_as_uint(__fadd_rn(__fmul_rn(b.x, inv), MAGIC)), u3 = __float_as_uint(__fadd_rn(__fmul_rn(b.y, inv), MAGIC));
+                out[k] = __byte_perm(__byte_perm(u0, u1, 0x0040), __byte_perm(u2, u3, 0x0040), 0x5410);
+            } else {
+                out[k] = code8(a.x, inv) | uint32_t(code8(a.y, inv)) << 8 | uint32_t(code8(b.x, inv)) << 16 | uint32_t(code8(b.y, inv)) << 24;
+            }
+        }
+        *reinterpret_cast<uint2*>(codes + (t.row0 + r) * P.d + c) = uint2{out[0], out[1]};
+    }
+    if (threadIdx.x == 0) *scale = s;          // every thread has read the old one before block_top's barrier
+}
+
+// 16 codes a thread and round; a byte b becomes the float32 pattern 0x4b000000 | b = 2^23 + b, less 2^23 + 128: exact.
+template <typename T>
+__global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_constant__ PageRowsParams A) {
+    const PagesView& P = A.P;
+    const int h = blockIdx.y, side = blockIdx.z;
+    const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
+    if (t.slot < 0) return;
+    const int64_t page = touch_page(P, t);
+    if (page < 0) return;
+    const uint8_t* codes = (side ? P.vc : P.kc) + (page * P.Hkv + h) * int64_t(P.page) * P.d + t.row0 * P.d;
+    const float s = (side ? P.vs : P.ks)[page * P.Hkv + h];
     T* out = static_cast<T*>(A.out[side]) + (t.token0 * P.Hkv + h) * P.d;
-    for (int e = threadIdx.x; e < t.rows * P.d; e += blockDim.x)
-        out[int64_t(e / P.d) * P.Hkv * P.d + e % P.d] = from_f32<T>(float(int(codes[e]) - 128) * s);
+    const int shift = P.d == 128 ? 7 : 6;
+#pragma unroll 4
+    for (int e = threadIdx.x * 16; e < t.rows * P.d; e += PW_THREADS * 16) {
+        const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes + e));
+        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+        float f[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+            f[i] = (__uint_as_float(__byte_perm(ws[i >> 2], 0x4b000000u, 0x7440 | (i & 3))) - 8388736.f) * s;
+        T* to = out + int64_t(e >> shift) * P.Hkv * P.d + (e & ((1 << shift) - 1));
+        if constexpr (sizeof(T) == 4) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(to)[i] = float4{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+        } else {
+            T o[16];
+#pragma unroll
+            for (int i = 0; i < 16; ++i) o[i] = from_f32<T>(f[i]);
+            reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(o)[0];
+            reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(o)[1];
+        }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -305,15 +446,31 @@ __global__ void page_free_kernel(PagesView P, const int32_t* slots) {
     }
 }
 
-// Copy one page's codes and scales; whole block.
+constexpr int PG_COPY_THREADS = 256;
+
+// Part `part` of `parts` of one page's codes (and, part 0, its scales); whole block of PG_COPY_THREADS, 8 loads in flight.
 __device__ __forceinline__ void copy_page(const PagesView& P, int64_t from, int64_t to, int part, int parts) {
-    const int64_t n16 = int64_t(P.Hkv) * P.page * P.d / 16;
-    const uint4* a[2] = {reinterpret_cast<const uint4*>(P.kc) + from * n16, reinterpret_cast<const uint4*>(P.vc) + from * n16};
-    uint4* b[2] = {reinterpret_cast<uint4*>(P.kc) + to * n16, reinterpret_cast<uint4*>(P.vc) + to * n16};
-    for (int side = 0; side < 2; ++side)
-        for (int64_t i = int64_t(part) * blockDim.x + threadIdx.x; i < n16; i += int64_t(parts) * blockDim.x) b[side][i] = a[side][i];
+    const int side16 = P.Hkv * P.page * P.d / 16, all16 = 2 * side16;        // 16-byte words: keys, then values
+    const uint4* k0 = reinterpret_cast<const uint4*>(P.kc) + from * side16;
+    const uint4* v0 = reinterpret_cast<const uint4*>(P.vc) + from * side16 - side16;
+    uint4* k1 = reinterpret_cast<uint4*>(P.kc) + to * side16;
+    uint4* v1 = reinterpret_cast<uint4*>(P.vc) + to * side16 - side16;
+    const int per = (all16 + parts - 1) / parts, end = min(all16, per * (part + 1));
+    for (int i0 = per * part + threadIdx.x; i0 < end; i0 += 8 * PG_COPY_THREADS) {
+        uint4 w[8];
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * PG_COPY_THREADS;
+            if (i < end) w[k] = __ldcs((i < side16 ? k0 : v0) + i);
+        }
+#pragma unroll
+        for (int k = 0; k < 8; ++k) {
+            const int i = i0 + k * PG_COPY_THREADS;
+            if (i < end) __stcs((i < side16 ? k1 : v1) + i, w[k]);
+        }
+    }
     if (part == 0)
-        for (int h = threadIdx.x; h < P.Hkv; h += blockDim.x) {
+        for (int h = threadIdx.x; h < P.Hkv; h += PG_COPY_THREADS) {
             P.ks[to * P.Hkv + h] = P.ks[from * P.Hkv + h];
             P.vs[to * P.Hkv + h] = P.vs[from * P.Hkv + h];
         }

@@ -110,6 +110,29 @@ def test_write_codes_and_scales_are_exact(cuda_dev, page, d, hkv, dtype, starts,
                     assert torch.equal(got[cu[i]:cu[i + 1]].cpu(), torch.from_numpy(want).to(out))
 
 
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("page,d", [(16, 64), (64, 128), (128, 128)])
+def test_write_odd_values_of_16_bits_and_odd_addresses(cuda_dev, dtype, page, d):
+    """Non-finite values among 16-bit rows, the largest and smallest magnitudes, rows off any 16-byte boundary."""
+    rng = np.random.default_rng(19)
+    n = 3 * page + 5
+    pool = O.empty_pool(4, 1, d, page, 1, 4)
+    O.extend(pool, [0], [n])
+    g = on_gpu(pool)
+    x = torch.from_numpy(rng.standard_normal((n, 1, d)) * np.exp(2 * rng.standard_normal((n, 1, 1)))).to(dtype)
+    y = x.flip(0).clone()
+    x[2, 0, 3], x[page, 0, 1], x[page + 1, 0, 2], x[2 * page:3 * page] = float("nan"), float("inf"), -float("inf"), 0
+    y[:page] *= torch.finfo(dtype).tiny
+    y[page:2 * page, 0, 7] = torch.finfo(dtype).max
+    y[2 * page:3 * page] = float("nan")
+    odd = torch.empty(n * (d + 3) + 1, dtype=dtype, device="cuda")[1:].view(n, 1, d + 3)[:, :, :d]
+    odd.copy_(y)
+    O.write(pool, [0], [0], [0, n], x.float().numpy(), y.float().numpy())
+    for v in (y.cuda(), odd):
+        g.write(ints([0]), ints([0]), ints([0, n]), x.cuda(), v)
+        same(g, pool)
+
+
 def test_write_takes_odd_values(cuda_dev):
     """NaN and infinities, rows of zeros, values near the smallest and largest magnitudes, a larger scale later."""
     pool = O.empty_pool(3, 1, 64, 16, 1, 3)
