@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int kMaxSequences = 12000;       // offsets of one call's sequences in the planning block's shared memory
+constexpr int kMaxSequences = 6000;        // offsets of one call's sequences in the planning block's shared memory
 
 // "" or what is wrong with a packed rows call
 kvb_status check_rows(const char* who, const kvb_pages* p, const int32_t* slots, const int32_t* start, const int32_t* cu,
@@ -90,7 +90,8 @@ kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t
     if (n == 0 || rows == 0) return KVB_OK;
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(KVB_EINVAL, "page_read: k and v need 16-byte alignment");
     kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {}, {}, {}, {k, v}};
-    const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)), unsigned(p->Hkv), 2);
+    const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)),
+                    unsigned((2 * int64_t(p->Hkv) * p->page * p->d + kvb::PR_SHARE - 1) / kvb::PR_SHARE));
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (dtype == KVB_F32) kvb::page_read_kernel<float><<<grid, kvb::PW_THREADS, 0, s>>>(a);
     else if (dtype == KVB_F16) kvb::page_read_kernel<__half><<<grid, kvb::PW_THREADS, 0, s>>>(a);

@@ -258,37 +258,52 @@ __global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_con
     if (threadIdx.x == 0) *scale = s;          // every thread has read the old one before block_top's barrier
 }
 
-// 16 codes a thread and round; a byte b becomes the float32 pattern 0x4b000000 | b = 2^23 + b, less 2^23 + 128: exact.
+// The codes of a touched page (both sides, all heads) in shares of 8192, one to a block: a thread takes 16 codes in each of
+// 4 rounds, its loads in flight together.  A byte b becomes the float32 pattern 0x4b000000 | b = 2^23 + b, less 2^23 +
+// 128: exact.  Bound by the bytes; a block per head and side took 47 us where pages are small (16 x 64, 20600 rows of 4
+// heads).  grid (touch slots, ceil(2 Hkv page d / 8192))
+constexpr int PR_SHARE = 8192;
+
 template <typename T>
 __global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_constant__ PageRowsParams A) {
     const PagesView& P = A.P;
-    const int h = blockIdx.y, side = blockIdx.z;
     const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
     if (t.slot < 0) return;
     const int64_t page = touch_page(P, t);
     if (page < 0) return;
-    const uint8_t* codes = (side ? P.vc : P.kc) + (page * P.Hkv + h) * int64_t(P.page) * P.d + t.row0 * P.d;
-    const float s = (side ? P.vs : P.ks)[page * P.Hkv + h];
-    T* out = static_cast<T*>(A.out[side]) + (t.token0 * P.Hkv + h) * P.d;
-    const int shift = P.d == 128 ? 7 : 6;
-#pragma unroll 4
-    for (int e = threadIdx.x * 16; e < t.rows * P.d; e += PW_THREADS * 16) {
-        const uint4 w = __ldg(reinterpret_cast<const uint4*>(codes + e));
-        const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
+    const int log_d = P.d == 128 ? 7 : 6, log_block = log_d + 31 - __clz(P.page);
+    constexpr int ROUNDS = PR_SHARE / (16 * PW_THREADS);
+    uint4 w[ROUNDS];
+    float s[ROUNDS];
+    T* to[ROUNDS];
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        const int e = blockIdx.y * PR_SHARE + (i * PW_THREADS + threadIdx.x) * 16, hs = e >> log_block;
+        const int side = hs >= P.Hkv, h = hs - side * P.Hkv, in = e & ((1 << log_block) - 1), r = (in >> log_d) - t.row0;
+        to[i] = nullptr;
+        if (hs >= 2 * P.Hkv || r < 0 || r >= t.rows) continue;
+        const int64_t ph = page * P.Hkv + h;
+        w[i] = __ldg(reinterpret_cast<const uint4*>((side ? P.vc : P.kc) + (ph << log_block) + in));
+        s[i] = (side ? P.vs : P.ks)[ph];
+        to[i] = static_cast<T*>(A.out[side]) + ((t.token0 + r) * P.Hkv + h) * P.d + (in & (P.d - 1));
+    }
+#pragma unroll
+    for (int i = 0; i < ROUNDS; ++i) {
+        if (!to[i]) continue;
+        const uint32_t ws[4] = {w[i].x, w[i].y, w[i].z, w[i].w};
         float f[16];
 #pragma unroll
-        for (int i = 0; i < 16; ++i)
-            f[i] = (__uint_as_float(__byte_perm(ws[i >> 2], 0x4b000000u, 0x7440 | (i & 3))) - 8388736.f) * s;
-        T* to = out + int64_t(e >> shift) * P.Hkv * P.d + (e & ((1 << shift) - 1));
+        for (int k = 0; k < 16; ++k)
+            f[k] = (__uint_as_float(__byte_perm(ws[k >> 2], 0x4b000000u, 0x7440 | (k & 3))) - 8388736.f) * s[i];
         if constexpr (sizeof(T) == 4) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) reinterpret_cast<float4*>(to)[i] = float4{f[4 * i], f[4 * i + 1], f[4 * i + 2], f[4 * i + 3]};
+            for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(to[i])[k] = float4{f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]};
         } else {
             T o[16];
 #pragma unroll
-            for (int i = 0; i < 16; ++i) o[i] = from_f32<T>(f[i]);
-            reinterpret_cast<uint4*>(to)[0] = reinterpret_cast<const uint4*>(o)[0];
-            reinterpret_cast<uint4*>(to)[1] = reinterpret_cast<const uint4*>(o)[1];
+            for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(f[k]);
+            reinterpret_cast<uint4*>(to[i])[0] = reinterpret_cast<const uint4*>(o)[0];
+            reinterpret_cast<uint4*>(to[i])[1] = reinterpret_cast<const uint4*>(o)[1];
         }
     }
 }
@@ -343,33 +358,41 @@ __device__ __forceinline__ uint32_t free_mask(const int32_t* refs, int64_t n_pag
     return mine;
 }
 
-// The `total` lowest free pages, in ascending order, to give(rank, page).  False (and nothing given) when the
-// pool has fewer.
+// The `total` lowest free pages, in ascending order, to give(rank, page), every thread a rank (a lane's 32 pages may all
+// be free and then hold consecutive ranks: they are listed in shared memory first, PG_LIST at a time).  False, and
+// nothing given, when the pool has fewer.  Whole block; ends with a barrier.
+constexpr int PG_LIST = 4096;
+
 template <typename F>
-__device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh, F give) {
+__device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh, int* list, F give) {
     if (total == 0) return true;
-    int found = 0, sum = 0, at0 = 0;
-    uint32_t first = 0;
+    int found = 0, sum = 0, at = 0;
+    uint32_t mask = 0;
+    int64_t tile = -1;                         // whose mask and ranks are held
     for (int64_t t0 = 0; t0 < P.n_pages && found < total; t0 += PG_TILE) {
-        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
-        const int at = block_scan(__popc(m), sh, sum);
-        if (t0 == 0) { first = m; at0 = at; }
+        mask = free_mask(P.refs, P.n_pages, t0);
+        at = block_scan(__popc(mask), sh, sum);
+        tile = t0;
         found += sum;
     }
     if (found < total) return false;
     int before = 0;
     for (int64_t t0 = 0; t0 < P.n_pages && before < total; t0 += PG_TILE) {
-        uint32_t m = first;
-        int at = at0;
-        if (t0 > 0) {
-            m = free_mask(P.refs, P.n_pages, t0);
-            at = block_scan(__popc(m), sh, sum);
-        } else if (P.n_pages > PG_TILE) {
-            at = block_scan(__popc(m), sh, sum);          // sum of this tile again
+        if (tile != t0) {                      // a pool of one tile is read once
+            mask = free_mask(P.refs, P.n_pages, t0);
+            at = block_scan(__popc(mask), sh, sum);
+            tile = t0;
         }
-        int rank = before + at;
         const int64_t base = t0 + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 32;
-        for (; m && rank < total; m &= m - 1, ++rank) give(rank, int(base + __ffs(m) - 1));
+        const int take = min(sum, total - before);
+        for (int w0 = 0; w0 < take; w0 += PG_LIST) {
+            int rank = at - w0;
+            for (uint32_t m = mask; m && rank < min(take - w0, PG_LIST); m &= m - 1, ++rank)
+                if (rank >= 0) list[rank] = int(base + __ffs(m) - 1);
+            __syncthreads();
+            for (int r = threadIdx.x; r < min(take - w0, PG_LIST); r += PG_THREADS) give(before + w0 + r, list[r]);
+            __syncthreads();
+        }
         before += sum;
     }
     return true;
@@ -391,7 +414,7 @@ __device__ __forceinline__ int owner_of(const int* off, int n, int r) {
 __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, const int32_t* slots, const int32_t* add, int n,
                                                                  int32_t* start) {
     extern __shared__ int off[];               // off[i]: pages of the sequences before i
-    __shared__ int sh[32];
+    __shared__ int sh[32], list[PG_LIST];
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
@@ -413,7 +436,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
     __syncthreads();
     if (bad) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
-    } else if (!take_free(P, total, sh, [&](int rank, int id) {
+    } else if (!take_free(P, total, sh, list, [&](int rank, int id) {
                    const int i = owner_of(off, n, rank);
                    const int s = slots[i];
                    P.table[int64_t(s) * P.max_blocks + blocks_of(P.lens[s], P.page) + rank - off[i]] = id;
@@ -498,7 +521,7 @@ struct ForkWork {
 __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, const int32_t* src, const int32_t* dst, int n,
                                                                ForkWork W) {
     extern __shared__ int off[];
-    __shared__ int sh[32];
+    __shared__ int sh[32], list[PG_LIST];
     __shared__ int bad;
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
@@ -526,7 +549,7 @@ __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, cons
     // rank r belongs to the last i with off[i] <= r: that i has a partial page, those sharing its offset before it none
     if (bad) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
-    } else if (!take_free(P, total, sh, [&](int rank, int id) { W.fresh[owner_of(off, n, rank)] = id; })) {
+    } else if (!take_free(P, total, sh, list, [&](int rank, int id) { W.fresh[owner_of(off, n, rank)] = id; })) {
         if (threadIdx.x == 0) { raise_status(KVB_DEV_POOL); bad = 1; }
     }
     __syncthreads();
@@ -575,33 +598,50 @@ struct CompactWork {
     int32_t* new_id;
 };
 
-// One block.
+// One block.  A pool of one tile (32768 pages) is read once.
 __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, CompactWork W) {
-    __shared__ int sh[32];
+    __shared__ int sh[32], hole_list[PG_LIST], mover_list[PG_LIST];
     int live = 0, sum;
+    uint32_t m = 0;
     for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
-        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
+        m = free_mask(P.refs, P.n_pages, t0);
         block_scan(__popc(m), sh, sum);
         live += int(imin64(PG_TILE, P.n_pages - t0)) - sum;
     }
-    // holes and movers in ascending order: as many of the one as of the other
+    // holes and movers in ascending order: as many of the one as of the other.  Where they fit they are listed in shared
+    // memory and written out together.
     int holes = 0, movers = 0;
+    const bool one = P.n_pages <= PG_TILE;
     for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
-        const uint32_t m = free_mask(P.refs, P.n_pages, t0);
+        if (!one) m = free_mask(P.refs, P.n_pages, t0);
         const int64_t base = t0 + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 32;
         const int64_t below = imin64(imax64(live - base, 0), 32), valid = imin64(imax64(P.n_pages - base, 0), 32);
         const uint32_t lo = below == 32 ? 0xffffffffu : (1u << below) - 1, in = valid == 32 ? 0xffffffffu : (1u << valid) - 1;
         uint32_t hole = m & lo, mover = ~m & in & ~lo;
-        int nh, nm;
-        int rh = holes + block_scan(__popc(hole), sh, nh);
-        int rm = movers + block_scan(__popc(mover), sh, nm);
-        for (; hole; hole &= hole - 1) W.to[rh++] = int(base + __ffs(hole) - 1);
-        for (; mover; mover &= mover - 1) W.from[rm++] = int(base + __ffs(mover) - 1);
+        int both;                                                // two counts of at most 2^15 in one scan
+        const int at = block_scan(__popc(hole) | __popc(mover) << 16, sh, both);
+        const int nh = both & 0xffff, nm = int(uint32_t(both) >> 16);
+        int rh = at & 0xffff, rm = int(uint32_t(at) >> 16);
+        for (; hole; hole &= hole - 1, ++rh) {
+            const int id = int(base + __ffs(hole) - 1);
+            if (rh < PG_LIST) hole_list[rh] = id;
+            else W.to[holes + rh] = id;
+        }
+        for (; mover; mover &= mover - 1, ++rm) {
+            const int id = int(base + __ffs(mover) - 1);
+            if (rm < PG_LIST) mover_list[rm] = id;
+            else W.from[movers + rm] = id;
+        }
+        __syncthreads();
+        for (int r = threadIdx.x; r < min(nh, PG_LIST); r += PG_THREADS) W.to[holes + r] = hole_list[r];
+        for (int r = threadIdx.x; r < min(nm, PG_LIST); r += PG_THREADS) W.from[movers + r] = mover_list[r];
+        if (one)
+            for (int r = threadIdx.x; r < min(nm, PG_LIST); r += PG_THREADS) W.new_id[mover_list[r]] = hole_list[r];
         holes += nh;
         movers += nm;
+        __syncthreads();
     }
-    __syncthreads();
-    for (int r = threadIdx.x; r < movers; r += PG_THREADS) W.new_id[W.from[r]] = W.to[r];
+    for (int r = (one ? PG_LIST : 0) + threadIdx.x; r < movers; r += PG_THREADS) W.new_id[W.from[r]] = W.to[r];
     if (threadIdx.x == 0) {
         W.head[0] = live;
         W.head[1] = movers;
