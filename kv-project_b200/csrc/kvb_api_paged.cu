@@ -50,8 +50,7 @@ kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
         a.out = out + i * per * D * 2;
         a.lse = lse ? lse + i * per : nullptr;
         a.slots = slots + i;
-        kern<<<grid, kvb::PdShape<D, NT>::THREADS, SM, s>>>(a);
-        if (kvb_status st = launch_check("page_attend")) return st;
+        if (kvb_status st = launch_chained("page_attend", kern, grid, kvb::PdShape<D, NT>::THREADS, SM, s, a)) return st;
     }
     return KVB_OK;
 }

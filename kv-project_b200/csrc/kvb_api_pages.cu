@@ -25,13 +25,14 @@ kvb_status check_rows(const char* who, const kvb_pages* p, const int32_t* slots,
 
 // Rounds of 8 values a thread that hold a whole page of rows.
 template <typename T>
-void launch_write(const kvb::PageRowsParams& a, dim3 grid, cudaStream_t s) {
+kvb_status launch_write(const kvb::PageRowsParams& a, dim3 grid, cudaStream_t s) {
     const int rounds = a.P.page * a.P.d / (8 * kvb::PW_THREADS);
-    if (rounds <= 1) kvb::page_write_kernel<T, 1><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else if (rounds == 2) kvb::page_write_kernel<T, 2><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else if (rounds == 4) kvb::page_write_kernel<T, 4><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else if (rounds == 8) kvb::page_write_kernel<T, 8><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else kvb::page_write_kernel<T, 16><<<grid, kvb::PW_THREADS, 0, s>>>(a);
+    const auto kern = rounds <= 1   ? kvb::page_write_kernel<T, 1>
+                      : rounds == 2 ? kvb::page_write_kernel<T, 2>
+                      : rounds == 4 ? kvb::page_write_kernel<T, 4>
+                      : rounds == 8 ? kvb::page_write_kernel<T, 8>
+                                    : kvb::page_write_kernel<T, 16>;
+    return launch_chained("page_write", kern, grid, kvb::PW_THREADS, 0, s, a);
 }
 
 size_t fork_rows_offset(int n) { return (size_t(64 + 2 * size_t(n)) * 4 + 255) / 256 * 256; }
@@ -75,13 +76,11 @@ kvb_status kvb_page_write(const kvb_pages* p, const int32_t* slots, const int32_
     const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)), unsigned(p->Hkv), 2);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const bool vectors = dtype != KVB_F32 && aligned(k, 16) && aligned(v, 16) && (k_row | k_head | v_row | v_head) % 8 == 0;
-    if (vectors) {
-        if (dtype == KVB_F16) launch_write<__half>(a, grid, s);
-        else launch_write<__nv_bfloat16>(a, grid, s);
-    } else if (dtype == KVB_F32) kvb::page_write_any_kernel<float><<<grid, 256, 0, s>>>(a);
-    else if (dtype == KVB_F16) kvb::page_write_any_kernel<__half><<<grid, 256, 0, s>>>(a);
-    else kvb::page_write_any_kernel<__nv_bfloat16><<<grid, 256, 0, s>>>(a);
-    return launch_check("page_write");
+    if (vectors) return dtype == KVB_F16 ? launch_write<__half>(a, grid, s) : launch_write<__nv_bfloat16>(a, grid, s);
+    const auto kern = dtype == KVB_F32   ? kvb::page_write_any_kernel<float>
+                      : dtype == KVB_F16 ? kvb::page_write_any_kernel<__half>
+                                         : kvb::page_write_any_kernel<__nv_bfloat16>;
+    return launch_chained("page_write", kern, grid, 256, 0, s, a);
 }
 
 kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t* start, const int32_t* cu, int n, void* k,
@@ -92,11 +91,10 @@ kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t
     kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {}, {}, {}, {k, v}};
     const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)),
                     unsigned((2 * int64_t(p->Hkv) * p->page * p->d + kvb::PR_SHARE - 1) / kvb::PR_SHARE));
-    cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == KVB_F32) kvb::page_read_kernel<float><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else if (dtype == KVB_F16) kvb::page_read_kernel<__half><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    else kvb::page_read_kernel<__nv_bfloat16><<<grid, kvb::PW_THREADS, 0, s>>>(a);
-    return launch_check("page_read");
+    const auto kern = dtype == KVB_F32   ? kvb::page_read_kernel<float>
+                      : dtype == KVB_F16 ? kvb::page_read_kernel<__half>
+                                         : kvb::page_read_kernel<__nv_bfloat16>;
+    return launch_chained("page_read", kern, grid, kvb::PW_THREADS, 0, static_cast<cudaStream_t>(stream), a);
 }
 
 kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32_t* add, int n, int32_t* start, void* stream) {
@@ -104,9 +102,8 @@ kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32
     if (n > 0 && (!slots || !add || !start)) return fail(KVB_EINVAL, "page_extend: null argument");
     if (n < 0 || n > kMaxSequences) return fail(KVB_EINVAL, "page_extend: 0 <= n <= %d sequences a call", kMaxSequences);
     if (n == 0) return KVB_OK;
-    kvb::page_extend_kernel<<<1, kvb::PG_THREADS, size_t(n) * 4, static_cast<cudaStream_t>(stream)>>>(kvbh::view_of(p), slots,
-                                                                                                   add, n, start);
-    return launch_check("page_extend");
+    return launch_chained("page_extend", kvb::page_extend_kernel, 1, kvb::PG_THREADS, size_t(n) * 4, static_cast<cudaStream_t>(stream),
+                          kvbh::view_of(p), slots, add, n, start);
 }
 
 kvb_status kvb_page_free(const kvb_pages* p, const int32_t* slots, int n, void* stream) {
@@ -114,8 +111,8 @@ kvb_status kvb_page_free(const kvb_pages* p, const int32_t* slots, int n, void* 
     if (n > 0 && !slots) return fail(KVB_EINVAL, "page_free: null argument");
     if (n < 0) return fail(KVB_EINVAL, "page_free: n >= 0");
     if (n == 0) return KVB_OK;
-    kvb::page_free_kernel<<<unsigned(n), 128, 0, static_cast<cudaStream_t>(stream)>>>(kvbh::view_of(p), slots);
-    return launch_check("page_free");
+    return launch_chained("page_free", kvb::page_free_kernel, unsigned(n), 128, 0, static_cast<cudaStream_t>(stream), kvbh::view_of(p),
+                          slots);
 }
 
 kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* stream) {
@@ -123,8 +120,8 @@ kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* 
     if (n > 0 && (!src || !dst)) return fail(KVB_EINVAL, "page_copy: null argument");
     if (n < 0) return fail(KVB_EINVAL, "page_copy: n >= 0");
     if (n == 0) return KVB_OK;
-    kvb::page_copy_kernel<<<dim3(unsigned(n), 4), kvb::PG_COPY_THREADS, 0, static_cast<cudaStream_t>(stream)>>>(kvbh::view_of(p), src, dst);
-    return launch_check("page_copy");
+    return launch_chained("page_copy", kvb::page_copy_kernel, dim3(unsigned(n), 4), kvb::PG_COPY_THREADS, 0,
+                          static_cast<cudaStream_t>(stream), kvbh::view_of(p), src, dst);
 }
 
 size_t kvb_page_fork_workspace(const kvb_pages* p, int n) {
@@ -144,12 +141,11 @@ kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* 
     const kvb::PagesView v = kvbh::view_of(p);
     const kvb::ForkWork w = fork_work(workspace, n);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    kvb::fork_plan_kernel<<<1, kvb::PG_THREADS, size_t(n + 1) * 4, s>>>(v, src, dst, n, w);
-    if (kvb_status st = launch_check("page_fork plan")) return st;
-    kvb::fork_copy_kernel<<<dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s>>>(v, src, w);
-    if (kvb_status st = launch_check("page_fork copy")) return st;
-    kvb::fork_commit_kernel<<<unsigned(n), 128, 0, s>>>(v, src, dst, w);
-    return launch_check("page_fork commit");
+    if (kvb_status st = launch_chained("page_fork plan", kvb::fork_plan_kernel, 1, kvb::PG_THREADS, size_t(n + 1) * 4, s, v, src, dst, n, w))
+        return st;
+    if (kvb_status st = launch_chained("page_fork copy", kvb::fork_copy_kernel, dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s, v, src, w))
+        return st;
+    return launch_chained("page_fork commit", kvb::fork_commit_kernel, unsigned(n), 128, 0, s, v, src, dst, w);
 }
 
 size_t kvb_page_compact_workspace(const kvb_pages* p) {
@@ -167,10 +163,8 @@ kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace
     int32_t* b = static_cast<int32_t*>(workspace);
     const kvb::CompactWork w{b, b + 64, b + 64 + p->n_pages, b + 64 + 2 * p->n_pages};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    kvb::compact_plan_kernel<<<1, kvb::PG_THREADS, 0, s>>>(v, w);
-    if (kvb_status st = launch_check("page_compact plan")) return st;
-    kvb::compact_move_kernel<<<148 * 4, kvb::PG_COPY_THREADS, 0, s>>>(v, w, n_live);
-    return launch_check("page_compact move");
+    if (kvb_status st = launch_chained("page_compact plan", kvb::compact_plan_kernel, 1, kvb::PG_THREADS, 0, s, v, w)) return st;
+    return launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 4, kvb::PG_COPY_THREADS, 0, s, v, w, n_live);
 }
 
 }  // extern "C"

@@ -37,8 +37,7 @@ kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
     if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "prefill_attention"))
         return st;
     const int64_t items = a.Hkv * (a.nq / (2 * a.tt) + a.n);         // at least as many as there are
-    kern<<<unsigned(std::min<int64_t>(items, resolve_ctas(0))), kvb::PF_THREADS, SM, s>>>(a);
-    return launch_check("prefill_attention");
+    return launch_chained("prefill_attention", kern, unsigned(std::min<int64_t>(items, resolve_ctas(0))), kvb::PF_THREADS, SM, s, a);
 }
 
 }  // namespace

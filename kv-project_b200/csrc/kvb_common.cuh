@@ -49,6 +49,13 @@ __device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t* p) {
     return v;
 }
 
+// First thing in a kernel that is launched with programmatic stream serialization (kvbh::launch_chained): the next kernel's
+// blocks may take their places now, and this one's memory accesses begin when everything before it has completed.
+__device__ __forceinline__ void chain_kernels() {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+}
+
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
     return static_cast<uint32_t>(__cvta_generic_to_shared(p));
 }

@@ -26,6 +26,23 @@ int elem_size(int dt);
 // CTA count of a persistent kernel: the caller's, else the current device's SM count (capped).
 int resolve_ctas(int n_ctas);
 
+// Launch with programmatic stream serialization: the kernel's blocks may be placed while the kernel before it finishes
+// (its launch is then hidden, 1 to 2 us); it begins with kvb::chain_kernels().
+template <typename... P, typename... A>
+kvb_status launch_chained(const char* what, void (*fn)(P...), dim3 grid, dim3 block, size_t smem, cudaStream_t s, A&&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = block;
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute at[1];
+    at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = at;
+    cfg.numAttrs = 1;
+    return cuda_check(cudaLaunchKernelEx(&cfg, fn, P(args)...), what);
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
@@ -95,5 +112,6 @@ using kvbh::elem_size;
 using kvbh::encode_tiled;
 using kvbh::EncodeTiledFn;
 using kvbh::fail;
+using kvbh::launch_chained;
 using kvbh::launch_check;
 using kvbh::resolve_ctas;

@@ -168,6 +168,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         fence_mbar_init();
         pre[0] = 0;
     }
+    chain_kernels();
     // units before each sequence: an inclusive scan, S::THREADS sequences at a time; an empty sequence is one unit
     // without keys, whose rows still have to be written
     int before = 0;

@@ -127,6 +127,7 @@ __device__ __forceinline__ void recode_rows(uint8_t* codes, int n, float ratio) 
 // Any type, strides and alignment, the rows read twice.  grid (touch slots, Hkv, 2)
 template <typename T>
 __global__ void page_write_any_kernel(const __grid_constant__ PageRowsParams A) {
+    chain_kernels();
     __shared__ float sh[32];
     const PagesView& P = A.P;
     const int h = blockIdx.y, side = blockIdx.z;
@@ -174,6 +175,7 @@ __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
 // d 128: 67 MB read and 34 MB written.
 template <typename T, int ROUNDS>
 __global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_constant__ PageRowsParams A) {
+    chain_kernels();
     __shared__ uint32_t sh[PW_THREADS / 32];
     const PagesView& P = A.P;
     const int h = blockIdx.y, side = blockIdx.z;
@@ -266,6 +268,7 @@ constexpr int PR_SHARE = 8192;
 
 template <typename T>
 __global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_constant__ PageRowsParams A) {
+    chain_kernels();
     const PagesView& P = A.P;
     const Touch t = find_touch(P, A.slots, A.start, A.cu, A.n, A.rows, blockIdx.x);
     if (t.slot < 0) return;
@@ -283,7 +286,7 @@ __global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_cons
         to[i] = nullptr;
         if (hs >= 2 * P.Hkv || r < 0 || r >= t.rows) continue;
         const int64_t ph = page * P.Hkv + h;
-        w[i] = __ldg(reinterpret_cast<const uint4*>((side ? P.vc : P.kc) + (ph << log_block) + in));
+        w[i] = *reinterpret_cast<const uint4*>((side ? P.vc : P.kc) + (ph << log_block) + in);
         s[i] = (side ? P.vs : P.ks)[ph];
         to[i] = static_cast<T*>(A.out[side]) + ((t.token0 + r) * P.Hkv + h) * P.d + (in & (P.d - 1));
     }
@@ -413,6 +416,7 @@ __device__ __forceinline__ int owner_of(const int* off, int n, int r) {
 // range, a row too short, not enough free pages): then nothing is changed.
 __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, const int32_t* slots, const int32_t* add, int n,
                                                                  int32_t* start) {
+    chain_kernels();
     extern __shared__ int off[];               // off[i]: pages of the sequences before i
     __shared__ int sh[32], list[PG_LIST];
     __shared__ int bad;
@@ -453,6 +457,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
 
 // One block per sequence.
 __global__ void page_free_kernel(PagesView P, const int32_t* slots) {
+    chain_kernels();
     __shared__ int len;
     const int s = slots[blockIdx.x];
     if (s < 0 || s >= P.n_slots) {
@@ -501,6 +506,7 @@ __device__ __forceinline__ void copy_page(const PagesView& P, int64_t from, int6
 
 // grid (pages, parts)
 __global__ void page_copy_kernel(PagesView P, const int32_t* src, const int32_t* dst) {
+    chain_kernels();
     const int a = src[blockIdx.x], b = dst[blockIdx.x];
     if (a < 0 || b < 0 || a >= P.n_pages || b >= P.n_pages) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
@@ -520,6 +526,7 @@ struct ForkWork {
 // One block: lengths and fresh pages of all forks, from the state before any of them.
 __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, const int32_t* src, const int32_t* dst, int n,
                                                                ForkWork W) {
+    chain_kernels();
     extern __shared__ int off[];
     __shared__ int sh[32], list[PG_LIST];
     __shared__ int bad;
@@ -558,6 +565,7 @@ __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, cons
 
 // grid (forks, 1 + parts): part 0 snapshots the source's row, the others copy its partial page
 __global__ void fork_copy_kernel(PagesView P, const int32_t* src, ForkWork W) {
+    chain_kernels();
     if (!W.head[0]) return;
     const int i = blockIdx.x;
     const int32_t* row = P.table + int64_t(src[i]) * P.max_blocks;
@@ -573,6 +581,7 @@ __global__ void fork_copy_kernel(PagesView P, const int32_t* src, ForkWork W) {
 
 // grid (forks): references and rows
 __global__ void fork_commit_kernel(PagesView P, const int32_t* src, const int32_t* dst, ForkWork W) {
+    chain_kernels();
     if (!W.head[0]) return;
     const int i = blockIdx.x, t = dst[i];
     if (src[i] == t) return;
@@ -600,6 +609,7 @@ struct CompactWork {
 
 // One block.  A pool of one tile (32768 pages) is read once.
 __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, CompactWork W) {
+    chain_kernels();
     __shared__ int sh[32], hole_list[PG_LIST], mover_list[PG_LIST];
     int live = 0, sum;
     uint32_t m = 0;
@@ -649,6 +659,7 @@ __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, C
 }
 
 __global__ void compact_move_kernel(PagesView P, CompactWork W, int32_t* n_live) {
+    chain_kernels();
     const int live = W.head[0], moves = W.head[1];
     if (blockIdx.x == 0 && threadIdx.x == 0) *n_live = live;
     constexpr int PARTS = 4;

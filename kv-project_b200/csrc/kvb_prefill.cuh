@@ -379,6 +379,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    chain_kernels();
     const uint32_t tmem = sh.tmem;
     volatile int* abort = &sh.abort;
     // a wait that gave up stops every role

@@ -26,11 +26,20 @@ _I32 = torch.int32
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _device_ints(who: str, n, **ts):
-    """int32, contiguous, one-dimensional CUDA tensors of n entries (None: any number)."""
-    for name, t in ts.items():
-        if not t.is_cuda or t.dtype is not _I32 or t.dim() != 1 or not t.is_contiguous() or (n is not None and t.shape[0] != n):
-            raise ValueError(f"{who}: {name} must be a contiguous int32 CUDA tensor of {'n' if n is None else n} entries")
+def _check_ints(who: str, n: int, *ts):
+    """int32, contiguous, one-dimensional CUDA tensors of n entries."""
+    for t in ts:
+        if t.dtype is not _I32 or t.shape != (n,) or not t.is_cuda or not t.is_contiguous():
+            raise ValueError(f"{who}: slots, starts, counts and offsets must be contiguous int32 CUDA tensors of {n} entries")
+
+
+def _dense(shape, dtype, device):
+    """A new contiguous tensor (empty_strided takes 1.6 us where empty takes 2.4)."""
+    strides, n = [], 1
+    for s in reversed(shape):
+        strides.append(n)
+        n *= s if s > 1 else 1
+    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
 
 
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor = None,
@@ -51,18 +60,18 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
         raise ValueError("prefill_attention: q, k and v of one dtype")
     nq, hq, d = q.shape
     nk, hkv, _ = k.shape
-    _device_ints("prefill_attention", None, cu_q=cu_q, cu_k=cu_k)
-    n = cu_q.shape[0] - 1
-    if n < 0 or cu_k.shape[0] != n + 1:
+    n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
+    if n < 0:
         raise ValueError("prefill_attention: cu_q and cu_k hold n + 1 offsets each")
+    _check_ints("prefill_attention", n + 1, cu_q, cu_k)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if d and not qs[2] == ks[2] == vs[2] == 1:
         raise ValueError("prefill_attention: d must be contiguous")
     if out is None:
-        out = torch.empty((nq, hq, d), dtype=q.dtype, device=q.device)
+        out = _dense((nq, hq, d), q.dtype, q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype")
-    lse = torch.empty((nq, hq), dtype=torch.float32, device=q.device) if return_lse else None
+    lse = _dense((nq, hq), torch.float32, q.device) if return_lse else None
     st = L.lib().kvb_prefill_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
         vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
@@ -118,7 +127,7 @@ class PagePool:
         """Pages for add[i] more tokens of sequence slots[i]; returns the positions (n,) int32 where they go (-1: the call
         was refused, nothing changed)."""
         n = slots.shape[0]
-        _device_ints("extend", n, slots=slots, add=add)
+        _check_ints("extend", n, slots, add)
         start = torch.empty_like(slots)
         st = L.lib().kvb_page_extend(self._p, slots.data_ptr(), add.data_ptr(), n, start.data_ptr(), _raw_stream(self._index))
         if st:
@@ -129,8 +138,8 @@ class PagePool:
         """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
         sequence slots[i] (as extend returned them)."""
         n = slots.shape[0]
-        _device_ints("write", n, slots=slots, start=start)
-        _device_ints("write", n + 1, cu=cu)
+        _check_ints("write", n, slots, start)
+        _check_ints("write", n + 1, cu)
         if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (self.Hkv, self.d) or k.dtype != v.dtype or not (k.is_cuda and v.is_cuda):
             raise ValueError("write: k and v (N, Hkv, d) CUDA tensors of one dtype")
         a, b = k.stride(), v.stride()
@@ -145,9 +154,10 @@ class PagePool:
         """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
         write (rows = cu[-1])."""
         n = slots.shape[0]
-        _device_ints("read", n, slots=slots, start=start)
-        _device_ints("read", n + 1, cu=cu)
-        k, v = (torch.empty((rows, self.Hkv, self.d), dtype=dtype, device=self.device) for _ in range(2))
+        _check_ints("read", n, slots, start)
+        _check_ints("read", n + 1, cu)
+        shape = (rows, self.Hkv, self.d)
+        k, v = _dense(shape, dtype, self.device), _dense(shape, dtype, self.device)
         st = L.lib().kvb_page_read(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                                    _DT.get(dtype, -1), rows, _raw_stream(self._index))
         if st:
@@ -160,14 +170,14 @@ class PagePool:
         if q.dim() != 4 or q.shape[3] != self.d or not q.is_cuda:
             raise ValueError("attend: q (n, Hq, Tq, d) on the pool's device")
         n, hq, tq, d = q.shape
-        _device_ints("attend", n, slots=slots)
+        _check_ints("attend", n, slots)
         if not q.is_contiguous():
             q = q.contiguous()
         if out is None:
-            out = torch.empty((n, tq, hq, d), dtype=q.dtype, device=q.device)
+            out = _dense((n, tq, hq, d), q.dtype, q.device)
         elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype")
-        lse = torch.empty((n, tq, hq), dtype=torch.float32, device=q.device) if return_lse else None
+        lse = _dense((n, tq, hq), torch.float32, q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._ws.get((stream, n, hq, tq))
         if ws is None:
@@ -183,7 +193,7 @@ class PagePool:
         """Sequence dst[i] becomes a copy of src[i] (full pages shared, a partial last page copied); what it held is
         released.  All sources are taken as they were before the call."""
         n = src.shape[0]
-        _device_ints("fork", n, src=src, dst=dst)
+        _check_ints("fork", n, src, dst)
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
         st = lib.kvb_page_fork(self._p, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
@@ -192,8 +202,9 @@ class PagePool:
 
     def free(self, slots) -> None:
         """Drops the sequences and their references to pages."""
-        _device_ints("free", None, slots=slots)
-        st = L.lib().kvb_page_free(self._p, slots.data_ptr(), slots.shape[0], _raw_stream(self._index))
+        n = slots.shape[0]
+        _check_ints("free", n, slots)
+        st = L.lib().kvb_page_free(self._p, slots.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_free")
 
@@ -210,7 +221,7 @@ class PagePool:
     def copy_pages(self, src, dst) -> None:
         """Page src[i] over page dst[i], codes and scales."""
         n = src.shape[0]
-        _device_ints("copy_pages", n, src=src, dst=dst)
+        _check_ints("copy_pages", n, src, dst)
         st = L.lib().kvb_page_copy(self._p, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_copy")
