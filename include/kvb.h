@@ -473,11 +473,15 @@ kvb_status kvb_operational_rd(const float* A, int64_t rows, int64_t n, int64_t l
  * positions.  A row that sees no key gives zeros and -inf.  q (nq, Hq, d), k and v (nk, Hkv, d) of one dtype
  * (f16 / bf16) with d in {64, 128} contiguous, the element strides below multiples of 8 and 16-byte aligned
  * bases; cu_q, cu_k (n + 1) int32 on the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype;
- * lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written. */
+ * lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written.
+ * workspace (kvb_prefill_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
+ * (every call leaves its counters at zero), one per stream that runs calls concurrently; with it the work of
+ * long rows is split over the keys, without it (null) every query tile is computed in one piece. */
+size_t kvb_prefill_workspace(int d);
 kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq,
                                  int Hkv, int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                                  int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, int n,
-                                 float scaling, void* out, float* lse, void* stream);
+                                 float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
 /* A pool of pages of `page` (16, 32, 64 or 128) tokens, device tensors, dense: codes kc, vc (n_pages, Hkv,
  * page, d) uint8 (16-byte aligned) and scales ks, vs (n_pages, Hkv) float32, a stored value being

@@ -11,6 +11,9 @@
 
 namespace {
 
+constexpr int kMaxCtas = 256;
+constexpr size_t kCountBytes = 2 * kMaxCtas * 8 * 4;          // per piece and warp
+
 // Rows of `heads` heads of d 16-bit channels as a 3D tensor (d, heads, rows): box 64 x box_heads x box_rows, 128-byte
 // swizzle.
 kvb_status make_map(CUtensorMap* m, const char* name, const void* base, int bf16, int d, int heads, int64_t rows,
@@ -36,18 +39,24 @@ kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
     const auto kern = kvb::prefill_kernel<T, D>;
     if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "prefill_attention"))
         return st;
-    const int64_t items = a.Hkv * (a.nq / (2 * a.tt) + a.n);         // at least as many as there are
-    return launch_chained("prefill_attention", kern, unsigned(std::min<int64_t>(items, resolve_ctas(0))), kvb::PF_THREADS, SM, s, a);
+    // without pieces no more CTAs than items (at most so many) have work
+    const int64_t items = a.part ? kMaxCtas : a.Hkv * (a.nq / (2 * a.tt) + a.n);
+    const int ctas = std::min(resolve_ctas(0), kMaxCtas);
+    return launch_chained("prefill_attention", kern, unsigned(std::min<int64_t>(items, ctas)), kvb::PF_THREADS, SM, s, a);
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t kvb_prefill_workspace(int d) {
+    return d == 64 || d == 128 ? kCountBytes + size_t(resolve_ctas(0)) * 2 * 2 * (d + 2) * 128 * 4 : 0;
+}
+
 kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq,
                                  int Hkv, int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
                                  int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, int n,
-                                 float scaling, void* out, float* lse, void* stream) {
+                                 float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream) {
     if (n < 0 || nq < 0 || nk < 0 || nq > INT32_MAX || nk > INT32_MAX)
         return fail(KVB_EINVAL, "prefill_attention: n >= 0 and row counts in [0, 2^31)");
     if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Hq > 65535)
@@ -62,7 +71,11 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16))
         return fail(KVB_EINVAL, "prefill_attention: q, k, v and out need 16-byte alignment");
     if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "prefill_attention: scaling must be finite");
+    if (workspace && (workspace_bytes < kvb_prefill_workspace(d) || !aligned(workspace, 256)))
+        return fail(KVB_EINVAL, "prefill_attention: workspace of %zu bytes, 256-byte aligned (or none)", kvb_prefill_workspace(d));
     kvb::PrefillParams a{};
+    a.count = static_cast<uint32_t*>(workspace);
+    a.part = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes) : nullptr;
     a.rep = Hq / Hkv;
     a.tt = 128 / a.rep;
     const int bf16 = dtype == KVB_BF16;

@@ -31,9 +31,14 @@
 // whole, value rows past the sequence become zeros in shared memory, and non-finite entries of the sequence's own
 // later tokens too, which the rows that do see them get added back at the end.
 //
-// Work items are dealt in descending order of their key tiles, forth and back over the CTAs: every CTA finds its
-// next item by bisection on the tile count (a warp reduction over the sequences per step), so no plan is built
-// before the launch and no counter is kept.
+// Work items are dealt in descending order of their key tiles, forth and back over the CTAs; items of more tiles than a
+// CTA's fair share (few rows over long keys) come first, cut into equal pieces of at most that many: each piece leaves
+// its O, m and l in the workspace, and the warp that completes the last piece of its 32 rows joins them in the order of
+// the keys.  Every CTA finds its next item from the lengths (bisection on the tile count, sums of tile counts in closed
+// form, a warp's lanes over the sequences), so no plan is built before the launch and no counter is kept.  Two chunks after
+// prefixes (500 after 7000 and 1100 after 333, 16 heads over 4, d 64): 134 us without pieces.  Equal shares of
+// consecutive work, cut anywhere, balance as well but cut almost every share's ends: packed prompts 167 to 189
+// instead of 150 us.
 //
 // Every wait is bounded; after a timeout all roles stop, copies in flight are waited for and tensor memory is freed.
 #pragma once
@@ -64,6 +69,8 @@ struct PrefillParams {
     const int32_t* cu_k;
     int64_t nq, nk;
     int n, Hq, Hkv, rep, tt;                  // tt = 128 / rep tokens per tile
+    float* part;                              // [2 grid pieces][2 tiles][d + 2][128]: O by column, m, l; null: no item is cut
+    uint32_t* count;                          // [2 grid pieces][8 warps]
     float lam;                                // |scaling| log2(e), > 0
     int negate;                               // scaling < 0
     void* out;                                // (nq, Hq, d)
@@ -83,7 +90,9 @@ struct PfItem {
     int q0, ql, k0, kl;                       // the sequence's rows
     int t0;                                   // first token of tile A within it
     int head;                                 // KV head; < 0: no more work
-    int n[2];                                 // key tiles of A and B
+    int j0;                                   // first key tile of this piece
+    int n[2];                                 // key tiles of A and B in this piece
+    int piece, first, pieces;                 // number of this piece and of the item's first; how many the item has
     int jm;                                   // first key tile that some row does not see whole
     uint32_t bad[4][4];                       // non-finite value rows of the tiles jm ..
 };
@@ -242,7 +251,7 @@ __device__ __forceinline__ bool pf_not_finite(const uint4& w) {
 }
 
 // ---------------------------------------------------------------------------------------------
-// Work items in descending order of key tiles.
+// Work items: those of more tiles than the fair share, in pieces, then the others in descending order of key tiles.
 // ---------------------------------------------------------------------------------------------
 struct PfSeq {
     int q0, ql, k0, kl, pairs;
@@ -277,10 +286,152 @@ __device__ __forceinline__ int pf_count(const PfSeq& q, int t, int tt) {
 
 __device__ __forceinline__ int pf_warp_sum(int v) { return __reduce_add_sync(0xffffffffu, v); }
 
+// sum over i < n of floor((a i + b) / m), for a, b >= 0 (the Euclidean reduction of a and the divisor).  Intermediate
+// values stay below 2^32: n is a count of tile pairs, whose rows have to fit the GPU's memory.
+__device__ __forceinline__ int64_t pf_floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    int64_t sum = 0;
+    while (n > 0) {
+        sum += int64_t(a / m) * (int64_t(n) * (n - 1) / 2) + int64_t(b / m) * n;
+        a %= m;
+        b %= m;
+        const uint32_t y = a * n + b;
+        if (y < m) break;
+        n = y / m;
+        b = y % m;
+        const uint32_t t = m;
+        m = a;
+        a = t;
+    }
+    return sum;
+}
+
+// Pieces of up to `keys` keys (a multiple of the tile) in the pairs before p, a pair counting one at least unless it sees
+// no key.
+__device__ __forceinline__ int pf_pieces(const PfSeq& q, int p, int tt, uint32_t keys) {
+    const int full = min(p, q.pairs - 1), a = q.kl - q.ql, b = 2 * tt;         // pairs that end before the sequence does
+    const int i0 = a < 0 ? min(-a / b, full) : 0;                              // those before see no key
+    int c = full > i0 ? int(pf_floor_sum(full - i0, keys, b, uint32_t(a + b * (i0 + 1)) + keys - 1)) : 0;
+    if (p == q.pairs && p > 0) c += int((uint32_t(q.kl) + keys - 1) / keys);
+    return c;
+}
+
+// The tiles j0 .. j1 - 1 of a pair (out: its sequence and head).
+__device__ __forceinline__ void pf_tiles_of(const PrefillParams& A, int pair, int j0, int j1, PfItem& out) {
+    out.t0 = pair * 2 * A.tt;
+    out.j0 = j0;
+    for (int w = 0; w < 2; ++w) {
+        const int last = min(out.t0 + (w + 1) * A.tt, out.ql);              // tokens before it
+        const int keys = last > out.t0 + w * A.tt ? min(max(out.kl - out.ql + last, 0), out.kl) : 0;
+        out.n[w] = max(min((keys + PF_KT - 1) / PF_KT, j1) - j0, 0);
+    }
+    out.jm = max(out.kl - out.ql + out.t0 + 1, 0) / PF_KT;
+}
+
+constexpr int PF_SHARE = 8;                   // items of fewer tiles are never cut
+
+struct PfCuts {
+    int share;                                // items of more tiles are cut into pieces of at most so many
+    int64_t items;                            // how many are,
+    int64_t pieces;                           // into how many pieces
+};
+
+// The fair share, or eight tiles, and what it cuts; whole warp.  There are fewer pieces than 2 ctas: each has more than half
+// a share.
+__device__ __forceinline__ PfCuts pf_cuts(const PrefillParams& A, int ctas) {
+    const int lane = threadIdx.x & 31;
+    PfCuts c{INT_MAX, 0, 0};
+    if (!A.part) return c;
+    int64_t tiles = 0;
+    int most = 0;
+    for (int s0 = 0; s0 < A.n; s0 += 32) {
+        const PfSeq q = pf_seq(A, s0 + lane);
+        tiles += int64_t(pf_pieces(q, q.pairs, A.tt, PF_KT)) * A.Hkv;
+        most = max(most, q.pairs ? (q.kl + PF_KT - 1) / PF_KT : 0);
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    most = __reduce_max_sync(0xffffffffu, most);
+    const int64_t share = imax64(PF_SHARE, (tiles + ctas - 1) / ctas);
+    if (most <= share) return c;
+    c.share = int(share);
+    for (int s0 = 0; s0 < A.n; s0 += 32) {
+        const PfSeq q = pf_seq(A, s0 + lane);
+        const int cut = q.pairs ? pf_count(q, c.share + 1, A.tt) : 0;
+        const uint32_t keys = uint32_t(c.share) * PF_KT;
+        c.items += int64_t(cut) * A.Hkv;
+        if (cut) c.pieces += int64_t(pf_pieces(q, q.pairs, A.tt, keys) - pf_pieces(q, q.pairs - cut, A.tt, keys)) * A.Hkv;
+    }
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) {
+        c.items += __shfl_xor_sync(0xffffffffu, c.items, o);
+        c.pieces += __shfl_xor_sync(0xffffffffu, c.pieces, o);
+    }
+    return c;
+}
+
+// Piece `idx` of the cut items; whole warp.
+__device__ __forceinline__ void pf_piece(const PrefillParams& A, const PfCuts& cuts, int idx, PfItem& out) {
+    const int lane = threadIdx.x & 31;
+    const uint32_t keys = uint32_t(cuts.share) * PF_KT;
+    int r = idx;
+    for (int s0 = 0; s0 < A.n; s0 += 32) {
+        const PfSeq q = pf_seq(A, s0 + lane);
+        const int cut = q.pairs ? pf_count(q, cuts.share + 1, A.tt) : 0;
+        const int before = cut ? pf_pieces(q, q.pairs - cut, A.tt, keys) : 0;
+        const int per = cut ? pf_pieces(q, q.pairs, A.tt, keys) - before : 0;                  // pieces of one head
+        int x = per * A.Hkv;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int y = __shfl_up_sync(0xffffffffu, x, o);
+            if (lane >= o) x += y;
+        }
+        const uint32_t after = __ballot_sync(0xffffffffu, x > r);
+        if (after == 0) {
+            r -= __shfl_sync(0xffffffffu, x, 31);
+            continue;
+        }
+        const int src = __ffs(int(after)) - 1;
+        PfSeq c;
+        c.q0 = __shfl_sync(0xffffffffu, q.q0, src);
+        c.ql = __shfl_sync(0xffffffffu, q.ql, src);
+        c.k0 = __shfl_sync(0xffffffffu, q.k0, src);
+        c.kl = __shfl_sync(0xffffffffu, q.kl, src);
+        c.pairs = __shfl_sync(0xffffffffu, q.pairs, src);
+        r -= __shfl_sync(0xffffffffu, x - per * A.Hkv, src);
+        const int one = __shfl_sync(0xffffffffu, per, src), skipped = __shfl_sync(0xffffffffu, before, src);
+        const int head = r / one;
+        r -= head * one;
+        // the largest pair whose pieces begin at or before r, by 32-way search
+        int lo = c.pairs - __shfl_sync(0xffffffffu, cut, src), len = c.pairs - lo, at = 0;
+        while (true) {
+            const int step = (len + 31) / 32, p = lo + lane * step;
+            const int v = p < lo + len ? pf_pieces(c, p, A.tt, keys) - skipped : 0;
+            const int k = 31 - __clz(int(__ballot_sync(0xffffffffu, p < lo + len && v <= r) | 1u));
+            at = __shfl_sync(0xffffffffu, v, k);
+            lo += k * step;
+            len = min(step, c.pairs - lo);
+            if (step == 1) break;
+        }
+        out.q0 = c.q0, out.ql = c.ql, out.k0 = c.k0, out.kl = c.kl;
+        out.head = head;
+        const int e = c.kl - c.ql + min(2 * A.tt * (lo + 1), c.ql), tiles = (e + PF_KT - 1) / PF_KT, k = r - at;
+        out.pieces = (tiles + cuts.share - 1) / cuts.share;
+        out.piece = idx;
+        out.first = idx - k;
+        pf_tiles_of(A, lo, int(int64_t(tiles) * k / out.pieces), int(int64_t(tiles) * (k + 1) / out.pieces), out);
+        return;
+    }
+}
+
 // Item `idx`; `t` the last item's key tiles (a bound for the search), or < 0 at first.  Whole warp; false when there
 // are no more.
-__device__ __forceinline__ bool pf_item(const PrefillParams& A, int64_t idx, int& t, PfItem& out) {
+__device__ __forceinline__ bool pf_item(const PrefillParams& A, const PfCuts& cuts, int64_t idx, int& t, PfItem& out) {
     const int lane = threadIdx.x & 31;
+    if (idx < cuts.pieces) {
+        pf_piece(A, cuts, int(idx), out);
+        return true;
+    }
+    idx += cuts.items - cuts.pieces;              // place among all items by their tiles
     PfSeq mine = pf_seq(A, lane);
     auto total = [&](int tiles) {
         int64_t c = 0;
@@ -297,7 +448,7 @@ __device__ __forceinline__ bool pf_item(const PrefillParams& A, int64_t idx, int
             const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
             most = max(most, __reduce_max_sync(0xffffffffu, (q.kl + PF_KT - 1) / PF_KT));
         }
-        hi = most;
+        hi = min(most, cuts.share);
     }
     if (idx >= total(0)) return false;
     int lo = 0;                                   // the largest t with total(t) > idx
@@ -328,14 +479,10 @@ __device__ __forceinline__ bool pf_item(const PrefillParams& A, int64_t idx, int
         out.ql = __shfl_sync(0xffffffffu, q.ql, src);
         out.k0 = __shfl_sync(0xffffffffu, q.k0, src);
         out.kl = __shfl_sync(0xffffffffu, q.kl, src);
-        out.t0 = __shfl_sync(0xffffffffu, pair, src) * 2 * A.tt;
         out.head = __shfl_sync(0xffffffffu, head, src);
-        for (int w = 0; w < 2; ++w) {
-            const int last = min(out.t0 + (w + 1) * A.tt, out.ql);          // tokens before it
-            const int keys = last > out.t0 + w * A.tt ? min(max(out.kl - out.ql + last, 0), out.kl) : 0;
-            out.n[w] = (keys + PF_KT - 1) / PF_KT;
-        }
-        out.jm = max(out.kl - out.ql + out.t0 + 1, 0) / PF_KT;
+        out.first = out.piece = 0;
+        out.pieces = 1;
+        pf_tiles_of(A, __shfl_sync(0xffffffffu, pair, src), 0, INT_MAX, out);
         return true;
     }
     return false;
@@ -398,10 +545,11 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         uint32_t it = 0, items = 0;
         int t = -1;
         bool ok = true;
+        const PfCuts cuts = pf_cuts(A, gridDim.x);
         for (int64_t round = 0; ok; ++round) {
             const int64_t idx = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
             PfItem x;
-            const bool more = pf_item(A, idx, t, x);
+            const bool more = pf_item(A, cuts, idx, t, x);
             PfItem& slot = sh.item[round & 1];
             if (round >= 2) ok = __all_sync(0xffffffffu, wait(&sh.item_empty[round & 1], uint32_t(round / 2 - 1)));
             if (!ok) break;
@@ -430,7 +578,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                     mbar_arrive_expect_tx(&sh.kv_full[st], S::TILE_BYTES);
                     for (int h = 0; h < S::HALVES; ++h)
                         tma_load_3d(skv + st * S::TILE_BYTES + h * (128 * 128), j & 1 ? &A.tm_v : &A.tm_k, h * 64, x.head,
-                                    x.k0 + (j >> 1) * PF_KT, &sh.kv_full[st]);
+                                    x.k0 + (x.j0 + (j >> 1)) * PF_KT, &sh.kv_full[st]);
                     sh.kv_issued = it + 1;
                 }
             }
@@ -531,11 +679,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             PfItem& x = sh.item[round & 1];
             const int head = x.head;
             if (head < 0) break;
-            const int n = x.n[w], nt = max(x.n[0], x.n[1]), jm = x.jm, kl = x.kl;
+            const int n = x.n[w], nt = max(x.n[0], x.n[1]), kl = x.kl;
+            const int j0 = x.j0, jm = x.jm - j0;                 // key tiles are counted from the piece's first
             const int tok = x.t0 + w * A.tt + row / A.rep;       // token of the sequence
             const bool valid = row < A.tt * A.rep && tok < x.ql;
             const int limit = valid ? min(max(kl - x.ql + tok + 1, 0), kl) : INT_MAX;    // rows of no token mask nothing
-            const int jmask = __reduce_min_sync(0xffffffffu, limit) / PF_KT;     // first tile that a row of the warp does not see whole
+            const int jmask = __reduce_min_sync(0xffffffffu, limit) / PF_KT - j0;        // first tile that a row of the warp does not see whole
             float m = -INFINITY, l = 0.f;
             bool ok = true;
             for (int j = 0; j < n; ++j, ++steps) {
@@ -552,7 +701,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                 }
                 // The first 64 weights are computed with the reference so far while the maximum is taken: it serves unless
                 // a row's maximum grew by 2^8, has not begun, or is not finite.
-                const int lim = limit - j * PF_KT;
+                const int lim = limit - (j0 + j) * PF_KT;
                 const bool masked = j >= jmask;
                 uint32_t p[32];
                 uint64_t sum[2] = {0, 0};
@@ -617,7 +766,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                     const uint32_t vj = kv + 2 * j + 1;
                     if (!(ok = all(wait(&sh.kv_full[vj % S::STAGES], vj / S::STAGES)))) break;
                     uint8_t* vt = skv + (vj % S::STAGES) * S::TILE_BYTES + row * 128;
-                    const bool past = j * PF_KT + row >= kl;
+                    const bool past = (j0 + j) * PF_KT + row >= kl;
                     bool bad = false;
                     if (!past) {
 #pragma unroll
@@ -664,8 +813,28 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                 for (int i = 0; i < 16; ++i) any_bad |= reinterpret_cast<volatile uint32_t*>(x.bad)[i] != 0;
             const int64_t out_row = int64_t(x.q0) + tok;
             const int hq = head * A.rep + row % A.rep;
-            const float inv = l > 0.f ? 1.f / l : (l == l ? 0.f : l);
             T* dst = static_cast<T*>(A.out) + (out_row * A.Hq + hq) * D;
+            auto store = [&](const uint32_t (&o)[32], int c, float sum) {
+                const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+                if (!valid) return;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    uint32_t h[4];
+#pragma unroll
+                    for (int k = 0; k < 4; ++k)
+                        h[k] = pf_pack<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
+                    *reinterpret_cast<uint4*>(dst + c + 8 * i) = uint4{h[0], h[1], h[2], h[3]};
+                }
+            };
+            auto store_lse = [&](float top, float sum) {
+                if (valid && A.lse)
+                    A.lse[out_row * A.Hq + hq] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+            };
+            const bool whole = x.pieces == 1;
+            auto slot_of = [&](int piece) {                      // this tile's part: O by column, then m and l
+                return A.part + (int64_t(piece) * 2 + w) * ((D + 2) * 128) + row;
+            };
+            float* part = whole ? nullptr : slot_of(x.piece);
 #pragma unroll 1
             for (int c = 0; c < D; c += 32) {
                 uint32_t o[32];
@@ -679,7 +848,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                 if (any_bad && valid && l != 0.f) {
                     const T* vp = static_cast<const T*>(A.v) + int64_t(x.k0) * A.v_row + head * A.v_head + c;
                     for (int b = 0; b < 4 * PF_KT; ++b) {
-                        const int key = jm * PF_KT + b;
+                        const int key = (j0 + jm) * PF_KT + b;
                         if (key < limit && (x.bad[b >> 7][(b >> 5) & 3] >> (b & 31) & 1)) {
 #pragma unroll
                             for (int i = 0; i < 32; ++i) {
@@ -689,18 +858,55 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                         }
                     }
                 }
-                if (valid) {
-                    uint32_t h[16];
+                if (whole) {
+                    store(o, c, l);
+                } else {
 #pragma unroll
-                    for (int i = 0; i < 16; ++i)
-                        h[i] = pf_pack<T>(__uint_as_float(o[2 * i]) * inv, __uint_as_float(o[2 * i + 1]) * inv);
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        *reinterpret_cast<uint4*>(dst + c + 8 * i) = uint4{h[4 * i], h[4 * i + 1], h[4 * i + 2], h[4 * i + 3]};
+                    for (int i = 0; i < 32; ++i) __stcg(part + (c + i) * 128, __uint_as_float(o[i]));
                 }
             }
-            if (valid && A.lse)
-                A.lse[out_row * A.Hq + hq] = l == 0.f ? -INFINITY : m * 0.693147180559945309f + logf(l);
+            if (whole) {
+                store_lse(m, l);
+            } else {
+                __stcg(part + D * 128, m);
+                __stcg(part + (D + 1) * 128, l);
+                __threadfence();
+                __syncwarp();
+                uint32_t* count = A.count + x.first * 8 + warp;
+                uint32_t before = 0;
+                if (lane == 0) before = atomicAdd(count, 1u);
+                before = __shfl_sync(0xffffffffu, before, 0);
+                if (before + 1 > uint32_t(x.pieces)) {
+                    if (lane == 0) raise_status(KVB_DEV_WORKSPACE);
+                } else if (before + 1 == uint32_t(x.pieces)) {
+                    // all pieces of these 32 rows are there: join them in the order of the keys
+                    if (lane == 0) *count = 0;
+                    __threadfence();
+                    float top = -INFINITY;
+                    for (int c = x.first; c < x.first + x.pieces; ++c) top = fmaxf(top, __ldcg(slot_of(c) + D * 128));
+                    const float ref = top == -INFINITY ? 0.f : top;
+                    float sum = 0.f;
+                    for (int c = x.first; c < x.first + x.pieces; ++c)
+                        sum = __fmaf_rn(__ldcg(slot_of(c) + (D + 1) * 128), ex2(__ldcg(slot_of(c) + D * 128) - ref), sum);
+#pragma unroll 1
+                    for (int ch = 0; ch < D; ch += 32) {
+                        float acc[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) acc[i] = 0.f;
+                        for (int c = x.first; c < x.first + x.pieces; ++c) {
+                            const float* q = slot_of(c);
+                            const float f = ex2(__ldcg(q + D * 128) - ref);
+#pragma unroll
+                            for (int i = 0; i < 32; ++i) acc[i] = __fmaf_rn(__ldcg(q + (ch + i) * 128), f, acc[i]);
+                        }
+                        uint32_t o[32];
+#pragma unroll
+                        for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(acc[i]);
+                        store(o, ch, sum);
+                    }
+                    store_lse(top, sum);
+                }
+            }
             tc_fence_before();
             __syncwarp();
             if (lane == 0) mbar_arrive(&sh.item_empty[round & 1]);

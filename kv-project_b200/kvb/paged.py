@@ -42,6 +42,18 @@ def _dense(shape, dtype, device):
     return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
 
 
+_PREFILL_WS = {}
+_UNSPLIT_KEYS = 896
+
+
+def _prefill_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
+    """The zero-filled workspace of one stream (40 MB), made at the first call that may need it."""
+    ws = _PREFILL_WS.get((device.index, stream, d))
+    if ws is None:
+        ws = _PREFILL_WS[(device.index, stream, d)] = torch.zeros(lib.kvb_prefill_workspace(d), dtype=torch.uint8, device=device)
+    return ws
+
+
 def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor = None,
                       scaling: float = None, out: torch.Tensor = None, return_lse: bool = False):
     """Causal attention of packed sequences: q (Nq, Hq, d), k and v (Nk, Hkv, d) float16 / bfloat16, any row and head
@@ -72,10 +84,13 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype")
     lse = _dense((nq, hq), torch.float32, q.device) if return_lse else None
-    st = L.lib().kvb_prefill_attention(
+    # a query tile has as many as 8 key tiles of 128, and may be split over them, only when there are so many keys
+    lib, stream = L.lib(), _raw_stream(q.device.index)
+    ws = _prefill_workspace(lib, q.device, stream, d) if nk > _UNSPLIT_KEYS else None
+    st = lib.kvb_prefill_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
         vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
-        lse.data_ptr() if return_lse else None, _raw_stream(q.device.index))
+        lse.data_ptr() if return_lse else None, None if ws is None else ws.data_ptr(), 0 if ws is None else ws.numel(), stream)
     if st:
         L.check(st, "kvb_prefill_attention")
     return (out, lse) if return_lse else out

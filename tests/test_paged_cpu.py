@@ -62,10 +62,10 @@ def test_page_calls(name, args, status, word):
     (dict(q=0), 1, "null"), (dict(cu_q=0), 1, "null"), (dict(nq=-1), 1, "n >= 0"), (dict(nk=1 << 31), 1, "row counts"),
     (dict(Hq=5), 1, "Hq"), (dict(Hkv=0), 1, "Hq"), (dict(dtype=0), 4, "float16"), (dict(d=32), 4, "d 64"),
     (dict(q_row=516), 1, "strides"), (dict(v_head=-128), 1, "strides"), (dict(q=A + 8), 1, "alignment"),
-    (dict(out=A + 2), 1, "alignment")])
+    (dict(out=A + 2), 1, "alignment"), (dict(workspace=A, workspace_bytes=64), 1, "workspace"), (dict(workspace=A + 8, workspace_bytes=1 << 30), 1, "workspace")])
 def test_prefill_call(change, status, word):
     a = dict(q=A, k=A, v=A, dtype=2, nq=10, nk=10, Hq=4, Hkv=2, d=128, q_row=512, q_head=128, k_row=256, k_head=128, v_row=256,
-             v_head=128, cu_q=A, cu_k=A, n=1, scaling=0.1, out=A, lse=None, stream=None)
+             v_head=128, cu_q=A, cu_k=A, n=1, scaling=0.1, out=A, lse=None, workspace=None, workspace_bytes=0, stream=None)
     a.update(change)
     st, msg = call("kvb_prefill_attention", *a.values())
     assert st == status and word in msg, (st, msg)
