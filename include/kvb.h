@@ -531,12 +531,15 @@ size_t kvb_page_attend_workspace(const kvb_pages* p, int n, int Hq, int Tq);
 kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
                            float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
-/* Sequence dst[i] becomes a copy of src[i], all from the state before the call (distinct dst; a dst may be a src):
+/* The calls below that move pages take the pools of all layers that share a table: p[0 .. n_pools), alike but for codes,
+ * scales, Hkv and d; the table is changed once.
+ *
+ * Sequence dst[i] becomes a copy of src[i], all from the state before the call (distinct dst; a dst may be a src):
  * full pages are shared, a partial last page is copied to a fresh page (the lowest ones free before the call, in
  * the order of the list), what dst held before is released.  src[i] == dst[i] keeps the sequence as it is.  With
  * too few free pages nothing changes (status bit 4).  workspace 256-byte aligned. */
 size_t kvb_page_fork_workspace(const kvb_pages* p, int n);
-kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* workspace,
+kvb_status kvb_page_fork(const kvb_pages* p, int n_pools, const int32_t* src, const int32_t* dst, int n, void* workspace,
                          size_t workspace_bytes, void* stream);
 
 /* Drops the sequences: references down, rows -1, lens 0. */
@@ -545,10 +548,11 @@ kvb_status kvb_page_free(const kvb_pages* p, const int32_t* slots, int n, void* 
 /* Moves the live pages with id >= *n_live, in ascending order, into the free pages below, in ascending order, and
  * renames them in the table; *n_live (device int32) = the number of live pages, which are then the first ones. */
 size_t kvb_page_compact_workspace(const kvb_pages* p);
-kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream);
+kvb_status kvb_page_compact(const kvb_pages* p, int n_pools, int32_t* n_live, void* workspace, size_t workspace_bytes,
+                            void* stream);
 
 /* Whole pages, codes and scales: page src[i] over page dst[i] (distinct dst, none of them a src). */
-kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* stream);
+kvb_status kvb_page_copy(const kvb_pages* p, int n_pools, const int32_t* src, const int32_t* dst, int n, void* stream);
 
 /* Build the split-K plan (pure host computation, no CUDA calls) for n_ctas CTAs.  plan_out receives
  * [n_ctas, n_pieces, n_heads, cta_begin[n_ctas + 1], n_pieces x (head, stratum, first chunk, end

@@ -35,6 +35,18 @@ kvb_status launch_write(const kvb::PageRowsParams& a, dim3 grid, cudaStream_t s)
     return launch_chained("page_write", kern, grid, kvb::PW_THREADS, 0, s, a);
 }
 
+// Pools of one table: the layers of a model.
+kvb_status check_layers(const char* who, const kvb_pages* p, int n_pools) {
+    if (!p || n_pools <= 0) return fail(KVB_EINVAL, "%s: null argument", who);
+    for (int i = 0; i < n_pools; ++i) {
+        if (kvb_status st = kvbh::check_pages(who, p + i)) return st;
+        if (p[i].table != p->table || p[i].lens != p->lens || p[i].refs != p->refs || p[i].n_pages != p->n_pages ||
+            p[i].page != p->page || p[i].n_slots != p->n_slots || p[i].max_blocks != p->max_blocks)
+            return fail(KVB_EINVAL, "%s: pools of one call share table, lens, refs and sizes", who);
+    }
+    return KVB_OK;
+}
+
 size_t fork_rows_offset(int n) { return (size_t(64 + 2 * size_t(n)) * 4 + 255) / 256 * 256; }
 
 kvb::ForkWork fork_work(void* ws, int n) {
@@ -115,13 +127,16 @@ kvb_status kvb_page_free(const kvb_pages* p, const int32_t* slots, int n, void* 
                           slots);
 }
 
-kvb_status kvb_page_copy(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* stream) {
-    if (kvb_status st = kvbh::check_pages("page_copy", p)) return st;
+kvb_status kvb_page_copy(const kvb_pages* p, int n_pools, const int32_t* src, const int32_t* dst, int n, void* stream) {
+    if (kvb_status st = check_layers("page_copy", p, n_pools)) return st;
     if (n > 0 && (!src || !dst)) return fail(KVB_EINVAL, "page_copy: null argument");
     if (n < 0) return fail(KVB_EINVAL, "page_copy: n >= 0");
     if (n == 0) return KVB_OK;
-    return launch_chained("page_copy", kvb::page_copy_kernel, dim3(unsigned(n), 4), kvb::PG_COPY_THREADS, 0,
-                          static_cast<cudaStream_t>(stream), kvbh::view_of(p), src, dst);
+    for (int i = 0; i < n_pools; ++i)
+        if (kvb_status st = launch_chained("page_copy", kvb::page_copy_kernel, dim3(unsigned(n), 4), kvb::PG_COPY_THREADS, 0,
+                                           static_cast<cudaStream_t>(stream), kvbh::view_of(p + i), src, dst))
+            return st;
+    return KVB_OK;
 }
 
 size_t kvb_page_fork_workspace(const kvb_pages* p, int n) {
@@ -129,9 +144,9 @@ size_t kvb_page_fork_workspace(const kvb_pages* p, int n) {
     return fork_rows_offset(n) + size_t(n) * p->max_blocks * 4;
 }
 
-kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* dst, int n, void* workspace,
+kvb_status kvb_page_fork(const kvb_pages* p, int n_pools, const int32_t* src, const int32_t* dst, int n, void* workspace,
                          size_t workspace_bytes, void* stream) {
-    if (kvb_status st = kvbh::check_pages("page_fork", p)) return st;
+    if (kvb_status st = check_layers("page_fork", p, n_pools)) return st;
     if (n > 0 && (!src || !dst || !workspace)) return fail(KVB_EINVAL, "page_fork: null argument");
     if (n < 0 || n > kMaxSequences) return fail(KVB_EINVAL, "page_fork: 0 <= n <= %d sequences a call", kMaxSequences);
     if (n == 0) return KVB_OK;
@@ -143,8 +158,10 @@ kvb_status kvb_page_fork(const kvb_pages* p, const int32_t* src, const int32_t* 
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (kvb_status st = launch_chained("page_fork plan", kvb::fork_plan_kernel, 1, kvb::PG_THREADS, size_t(n + 1) * 4, s, v, src, dst, n, w))
         return st;
-    if (kvb_status st = launch_chained("page_fork copy", kvb::fork_copy_kernel, dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s, v, src, w))
-        return st;
+    for (int i = 0; i < n_pools; ++i)
+        if (kvb_status st = launch_chained("page_fork copy", kvb::fork_copy_kernel, dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s,
+                                           kvbh::view_of(p + i), src, w))
+            return st;
     return launch_chained("page_fork commit", kvb::fork_commit_kernel, unsigned(n), 128, 0, s, v, src, dst, w);
 }
 
@@ -153,8 +170,9 @@ size_t kvb_page_compact_workspace(const kvb_pages* p) {
     return (64 + 3 * size_t(p->n_pages)) * 4;
 }
 
-kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace, size_t workspace_bytes, void* stream) {
-    if (kvb_status st = kvbh::check_pages("page_compact", p)) return st;
+kvb_status kvb_page_compact(const kvb_pages* p, int n_pools, int32_t* n_live, void* workspace, size_t workspace_bytes,
+                            void* stream) {
+    if (kvb_status st = check_layers("page_compact", p, n_pools)) return st;
     if (!n_live || !workspace) return fail(KVB_EINVAL, "page_compact: null argument");
     const size_t need = kvb_page_compact_workspace(p);
     if (workspace_bytes < need) return fail(KVB_EINVAL, "page_compact: workspace of %zu bytes, need %zu", workspace_bytes, need);
@@ -164,7 +182,11 @@ kvb_status kvb_page_compact(const kvb_pages* p, int32_t* n_live, void* workspace
     const kvb::CompactWork w{b, b + 64, b + 64 + p->n_pages, b + 64 + 2 * p->n_pages};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (kvb_status st = launch_chained("page_compact plan", kvb::compact_plan_kernel, 1, kvb::PG_THREADS, 0, s, v, w)) return st;
-    return launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 4, kvb::PG_COPY_THREADS, 0, s, v, w, n_live);
+    for (int i = 0; i < n_pools; ++i)
+        if (kvb_status st = launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 4, kvb::PG_COPY_THREADS, 0, s,
+                                           kvbh::view_of(p + i), w, n_live, i + 1 == n_pools))
+            return st;
+    return KVB_OK;
 }
 
 }  // extern "C"

@@ -658,19 +658,21 @@ __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, C
     }
 }
 
-__global__ void compact_move_kernel(PagesView P, CompactWork W, int32_t* n_live) {
+// The moves of one pool; with `commit` also the reference counts and the table (once, where pools share them).
+__global__ void compact_move_kernel(PagesView P, CompactWork W, int32_t* n_live, int commit) {
     chain_kernels();
     const int live = W.head[0], moves = W.head[1];
-    if (blockIdx.x == 0 && threadIdx.x == 0) *n_live = live;
     constexpr int PARTS = 4;
     for (int w = blockIdx.x; w < moves * PARTS; w += gridDim.x) {
         const int r = w / PARTS;
         copy_page(P, W.from[r], W.to[r], w % PARTS, PARTS);
-        if (w % PARTS == 0 && threadIdx.x == 0) {
+        if (commit && w % PARTS == 0 && threadIdx.x == 0) {
             P.refs[W.to[r]] = P.refs[W.from[r]];
             P.refs[W.from[r]] = 0;
         }
     }
+    if (!commit) return;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *n_live = live;
     const int64_t entries = int64_t(P.n_slots) * P.max_blocks;
     for (int64_t e = int64_t(blockIdx.x) * blockDim.x + threadIdx.x; e < entries; e += int64_t(gridDim.x) * blockDim.x) {
         const int id = P.table[e];

@@ -113,11 +113,11 @@ SIGNATURES = {
     "kvb_page_attend_workspace": (C.c_size_t, [_p, _i32, _i32, _i32]),
     "kvb_page_attend": (_i32, [_p, _p, _i32, _i32, _i32, _p, _i32, _f32, _p, _p, _p, C.c_size_t, _p]),
     "kvb_page_fork_workspace": (C.c_size_t, [_p, _i32]),
-    "kvb_page_fork": (_i32, [_p, _p, _p, _i32, _p, C.c_size_t, _p]),
+    "kvb_page_fork": (_i32, [_p, _i32, _p, _p, _i32, _p, C.c_size_t, _p]),
     "kvb_page_free": (_i32, [_p, _p, _i32, _p]),
     "kvb_page_compact_workspace": (C.c_size_t, [_p]),
-    "kvb_page_compact": (_i32, [_p, _p, _p, C.c_size_t, _p]),
-    "kvb_page_copy": (_i32, [_p, _p, _p, _i32, _p]),
+    "kvb_page_compact": (_i32, [_p, _i32, _p, _p, C.c_size_t, _p]),
+    "kvb_page_copy": (_i32, [_p, _i32, _p, _p, _i32, _p]),
     "kvb_quasar_scores": (_i32, [_p, _i32, _i32, _i32, _p, C.c_size_t, _p, _i32, _p, _i32, _i64, _p, _p]),
     "kvb_quasar_values_workspace": (C.c_size_t, [_i32, _i32, _i64, _i32]),
     "kvb_quasar_values": (_i32, [_p, _i32, _i32, _i64, _p, C.c_size_t, _p, _i32, _p, _i32, _i32, _p, _p, C.c_size_t, _p]),

@@ -99,8 +99,9 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
 class PagePool:
     """Pages of ``page`` tokens for Hkv KV heads: codes kc, vc (n_pages, Hkv, page, d) uint8 and scales ks, vs (n_pages,
     Hkv) float32 (a stored value is (code - 128) * scale), table (n_slots, max_blocks) int32 with each sequence's pages,
-    lens (n_slots) int32, refs (n_pages) int32.  The pool works on the tensors it is given; layers that share table,
-    lens and refs call extend / free once and write / attend per layer."""
+    lens (n_slots) int32, refs (n_pages) int32.  The pool works on the tensors it is given.  The other layers of a model are
+    pools of their own over the same table (add_layer): write, read and attend go to each, the calls that change the table
+    (extend, fork, free, compact, copy_pages) once to the first pool, which moves the pages of all."""
 
     def __init__(self, kc, vc, ks, vs, table, lens, refs):
         ts = (kc, vc, ks, vs, table, lens, refs)
@@ -119,6 +120,7 @@ class PagePool:
         self.device, self._index = kc.device, kc.device.index
         self._c = L.Pages(*[t.data_ptr() for t in ts], n_pages, hkv, d, page, *table.shape)
         self._p = C.byref(self._c)
+        self._layers, self._n = (L.Pages * 1)(self._c), 1
         self._ws = {}
 
     @classmethod
@@ -130,6 +132,18 @@ class PagePool:
                    torch.zeros((n_pages, Hkv), **z), torch.zeros((n_pages, Hkv), **z),
                    torch.full((n_slots, n_pages if max_blocks is None else max_blocks), -1, dtype=_I32, **z),
                    torch.zeros(n_slots, dtype=_I32, **z), torch.zeros(n_pages, dtype=_I32, **z))
+
+    def add_layer(self, kc=None, vc=None, ks=None, vs=None) -> "PagePool":
+        """The pool of another layer over this pool's table (empty codes and scales of the same shape by default)."""
+        if kc is None:
+            kc, vc = torch.full_like(self.kc, 128), torch.full_like(self.vc, 128)
+            ks, vs = torch.zeros_like(self.ks), torch.zeros_like(self.vs)
+        other = PagePool(kc, vc, ks, vs, self.table, self.lens, self.refs)
+        if (other.n_pages, other.page) != (self.n_pages, self.page):
+            raise ValueError("add_layer: as many pages of as many tokens as the first pool has")
+        self._layers = (L.Pages * (self._n + 1))(*self._layers, other._c)
+        self._n += 1
+        return other
 
     def _workspace(self, kind: str, stream: int, size: int) -> torch.Tensor:
         """A zero-filled buffer for one kind of call on one stream, kept while it is large enough."""
@@ -211,7 +225,7 @@ class PagePool:
         _check_ints("fork", n, src, dst)
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
-        st = lib.kvb_page_fork(self._p, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
+        st = lib.kvb_page_fork(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_fork")
 
@@ -228,7 +242,7 @@ class PagePool:
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._workspace("compact", stream, lib.kvb_page_compact_workspace(self._p))
         live = torch.empty((), dtype=_I32, device=self.device)
-        st = lib.kvb_page_compact(self._p, live.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        st = lib.kvb_page_compact(self._layers, self._n, live.data_ptr(), ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_compact")
         return live
@@ -237,6 +251,6 @@ class PagePool:
         """Page src[i] over page dst[i], codes and scales."""
         n = src.shape[0]
         _check_ints("copy_pages", n, src, dst)
-        st = L.lib().kvb_page_copy(self._p, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
+        st = L.lib().kvb_page_copy(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_copy")

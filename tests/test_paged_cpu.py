@@ -29,8 +29,8 @@ def test_pool_descriptor(field, value, status):
     p = C.byref(pages(**{field: value}))
     calls = [("kvb_page_extend", (p, A, A, 1, A, None)), ("kvb_page_write", (p, A, A, A, 1, A, A, 2, 5, 256, 128, 256, 128, None)),
              ("kvb_page_read", (p, A, A, A, 1, A, A, 2, 5, None)), ("kvb_page_free", (p, A, 1, None)),
-             ("kvb_page_copy", (p, A, A, 1, None)), ("kvb_page_fork", (p, A, A, 1, A, B, None)),
-             ("kvb_page_compact", (p, A, A, B, None)), ("kvb_page_attend", (p, A, 1, 4, 1, A, 1, 0.1, A, None, A, B, None))]
+             ("kvb_page_copy", (p, 1, A, A, 1, None)), ("kvb_page_fork", (p, 1, A, A, 1, A, B, None)),
+             ("kvb_page_compact", (p, 1, A, A, B, None)), ("kvb_page_attend", (p, A, 1, 4, 1, A, 1, 0.1, A, None, A, B, None))]
     for name, args in calls:
         st, msg = call(name, *args)
         assert st == status and name[4:] in msg, (name, st, msg)
@@ -45,9 +45,9 @@ def test_pool_descriptor(field, value, status):
     ("kvb_page_write", (A, A, A, 1, A, A, 3, 5, 256, 128, 256, 128, None), 1, "dtype"),
     ("kvb_page_write", (A, A, A, 1, A, A, 2, 1 << 31, 256, 128, 256, 128, None), 1, "rows"),
     ("kvb_page_read", (A, A, A, -1, A, A, 2, 5, None), 1, "n >= 0"),
-    ("kvb_page_free", (0, 1, None), 1, "null"), ("kvb_page_copy", (A, 0, 1, None), 1, "null"),
-    ("kvb_page_fork", (A, A, 1, A, 16, None), 1, "workspace"), ("kvb_page_fork", (A, A, 1, A + 16, B, None), 1, "alignment"),
-    ("kvb_page_compact", (A, A, 16, None), 1, "workspace"), ("kvb_page_compact", (0, A, B, None), 1, "null"),
+    ("kvb_page_free", (0, 1, None), 1, "null"), ("kvb_page_copy", (1, A, 0, 1, None), 1, "null"), ("kvb_page_copy", (0, A, A, 1, None), 1, "null"),
+    ("kvb_page_fork", (1, A, A, 1, A, 16, None), 1, "workspace"), ("kvb_page_fork", (1, A, A, 1, A + 16, B, None), 1, "alignment"),
+    ("kvb_page_compact", (1, A, A, 16, None), 1, "workspace"), ("kvb_page_compact", (1, 0, A, B, None), 1, "null"),
     ("kvb_page_attend", (A, 1, 3, 1, A, 1, 0.1, A, None, A, B, None), 1, "Hq"),
     ("kvb_page_attend", (A, 1, 4, 0, A, 1, 0.1, A, None, A, B, None), 1, "Tq"),
     ("kvb_page_attend", (A, 0, 4, 1, A, 1, 0.1, A, None, A, B, None), 4, "float16"),
@@ -56,6 +56,14 @@ def test_pool_descriptor(field, value, status):
 def test_page_calls(name, args, status, word):
     st, msg = call(name, C.byref(pages()), *args)
     assert st == status and word in msg, (st, msg)
+
+
+def test_layers_share_their_table():
+    from kvb import _lib
+    two = (_lib.Pages * 2)(pages(), pages(table=2 * A))
+    for name, args in (("kvb_page_copy", (A, A, 1, None)), ("kvb_page_fork", (A, A, 1, A, B, None)), ("kvb_page_compact", (A, A, B, None))):
+        st, msg = call(name, two, 2, *args)
+        assert st == 1 and "share" in msg
 
 
 @pytest.mark.parametrize("change,status,word", [

@@ -251,6 +251,31 @@ def test_compact_large_pools(cuda_dev, n_pages):
     same(g, pool)
 
 
+def test_layers_of_one_table(cuda_dev):
+    """fork, compact and copy_pages on the first pool move the pages of every layer and change the table once."""
+    rng = np.random.default_rng(20)
+    pool = random_pool(rng, [40, 33, 64, 0], 2, 64, 16, spare=9)
+    other = {x: pool[x].copy() for x in NAMES}
+    other["kc"], other["vs"] = rng.integers(1, 256, pool["kc"].shape).astype(np.uint8), rng.random(pool["vs"].shape, np.float32)
+    g = on_gpu(pool)
+    h = g.add_layer(*[torch.from_numpy(other[x].copy()).cuda() for x in ("kc", "vc", "ks", "vs")])
+    for p in (pool, other):
+        O.fork(p, [0, 1], [3, 4])
+        O.free(p, [0, 2])
+        O.compact(p)
+        O.copy_page(p, 1, len(p["refs"]) - 1)
+    g.fork(ints([0, 1]), ints([3, 4]))
+    g.free(ints([0, 2]))
+    g.compact()
+    g.copy_pages(ints([1]), ints([len(pool["refs"]) - 1]))
+    same(g, pool)
+    same(h, other)
+    with pytest.raises(ValueError):
+        g.add_layer(*[x[:-1] for x in (h.kc, h.vc, h.ks, h.vs)])
+    q = torch.randn(1, 4, 1, 64, device="cuda", dtype=torch.float16)
+    check_attend(h, other, q, [4])
+
+
 def test_fork_and_free_refusals(cuda_dev):
     rng = np.random.default_rng(10)
     pool = random_pool(rng, [20, 33, 0], spare=1)
