@@ -34,8 +34,8 @@ template <typename T, int D, int NT>
 kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
     constexpr int SM = kvb::PdShape<D, NT>::SMEM;
     const auto kern = kvb::paged_decode_kernel<T, D, NT>;
-    if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "page_attend"))
-        return st;
+    static std::atomic<uint64_t> done{0};
+    if (kvb_status st = kvbh::allow_smem("page_attend", reinterpret_cast<const void*>(kern), SM, done)) return st;
     a.groups = (a.rep * a.Tq + 8 * NT - 1) / (8 * NT);
     const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
     const int n = a.n;

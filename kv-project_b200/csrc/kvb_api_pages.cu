@@ -35,6 +35,9 @@ kvb_status launch_write(const kvb::PageRowsParams& a, dim3 grid, cudaStream_t s)
     return launch_chained("page_write", kern, grid, kvb::PW_THREADS, 0, s, a);
 }
 
+// Threads of a planning block: 32 per 1024 pages (their barriers cost more than the pages of a small pool), 128 to 1024.
+unsigned page_block(const kvb_pages* p) { return unsigned(std::min<int64_t>(kvb::PG_THREADS, std::max<int64_t>(128, (p->n_pages + 1023) / 1024 * 32))); }
+
 // Pools of one table: the layers of a model.
 kvb_status check_layers(const char* who, const kvb_pages* p, int n_pools) {
     if (!p || n_pools <= 0) return fail(KVB_EINVAL, "%s: null argument", who);
@@ -114,7 +117,7 @@ kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32
     if (n > 0 && (!slots || !add || !start)) return fail(KVB_EINVAL, "page_extend: null argument");
     if (n < 0 || n > kMaxSequences) return fail(KVB_EINVAL, "page_extend: 0 <= n <= %d sequences a call", kMaxSequences);
     if (n == 0) return KVB_OK;
-    return launch_chained("page_extend", kvb::page_extend_kernel, 1, kvb::PG_THREADS, size_t(n) * 4, static_cast<cudaStream_t>(stream),
+    return launch_chained("page_extend", kvb::page_extend_kernel, 1, page_block(p), size_t(n) * 4, static_cast<cudaStream_t>(stream),
                           kvbh::view_of(p), slots, add, n, start);
 }
 
@@ -156,7 +159,7 @@ kvb_status kvb_page_fork(const kvb_pages* p, int n_pools, const int32_t* src, co
     const kvb::PagesView v = kvbh::view_of(p);
     const kvb::ForkWork w = fork_work(workspace, n);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (kvb_status st = launch_chained("page_fork plan", kvb::fork_plan_kernel, 1, kvb::PG_THREADS, size_t(n + 1) * 4, s, v, src, dst, n, w))
+    if (kvb_status st = launch_chained("page_fork plan", kvb::fork_plan_kernel, 1, page_block(p), size_t(n + 1) * 4, s, v, src, dst, n, w))
         return st;
     for (int i = 0; i < n_pools; ++i)
         if (kvb_status st = launch_chained("page_fork copy", kvb::fork_copy_kernel, dim3(unsigned(n), 1 + 8), kvb::PG_COPY_THREADS, 0, s,
@@ -181,7 +184,7 @@ kvb_status kvb_page_compact(const kvb_pages* p, int n_pools, int32_t* n_live, vo
     int32_t* b = static_cast<int32_t*>(workspace);
     const kvb::CompactWork w{b, b + 64, b + 64 + p->n_pages, b + 64 + 2 * p->n_pages};
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (kvb_status st = launch_chained("page_compact plan", kvb::compact_plan_kernel, 1, kvb::PG_THREADS, 0, s, v, w)) return st;
+    if (kvb_status st = launch_chained("page_compact plan", kvb::compact_plan_kernel, 1, page_block(p), 0, s, v, w)) return st;
     for (int i = 0; i < n_pools; ++i)
         if (kvb_status st = launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 4, kvb::PG_COPY_THREADS, 0, s,
                                            kvbh::view_of(p + i), w, n_live, i + 1 == n_pools))

@@ -37,8 +37,8 @@ template <typename T, int D>
 kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
     constexpr int SM = kvb::PfShape<D>::SMEM;
     const auto kern = kvb::prefill_kernel<T, D>;
-    if (kvb_status st = cuda_check(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, SM), "prefill_attention"))
-        return st;
+    static std::atomic<uint64_t> done{0};
+    if (kvb_status st = kvbh::allow_smem("prefill_attention", reinterpret_cast<const void*>(kern), SM, done)) return st;
     // without pieces no more CTAs than items (at most so many) have work
     const int64_t items = a.part ? kMaxCtas : a.Hkv * (a.nq / (2 * a.tt) + a.n);
     const int ctas = std::min(resolve_ctas(0), kMaxCtas);

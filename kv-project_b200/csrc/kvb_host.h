@@ -8,6 +8,7 @@
 #include <cuda.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstddef>
 #include <cstdint>
 
@@ -41,6 +42,18 @@ kvb_status launch_chained(const char* what, void (*fn)(P...), dim3 grid, dim3 bl
     cfg.attrs = at;
     cfg.numAttrs = 1;
     return cuda_check(cudaLaunchKernelEx(&cfg, fn, P(args)...), what);
+}
+
+// cudaFuncAttributeMaxDynamicSharedMemorySize, set once per kernel and device (`done`: a static of the kernel's launcher, a
+// bit per device; the attribute stays with the device's module).
+inline kvb_status allow_smem(const char* what, const void* fn, int bytes, std::atomic<uint64_t>& done) {
+    int dev = 0;
+    if (kvb_status st = cuda_check(cudaGetDevice(&dev), what)) return st;
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (dev < 64 && (done.load(std::memory_order_acquire) & bit)) return KVB_OK;
+    if (kvb_status st = cuda_check(cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes), what)) return st;
+    if (dev < 64) done.fetch_or(bit, std::memory_order_release);
+    return KVB_OK;
 }
 
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,

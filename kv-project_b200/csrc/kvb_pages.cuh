@@ -315,10 +315,11 @@ __global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_cons
 // Page tables.  One block of 1024 threads plans (which pages are free, who gets which), blocks of the
 // following launch move the data.
 // ------------------------------------------------------------------------------------------------
-constexpr int PG_THREADS = 1024;
-constexpr int PG_TILE = 32 * PG_THREADS;       // pages whose state the planning block holds in registers
+constexpr int PG_THREADS = 1024;               // at most; a block of 32 threads per 1024 pages where that is less (page_block)
+// pages whose state the planning block holds in registers
+__device__ __forceinline__ int page_tile() { return int(blockDim.x) * 32; }
 
-// Exclusive scan of one int per thread of a PG_THREADS block; total in `sum`.
+// Exclusive scan of one int per thread of the block; total in `sum`.
 __device__ __forceinline__ int block_scan(int v, int* sh, int& sum) {
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     int x = v;
@@ -330,7 +331,7 @@ __device__ __forceinline__ int block_scan(int v, int* sh, int& sum) {
     __syncthreads();
     if (lane == 31) sh[w] = x;
     __syncthreads();
-    int t = sh[lane];
+    int t = lane < int(blockDim.x >> 5) ? sh[lane] : 0;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const int y = __shfl_up_sync(0xffffffffu, t, o);
@@ -372,7 +373,7 @@ __device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh
     int found = 0, sum = 0, at = 0;
     uint32_t mask = 0;
     int64_t tile = -1;                         // whose mask and ranks are held
-    for (int64_t t0 = 0; t0 < P.n_pages && found < total; t0 += PG_TILE) {
+    for (int64_t t0 = 0; t0 < P.n_pages && found < total; t0 += page_tile()) {
         mask = free_mask(P.refs, P.n_pages, t0);
         at = block_scan(__popc(mask), sh, sum);
         tile = t0;
@@ -380,7 +381,7 @@ __device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh
     }
     if (found < total) return false;
     int before = 0;
-    for (int64_t t0 = 0; t0 < P.n_pages && before < total; t0 += PG_TILE) {
+    for (int64_t t0 = 0; t0 < P.n_pages && before < total; t0 += page_tile()) {
         if (tile != t0) {                      // a pool of one tile is read once
             mask = free_mask(P.refs, P.n_pages, t0);
             at = block_scan(__popc(mask), sh, sum);
@@ -393,7 +394,7 @@ __device__ __forceinline__ bool take_free(const PagesView& P, int total, int* sh
             for (uint32_t m = mask; m && rank < min(take - w0, PG_LIST); m &= m - 1, ++rank)
                 if (rank >= 0) list[rank] = int(base + __ffs(m) - 1);
             __syncthreads();
-            for (int r = threadIdx.x; r < min(take - w0, PG_LIST); r += PG_THREADS) give(before + w0 + r, list[r]);
+            for (int r = threadIdx.x; r < min(take - w0, PG_LIST); r += blockDim.x) give(before + w0 + r, list[r]);
             __syncthreads();
         }
         before += sum;
@@ -423,7 +424,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
     int total = 0;
-    for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
+    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
         const int i = i0 + threadIdx.x;
         int need = 0;
         if (i < n) {
@@ -449,7 +450,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
         if (threadIdx.x == 0) { raise_status(KVB_DEV_POOL); bad = 1; }
     }
     __syncthreads();                           // the lengths were read by every thread's give()
-    for (int i = threadIdx.x; i < n; i += PG_THREADS) {
+    for (int i = threadIdx.x; i < n; i += blockDim.x) {
         start[i] = bad ? -1 : P.lens[slots[i]];
         if (!bad) P.lens[slots[i]] += add[i];
     }
@@ -533,7 +534,7 @@ __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, cons
     if (threadIdx.x == 0) bad = 0;
     __syncthreads();
     int total = 0;
-    for (int i0 = 0; i0 < n; i0 += PG_THREADS) {
+    for (int i0 = 0; i0 < n; i0 += blockDim.x) {
         const int i = i0 + threadIdx.x;
         int part = 0;
         if (i < n) {
@@ -607,22 +608,22 @@ struct CompactWork {
     int32_t* new_id;
 };
 
-// One block.  A pool of one tile (32768 pages) is read once.
+// One block.  A pool of one tile is read once.
 __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, CompactWork W) {
     chain_kernels();
     __shared__ int sh[32], hole_list[PG_LIST], mover_list[PG_LIST];
     int live = 0, sum;
     uint32_t m = 0;
-    for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
+    for (int64_t t0 = 0; t0 < P.n_pages; t0 += page_tile()) {
         m = free_mask(P.refs, P.n_pages, t0);
         block_scan(__popc(m), sh, sum);
-        live += int(imin64(PG_TILE, P.n_pages - t0)) - sum;
+        live += int(imin64(page_tile(), P.n_pages - t0)) - sum;
     }
     // holes and movers in ascending order: as many of the one as of the other.  Where they fit they are listed in shared
     // memory and written out together.
     int holes = 0, movers = 0;
-    const bool one = P.n_pages <= PG_TILE;
-    for (int64_t t0 = 0; t0 < P.n_pages; t0 += PG_TILE) {
+    const bool one = P.n_pages <= page_tile();
+    for (int64_t t0 = 0; t0 < P.n_pages; t0 += page_tile()) {
         if (!one) m = free_mask(P.refs, P.n_pages, t0);
         const int64_t base = t0 + (threadIdx.x >> 5) * 1024 + (threadIdx.x & 31) * 32;
         const int64_t below = imin64(imax64(live - base, 0), 32), valid = imin64(imax64(P.n_pages - base, 0), 32);
@@ -643,15 +644,15 @@ __global__ void __launch_bounds__(PG_THREADS) compact_plan_kernel(PagesView P, C
             else W.from[movers + rm] = id;
         }
         __syncthreads();
-        for (int r = threadIdx.x; r < min(nh, PG_LIST); r += PG_THREADS) W.to[holes + r] = hole_list[r];
-        for (int r = threadIdx.x; r < min(nm, PG_LIST); r += PG_THREADS) W.from[movers + r] = mover_list[r];
+        for (int r = threadIdx.x; r < min(nh, PG_LIST); r += blockDim.x) W.to[holes + r] = hole_list[r];
+        for (int r = threadIdx.x; r < min(nm, PG_LIST); r += blockDim.x) W.from[movers + r] = mover_list[r];
         if (one)
-            for (int r = threadIdx.x; r < min(nm, PG_LIST); r += PG_THREADS) W.new_id[mover_list[r]] = hole_list[r];
+            for (int r = threadIdx.x; r < min(nm, PG_LIST); r += blockDim.x) W.new_id[mover_list[r]] = hole_list[r];
         holes += nh;
         movers += nm;
         __syncthreads();
     }
-    for (int r = (one ? PG_LIST : 0) + threadIdx.x; r < movers; r += PG_THREADS) W.new_id[W.from[r]] = W.to[r];
+    for (int r = (one ? PG_LIST : 0) + threadIdx.x; r < movers; r += blockDim.x) W.new_id[W.from[r]] = W.to[r];
     if (threadIdx.x == 0) {
         W.head[0] = live;
         W.head[1] = movers;

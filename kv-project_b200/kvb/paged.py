@@ -22,6 +22,8 @@ from . import _lib as L
 from .ops import _DT
 
 _I32 = torch.int32
+# a new dense tensor by its strides: 1.6 us where torch.empty takes 2.4
+_new = torch.empty_strided
 # the current stream's handle without building a Stream object, which costs as much as the launch (4.5 against 0.1 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
@@ -31,15 +33,6 @@ def _check_ints(who: str, n: int, *ts):
     for t in ts:
         if t.dtype is not _I32 or t.shape != (n,) or not t.is_cuda or not t.is_contiguous():
             raise ValueError(f"{who}: slots, starts, counts and offsets must be contiguous int32 CUDA tensors of {n} entries")
-
-
-def _dense(shape, dtype, device):
-    """A new contiguous tensor (empty_strided takes 1.6 us where empty takes 2.4)."""
-    strides, n = [], 1
-    for s in reversed(shape):
-        strides.append(n)
-        n *= s if s > 1 else 1
-    return torch.empty_strided(shape, strides[::-1], dtype=dtype, device=device)
 
 
 _PREFILL_WS = {}
@@ -80,10 +73,10 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     if d and not qs[2] == ks[2] == vs[2] == 1:
         raise ValueError("prefill_attention: d must be contiguous")
     if out is None:
-        out = _dense((nq, hq, d), q.dtype, q.device)
+        out = _new((nq, hq, d), (hq * d, d, 1), dtype=q.dtype, device=q.device)
     elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
         raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype")
-    lse = _dense((nq, hq), torch.float32, q.device) if return_lse else None
+    lse = _new((nq, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
     # a query tile has as many as 8 key tiles of 128, and may be split over them, only when there are so many keys
     lib, stream = L.lib(), _raw_stream(q.device.index)
     ws = _prefill_workspace(lib, q.device, stream, d) if nk > _UNSPLIT_KEYS else None
@@ -185,8 +178,7 @@ class PagePool:
         n = slots.shape[0]
         _check_ints("read", n, slots, start)
         _check_ints("read", n + 1, cu)
-        shape = (rows, self.Hkv, self.d)
-        k, v = _dense(shape, dtype, self.device), _dense(shape, dtype, self.device)
+        k, v = (_new((rows, self.Hkv, self.d), (self.Hkv * self.d, self.d, 1), dtype=dtype, device=self.device) for _ in "kv")
         st = L.lib().kvb_page_read(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                                    _DT.get(dtype, -1), rows, _raw_stream(self._index))
         if st:
@@ -203,10 +195,10 @@ class PagePool:
         if not q.is_contiguous():
             q = q.contiguous()
         if out is None:
-            out = _dense((n, tq, hq, d), q.dtype, q.device)
+            out = _new((n, tq, hq, d), (tq * hq * d, hq * d, d, 1), dtype=q.dtype, device=q.device)
         elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
             raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype")
-        lse = _dense((n, tq, hq), torch.float32, q.device) if return_lse else None
+        lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._ws.get((stream, n, hq, tq))
         if ws is None:
