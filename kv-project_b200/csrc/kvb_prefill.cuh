@@ -288,16 +288,17 @@ __device__ __forceinline__ int pf_warp_sum(int v) { return __reduce_add_sync(0xf
 
 // sum over i < n of floor((a i + b) / m), for a, b >= 0 (the Euclidean reduction of a and the divisor).  Intermediate
 // values stay below 2^32: n is a count of tile pairs, whose rows have to fit the GPU's memory.
-__device__ __forceinline__ int64_t pf_floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
-    int64_t sum = 0;
+__device__ __forceinline__ uint32_t pf_floor_sum(uint32_t n, uint32_t m, uint32_t a, uint32_t b) {
+    uint32_t sum = 0;
     while (n > 0) {
-        sum += int64_t(a / m) * (int64_t(n) * (n - 1) / 2) + int64_t(b / m) * n;
-        a %= m;
-        b %= m;
+        const uint32_t qa = a / m, qb = b / m;
+        sum += qa * uint32_t(uint64_t(n) * (n - 1) / 2) + qb * n;
+        a -= qa * m;
+        b -= qb * m;
         const uint32_t y = a * n + b;
         if (y < m) break;
         n = y / m;
-        b = y % m;
+        b = y - n * m;
         const uint32_t t = m;
         m = a;
         a = t;
@@ -331,41 +332,42 @@ constexpr int PF_SHARE = 8;                   // items of fewer tiles are never 
 
 struct PfCuts {
     int share;                                // items of more tiles are cut into pieces of at most so many
-    int64_t items;                            // how many are,
-    int64_t pieces;                           // into how many pieces
+    int items;                                // how many are,
+    int pieces;                               // into how many pieces
 };
 
-// The fair share, or eight tiles, and what it cuts; whole warp.  There are fewer pieces than 2 ctas: each has more than half
-// a share.
+// The fair share (not below eight tiles), and what it cuts; whole warp.  The share is that of a bound on the number of
+// tiles, at most half a tile an item too high; so there are at most 2 ctas pieces, each having half a share or more.
+// Item and piece counts fit 32 bits by far: 256 query rows an item.
 __device__ __forceinline__ PfCuts pf_cuts(const PrefillParams& A, int ctas) {
     const int lane = threadIdx.x & 31;
     PfCuts c{INT_MAX, 0, 0};
     if (!A.part) return c;
-    int64_t tiles = 0;
+    float tiles = 0.f;
     int most = 0;
     for (int s0 = 0; s0 < A.n; s0 += 32) {
         const PfSeq q = pf_seq(A, s0 + lane);
-        tiles += int64_t(pf_pieces(q, q.pairs, A.tt, PF_KT)) * A.Hkv;
-        most = max(most, q.pairs ? (q.kl + PF_KT - 1) / PF_KT : 0);
+        if (q.pairs == 0) continue;
+        // the pairs from the first that sees a key on end at a + b (i + 1) keys or before
+        const int a = q.kl - q.ql, b = 2 * A.tt, i0 = a < 0 ? min(-a / b, q.pairs) : 0;
+        const float k = float(q.pairs - i0);
+        tiles += k * (float(a) + float(b) * (float(i0) + 0.5f * (k + 1.f))) * (1.f / PF_KT) + k;
+        most = max(most, (q.kl + PF_KT - 1) / PF_KT);
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) tiles += __shfl_xor_sync(0xffffffffu, tiles, o);
+    tiles = warp_sum(tiles) * float(A.Hkv);
     most = __reduce_max_sync(0xffffffffu, most);
-    const int64_t share = imax64(PF_SHARE, (tiles + ctas - 1) / ctas);
-    if (most <= share) return c;
+    const float share = fmaxf(float(PF_SHARE), tiles * 1.0001f / float(ctas) + 1.f);
+    if (float(most) <= share) return c;
     c.share = int(share);
     for (int s0 = 0; s0 < A.n; s0 += 32) {
         const PfSeq q = pf_seq(A, s0 + lane);
         const int cut = q.pairs ? pf_count(q, c.share + 1, A.tt) : 0;
         const uint32_t keys = uint32_t(c.share) * PF_KT;
-        c.items += int64_t(cut) * A.Hkv;
-        if (cut) c.pieces += int64_t(pf_pieces(q, q.pairs, A.tt, keys) - pf_pieces(q, q.pairs - cut, A.tt, keys)) * A.Hkv;
+        c.items += cut * A.Hkv;
+        if (cut) c.pieces += (pf_pieces(q, q.pairs, A.tt, keys) - pf_pieces(q, q.pairs - cut, A.tt, keys)) * A.Hkv;
     }
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) {
-        c.items += __shfl_xor_sync(0xffffffffu, c.items, o);
-        c.pieces += __shfl_xor_sync(0xffffffffu, c.pieces, o);
-    }
+    c.items = __reduce_add_sync(0xffffffffu, c.items);
+    c.pieces = __reduce_add_sync(0xffffffffu, c.pieces);
     return c;
 }
 
@@ -425,64 +427,70 @@ __device__ __forceinline__ void pf_piece(const PrefillParams& A, const PfCuts& c
 
 // Item `idx`; `t` the last item's key tiles (a bound for the search), or < 0 at first.  Whole warp; false when there
 // are no more.
-__device__ __forceinline__ bool pf_item(const PrefillParams& A, const PfCuts& cuts, int64_t idx, int& t, PfItem& out) {
+__device__ __forceinline__ bool pf_item(const PrefillParams& A, const PfCuts& cuts, int idx, int& t, PfItem& out) {
     const int lane = threadIdx.x & 31;
     if (idx < cuts.pieces) {
-        pf_piece(A, cuts, int(idx), out);
+        pf_piece(A, cuts, idx, out);
         return true;
     }
     idx += cuts.items - cuts.pieces;              // place among all items by their tiles
-    PfSeq mine = pf_seq(A, lane);
-    auto total = [&](int tiles) {
-        int64_t c = 0;
-        for (int s0 = 0; s0 < A.n; s0 += 32) {
-            const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
-            c += pf_warp_sum(q.pairs ? pf_count(q, tiles, A.tt) : 0);
+    const PfSeq mine = pf_seq(A, lane);
+    auto total = [&](int tiles) {                 // items of `tiles` key tiles or more
+        int c = mine.pairs ? pf_count(mine, tiles, A.tt) : 0;
+        for (int s0 = 32; s0 < A.n; s0 += 32) {
+            const PfSeq q = pf_seq(A, s0 + lane);
+            if (q.pairs) c += pf_count(q, tiles, A.tt);
         }
-        return c * A.Hkv;
+        return pf_warp_sum(c) * A.Hkv;
     };
     int hi = t;
     if (t < 0) {
-        int most = 0;
-        for (int s0 = 0; s0 < A.n; s0 += 32) {
-            const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
-            most = max(most, __reduce_max_sync(0xffffffffu, (q.kl + PF_KT - 1) / PF_KT));
-        }
-        hi = min(most, cuts.share);
+        int most = (mine.kl + PF_KT - 1) / PF_KT;
+        for (int s0 = 32; s0 < A.n; s0 += 32) most = max(most, (pf_seq(A, s0 + lane).kl + PF_KT - 1) / PF_KT);
+        hi = min(__reduce_max_sync(0xffffffffu, most), cuts.share);
+        if (idx >= total(0)) return false;
     }
-    if (idx >= total(0)) return false;
-    int lo = 0;                                   // the largest t with total(t) > idx
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) / 2;
-        if (total(mid) > idx) lo = mid;
-        else hi = mid - 1;
+    int lo = 0, above = 0;                        // the largest t with total(t) > idx, and total(t + 1)
+    if (const int c = total(hi); c > idx) {
+        lo = hi;
+        above = total(hi + 1);
+    } else {
+        above = c;
+        --hi;
+        while (lo < hi) {
+            const int mid = (lo + hi + 1) / 2, m = total(mid);
+            if (m > idx) lo = mid;
+            else {
+                hi = mid - 1;
+                above = m;
+            }
+        }
+        if (lo == 0 && total(0) <= idx) return false;
     }
     t = lo;
-    int64_t r = idx - total(t + 1);               // rank among the items of t tiles
+    int r = idx - above;                          // rank among the items of t tiles
     for (int s0 = 0; s0 < A.n; s0 += 32) {
-        const PfSeq q = A.n <= 32 ? mine : pf_seq(A, s0 + lane);
-        const int above = q.pairs ? pf_count(q, t + 1, A.tt) : 0;
-        const int c = (q.pairs ? pf_count(q, t, A.tt) : 0) - above;
+        const PfSeq q = s0 == 0 ? mine : pf_seq(A, s0 + lane);
+        const int before = q.pairs ? pf_count(q, t + 1, A.tt) : 0, c = (q.pairs ? pf_count(q, t, A.tt) : 0) - before;
         int x = c;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int y = __shfl_up_sync(0xffffffffu, x, o);
             if (lane >= o) x += y;
         }
-        const int64_t sum = int64_t(__shfl_sync(0xffffffffu, x, 31)) * A.Hkv;
+        const int sum = __shfl_sync(0xffffffffu, x, 31) * A.Hkv;
         if (r >= sum) { r -= sum; continue; }
-        const uint32_t b = __ballot_sync(0xffffffffu, int64_t(x) * A.Hkv > r);
-        const int src = __ffs(int(b)) - 1;
-        const int64_t before = int64_t(x - c) * A.Hkv;
-        const int pair = q.pairs - above - c + int((r - before) / A.Hkv), head = int((r - before) % A.Hkv);
+        const int src = __ffs(int(__ballot_sync(0xffffffffu, x * A.Hkv > r))) - 1;
         out.q0 = __shfl_sync(0xffffffffu, q.q0, src);
         out.ql = __shfl_sync(0xffffffffu, q.ql, src);
         out.k0 = __shfl_sync(0xffffffffu, q.k0, src);
         out.kl = __shfl_sync(0xffffffffu, q.kl, src);
-        out.head = __shfl_sync(0xffffffffu, head, src);
+        r -= __shfl_sync(0xffffffffu, x - c, src) * A.Hkv;
+        const int step = r / A.Hkv;
+        out.head = r - step * A.Hkv;
         out.first = out.piece = 0;
         out.pieces = 1;
-        pf_tiles_of(A, __shfl_sync(0xffffffffu, pair, src), 0, INT_MAX, out);
+        pf_tiles_of(A, __shfl_sync(0xffffffffu, q.pairs - before - c, src) + step, 0, INT_MAX, out);
         return true;
     }
     return false;
@@ -547,7 +555,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         bool ok = true;
         const PfCuts cuts = pf_cuts(A, gridDim.x);
         for (int64_t round = 0; ok; ++round) {
-            const int64_t idx = round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x);
+            const int idx = int(round * gridDim.x + (round & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x));
             PfItem x;
             const bool more = pf_item(A, cuts, idx, t, x);
             PfItem& slot = sh.item[round & 1];
@@ -818,12 +826,12 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                 const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
                 if (!valid) return;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint32_t h[4];
+                for (int i = 0; i < 2; ++i) {                    // whole 32-byte sectors: a lane has a row of its own
+                    uint32_t h[8];
 #pragma unroll
-                    for (int k = 0; k < 4; ++k)
-                        h[k] = pf_pack<T>(__uint_as_float(o[8 * i + 2 * k]) * inv, __uint_as_float(o[8 * i + 2 * k + 1]) * inv);
-                    *reinterpret_cast<uint4*>(dst + c + 8 * i) = uint4{h[0], h[1], h[2], h[3]};
+                    for (int k = 0; k < 8; ++k)
+                        h[k] = pf_pack<T>(__uint_as_float(o[16 * i + 2 * k]) * inv, __uint_as_float(o[16 * i + 2 * k + 1]) * inv);
+                    asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::PF_W8(h, 0), "l"(dst + c + 16 * i) : "memory");
                 }
             };
             auto store_lse = [&](float top, float sum) {
