@@ -64,8 +64,8 @@ namespace kvbh {
 kvb_status check_pages(const char* who, const kvb_pages* p) {
     if (!p || !p->kc || !p->vc || !p->ks || !p->vs || !p->table || !p->lens || !p->refs)
         return fail(KVB_EINVAL, "%s: null argument", who);
-    if (p->n_pages <= 0 || p->n_pages > INT32_MAX || p->Hkv <= 0 || p->Hkv > 65535 || p->n_slots <= 0 || p->max_blocks <= 0)
-        return fail(KVB_EINVAL, "%s: sizes of the pool (0 < Hkv <= 65535, 0 < n_pages < 2^31)", who);
+    if (p->n_pages <= 0 || p->n_pages > INT32_MAX || p->Hkv <= 0 || p->Hkv > 4096 || p->n_slots <= 0 || p->max_blocks <= 0)
+        return fail(KVB_EINVAL, "%s: sizes of the pool (0 < Hkv <= 4096, 0 < n_pages < 2^31)", who);
     if (p->page != 16 && p->page != 32 && p->page != 64 && p->page != 128)
         return fail(KVB_EUNSUPPORTED, "%s: pages of 16, 32, 64 or 128 tokens", who);
     if (p->d != 64 && p->d != 128) return fail(KVB_EUNSUPPORTED, "%s: d 64 or 128", who);

@@ -377,6 +377,72 @@ def test_attend_peaked_and_flat(cuda_dev):
     check_attend(g, pool, q, [0], 0.5)
 
 
+@pytest.mark.parametrize("scaling", [-0.1, 0.0, 1e-30])
+def test_attend_any_scaling(cuda_dev, scaling):
+    rng = np.random.default_rng(21)
+    pool = random_pool(rng, [333, 20], 2, 64, 16)
+    q = torch.from_numpy(rng.standard_normal((2, 4, 3, 64))).half().cuda()
+    out, lse = on_gpu(pool).attend(q, ints([0, 1]), scaling, return_lse=True)
+    want, wl, mean_abs = O.attend(pool, q.float().cpu().numpy(), [0, 1], scaling)
+    assert (np.abs(out.double().cpu().numpy() - want) <= 2.0 ** -9 * mean_abs + 1e-4).all()
+    assert np.abs(lse.double().cpu().numpy() - wl).max() <= 1e-3
+
+
+def test_attend_more_sequences_than_one_launch_takes(cuda_dev):
+    rng = np.random.default_rng(22)
+    lens = [(i * 7) % 50 for i in range(1100)]
+    pool = random_pool(rng, lens, 1, 64, 16)
+    slots = rng.permutation(1100)
+    q = torch.from_numpy(rng.standard_normal((1100, 2, 1, 64))).half().cuda()
+    check_attend(on_gpu(pool), pool, q, slots)
+
+
+def test_attend_rows_do_not_touch_each_other(cuda_dev):
+    """NaN and infinities in one query leave the other rows as they are."""
+    rng = np.random.default_rng(23)
+    pool = random_pool(rng, [700, 90], 2, 128, 32)
+    g = on_gpu(pool)
+    q = torch.from_numpy(rng.standard_normal((2, 8, 2, 128))).half().cuda()
+    clean = g.attend(q, ints([0, 1]))
+    for bad in (float("nan"), float("inf")):
+        p = q.clone()
+        p[0, 3, 1, 7] = bad
+        got = g.attend(p, ints([0, 1]))
+        assert not torch.isfinite(got[0, 1, 3]).any()
+        got[0, 1, 3] = clean[0, 1, 3]
+        assert torch.equal(got, clean)
+
+
+def test_attend_reports_a_workspace_that_was_not_zero(cuda_dev):
+    rng = np.random.default_rng(24)
+    g = on_gpu(random_pool(rng, [30000], 1, 64, 64))
+    q = torch.randn(1, 2, 1, 64, device="cuda", dtype=torch.float16)
+    g.attend(q, ints([0]))
+    for ws in g._ws.values():
+        ws[:1024] = 77
+    g.attend(q, ints([0]))
+    assert status() == 8
+
+
+def test_many_sequences_in_one_call(cuda_dev):
+    rng = np.random.default_rng(25)
+    n = 1500
+    pool = O.empty_pool(5000, 1, 64, 16, 2 * n, 4)
+    g = on_gpu(pool)
+    slots, add = rng.permutation(2 * n)[:n], rng.integers(0, 30, n)
+    got = g.extend(ints(slots), ints(add))
+    assert np.array_equal(got.cpu().numpy(), O.extend(pool, slots, add))
+    same(g, pool)
+    dst = rng.permutation(2 * n)[:n]
+    assert O.fork(pool, slots, dst)
+    g.fork(ints(slots), ints(dst))
+    same(g, pool)
+    O.free(pool, slots[:700])
+    g.free(ints(slots[:700]))
+    assert int(g.compact()) == O.compact(pool)
+    same(g, pool)
+
+
 def test_attend_refuses_what_does_not_fit(cuda_dev):
     rng = np.random.default_rng(16)
     pool = random_pool(rng, [100, 50])

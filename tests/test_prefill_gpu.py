@@ -61,7 +61,7 @@ def check(q, k, v, cu_q, cu_k, scaling=None, out_rows=slice(None), **kw):
     want, wl, mean_abs = exact(q, k, v, cu_q, cu_k, sc)
     u, d = U[q.dtype], q.shape[2]
     fin = torch.where(torch.isfinite(k.float()), k.float(), 0.0)
-    e = d * 2.0 ** -24 * float(fin.abs().sum(-1).max() if k.numel() else 0) * float(q.float().abs().max()) * sc
+    e = d * 2.0 ** -24 * float(fin.abs().sum(-1).max() if k.numel() else 0) * float(q.float().abs().max()) * abs(sc)
     vmax = float(torch.where(torch.isfinite(v.float()), v.float(), 0.0).abs().max()) if v.numel() else 0.0
     keys = int((cu_k[1:] - cu_k[:-1]).max())
     tol = (2 * u + 2.0 ** -13 + 2 * e) * mean_abs + keys * 2.0 ** -24 * vmax
@@ -158,6 +158,60 @@ def test_prefill_extreme_logits(cuda_dev):
     q2 = torch.sign(q) * 16
     check(q2, k, v, cu_of([300]), cu_of([300]), scaling=64.0)
     check(torch.zeros_like(q), k, v, cu_of([300]), cu_of([300]))
+
+
+@pytest.mark.parametrize("scaling", [-0.1, 0.0, 1e-30])
+def test_prefill_any_scaling(cuda_dev, scaling):
+    g = torch.Generator(device="cuda").manual_seed(28)
+    q, k, v = rand(g, 300, 4, 64, dtype=torch.float16), rand(g, 300, 2, 64, dtype=torch.float16), rand(g, 300, 2, 64, dtype=torch.float16)
+    check(q, k, v, cu_of([100, 200]), cu_of([100, 200]), scaling)
+
+
+SPLIT = [       # few rows over long keys: their items are computed in pieces
+    (torch.float16, 64, 4, 4, [500, 1100], [7500, 1433]),
+    (torch.bfloat16, 128, 1, 8, [1, 70, 3], [9001, 4000, 129]),
+    (torch.bfloat16, 128, 2, 1, [200], [20000]),
+    (torch.float16, 128, 1, 3, [5, 2000], [12345, 2000]),
+    (torch.bfloat16, 64, 2, 2, [64] * 40, [1100 + 37 * i for i in range(40)]),
+]
+
+
+@pytest.mark.parametrize("dtype,d,hkv,rep,ql,kl", SPLIT)
+def test_prefill_in_pieces(cuda_dev, dtype, d, hkv, rep, ql, kl):
+    g = torch.Generator(device="cuda").manual_seed(29)
+    q, k, v = rand(g, sum(ql), hkv * rep, d, dtype=dtype), rand(g, sum(kl), hkv, d, dtype=dtype), rand(g, sum(kl), hkv, d, dtype=dtype)
+    check(q, k, v, cu_of(ql), cu_of(kl))
+    check(3 * q, k, v, cu_of(ql), cu_of(kl))
+
+
+def test_pieces_keep_non_finite_values_where_they_are_seen(cuda_dev):
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(30)
+    q, k, v = rand(g, 40, 4, 128, dtype=torch.bfloat16), rand(g, 9000, 1, 128, dtype=torch.bfloat16), rand(g, 9000, 1, 128, dtype=torch.bfloat16)
+    cu_q, cu_k = cu_of([40]), cu_of([9000])
+    clean = check(q, k, v, cu_q, cu_k)
+    for key in (100, 5000, 8965, 8999):
+        p = v.clone()
+        p[key, 0, 9] = float("nan")
+        got = kvb.prefill_attention(q, k, p, cu_q, cu_k)
+        first = max(0, key - 8960)                       # the first query that sees the key
+        assert torch.equal(got[:first], clean[:first]) and torch.isnan(got[first:, :, 9]).all()
+        assert torch.equal(got[..., :9], clean[..., :9]) and torch.equal(got[..., 10:], clean[..., 10:])
+
+
+def test_prefill_reports_a_workspace_that_was_not_zero(cuda_dev):
+    import kvb
+    from kvb import paged
+    q, k = torch.randn(40, 4, 64, device="cuda", dtype=torch.float16), torch.randn(9000, 1, 64, device="cuda", dtype=torch.float16)
+    cu_q, cu_k = cu_of([40]), cu_of([9000])
+    want = kvb.prefill_attention(q, k, k, cu_q, cu_k)
+    for ws in paged._PREFILL_WS.values():
+        ws[:16384] = 77
+    kvb.prefill_attention(q, k, k, cu_q, cu_k)
+    assert kvb.device_status() == 8
+    for ws in paged._PREFILL_WS.values():
+        ws[:16384] = 0
+    assert torch.equal(kvb.prefill_attention(q, k, k, cu_q, cu_k), want) and kvb.device_status() == 0
 
 
 @pytest.mark.parametrize("dtype,d", [(torch.float16, 128), (torch.bfloat16, 64)])
