@@ -24,7 +24,9 @@
 // runs converged.  16384 tokens, 32 heads over 8, d 128: 2102 us without these three, 1885 with the converged warp, 1799
 // with the early weights and P in halves, 1728 with the masked tiles known ahead, 1649 with P in 96 + 32 and 224
 // registers (1334 TFLOP/s).  Measured and left: two threads a row (1971), steps of 64 keys with two score buffers (1894), an MMA warp
-// per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906).
+// per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906), growth seen from the sum of the
+// weights instead of the maximum (no difference).  At 8192 tokens (463 us, 1187 TFLOP/s at the 1.63 GHz that the power cap leaves)
+// the tensor pipe is busy 64 % of the time and the special function unit 64 %.
 //
 // Masks: logits of keys past a row's limit become -inf by selection, so what lies there does not matter; values
 // there would still meet a weight of zero in the MMA (0 * NaN), so in tiles that some row of the item does not see
