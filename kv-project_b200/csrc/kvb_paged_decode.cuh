@@ -292,11 +292,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     int copied = 0;
     auto copy = [&]() {                                          // the warp's next unit
         if (copied >= mine) return;
-        if ((copied & 31) == 0) {
-            if (copied > 0) at = ahead;
-            sc_next = scales_of(at);
-            ahead = place(copied + 32 + lane);
-        }
+        if ((copied & 31) == 0 && copied > 0) at = ahead;
         if (lane == (copied & 31)) {
             const int st = copied % S::STAGES;
             uint64_t* bar = &full[warp][st];
@@ -308,6 +304,10 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     tma_load_3d(dst + i * box * D, &A.tm_k, 0, at.off, at.row[i], bar);
                     tma_load_3d(dst + S::SIDE + i * box * D, &A.tm_v, 0, at.off, at.row[i], bar);
                 }
+        }
+        if ((copied & 31) == 0) {                                // needed a unit or more later
+            sc_next = scales_of(at);
+            ahead = place(copied + 32 + lane);
         }
         ++copied;
     };
