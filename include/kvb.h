@@ -473,8 +473,7 @@ kvb_status kvb_operational_rd(const float* A, int64_t rows, int64_t n, int64_t l
  * positions.  A row that sees no key gives zeros and -inf.  q (nq, Hq, d), k and v (nk, Hkv, d) of one dtype
  * (f16 / bf16) with d in {64, 128} contiguous, the element strides below multiples of 8 and 16-byte aligned
  * bases; cu_q, cu_k (n + 1) int32 on the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 32-byte
- * aligned;
- * lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written.
+ * aligned; lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written.
  * workspace (kvb_prefill_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
  * (every call leaves its counters at zero), one per stream that runs calls concurrently; with it the work of
  * long rows is split over the keys, without it (null) every query tile is computed in one piece. */

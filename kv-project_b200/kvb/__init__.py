@@ -3,7 +3,8 @@
 Drop-in native replacement for the decode-time hot path shared by the KV-cache compression
 methods of TahirSher/KV-Project: quantise + pack (K1), importance scores + budgeted eviction /
 strata assignment (K2), fused split-K flash decoding over packed codes (K3), the spectral code
-(K4) and per-vector row codes (K5: absmax tails, HEDGE, TILT chunk selection, MSB-first packing).  All compute runs in ``libkvb.so`` (hand-written CUDA for sm_100a behind the C ABI of
+(K4) and per-vector row codes (K5: absmax tails, HEDGE, TILT chunk selection, MSB-first packing); and the
+paged path (prefill attention of packed prompts, a pool of 8-bit pages).  All compute runs in ``libkvb.so`` (hand-written CUDA for sm_100a behind the C ABI of
 ``include/kvb.h``); this package only moves tensors and builds descriptors.
 """
 
