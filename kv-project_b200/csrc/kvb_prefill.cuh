@@ -536,7 +536,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
-    chain_kernels();
     const uint32_t tmem = sh.tmem;
     volatile int* abort = &sh.abort;
     // a wait that gave up stops every role
@@ -840,13 +839,13 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                 if (valid && A.lse)
                     A.lse[out_row * A.Hq + hq] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
             };
-            const bool whole = x.pieces == 1;
+            const bool whole = x.pieces == 1, used = __any_sync(0xffffffffu, valid);
             auto slot_of = [&](int piece) {                      // this tile's part: O by column, then m and l
                 return A.part + (int64_t(piece) * 2 + w) * ((D + 2) * 128) + row;
             };
             float* part = whole ? nullptr : slot_of(x.piece);
 #pragma unroll 1
-            for (int c = 0; c < D; c += 32) {
+            for (int c = 0; c < (used ? D : 0); c += 32) {
                 uint32_t o[32];
                 if (n > 0) {
                     pf_ld32(o_col + c, o);
@@ -877,7 +876,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             }
             if (whole) {
                 store_lse(m, l);
-            } else {
+            } else if (used) {
                 __stcg(part + D * 128, m);
                 __stcg(part + (D + 1) * 128, l);
                 __threadfence();
