@@ -49,11 +49,13 @@ __device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t* p) {
     return v;
 }
 
-// First thing in a kernel that is launched with programmatic stream serialization (kvbh::launch_chained): the next kernel's
-// blocks may take their places now, and this one's memory accesses begin when everything before it has completed.
+// First thing in a kernel that is launched with programmatic stream serialization (kvbh::launch_chained): this one's memory
+// accesses begin when everything before it has completed, and from then on the next kernel's blocks may take their places
+// (let in before the wait, so that several kernels queue up on the SMs, short chains took longer: freeing, compacting and
+// extending 45.1 us instead of 43.8).
 __device__ __forceinline__ void chain_kernels() {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
