@@ -11,10 +11,10 @@
 
 namespace {
 
-constexpr int64_t kCountBytes = kvb::PD_MAX_CTAS * 4;
+constexpr int64_t kCountBytes = kvb::PD_MAX_CTAS * 8 * 4;      // per warp
 
 // floats of one partial: up to 16 query rows
-int64_t part_floats(int d) { return 16 * (int64_t(d) + 2); }
+int64_t part_floats(int d) { return 16 * (int64_t(d) + 4); }
 
 // Codes as (d, page, n_pages * Hkv) bytes: box d x min(page, 32) x 1, swizzled over the d bytes of a row.
 kvb_status make_map(CUtensorMap* m, const kvb_pages* p, const void* codes) {

@@ -49,6 +49,14 @@ __device__ __forceinline__ uint32_t ld_acquire_sys(const uint32_t* p) {
     return v;
 }
 
+// After a barrier of the threads whose writes it publishes; before one of the threads that read what it acquires (with
+// loads that pass the L1).
+__device__ __forceinline__ uint32_t atomic_add_acq_rel(uint32_t* p, uint32_t v) {
+    uint32_t old;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], %2;" : "=r"(old) : "l"(p), "r"(v) : "memory");
+    return old;
+}
+
 // First thing in a kernel that is launched with programmatic stream serialization (kvbh::launch_chained): this one's memory
 // accesses begin when everything before it has completed, and from then on the next kernel's blocks may take their places
 // (let in before the wait, so that several kernels queue up on the SMs, short chains took longer: freeing, compacting and

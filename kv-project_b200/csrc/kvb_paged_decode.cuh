@@ -12,7 +12,7 @@
 // was slower than the copies: 178 us for 537 MB without any arithmetic) and keeps its own running softmax.  Page numbers
 // and scales are fetched 32 units ahead, a lane a unit.  At the end of a run the warps' states are joined in shared
 // memory; a run that is only a part of a (sequence, head, group) leaves a partial, and the CTA that completes the last
-// part joins the partials in the order of the tokens, so the result does not depend on timing.
+// part joins the partials in the order of the tokens (each warp its rows), so the result does not depend on timing.
 //
 // A step of 8 sequences of 32768 tokens, 8 heads, d 128 (537 MB), with the write of its rows: 99.8 us, 5.4 TB/s; about 7
 // TB/s at the margin, the rest is the start (4 us), the first copies' latency and the join (the same step without any
@@ -57,8 +57,8 @@ struct PagedDecodeParams {
     float lam;
     void* out;                                // (n, Tq, Hq, d)
     float* lse;                               // (n, Tq, Hq) or null
-    float* part;                              // [2 grid][8 NT x (2 + d)]: m, l, then O
-    uint32_t* count;                          // [grid]
+    float* part;                              // [2 grid][8 NT x (4 + d)]
+    uint32_t* count;                          // [grid][8 warps]
 };
 
 template <int D, int NT>
@@ -70,7 +70,8 @@ struct PdShape {
     static constexpr int STAGE = 2 * SIDE;
     static constexpr int STAGES = 3 * (128 / D);             // per warp
     static constexpr int JOIN = WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
-    static constexpr int PART = ROWS * (D + 2);
+    static constexpr int PAIRS = NT * (D / 64);              // (row, 64 channels) that a warp joins
+    static constexpr int PART = ROWS * (D + 4);              // m, l of the rows, twice (see the joining), then O
     static constexpr int SMEM = 1024 + WARPS * STAGES * STAGE + JOIN;
 };
 
@@ -162,7 +163,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     __shared__ uint64_t full[S::WARPS][S::STAGES];
     __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS];
     __shared__ int warp_sum[S::WARPS];
-    __shared__ int s_abort, s_last;
+    __shared__ int s_abort;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
     float* join = reinterpret_cast<float*>(base + S::WARPS * S::STAGES * S::STAGE);      // [warp][8 rows][64 + 4]
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -523,8 +524,14 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 pn = pd_piece(W, next, u1);
                 load_q(pn);
             }
-            // ---- join the warps: row sums, then O, 8 rows at a time
-            asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");           // the last join's reads are done
+            // ---- join the warps.  Warp w joins the rows w and 8 + w, 64 channels at a time; where there are at most four
+            // rows of 128 channels, row w % 4 and the half w / 4 of its channels, all at once.  Column c of the buffer is
+            // channel (D / 8) (c / 8) + 8 y + c % 8 of the half y.
+            const bool few = D == 128 && NT == 1 && nrows <= 4;
+            const bool whole = p.a == 0 && p.b == p.units;
+            // the CTAs c0 .. c1 hold its units
+            const int c0 = whole ? 0 : W.holder(p.v0 + PD_FIXED), c1 = whole ? 0 : W.holder(p.v0 + PD_FIXED + p.units - 1);
+            if (!first) asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");       // the last join's reads are done
 #pragma unroll
             for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -538,22 +545,31 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         s_l[warp][8 * x + 2 * t + k] = v;
                     }
                 }
-            const bool whole = p.a == 0 && p.b == p.units;
             float* part = A.part + int64_t(2 * blockIdx.x + (first ? 0 : 1)) * S::PART;
+            const int ml = few ? warp >> 2 : 0;                  // which copy of m and l
+            const bool used = (few ? warp & 3 : warp) < nrows;
+            auto row_of = [&](int x) { return few ? warp & 3 : 8 * x + warp; };
+            auto channel_of = [&](int y) { return (D / 8) * (lane >> 2) + 8 * (few ? warp >> 2 : y) + 2 * (lane & 3); };
+            auto put = [&](int x, int y, int slot) {             // O of the rows 2t, 2t + 1, half y
+                float* to = join + warp * 8 * 68 + slot * 68 + 8 * g;
+#pragma unroll
+                for (int c = 0; c < 4; ++c) {
+                    *reinterpret_cast<float2*>(to + 2 * c) = float2{o[x][4 * y + c][0], o[x][4 * y + c][2]};
+                    *reinterpret_cast<float2*>(to + 68 + 2 * c) = float2{o[x][4 * y + c][1], o[x][4 * y + c][3]};
+                }
+            };
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                // warp w joins query row 8 x + w; column c of the buffer is channel (D / 8) (c / 8) + 8 y + c % 8
-                const int r = 8 * x + warp;
+                const int r = row_of(x);
                 float top = -INFINITY, sum = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
+                    if (few && y > 0) break;
                     if (x + y > 0) asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
-                    float* to = join + warp * 8 * 68 + 2 * t * 68 + 8 * g;
+                    if (!few) put(x, y, 2 * t);
+                    else if (t < 2)
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        *reinterpret_cast<float2*>(to + 2 * c) = float2{o[x][4 * y + c][0], o[x][4 * y + c][2]};
-                        *reinterpret_cast<float2*>(to + 68 + 2 * c) = float2{o[x][4 * y + c][1], o[x][4 * y + c][3]};
-                    }
+                        for (int k = 0; k < D / 64; ++k) put(x, k, 4 * k + 2 * t);
                     asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                     if (y == 0) {
 #pragma unroll
@@ -572,65 +588,97 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.x = __fmaf_rn(v.x, f[w], acc.x);
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
-                    const int ch = (D / 8) * (lane >> 2) + 8 * y + 2 * (lane & 3);
                     if (whole) {
-                        if (r < nrows) store_pair(p.seq, h, row0 + r, ch, acc.x, acc.y, sum);
-                    } else {
-                        *reinterpret_cast<float2*>(part + 2 * S::ROWS + r * D + ch) = acc;
+                        if (r < nrows) store_pair(p.seq, h, row0 + r, channel_of(y), acc.x, acc.y, sum);
+                    } else if (r < nrows) {
+                        *reinterpret_cast<float2*>(part + 4 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
                 }
-                if (whole) {
-                    if (r < nrows && lane == 0) store_lse(p.seq, h, row0 + r, top, sum);
-                } else if (lane == 0) {
-                    part[r] = top;
-                    part[S::ROWS + r] = sum;
+                if (lane == 0 && r < nrows) {
+                    if (whole) {
+                        if (ml == 0) store_lse(p.seq, h, row0 + r, top, sum);
+                    } else {
+                        part[2 * ml * S::ROWS + r] = top;
+                        part[(2 * ml + 1) * S::ROWS + r] = sum;
+                    }
                 }
             }
-            if (!whole) {
-                // its units belong to the CTAs c0 .. c1; the last of them to arrive joins
-                const int c0 = W.holder(p.v0 + PD_FIXED), c1 = W.holder(p.v0 + PD_FIXED + p.units - 1);
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
-                if (threadIdx.x == 0) {
-                    __threadfence();
-                    const uint32_t seen = atomicAdd(&A.count[c0], 1u);
-                    s_last = seen == uint32_t(c1 - c0);
-                    if (s_last) A.count[c0] = 0;
-                    else if (seen > uint32_t(c1 - c0)) raise_status(KVB_DEV_WORKSPACE);
-                    __threadfence();
-                }
-                asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
-                if (s_last) {
+            if (!whole && used) {
+                // each warp for its rows: the last CTA to arrive joins the CTAs' partials.  The loops are kept short: code
+                // that runs once per call is fetched as it runs (with 24 partials unrolled the joining took 3.9 us)
+                uint32_t* count = A.count + c0 * S::WARPS + warp;
+                uint32_t seen = 0;
+                __syncwarp();
+                if (lane == 0) seen = atomic_add_acq_rel(count, 1u);
+                seen = __shfl_sync(0xffffffffu, seen, 0);
+                if (seen > uint32_t(c1 - c0)) {
+                    if (lane == 0) raise_status(KVB_DEV_WORKSPACE);
+                } else if (seen == uint32_t(c1 - c0)) {
+                    if (lane == 0) *count = 0;
                     // the partial of c is its first one, unless the (sequence, head, group) begins inside c's run
                     const float* slot0 = A.part + int64_t(2 * c0 + (W.share(c0) < p.v0 ? 1 : 0)) * S::PART;
                     auto slot_of = [&](int c) { return c == c0 ? slot0 : A.part + int64_t(2 * c) * S::PART; };
-                    for (int r = warp; r < nrows; r += S::WARPS) {
-                        float top = -INFINITY;
-                        for (int c = c0 + lane; c <= c1; c += 32) top = fmaxf(top, __ldcg(slot_of(c) + r));
-                        top = warp_max(top);
-                        const float ref = top == -INFINITY ? 0.f : top;
-                        float sum = 0.f;
-                        float2 acc[D / 64];
+                    float top[NT], sum[NT];
+                    float2 acc[NT][D / 64];
 #pragma unroll
-                        for (int i = 0; i < D / 64; ++i) acc[i] = float2{0.f, 0.f};
-                        for (int cc = c0; cc <= c1; cc += 32) {
-                            const int mine_c = min(cc + lane, c1);
-                            const float f_mine = ex2(__ldcg(slot_of(mine_c) + r) - ref), l_mine = __ldcg(slot_of(mine_c) + S::ROWS + r);
-#pragma unroll 8
-                            for (int k = 0; k < min(32, c1 - cc + 1); ++k) {
-                                const float f = __shfl_sync(0xffffffffu, f_mine, k);
-                                sum = __fmaf_rn(__shfl_sync(0xffffffffu, l_mine, k), f, sum);
-                                const float* q = slot_of(cc + k) + 2 * S::ROWS + r * D + 2 * lane;
+                    for (int x = 0; x < NT; ++x) {
+                        top[x] = -INFINITY;
+                        sum[x] = 0.f;
 #pragma unroll
-                                for (int i = 0; i < D / 64; ++i) {
-                                    const float2 v = __ldcg(reinterpret_cast<const float2*>(q + 64 * i));
-                                    acc[i].x = __fmaf_rn(v.x, f, acc[i].x);
-                                    acc[i].y = __fmaf_rn(v.y, f, acc[i].y);
-                                }
-                            }
+                        for (int y = 0; y < D / 64; ++y) acc[x][y] = float2{0.f, 0.f};
+                    }
+                    for (int cc = c0; cc <= c1; cc += 32) {      // 32 partials: a lane has the m and l of one
+                        const int cnt = min(32, c1 - cc + 1);
+                        const float* mine_p = slot_of(min(cc + lane, c1)) + 2 * ml * S::ROWS;
+                        float f[NT];
+#pragma unroll
+                        for (int x = 0; x < NT; ++x) {
+                            const float mv = lane < cnt ? __ldcg(mine_p + row_of(x)) : -INFINITY;
+                            const float lv = lane < cnt ? __ldcg(mine_p + S::ROWS + row_of(x)) : 0.f;
+                            const float to = fmaxf(top[x], warp_max(mv)), ref = to == -INFINITY ? 0.f : to, old = ex2(top[x] - ref);
+                            top[x] = to;
+                            f[x] = ex2(mv - ref);
+                            sum[x] = __fmaf_rn(sum[x], old, kvb::warp_sum(lv * f[x]));
+#pragma unroll
+                            for (int y = 0; y < D / 64; ++y) acc[x][y].x *= old, acc[x][y].y *= old;
                         }
+                        constexpr int B = 16 / NT;               // partials whose loads are in flight together
+#pragma unroll 1
+                        for (int k0 = 0; k0 < cnt; k0 += B) {
+                            float2 v[B][NT][D / 64];
+                            const float* q = A.part + int64_t(2 * (cc + k0)) * S::PART + 4 * S::ROWS;
 #pragma unroll
-                        for (int i = 0; i < D / 64; ++i) store_pair(p.seq, h, row0 + r, 2 * lane + 64 * i, acc[i].x, acc[i].y, sum);
-                        if (lane == 0) store_lse(p.seq, h, row0 + r, top, sum);
+                            for (int k = 0; k < B; ++k) {
+                                const float* qk = k == 0 && cc + k0 == c0 ? slot0 + 4 * S::ROWS : q + 2 * k * S::PART;
+#pragma unroll
+                                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                                    for (int y = 0; y < D / 64; ++y) {
+                                        v[k][x][y] = float2{0.f, 0.f};
+                                        if (k0 + k < cnt && !(few && y > 0))
+                                            v[k][x][y] = __ldcg(reinterpret_cast<const float2*>(qk + row_of(x) * D + channel_of(y)));
+                                    }
+                            }
+#pragma unroll
+                            for (int k = 0; k < B; ++k)
+#pragma unroll
+                                for (int x = 0; x < NT; ++x) {
+                                    const float fk = __shfl_sync(0xffffffffu, f[x], (k0 + k) & 31);
+#pragma unroll
+                                    for (int y = 0; y < D / 64; ++y) {
+                                        acc[x][y].x = __fmaf_rn(v[k][x][y].x, fk, acc[x][y].x);
+                                        acc[x][y].y = __fmaf_rn(v[k][x][y].y, fk, acc[x][y].y);
+                                    }
+                                }
+                        }
+                    }
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        if (row_of(x) >= nrows) continue;
+#pragma unroll
+                        for (int y = 0; y < D / 64; ++y)
+                            if (!(few && y > 0)) store_pair(p.seq, h, row0 + row_of(x), channel_of(y), acc[x][y].x, acc[x][y].y, sum[x]);
+                        if (lane == 0 && ml == 0) store_lse(p.seq, h, row0 + row_of(x), top[x], sum[x]);
                     }
                 }
             }
