@@ -16,6 +16,9 @@ constexpr int64_t kCountBytes = kvb::PD_MAX_CTAS * 8 * 4;      // per warp
 // floats of one partial: up to 16 query rows
 int64_t part_floats(int d) { return 16 * (int64_t(d) + 4); }
 
+// ceil(2^64 / d) for kvb::pd_div; 0 for 1
+uint64_t reciprocal(int d) { return d == 1 ? 0 : UINT64_MAX / uint64_t(d) + 1; }
+
 // Codes as (d, page, n_pages * Hkv) bytes: box d x min(page, 32) x 1, swizzled over the d bytes of a row.
 kvb_status make_map(CUtensorMap* m, const kvb_pages* p, const void* codes) {
     EncodeTiledFn fn = encode_tiled();
@@ -37,6 +40,9 @@ kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = kvbh::allow_smem("page_attend", reinterpret_cast<const void*>(kern), SM, done)) return st;
     a.groups = (a.rep * a.Tq + 8 * NT - 1) / (8 * NT);
+    a.by_groups = reciprocal(a.groups);
+    a.by_rep = reciprocal(a.rep);
+    a.page_log2 = 31 - __builtin_clz(unsigned(a.P.page));
     const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
     const int n = a.n;
     const char* q = static_cast<const char*>(a.q);

@@ -54,6 +54,8 @@ struct PagedDecodeParams {
     const void* q;                            // (n, Hq, Tq, d)
     const int32_t* slots;
     int n, Hq, Tq, rep, groups;               // groups of 8 NT query rows per (sequence, KV head)
+    uint64_t by_rep, by_groups;               // for pd_div
+    int page_log2;
     float lam;
     void* out;                                // (n, Tq, Hq, d)
     float* lse;                               // (n, Tq, Hq) or null
@@ -154,6 +156,10 @@ __device__ __forceinline__ int pd_exponent(float amax) {
     return amax > 0.f ? min(3 - (e - 127), 126) : 0;
 }
 
+// n / d for by = ceil(2^64 / d), 0 for d = 1.  The kernel's parts run once or twice a call, so what their instructions cost
+// is mostly their number: a division by a variable is 20 and more.
+__device__ __forceinline__ int pd_div(int n, uint64_t by) { return by ? int(__umul64hi(uint64_t(uint32_t(n)), by)) : n; }
+
 template <typename T, int D, int NT>
 __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kernel(const __grid_constant__ PagedDecodeParams A) {
     using S = PdShape<D, NT>;
@@ -233,27 +239,30 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         return false;
     };
 
-    auto row_at = [&](int seq, int h, int r) { return (int64_t(seq) * A.Tq + r / A.rep) * A.Hq + h * A.rep + r % A.rep; };
-    auto store_pair = [&](int seq, int h, int r, int ch, float a, float b, float sum) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row_at(seq, h, r) * D + ch) = pf_pack<T>(a * inv, b * inv);
+    auto row_at = [&](int seq, int h, int r) {
+        const int tok = pd_div(r, A.by_rep);
+        return (int64_t(seq) * A.Tq + tok) * A.Hq + h * A.rep + r - tok * A.rep;
     };
-    auto store_lse = [&](int seq, int h, int r, float top, float sum) {
-        if (A.lse) A.lse[row_at(seq, h, r)] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+    auto store_pair = [&](int64_t row, int ch, float a, float b, float sum) {
+        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pf_pack<T>(a * inv, b * inv);
+    };
+    auto store_lse = [&](int64_t row, float top, float sum) {
+        if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
     };
 
     // the query rows of a piece: lane (g, t) holds row g of 8, channels (D / 4) t ..
     const int g = lane >> 2, t = lane & 3;
     uint4 raw[NT][KS / 2];
     auto load_q = [&](const PdPiece& p) {
-        const int h = p.vh / A.groups, row0 = (p.vh - h * A.groups) * S::ROWS;
+        const int h = pd_div(p.vh, A.by_groups), row0 = (p.vh - h * A.groups) * S::ROWS;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            const int r = row0 + 8 * x + g;
+            const int r = row0 + 8 * x + g, tok = pd_div(r, A.by_rep);
 #pragma unroll
             for (int i = 0; i < KS / 2; ++i) raw[x][i] = uint4{0, 0, 0, 0};
             if (r < A.rep * A.Tq) {
-                const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r % A.rep) * A.Tq + r / A.rep) * D + (D / 4) * t;
+                const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r - tok * A.rep) * A.Tq + tok) * D + (D / 4) * t;
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) raw[x][i] = __ldg(reinterpret_cast<const uint4*>(q + 8 * i));
             }
@@ -275,12 +284,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
         const PdPiece p = pd_piece(W, u0 + warp + k * S::WARPS, u1);
-        const int h = p.vh / A.groups, t0 = p.a * PD_UNIT, len = s_len[p.seq];
-        x.off = t0 % P.page;
+        const int h = pd_div(p.vh, A.by_groups), t0 = p.a * PD_UNIT, len = s_len[p.seq];
+        x.off = t0 & (P.page - 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
-            const int id = P.table[int64_t(s_slot[p.seq]) * P.max_blocks + (t0 + i * box) / P.page];
+            const int id = P.table[int64_t(s_slot[p.seq]) * P.max_blocks + ((t0 + i * box) >> A.page_log2)];
             if (id >= 0 && id < P.n_pages) x.row[i] = id * P.Hkv + h;
             else raise_status(KVB_DEV_BOUNDS);
         }
@@ -321,7 +330,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     {
         int first = 1, unit = 0;
         for (int cur = u0; cur < u1;) {
-            const int h = p.vh / A.groups, row0 = (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
+            const int h = pd_div(p.vh, A.by_groups), row0 = (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
             const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
@@ -363,7 +372,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 for (int k = 0; k < 2; ++k) {
                     lam[x][k] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + k));
                     bias[x][k] = -1152.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + k));
-                    lim[x][k] = len - A.Tq + (row0 + 8 * x + 2 * t + k) / A.rep + 1;
+                    lim[x][k] = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1;
                 }
             }
             float o[NT][KS][4], m[NT][2], l[NT][2];
@@ -561,6 +570,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 const int r = row_of(x);
+                const int64_t row = whole ? row_at(p.seq, h, row0 + r) : 0;
                 float top = -INFINITY, sum = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
@@ -589,14 +599,14 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
                     if (whole) {
-                        if (r < nrows) store_pair(p.seq, h, row0 + r, channel_of(y), acc.x, acc.y, sum);
+                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, sum);
                     } else if (r < nrows) {
                         *reinterpret_cast<float2*>(part + 4 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
                 }
                 if (lane == 0 && r < nrows) {
                     if (whole) {
-                        if (ml == 0) store_lse(p.seq, h, row0 + r, top, sum);
+                        if (ml == 0) store_lse(row, top, sum);
                     } else {
                         part[2 * ml * S::ROWS + r] = top;
                         part[(2 * ml + 1) * S::ROWS + r] = sum;
@@ -675,10 +685,11 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
                         if (row_of(x) >= nrows) continue;
+                        const int64_t row = row_at(p.seq, h, row0 + row_of(x));
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y)
-                            if (!(few && y > 0)) store_pair(p.seq, h, row0 + row_of(x), channel_of(y), acc[x][y].x, acc[x][y].y, sum[x]);
-                        if (lane == 0 && ml == 0) store_lse(p.seq, h, row0 + row_of(x), top[x], sum[x]);
+                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, sum[x]);
+                        if (lane == 0 && ml == 0) store_lse(row, top[x], sum[x]);
                     }
                 }
             }
