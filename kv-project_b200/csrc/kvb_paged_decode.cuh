@@ -640,17 +640,11 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     for (int cc = c0; cc <= c1; cc += 32) {      // 32 partials: a lane has the m and l of one
                         const int cnt = min(32, c1 - cc + 1);
                         const float* mine_p = slot_of(min(cc + lane, c1)) + 2 * ml * S::ROWS;
-                        float f[NT];
+                        float f[NT], lv[NT];                     // f: m until the first loads of O are on their way
 #pragma unroll
                         for (int x = 0; x < NT; ++x) {
-                            const float mv = lane < cnt ? __ldcg(mine_p + row_of(x)) : -INFINITY;
-                            const float lv = lane < cnt ? __ldcg(mine_p + S::ROWS + row_of(x)) : 0.f;
-                            const float to = fmaxf(top[x], warp_max(mv)), ref = to == -INFINITY ? 0.f : to, old = ex2(top[x] - ref);
-                            top[x] = to;
-                            f[x] = ex2(mv - ref);
-                            sum[x] = __fmaf_rn(sum[x], old, kvb::warp_sum(lv * f[x]));
-#pragma unroll
-                            for (int y = 0; y < D / 64; ++y) acc[x][y].x *= old, acc[x][y].y *= old;
+                            f[x] = lane < cnt ? __ldcg(mine_p + row_of(x)) : -INFINITY;
+                            lv[x] = lane < cnt ? __ldcg(mine_p + S::ROWS + row_of(x)) : 0.f;
                         }
                         constexpr int B = 16 / NT;               // partials whose loads are in flight together
 #pragma unroll 1
@@ -668,6 +662,17 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                                         if (k0 + k < cnt && !(few && y > 0))
                                             v[k][x][y] = __ldcg(reinterpret_cast<const float2*>(qk + row_of(x) * D + channel_of(y)));
                                     }
+                            }
+                            if (k0 == 0) {
+#pragma unroll
+                                for (int x = 0; x < NT; ++x) {
+                                    const float to = fmaxf(top[x], warp_max(f[x])), ref = to == -INFINITY ? 0.f : to, old = ex2(top[x] - ref);
+                                    top[x] = to;
+                                    f[x] = ex2(f[x] - ref);
+                                    sum[x] = __fmaf_rn(sum[x], old, kvb::warp_sum(lv[x] * f[x]));
+#pragma unroll
+                                    for (int y = 0; y < D / 64; ++y) acc[x][y].x *= old, acc[x][y].y *= old;
+                                }
                             }
 #pragma unroll
                             for (int k = 0; k < B; ++k)
