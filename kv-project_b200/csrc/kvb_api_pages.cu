@@ -103,7 +103,7 @@ kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t
     if (kvb_status st = check_rows("page_read", p, slots, start, cu, n, k, v, dtype, rows)) return st;
     if (n == 0 || rows == 0) return KVB_OK;
     if (!aligned(k, 16) || !aligned(v, 16)) return fail(KVB_EINVAL, "page_read: k and v need 16-byte alignment");
-    kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {}, {}, {}, {k, v}};
+    kvb::PageRowsParams a{kvbh::view_of(p), slots, start, cu, n, rows, {}, {}, {}, {k, v}, aligned(k, 32) && aligned(v, 32)};
     const dim3 grid(unsigned(rows / p->page + 2 * int64_t(n)),
                     unsigned((2 * int64_t(p->Hkv) * p->page * p->d + kvb::PR_SHARE - 1) / kvb::PR_SHARE));
     const auto kern = dtype == KVB_F32   ? kvb::page_read_kernel<float>

@@ -108,6 +108,7 @@ struct PageRowsParams {
     const void* x[2];              // k, v
     int64_t row_stride[2], head_stride[2];
     void* out[2];                  // read: dense (rows, Hkv, d)
+    int whole;                     // read: out is 32-byte aligned, a thread stores whole sectors
 };
 
 // scale of a page that has `old` and takes rows of magnitude up to a
@@ -298,15 +299,20 @@ __global__ void __launch_bounds__(PW_THREADS) page_read_kernel(const __grid_cons
 #pragma unroll
         for (int k = 0; k < 16; ++k)
             f[k] = (__uint_as_float(__byte_perm(ws[k >> 2], 0x4b000000u, 0x7440 | (k & 3))) - 8388736.f) * s[i];
-        if constexpr (sizeof(T) == 4) {
+        alignas(16) T o[16];
 #pragma unroll
-            for (int k = 0; k < 4; ++k) reinterpret_cast<float4*>(to[i])[k] = float4{f[4 * k], f[4 * k + 1], f[4 * k + 2], f[4 * k + 3]};
+        for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(f[k]);
+        const uint32_t* u = reinterpret_cast<const uint32_t*>(o);
+        constexpr int WORDS = sizeof(T) * 4;
+        if (A.whole) {
+#pragma unroll
+            for (int k = 0; k < WORDS; k += 8)
+                asm volatile("st.global.v8.b32 [%8], {%0, %1, %2, %3, %4, %5, %6, %7};" ::"r"(u[k]), "r"(u[k + 1]), "r"(u[k + 2]), "r"(u[k + 3]),
+                             "r"(u[k + 4]), "r"(u[k + 5]), "r"(u[k + 6]), "r"(u[k + 7]), "l"(reinterpret_cast<uint32_t*>(to[i]) + k)
+                             : "memory");
         } else {
-            T o[16];
 #pragma unroll
-            for (int k = 0; k < 16; ++k) o[k] = from_f32<T>(f[k]);
-            reinterpret_cast<uint4*>(to[i])[0] = reinterpret_cast<const uint4*>(o)[0];
-            reinterpret_cast<uint4*>(to[i])[1] = reinterpret_cast<const uint4*>(o)[1];
+            for (int k = 0; k < WORDS; k += 4) reinterpret_cast<uint4*>(to[i])[k / 4] = uint4{u[k], u[k + 1], u[k + 2], u[k + 3]};
         }
     }
 }
