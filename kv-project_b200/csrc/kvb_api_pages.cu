@@ -186,7 +186,7 @@ kvb_status kvb_page_compact(const kvb_pages* p, int n_pools, int32_t* n_live, vo
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     if (kvb_status st = launch_chained("page_compact plan", kvb::compact_plan_kernel, 1, page_block(p), 0, s, v, w)) return st;
     for (int i = 0; i < n_pools; ++i)
-        if (kvb_status st = launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 4, kvb::PG_COPY_THREADS, 0, s,
+        if (kvb_status st = launch_chained("page_compact move", kvb::compact_move_kernel, 148 * 16, kvb::PG_COPY_THREADS, 0, s,
                                            kvbh::view_of(p + i), w, n_live, i + 1 == n_pools))
             return st;
     return KVB_OK;

@@ -18,7 +18,9 @@ struct PagesView {
     int Hkv, d, page, n_slots, max_blocks;
 };
 
-__device__ __forceinline__ int blocks_of(int n, int page) { return (n + page - 1) / page; }
+// pages are 16, 32, 64 or 128 tokens: a shift instead of the 20 and more instructions of a division
+__device__ __forceinline__ int page_shift(int page) { return 31 - __clz(page); }
+__device__ __forceinline__ int blocks_of(int n, int page) { return (n + page - 1) >> page_shift(page); }
 
 template <typename T>
 __device__ __forceinline__ T from_f32(float v);
