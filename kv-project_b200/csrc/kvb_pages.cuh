@@ -172,8 +172,9 @@ __device__ __forceinline__ float2 pair_f32<__nv_bfloat16>(uint32_t w) {
 // 16-bit rows on 16-byte strides: a thread holds 8 values of up to ROUNDS rounds in registers, so the rows are read
 // once.  The maximum is taken on the magnitudes' bits, two a word (they order like the values), which also shows whether
 // a value is not finite; without one, rint(x inv) + 128 is the low byte of x inv + (1.5 2^23 + 128), as |x inv| <= 127 up to
-// the roundings of s and 1 / s.  Bound by the bytes; many small blocks keep enough loads in flight.  16384 tokens, 8 heads,
-// d 128 (67 MB read, 34 MB written), and read back: 41.4 us, 4.9 TB/s.
+// the roundings of s and 1 / s.  Bound by the bytes; many small blocks keep enough loads in flight (blocks of 256: 42.6 us
+// below), and rows read with the streaming hint leave the codes in the L2 (38.0 without).  16384 tokens, 8 heads,
+// d 128 (67 MB read, 34 MB written), and read back: 36.7 us, 5.5 TB/s.
 template <typename T, int ROUNDS>
 __global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_constant__ PageRowsParams A) {
     chain_kernels();
@@ -190,7 +191,7 @@ __global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_con
 #pragma unroll
     for (int i = 0; i < ROUNDS; ++i) {
         const int r = r0 + i * step;
-        raw[i] = r < t.rows ? __ldg(reinterpret_cast<const uint4*>(x + r * A.row_stride[side])) : uint4{0, 0, 0, 0};
+        raw[i] = r < t.rows ? __ldcs(reinterpret_cast<const uint4*>(x + r * A.row_stride[side])) : uint4{0, 0, 0, 0};
     }
     const int64_t page = touch_page(P, t);
     if (page < 0) return;
@@ -264,7 +265,7 @@ __global__ void __launch_bounds__(PW_THREADS) page_write_kernel(const __grid_con
 // The codes of a touched page (both sides, all heads) in shares of 8192, one to a block: a thread takes 16 codes in each of
 // 4 rounds, its loads in flight together.  A byte b becomes the float32 pattern 0x4b000000 | b = 2^23 + b, less 2^23 +
 // 128: exact.  Bound by the bytes; a block per head and side took 47 us where pages are small (16 x 64, 20600 rows of 4
-// heads), these 14.  grid (touch slots, ceil(2 Hkv page d / 8192))
+// heads), 14 with stores of 16 bytes, these 11.  grid (touch slots, ceil(2 Hkv page d / 8192))
 constexpr int PR_SHARE = 8192;
 
 template <typename T>
