@@ -42,8 +42,8 @@ kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
     // without pieces no more CTAs than items (at most so many) have work
     const int64_t items = a.part ? kMaxCtas : a.Hkv * (a.nq / (2 * a.tt) + a.n);
     const int ctas = std::min(resolve_ctas(0), kMaxCtas);
-    // Launched plainly: placed early by programmatic serialization, a replayed graph of such calls ended in an illegal
-    // access (the kernel fills an SM's registers and tensor memory), and a launch's 2 us is little beside its work.
+    // Launched plainly: the kernel fills an SM, so that placing it early (programmatic serialization) saves the launch's 1 to 2
+    // us only, and it is kept out of what a captured graph may overlap.
     kern<<<unsigned(std::min<int64_t>(items, ctas)), kvb::PF_THREADS, SM, s>>>(a);
     return launch_check("prefill_attention");
 }

@@ -21,12 +21,14 @@
 // what the chain costs beside the products bounds the kernel.  So: the weights are computed with the reference maximum
 // so far while the new maximum is taken (the tile is redone in the rare case that it grew too far); P is handed over
 // in two parts, 96 columns and 32, and the first part's product runs while the second is computed; and the MMA warp
-// runs converged.  16384 tokens, 32 heads over 8, d 128: 2102 us without these three, 1885 with the converged warp, 1799
-// with the early weights and P in halves, 1728 with the masked tiles known ahead, 1649 with P in 96 + 32 and 224
-// registers (1334 TFLOP/s).  Measured and left: two threads a row (1971), steps of 64 keys with two score buffers (1894), an MMA warp
-// per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906), growth seen from the sum of the
-// weights instead of the maximum (no difference).  At 8192 tokens (463 us, 1187 TFLOP/s at the 1.63 GHz that the power cap leaves)
-// the tensor pipe is busy 64 % of the time and the special function unit 64 %.
+// runs converged.  Each of these took 3 to 10 % off (16384 tokens, 32 heads over 8, d 128: 2102 us without any).  All roles
+// run with the 168 registers that ten warps leave a thread, and a step with 128 logits, 64 weights and their sums wants
+// more: the last 32 logits are read twice, first for the maximum only (1983 us; 2068 with spills; 8 packed prompts of 7208
+// tokens 150 and 162).  Registers moved between the roles (setmaxnreg, 224 and 56) took 1876 and 135, but one of some
+// 45000 calls, and replayed graphs sooner, ended in an illegal access that nothing else in the kernel explains: not used.
+// Measured and left (some with those registers): two threads a row (1971), steps of 64 keys with two score buffers (1894), an
+// MMA warp per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906), growth seen from the sum
+// of the weights instead of the maximum (no difference).
 //
 // Masks: logits of keys past a row's limit become -inf by selection, so what lies there does not matter; values
 // there would still meet a weight of zero in the MMA (0 * NaN), so in tiles that some row of the item does not see
@@ -56,9 +58,7 @@
 namespace kvb {
 
 constexpr int PF_KT = 128;                    // keys per tile
-constexpr int PF_THREADS = 384;               // warps 10 and 11 only give up their registers
-// registers of a thread in the softmax warpgroups and in the third: 2 x 128 x 224 + 128 x 56 = 384 x 168, the launch's
-constexpr int PF_REGS_SOFTMAX = 224, PF_REGS_REST = 56;
+constexpr int PF_THREADS = 320;
 constexpr int PF_TMEM_COLS = 512;
 constexpr float PF_LAZY = 8.f;                // log2 of how far a maximum may grow before O is rescaled
 
@@ -244,7 +244,8 @@ __device__ __forceinline__ void pf_weights(const uint32_t* v, uint64_t lam, uint
 template <typename T>
 __device__ __forceinline__ bool pf_not_finite(const uint4& w) {
     using T2 = typename std::conditional<std::is_same<T, __half>::value, __half2, __nv_bfloat162>::type;
-    const T2 z = *reinterpret_cast<const T2*>("\0\0\0");
+    const uint32_t zero = 0;
+    const T2 z = *reinterpret_cast<const T2*>(&zero);
     const uint32_t a[4] = {w.x, w.y, w.z, w.w};
     T2 s = z;
 #pragma unroll
@@ -547,8 +548,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         return false;
     };
 
-    if (warp >= 8) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PF_REGS_REST));
     if (warp == 8) {
         // ---------------- schedule and loads ----------------
         uint32_t it = 0, items = 0;
@@ -593,6 +592,10 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             }
             ok = __shfl_sync(0xffffffffu, int(ok), 0);
         }
+        // the MMAs' last arrivals are in before the CTA may leave
+        for (uint32_t k = it > uint32_t(S::STAGES) ? it - S::STAGES : 0; ok && lane == 0 && k < it; ++k)
+            ok = wait(&sh.kv_empty[k % S::STAGES], k / S::STAGES);
+        if (ok && lane == 0 && items > 0) wait(&sh.q_empty, items - 1);
     } else if (warp == 9) {
         // ---------------- MMA issue ----------------
         constexpr uint32_t IDESC_S = pf_idesc(PF_KT, BF16, 0), IDESC_O = pf_idesc(D, BF16, 1);
@@ -674,9 +677,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
         if (*abort)
             for (int w = 0; w < 2; ++w)
                 if (pv[w] > 0) mbar_wait(&sh.o_full[w], (pv[w] - 1) & 1, 10000000ull);
-    }
     } else {
-        asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PF_REGS_SOFTMAX));
         // ---------------- softmax: warpgroup w, thread = row ----------------
         const int w = warp >> 2, row = threadIdx.x & 127;
         const uint32_t lanes = tmem + (uint32_t((warp & 3) * 32) << 16);
@@ -699,47 +700,61 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
             for (int j = 0; j < n; ++j, ++steps) {
                 if (!(ok = all(wait(&sh.s_full[w], steps)))) break;
                 tc_fence_after();
-                uint32_t r[PF_KT];
-#pragma unroll
-                for (int c = 0; c < PF_KT; c += 32) pf_ld32(s_col + c, r + c);
-                pf_wait_ld();
+                // The logits take 96 registers: of the last 32 only the maximum is kept, they are read again below.
+                uint32_t r[PF_KT - 32], p[32];
                 float* v = reinterpret_cast<float*>(r);
-                if (A.negate) {
-#pragma unroll
-                    for (int i = 0; i < PF_KT; ++i) v[i] = -v[i];
-                }
-                // The first 64 weights are computed with the reference so far while the maximum is taken: it serves unless
-                // a row's maximum grew by 2^8, has not begun, or is not finite.
                 const int lim = limit - (j0 + j) * PF_KT;
                 const bool masked = j >= jmask;
-                uint32_t p[32];
+                auto logits = [&](uint32_t* x, int c0, int n) {  // the sign of the scaling, and the mask
+                    if (A.negate) {
+#pragma unroll
+                        for (int i = 0; i < n; ++i) x[i] ^= 0x80000000u;
+                    }
+                    if (masked) {
+#pragma unroll
+                        for (int i = 0; i < n; ++i) x[i] = c0 + i < lim ? x[i] : 0xff800000u;
+                    }
+                };
+                pf_ld32(s_col + PF_KT - 32, p);
+#pragma unroll
+                for (int c = 0; c < PF_KT - 32; c += 32) pf_ld32(s_col + c, r + c);
+                pf_wait_ld();
+                logits(p, PF_KT - 32, 32);
+                float last[2] = {__uint_as_float(p[0]), __uint_as_float(p[1])};
+#pragma unroll
+                for (int i = 2; i < 32; i += 2) last[i / 2 & 1] = pf_max3_nan(last[i / 2 & 1], __uint_as_float(p[i]), __uint_as_float(p[i + 1]));
+                logits(r, 0, PF_KT - 32);
+                // The first 64 weights are computed with the reference so far while the maximum is taken: it serves unless
+                // a row's maximum grew by 2^8, has not begun, or is not finite.
                 uint64_t sum[2] = {0, 0};
-                auto weights = [&](int c) {                      // of the columns c .. c + 31, into half of p
+                auto weights = [&](const uint32_t* x, uint32_t* to) {                // of 32 logits
                     const float ref = m == -INFINITY ? 0.f : m;
-                    pf_weights<T>(r + c, pf_two(A.lam, A.lam), pf_two(-ref, -ref), p + (c & 32) / 2, sum);
+                    pf_weights<T>(x, pf_two(A.lam, A.lam), pf_two(-ref, -ref), to, sum);
                 };
                 auto maximum = [&]() {
-                    float mx[4] = {v[0], v[1], v[2], v[3]};
+                    float mx[4] = {last[0], last[1], v[0], v[1]};
 #pragma unroll
-                    for (int i = 4; i < PF_KT - 4; i += 8)
+                    for (int i = 2; i < PF_KT - 34; i += 8)
 #pragma unroll
-                        for (int k = 0; k < 4; ++k) mx[k] = pf_max3_nan(mx[k], v[i + k], v[i + 4 + k]);
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) mx[k] = pf_max3_nan(mx[k], mx[k], v[PF_KT - 4 + k]);
+                        for (int k = 0; k < 4; ++k)
+                            if (i + 4 + k < PF_KT - 32) mx[k] = pf_max3_nan(mx[k], v[i + k], v[i + 4 + k]);
+                            else if (i + k < PF_KT - 32) mx[k] = pf_max3_nan(mx[k], v[i + k], v[i + k]);
                     return pf_max3_nan(pf_max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * A.lam;
                 };
                 bool fast = j > 0 && !masked;
                 if (fast) {
-                    weights(0);
-                    weights(32);
+                    weights(r, p);
+                    weights(r + 32, p + 16);
                     const float top = maximum();
                     fast = !__any_sync(0xffffffffu, valid && !(top <= m + PF_LAZY && m > -INFINITY));
+                    if (!fast) {                                 // the weights took the logits' registers
+                        pf_ld32(s_col, r);
+                        pf_ld32(s_col + 32, r + 32);
+                        pf_wait_ld();
+                        logits(r, 0, 64);
+                    }
                 }
                 if (!fast) {
-                    if (masked) {
-#pragma unroll
-                        for (int i = 0; i < PF_KT; ++i) v[i] = i < lim ? v[i] : -INFINITY;
-                    }
                     const float top = maximum();
                     // a row that has seen nothing takes its first maximum as it is; O is zero until then.  NaN and +inf
                     // make the row NaN, as they do in the formula.
@@ -756,18 +771,17 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                             tc_fence_after();
 #pragma unroll 1
                             for (int c = 0; c < D; c += 32) {
-                                uint32_t o[32];
-                                pf_ld32(o_col + c, o);
+                                pf_ld32(o_col + c, p);
                                 pf_wait_ld();
 #pragma unroll
-                                for (int i = 0; i < 32; ++i) o[i] = __float_as_uint(__uint_as_float(o[i]) * f);
-                                pf_st32(o_col + c, o);
+                                for (int i = 0; i < 32; ++i) p[i] = __float_as_uint(__uint_as_float(p[i]) * f);
+                                pf_st32(o_col + c, p);
                             }
                         }
                     }
                     sum[0] = sum[1] = 0;
-                    weights(0);
-                    weights(32);
+                    weights(r, p);
+                    weights(r + 32, p + 16);
                 }
                 pf_st32(s_col, p);
                 if (j >= jm) {
@@ -796,13 +810,16 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                     }
                     fence_proxy_async_smem();
                 }
-                weights(64);
+                weights(r + 64, p);
                 pf_st16(s_col + 32, p);
                 pf_wait_st();
                 tc_fence_before();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&sh.p_most[w]);
-                weights(96);
+                pf_ld32(s_col + PF_KT - 32, r);
+                pf_wait_ld();
+                logits(r, PF_KT - 32, 32);
+                weights(r, p + 16);
                 pf_st16(s_col + 48, p + 16);
                 const float2 s0 = pf_split(sum[0]), s1 = pf_split(sum[1]);
                 l += (s0.x + s0.y) + (s1.x + s1.y);
@@ -847,6 +864,7 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
 #pragma unroll 1
             for (int c = 0; c < (used ? D : 0); c += 32) {
                 uint32_t o[32];
+                __syncwarp();                                    // after the stores of some lanes
                 if (n > 0) {
                     pf_ld32(o_col + c, o);
                     pf_wait_ld();
