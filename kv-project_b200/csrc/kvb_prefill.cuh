@@ -724,8 +724,6 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
 #pragma unroll
                 for (int i = 2; i < 32; i += 2) last[i / 2 & 1] = pf_max3_nan(last[i / 2 & 1], __uint_as_float(p[i]), __uint_as_float(p[i + 1]));
                 logits(r, 0, PF_KT - 32);
-                // The first 64 weights are computed with the reference so far while the maximum is taken: it serves unless
-                // a row's maximum grew by 2^8, has not begun, or is not finite.
                 uint64_t sum[2] = {0, 0};
                 auto weights = [&](const uint32_t* x, uint32_t* to) {                // of 32 logits
                     const float ref = m == -INFINITY ? 0.f : m;
@@ -741,21 +739,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                             else if (i + k < PF_KT - 32) mx[k] = pf_max3_nan(mx[k], v[i + k], v[i + k]);
                     return pf_max3_nan(pf_max3_nan(mx[0], mx[1], mx[2]), mx[3], mx[3]) * A.lam;
                 };
-                bool fast = j > 0 && !masked;
-                if (fast) {
-                    weights(r, p);
-                    weights(r + 32, p + 16);
-                    const float top = maximum();
-                    fast = !__any_sync(0xffffffffu, valid && !(top <= m + PF_LAZY && m > -INFINITY));
-                    if (!fast) {                                 // the weights took the logits' registers
-                        pf_ld32(s_col, r);
-                        pf_ld32(s_col + 32, r + 32);
-                        pf_wait_ld();
-                        logits(r, 0, 64);
-                    }
-                }
-                if (!fast) {
-                    const float top = maximum();
+                // the reference so far serves unless a row's maximum grew by 2^8, has not begun, or is not finite
+                const float top = maximum();
+                if (__any_sync(0xffffffffu, valid && !(top <= m + PF_LAZY && m > -INFINITY))) {
                     // a row that has seen nothing takes its first maximum as it is; O is zero until then.  NaN and +inf
                     // make the row NaN, as they do in the formula.
                     const bool odd = !(top < INFINITY), grow = valid && (top > m + PF_LAZY || odd) && m > -INFINITY;
@@ -779,10 +765,9 @@ __global__ void __launch_bounds__(PF_THREADS, 1) prefill_kernel(const __grid_con
                             }
                         }
                     }
-                    sum[0] = sum[1] = 0;
-                    weights(r, p);
-                    weights(r + 32, p + 16);
                 }
+                weights(r, p);
+                weights(r + 32, p + 16);
                 pf_st32(s_col, p);
                 if (j >= jm) {
                     // value rows that some row of the item does not see: see the head of this file
