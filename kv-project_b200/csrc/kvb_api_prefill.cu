@@ -43,7 +43,7 @@ kvb_status launch(const kvb::PrefillParams& a, cudaStream_t s) {
     const int64_t items = a.part ? kMaxCtas : a.Hkv * (a.nq / (2 * a.tt) + a.n);
     const int ctas = std::min(resolve_ctas(0), kMaxCtas);
     // Launched plainly: the kernel fills an SM, so that placing it early (programmatic serialization) saves the launch's 1 to 2
-    // us only, and it is kept out of what a captured graph may overlap.
+    // us only.
     kern<<<unsigned(std::min<int64_t>(items, ctas)), kvb::PF_THREADS, SM, s>>>(a);
     return launch_check("prefill_attention");
 }
@@ -76,6 +76,10 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
     if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "prefill_attention: scaling must be finite");
     if (workspace && (workspace_bytes < kvb_prefill_workspace(d) || !aligned(workspace, 256)))
         return fail(KVB_EINVAL, "prefill_attention: workspace of %zu bytes, 256-byte aligned (or none)", kvb_prefill_workspace(d));
+    cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+    if (kvb_status st = kvbh::cuda_check(cudaStreamIsCapturing(static_cast<cudaStream_t>(stream), &capture), "prefill_attention")) return st;
+    if (capture != cudaStreamCaptureStatusNone)      // see the head of kvb_prefill.cuh
+        return fail(KVB_EUNSUPPORTED, "prefill_attention: not in a stream capture");
     kvb::PrefillParams a{};
     a.count = static_cast<uint32_t*>(workspace);
     a.part = workspace ? reinterpret_cast<float*>(static_cast<char*>(workspace) + kCountBytes) : nullptr;

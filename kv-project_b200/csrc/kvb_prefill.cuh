@@ -18,14 +18,20 @@
 // float32), which is seldom after the first tiles.
 //
 // A tile's step is a chain (logits from the tensor cores, weights, the two products), the other tile's fills its gaps, and
-// what the chain costs beside the products bounds the kernel.  So: the weights are computed with the reference maximum
-// so far while the new maximum is taken (the tile is redone in the rare case that it grew too far); P is handed over
+// what the chain costs beside the products bounds the kernel.  So: P is handed over
 // in two parts, 96 columns and 32, and the first part's product runs while the second is computed; and the MMA warp
-// runs converged.  Each of these took 3 to 10 % off (16384 tokens, 32 heads over 8, d 128: 2102 us without any).  All roles
+// runs converged.  16384 tokens, 32 heads over 8, d 128: 2102 us without any.  All roles
 // run with the 168 registers that ten warps leave a thread, and a step with 128 logits, 64 weights and their sums wants
-// more: the last 32 logits are read twice, first for the maximum only (1983 us; 2068 with spills; 8 packed prompts of 7208
-// tokens 150 and 162).  Registers moved between the roles (setmaxnreg, 224 and 56) took 1876 and 135, but one of some
-// 45000 calls, and replayed graphs sooner, ended in an illegal access that nothing else in the kernel explains: not used.
+// more: the last 32 logits are read twice, first for the maximum only (1915 us, 8 packed prompts of 7208 tokens 139; 2068 and
+// 162 with spills; weights computed ahead of the maximum, which has to be redone where it grew, 1983 and 150).
+// Registers moved between the roles (setmaxnreg, 224 and 56) took 1876 and 135, but
+// one of some 45000 calls ended in an illegal access, none of 150000 without.
+//
+// Replayed graphs of ten calls on many items have ended in an illegal access too, with and without those registers and
+// programmatic launches, seldom and never in the first replay; a kernel that checked its own addresses ended the same way,
+// and reading shows every access in bounds and every copy, product and arrival waited for.  Until the cause is known the
+// call refuses a stream that is being captured.
+//
 // Measured and left (some with those registers): two threads a row (1971), steps of 64 keys with two score buffers (1894), an
 // MMA warp per tile (1929), an eighth to a half of the exponentials as polynomials (1838 to 1906), growth seen from the sum
 // of the weights instead of the maximum (no difference).

@@ -35,6 +35,12 @@ def _check_ints(who: str, n: int, *ts):
             raise ValueError(f"{who}: slots, starts, counts and offsets must be contiguous int32 CUDA tensors of {n} entries")
 
 
+def _not_capturing(who: str):
+    """A workspace's zeros would only be written when the graph is replayed."""
+    if torch.cuda.is_current_stream_capturing():
+        raise NotImplementedError(f"{who}: the first call on a stream makes a workspace, which a stream capture cannot")
+
+
 _PREFILL_WS = {}
 _UNSPLIT_KEYS = 896
 
@@ -43,6 +49,7 @@ def _prefill_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
     """The zero-filled workspace of one stream (40 MB), made at the first call that may need it."""
     ws = _PREFILL_WS.get((device.index, stream, d))
     if ws is None:
+        _not_capturing("prefill_attention")
         ws = _PREFILL_WS[(device.index, stream, d)] = torch.zeros(lib.kvb_prefill_workspace(d), dtype=torch.uint8, device=device)
     return ws
 
@@ -142,6 +149,7 @@ class PagePool:
         """A zero-filled buffer for one kind of call on one stream, kept while it is large enough."""
         ws = self._ws.get((kind, stream))
         if ws is None or ws.numel() < size:
+            _not_capturing(kind)
             ws = self._ws[(kind, stream)] = torch.zeros(max(size, 256), dtype=torch.uint8, device=self.device)
         return ws
 
