@@ -476,7 +476,8 @@ kvb_status kvb_operational_rd(const float* A, int64_t rows, int64_t n, int64_t l
  * aligned; lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written.
  * workspace (kvb_prefill_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
  * (every call leaves its counters at zero), one per stream that runs calls concurrently; with it the work of
- * long rows is split over the keys, without it (null) every query tile is computed in one piece. */
+ * long rows is split over the keys, without it (null) every query tile is computed in one piece.  A stream that is being
+ * captured is refused (KVB_EUNSUPPORTED). */
 size_t kvb_prefill_workspace(int d);
 kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq,
                                  int Hkv, int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,

@@ -14,7 +14,7 @@
 // memory; a run that is only a part of a (sequence, head, group) leaves a partial, and the CTA that completes the last
 // part joins the partials in the order of the tokens (each warp its rows), so the result does not depend on timing.
 //
-// A step of 8 sequences of 32768 tokens, 8 heads, d 128 (537 MB), with the write of its rows: 99.8 us, 5.4 TB/s; about 7
+// A step of 8 sequences of 32768 tokens, 8 heads, d 128 (537 MB), with the write of its rows: 97.5 us, 5.5 TB/s; about 7
 // TB/s at the margin, the rest is the start (4 us), the first copies' latency and the join (the same step without any
 // arithmetic took 97 us when it took 103 with).  At 8 x 16384 (269 MB, all of the DRAM traffic): ALU pipe 39 % busy (the
 // codes' permutes), tensor pipe 17 %, issue slots 38 %, no shared-memory bank conflicts.

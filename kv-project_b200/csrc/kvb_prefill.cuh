@@ -18,14 +18,13 @@
 // float32), which is seldom after the first tiles.
 //
 // A tile's step is a chain (logits from the tensor cores, weights, the two products), the other tile's fills its gaps, and
-// what the chain costs beside the products bounds the kernel.  So: P is handed over
-// in two parts, 96 columns and 32, and the first part's product runs while the second is computed; and the MMA warp
-// runs converged.  16384 tokens, 32 heads over 8, d 128: 2102 us without any.  All roles
-// run with the 168 registers that ten warps leave a thread, and a step with 128 logits, 64 weights and their sums wants
-// more: the last 32 logits are read twice, first for the maximum only (1915 us, 8 packed prompts of 7208 tokens 139; 2068 and
-// 162 with spills; weights computed ahead of the maximum, which has to be redone where it grew, 1983 and 150).
-// Registers moved between the roles (setmaxnreg, 224 and 56) took 1876 and 135, but
-// one of some 45000 calls ended in an illegal access, none of 150000 without.
+// what the chain costs beside the products bounds the kernel.  So P is handed over in two parts, 96 columns and 32, and the
+// first part's product runs while the second is computed; and the MMA warp runs converged (16384 tokens, 32 heads over 8,
+// d 128: 2102 us without either).  All roles run with the 168 registers that ten warps leave a thread, and a step with 128
+// logits, their weights and sums wants more: the last 32 logits are read twice, first for the maximum only (1915 us, 8
+// packed prompts of 7208 tokens 139; 2068 and 162 with spills; weights computed ahead of the maximum, which has to be redone
+// where it grew, 1983 and 150).  Registers moved between the roles (setmaxnreg, 224 and 56) took 1876 and 135, but one of
+// some 45000 calls ended in an illegal access, none of 150000 without.
 //
 // Replayed graphs of ten calls on many items have ended in an illegal access too, with and without those registers and
 // programmatic launches, seldom and never in the first replay; a kernel that checked its own addresses ended the same way,
