@@ -35,7 +35,6 @@
 
 #include "kvb_common.cuh"
 #include "kvb_pages_view.cuh"
-#include "kvb_prefill.cuh"
 
 namespace kvb {
 
@@ -124,6 +123,14 @@ __device__ __forceinline__ PdPiece pd_piece(const PdPlan& W, int cur, int end) {
     p.b = min(p.units, p.a + (end - cur));
     p.v0 = (W.pre[lo] + lo * PD_FIXED) * W.hg + p.vh * (p.units + PD_FIXED);
     return p;
+}
+
+__device__ __forceinline__ void tma_load_3d(void* dst, const CUtensorMap* map, int x, int y, int z, uint64_t* bar) {
+    asm volatile(
+        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(
+            smem_u32(dst)),
+        "l"(map), "r"(x), "r"(y), "r"(z), "r"(smem_u32(bar))
+        : "memory");
 }
 
 __device__ __forceinline__ uint32_t pd_prmt(uint32_t a, uint32_t b, uint32_t sel) { return __byte_perm(a, b, sel); }
@@ -245,7 +252,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     };
     auto store_pair = [&](int64_t row, int ch, float a, float b, float sum) {
         const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pf_pack<T>(a * inv, b * inv);
+        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a * inv, b * inv);
     };
     auto store_lse = [&](int64_t row, float top, float sum) {
         if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);

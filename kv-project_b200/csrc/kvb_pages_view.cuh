@@ -1,4 +1,4 @@
-// kvb_pages_view.cuh - the 8-bit paged cache as kernels see it, and the rounding to an output type.
+// kvb_pages_view.cuh - the 8-bit paged cache as kernels see it, and the rounding to 16-bit types.
 #pragma once
 
 #include "kvb_common.cuh"
@@ -30,5 +30,16 @@ template <>
 __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+
+// two values of a 16-bit type in a word, the first in its low half
+template <typename T>
+__device__ __forceinline__ uint32_t pack_f32(float lo, float hi);
+template <>
+__device__ __forceinline__ uint32_t pack_f32<__half>(float lo, float hi) { return pack_half2(lo, hi); }
+template <>
+__device__ __forceinline__ uint32_t pack_f32<__nv_bfloat16>(float lo, float hi) {
+    __nv_bfloat162 h = __floats2bfloat162_rn(lo, hi);
+    return *reinterpret_cast<uint32_t*>(&h);
+}
 
 }  // namespace kvb
