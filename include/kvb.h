@@ -524,8 +524,8 @@ kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t
                          void* v, int dtype, int64_t rows, void* stream);
 
 /* Attention of the last Tq positions of each sequence over its pages: q (n, Hq, Tq, d) dense (f16 / bf16), query
- * t of sequence slots[i] sees the keys j <= lens - Tq + t.  out (n, Tq, Hq, d) in q's dtype; lse (n, Tq, Hq)
- * float32 or null.  A row that sees no key gives zeros and -inf.  workspace: 256-byte aligned, zero-filled once
+ * t of sequence slots[i] sees the keys j <= lens - Tq + t.  out (n, Tq, Hq, d) in q's dtype, 4-byte aligned; lse (n, Tq,
+ * Hq) float32, 4-byte aligned, or null.  A row that sees no key gives zeros and -inf.  workspace: 256-byte aligned, zero-filled once
  * before its first use and then reused (every call leaves its counters at zero), one per stream that runs
  * calls concurrently. */
 size_t kvb_page_attend_workspace(const kvb_pages* p, int n, int Hq, int Tq);

@@ -86,7 +86,8 @@ kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq,
     if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "page_attend: scaling must be finite");
     if (p->n_pages * p->Hkv > INT32_MAX) return fail(KVB_EINVAL, "page_attend: n_pages * Hkv < 2^31");
     if (n == 0) return KVB_OK;
-    if (!aligned(q, 16)) return fail(KVB_EINVAL, "page_attend: q needs 16-byte alignment");
+    if (!aligned(q, 16) || !aligned(out, 4) || !aligned(lse, 4))
+        return fail(KVB_EINVAL, "page_attend: q needs 16-byte alignment, out and lse 4-byte");
     if (workspace_bytes < kvb_page_attend_workspace(p, n, Hq, Tq) || !aligned(workspace, 256))
         return fail(KVB_EINVAL, "page_attend: workspace of %zu bytes, 256-byte aligned", kvb_page_attend_workspace(p, n, Hq, Tq));
     kvb::PagedDecodeParams a{};

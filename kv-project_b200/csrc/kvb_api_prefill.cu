@@ -52,8 +52,8 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
     if (!q || (!k && nk) || (!v && nk) || !cu_q || !cu_k || !out) return fail(KVB_EINVAL, "prefill_attention: null argument");
     for (int64_t st : {q_row, q_head, k_row, k_head, v_row, v_head})
         if (st < 0 || st % 8 != 0) return fail(KVB_EINVAL, "prefill_attention: row and head strides multiples of 8 elements");
-    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 32))
-        return fail(KVB_EINVAL, "prefill_attention: q, k and v need 16-byte alignment, out 32-byte");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 32) || !aligned(lse, 4))
+        return fail(KVB_EINVAL, "prefill_attention: q, k and v need 16-byte alignment, out 32-byte, lse 4-byte");
     if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "prefill_attention: scaling must be finite");
     if (workspace && (workspace_bytes < kvb_prefill_workspace(d) || !aligned(workspace, 256)))
         return fail(KVB_EINVAL, "prefill_attention: workspace of %zu bytes, 256-byte aligned (or none)", kvb_prefill_workspace(d));

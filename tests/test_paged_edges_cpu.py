@@ -1,0 +1,31 @@
+"""What the paged path refuses on the host, beside the descriptors and sizes: addresses and devices."""
+
+import ctypes as C
+
+import pytest
+
+A, B = 4096, 1 << 30        # stand-ins for aligned device addresses: never read
+
+
+def pages(**kw):
+    from kvb import _lib
+    f = dict(kc=A, vc=A, ks=A, vs=A, table=A, lens=A, refs=A, n_pages=10, Hkv=2, d=128, page=64, n_slots=4, max_blocks=8)
+    f.update(kw)
+    return _lib.Pages(*[f[n] for n, _ in _lib.Pages._fields_])
+
+
+@pytest.mark.parametrize("out,lse", [(A + 1, None), (A + 2, None), (A, A + 2), (A, A + 1)])
+def test_attend_refuses_outputs_off_their_words(out, lse):
+    """Outputs are stored two 16-bit values at a time, the log-sum-exp as float32."""
+    from kvb import _lib
+    lib = _lib.lib()
+    st = lib.kvb_page_attend(C.byref(pages()), A, 1, 4, 1, A, 1, 0.1, out, lse, A, B, None)
+    assert st == 1 and "alignment" in lib.kvb_last_error().decode()
+
+
+@pytest.mark.parametrize("lse", [A + 1, A + 2])
+def test_prefill_refuses_a_log_sum_exp_off_its_words(lse):
+    from kvb import _lib
+    lib = _lib.lib()
+    st = lib.kvb_prefill_attention(A, A, A, 2, 10, 10, 4, 2, 128, 512, 128, 256, 128, 256, 128, A, A, 1, 0.1, A, lse, None, 0, None)
+    assert st == 1 and "alignment" in lib.kvb_last_error().decode()
