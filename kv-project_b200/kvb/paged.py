@@ -28,11 +28,19 @@ _new = torch.empty_strided
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
 
 
-def _check_ints(who: str, n: int, *ts):
-    """int32, contiguous, one-dimensional CUDA tensors of n entries."""
+def _check_on(who: str, index: int, *ts):
+    """Tensors of CUDA device `index`: an address of the host or of another device would be read or written as one of this."""
     for t in ts:
-        if t.dtype is not _I32 or t.shape != (n,) or not t.is_cuda or not t.is_contiguous():
-            raise ValueError(f"{who}: slots, starts, counts and offsets must be contiguous int32 CUDA tensors of {n} entries")
+        if t.get_device() != index:
+            raise ValueError(f"{who}: every tensor must live on CUDA device {index}")
+
+
+def _check_ints(who: str, n: int, index: int, *ts):
+    """int32, contiguous, one-dimensional tensors of n entries on CUDA device `index`."""
+    for t in ts:
+        if t.dtype is not _I32 or t.shape != (n,) or t.get_device() != index or not t.is_contiguous():
+            raise ValueError(f"{who}: slots, starts, counts and offsets must be contiguous int32 tensors of {n} entries on "
+                             f"CUDA device {index}")
 
 
 def _not_capturing(who: str):
@@ -66,8 +74,10 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
         cu_k = cu_q
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
         raise ValueError("prefill_attention: q (Nq, Hq, d), k and v (Nk, Hkv, d)")
-    if not (q.is_cuda and k.is_cuda and v.is_cuda):
+    if not q.is_cuda:
         raise ValueError("kvb: tensors must live on a CUDA device")
+    index = q.get_device()
+    _check_on("prefill_attention", index, k, v)
     if not (q.dtype == k.dtype == v.dtype):
         raise ValueError("prefill_attention: q, k and v of one dtype")
     nq, hq, d = q.shape
@@ -75,17 +85,17 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
     if n < 0:
         raise ValueError("prefill_attention: cu_q and cu_k hold n + 1 offsets each")
-    _check_ints("prefill_attention", n + 1, cu_q, cu_k)
+    _check_ints("prefill_attention", n + 1, index, cu_q, cu_k)
     qs, ks, vs = q.stride(), k.stride(), v.stride()
     if d and not qs[2] == ks[2] == vs[2] == 1:
         raise ValueError("prefill_attention: d must be contiguous")
     if out is None:
         out = _new((nq, hq, d), (hq * d, d, 1), dtype=q.dtype, device=q.device)
-    elif out.shape != q.shape or out.dtype != q.dtype or not out.is_contiguous():
-        raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype")
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
+        raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype and on its device")
     lse = _new((nq, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
     # a query tile has as many as 8 key tiles of 128, and may be split over them, only when there are so many keys
-    lib, stream = L.lib(), _raw_stream(q.device.index)
+    lib, stream = L.lib(), _raw_stream(index)
     ws = _prefill_workspace(lib, q.device, stream, d) if nk > _UNSPLIT_KEYS else None
     st = lib.kvb_prefill_attention(
         q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
@@ -157,7 +167,7 @@ class PagePool:
         """Pages for add[i] more tokens of sequence slots[i]; returns the positions (n,) int32 where they go (-1: the call
         was refused, nothing changed)."""
         n = slots.shape[0]
-        _check_ints("extend", n, slots, add)
+        _check_ints("extend", n, self._index, slots, add)
         start = torch.empty_like(slots)
         st = L.lib().kvb_page_extend(self._p, slots.data_ptr(), add.data_ptr(), n, start.data_ptr(), _raw_stream(self._index))
         if st:
@@ -168,10 +178,11 @@ class PagePool:
         """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
         sequence slots[i] (as extend returned them)."""
         n = slots.shape[0]
-        _check_ints("write", n, slots, start)
-        _check_ints("write", n + 1, cu)
-        if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (self.Hkv, self.d) or k.dtype != v.dtype or not (k.is_cuda and v.is_cuda):
-            raise ValueError("write: k and v (N, Hkv, d) CUDA tensors of one dtype")
+        _check_ints("write", n, self._index, slots, start)
+        _check_ints("write", n + 1, self._index, cu)
+        if k.dim() != 3 or k.shape != v.shape or k.shape[1:] != (self.Hkv, self.d) or k.dtype != v.dtype:
+            raise ValueError("write: k and v (N, Hkv, d) of one dtype")
+        _check_on("write", self._index, k, v)
         a, b = k.stride(), v.stride()
         if a[2] != 1 or b[2] != 1:
             raise ValueError("write: d must be contiguous")
@@ -184,8 +195,8 @@ class PagePool:
         """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
         write (rows = cu[-1])."""
         n = slots.shape[0]
-        _check_ints("read", n, slots, start)
-        _check_ints("read", n + 1, cu)
+        _check_ints("read", n, self._index, slots, start)
+        _check_ints("read", n + 1, self._index, cu)
         k, v = (_new((rows, self.Hkv, self.d), (self.Hkv * self.d, self.d, 1), dtype=dtype, device=self.device) for _ in "kv")
         st = L.lib().kvb_page_read(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
                                    _DT.get(dtype, -1), rows, _raw_stream(self._index))
@@ -196,16 +207,17 @@ class PagePool:
     def attend(self, q, slots, scaling: float = None, out=None, return_lse: bool = False):
         """Attention of q (n, Hq, Tq, d), the last Tq positions of each sequence, over its pages -> (n, Tq, Hq, d) in q's
         dtype (float16 / bfloat16); with return_lse also the log-sum-exp (n, Tq, Hq) float32."""
-        if q.dim() != 4 or q.shape[3] != self.d or not q.is_cuda:
+        if q.dim() != 4 or q.shape[3] != self.d:
             raise ValueError("attend: q (n, Hq, Tq, d) on the pool's device")
+        _check_on("attend", self._index, q)
         n, hq, tq, d = q.shape
-        _check_ints("attend", n, slots)
+        _check_ints("attend", n, self._index, slots)
         if not q.is_contiguous():
             q = q.contiguous()
         if out is None:
             out = _new((n, tq, hq, d), (tq * hq * d, hq * d, d, 1), dtype=q.dtype, device=q.device)
-        elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or not out.is_contiguous():
-            raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype")
+        elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or out.get_device() != self._index or not out.is_contiguous():
+            raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype on the pool's device")
         lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._ws.get((stream, n, hq, tq))
@@ -222,7 +234,7 @@ class PagePool:
         """Sequence dst[i] becomes a copy of src[i] (full pages shared, a partial last page copied); what it held is
         released.  All sources are taken as they were before the call."""
         n = src.shape[0]
-        _check_ints("fork", n, src, dst)
+        _check_ints("fork", n, self._index, src, dst)
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
         st = lib.kvb_page_fork(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
@@ -232,7 +244,7 @@ class PagePool:
     def free(self, slots) -> None:
         """Drops the sequences and their references to pages."""
         n = slots.shape[0]
-        _check_ints("free", n, slots)
+        _check_ints("free", n, self._index, slots)
         st = L.lib().kvb_page_free(self._p, slots.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_free")
@@ -250,7 +262,7 @@ class PagePool:
     def copy_pages(self, src, dst) -> None:
         """Page src[i] over page dst[i], codes and scales."""
         n = src.shape[0]
-        _check_ints("copy_pages", n, src, dst)
+        _check_ints("copy_pages", n, self._index, src, dst)
         st = L.lib().kvb_page_copy(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_copy")

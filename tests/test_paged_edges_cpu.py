@@ -29,3 +29,28 @@ def test_prefill_refuses_a_log_sum_exp_off_its_words(lse):
     lib = _lib.lib()
     st = lib.kvb_prefill_attention(A, A, A, 2, 10, 10, 4, 2, 128, 512, 128, 256, 128, 256, 128, A, A, 1, 0.1, A, lse, None, 0, None)
     assert st == 1 and "alignment" in lib.kvb_last_error().decode()
+
+
+class _Ints:
+    """Looks like an int32 tensor of n entries on a device."""
+
+    def __init__(self, n, index):
+        import torch
+        self.dtype, self.shape, self._index = torch.int32, (n,), index
+
+    def get_device(self):
+        return self._index
+
+    def is_contiguous(self):
+        return True
+
+
+def test_whole_numbers_of_another_device_are_refused():
+    from kvb import paged
+    paged._check_ints("call", 3, 1, _Ints(3, 1), _Ints(3, 1))
+    paged._check_on("call", 1, _Ints(3, 1))
+    for other in (0, 2, -1):
+        with pytest.raises(ValueError, match="CUDA device 1"):
+            paged._check_ints("call", 3, 1, _Ints(3, 1), _Ints(3, other))
+        with pytest.raises(ValueError, match="CUDA device 1"):
+            paged._check_on("call", 1, _Ints(3, 1), _Ints(3, other))

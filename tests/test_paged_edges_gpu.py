@@ -1,0 +1,72 @@
+"""The paged path at the edges of what a caller may hand it: outputs of the wrong place, lengths that do not fit, graphs
+that outlive a workspace, scales at the ends of their range."""
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import paged as O
+
+pytestmark = pytest.mark.gpu
+NAMES = ("kc", "vc", "ks", "vs", "table", "lens", "refs")
+
+
+@pytest.fixture(autouse=True)
+def clean_status(cuda_dev):
+    import kvb
+    kvb.device_status()
+    yield
+    assert kvb.device_status() == 0, "a test left the device status word set"
+
+
+def status():
+    import kvb
+    return kvb.device_status()
+
+
+def ints(x):
+    return torch.tensor(np.asarray(x), dtype=torch.int32, device="cuda")
+
+
+def on_gpu(pool):
+    import kvb
+    return kvb.PagePool(*[torch.from_numpy(pool[x].copy()).cuda() for x in NAMES])
+
+
+def same(g, pool, names=NAMES):
+    for x in names:
+        assert np.array_equal(getattr(g, x).cpu().numpy(), pool[x]), x
+
+
+def filled(rng, lens, hkv=1, d=64, page=16, spare=8, max_blocks=None, n_slots=None):
+    """A pool of sequences 0 .. with rows of N(0, 1)."""
+    nb = [O.blocks(n, page) for n in lens]
+    pool = O.empty_pool(sum(nb) + spare, hkv, d, page, n_slots or len(lens), max_blocks or max(nb) + 2)
+    O.extend(pool, range(len(lens)), lens)
+    cu = np.concatenate([[0], np.cumsum(lens)])
+    O.write(pool, range(len(lens)), [0] * len(lens), cu, *(rng.standard_normal((cu[-1], hkv, d)).astype(np.float32) for _ in "kv"))
+    return pool
+
+
+def test_outputs_and_inputs_of_another_place_are_refused(cuda_dev):
+    """Refused on the host, nothing is launched."""
+    import kvb
+    rng = np.random.default_rng(1)
+    g = on_gpu(filled(rng, [40, 7]))
+    q, slots = torch.randn(2, 4, 1, 64, device="cuda", dtype=torch.float16), ints([0, 1])
+    odd = torch.zeros(2 * 4 * 64 + 1, device="cuda", dtype=torch.float16)[1:].view(2, 1, 4, 64)
+    for out in (torch.zeros(2, 1, 4, 64, dtype=torch.float16), odd):
+        with pytest.raises(ValueError):
+            g.attend(q, slots, out=out)
+    for args in ((q.cpu(), slots), (q, slots.cpu())):
+        with pytest.raises(ValueError):
+            g.attend(*args)
+    rows, start, cu = torch.zeros(2, 1, 64, device="cuda"), ints([40, 7]), ints([0, 1, 2])
+    for args in ((slots, start, cu, rows.cpu(), rows), (slots, start, cu, rows, rows.cpu()), (slots, start.cpu(), cu, rows, rows)):
+        with pytest.raises(ValueError):
+            g.write(*args)
+    p, cu = torch.zeros(8, 2, 64, device="cuda", dtype=torch.float16), ints([0, 8])
+    for args, kw in (((p, p, p, cu), dict(out=p.cpu())), ((p, p.cpu(), p, cu), {}), ((p, p, p.cpu(), cu), {}), ((p, p, p, cu, cu.cpu()), {})):
+        with pytest.raises(ValueError):
+            kvb.prefill_attention(*args, **kw)
+    assert not odd.any()
