@@ -15,6 +15,7 @@ free pages).
 from __future__ import annotations
 
 import ctypes as C
+import functools
 
 import torch
 
@@ -26,6 +27,23 @@ _I32 = torch.int32
 _new = torch.empty_strided
 # the current stream's handle without building a Stream object, which costs as much as the launch (4.5 against 0.1 us)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i: torch.cuda.current_stream(i).cuda_stream)
+
+
+def _elsewhere(index: int) -> bool:
+    """Whether a call on tensors of CUDA device `index` needs that device made current first (< 0: it will be refused):
+    launches, attributes and the workspaces' sizes are those of the current device, whatever the addresses are."""
+    return index >= 0 and index != torch._C._cuda_getDevice()
+
+
+def _on_pool(method):
+    """A pool's call, with its device current."""
+    @functools.wraps(method)
+    def call(self, *args, **kw):
+        if not _elsewhere(self._index):
+            return method(self, *args, **kw)
+        with torch.cuda.device(self._index):
+            return method(self, *args, **kw)
+    return call
 
 
 def _check_on(who: str, index: int, *ts):
@@ -70,6 +88,9 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     mask, with more the queries are the last positions.  Query head a reads KV head a // (Hq // Hkv).  scaling defaults
     to d ** -0.5.  Returns out (Nq, Hq, d), with return_lse also the log-sum-exp (Nq, Hq) float32; a row that sees no
     key gives zeros and -inf."""
+    if _elsewhere(q.get_device()):
+        with torch.cuda.device(q.get_device()):
+            return prefill_attention(q, k, v, cu_q, cu_k, scaling, out, return_lse)
     if cu_k is None:
         cu_k = cu_q
     if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
@@ -163,6 +184,7 @@ class PagePool:
             ws = self._ws[(kind, stream)] = torch.zeros(max(size, 256), dtype=torch.uint8, device=self.device)
         return ws
 
+    @_on_pool
     def extend(self, slots: torch.Tensor, add: torch.Tensor) -> torch.Tensor:
         """Pages for add[i] more tokens of sequence slots[i]; returns the positions (n,) int32 where they go (-1: the call
         was refused, nothing changed)."""
@@ -174,6 +196,7 @@ class PagePool:
             L.check(st, "kvb_page_extend")
         return start
 
+    @_on_pool
     def write(self, slots, start, cu, k, v) -> None:
         """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
         sequence slots[i] (as extend returned them)."""
@@ -191,6 +214,7 @@ class PagePool:
         if st:
             L.check(st, "kvb_page_write")
 
+    @_on_pool
     def read(self, slots, start, cu, rows: int, dtype=torch.bfloat16):
         """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
         write (rows = cu[-1])."""
@@ -204,6 +228,7 @@ class PagePool:
             L.check(st, "kvb_page_read")
         return k, v
 
+    @_on_pool
     def attend(self, q, slots, scaling: float = None, out=None, return_lse: bool = False):
         """Attention of q (n, Hq, Tq, d), the last Tq positions of each sequence, over its pages -> (n, Tq, Hq, d) in q's
         dtype (float16 / bfloat16); with return_lse also the log-sum-exp (n, Tq, Hq) float32."""
@@ -230,6 +255,7 @@ class PagePool:
             L.check(st, "kvb_page_attend")
         return (out, lse) if return_lse else out
 
+    @_on_pool
     def fork(self, src, dst) -> None:
         """Sequence dst[i] becomes a copy of src[i] (full pages shared, a partial last page copied); what it held is
         released.  All sources are taken as they were before the call."""
@@ -241,6 +267,7 @@ class PagePool:
         if st:
             L.check(st, "kvb_page_fork")
 
+    @_on_pool
     def free(self, slots) -> None:
         """Drops the sequences and their references to pages."""
         n = slots.shape[0]
@@ -249,6 +276,7 @@ class PagePool:
         if st:
             L.check(st, "kvb_page_free")
 
+    @_on_pool
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the pool's start; returns their number (one int32 on the device)."""
         lib, stream = L.lib(), _raw_stream(self._index)
@@ -259,6 +287,7 @@ class PagePool:
             L.check(st, "kvb_page_compact")
         return live
 
+    @_on_pool
     def copy_pages(self, src, dst) -> None:
         """Page src[i] over page dst[i], codes and scales."""
         n = src.shape[0]

@@ -54,3 +54,50 @@ def test_whole_numbers_of_another_device_are_refused():
             paged._check_ints("call", 3, 1, _Ints(3, 1), _Ints(3, other))
         with pytest.raises(ValueError, match="CUDA device 1"):
             paged._check_on("call", 1, _Ints(3, 1), _Ints(3, other))
+
+
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
+    """With device 0 current, a pool of device 1 switches for the call and back; one of device 0 does not switch."""
+    import torch
+    from kvb import paged
+    now, switched = [0], []
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+            switched.append(self.index)
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+
+    class Pool:
+        def __init__(self, index):
+            self._index = index
+
+        @paged._on_pool
+        def call(self, a, b=0):
+            return now[0], a, b
+
+    assert Pool(1).call(5, b=6) == (1, 5, 6) and switched == [1] and now == [0]
+    assert Pool(0).call(7) == (0, 7, 0) and switched == [1]
+    for name in ("extend", "write", "read", "attend", "fork", "free", "compact", "copy_pages"):
+        assert hasattr(getattr(paged.PagePool, name), "__wrapped__"), name
+
+    class Tensor:
+        def get_device(self):
+            return 1
+
+    def seen(*args):
+        return args, now[0]
+
+    # the call begins again with device 1 current
+    whole = paged.prefill_attention
+    monkeypatch.setattr(paged, "prefill_attention", seen)
+    q = Tensor()
+    assert whole(q, 2, 3, 4, scaling=5) == ((q, 2, 3, 4, None, 5, None, False), 1) and now == [0]
