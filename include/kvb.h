@@ -503,8 +503,8 @@ typedef struct kvb_pages {
 } kvb_pages;
 
 /* Room for add[i] more tokens in sequence slots[i] (distinct slots): fresh pages are the lowest free ones in
- * the order of the list; lens grow; start[i] = the length before.  When a slot is out of range, a row of the
- * table too short or the pool has too few free pages, nothing changes and every start[i] is -1 (status bit 1
+ * the order of the list; lens grow; start[i] = the length before.  When a slot is out of range, a length outside [0,
+ * max_blocks * page], a row of the table too short or the pool has too few free pages, nothing changes and every start[i] is -1 (status bit 1
  * or 4).  slots, add, start: n int32 on the device. */
 kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32_t* add, int n, int32_t* start, void* stream);
 
@@ -537,8 +537,9 @@ kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq,
  *
  * Sequence dst[i] becomes a copy of src[i], all from the state before the call (distinct dst; a dst may be a src):
  * full pages are shared, a partial last page is copied to a fresh page (the lowest ones free before the call, in
- * the order of the list), what dst held before is released.  src[i] == dst[i] keeps the sequence as it is.  With
- * too few free pages nothing changes (status bit 4).  workspace 256-byte aligned. */
+ * the order of the list), what dst held before is released.  src[i] == dst[i] keeps the sequence as it is.  With a slot out
+ * of range or a length (of a source or a destination) outside [0, max_blocks * page] (status bit 1), or too few free pages
+ * (bit 4), nothing changes.  workspace 256-byte aligned. */
 size_t kvb_page_fork_workspace(const kvb_pages* p, int n);
 kvb_status kvb_page_fork(const kvb_pages* p, int n_pools, const int32_t* src, const int32_t* dst, int n, void* workspace,
                          size_t workspace_bytes, void* stream);

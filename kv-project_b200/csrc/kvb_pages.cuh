@@ -420,8 +420,11 @@ __device__ __forceinline__ int owner_of(const int* off, int n, int r) {
     return lo;
 }
 
+// Whether a length is one that its row of the table can hold: the pool works on the caller's lengths.
+__device__ __forceinline__ bool fits_row(const PagesView& P, int64_t len) { return len >= 0 && len <= int64_t(P.max_blocks) * P.page; }
+
 // One block.  start[i] = the tokens that sequence slots[i] had, or -1 where the call was refused (a slot out of
-// range, a row too short, not enough free pages): then nothing is changed.
+// range, a length that does not fit, a row too short, not enough free pages): then nothing is changed.
 __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, const int32_t* slots, const int32_t* add, int n,
                                                                  int32_t* start) {
     chain_kernels();
@@ -437,7 +440,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
         if (i < n) {
             const int s = slots[i], a = add[i];
             const int have = s >= 0 && s < P.n_slots ? P.lens[s] : 0;
-            if (s < 0 || s >= P.n_slots || a < 0 || int64_t(have) + a > int64_t(P.max_blocks) * P.page) bad = 1;
+            if (s < 0 || s >= P.n_slots || a < 0 || !fits_row(P, have) || !fits_row(P, int64_t(have) + a)) bad = 1;
             else need = blocks_of(have + a, P.page) - blocks_of(have, P.page);
         }
         int sum;
@@ -546,7 +549,7 @@ __global__ void __launch_bounds__(PG_THREADS) fork_plan_kernel(PagesView P, cons
         int part = 0;
         if (i < n) {
             const int s = src[i], t = dst[i];
-            if (s < 0 || s >= P.n_slots || t < 0 || t >= P.n_slots) bad = 1;
+            if (s < 0 || s >= P.n_slots || t < 0 || t >= P.n_slots || !fits_row(P, P.lens[s]) || !fits_row(P, P.lens[t])) bad = 1;
             else {
                 const int len = P.lens[s];
                 W.len[i] = len;

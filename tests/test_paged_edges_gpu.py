@@ -70,3 +70,22 @@ def test_outputs_and_inputs_of_another_place_are_refused(cuda_dev):
         with pytest.raises(ValueError):
             kvb.prefill_attention(*args, **kw)
     assert not odd.any()
+
+
+@pytest.mark.parametrize("length", [-1, -2 ** 31, 5 * 16 + 1, 2 ** 31 - 1])
+def test_lengths_that_no_row_holds_are_refused_as_a_whole(cuda_dev, length):
+    """The pool takes the caller's lengths: extend, and fork from and onto such a sequence, change nothing."""
+    rng = np.random.default_rng(2)
+    pool = filled(rng, [40, 7, 0], max_blocks=5, n_slots=4)
+    pool["lens"][3] = length
+    g = on_gpu(pool)
+    for slots, add in (([3], [1]), ([0, 3], [1, 0]), ([3, 1], [0, 1])):
+        assert (g.extend(ints(slots), ints(add)).cpu().numpy() == -1).all() and status() == 2
+        same(g, pool)
+    for src, dst in (([3], [2]), ([0], [3]), ([0, 3], [2, 1]), ([0, 1], [2, 3]), ([3], [3])):
+        g.fork(ints(src), ints(dst))
+        assert status() == 2
+        same(g, pool)
+    assert O.fork(pool, [0], [2])                       # the others go on
+    g.fork(ints([0]), ints([2]))
+    same(g, pool)
