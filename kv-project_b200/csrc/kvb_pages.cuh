@@ -431,7 +431,8 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
     extern __shared__ int off[];               // off[i]: pages of the sequences before i
     __shared__ int sh[32], list[PG_LIST];
     __shared__ int bad;
-    if (threadIdx.x == 0) bad = 0;
+    __shared__ unsigned long long want;        // all pages that are needed: the sums below may pass 32 bits
+    if (threadIdx.x == 0) bad = 0, want = 0;
     __syncthreads();
     int total = 0;
     for (int i0 = 0; i0 < n; i0 += blockDim.x) {
@@ -442,6 +443,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
             const int have = s >= 0 && s < P.n_slots ? P.lens[s] : 0;
             if (s < 0 || s >= P.n_slots || a < 0 || !fits_row(P, have) || !fits_row(P, int64_t(have) + a)) bad = 1;
             else need = blocks_of(have + a, P.page) - blocks_of(have, P.page);
+            if (need > 0) atomicAdd(&want, static_cast<unsigned long long>(need));
         }
         int sum;
         const int at = block_scan(need, sh, sum);
@@ -451,7 +453,7 @@ __global__ void __launch_bounds__(PG_THREADS) page_extend_kernel(PagesView P, co
     __syncthreads();
     if (bad) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
-    } else if (!take_free(P, total, sh, list, [&](int rank, int id) {
+    } else if (want > static_cast<unsigned long long>(P.n_pages) || !take_free(P, total, sh, list, [&](int rank, int id) {
                    const int i = owner_of(off, n, rank);
                    const int s = slots[i];
                    P.table[int64_t(s) * P.max_blocks + blocks_of(P.lens[s], P.page) + rank - off[i]] = id;

@@ -89,3 +89,19 @@ def test_lengths_that_no_row_holds_are_refused_as_a_whole(cuda_dev, length):
     assert O.fork(pool, [0], [2])                       # the others go on
     g.fork(ints([0]), ints([2]))
     same(g, pool)
+
+
+@pytest.mark.parametrize("n", [16, 17, 32])
+def test_extend_refuses_needs_whose_sum_passes_32_bits(cuda_dev, n):
+    """n sequences of 2^27 - 1 pages each: the sum is just below 2^31, above it, and just below 2^32."""
+    import kvb
+    blocks = 2 ** 27 - 1
+    table = torch.empty(n, blocks, dtype=torch.int32, device="cuda")        # rows that the call may not touch
+    z = dict(device="cuda")
+    codes, scales = torch.full((40, 1, 16, 64), 128, dtype=torch.uint8, **z), torch.zeros(40, 1, **z)
+    lens, refs = torch.zeros(n, dtype=torch.int32, **z), torch.zeros(40, dtype=torch.int32, **z)
+    g = kvb.PagePool(codes, codes.clone(), scales, scales.clone(), table, lens, refs)
+    start = g.extend(ints(range(n)), ints([blocks * 16] * n))
+    assert status() == 16 and (start == -1).all() and not lens.any() and not refs.any()
+    del g, table
+    torch.cuda.empty_cache()
