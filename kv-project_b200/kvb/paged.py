@@ -152,7 +152,7 @@ class PagePool:
         self._c = L.Pages(*[t.data_ptr() for t in ts], n_pages, hkv, d, page, *table.shape)
         self._p = C.byref(self._c)
         self._layers, self._n = (L.Pages * 1)(self._c), 1
-        self._ws = {}
+        self._ws, self._replaced = {}, []
 
     @classmethod
     def create(cls, n_pages: int, Hkv: int, d: int, page: int = 64, n_slots: int = 64, max_blocks: int = None, device="cuda"):
@@ -177,10 +177,14 @@ class PagePool:
         return other
 
     def _workspace(self, kind: str, stream: int, size: int) -> torch.Tensor:
-        """A zero-filled buffer for one kind of call on one stream, kept while it is large enough."""
+        """A zero-filled buffer for one kind of call on one stream.  One that became too small stays allocated, because a
+        captured graph may hold its address; each is twice the one before at least, so that they do not add up."""
         ws = self._ws.get((kind, stream))
         if ws is None or ws.numel() < size:
             _not_capturing(kind)
+            if ws is not None:
+                self._replaced.append(ws)
+                size = max(size, 2 * ws.numel())
             ws = self._ws[(kind, stream)] = torch.zeros(max(size, 256), dtype=torch.uint8, device=self.device)
         return ws
 

@@ -105,3 +105,36 @@ def test_extend_refuses_needs_whose_sum_passes_32_bits(cuda_dev, n):
     assert status() == 16 and (start == -1).all() and not lens.any() and not refs.any()
     del g, table
     torch.cuda.empty_cache()
+
+
+def test_a_captured_fork_and_compact_outlive_larger_calls(cuda_dev):
+    """A later, larger fork takes another workspace; what the graph holds is still its own."""
+    rng = np.random.default_rng(3)
+    pool = filled(rng, [40, 33, 5] + [20] * 30, spare=80, n_slots=40)
+    g = on_gpu(pool)
+    src, dst = ints([0, 1]), ints([33, 34])
+    with torch.cuda.stream(torch.cuda.Stream()):
+        stream = torch.cuda.current_stream()
+        g.fork(src, dst)
+        g.compact()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=stream):
+            g.fork(src, dst)
+            live = g.compact()
+        many = list(range(3, 33))
+        held = {ws.data_ptr(): ws.numel() for ws in g._ws.values()}
+        g.fork(ints(many), ints(many))                  # larger: sequences kept as they are
+    torch.cuda.synchronize()
+    assert held.keys() - {ws.data_ptr() for ws in g._ws.values()}           # the workspace was replaced
+    others = [torch.full((n,), 9, dtype=torch.uint8, device="cuda") for n in held.values() for _ in range(8)]
+    assert not held.keys() & {x.data_ptr() for x in others}
+    assert O.fork(pool, [0, 1], [33, 34])
+    O.compact(pool)
+    same(g, pool)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert O.fork(pool, [0, 1], [33, 34])
+        assert int(live) == O.compact(pool)
+        same(g, pool)
+    assert all((x == 9).all() for x in others)
