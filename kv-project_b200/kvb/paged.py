@@ -153,6 +153,7 @@ class PagePool:
         self._p = C.byref(self._c)
         self._layers, self._n = (L.Pages * 1)(self._c), 1
         self._ws, self._replaced = {}, []
+        self._attend_bytes = L.lib().kvb_page_attend_workspace(self._p, 1, hkv, 1)      # the same for any call
 
     @classmethod
     def create(cls, n_pages: int, Hkv: int, d: int, page: int = 64, n_slots: int = 64, max_blocks: int = None, device="cuda"):
@@ -172,6 +173,7 @@ class PagePool:
         other = PagePool(kc, vc, ks, vs, self.table, self.lens, self.refs)
         if (other.n_pages, other.page) != (self.n_pages, self.page):
             raise ValueError("add_layer: as many pages of as many tokens as the first pool has")
+        other._ws, other._replaced = self._ws, self._replaced           # one workspace a stream for all layers: their calls take turns
         self._layers = (L.Pages * (self._n + 1))(*self._layers, other._c)
         self._n += 1
         return other
@@ -249,9 +251,7 @@ class PagePool:
             raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype on the pool's device")
         lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
-        ws = self._ws.get((stream, n, hq, tq))
-        if ws is None:
-            ws = self._ws[(stream, n, hq, tq)] = self._workspace("attend", stream, lib.kvb_page_attend_workspace(self._p, n, hq, tq))
+        ws = self._workspace("attend", stream, self._attend_bytes)
         st = lib.kvb_page_attend(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, slots.data_ptr(), n,
                                  d ** -0.5 if scaling is None else scaling, out.data_ptr(), lse.data_ptr() if return_lse else None,
                                  ws.data_ptr(), ws.numel(), stream)

@@ -138,3 +138,23 @@ def test_a_captured_fork_and_compact_outlive_larger_calls(cuda_dev):
         assert int(live) == O.compact(pool)
         same(g, pool)
     assert all((x == 9).all() for x in others)
+
+
+def test_attention_keeps_one_workspace_a_stream(cuda_dev):
+    """Whatever the batches are, and for all layers of a table: they attend one after the other."""
+    rng = np.random.default_rng(4)
+    pool = filled(rng, [40, 33, 5, 20], hkv=2, d=64)
+    g = on_gpu(pool)
+    layers = [g] + [g.add_layer(*(x.clone() for x in (g.kc, g.vc, g.ks, g.vs))) for _ in range(3)]
+    z = dict(device="cuda")
+    wide = g.add_layer(torch.full((g.n_pages, 1, 16, 128), 128, dtype=torch.uint8, **z), torch.full((g.n_pages, 1, 16, 128), 128, dtype=torch.uint8, **z),
+                       torch.zeros(g.n_pages, 1, **z), torch.zeros(g.n_pages, 1, **z))
+    outs = []
+    for n in (1, 2, 4, 3):
+        for hq, tq in ((2, 1), (4, 3)):
+            q = torch.from_numpy(rng.standard_normal((n, hq, tq, 64))).half().cuda()
+            outs.append([p.attend(q, ints(range(n))) for p in layers])
+    assert len(layers[-1]._ws) == 1 and sum(ws.numel() for ws in g._ws.values()) < 4 << 20
+    assert all(torch.equal(x, row[0]) for row in outs for x in row)
+    wide.attend(torch.zeros(1, 4, 1, 128, dtype=torch.float16, **z), ints([0]))         # needs a larger one
+    assert len(g._ws) == 1 and torch.equal(layers[2].attend(q, ints(range(n))), outs[-1][0])
