@@ -14,7 +14,7 @@ namespace {
 constexpr int64_t kCountBytes = kvb::PD_MAX_CTAS * 8 * 4;      // per warp
 
 // floats of one partial: up to 16 query rows
-int64_t part_floats(int d) { return 16 * (int64_t(d) + 4); }
+int64_t part_floats(int d) { return 16 * (int64_t(d) + 6); }
 
 // ceil(2^64 / d) for kvb::pd_div; 0 for 1
 uint64_t reciprocal(int d) { return d == 1 ? 0 : UINT64_MAX / uint64_t(d) + 1; }

@@ -23,8 +23,9 @@
 //   S (tokens x rows) = K Q^T: a code byte becomes the fp16 pattern 0x6400 | byte = 1024 + code (one byte permute per
 //     two codes), less 1152: exact.  The channels are dealt to the lanes so that a lane reads 16-byte pieces of a row;
 //     with the 128-byte (64-byte for d = 64) swizzle these reads meet no bank twice.
-//   w = 2^(s + log2 vs - m): the value scale goes into the exponent, l takes w / vs.  m is a reference that is only
-//     raised when a logit passes it by 2^8.
+//   l takes p = 2^(s - m); the weight of the value product is w = 2^(s + log2 vs - mw), the value scale in the exponent, with
+//     a reference of its own, so that pages whose scales lie far apart lose neither mass nor values (a page of zeros has
+//     log2 vs = -inf: mass, no values).  The references are only raised when passed by 2^8; out = 2^(mw - m) O / l.
 //   O^T (channels x rows) += V^T W^T: the tokens of a lane's codes are interleaved by byte permutes, W goes through
 //     movmatrix and is rounded to fp16 (2^-11; it is the MMA's operand type).
 // Queries are scaled by a power of two per row before they become fp16, so bfloat16 queries are exact too.
@@ -58,7 +59,7 @@ struct PagedDecodeParams {
     float lam;
     void* out;                                // (n, Tq, Hq, d)
     float* lse;                               // (n, Tq, Hq) or null
-    float* part;                              // [2 grid][8 NT x (4 + d)]
+    float* part;                              // [2 grid][8 NT x (6 + d)]
     uint32_t* count;                          // [grid][8 warps]
 };
 
@@ -72,7 +73,7 @@ struct PdShape {
     static constexpr int STAGES = 3 * (128 / D);             // per warp
     static constexpr int JOIN = WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
     static constexpr int PAIRS = NT * (D / 64);              // (row, 64 channels) that a warp joins
-    static constexpr int PART = ROWS * (D + 4);              // m, l of the rows, twice (see the joining), then O
+    static constexpr int PART = ROWS * (D + 6);              // m, l, mw of the rows, twice (see the joining), then O
     static constexpr int SMEM = 1024 + WARPS * STAGES * STAGE + JOIN;
 };
 
@@ -174,7 +175,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     extern __shared__ uint8_t pd_raw[];
     __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS];
     __shared__ uint64_t full[S::WARPS][S::STAGES];
-    __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS];
+    __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS], s_w[S::WARPS][S::ROWS];
     __shared__ int warp_sum[S::WARPS];
     __shared__ int s_abort;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(pd_raw) + 1023) & ~uintptr_t(1023));
@@ -250,8 +251,10 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         const int tok = pd_div(r, A.by_rep);
         return (int64_t(seq) * A.Tq + tok) * A.Hq + h * A.rep + r - tok * A.rep;
     };
-    auto store_pair = [&](int64_t row, int ch, float a, float b, float sum) {
-        const float inv = sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum);
+    auto finite_ref = [](float m) { return m == -INFINITY ? 0.f : m; };
+    // 2^(mw - m) / l; rows that see nothing give 0, NaN stays
+    auto scale_of = [&](float m, float mw, float sum) { return sum > 0.f ? ex2(mw - finite_ref(m)) / sum : (sum == sum ? 0.f : sum); };
+    auto store_pair = [&](int64_t row, int ch, float a, float b, float inv) {
         *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a * inv, b * inv);
     };
     auto store_lse = [&](int64_t row, float top, float sum) {
@@ -308,7 +311,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         if (x.row[1] >= 0) f.y = P.ks[x.row[1]], f.w = P.vs[x.row[1]];
         return f;
     };
-    auto log_scale = [](float v) { return v > 0.f ? __log2f(v) : 0.f; };      // a page of zeros: any scale does
+    auto log_scale = [](float v) { return v > 0.f ? __log2f(v) : -INFINITY; };
     Place at = place(lane), ahead{};                             // of the units being copied, and of the 32 after
     float4 sc_now{0.f, 0.f, 0.f, 0.f}, sc_next{0.f, 0.f, 0.f, 0.f};      // ks, log2 vs of the units being computed; scales of the next
     int copied = 0;
@@ -342,7 +345,6 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
             float lam[NT][2], bias[NT][2];                       // bias: -1152 sum q, what the codes' pattern adds
-            int lim[NT][2];                                      // keys that the rows 2t, 2t + 1 see
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 float amax = 0.f;
@@ -379,13 +381,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 for (int k = 0; k < 2; ++k) {
                     lam[x][k] = __shfl_sync(0xffffffffu, down, 4 * (2 * t + k));
                     bias[x][k] = -1152.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + k));
-                    lim[x][k] = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1;
                 }
             }
-            float o[NT][KS][4], m[NT][2], l[NT][2];
+            float o[NT][KS][4], m[NT][2], mw[NT][2], l[NT][2];
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
-                m[x][0] = m[x][1] = -INFINITY;
+                m[x][0] = m[x][1] = mw[x][0] = mw[x][1] = -INFINITY;
                 l[x][0] = l[x][1] = 0.f;
 #pragma unroll
                 for (int c = 0; c < KS; ++c) o[x][c][0] = o[x][c][1] = o[x][c][2] = o[x][c][3] = 0.f;
@@ -440,46 +441,56 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
                         for (int i = 0; i < 4; ++i) s[half][x][i] = s2[0][x][i] + s2[1][x][i];
                 }
-                // ---- weights: y = s + log2 vs; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1 of either half
-                const float rv[2] = {ex2(-lv[0]), ex2(-lv[1])};
-                bool grow = false;
+                // ---- weights; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1 of either half
 #pragma unroll
-                for (int half = 0; half < 2; ++half) {
+                for (int half = 0; half < 2; ++half)
 #pragma unroll
                     for (int x = 0; x < NT; ++x)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[half][x][i] = __fmaf_rn(s[half][x][i], lam[x][i & 1] * ks[half], lv[half]);
-                }
+                        for (int i = 0; i < 4; ++i) s[half][x][i] *= lam[x][i & 1] * ks[half];
                 if (edge) {
 #pragma unroll
-                    for (int half = 0; half < 2; ++half)
+                    for (int x = 0; x < NT; ++x)
 #pragma unroll
-                        for (int x = 0; x < NT; ++x)
+                        for (int k = 0; k < 2; ++k) {
+                            // keys from this unit on that the row 2t + k sees
+                            const int lim = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1 - t0;
 #pragma unroll
-                            for (int i = 0; i < 4; ++i)
-                                if (t0 + 16 * half + g + 8 * (i >> 1) >= lim[x][i & 1]) s[half][x][i] = -INFINITY;
+                            for (int half = 0; half < 2; ++half)
+#pragma unroll
+                                for (int i = k; i < 4; i += 2)
+                                    if (16 * half + g + 8 * (i >> 1) >= lim) s[half][x][i] = -INFINITY;
+                        }
                 }
-                float top[NT][2];
+                bool grow = false;
+                float top[NT][2], topw[NT][2];
 #pragma unroll
                 for (int x = 0; x < NT; ++x)
 #pragma unroll
                     for (int i = 0; i < 2; ++i) {
-                        top[x][i] = fmaxf(fmaxf(s[0][x][i], s[0][x][i + 2]), fmaxf(s[1][x][i], s[1][x][i + 2]));
-                        grow |= top[x][i] > m[x][i] + PD_LAZY;
+                        const float a = fmaxf(s[0][x][i], s[0][x][i + 2]), b = fmaxf(s[1][x][i], s[1][x][i + 2]);
+                        top[x][i] = fmaxf(a, b);
+                        topw[x][i] = fmaxf(a + lv[0], b + lv[1]);
+                        grow |= top[x][i] > m[x][i] + PD_LAZY || topw[x][i] > mw[x][i] + PD_LAZY;
                     }
                 if (__any_sync(0xffffffffu, grow)) {
+                    auto quad_max = [](float y) {                // over the lanes of a row
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
+                        y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
+                        return fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                    };
 #pragma unroll
                     for (int x = 0; x < NT; ++x)
 #pragma unroll
                         for (int i = 0; i < 2; ++i) {
-                            float y = top[x][i];
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 4));
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 8));
-                            y = fmaxf(y, __shfl_xor_sync(0xffffffffu, y, 16));
+                            const float y = quad_max(top[x][i]), yw = quad_max(topw[x][i]);
                             if (y > m[x][i] + PD_LAZY) {
-                                const float f = ex2(m[x][i] - y);
+                                l[x][i] *= ex2(m[x][i] - y);
                                 m[x][i] = y;
-                                l[x][i] *= f;
+                            }
+                            if (yw > mw[x][i] + PD_LAZY) {
+                                const float f = ex2(mw[x][i] - yw);
+                                mw[x][i] = yw;
 #pragma unroll
                                 for (int c = 0; c < KS; ++c) {
                                     o[x][c][i] *= f;
@@ -491,14 +502,20 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 uint32_t wf[2][NT][2];
 #pragma unroll
                 for (int x = 0; x < NT; ++x) {
-                    const float r[2] = {m[x][0] == -INFINITY ? 0.f : m[x][0], m[x][1] == -INFINITY ? 0.f : m[x][1]};
+                    // w = p 2^e; e from the references' difference, which is the final factor's too, so that roundings of large
+                    // logits cancel
+                    const float r[2] = {finite_ref(m[x][0]), finite_ref(m[x][1])};
+                    const float dr[2] = {r[0] - finite_ref(mw[x][0]), r[1] - finite_ref(mw[x][1])};
 #pragma unroll
                     for (int half = 0; half < 2; ++half) {
+                        const float e[2] = {lv[half] + dr[0], lv[half] + dr[1]};
                         float w[4];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) w[i] = ex2(s[half][x][i] - r[i & 1]);
-                        l[x][0] = __fmaf_rn(w[0] + w[2], rv[half], l[x][0]);
-                        l[x][1] = __fmaf_rn(w[1] + w[3], rv[half], l[x][1]);
+                        for (int i = 0; i < 4; ++i) {
+                            const float u = s[half][x][i] - r[i & 1];
+                            w[i] = ex2(u + e[i & 1]);
+                            l[x][i & 1] += ex2(u);
+                        }
                         wf[half][x][0] = movmatrix_trans(pack_half2(w[0], w[1]));
                         wf[half][x][1] = movmatrix_trans(pack_half2(w[2], w[3]));
                     }
@@ -559,10 +576,11 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     if (g == 0) {
                         s_m[warp][8 * x + 2 * t + k] = m[x][k];
                         s_l[warp][8 * x + 2 * t + k] = v;
+                        s_w[warp][8 * x + 2 * t + k] = mw[x][k];
                     }
                 }
             float* part = A.part + int64_t(2 * blockIdx.x + (first ? 0 : 1)) * S::PART;
-            const int ml = few ? warp >> 2 : 0;                  // which copy of m and l
+            const int ml = few ? warp >> 2 : 0;                  // which copy of m, l and mw
             const bool used = (few ? warp & 3 : warp) < nrows;
             auto row_of = [&](int x) { return few ? warp & 3 : 8 * x + warp; };
             auto channel_of = [&](int y) { return (D / 8) * (lane >> 2) + 8 * (few ? warp >> 2 : y) + 2 * (lane & 3); };
@@ -578,7 +596,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             for (int x = 0; x < NT; ++x) {
                 const int r = row_of(x);
                 const int64_t row = whole ? row_at(p.seq, h, row0 + r) : 0;
-                float top = -INFINITY, sum = 0.f, f[S::WARPS];
+                float top = -INFINITY, topw = -INFINITY, sum = 0.f, inv = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
                     if (few && y > 0) break;
@@ -590,13 +608,14 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");
                     if (y == 0) {
 #pragma unroll
-                        for (int w = 0; w < S::WARPS; ++w) top = fmaxf(top, s_m[w][r]);
-                        const float ref = top == -INFINITY ? 0.f : top;
+                        for (int w = 0; w < S::WARPS; ++w) top = fmaxf(top, s_m[w][r]), topw = fmaxf(topw, s_w[w][r]);
+                        const float ref = finite_ref(top), refw = finite_ref(topw);
 #pragma unroll
                         for (int w = 0; w < S::WARPS; ++w) {
-                            f[w] = ex2(s_m[w][r] - ref);
-                            sum = __fmaf_rn(s_l[w][r], f[w], sum);
+                            f[w] = ex2(s_w[w][r] - refw);
+                            sum = __fmaf_rn(s_l[w][r], ex2(s_m[w][r] - ref), sum);
                         }
+                        inv = scale_of(top, topw, sum);
                     }
                     float2 acc{0.f, 0.f};
 #pragma unroll
@@ -606,17 +625,18 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
                     if (whole) {
-                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, sum);
+                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, inv);
                     } else if (r < nrows) {
-                        *reinterpret_cast<float2*>(part + 4 * S::ROWS + r * D + channel_of(y)) = acc;
+                        *reinterpret_cast<float2*>(part + 6 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
                 }
                 if (lane == 0 && r < nrows) {
                     if (whole) {
                         if (ml == 0) store_lse(row, top, sum);
                     } else {
-                        part[2 * ml * S::ROWS + r] = top;
-                        part[(2 * ml + 1) * S::ROWS + r] = sum;
+                        part[3 * ml * S::ROWS + r] = top;
+                        part[(3 * ml + 1) * S::ROWS + r] = sum;
+                        part[(3 * ml + 2) * S::ROWS + r] = topw;
                     }
                 }
             }
@@ -635,32 +655,33 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     // the partial of c is its first one, unless the (sequence, head, group) begins inside c's run
                     const float* slot0 = A.part + int64_t(2 * c0 + (W.share(c0) < p.v0 ? 1 : 0)) * S::PART;
                     auto slot_of = [&](int c) { return c == c0 ? slot0 : A.part + int64_t(2 * c) * S::PART; };
-                    float top[NT], sum[NT];
+                    float top[NT], topw[NT], sum[NT];
                     float2 acc[NT][D / 64];
 #pragma unroll
                     for (int x = 0; x < NT; ++x) {
-                        top[x] = -INFINITY;
+                        top[x] = topw[x] = -INFINITY;
                         sum[x] = 0.f;
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y) acc[x][y] = float2{0.f, 0.f};
                     }
-                    for (int cc = c0; cc <= c1; cc += 32) {      // 32 partials: a lane has the m and l of one
+                    for (int cc = c0; cc <= c1; cc += 32) {      // 32 partials: a lane has the m, l and mw of one
                         const int cnt = min(32, c1 - cc + 1);
-                        const float* mine_p = slot_of(min(cc + lane, c1)) + 2 * ml * S::ROWS;
-                        float f[NT], lv[NT];                     // f: m until the first loads of O are on their way
+                        const float* mine_p = slot_of(min(cc + lane, c1)) + 3 * ml * S::ROWS;
+                        float f[NT], ms[NT], lv[NT];             // f: mw until the first loads of O are on their way
 #pragma unroll
                         for (int x = 0; x < NT; ++x) {
-                            f[x] = lane < cnt ? __ldcg(mine_p + row_of(x)) : -INFINITY;
+                            ms[x] = lane < cnt ? __ldcg(mine_p + row_of(x)) : -INFINITY;
                             lv[x] = lane < cnt ? __ldcg(mine_p + S::ROWS + row_of(x)) : 0.f;
+                            f[x] = lane < cnt ? __ldcg(mine_p + 2 * S::ROWS + row_of(x)) : -INFINITY;
                         }
                         constexpr int B = 16 / NT;               // partials whose loads are in flight together
 #pragma unroll 1
                         for (int k0 = 0; k0 < cnt; k0 += B) {
                             float2 v[B][NT][D / 64];
-                            const float* q = A.part + int64_t(2 * (cc + k0)) * S::PART + 4 * S::ROWS;
+                            const float* q = A.part + int64_t(2 * (cc + k0)) * S::PART + 6 * S::ROWS;
 #pragma unroll
                             for (int k = 0; k < B; ++k) {
-                                const float* qk = k == 0 && cc + k0 == c0 ? slot0 + 4 * S::ROWS : q + 2 * k * S::PART;
+                                const float* qk = k == 0 && cc + k0 == c0 ? slot0 + 6 * S::ROWS : q + 2 * k * S::PART;
 #pragma unroll
                                 for (int x = 0; x < NT; ++x)
 #pragma unroll
@@ -673,10 +694,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                             if (k0 == 0) {
 #pragma unroll
                                 for (int x = 0; x < NT; ++x) {
-                                    const float to = fmaxf(top[x], warp_max(f[x])), ref = to == -INFINITY ? 0.f : to, old = ex2(top[x] - ref);
+                                    const float to = fmaxf(top[x], warp_max(ms[x])), ref = finite_ref(to);
+                                    sum[x] = __fmaf_rn(sum[x], ex2(top[x] - ref), kvb::warp_sum(lv[x] * ex2(ms[x] - ref)));
                                     top[x] = to;
-                                    f[x] = ex2(f[x] - ref);
-                                    sum[x] = __fmaf_rn(sum[x], old, kvb::warp_sum(lv[x] * f[x]));
+                                    const float tow = fmaxf(topw[x], warp_max(f[x])), refw = finite_ref(tow), old = ex2(topw[x] - refw);
+                                    topw[x] = tow;
+                                    f[x] = ex2(f[x] - refw);
 #pragma unroll
                                     for (int y = 0; y < D / 64; ++y) acc[x][y].x *= old, acc[x][y].y *= old;
                                 }
@@ -698,9 +721,10 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     for (int x = 0; x < NT; ++x) {
                         if (row_of(x) >= nrows) continue;
                         const int64_t row = row_at(p.seq, h, row0 + row_of(x));
+                        const float inv = scale_of(top[x], topw[x], sum[x]);
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y)
-                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, sum[x]);
+                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
                         if (lane == 0 && ml == 0) store_lse(row, top[x], sum[x]);
                     }
                 }

@@ -158,3 +158,64 @@ def test_attention_keeps_one_workspace_a_stream(cuda_dev):
     assert all(torch.equal(x, row[0]) for row in outs for x in row)
     wide.attend(torch.zeros(1, 4, 1, 128, dtype=torch.float16, **z), ints([0]))         # needs a larger one
     assert len(g._ws) == 1 and torch.equal(layers[2].attend(q, ints(range(n))), outs[-1][0])
+
+
+def check_scales(pool, g, q, slot, n):
+    """One sequence against float64.  Beside the relative terms (bfloat16 output 2^-8, float16 weights 2^-11, float32 sums and
+    exponentials 2^-13) a weight may be subnormal: 2^-25 of the largest p_j s_j a key, s_j = 127 scales being the most that the
+    key's page can hold; the reference may lag behind by 2^8 and halve nothing, as the weights then only grow."""
+    out, lse = g.attend(q, ints([slot]), 1.0, return_lse=True)
+    out, lse = out.double().cpu().numpy()[0, 0], lse.double().cpu().numpy()[0, 0]
+    k, v = (x.astype(np.float64) for x in O.rows(pool, slot, 0, n))
+    page, rep = pool["kc"].shape[2], q.shape[1] // k.shape[1]
+    most = 127.0 * pool["vs"][pool["table"][slot, np.arange(n) // page]].astype(np.float64)         # (n, Hkv)
+    for a in range(q.shape[1]):
+        h, qa = a // rep, q[0, a, 0].double().cpu().numpy()
+        s = k[:, h] @ qa
+        e = k.shape[2] * 2.0 ** -24 * float((np.abs(k[:, h]) @ np.abs(qa)).max())
+        p = np.exp(s - s.max())
+        p, want_lse = p / p.sum(), s.max() + np.log(p.sum())
+        tol = (2.0 ** -8 + 2.0 ** -11 + 2.0 ** -13 + 2 * e) * (p @ np.abs(v[:, h])) + n * 2.0 ** -25 * (p * most[:, h]).max()
+        bad = np.abs(out[a] - p @ v[:, h]) > tol
+        assert not bad.any(), (a, int(bad.sum()), out[a][bad][:4], (p @ v[:, h])[bad][:4])
+        assert abs(lse[a] - want_lse) <= e + 2.0 ** -16 + 2.0 ** -22 * abs(want_lse)
+
+
+SCALES = [      # magnitude of the values of each run of tokens; 0: pages of zeros
+    [1e-6, 0, 1e-6, 1e-6],
+    [1e-3, 1e-3, 0, 1e-3, 0],
+    [0, 0, 1e-20],
+    [2.0 ** -98, 1e12, 1],
+    [1e12, 2.0 ** -98, 0, 1e-6],
+    [2.0 ** -98],
+    [1e30, 1e-28, 1e30],
+]
+
+
+@pytest.mark.parametrize("d,hq,run", [(64, 2, 48), (128, 4, 160), (128, 32, 200)])
+@pytest.mark.parametrize("mags", SCALES)
+def test_attention_over_values_of_any_scale(cuda_dev, mags, d, hq, run):
+    """Pages of zeros take their mass and give no values; pages of tiny values keep both beside large ones."""
+    rng = np.random.default_rng(5)
+    n = run * len(mags) - 3
+    nb = O.blocks(n, 16)
+    pool = O.empty_pool(nb + 2, 2, d, 16, 1, nb)
+    O.extend(pool, [0], [n])
+    mag = np.repeat(mags, run)[:n, None, None]
+    v = (rng.uniform(0.5, 1, (n, 2, d)) * rng.choice([-1, 1], (n, 1, 1)) * mag).astype(np.float32)
+    k = rng.standard_normal((n, 2, d)).astype(np.float32)
+    O.write(pool, [0], [0], [0, n], k, v)
+    g = on_gpu(pool)
+    for size in (0.03, 0.5):
+        q = torch.from_numpy(size * rng.standard_normal((1, hq, 1, d))).bfloat16().cuda()
+        check_scales(pool, g, q, 0, n)
+
+
+def test_all_values_zero(cuda_dev):
+    rng = np.random.default_rng(6)
+    pool = O.empty_pool(8, 1, 64, 16, 1, 8)
+    O.extend(pool, [0], [100])
+    k = rng.standard_normal((100, 1, 64)).astype(np.float32)
+    O.write(pool, [0], [0], [0, 100], k, 0 * k)
+    out, lse = on_gpu(pool).attend(torch.randn(1, 2, 3, 64, device="cuda").half(), ints([0]), return_lse=True)
+    assert (out == 0).all() and torch.isfinite(lse).all()
