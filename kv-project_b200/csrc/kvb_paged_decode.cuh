@@ -305,9 +305,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         }
         return x;
     };
-    auto scales_of = [&](const Place& x) {                       // ks and vs of the tokens 0 .. and 16 ..
-        float4 f{0.f, 0.f, 0.f, 0.f};
-        if (x.row[0] >= 0) f.x = f.y = P.ks[x.row[0]], f.z = f.w = P.vs[x.row[0]];
+    auto scales_of = [&](const Place& x) {                       // ks and vs of the tokens 0 .. and 16 ..; ks < 0: no page
+        float4 f{-1.f, -1.f, 0.f, 0.f};
+        if (x.row[0] >= 0) {
+            f.x = P.ks[x.row[0]], f.z = P.vs[x.row[0]];
+            if (box == PD_UNIT) f.y = f.x, f.w = f.z;
+        }
         if (x.row[1] >= 0) f.y = P.ks[x.row[1]], f.w = P.vs[x.row[1]];
         return f;
     };
@@ -443,11 +446,13 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 }
                 // ---- weights; lane (g, t) holds tokens g, g + 8 and rows 2t, 2t + 1 of either half
 #pragma unroll
-                for (int half = 0; half < 2; ++half)
+                for (int half = 0; half < 2; ++half) {
+                    const float off = ks[half] < 0.f ? -INFINITY : 0.f;          // tokens without a page are left out
 #pragma unroll
                     for (int x = 0; x < NT; ++x)
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) s[half][x][i] *= lam[x][i & 1] * ks[half];
+                        for (int i = 0; i < 4; ++i) s[half][x][i] = __fmaf_rn(s[half][x][i], lam[x][i & 1] * ks[half], off);
+                }
                 if (edge) {
 #pragma unroll
                     for (int x = 0; x < NT; ++x)

@@ -219,3 +219,28 @@ def test_all_values_zero(cuda_dev):
     O.write(pool, [0], [0], [0, 100], k, 0 * k)
     out, lse = on_gpu(pool).attend(torch.randn(1, 2, 3, 64, device="cuda").half(), ints([0]), return_lse=True)
     assert (out == 0).all() and torch.isfinite(lse).all()
+
+
+@pytest.mark.parametrize("page,gone", [(16, [1]), (16, [0, 4]), (64, [2]), (32, [0]), (16, list(range(13)))])
+def test_pages_that_are_not_there_are_left_out(cuda_dev, page, gone):
+    """Tokens whose page number does not fit have no mass: the others' mean is the result, the status word says so."""
+    rng = np.random.default_rng(7)
+    n = 200
+    pool = filled(rng, [n], hkv=2, d=64, page=page, max_blocks=O.blocks(n, page))
+    q = rng.standard_normal((1, 4, 1, 64)).astype(np.float32)
+    q = torch.from_numpy(q).half().cuda()
+    k, v = O.rows(pool, 0, 0, n)
+    keep = ~np.isin(np.arange(n) // page, gone)
+    hurt = {x: pool[x].copy() for x in NAMES}
+    hurt["table"][0, gone] = [-1 if i % 2 else len(pool["refs"]) for i in range(len(gone))]
+    out, lse = on_gpu(hurt).attend(q, ints([0]), return_lse=True)
+    assert status() == 2
+    for a in range(4):
+        s = k[keep, a // 2].astype(np.float64) @ q[0, a, 0].double().cpu().numpy() / 8
+        if not keep.any():
+            assert (out == 0).all() and torch.isneginf(lse).all()
+            break
+        p = np.exp(s - s.max())
+        want = p @ v[keep, a // 2] / p.sum()
+        assert np.abs(out[0, 0, a].double().cpu().numpy() - want).max() <= 4 * 2.0 ** -10         # values below 4, weights and output of float16
+        assert abs(float(lse[0, 0, a]) - (s.max() + np.log(p.sum()))) <= 1e-4
