@@ -39,24 +39,33 @@ kvb_status launch(kvb::PagedDecodeParams a, cudaStream_t s) {
     const auto kern = kvb::paged_decode_kernel<T, D, NT>;
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = kvbh::allow_smem("page_attend", reinterpret_cast<const void*>(kern), SM, done)) return st;
-    a.groups = (a.rep * a.Tq + 8 * NT - 1) / (8 * NT);
-    a.by_groups = reciprocal(a.groups);
     a.by_rep = reciprocal(a.rep);
     a.page_log2 = 31 - __builtin_clz(unsigned(a.P.page));
     const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
+    // A launch's work has to fit 32 bits whatever the lengths are: fewer sequences, and where one alone can be too much, fewer
+    // row groups a launch.
+    const int rows = a.rep * a.Tq, groups = (rows + 8 * NT - 1) / (8 * NT);
+    const int64_t one = (int64_t(a.P.max_blocks) * a.P.page / kvb::PD_UNIT + 1 + kvb::PD_FIXED) * a.P.Hkv;
+    const int per_launch = int(std::max<int64_t>(1, std::min<int64_t>(groups, INT32_MAX / one)));
+    const int seqs = int(std::max<int64_t>(1, std::min<int64_t>(kvb::PD_MAX_SEQS, INT32_MAX / (one * per_launch))));
     const int n = a.n;
     const char* q = static_cast<const char*>(a.q);
     char* out = static_cast<char*>(a.out);
     const int64_t per = int64_t(a.Hq) * a.Tq;
     const int32_t* slots = a.slots;
     float* lse = a.lse;
-    for (int i = 0; i < n; i += kvb::PD_MAX_SEQS) {
-        a.n = std::min(n - i, kvb::PD_MAX_SEQS);
+    for (int i = 0; i < n; i += seqs) {
+        a.n = std::min(n - i, seqs);
         a.q = q + i * per * D * 2;
         a.out = out + i * per * D * 2;
         a.lse = lse ? lse + i * per : nullptr;
         a.slots = slots + i;
-        if (kvb_status st = launch_chained("page_attend", kern, grid, kvb::PdShape<D, NT>::THREADS, SM, s, a)) return st;
+        for (int first = 0; first < groups; first += per_launch) {
+            a.groups = std::min(groups - first, per_launch);
+            a.by_groups = reciprocal(a.groups);
+            a.row0 = first * 8 * NT;
+            if (kvb_status st = launch_chained("page_attend", kern, grid, kvb::PdShape<D, NT>::THREADS, SM, s, a)) return st;
+        }
     }
     return KVB_OK;
 }
@@ -82,6 +91,7 @@ kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq,
     if (n > 0 && (!q || !slots || !out || !workspace)) return fail(KVB_EINVAL, "page_attend: null argument");
     if (Hq <= 0 || Hq % p->Hkv != 0 || Hq > 65535) return fail(KVB_EINVAL, "page_attend: Hq a multiple of Hkv, at most 65535");
     if (n < 0 || Tq <= 0 || Tq > (1 << 20)) return fail(KVB_EINVAL, "page_attend: n >= 0, 1 <= Tq <= 2^20");
+    if (int64_t(Hq / p->Hkv) * Tq > INT32_MAX) return fail(KVB_EINVAL, "page_attend: query heads per KV head times Tq below 2^31");
     if (dtype != KVB_F16 && dtype != KVB_BF16) return fail(KVB_EUNSUPPORTED, "page_attend: q of float16 or bfloat16");
     if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "page_attend: scaling must be finite");
     if (p->n_pages * p->Hkv > INT32_MAX) return fail(KVB_EINVAL, "page_attend: n_pages * Hkv < 2^31");

@@ -53,7 +53,8 @@ struct PagedDecodeParams {
     PagesView P;
     const void* q;                            // (n, Hq, Tq, d)
     const int32_t* slots;
-    int n, Hq, Tq, rep, groups;               // groups of 8 NT query rows per (sequence, KV head)
+    int n, Hq, Tq, rep, groups;               // groups of 8 NT query rows per (sequence, KV head), from the row row0 on
+    int row0;
     uint64_t by_rep, by_groups;               // for pd_div
     int page_log2;
     float lam;
@@ -229,7 +230,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     W.n = A.n;
     W.hg = P.Hkv * A.groups;
     const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
-    if (work > INT_MAX) {                                        // 2^36 token-heads: more than the memory holds
+    if (work > INT_MAX) {                                        // the host's launches hold less, but for one group of 2^31 units
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return;
     }
@@ -265,7 +266,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     const int g = lane >> 2, t = lane & 3;
     uint4 raw[NT][KS / 2];
     auto load_q = [&](const PdPiece& p) {
-        const int h = pd_div(p.vh, A.by_groups), row0 = (p.vh - h * A.groups) * S::ROWS;
+        const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
             const int r = row0 + 8 * x + g, tok = pd_div(r, A.by_rep);
@@ -343,7 +344,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     {
         int first = 1, unit = 0;
         for (int cur = u0; cur < u1;) {
-            const int h = pd_div(p.vh, A.by_groups), row0 = (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
+            const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
             const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];

@@ -101,3 +101,10 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     monkeypatch.setattr(paged, "prefill_attention", seen)
     q = Tensor()
     assert whole(q, 2, 3, 4, scaling=5) == ((q, 2, 3, 4, None, 5, None, False), 1) and now == [0]
+
+
+def test_attend_refuses_more_rows_a_head_than_32_bits():
+    from kvb import _lib
+    lib = _lib.lib()
+    st = lib.kvb_page_attend(C.byref(pages(Hkv=1)), A, 1, 4096, 1 << 20, A, 1, 0.1, A, None, A, B, None)
+    assert st == 1 and "2^31" in lib.kvb_last_error().decode()

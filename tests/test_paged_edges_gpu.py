@@ -244,3 +244,43 @@ def test_pages_that_are_not_there_are_left_out(cuda_dev, page, gone):
         want = p @ v[keep, a // 2] / p.sum()
         assert np.abs(out[0, 0, a].double().cpu().numpy() - want).max() <= 4 * 2.0 ** -10         # values below 4, weights and output of float16
         assert abs(float(lse[0, 0, a]) - (s.max() + np.log(p.sum()))) <= 1e-4
+
+
+@pytest.mark.parametrize("page,tq,hq,lens", [(16, 150, 4, [300, 7, 0, 1000]), (128, 1, 2, [500] * 5), (16, 40, 32, [129])])
+def test_attention_over_a_table_of_the_longest_rows(cuda_dev, page, tq, hq, lens):
+    """Rows of 2^31 tokens: the call is divided over launches whose work fits 32 bits at any lengths, with the same bits."""
+    import kvb
+    rng = np.random.default_rng(8)
+    pool = filled(rng, lens, hkv=2, d=64, page=page)
+    g = on_gpu(pool)
+    q = torch.from_numpy(rng.standard_normal((len(lens), hq, tq, 64))).half().cuda()
+    want, lse = g.attend(q, ints(range(len(lens))), return_lse=True)
+    table = torch.empty(len(lens), (2 ** 31 - 1) // page, dtype=torch.int32, device="cuda")
+    table[:, :pool["table"].shape[1]] = g.table
+    h = kvb.PagePool(g.kc, g.vc, g.ks, g.vs, table, g.lens, g.refs)
+    got, gl = h.attend(q, ints(range(len(lens))), return_lse=True)
+    err = (got.float() - want.float()).abs().max()
+    assert err <= 2.0 ** -8 and torch.equal(torch.isneginf(gl), torch.isneginf(lse))       # other shares, other order of joining
+    seen = ~torch.isneginf(lse)
+    assert (gl - lse)[seen].abs().max() <= 2.0 ** -16 * 20
+
+
+def test_attention_whose_work_passes_32_bits(cuda_dev):
+    """Many query rows over a long sequence: 2^31 units of (token, row group) and more.  The last positions' rows are looked at."""
+    rng = np.random.default_rng(9)
+    n, tq, hq = 36000, 2 ** 19, 64
+    pool = filled(rng, [n], hkv=1, d=64, page=128)
+    g = on_gpu(pool)
+    q = torch.zeros(1, hq, tq, 64, dtype=torch.float16, device="cuda")
+    q[0, :, -3:] = torch.randn(hq, 3, 64, device="cuda")
+    out = torch.full((1, tq, hq, 64), 7.0, dtype=torch.float16, device="cuda")
+    got, lse = g.attend(q, ints([0]), out=out, return_lse=True)
+    assert status() == 0 and (got[0, :tq - n] == 0).all() and torch.isneginf(lse[0, :tq - n]).all()
+    k, v = (torch.from_numpy(x[:, 0]).double().cuda() for x in O.rows(pool, 0, 0, n))
+    for t in range(3):
+        seen = n - 2 + t
+        s = q[0, :, tq - 3 + t].double() @ k[:seen].t() / 8
+        want = torch.softmax(s, -1) @ v[:seen]
+        assert (got[0, tq - 3 + t].double() - want).abs().max() <= 1e-3
+    mean = v[:n - 1000].mean(0)
+    assert (got[0, tq - 1001].double() - mean).abs().max() <= 1e-3                          # a query of zeros: the mean of what it sees
