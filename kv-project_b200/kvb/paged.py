@@ -15,7 +15,6 @@ free pages).
 from __future__ import annotations
 
 import ctypes as C
-import functools
 
 import torch
 
@@ -31,19 +30,9 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda i:
 
 def _elsewhere(index: int) -> bool:
     """Whether a call on tensors of CUDA device `index` needs that device made current first (< 0: it will be refused):
-    launches, attributes and the workspaces' sizes are those of the current device, whatever the addresses are."""
+    launches, attributes and the workspaces' sizes are those of the current device, whatever the addresses are.  (Asked in
+    each call: a decorator's two more frames cost 0.4 us.)"""
     return index >= 0 and index != torch._C._cuda_getDevice()
-
-
-def _on_pool(method):
-    """A pool's call, with its device current."""
-    @functools.wraps(method)
-    def call(self, *args, **kw):
-        if not _elsewhere(self._index):
-            return method(self, *args, **kw)
-        with torch.cuda.device(self._index):
-            return method(self, *args, **kw)
-    return call
 
 
 def _check_on(who: str, index: int, *ts):
@@ -153,6 +142,7 @@ class PagePool:
         self._p = C.byref(self._c)
         self._layers, self._n = (L.Pages * 1)(self._c), 1
         self._ws, self._replaced = {}, []
+        self._attend_ws = {}                                            # stream: address and bytes
         self._attend_bytes = L.lib().kvb_page_attend_workspace(self._p, 1, hkv, 1)      # the same for any call
 
     @classmethod
@@ -190,10 +180,17 @@ class PagePool:
             ws = self._ws[(kind, stream)] = torch.zeros(max(size, 256), dtype=torch.uint8, device=self.device)
         return ws
 
-    @_on_pool
+    def _attend_workspace(self, stream: int):
+        ws = self._workspace("attend", stream, self._attend_bytes)
+        self._attend_ws[stream] = at = (ws.data_ptr(), ws.numel())
+        return at
+
     def extend(self, slots: torch.Tensor, add: torch.Tensor) -> torch.Tensor:
         """Pages for add[i] more tokens of sequence slots[i]; returns the positions (n,) int32 where they go (-1: the call
         was refused, nothing changed)."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.extend(slots, add)
         n = slots.shape[0]
         _check_ints("extend", n, self._index, slots, add)
         start = torch.empty_like(slots)
@@ -202,10 +199,12 @@ class PagePool:
             L.check(st, "kvb_page_extend")
         return start
 
-    @_on_pool
     def write(self, slots, start, cu, k, v) -> None:
         """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
         sequence slots[i] (as extend returned them)."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.write(slots, start, cu, k, v)
         n = slots.shape[0]
         _check_ints("write", n, self._index, slots, start)
         _check_ints("write", n + 1, self._index, cu)
@@ -220,10 +219,12 @@ class PagePool:
         if st:
             L.check(st, "kvb_page_write")
 
-    @_on_pool
     def read(self, slots, start, cu, rows: int, dtype=torch.bfloat16):
         """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
         write (rows = cu[-1])."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.read(slots, start, cu, rows, dtype)
         n = slots.shape[0]
         _check_ints("read", n, self._index, slots, start)
         _check_ints("read", n + 1, self._index, cu)
@@ -234,10 +235,12 @@ class PagePool:
             L.check(st, "kvb_page_read")
         return k, v
 
-    @_on_pool
     def attend(self, q, slots, scaling: float = None, out=None, return_lse: bool = False):
         """Attention of q (n, Hq, Tq, d), the last Tq positions of each sequence, over its pages -> (n, Tq, Hq, d) in q's
         dtype (float16 / bfloat16); with return_lse also the log-sum-exp (n, Tq, Hq) float32."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.attend(q, slots, scaling, out, return_lse)
         if q.dim() != 4 or q.shape[3] != self.d:
             raise ValueError("attend: q (n, Hq, Tq, d) on the pool's device")
         _check_on("attend", self._index, q)
@@ -251,18 +254,20 @@ class PagePool:
             raise ValueError("attend: out must be contiguous (n, Tq, Hq, d) in q's dtype on the pool's device")
         lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
-        ws = self._workspace("attend", stream, self._attend_bytes)
+        ws, size = self._attend_ws.get(stream) or self._attend_workspace(stream)
         st = lib.kvb_page_attend(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, slots.data_ptr(), n,
                                  d ** -0.5 if scaling is None else scaling, out.data_ptr(), lse.data_ptr() if return_lse else None,
-                                 ws.data_ptr(), ws.numel(), stream)
+                                 ws, size, stream)
         if st:
             L.check(st, "kvb_page_attend")
         return (out, lse) if return_lse else out
 
-    @_on_pool
     def fork(self, src, dst) -> None:
         """Sequence dst[i] becomes a copy of src[i] (full pages shared, a partial last page copied); what it held is
         released.  All sources are taken as they were before the call."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.fork(src, dst)
         n = src.shape[0]
         _check_ints("fork", n, self._index, src, dst)
         lib, stream = L.lib(), _raw_stream(self._index)
@@ -271,18 +276,22 @@ class PagePool:
         if st:
             L.check(st, "kvb_page_fork")
 
-    @_on_pool
     def free(self, slots) -> None:
         """Drops the sequences and their references to pages."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.free(slots)
         n = slots.shape[0]
         _check_ints("free", n, self._index, slots)
         st = L.lib().kvb_page_free(self._p, slots.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_free")
 
-    @_on_pool
     def compact(self) -> torch.Tensor:
         """Moves the live pages to the pool's start; returns their number (one int32 on the device)."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.compact()
         lib, stream = L.lib(), _raw_stream(self._index)
         ws = self._workspace("compact", stream, lib.kvb_page_compact_workspace(self._p))
         live = torch.empty((), dtype=_I32, device=self.device)
@@ -291,9 +300,11 @@ class PagePool:
             L.check(st, "kvb_page_compact")
         return live
 
-    @_on_pool
     def copy_pages(self, src, dst) -> None:
         """Page src[i] over page dst[i], codes and scales."""
+        if _elsewhere(self._index):
+            with torch.cuda.device(self._index):
+                return self.copy_pages(src, dst)
         n = src.shape[0]
         _check_ints("copy_pages", n, self._index, src, dst)
         st = L.lib().kvb_page_copy(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))

@@ -76,18 +76,22 @@ def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
     monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
     monkeypatch.setattr(torch.cuda, "device", device)
 
-    class Pool:
-        def __init__(self, index):
-            self._index = index
+    def again(name):
+        return lambda self, *args: (name, now[0], args)
 
-        @paged._on_pool
-        def call(self, a, b=0):
-            return now[0], a, b
-
-    assert Pool(1).call(5, b=6) == (1, 5, 6) and switched == [1] and now == [0]
-    assert Pool(0).call(7) == (0, 7, 0) and switched == [1]
-    for name in ("extend", "write", "read", "attend", "fork", "free", "compact", "copy_pages"):
-        assert hasattr(getattr(paged.PagePool, name), "__wrapped__"), name
+    calls = dict(extend=2, write=5, read=5, attend=5, fork=2, free=1, compact=0, copy_pages=2)
+    Pool = type("Pool", (paged.PagePool,), {name: again(name) for name in calls})
+    pool = Pool.__new__(Pool)
+    pool._index = 1
+    for name, n in calls.items():                       # each begins again with device 1 current, then the first is back
+        given = tuple(range(n - (name == "read")))
+        got = getattr(paged.PagePool, name)(pool, *given)
+        assert got[:2] == (name, 1) and got[2][:len(given)] == given and now == [0]
+    assert switched == [1] * len(calls)
+    pool._index = 0
+    with pytest.raises(AttributeError):                 # device 0 is current: no switch, the call itself begins
+        paged.PagePool.free(pool, None)
+    assert switched == [1] * len(calls)
 
     class Tensor:
         def get_device(self):
