@@ -475,9 +475,10 @@ kvb_status kvb_operational_rd(const float* A, int64_t rows, int64_t n, int64_t l
  * bases; cu_q, cu_k (n + 1) int32 on the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 32-byte
  * aligned; lse (nq, Hq) float32 (natural log of the attended mass) or null.  Rows of no sequence are not written.
  * workspace (kvb_prefill_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
- * (every call leaves its counters at zero), one per stream that runs calls concurrently; with it the work of
- * long rows is split over the keys, without it (null) every query tile is computed in one piece.  A stream that is being
- * captured is refused (KVB_EUNSUPPORTED). */
+ * (every call leaves its counters at zero; what another call left in them is not counted and raises status bit 3), one per
+ * stream that runs calls concurrently; with it the work of long rows is split over the keys, without it (null) every query
+ * tile is computed in one piece.  Offsets that do not fit the rows raise status bit 1 and their sequences are left out.  A
+ * stream that is being captured is refused (KVB_EUNSUPPORTED). */
 size_t kvb_prefill_workspace(int d);
 kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq,
                                  int Hkv, int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head,
@@ -509,7 +510,7 @@ typedef struct kvb_pages {
 kvb_status kvb_page_extend(const kvb_pages* p, const int32_t* slots, const int32_t* add, int n, int32_t* start, void* stream);
 
 /* Codes of packed rows: the rows [cu[i], cu[i + 1]) of k and v (rows, Hkv, d) go to the positions start[i],
- * start[i] + 1, ... of sequence slots[i] (start[i] < 0: left out).  Per (page, head) and side, s = max |x| / 127 over
+ * start[i] + 1, ... of sequence slots[i] (distinct slots; start[i] < 0: left out).  Per (page, head) and side, s = max |x| / 127 over
  * the page's rows so far (non-finite values left out; 0 where the maximum is below 2^-100), code = clamp(rint(x *
  * (1 / s)), -127, 127) + 128, NaN as 128.  Rows before the first one written keep the page's scale as long as it
  * suffices (s = max(old s, new rows)) and are recoded from their codes where it grows, code' = rint((code - 128) *
@@ -519,7 +520,8 @@ kvb_status kvb_page_write(const kvb_pages* p, const int32_t* slots, const int32_
                           const void* k, const void* v, int dtype, int64_t rows, int64_t k_row, int64_t k_head,
                           int64_t v_row, int64_t v_head, void* stream);
 
-/* The stored values of the same ranges, rounded to dtype: k and v (rows, Hkv, d) dense. */
+/* The stored values of the same ranges, rounded to dtype: k and v (rows, Hkv, d) dense, 16-byte aligned; rows of ranges
+ * that are left out are not written. */
 kvb_status kvb_page_read(const kvb_pages* p, const int32_t* slots, const int32_t* start, const int32_t* cu, int n, void* k,
                          void* v, int dtype, int64_t rows, void* stream);
 

@@ -14,21 +14,23 @@
 // memory; a run that is only a part of a (sequence, head, group) leaves a partial, and the CTA that completes the last
 // part joins the partials in the order of the tokens (each warp its rows), so the result does not depend on timing.
 //
-// A step of 8 sequences of 32768 tokens, 8 heads, d 128 (537 MB), with the write of its rows: 97.5 us, 5.5 TB/s; about 7
-// TB/s at the margin, the rest is the start (4 us), the first copies' latency and the join (the same step without any
-// arithmetic took 97 us when it took 103 with).  At 8 x 16384 (269 MB, all of the DRAM traffic): ALU pipe 39 % busy (the
-// codes' permutes), tensor pipe 17 %, issue slots 38 %, no shared-memory bank conflicts.
+// A step of 8 sequences of 32768 tokens, 8 heads, d 128 (537 MB), with the write of its rows: 97 us in a loop, 5.5 TB/s;
+// about 7 TB/s at the margin, the rest is the start (4 us), the first copies' latency and the join.  At 8 x 16384 (269 MB,
+// all of the DRAM traffic): ALU pipe 39 % busy (the codes' permutes), tensor pipe 17 %, issue slots 41 %, no bank conflicts
+// in the loads.
 //
 // Per 16 tokens, with the query rows (rep heads x Tq queries, 8 per MMA column group) as the N operand:
 //   S (tokens x rows) = K Q^T: a code byte becomes the fp16 pattern 0x6400 | byte = 1024 + code (one byte permute per
-//     two codes), less 1152: exact.  The channels are dealt to the lanes so that a lane reads 16-byte pieces of a row;
+//     two codes), less 1152: exact operands.  The sums begin at -1152 sum q, so they are rounded at its size where a
+//     query's entries have one sign.  The channels are dealt to the lanes so that a lane reads 16-byte pieces of a row;
 //     with the 128-byte (64-byte for d = 64) swizzle these reads meet no bank twice.
 //   l takes p = 2^(s - m); the weight of the value product is w = 2^(s + log2 vs - mw), the value scale in the exponent, with
 //     a reference of its own, so that pages whose scales lie far apart lose neither mass nor values (a page of zeros has
 //     log2 vs = -inf: mass, no values).  The references are only raised when passed by 2^8; out = 2^(mw - m) O / l.
 //   O^T (channels x rows) += V^T W^T: the tokens of a lane's codes are interleaved by byte permutes, W goes through
 //     movmatrix and is rounded to fp16 (2^-11; it is the MMA's operand type).
-// Queries are scaled by a power of two per row before they become fp16, so bfloat16 queries are exact too.
+// Queries are scaled by a power of two per row, their largest entry to [8, 16), before they become fp16: entries down to
+// 2^-20 of it (bfloat16; float16 2^-17) are exact, those below lose bits to the subnormal range and are gone at 2^-28.
 #pragma once
 #include <cuda.h>
 

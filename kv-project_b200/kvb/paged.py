@@ -6,10 +6,11 @@
                       side): extend, write, attend, read, fork, free, compact, copy_pages.  It stands where
                       the reference's per-sequence buffers do (LayerState, STRATA_KV.py:682-720), for a batch.
 
-Every call enqueues on the current stream and never synchronises.  Whole numbers (slots, lengths, page
-numbers) are int32 tensors on the device, so a captured graph serves any lengths; ranges that do not fit are
-left out and raise the device status word (``kvb.device_status``: bit 1 a range, bit 4 a pool without enough
-free pages).
+Every call enqueues on the current stream of its tensors' device and never synchronises.  Whole numbers (slots, lengths,
+page numbers) are int32 tensors on the device, so a captured graph of a pool's calls serves any lengths (one call of each
+kind on the stream first: workspaces are not made inside a capture); prefill_attention is not captured, it raises
+NotImplementedError.  Ranges that do not fit are left out and raise the device status word (``kvb.device_status``: bit 1 a
+range, bit 4 a pool without enough free pages); rows that are left out of a result are not written.
 """
 
 from __future__ import annotations
@@ -57,11 +58,11 @@ def _not_capturing(who: str):
 
 
 _PREFILL_WS = {}
-_UNSPLIT_KEYS = 896
+_UNSPLIT_KEYS = 1024
 
 
 def _prefill_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
-    """The zero-filled workspace of one stream (40 MB), made at the first call that may need it."""
+    """The zero-filled workspace of one stream (40 MB at d 128), made at the first call that may need it."""
     ws = _PREFILL_WS.get((device.index, stream, d))
     if ws is None:
         _not_capturing("prefill_attention")
@@ -104,7 +105,7 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
         raise ValueError("prefill_attention: out must be contiguous (Nq, Hq, d) in q's dtype and on its device")
     lse = _new((nq, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
-    # a query tile has as many as 8 key tiles of 128, and may be split over them, only when there are so many keys
+    # only query tiles of more than 16 steps of 64 keys are ever cut into pieces
     lib, stream = L.lib(), _raw_stream(index)
     ws = _prefill_workspace(lib, q.device, stream, d) if nk > _UNSPLIT_KEYS else None
     st = lib.kvb_prefill_attention(
@@ -201,7 +202,7 @@ class PagePool:
 
     def write(self, slots, start, cu, k, v) -> None:
         """Codes of the packed rows k, v (N, Hkv, d): rows cu[i] .. cu[i + 1] - 1 go to the positions start[i] ... of
-        sequence slots[i] (as extend returned them)."""
+        sequence slots[i] (as extend returned them; distinct slots, as two ranges of one page would be written at once)."""
         if _elsewhere(self._index):
             with torch.cuda.device(self._index):
                 return self.write(slots, start, cu, k, v)
@@ -221,7 +222,7 @@ class PagePool:
 
     def read(self, slots, start, cu, rows: int, dtype=torch.bfloat16):
         """The stored keys and values (rows, Hkv, d) of the positions start[i] ... of sequence slots[i], packed as in
-        write (rows = cu[-1])."""
+        write (rows = cu[-1]); rows of a range that is left out (start[i] < 0, or one that does not fit) are not written."""
         if _elsewhere(self._index):
             with torch.cuda.device(self._index):
                 return self.read(slots, start, cu, rows, dtype)

@@ -63,3 +63,36 @@ def test_many_calls_in_a_row_give_the_same_bits(cuda_dev):
     want = [kvb.prefill_attention(*c) for c in cases]
     outs = [[kvb.prefill_attention(*c) for c in cases] for _ in range(30)]
     assert all(torch.equal(o, w) for row in outs for o, w in zip(row, want))
+
+
+@pytest.mark.parametrize("dtype,d,hkv", [(torch.float16, 128, 2), (torch.bfloat16, 64, 1)])
+@pytest.mark.parametrize("poison", [float("nan"), -float("inf")])
+def test_non_finite_values_in_cut_items(cuda_dev, dtype, d, hkv, poison):
+    """Rows before a non-finite value keep their bits, rows from it on are not finite in its channel only, whichever piece
+    of the keys it lies in."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(3)
+    ql, kl = [70, 3], [6000, 2500]
+    q = torch.randn(sum(ql), 4 * hkv, d, generator=g, device="cuda").to(dtype)
+    k, v = (torch.randn(sum(kl), hkv, d, generator=g, device="cuda").to(dtype) for _ in range(2))
+    cu_q, cu_k = ints([0, 70, 73]), ints([0, 6000, 8500])
+    clean = kvb.prefill_attention(q, k, v, cu_q, cu_k)
+    assert torch.isfinite(clean).all()
+    for key in (0, 3000, 5930, 5995, 5999):
+        p = v.clone()
+        p[key, -1, 11] = poison
+        got = kvb.prefill_attention(q, k, p, cu_q, cu_k)
+        first, heads = max(0, key - 5930), slice(4 * (hkv - 1), None)
+        assert not torch.isfinite(got[first:70, heads, 11]).any()
+        got[first:70, heads, 11] = clean[first:70, heads, 11]
+        assert torch.equal(got, clean)
+
+
+def test_broadcast_rows_and_heads(cuda_dev):
+    """Strides of zero: one key head expanded over all, one query row for every token."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(4)
+    q = torch.randn(1, 8, 64, generator=g, device="cuda").half().expand(90, 8, 64)
+    k, v = (torch.randn(90, 1, 64, generator=g, device="cuda").half().expand(90, 4, 64) for _ in range(2))
+    cu = ints([0, 33, 90])
+    assert torch.equal(kvb.prefill_attention(q, k, v, cu), kvb.prefill_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu))
