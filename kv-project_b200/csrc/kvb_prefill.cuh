@@ -493,6 +493,7 @@ __global__ void __launch_bounds__(PF_THREADS, PF_CTAS_PER_SM) prefill_kernel(con
                     if (!(fabsf(to_f32(e[c])) < INFINITY)) e[c] = from_f32<T>(0.f);
                 atomicOr(&s_bad[x.j0 + j - x.jm][row >> 5], 1u << (row & 31));
             }
+            __syncwarp();                                        // the products below want the lanes together
         }
         const bool seen = key0 < hi;                             // by some row of the warp
         uint32_t p[2][NT / 2][4];
