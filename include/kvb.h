@@ -534,6 +534,27 @@ size_t kvb_page_attend_workspace(const kvb_pages* p, int n, int Hq, int Tq);
 kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
                            float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Which leading pages the sequences slots[0 .. n) share, n <= 1024 (distinct or not): plan, (8 n + 1) int32 on the device.
+ * In up to 4 rounds, the sequences of one class (at first all) that hold the same page in the block behind their common
+ * ones, a block that is full in each, form a class of the next round; a class of two or more gets a segment, from the blocks
+ * before to the last that all its members hold in full.  order = plan[0 .. n): places in the list, a class's members
+ * together, classes by their first member; own = plan[n .. 2 n): the first token of a sequence that no segment covers; depth =
+ * plan[2 n .. 3 n): how many cover it; segments = plan[3 n .. 8 n), five each by level and place: first member's place in order,
+ * members, first token, end, level, zeros behind the last; plan[8 n]: their number.  Table entries that are no page are
+ * nobody's; a slot out of range raises status bit 1 and shares nothing. */
+kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, void* stream);
+
+/* kvb_page_attend for the slots of a plan: the same results up to rounding, each segment's codes read once for all its
+ * members.  The plan stays good while the sequences only grow (extend, write); after fork, free, compact or copy it has to be
+ * made anew (what it says is checked, so that a stale plan reads no wrong address; segments that do not fit raise status bit 1
+ * and the results of their members are not defined).  workspace: 256-byte aligned, its first
+ * kvb_page_attend_workspace(p, n, Hq, Tq) bytes zero-filled once before its first use and then reused (every call leaves its
+ * counters at zero), one per stream that runs calls concurrently. */
+size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq);
+kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
+                                  const int32_t* plan, float scaling, void* out, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream);
+
 /* The calls below that move pages take the pools of all layers that share a table: p[0 .. n_pools), alike but for codes,
  * scales, Hkv and d; the table is changed once.
  *

@@ -1,0 +1,63 @@
+// kvb_api_shared.cu - kvb_page_share and kvb_page_attend_shared (include/kvb.h): validation and launches of the search for
+// shared pages (kvb_share.cuh) and of the attention that computes them once for all their sequences (kvb_paged_decode.cuh).
+#include "kvb_paged_host.cuh"
+#include "kvb_share.cuh"
+
+namespace {
+
+// Segments cover a sequence at most this often: each has two or more parts below it.
+int levels_of(int n) { return std::min(kvb::PS_LEVELS, std::max(n - 1, 0)); }
+
+int64_t level_offset(int d) { return (int64_t(kvbh::paged_part_bytes(d)) + 255) / 256 * 256; }
+
+}  // namespace
+
+extern "C" {
+
+kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, void* stream) {
+    if (kvb_status st = kvbh::check_pages("page_share", p)) return st;
+    if (!plan || (n > 0 && !slots)) return fail(KVB_EINVAL, "page_share: null argument");
+    if (n < 0 || n > kvb::PS_MAX_SEQS) return fail(KVB_EINVAL, "page_share: 0 <= n <= %d sequences a call", kvb::PS_MAX_SEQS);
+    static std::atomic<uint64_t> done{0};
+    if (kvb_status st = kvbh::allow_smem("page_share", reinterpret_cast<const void*>(kvb::page_share_kernel), int(sizeof(kvb::ShareSmem)), done))
+        return st;
+    return launch_chained("page_share", kvb::page_share_kernel, 1, kvb::PS_THREADS, sizeof(kvb::ShareSmem), static_cast<cudaStream_t>(stream),
+                          kvbh::view_of(p), slots, n, plan);
+}
+
+size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq) {
+    if (kvbh::check_pages("page_attend_shared", p) || n < 0 || n > kvb::PS_MAX_SEQS || Hq <= 0 || Tq <= 0) return 0;
+    return size_t(level_offset(p->d)) + size_t(levels_of(n)) * n * Hq * Tq * (p->d + 2) * 4;
+}
+
+kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
+                                  const int32_t* plan, float scaling, void* out, float* lse, void* workspace,
+                                  size_t workspace_bytes, void* stream) {
+    if (kvb_status st = kvbh::check_pages("page_attend_shared", p)) return st;
+    if (n > 0 && !plan) return fail(KVB_EINVAL, "page_attend_shared: null argument");
+    if (n > kvb::PS_MAX_SEQS) return fail(KVB_EINVAL, "page_attend_shared: n <= %d sequences a call", kvb::PS_MAX_SEQS);
+    kvb::PagedDecodeParams a{};
+    if (kvb_status st = kvbh::paged_params("page_attend_shared", p, q, dtype, Hq, Tq, slots, n, scaling, out, lse, workspace, a)) return st;
+    if (n == 0) return KVB_OK;
+    // units x row groups of all segments fit 32 bits: on a level they are those of disjoint sequences
+    const int64_t units = int64_t(p->max_blocks) * p->page / kvb::PD_UNIT + kvb::PS_LEVELS * (1 + kvb::PD_FIXED), groups = int64_t(n) * a.rep * Tq / 8 + n;
+    if (units > INT32_MAX / p->Hkv / groups)
+        return fail(KVB_EUNSUPPORTED, "page_attend_shared: tokens of a table row times query rows too many for one call");
+    if (workspace_bytes < kvb_page_attend_shared_workspace(p, n, Hq, Tq) || !aligned(workspace, 256))
+        return fail(KVB_EINVAL, "page_attend_shared: workspace of %zu bytes, 256-byte aligned", kvb_page_attend_shared_workspace(p, n, Hq, Tq));
+    if (kvb_status st = kvbh::paged_maps("page_attend_shared", p, a)) return st;
+    kvbh::paged_workspace(workspace, a);
+    a.shared = kvb::SharedView{plan, slots, n, p->page, p->max_blocks * p->page, levels_of(n)};
+    a.rows = int64_t(n) * Tq * Hq;
+    a.level_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + level_offset(p->d));
+    a.level_ml = a.level_o + levels_of(n) * a.rows * p->d;
+    a.by_rows = kvbh::reciprocal(a.rep * Tq);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (n > 1)
+        if (kvb_status st = kvbh::paged_launch_any<kvb::PD_SEGMENTS>("page_attend_shared", a, dtype, int64_t(n) * a.rep * Tq, s)) return st;
+    return kvbh::paged_launch_any<kvb::PD_OWN>("page_attend_shared", a, dtype, int64_t(a.rep) * Tq, s);
+}
+
+}  // extern "C"
+
+KVB_STATUS_WORDS(status_words_shared)

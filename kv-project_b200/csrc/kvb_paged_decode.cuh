@@ -38,6 +38,7 @@
 
 #include "kvb_common.cuh"
 #include "kvb_pages_view.cuh"
+#include "kvb_share_view.cuh"
 
 namespace kvb {
 
@@ -49,6 +50,11 @@ constexpr int PD_MAX_CTAS = 256;
 constexpr int PD_FIXED = 16;
 constexpr int PD_LEAST = 4;                   // a CTA's least share
 constexpr float PD_LAZY = 8.f;
+
+// What a launch attends over.
+constexpr int PD_ALL = 0;                     // every sequence's tokens
+constexpr int PD_OWN = 1;                     // the tokens behind a sequence's shared ones; its segments' parts are joined in
+constexpr int PD_SEGMENTS = 2;                // the tokens that several sequences share, for all of them at once
 
 struct PagedDecodeParams {
     CUtensorMap tm_k, tm_v;                   // codes as (d, page, n_pages * Hkv), box d x min(page, 32) x 1
@@ -64,6 +70,13 @@ struct PagedDecodeParams {
     float* lse;                               // (n, Tq, Hq) or null
     float* part;                              // [2 grid][8 NT x (6 + d)]
     uint32_t* count;                          // [grid][8 warps]
+    // PD_OWN and PD_SEGMENTS
+    SharedView shared;
+    int seq0;                                 // PD_OWN: the launch's first sequence in the plan
+    int64_t rows;                             // of the call, all sequences: n Tq Hq
+    float* level_o;                           // [PS_LEVELS][rows][d], normalised
+    float* level_ml;                          // [PS_LEVELS][rows][2]: maximum, sum
+    uint64_t by_rows;                         // for pd_div by rep Tq
 };
 
 template <int D, int NT>
@@ -82,11 +95,21 @@ struct PdShape {
 
 // The work of a call: per (sequence, KV head, row group) its units, and PD_FIXED more in the shares that the CTAs get
 // (preparing the queries and joining the warps costs about as much time as that many units).
+template <int MODE>
 struct PdPlan {
-    const int* pre;                           // [n + 1] units before each sequence, for one head and group
+    const int* pre;                           // [n + 1] units before each sequence, for one head and group (segments: for all)
+    const int* shares;                        // segments: [n + 1] places before each
     int n, hg;                                // sequences; KV heads x groups
     int quota, extra, ctas;                   // shares: the first `extra` CTAs get quota + 1
 
+    __device__ __forceinline__ int unit0(int i) const { return MODE == PD_SEGMENTS ? pre[i] : pre[i] * hg; }
+    __device__ __forceinline__ int place0(int i) const { return MODE == PD_SEGMENTS ? shares[i] : (pre[i] + i * PD_FIXED) * hg; }
+    __device__ __forceinline__ int heads(int i) const {          // KV heads x groups of a sequence
+        return MODE == PD_SEGMENTS ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / PD_FIXED : hg;
+    }
+    __device__ __forceinline__ int units(int i) const {
+        return MODE == PD_SEGMENTS ? (pre[i + 1] - pre[i]) / heads(i) : pre[i + 1] - pre[i];
+    }
     __device__ __forceinline__ int share(int c) const { return c * quota + min(c, extra); }
     __device__ __forceinline__ int holder(int v) const {
         const int big = extra * (quota + 1);
@@ -97,11 +120,11 @@ struct PdPlan {
         int lo = 0, hi = n;
         while (hi - lo > 1) {
             const int mid = (lo + hi) >> 1;
-            if ((pre[mid] + mid * PD_FIXED) * hg <= v) lo = mid;
+            if (place0(mid) <= v) lo = mid;
             else hi = mid;
         }
-        const int u = pre[lo + 1] - pre[lo], local = v - (pre[lo] + lo * PD_FIXED) * hg, vh = min(local / (u + PD_FIXED), hg);
-        return pre[lo] * hg + vh * u + max(local - vh * (u + PD_FIXED) - PD_FIXED, 0);
+        const int u = units(lo), local = v - place0(lo), vh = min(local / (u + PD_FIXED), heads(lo));
+        return unit0(lo) + vh * u + max(local - vh * (u + PD_FIXED) - PD_FIXED, 0);
     }
 };
 
@@ -111,21 +134,22 @@ struct PdPiece {
 };
 
 // The piece that begins at unit `cur` of all work.
-__device__ __forceinline__ PdPiece pd_piece(const PdPlan& W, int cur, int end) {
+template <int MODE>
+__device__ __forceinline__ PdPiece pd_piece(const PdPlan<MODE>& W, int cur, int end) {
     int lo = 0, hi = W.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
-        if (W.pre[mid] * W.hg <= cur) lo = mid;
+        if (W.unit0(mid) <= cur) lo = mid;
         else hi = mid;
     }
     PdPiece p;
     p.seq = lo;
-    p.units = W.pre[lo + 1] - W.pre[lo];
-    const int local = cur - W.pre[lo] * W.hg;
+    p.units = W.units(lo);
+    const int local = cur - W.unit0(lo);
     p.vh = local / p.units;
     p.a = local - p.vh * p.units;
     p.b = min(p.units, p.a + (end - cur));
-    p.v0 = (W.pre[lo] + lo * PD_FIXED) * W.hg + p.vh * (p.units + PD_FIXED);
+    p.v0 = W.place0(lo) + p.vh * (p.units + PD_FIXED);
     return p;
 }
 
@@ -171,12 +195,15 @@ __device__ __forceinline__ int pd_exponent(float amax) {
 // is mostly their number: a division by a variable is 20 and more.
 __device__ __forceinline__ int pd_div(int n, uint64_t by) { return by ? int(__umul64hi(uint64_t(uint32_t(n)), by)) : n; }
 
-template <typename T, int D, int NT>
+template <typename T, int D, int NT, int MODE>
 __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kernel(const __grid_constant__ PagedDecodeParams A) {
     using S = PdShape<D, NT>;
     constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
     extern __shared__ uint8_t pd_raw[];
-    __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS];
+    // of the sequences (or segments): units before them, slot, tokens up to which they go and from which on; of segments the
+    // places before them, the others stay in global memory
+    constexpr int MAX = MODE == PD_SEGMENTS ? PS_MAX_SEQS : PD_MAX_SEQS, HELD = MODE == PD_SEGMENTS ? 1 : PD_MAX_SEQS;
+    __shared__ int pre[MAX + 1], s_shares[MODE == PD_SEGMENTS ? MAX + 1 : 1], s_slot[HELD], s_len[HELD], s_first[MODE == PD_OWN ? HELD : 1];
     __shared__ uint64_t full[S::WARPS][S::STAGES];
     __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS], s_w[S::WARPS][S::ROWS];
     __shared__ int warp_sum[S::WARPS];
@@ -192,22 +219,62 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         s_abort = 0;
         fence_mbar_init();
         pre[0] = 0;
+        if (MODE == PD_SEGMENTS) s_shares[0] = 0;
     }
     chain_kernels();
+    const SharedView& V = A.shared;
+    const int n_seqs = MODE == PD_SEGMENTS ? V.segment_count() : A.n;
+    auto first_of = [&](int i) { return MODE == PD_OWN ? s_first[i] : MODE == PD_SEGMENTS ? V.segment(i).start : 0; };
+    auto end_of = [&](int i) { return MODE == PD_SEGMENTS ? V.segment(i).end : s_len[i]; };
+    auto slot_of_seq = [&](int i) { return MODE == PD_SEGMENTS ? V.slot_of(V.segment(i), P.n_slots) : s_slot[i]; };
+    // query rows of a sequence (or segment) for one KV head, and their groups
+    auto rows_of = [&](int i) { return MODE == PD_SEGMENTS ? V.segment(i).members * A.rep * A.Tq : A.rep * A.Tq; };
     // units before each sequence: an inclusive scan, S::THREADS sequences at a time; an empty sequence is one unit
     // without keys, whose rows still have to be written
     int before = 0;
-    for (int i0 = 0; i0 < A.n; i0 += S::THREADS) {
+    int before_places = 0;
+    for (int i0 = 0; i0 < n_seqs; i0 += S::THREADS) {
         const int i = i0 + threadIdx.x;
-        int u = 0;
-        if (i < A.n) {
+        int u = 0, places = 0;
+        if constexpr (MODE == PD_SEGMENTS) {
+            if (i < n_seqs) {
+                const SharedSegment g = V.segment(i);
+                const int hg = (g.members * A.rep * A.Tq + S::ROWS - 1) / S::ROWS * P.Hkv, units = (g.end - g.start + PD_UNIT - 1) / PD_UNIT;
+                // a plan's segments fit 32 bits together (the host has seen to it); what is no plan may not
+                u = units <= INT_MAX / hg - PD_FIXED ? units * hg : 0;
+                places = u + PD_FIXED * hg;
+            }
+        } else if (i < A.n) {
             const int slot = A.slots[i];
             int len = 0;
             if (slot >= 0 && slot < P.n_slots) len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
             else raise_status(KVB_DEV_BOUNDS);
             s_slot[i] = slot;
             s_len[i] = len;
+            if constexpr (MODE == PD_OWN) {
+                const int own = V.own_of(A.seq0 + i, len);
+                s_first[i] = own;
+                len -= own;
+            }
             u = max(1, (len + PD_UNIT - 1) / PD_UNIT);
+        }
+        if constexpr (MODE == PD_SEGMENTS) {                     // the places the same way
+            int y = places;
+#pragma unroll
+            for (int o = 1; o < 32; o <<= 1) {
+                const int z = __shfl_up_sync(0xffffffffu, y, o);
+                if (lane >= o) y += z;
+            }
+            __syncthreads();
+            if (lane == 31) warp_sum[warp] = y;
+            __syncthreads();
+            int sum = 0;
+            for (int w = 0; w < S::WARPS; ++w) {
+                if (w == warp) y += sum;
+                sum += warp_sum[w];
+            }
+            if (i < n_seqs) s_shares[i + 1] = before_places + y;
+            before_places += sum;
         }
         int x = u;
 #pragma unroll
@@ -223,15 +290,26 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             if (w == warp) x += sum;
             sum += warp_sum[w];
         }
-        if (i < A.n) pre[i + 1] = before + x;
+        if (i < n_seqs) pre[i + 1] = before + x;
         before += sum;
     }
+    if constexpr (MODE == PD_SEGMENTS) {
+        __syncthreads();
+        bool fits = true;                                        // a sum that passed 32 bits shows as one that falls
+        for (int i = threadIdx.x; i < n_seqs; i += S::THREADS) fits &= s_shares[i + 1] >= s_shares[i] && pre[i + 1] >= pre[i];
+        if (!__syncthreads_and(fits)) {
+            if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+            return;
+        }
+        if (n_seqs == 0) return;
+    }
     __syncthreads();
-    PdPlan W;
+    PdPlan<MODE> W;
     W.pre = pre;
-    W.n = A.n;
+    W.shares = s_shares;
+    W.n = n_seqs;
     W.hg = P.Hkv * A.groups;
-    const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
+    const int64_t work = MODE == PD_SEGMENTS ? int64_t(s_shares[n_seqs]) : (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
     if (work > INT_MAX) {                                        // the host's launches hold less, but for one group of 2^31 units
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return;
@@ -250,32 +328,105 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         return false;
     };
 
+    // KV head and first row of a piece
+    auto head_of = [&](const PdPiece& p, int& row0) {
+        const int groups = MODE == PD_SEGMENTS ? W.heads(p.seq) / P.Hkv : A.groups;
+        const int h = MODE == PD_SEGMENTS ? p.vh / groups : pd_div(p.vh, A.by_groups);
+        row0 = A.row0 + (p.vh - h * groups) * S::ROWS;
+        return h;
+    };
+    // sequence, token and query head in its group of row r (segments: the rows of a member behind one another)
+    auto row_parts = [&](int seq, int r, int& tok, int& head) {
+        int of = seq;
+        if constexpr (MODE == PD_SEGMENTS) {
+            const int member = pd_div(r, A.by_rows);
+            r -= member * A.rep * A.Tq;
+            of = V.member(V.segment(seq), member);
+        }
+        tok = pd_div(r, A.by_rep);
+        head = r - tok * A.rep;
+        return of;
+    };
     auto row_at = [&](int seq, int h, int r) {
-        const int tok = pd_div(r, A.by_rep);
-        return (int64_t(seq) * A.Tq + tok) * A.Hq + h * A.rep + r - tok * A.rep;
+        int tok, head;
+        const int of = row_parts(seq, r, tok, head);
+        return (int64_t(of) * A.Tq + tok) * A.Hq + h * A.rep + head;
     };
     auto finite_ref = [](float m) { return m == -INFINITY ? 0.f : m; };
+    // Where a finished row goes: maximum `top`, sum, O and its factor `inv`, which becomes that of the whole row.  PD_OWN: the
+    // row's parts of its sequence's segments are joined in, weights sum 2^(top - the largest).
+    float wl[MODE == PD_OWN ? PS_LEVELS : 1];
+    int levels = 0;
+    auto weigh = [&](int seq, int64_t row, float& top, float& sum, float& inv) {
+        if constexpr (MODE == PD_OWN) {
+            levels = V.depth_of(A.seq0 + seq);
+            const int64_t at = row + int64_t(A.seq0) * A.Tq * A.Hq;
+            float m[PS_LEVELS], most = top;
+#pragma unroll
+            for (int k = 0; k < PS_LEVELS; ++k) {
+                m[k] = -INFINITY, wl[k] = 0.f;
+                if (k < levels) {
+                    const float2 ml = __ldcg(reinterpret_cast<const float2*>(A.level_ml) + k * A.rows + at);
+                    m[k] = ml.x, wl[k] = ml.y;
+                }
+                most = fmaxf(most, m[k]);
+            }
+            const float ref = most == -INFINITY ? 0.f : most;
+            const float mine = sum * ex2(top - ref);
+            float total = mine;
+#pragma unroll
+            for (int k = 0; k < PS_LEVELS; ++k) {
+                wl[k] *= ex2(m[k] - ref);
+                total += wl[k];
+            }
+            const float by = total > 0.f ? 1.f / total : (total == total ? 0.f : total);
+#pragma unroll
+            for (int k = 0; k < PS_LEVELS; ++k) wl[k] *= by;
+            inv *= mine * by;
+            top = most, sum = total;
+        }
+    };
     // 2^(mw - m) / l; rows that see nothing give 0, NaN stays
     auto scale_of = [&](float m, float mw, float sum) { return sum > 0.f ? ex2(mw - finite_ref(m)) / sum : (sum == sum ? 0.f : sum); };
-    auto store_pair = [&](int64_t row, int ch, float a, float b, float inv) {
-        *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a * inv, b * inv);
+    auto store_pair = [&](int seq, int64_t row, int ch, float a, float b, float inv) {
+        if constexpr (MODE == PD_SEGMENTS) {
+            *reinterpret_cast<float2*>(A.level_o + (V.segment(seq).level * A.rows + row) * D + ch) = float2{a * inv, b * inv};
+        } else if constexpr (MODE == PD_OWN) {
+            const float* from = A.level_o + (row + int64_t(A.seq0) * A.Tq * A.Hq) * D + ch;
+            a *= inv, b *= inv;
+#pragma unroll
+            for (int k = 0; k < PS_LEVELS; ++k)
+                if (k < levels) {
+                    const float2 o = __ldcg(reinterpret_cast<const float2*>(from + k * A.rows * D));
+                    a = __fmaf_rn(o.x, wl[k], a);
+                    b = __fmaf_rn(o.y, wl[k], b);
+                }
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a, b);
+        } else {
+            *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a * inv, b * inv);
+        }
     };
-    auto store_lse = [&](int64_t row, float top, float sum) {
-        if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+    auto store_lse = [&](int seq, int64_t row, float top, float sum) {
+        if constexpr (MODE == PD_SEGMENTS)
+            *reinterpret_cast<float2*>(A.level_ml + 2 * (V.segment(seq).level * A.rows + row)) = float2{top, sum};
+        else if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
     };
 
     // the query rows of a piece: lane (g, t) holds row g of 8, channels (D / 4) t ..
     const int g = lane >> 2, t = lane & 3;
     uint4 raw[NT][KS / 2];
     auto load_q = [&](const PdPiece& p) {
-        const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS;
+        int row0;
+        const int h = head_of(p, row0), rows = rows_of(p.seq);
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            const int r = row0 + 8 * x + g, tok = pd_div(r, A.by_rep);
+            const int r = row0 + 8 * x + g;
 #pragma unroll
             for (int i = 0; i < KS / 2; ++i) raw[x][i] = uint4{0, 0, 0, 0};
-            if (r < A.rep * A.Tq) {
-                const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r - tok * A.rep) * A.Tq + tok) * D + (D / 4) * t;
+            if (r < rows) {
+                int tok, head;
+                const int of = row_parts(p.seq, r, tok, head);
+                const T* q = static_cast<const T*>(A.q) + ((int64_t(of) * A.Hq + h * A.rep + head) * A.Tq + tok) * D + (D / 4) * t;
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) raw[x][i] = __ldg(reinterpret_cast<const uint4*>(q + 8 * i));
             }
@@ -297,12 +448,13 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
         const PdPiece p = pd_piece(W, u0 + warp + k * S::WARPS, u1);
-        const int h = pd_div(p.vh, A.by_groups), t0 = p.a * PD_UNIT, len = s_len[p.seq];
+        int row0;
+        const int h = head_of(p, row0), t0 = first_of(p.seq) + p.a * PD_UNIT, len = end_of(p.seq), slot = slot_of_seq(p.seq);
         x.off = t0 & (P.page - 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
-            const int id = P.table[int64_t(s_slot[p.seq]) * P.max_blocks + ((t0 + i * box) >> A.page_log2)];
+            const int id = MODE == PD_SEGMENTS && slot < 0 ? -1 : P.table[int64_t(slot) * P.max_blocks + ((t0 + i * box) >> A.page_log2)];
             if (id >= 0 && id < P.n_pages) x.row[i] = id * P.Hkv + h;
             else raise_status(KVB_DEV_BOUNDS);
         }
@@ -346,8 +498,9 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     {
         int first = 1, unit = 0;
         for (int cur = u0; cur < u1;) {
-            const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq];
-            const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
+            int row0;
+            const int h = head_of(p, row0), len = end_of(p.seq), start = first_of(p.seq);
+            const int nrows = min(rows_of(p.seq) - row0, S::ROWS);
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
             float lam[NT][2], bias[NT][2];                       // bias: -1152 sum q, what the codes' pattern adds
@@ -406,7 +559,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 const int src = unit & 31;
                 const float ks[2] = {__shfl_sync(0xffffffffu, sc_now.x, src), __shfl_sync(0xffffffffu, sc_now.y, src)};
                 const float lv[2] = {__shfl_sync(0xffffffffu, sc_now.z, src), __shfl_sync(0xffffffffu, sc_now.w, src)};
-                const int t0 = (p.a + k) * PD_UNIT;
+                const int t0 = start + (p.a + k) * PD_UNIT;
                 const uint8_t* kt = ring + st * S::STAGE;
                 const bool edge = t0 + PD_UNIT > len - A.Tq + 1;
                 // ---- S = K Q^T for the two halves of 16 tokens; past the sequence's end the codes are whatever the page
@@ -462,7 +615,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             // keys from this unit on that the row 2t + k sees
-                            const int lim = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1 - t0;
+                            int lim = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1 - t0;
+                            if constexpr (MODE == PD_SEGMENTS) { // by the member's own length; rows past the last see nothing new
+                                int tok, head;
+                                const int r = min(row0 + 8 * x + 2 * t + k, rows_of(p.seq) - 1), of = row_parts(p.seq, r, tok, head);
+                                lim = min(len, V.length_of(of, P) - A.Tq + tok + 1) - t0;
+                            }
 #pragma unroll
                             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -603,7 +761,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 const int r = row_of(x);
-                const int64_t row = whole ? row_at(p.seq, h, row0 + r) : 0;
+                const int64_t row = whole && (MODE != PD_SEGMENTS || r < nrows) ? row_at(p.seq, h, row0 + r) : 0;
                 float top = -INFINITY, topw = -INFINITY, sum = 0.f, inv = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
@@ -624,6 +782,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                             sum = __fmaf_rn(s_l[w][r], ex2(s_m[w][r] - ref), sum);
                         }
                         inv = scale_of(top, topw, sum);
+                        if (whole && r < nrows) weigh(p.seq, row, top, sum, inv);
                     }
                     float2 acc{0.f, 0.f};
 #pragma unroll
@@ -633,14 +792,14 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
                     if (whole) {
-                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, inv);
+                        if (r < nrows) store_pair(p.seq, row, channel_of(y), acc.x, acc.y, inv);
                     } else if (r < nrows) {
                         *reinterpret_cast<float2*>(part + 6 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
                 }
                 if (lane == 0 && r < nrows) {
                     if (whole) {
-                        if (ml == 0) store_lse(row, top, sum);
+                        if (ml == 0) store_lse(p.seq, row, top, sum);
                     } else {
                         part[3 * ml * S::ROWS + r] = top;
                         part[(3 * ml + 1) * S::ROWS + r] = sum;
@@ -729,11 +888,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     for (int x = 0; x < NT; ++x) {
                         if (row_of(x) >= nrows) continue;
                         const int64_t row = row_at(p.seq, h, row0 + row_of(x));
-                        const float inv = scale_of(top[x], topw[x], sum[x]);
+                        float inv = scale_of(top[x], topw[x], sum[x]);
+                        weigh(p.seq, row, top[x], sum[x], inv);
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y)
-                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
-                        if (lane == 0 && ml == 0) store_lse(row, top[x], sum[x]);
+                            if (!(few && y > 0)) store_pair(p.seq, row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
+                        if (lane == 0 && ml == 0) store_lse(p.seq, row, top[x], sum[x]);
                     }
                 }
             }

@@ -175,3 +175,49 @@ def compact(pool):
         pool["refs"][b], pool["refs"][a] = pool["refs"][a], 0
         pool["table"][pool["table"] == a] = b
     return n
+
+
+SHARE_LEVELS = 4
+
+
+def share(pool, slots, levels=SHARE_LEVELS):
+    """Which leading full pages the listed sequences hold in common: order, own, depth, segments (first place in order,
+    members, first token, end, level).  A class of two or more sequences that hold the same page behind the blocks they had in
+    common before gets a segment up to the last block that all its members hold in full; what is left of it is divided by the
+    next block's page, `levels` times at most.  Classes, and the order, go by their first member."""
+    n, page, n_pages = len(slots), pool["kc"].shape[2], len(pool["refs"])
+    full, rows = [], []
+    for s in slots:
+        ok = 0 <= s < len(pool["lens"])
+        ids = [int(x) for x in pool["table"][s]] if ok else []
+        k = min(max(int(pool["lens"][s]), 0) // page, len(ids)) if ok else 0
+        bad = [b for b in range(k) if not 0 <= ids[b] < n_pages]
+        full.append(bad[0] if bad else k)
+        rows.append(ids)
+    own, depth, found = [0] * n, [0] * n, []
+
+    def divide(members, at, level):
+        """Members in order of the list -> their order; segments as (level, first member's index, ...)."""
+        if level == levels:
+            return members
+        classes = {}
+        for i in members:
+            classes.setdefault(rows[i][at] if at < full[i] else ("alone", i), []).append(i)
+        order = []
+        for group in sorted(classes.values()):
+            if len(group) == 1:
+                order += group
+                continue
+            end = at
+            while all(end < full[i] and rows[i][end] == rows[group[0]][end] for i in group):
+                end += 1
+            for i in group:
+                own[i], depth[i] = end * page, level + 1
+            found.append((level, group[0], len(group), at * page, end * page))
+            order += divide(group, end, level + 1)
+        return order
+
+    order = divide(list(range(n)), 0, 0)
+    place = {i: p for p, i in enumerate(order)}
+    segments = [[place[f], m, a, e, level] for level, f, m, a, e in sorted(found, key=lambda x: (x[0], place[x[1]]))]
+    return dict(order=order, own=own, depth=depth, segments=segments)

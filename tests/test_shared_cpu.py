@@ -1,0 +1,69 @@
+"""Refusals of the C entry points for shared pages, checked on the host before any CUDA call."""
+
+import ctypes as C
+
+import pytest
+
+A, B = 4096, 1 << 30        # stand-ins for aligned device addresses: never read
+
+
+def pages(**kw):
+    from kvb import _lib
+    f = dict(kc=A, vc=A, ks=A, vs=A, table=A, lens=A, refs=A, n_pages=10, Hkv=2, d=128, page=64, n_slots=4, max_blocks=8)
+    f.update(kw)
+    return _lib.Pages(*[f[n] for n, _ in _lib.Pages._fields_])
+
+
+def call(name, *args):
+    from kvb import _lib
+    lib = _lib.lib()
+    st = getattr(lib, name)(*args)
+    return st, lib.kvb_last_error().decode()
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(slots=None), 1, "null"), (dict(plan=None), 1, "null"), (dict(n=-1), 1, "n <="), (dict(n=1025), 1, "n <=")])
+def test_share(change, status, word):
+    a = dict(slots=A, n=3, plan=A, stream=None)
+    a.update(change)
+    st, msg = call("kvb_page_share", C.byref(pages()), *a.values())
+    assert st == status and word in msg and "page_share" in msg, (st, msg)
+
+
+@pytest.mark.parametrize("pool,change,status,word", [
+    ({}, dict(q=None), 1, "null"), ({}, dict(plan=None), 1, "null"), ({}, dict(slots=None), 1, "null"), ({}, dict(workspace=None), 1, "null"),
+    ({}, dict(Hq=3), 1, "Hq"), ({}, dict(Tq=0), 1, "Tq"), ({}, dict(dtype=0), 4, "float16"), ({}, dict(n=-1), 1, "n >="),
+    ({}, dict(n=1025), 1, "n <="), ({}, dict(q=A + 8), 1, "alignment"), ({}, dict(out=A + 2), 1, "alignment"),
+    ({}, dict(scaling=float("inf")), 1, "finite"), ({}, dict(workspace_bytes=64), 1, "workspace"), ({}, dict(workspace=A + 16), 1, "workspace"),
+    (dict(max_blocks=1 << 20), dict(n=1000, Hq=64, Tq=8), 4, "too many"), (dict(page=48), {}, 4, "pages"), (dict(d=96), {}, 4, "d 64")])
+def test_attend_shared(pool, change, status, word):
+    a = dict(q=A, dtype=1, Hq=4, Tq=1, slots=A, n=3, plan=A, scaling=0.1, out=A, lse=None, workspace=A, workspace_bytes=B, stream=None)
+    a.update(change)
+    st, msg = call("kvb_page_attend_shared", C.byref(pages(**pool)), *a.values())
+    assert st == status and word in msg and "page_attend_shared" in msg, (st, msg)
+
+
+def test_sizes():
+    from kvb import _lib
+    f = _lib.lib().kvb_page_attend_shared_workspace
+    p = C.byref(pages())
+    one = _lib.lib().kvb_page_attend_workspace(p, 1, 4, 1)
+    assert f(p, 1, 4, 1) >= one and f(p, 3, 4, 2) >= one + 2 * 3 * 8 * 130 * 4 and f(p, 100, 4, 1) >= one + 4 * 400 * 130 * 4
+    assert f(p, 1025, 4, 1) == f(p, -1, 4, 1) == f(p, 3, 0, 1) == f(C.byref(pages(d=96)), 3, 4, 1) == 0
+
+
+def test_oracle_finds_what_forks_share():
+    """Hand-made rows: two levels, a sequence that ends inside a page, one that shares nothing."""
+    from oracle import paged as O
+    pool = O.empty_pool(20, 1, 64, 16, 5, 6)
+    pool["table"][0, :5] = [3, 4, 5, 6, 7]
+    pool["table"][1, :5] = [3, 4, 5, 9, 10]
+    pool["table"][2, :5] = [1, 2, 5, 6, 7]
+    pool["table"][3, :5] = [3, 4, 8, 11, 12]
+    pool["table"][4, :3] = [3, 4, 5]
+    pool["lens"][:] = [80, 75, 80, 80, 47]
+    s = O.share(pool, [2, 0, 3, 4, 1])
+    assert s["order"] == [0, 1, 4, 2, 3]
+    assert s["segments"] == [[1, 4, 0, 32, 0], [1, 2, 32, 48, 1]]
+    assert s["own"] == [0, 48, 32, 32, 48] and s["depth"] == [0, 2, 1, 1, 2]
+    assert O.share(pool, [2])["own"] == [0]
