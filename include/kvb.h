@@ -485,6 +485,20 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
                                  int64_t v_row, int64_t v_head, const int32_t* cu_q, const int32_t* cu_k, int n,
                                  float scaling, void* out, float* lse, void* workspace, size_t workspace_bytes, void* stream);
 
+/* Attention of packed queries to keys of another length (an encoder's states), grouped heads, no causal mask: sequence s
+ * has the query rows [cu_q[s], cu_q[s + 1]) and sees all of the key rows [cu_k[s], cu_k[s + 1]), which may be none (zeros and -inf).
+ * q (nq, Hq, d), k and v (nk, Hkv, d) of one dtype (f16 / bf16) with d in {64, 128} contiguous, 16-byte aligned, the element
+ * strides below multiples of 8 (a head stride of 0: one head for all; key rows have to lie apart); cu_q, cu_k (n + 1) int32 on
+ * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 16-byte aligned; lse (nq, Hq) float32 (natural log) or
+ * null.  Rows of no sequence are not written.  Offsets that do not fit the rows raise status bit 1 and their sequences are left
+ * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
+ * (every call leaves its counters at zero), one per stream that runs calls concurrently. */
+size_t kvb_cross_workspace(int d);
+kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
+                               int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                               const int32_t* cu_q, const int32_t* cu_k, int n, float scaling, void* out, float* lse,
+                               void* workspace, size_t workspace_bytes, void* stream);
+
 /* A pool of pages of `page` (16, 32, 64 or 128) tokens, device tensors, dense: codes kc, vc (n_pages, Hkv,
  * page, d) uint8 (16-byte aligned) and scales ks, vs (n_pages, Hkv) float32, a stored value being
  * (code - 128) * scale; table (n_slots, max_blocks) int32, the pages of each sequence (slot), -1 past its

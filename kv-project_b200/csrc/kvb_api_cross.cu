@@ -1,0 +1,107 @@
+// kvb_api_cross.cu - kvb_cross_attention (include/kvb.h): validation, tensor maps and launch of the attention of packed
+// queries to keys of another length (kvb_cross.cuh).
+#include "kvb_paged_host.cuh"
+#include "kvb_cross.cuh"
+
+namespace {
+
+constexpr size_t kCrossCounts = size_t(kvb::PD_MAX_CTAS) * kvb::CR_WARPS * 4;
+
+// Rows (nk, heads, d) with their strides as (d, heads, rows), box 64 channels x 1 x `rows`, 128-byte swizzle.  A head stride of
+// zero (one head for all) is a map of one head.
+kvb_status cross_map(CUtensorMap* m, const void* x, const void* other, int dtype, int d, int64_t nk, int Hkv, int64_t row, int64_t head, int rows) {
+    EncodeTiledFn fn = encode_tiled();
+    if (!fn) return fail(KVB_ECUDA, "cross_attention: cuTensorMapEncodeTiled unavailable");
+    const int heads = Hkv > 1 && head > 0 ? Hkv : 1;
+    const cuuint64_t dims[3] = {cuuint64_t(d), cuuint64_t(heads), cuuint64_t(std::max<int64_t>(nk, 1))};
+    const cuuint64_t strides[2] = {cuuint64_t(heads > 1 ? head : d) * 2, cuuint64_t(nk > 1 ? row : d) * 2};
+    const cuuint32_t box[3] = {64, 1, cuuint32_t(rows)}, estr[3] = {1, 1, 1};
+    const CUresult r = fn(m, dtype == KVB_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                          const_cast<void*>(nk ? x : other), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    return r == CUDA_SUCCESS ? KVB_OK : fail(KVB_EUNSUPPORTED, "cross_attention: no tensor map for keys or values of these strides");
+}
+
+template <typename T, int D>
+kvb_status launch_few(kvb::CrossParams a, cudaStream_t s) {
+    constexpr int SM = kvb::CrShape<D>::SMEM;
+    const auto kern = kvb::cross_few_kernel<T, D>;
+    static std::atomic<uint64_t> done{0};
+    if (kvb_status st = kvbh::allow_smem("cross_attention", reinterpret_cast<const void*>(kern), SM, done)) return st;
+    const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
+    const int n = a.n;
+    for (int i = 0; i < n; i += kvb::CR_MAX_SEQS) {
+        a.n = std::min(n - i, kvb::CR_MAX_SEQS);
+        if (kvb_status st = launch_chained("cross_attention", kern, grid, 32 * kvb::CR_WARPS, SM, s, a)) return st;
+        a.cu_q += kvb::CR_MAX_SEQS;
+        a.cu_k += kvb::CR_MAX_SEQS;
+    }
+    return KVB_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t kvb_cross_workspace(int d) {
+    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * kvb::PD_MAX_CTAS * kvb::CR_ROWS * (d + 2) * 4 : 0;
+}
+
+kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
+                               int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
+                               const int32_t* cu_q, const int32_t* cu_k, int n, float scaling, void* out, float* lse,
+                               void* workspace, size_t workspace_bytes, void* stream) {
+    if (n < 0 || nq < 0 || nk < 0 || nq > INT32_MAX - 65536 || nk > INT32_MAX - 65536)
+        return fail(KVB_EINVAL, "cross_attention: n >= 0 and row counts in [0, 2^31 - 2^16]");
+    if (Hkv <= 0 || Hq <= 0 || Hq % Hkv != 0 || Hq > 65535)
+        return fail(KVB_EINVAL, "cross_attention: Hq a multiple of Hkv, at most 65535");
+    if (dtype != KVB_F16 && dtype != KVB_BF16) return fail(KVB_EUNSUPPORTED, "cross_attention: float16 or bfloat16");
+    if (d != 64 && d != 128) return fail(KVB_EUNSUPPORTED, "cross_attention: d 64 or 128");
+    if (!std::isfinite(scaling)) return fail(KVB_EINVAL, "cross_attention: scaling must be finite");
+    if (n == 0 || nq == 0) return KVB_OK;
+    if (!q || (!k && nk) || (!v && nk) || !cu_q || !cu_k || !out || !workspace) return fail(KVB_EINVAL, "cross_attention: null argument");
+    // strides of an extent of one address nothing
+    if (nq == 1) q_row = 0;
+    if (Hq == 1) q_head = 0;
+    if (nk <= 1) k_row = v_row = 0;
+    if (Hkv == 1) k_head = v_head = 0;
+    for (int64_t st : {q_row, q_head, k_row, k_head, v_row, v_head})
+        if (st < 0 || st % 8 != 0 || st >= int64_t(1) << 38) return fail(KVB_EINVAL, "cross_attention: row and head strides multiples of 8 elements");
+    if (nk > 1 && (k_row == 0 || v_row == 0)) return fail(KVB_EUNSUPPORTED, "cross_attention: key and value rows of their own (row strides above 0)");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4))
+        return fail(KVB_EINVAL, "cross_attention: q, k, v and out need 16-byte alignment, lse 4-byte");
+    if (workspace_bytes < kvb_cross_workspace(d) || !aligned(workspace, 256))
+        return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
+    kvb::CrossParams a{};
+    a.rep = Hq / Hkv;
+    // units of a sequence times row groups of all fit 32 bits
+    const int64_t units = nk / (2048 / d) + 2 + kvb::PD_FIXED, groups = (nq * a.rep + kvb::CR_ROWS - 1) / kvb::CR_ROWS + n;
+    if (units > INT32_MAX / Hkv / groups) return fail(KVB_EUNSUPPORTED, "cross_attention: query rows times keys too many for one call");
+    if (kvb_status st = cross_map(&a.tm_k, k, q, dtype, d, nk, Hkv, k_row, k_head, 2048 / d)) return st;
+    if (kvb_status st = cross_map(&a.tm_v, v, q, dtype, d, nk, Hkv, v_row, v_head, 2048 / d)) return st;
+    a.q = q;
+    a.q_row = q_row;
+    a.q_head = q_head;
+    a.cu_q = cu_q;
+    a.cu_k = cu_k;
+    a.nq = nq;
+    a.nk = nk;
+    a.n = n;
+    a.Hq = Hq;
+    a.Hkv = Hkv;
+    a.k_heads = k_head > 0;
+    a.v_heads = v_head > 0;
+    a.by_rep = kvbh::reciprocal(a.rep);
+    a.lam = scaling * 1.44269504088896340736f;
+    a.out = out;
+    a.lse = lse;
+    a.count = static_cast<uint32_t*>(workspace);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCrossCounts);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    if (dtype == KVB_BF16) return d == 128 ? launch_few<__nv_bfloat16, 128>(a, s) : launch_few<__nv_bfloat16, 64>(a, s);
+    return d == 128 ? launch_few<__half, 128>(a, s) : launch_few<__half, 64>(a, s);
+}
+
+}  // extern "C"
+
+KVB_STATUS_WORDS(status_words_cross)

@@ -86,13 +86,15 @@ kvb_status status_words_pages(unsigned*, unsigned*, int, int, cudaStream_t);
 kvb_status status_words_paged(unsigned*, unsigned*, int, int, cudaStream_t);
 kvb_status status_words_prefill(unsigned*, unsigned*, int, int, cudaStream_t);
 kvb_status status_words_shared(unsigned*, unsigned*, int, int, cudaStream_t);
+kvb_status status_words_cross(unsigned*, unsigned*, int, int, cudaStream_t);
 inline const StatusWordsFn* status_word_files(int* n) {
     static const StatusWordsFn fns[] = {status_words_api,          status_words_spectral,     status_words_decode,
                                         status_words_main_token,   status_words_main_channel, status_words_main_midrise,
                                         status_words_main_xchg,    status_words_decode_tc,    status_words_alloc,
                                         status_words_quasar,       status_words_atoms,        status_words_coverage,
                                         status_words_lctc,         status_words_pages,        status_words_paged,
-                                        status_words_prefill,      status_words_shared};
+                                        status_words_prefill,      status_words_shared,
+                                        status_words_cross};
     *n = int(sizeof(fns) / sizeof(fns[0]));
     return fns;
 }

@@ -108,7 +108,7 @@ struct PdPlan {
         return MODE == PD_SEGMENTS ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / PD_FIXED : hg;
     }
     __device__ __forceinline__ int units(int i) const {
-        return MODE == PD_SEGMENTS ? (pre[i + 1] - pre[i]) / heads(i) : pre[i + 1] - pre[i];
+        return MODE == PD_SEGMENTS ? (pre[i + 1] - pre[i]) / max(heads(i), 1) : pre[i + 1] - pre[i];
     }
     __device__ __forceinline__ int share(int c) const { return c * quota + min(c, extra); }
     __device__ __forceinline__ int holder(int v) const {

@@ -13,8 +13,8 @@ from .ops import (PackedCache, quant_pack, key_energy, rank_split, query_scores,
                   device_status, overlap_previous, UNIFORM_STEP)
 from .state import KvbStrataState, KvbCodedState, tier_as_kvb  # noqa: F401
 from .coverage import coverage_groups, coverage_stats  # noqa: F401
-from .paged import PagePool, SharedPages, prefill_attention  # noqa: F401
+from .paged import PagePool, SharedPages, cross_attention, prefill_attention  # noqa: F401
 
 __all__ = ["ops", "cache", "workloads", "state", "seqsplit", "codebooks", "PackedCache", "quant_pack", "key_energy", "rank_split",
            "query_scores", "snapkv_scores", "decode", "decode_plan", "device_status", "overlap_previous", "UNIFORM_STEP",
-           "KvbStrataState", "KvbCodedState", "tier_as_kvb", "coverage", "coverage_groups", "coverage_stats", "lctc", "paged", "PagePool", "SharedPages", "prefill_attention"]
+           "KvbStrataState", "KvbCodedState", "tier_as_kvb", "coverage", "coverage_groups", "coverage_stats", "lctc", "paged", "PagePool", "SharedPages", "cross_attention", "prefill_attention"]

@@ -107,6 +107,9 @@ SIGNATURES = {
     "kvb_prefill_attention": (_i32, [_p, _p, _p, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
                                      _p, _p, _i32, _f32, _p, _p, _p, C.c_size_t, _p]),
     "kvb_prefill_workspace": (C.c_size_t, [_i32]),
+    "kvb_cross_attention": (_i32, [_p, _p, _p, _i32, _i64, _i64, _i32, _i32, _i32, _i64, _i64, _i64, _i64, _i64, _i64,
+                                   _p, _p, _i32, _f32, _p, _p, _p, C.c_size_t, _p]),
+    "kvb_cross_workspace": (C.c_size_t, [_i32]),
     "kvb_page_extend": (_i32, [_p, _p, _p, _i32, _p, _p]),
     "kvb_page_write": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _i32, _i64, _i64, _i64, _i64, _i64, _p]),
     "kvb_page_read": (_i32, [_p, _p, _p, _p, _i32, _p, _p, _i32, _i64, _p]),

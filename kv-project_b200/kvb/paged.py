@@ -2,6 +2,8 @@
 
   prefill_attention   attention of whole prompts packed without padding, or of chunks after their prefixes
                       (chunked_attention over a prompt, STRATA_KV.py:641-675)
+  cross_attention     attention of packed queries to keys of another length (an encoder's states), from single tokens to
+                      whole prompts
   PagePool            keys and values of growing sequences in 8-bit pages (one scale per page, KV head and
                       side): extend, write, attend, read, fork, free, compact, copy_pages; share and attend_shared for
                       batches whose sequences hold pages in common.  It stands where the reference's per-sequence
@@ -56,6 +58,14 @@ def _not_capturing(who: str):
     """A workspace's zeros would only be written when the graph is replayed."""
     if torch.cuda.is_current_stream_capturing():
         raise NotImplementedError(f"{who}: the first call on a stream makes a workspace, which a stream capture cannot")
+
+
+def _capture_workspace(size: int, zeroed: int, device) -> torch.Tensor:
+    """A workspace inside a stream capture, from the graph's own memory: two graphs never share one, and its counters are
+    zeroed by each replay."""
+    ws = torch.empty(size, dtype=torch.uint8, device=device)
+    ws[:zeroed].zero_()
+    return ws
 
 
 _PREFILL_WS = {}
@@ -118,12 +128,61 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
     return (out, lse) if return_lse else out
 
 
-def _capture_workspace(size: int, zeroed: int, device) -> torch.Tensor:
-    """A workspace inside a stream capture, from the graph's own memory: two graphs never share one, and its counters are
-    zeroed by each replay."""
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
-    ws[:zeroed].zero_()
+_CROSS_WS = {}
+
+
+def _cross_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
+    """The zero-filled workspace of one stream (4 MB at d 128)."""
+    if torch._C._cuda_isCurrentStreamCapturing():
+        size = lib.kvb_cross_workspace(d)
+        return _capture_workspace(size, size, device)
+    ws = _CROSS_WS.get((device.index, stream, d))
+    if ws is None:
+        ws = _CROSS_WS[(device.index, stream, d)] = torch.zeros(max(lib.kvb_cross_workspace(d), 256), dtype=torch.uint8, device=device)
     return ws
+
+
+def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
+                    scaling: float = None, out: torch.Tensor = None, return_lse: bool = False):
+    """Attention of packed queries to keys of another length (an encoder's states): q (Nq, Hq, d), k and v (Nk, Hkv, d)
+    float16 / bfloat16, any row and head strides of 16 bytes (d contiguous; an expanded head is read once); sequence s has the
+    query rows cu_q[s] .. cu_q[s + 1] - 1 and sees all of the key rows cu_k[s] .. cu_k[s + 1] - 1.  Query head a reads KV
+    head a // (Hq // Hkv).  scaling defaults to d ** -0.5.  Returns out (Nq, Hq, d), with return_lse also the log-sum-exp (Nq,
+    Hq) float32; rows of a sequence without keys are zeros and -inf, rows of no sequence are not written."""
+    if _elsewhere(q.get_device()):
+        with torch.cuda.device(q.get_device()):
+            return cross_attention(q, k, v, cu_q, cu_k, scaling, out, return_lse)
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[2] != k.shape[2]:
+        raise ValueError("cross_attention: q (Nq, Hq, d), k and v (Nk, Hkv, d)")
+    if not q.is_cuda:
+        raise ValueError("kvb: tensors must live on a CUDA device")
+    index = q.get_device()
+    _check_on("cross_attention", index, k, v)
+    if not (q.dtype == k.dtype == v.dtype):
+        raise ValueError("cross_attention: q, k and v of one dtype")
+    nq, hq, d = q.shape
+    nk, hkv, _ = k.shape
+    n = cu_q.shape[0] - 1 if cu_q.dim() == 1 else -1
+    if n < 0:
+        raise ValueError("cross_attention: cu_q and cu_k hold n + 1 offsets each")
+    _check_ints("cross_attention", n + 1, index, cu_q, cu_k)
+    qs, ks, vs = q.stride(), k.stride(), v.stride()
+    if d > 1 and not qs[2] == ks[2] == vs[2] == 1:
+        raise ValueError("cross_attention: d must be contiguous")
+    if out is None:
+        out = _new((nq, hq, d), (hq * d, d, 1), dtype=q.dtype, device=q.device)
+    elif out.shape != q.shape or out.dtype != q.dtype or out.get_device() != index or not out.is_contiguous():
+        raise ValueError("cross_attention: out must be contiguous (Nq, Hq, d) in q's dtype and on its device")
+    lse = _new((nq, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
+    lib, stream = L.lib(), _raw_stream(index)
+    ws = _cross_workspace(lib, q.device, stream, d)
+    st = lib.kvb_cross_attention(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
+        vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
+        lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
+    if st:
+        L.check(st, "kvb_cross_attention")
+    return (out, lse) if return_lse else out
 
 
 class SharedPages:
