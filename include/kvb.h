@@ -491,8 +491,8 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
  * strides below multiples of 8 (a head stride of 0: one head for all; key rows have to lie apart); cu_q, cu_k (n + 1) int32 on
  * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 16-byte aligned; lse (nq, Hq) float32 (natural log) or
  * null.  Rows of no sequence are not written.  Offsets that do not fit the rows raise status bit 1 and their sequences are left
- * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): zero-filled once before its first use and then reused
- * (every call leaves its counters at zero), one per stream that runs calls concurrently. */
+ * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): its first 8192 bytes zero-filled once before its first use
+ * and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently. */
 size_t kvb_cross_workspace(int d);
 kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
                                int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,

@@ -1,9 +1,12 @@
 // kvb_api_cross.cu - kvb_cross_attention (include/kvb.h): validation, tensor maps and launch of the attention of packed
 // queries to keys of another length (kvb_cross.cuh).
 #include "kvb_paged_host.cuh"
-#include "kvb_cross.cuh"
+#include "kvb_cross_tc.cuh"
 
 namespace {
+
+// Query rows (tokens x heads of a KV head) of a sequence, on average, up to which cross_few_kernel is taken.
+constexpr int kFewRows = 64;
 
 constexpr size_t kCrossCounts = size_t(kvb::PD_MAX_CTAS) * kvb::CR_WARPS * 4;
 
@@ -22,21 +25,29 @@ kvb_status cross_map(CUtensorMap* m, const void* x, const void* other, int dtype
     return r == CUDA_SUCCESS ? KVB_OK : fail(KVB_EUNSUPPORTED, "cross_attention: no tensor map for keys or values of these strides");
 }
 
-template <typename T, int D>
-kvb_status launch_few(kvb::CrossParams a, cudaStream_t s) {
-    constexpr int SM = kvb::CrShape<D>::SMEM;
-    const auto kern = kvb::cross_few_kernel<T, D>;
+int cross_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
+
+template <typename T, int D, bool MANY>
+kvb_status launch(kvb::CrossParams a, cudaStream_t s) {
+    constexpr int SM = MANY ? kvb::CmShape<D>::SMEM : kvb::CrShape<D>::SMEM, THREADS = 32 * (MANY ? kvb::CM_WARPS : kvb::CR_WARPS);
+    const auto kern = MANY ? kvb::cross_many_kernel<T, D> : kvb::cross_few_kernel<T, D>;
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = kvbh::allow_smem("cross_attention", reinterpret_cast<const void*>(kern), SM, done)) return st;
-    const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
+    const unsigned grid = unsigned(cross_ctas());
     const int n = a.n;
     for (int i = 0; i < n; i += kvb::CR_MAX_SEQS) {
         a.n = std::min(n - i, kvb::CR_MAX_SEQS);
-        if (kvb_status st = launch_chained("cross_attention", kern, grid, 32 * kvb::CR_WARPS, SM, s, a)) return st;
+        if (kvb_status st = launch_chained("cross_attention", kern, grid, THREADS, SM, s, a)) return st;
         a.cu_q += kvb::CR_MAX_SEQS;
         a.cu_k += kvb::CR_MAX_SEQS;
     }
     return KVB_OK;
+}
+
+template <bool MANY>
+kvb_status launch_any(const kvb::CrossParams& a, int dtype, int d, cudaStream_t s) {
+    if (dtype == KVB_BF16) return d == 128 ? launch<__nv_bfloat16, 128, MANY>(a, s) : launch<__nv_bfloat16, 64, MANY>(a, s);
+    return d == 128 ? launch<__half, 128, MANY>(a, s) : launch<__half, 64, MANY>(a, s);
 }
 
 }  // namespace
@@ -44,7 +55,8 @@ kvb_status launch_few(kvb::CrossParams a, cudaStream_t s) {
 extern "C" {
 
 size_t kvb_cross_workspace(int d) {
-    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * kvb::PD_MAX_CTAS * kvb::CR_ROWS * (d + 2) * 4 : 0;
+    // two partials a CTA: of 2 x 128 rows (cross_many_kernel), of 16 (cross_few_kernel)
+    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * cross_ctas() * 2 * kvb::CM_ROWS * (d + 2) * 4 : 0;
 }
 
 kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
@@ -74,11 +86,14 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
         return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
     kvb::CrossParams a{};
     a.rep = Hq / Hkv;
+    const bool many = nq * a.rep > int64_t(kFewRows) * n;
+    const int keys = many ? kvb::CM_KEYS : 2048 / d, rows = many ? 2 * kvb::CM_ROWS : kvb::CR_ROWS;
     // units of a sequence times row groups of all fit 32 bits
-    const int64_t units = nk / (2048 / d) + 2 + kvb::PD_FIXED, groups = (nq * a.rep + kvb::CR_ROWS - 1) / kvb::CR_ROWS + n;
-    if (units > INT32_MAX / Hkv / groups) return fail(KVB_EUNSUPPORTED, "cross_attention: query rows times keys too many for one call");
-    if (kvb_status st = cross_map(&a.tm_k, k, q, dtype, d, nk, Hkv, k_row, k_head, 2048 / d)) return st;
-    if (kvb_status st = cross_map(&a.tm_v, v, q, dtype, d, nk, Hkv, v_row, v_head, 2048 / d)) return st;
+    const int64_t units = nk / keys + 2 + kvb::PD_FIXED, groups = (nq * a.rep + rows - 1) / rows + n;
+    if (nq * a.rep > INT32_MAX - 65536 || units > INT32_MAX / Hkv / groups)
+        return fail(KVB_EUNSUPPORTED, "cross_attention: query rows times keys too many for one call");
+    if (kvb_status st = cross_map(&a.tm_k, k, q, dtype, d, nk, Hkv, k_row, k_head, keys)) return st;
+    if (kvb_status st = cross_map(&a.tm_v, v, q, dtype, d, nk, Hkv, v_row, v_head, keys)) return st;
     a.q = q;
     a.q_row = q_row;
     a.q_head = q_head;
@@ -93,13 +108,15 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
     a.v_heads = v_head > 0;
     a.by_rep = kvbh::reciprocal(a.rep);
     a.lam = scaling * 1.44269504088896340736f;
+    a.negate = scaling < 0;
+    // a scaling of zero becomes one too small to matter, so that -inf stays -inf
+    if (many) a.lam = std::max(std::fabs(a.lam), 1e-37f);
     a.out = out;
     a.lse = lse;
     a.count = static_cast<uint32_t*>(workspace);
     a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCrossCounts);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (dtype == KVB_BF16) return d == 128 ? launch_few<__nv_bfloat16, 128>(a, s) : launch_few<__nv_bfloat16, 64>(a, s);
-    return d == 128 ? launch_few<__half, 128>(a, s) : launch_few<__half, 64>(a, s);
+    return many ? launch_any<true>(a, dtype, d, s) : launch_any<false>(a, dtype, d, s);
 }
 
 }  // extern "C"

@@ -36,10 +36,11 @@ struct CrossParams {
     int n, Hq, Hkv, rep;
     int k_heads, v_heads;                     // 0: all KV heads read head 0
     uint64_t by_rep;                          // for pd_div
-    float lam;
+    float lam;                                // scaling log2(e); cross_many_kernel: its magnitude, above 0
+    int negate;                               // cross_many_kernel: scaling < 0
     void* out;                                // (nq, Hq, d)
     float* lse;                               // (nq, Hq) or null
-    float* part;                              // [2 grid][16][d + 2]: O, maximum, sum
+    float* part;                              // two a CTA: O, maximum, sum
     uint32_t* count;                          // [grid][8 warps]
 };
 

@@ -95,7 +95,7 @@ struct PdShape {
 
 // The work of a call: per (sequence, KV head, row group) its units, and PD_FIXED more in the shares that the CTAs get
 // (preparing the queries and joining the warps costs about as much time as that many units).
-template <int MODE>
+template <int MODE, int FIXED = PD_FIXED>
 struct PdPlan {
     const int* pre;                           // [n + 1] units before each sequence, for one head and group (segments: for all)
     const int* shares;                        // segments: [n + 1] places before each
@@ -103,9 +103,9 @@ struct PdPlan {
     int quota, extra, ctas;                   // shares: the first `extra` CTAs get quota + 1
 
     __device__ __forceinline__ int unit0(int i) const { return MODE == PD_SEGMENTS ? pre[i] : pre[i] * hg; }
-    __device__ __forceinline__ int place0(int i) const { return MODE == PD_SEGMENTS ? shares[i] : (pre[i] + i * PD_FIXED) * hg; }
+    __device__ __forceinline__ int place0(int i) const { return MODE == PD_SEGMENTS ? shares[i] : (pre[i] + i * FIXED) * hg; }
     __device__ __forceinline__ int heads(int i) const {          // KV heads x groups of a sequence
-        return MODE == PD_SEGMENTS ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / PD_FIXED : hg;
+        return MODE == PD_SEGMENTS ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / FIXED : hg;
     }
     __device__ __forceinline__ int units(int i) const {
         return MODE == PD_SEGMENTS ? (pre[i + 1] - pre[i]) / max(heads(i), 1) : pre[i + 1] - pre[i];
@@ -123,8 +123,8 @@ struct PdPlan {
             if (place0(mid) <= v) lo = mid;
             else hi = mid;
         }
-        const int u = units(lo), local = v - place0(lo), vh = min(local / (u + PD_FIXED), heads(lo));
-        return unit0(lo) + vh * u + max(local - vh * (u + PD_FIXED) - PD_FIXED, 0);
+        const int u = units(lo), local = v - place0(lo), vh = min(local / (u + FIXED), heads(lo));
+        return unit0(lo) + vh * u + max(local - vh * (u + FIXED) - FIXED, 0);
     }
 };
 
@@ -134,8 +134,8 @@ struct PdPiece {
 };
 
 // The piece that begins at unit `cur` of all work.
-template <int MODE>
-__device__ __forceinline__ PdPiece pd_piece(const PdPlan<MODE>& W, int cur, int end) {
+template <int MODE, int FIXED>
+__device__ __forceinline__ PdPiece pd_piece(const PdPlan<MODE, FIXED>& W, int cur, int end) {
     int lo = 0, hi = W.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -149,7 +149,7 @@ __device__ __forceinline__ PdPiece pd_piece(const PdPlan<MODE>& W, int cur, int 
     p.vh = local / p.units;
     p.a = local - p.vh * p.units;
     p.b = min(p.units, p.a + (end - cur));
-    p.v0 = W.place0(lo) + p.vh * (p.units + PD_FIXED);
+    p.v0 = W.place0(lo) + p.vh * (p.units + FIXED);
     return p;
 }
 
