@@ -104,18 +104,69 @@ __device__ __forceinline__ void cm_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// 16 columns of the thread's lane; cm_wait_st() before anyone else reads them
-__device__ __forceinline__ void cm_st16(uint32_t taddr, const uint32_t (&r)[16]) {
+// The 128 columns of S of the thread's lane, waited for in the same statement: nothing reads the registers before
+__device__ __forceinline__ void cm_ld128(uint32_t taddr, float (&v)[128]) {
+    uint32_t r[128];
     asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
+        "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
+        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
+        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
+        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
+        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "tcgen05.wait::ld.sync.aligned;"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
+          "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]),
+          "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
+          "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
+          "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
+          "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]),
+          "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
+          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]),
+          "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]),
+          "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
+          "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
+          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+        : "r"(taddr)
+        : "memory");
+#pragma unroll
+    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+}
+// 32 columns of the thread's lane; cm_wait_st() before anyone else reads them
+__device__ __forceinline__ void cm_st32(uint32_t taddr, const uint32_t (&r)[32]) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
+        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
         "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]),
-        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+        "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]),
+        "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]),
+        "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
         : "memory");
 }
 __device__ __forceinline__ void cm_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+// two float32 values at once
+__device__ __forceinline__ float2 cm_fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, c, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 c, {%6, %7};\n\t"
+        "fma.rn.f32x2 d, a, b, c;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 cm_add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 a, b, d;\n\tmov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tadd.rn.f32x2 d, a, b;\n\tmov.b64 {%0, %1}, d;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
 struct CmBars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], s_full[2], p_ready[2], pv_done[2], drained[2];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], s_full[2], p_half[2], p_ready[2], pv_done[2], drained[2];
 };
 
 template <typename T, int D>
@@ -127,12 +178,12 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     __shared__ CmBars B;
     __shared__ int warp_sum[2][CM_WARPS];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_abort;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const sq = base;                                    // [2 tiles], then keys and values [stage]
     uint8_t* const sk = sq + 2 * S::TILE;
     uint8_t* const sv = sk + S::STAGES * S::TILE;
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    // the warp's number from a shuffle: the compiler then knows it, and what follows from it, to be the same in all lanes
+    const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
 
     if (threadIdx.x == 0) {
         for (int i = 0; i < 4; ++i) {
@@ -144,11 +195,11 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.q_full[i], 4);
             mbar_init(&B.s_full[i], 1);
+            mbar_init(&B.p_half[i], 4);
             mbar_init(&B.p_ready[i], 4);
             mbar_init(&B.pv_done[i], 1);
             mbar_init(&B.drained[i], 1);
         }
-        s_abort = 0;
         fence_mbar_init();
         pre[0] = shares[0] = 0;
     }
@@ -210,16 +261,8 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     __syncthreads();
     cm_after();
     const uint32_t tmem = s_tmem;
-    volatile int* abort = &s_abort;
-    // a whole warp's wait, the same answer in all lanes; false once any wait of the block has run out
-    auto wait = [&](uint64_t* bar, uint32_t count) {
-        bool ok = *abort == 0;
-        if (ok && !mbar_wait(bar, count & 1)) {
-            *abort = 1;
-            ok = false;
-        }
-        return bool(__all_sync(0xffffffffu, ok));
-    };
+    // a whole warp's wait, the same answer in all lanes; after one that ran out a role ends, and so does what waits for it
+    auto wait = [&](uint64_t* bar, uint32_t count) { return bool(__all_sync(0xffffffffu, mbar_wait(bar, count & 1))); };
     // the piece that begins at unit `cur`
     struct Item {
         PdPiece p;
@@ -259,6 +302,17 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             __syncwarp();
             if (lane == 0) mbar_arrive(&B.q_full[t]);
         };
+        auto rescale = [&](float f) {                            // O of the row times f
+#pragma unroll 1
+            for (int c = 0; c < D / 32; ++c) {
+                float v[32];
+                cm_ld32(to + 32 * c, v);
+                uint32_t w[32];
+#pragma unroll
+                for (int i = 0; i < 32; ++i) w[i] = __float_as_uint(v[i] * f);
+                cm_st32(to + 32 * c, w);
+            }
+        };
         auto has_work = [&](const Item& x) { return x.tiles > 0 && x.nrows > t * CM_ROWS; };
         Item x{};
         if (u0 < u1) {
@@ -276,66 +330,53 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     if (!(ok = wait(&B.s_full[t], sn))) break;
                     cm_after();
                     const int left = x.s.kl - (x.p.a + j) * CM_KEYS;             // keys of the sequence from this tile on
-                    float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                    float v[128];
+                    cm_ld128(ts, v);
+                    if (A.negate) {
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float v[32];
-                        cm_ld32(ts + 32 * c, v);
-                        if (A.negate) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = -v[i];
-                        }
-                        if (left >= 32 * c + 32) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) top[i & 3] = fmaxf(top[i & 3], 32 * c + i < left ? v[i] : -INFINITY);
-                        }
+                        for (int i = 0; i < 128; ++i) v[i] = -v[i];
                     }
+                    if (left < CM_KEYS) {
+#pragma unroll
+                        for (int i = 0; i < 128; ++i) v[i] = i < left ? v[i] : -INFINITY;
+                    }
+                    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                    for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
                     const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * A.lam;
                     const bool grow = y > m + PF_LAZY;
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? ex2(m - y) : 1.f;
                         if (grow) m = y;
                         l *= f;
-                        if (j > 0) {                             // the product before is done: S came after it
-#pragma unroll 1
-                            for (int c = 0; c < D / 32; ++c) {
-                                float v[32];
-                                cm_ld32(to + 32 * c, v);
-#pragma unroll
-                                for (int k = 0; k < 2; ++k) {
-                                    uint32_t w[16];
-#pragma unroll
-                                    for (int i = 0; i < 16; ++i) w[i] = __float_as_uint(v[16 * k + i] * f);
-                                    cm_st16(to + 32 * c + 16 * k, w);
-                                }
-                            }
-                        }
+                        if (j > 0) rescale(f);                   // the product before is done: S came after it
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
-                    float sum[4] = {0.f, 0.f, 0.f, 0.f};
+                    const float2 lam2{A.lam, A.lam}, ref2{-ref, -ref};
+                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) {                // P of 32 keys takes 16 columns, behind the S still to be read
-                        float v[32];
-                        cm_ld32(ts + 32 * c, v);
-                        const float lam = A.negate ? -A.lam : A.lam;
+                    for (int c = 0; c < 2; ++c) {                // 64 keys at a time: their product begins beside the others' weights
+                        uint32_t w[32];
 #pragma unroll
-                        for (int i = 0; i < 32; ++i) v[i] = ex2(__fmaf_rn(v[i], lam, -ref));
-                        if (left < 32 * c + 32) {
-#pragma unroll
-                            for (int i = 0; i < 32; ++i) v[i] = 32 * c + i < left ? v[i] : 0.f;
+                        for (int i = 0; i < 32; ++i) {
+                            const int k = 64 * c + 2 * i;
+                            float2 e = cm_fma2(float2{v[k], v[k + 1]}, lam2, ref2);
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                            sum[i & 1] = cm_add2(sum[i & 1], e);
+                            w[i] = pack_f32<T>(e.x, e.y);
                         }
-                        uint32_t w[16];
-#pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            sum[i & 3] += v[2 * i] + v[2 * i + 1];
-                            w[i] = pack_f32<T>(v[2 * i], v[2 * i + 1]);
+                        cm_st32(ts + 32 * c, w);
+                        if (c == 0) {
+                            cm_wait_st();
+                            cm_before();
+                            __syncwarp();
+                            if (lane == 0 && left >= CM_KEYS) mbar_arrive(&B.p_half[t]);
+                            __syncwarp();
                         }
-                        cm_st16(ts + 16 * c, w);
                     }
-                    l += (sum[0] + sum[1]) + (sum[2] + sum[3]);
+                    const float2 both = cm_add2(sum[0], sum[1]);
+                    l += both.x + both.y;
                     if (left < CM_KEYS) {                        // value rows past the end, up to the last step's 16
                         const uint32_t st = (it + j) % S::STAGES;
                         if (!(ok = wait(&B.v_full[st], (it + j) / S::STAGES))) break;
@@ -350,7 +391,10 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     cm_wait_st();
                     cm_before();
                     __syncwarp();
-                    if (lane == 0) mbar_arrive(&B.p_ready[t]);
+                    if (lane == 0) {
+                        if (left < CM_KEYS) mbar_arrive(&B.p_half[t]);
+                        mbar_arrive(&B.p_ready[t]);
+                    }
                 }
             }
             if (!ok) break;
@@ -458,42 +502,57 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         const uint64_t dq = cm_desc_k(smem_u32(sq + t * S::TILE)), dk = cm_desc_k(smem_u32(sk)), dv = cm_desc_mn(smem_u32(sv), S::HALF);
         uint32_t it = 0, sn = 0, items = 0;
         bool ok = true;
+        auto scores = [&](uint32_t st) {                         // S = Q K^T of the stage's keys
+            cm_after();
+            const uint64_t k = dk + uint64_t(st * (S::TILE >> 4));
+#pragma unroll
+            for (int c = 0; c < D / 16; ++c) {                   // descriptors count 16 bytes
+                const uint32_t off = (c >> 2) * (S::HALF >> 4) + (c & 3) * 2;
+                cm_mma_ss(lead, ts, dq + off, k + off, IS, c > 0);
+            }
+            cm_commit(lead, &B.s_full[t]);
+            cm_commit(lead, &B.k_empty[st]);
+        };
         for (int cur = u0; cur < u1 && ok;) {
             const Item x = item_at(cur);
-            const bool mine = x.nrows > t * CM_ROWS;
-            if (mine && x.tiles > 0) ok = wait(&B.q_full[t], items++);
-            for (int j = 0; j < x.tiles && ok; ++j, ++it) {
-                const uint32_t st = it % S::STAGES, use = it / S::STAGES;
-                if (!(ok = wait(&B.k_full[st], use))) break;
-                if (!mine) {                                     // nothing to multiply: the stage is free for this tile
-                    if (lane == 0) mbar_arrive(&B.k_empty[st]);
-                    if (!(ok = wait(&B.v_full[st], use))) break;
-                    if (lane == 0) mbar_arrive(&B.v_empty[st]);
-                    continue;
+            const int tiles = __shfl_sync(0xffffffffu, x.tiles, 0), left = __shfl_sync(0xffffffffu, x.s.kl - x.p.a * CM_KEYS, 0);
+            if (__shfl_sync(0xffffffffu, x.nrows, 0) <= t * CM_ROWS) {
+                // nothing to multiply: the stages are free for this tile
+                for (int j = 0; j < tiles && ok; ++j, ++it) {
+                    const uint32_t st = it % S::STAGES, use = it / S::STAGES;
+                    ok = wait(&B.k_full[st], use);
+                    if (ok && lane == 0) mbar_arrive(&B.k_empty[st]);
+                    ok = ok && wait(&B.v_full[st], use);
+                    if (ok && lane == 0) mbar_arrive(&B.v_empty[st]);
                 }
-                if (sn > 0 && !(ok = wait(&B.pv_done[t], sn - 1))) break;        // P before is read: S may take its columns
-                cm_after();
-                const uint64_t k = dk + uint64_t(st * (S::TILE >> 4));
+            } else if (tiles > 0) {
+                // the queries have come, and the product before, which reads the weights in S's columns, is done
+                ok = wait(&B.q_full[t], items++) && wait(&B.k_full[it % S::STAGES], it / S::STAGES) && (sn == 0 || wait(&B.pv_done[t], sn - 1));
+                if (ok) scores(it % S::STAGES);
+                for (int j = 0; j < tiles && ok; ++j, ++it, ++sn) {
+                    const uint32_t st = it % S::STAGES, use = it / S::STAGES, nst = (it + 1) % S::STAGES, nuse = (it + 1) / S::STAGES;
+                    const uint64_t v = dv + uint64_t(st * (S::TILE >> 4));
+                    const int steps = min((left - j * CM_KEYS + 15) / 16, CM_KEYS / 16);
+                    if (!(ok = wait(&B.v_full[st], use) && wait(&B.p_half[t], sn))) break;
+                    cm_after();
 #pragma unroll
-                for (int c = 0; c < D / 16; ++c) {               // descriptors count 16 bytes
-                    const uint32_t off = (c >> 2) * (S::HALF >> 4) + (c & 3) * 2;
-                    cm_mma_ss(lead, ts, dq + off, k + off, IS, c > 0);
+                    for (int c = 0; c < CM_KEYS / 32; ++c)
+                        if (c < steps) cm_mma_ts(lead, to, ts + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, j > 0 || c > 0);
+                    const bool more = j + 1 < tiles;
+                    if (!(ok = (!more || wait(&B.k_full[nst], nuse)) && wait(&B.p_ready[t], sn))) break;
+                    cm_after();
+#pragma unroll
+                    for (int c = CM_KEYS / 32; c < CM_KEYS / 16; ++c)
+                        if (c < steps) cm_mma_ts(lead, to, ts + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, 1);
+                    cm_commit(lead, &B.pv_done[t]);
+                    cm_commit(lead, &B.v_empty[st]);
+                    if (more) {
+                        if (!(ok = wait(&B.pv_done[t], sn))) break;
+                        scores(nst);
+                    }
                 }
-                cm_commit(lead, &B.s_full[t]);
-                cm_commit(lead, &B.k_empty[st]);
-                if (!(ok = wait(&B.p_ready[t], sn))) break;
-                if (!(ok = wait(&B.v_full[st], use))) break;
-                cm_after();
-                const uint64_t v = dv + uint64_t(st * (S::TILE >> 4));
-                const int steps = min((x.s.kl - (x.p.a + j) * CM_KEYS + 15) / 16, CM_KEYS / 16);
-#pragma unroll
-                for (int c = 0; c < CM_KEYS / 16; ++c)
-                    if (c < steps) cm_mma_ts(lead, to, ts + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, j > 0 || c > 0);
-                cm_commit(lead, &B.pv_done[t]);
-                cm_commit(lead, &B.v_empty[st]);
-                ++sn;
             }
-            cur += x.p.b - x.p.a;
+            cur += __shfl_sync(0xffffffffu, x.p.b - x.p.a, 0);
         }
         if (!ok) {                                               // products in flight end before tensor memory is freed
             cm_commit(lead, &B.drained[t]);
