@@ -6,16 +6,16 @@
 //
 // One persistent CTA per SM.  A work item is a group of 256 query rows (row = token * rep + head in the group: the rep query
 // heads of a KV head and the sequence's queries packed together) of one (sequence, KV head), a unit of work its product with
-// 128 keys; every CTA takes an equal run of units, found from the offsets inside the kernel, so that any mixture of lengths is
+// 64 keys; every CTA takes an equal run of units, found from the offsets inside the kernel, so that any mixture of lengths is
 // balanced.  Items that a run's end cuts leave partial sums in the workspace, and the last warp to arrive joins them in the
 // order of the keys.
 //
 // The 256 rows are two tiles of 128, each with a warpgroup for its softmax (a thread a row) and a warp that issues its
-// products, so that one tile's softmax runs beside the other's products; both read the same key and value tiles, which one warp
-// copies with TMA through rings.  Tensor memory: S of the two tiles (128 columns each), O (128 each); P is rounded to the
-// inputs' type and takes the columns of its S, from where it is the A operand of P V.  A tile's products wait for one
-// another by barrier (S after the P V before it, which reads what S overwrites): the instruction set orders products of one
-// accumulator only.  O is rescaled only when a row's maximum grew by more than 2^8.
+// products, so that one tile's softmax runs beside the other's products; both read the same keys and values, which one warp
+// copies with TMA through rings.  Tensor memory: two S of 64 columns for each tile, O (128 columns each); P is rounded to the
+// inputs' type and takes the columns of its S, from where it is the A operand of P V.  While a tile's softmax works on one S,
+// the next is computed into the other columns, once the P V that reads the weights there is done (by barrier: the instruction
+// set orders products of one accumulator only).  O is rescaled only when a row's maximum grew by more than 2^8.
 //
 // Every aligned instruction (tensor memory loads, stores, allocation) is executed by whole warps: decisions before them are
 // votes, and loops over lanes' own conditions end in __syncwarp.  Waits are bounded; after one that ran out nothing is issued any
@@ -33,19 +33,19 @@
 namespace kvb {
 
 constexpr int CM_ROWS = 128;                  // of a tile
-constexpr int CM_KEYS = 128;                  // of a unit
+constexpr int CM_KEYS = 64;                   // of a unit
 constexpr int CM_SOFTMAX = 8;                 // warps
 constexpr int CM_WARPS = CM_SOFTMAX + 3;      // and an issuer per tile, and the copying warp
-constexpr int CM_FIXED = 2;                   // what an item costs beside its units, in units
+constexpr int CM_FIXED = 4;                   // what an item costs beside its units, in units
 constexpr int CM_TMEM = 512;
 
 template <int D>
 struct CmShape {
     static constexpr int HALVES = D / 64;
-    static constexpr int HALF = 128 * 128;                      // bytes of 64 channels of 128 rows
-    static constexpr int TILE = HALVES * HALF;
-    static constexpr int STAGES = 4 / HALVES;                   // of keys and of values
-    static constexpr int SMEM = 1024 + 2 * TILE + 2 * STAGES * TILE;
+    static constexpr int QHALF = CM_ROWS * 128, HALF = CM_KEYS * 128;           // bytes of 64 channels of a tile's queries, of a unit's keys
+    static constexpr int QTILE = HALVES * QHALF, TILE = HALVES * HALF;
+    static constexpr int STAGES = 4;                            // of keys and of values
+    static constexpr int SMEM = 1024 + 2 * QTILE + 2 * STAGES * TILE;
     static constexpr int PART = 2 * (D + 2) * CM_ROWS;          // floats: O by column and row, maximum, sum of the two tiles
 };
 
@@ -62,26 +62,26 @@ __host__ __device__ constexpr uint32_t cm_idesc(int N, int bf16, int b_mn) {
     return (1u << 4) | (uint32_t(bf16) << 7) | (uint32_t(bf16) << 10) | (uint32_t(b_mn) << 16) | (uint32_t(N >> 3) << 17) |
            (uint32_t(128 >> 4) << 24);
 }
-// issued by the lane whose `lead` is set, from a converged warp (from a branch of one lane a product takes half as long again)
-__device__ __forceinline__ void cm_mma_ss(uint32_t lead, uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
+// Issued by one lane of a converged warp, the same every time.  (With the lane's own predicate a product takes 64 cycles to
+// issue, from a branch of one lane more; elected, 64 x 64 x 16 and smaller ones go at their own rate.)
+__device__ __forceinline__ void cm_mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-        "l"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void cm_mma_ts(uint32_t lead, uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
+__device__ __forceinline__ void cm_mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, int acc) {
     asm volatile(
-        "{\n\t.reg .pred p, q;\n\tsetp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 q, %5, 0;\n\t"
-        "@q tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-        "r"(a), "l"(b), "r"(idesc), "r"(acc), "r"(lead)
+        "{\n\t.reg .pred p, e;\n\tsetp.ne.b32 p, %4, 0;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(acc)
         : "memory");
 }
-__device__ __forceinline__ void cm_commit(uint32_t lead, uint64_t* bar) {
+__device__ __forceinline__ void cm_commit(uint64_t* bar) {
     asm volatile(
-        "{\n\t.reg .pred q;\n\tsetp.ne.b32 q, %1, 0;\n\t"
-        "@q tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar)),
-        "r"(lead)
+        "{\n\t.reg .pred e;\n\telect.sync _|e, 0xffffffff;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(smem_u32(bar))
         : "memory");
 }
 
@@ -104,18 +104,14 @@ __device__ __forceinline__ void cm_ld32(uint32_t taddr, float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
 }
-// The 128 columns of S of the thread's lane, waited for in the same statement: nothing reads the registers before
-__device__ __forceinline__ void cm_ld128(uint32_t taddr, float (&v)[128]) {
-    uint32_t r[128];
+// The 64 columns of S of the thread's lane, waited for in the same statement: nothing reads the registers before
+__device__ __forceinline__ void cm_ld64(uint32_t taddr, float (&v)[64]) {
+    uint32_t r[64];
     asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x128.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
+        "tcgen05.ld.sync.aligned.32x32b.x64.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
         "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,"
         "%32,%33,%34,%35,%36,%37,%38,%39,%40,%41,%42,%43,%44,%45,%46,%47,"
-        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63,"
-        "%64,%65,%66,%67,%68,%69,%70,%71,%72,%73,%74,%75,%76,%77,%78,%79,"
-        "%80,%81,%82,%83,%84,%85,%86,%87,%88,%89,%90,%91,%92,%93,%94,%95,"
-        "%96,%97,%98,%99,%100,%101,%102,%103,%104,%105,%106,%107,%108,%109,%110,%111,"
-        "%112,%113,%114,%115,%116,%117,%118,%119,%120,%121,%122,%123,%124,%125,%126,%127}, [%128];\n\t"
+        "%48,%49,%50,%51,%52,%53,%54,%55,%56,%57,%58,%59,%60,%61,%62,%63}, [%64];\n\t"
         "tcgen05.wait::ld.sync.aligned;"
         : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
           "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]),
@@ -123,17 +119,11 @@ __device__ __forceinline__ void cm_ld128(uint32_t taddr, float (&v)[128]) {
           "=r"(r[30]), "=r"(r[31]), "=r"(r[32]), "=r"(r[33]), "=r"(r[34]), "=r"(r[35]), "=r"(r[36]), "=r"(r[37]), "=r"(r[38]), "=r"(r[39]),
           "=r"(r[40]), "=r"(r[41]), "=r"(r[42]), "=r"(r[43]), "=r"(r[44]), "=r"(r[45]), "=r"(r[46]), "=r"(r[47]), "=r"(r[48]), "=r"(r[49]),
           "=r"(r[50]), "=r"(r[51]), "=r"(r[52]), "=r"(r[53]), "=r"(r[54]), "=r"(r[55]), "=r"(r[56]), "=r"(r[57]), "=r"(r[58]), "=r"(r[59]),
-          "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63]), "=r"(r[64]), "=r"(r[65]), "=r"(r[66]), "=r"(r[67]), "=r"(r[68]), "=r"(r[69]),
-          "=r"(r[70]), "=r"(r[71]), "=r"(r[72]), "=r"(r[73]), "=r"(r[74]), "=r"(r[75]), "=r"(r[76]), "=r"(r[77]), "=r"(r[78]), "=r"(r[79]),
-          "=r"(r[80]), "=r"(r[81]), "=r"(r[82]), "=r"(r[83]), "=r"(r[84]), "=r"(r[85]), "=r"(r[86]), "=r"(r[87]), "=r"(r[88]), "=r"(r[89]),
-          "=r"(r[90]), "=r"(r[91]), "=r"(r[92]), "=r"(r[93]), "=r"(r[94]), "=r"(r[95]), "=r"(r[96]), "=r"(r[97]), "=r"(r[98]), "=r"(r[99]),
-          "=r"(r[100]), "=r"(r[101]), "=r"(r[102]), "=r"(r[103]), "=r"(r[104]), "=r"(r[105]), "=r"(r[106]), "=r"(r[107]), "=r"(r[108]), "=r"(r[109]),
-          "=r"(r[110]), "=r"(r[111]), "=r"(r[112]), "=r"(r[113]), "=r"(r[114]), "=r"(r[115]), "=r"(r[116]), "=r"(r[117]), "=r"(r[118]), "=r"(r[119]),
-          "=r"(r[120]), "=r"(r[121]), "=r"(r[122]), "=r"(r[123]), "=r"(r[124]), "=r"(r[125]), "=r"(r[126]), "=r"(r[127])
+          "=r"(r[60]), "=r"(r[61]), "=r"(r[62]), "=r"(r[63])
         : "r"(taddr)
         : "memory");
 #pragma unroll
-    for (int i = 0; i < 128; ++i) v[i] = __uint_as_float(r[i]);
+    for (int i = 0; i < 64; ++i) v[i] = __uint_as_float(r[i]);
 }
 // 32 columns of the thread's lane; cm_wait_st() before anyone else reads them
 __device__ __forceinline__ void cm_st32(uint32_t taddr, const uint32_t (&r)[32]) {
@@ -166,7 +156,8 @@ __device__ __forceinline__ float2 cm_add2(float2 a, float2 b) {
 }
 
 struct CmBars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], s_full[2], p_half[2], p_ready[2], pv_done[2], drained[2];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], drained[2];
+    uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];         // of a tile, by the half of its columns
 };
 
 template <typename T, int D>
@@ -180,7 +171,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     __shared__ uint32_t s_tmem;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const sq = base;                                    // [2 tiles], then keys and values [stage]
-    uint8_t* const sk = sq + 2 * S::TILE;
+    uint8_t* const sk = sq + 2 * S::QTILE;
     uint8_t* const sv = sk + S::STAGES * S::TILE;
     // the warp's number from a shuffle: the compiler then knows it, and what follows from it, to be the same in all lanes
     const int warp = __shfl_sync(0xffffffffu, int(threadIdx.x >> 5), 0), lane = threadIdx.x & 31;
@@ -194,11 +185,12 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.q_full[i], 4);
-            mbar_init(&B.s_full[i], 1);
-            mbar_init(&B.p_half[i], 4);
-            mbar_init(&B.p_ready[i], 4);
-            mbar_init(&B.pv_done[i], 1);
             mbar_init(&B.drained[i], 1);
+            for (int k = 0; k < 2; ++k) {
+                mbar_init(&B.s_full[i][k], 1);
+                mbar_init(&B.p_ready[i][k], 4);
+                mbar_init(&B.pv_done[i][k], 1);
+            }
         }
         fence_mbar_init();
         pre[0] = shares[0] = 0;
@@ -296,7 +288,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (int64_t(x.s.q0) + tok) * A.q_row +
                                                               int64_t(x.h * A.rep + at - tok * A.rep) * A.q_head + 8 * c));
                 }
-                *reinterpret_cast<uint4*>(sq + t * S::TILE + (c >> 3) * S::HALF + row * 128 + (((c ^ row) & 7) * 16)) = v;
+                *reinterpret_cast<uint4*>(sq + t * S::QTILE + (c >> 3) * S::QHALF + row * 128 + (((c ^ row) & 7) * 16)) = v;
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -327,54 +319,48 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             float m = -INFINITY, l = 0.f;
             if (mine) {
                 for (int j = 0; j < x.tiles; ++j, ++sn) {
-                    if (!(ok = wait(&B.s_full[t], sn))) break;
+                    const uint32_t half = sn & 1, cols = ts + CM_KEYS * half;
+                    if (!(ok = wait(&B.s_full[t][half], sn >> 1))) break;
                     cm_after();
-                    const int left = x.s.kl - (x.p.a + j) * CM_KEYS;             // keys of the sequence from this tile on
-                    float v[128];
-                    cm_ld128(ts, v);
+                    const int left = x.s.kl - (x.p.a + j) * CM_KEYS;             // keys of the sequence from this unit on
+                    float v[CM_KEYS];
+                    cm_ld64(cols, v);
                     if (A.negate) {
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) v[i] = -v[i];
+                        for (int i = 0; i < CM_KEYS; ++i) v[i] = -v[i];
                     }
                     if (left < CM_KEYS) {
 #pragma unroll
-                        for (int i = 0; i < 128; ++i) v[i] = i < left ? v[i] : -INFINITY;
+                        for (int i = 0; i < CM_KEYS; ++i) v[i] = i < left ? v[i] : -INFINITY;
                     }
                     float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 4; i < 128; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
+                    for (int i = 4; i < CM_KEYS; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
                     const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * A.lam;
                     const bool grow = y > m + PF_LAZY;
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? ex2(m - y) : 1.f;
                         if (grow) m = y;
                         l *= f;
-                        if (j > 0) rescale(f);                   // the product before is done: S came after it
+                        if (j > 0) {                             // once the product before is done
+                            if (!(ok = wait(&B.pv_done[t][half ^ 1], (sn - 1) >> 1))) break;
+                            cm_after();
+                            rescale(f);
+                        }
                     }
                     const float ref = m == -INFINITY ? 0.f : m;
                     const float2 lam2{A.lam, A.lam}, ref2{-ref, -ref};
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                    uint32_t w[CM_KEYS / 2];
 #pragma unroll
-                    for (int c = 0; c < 2; ++c) {                // 64 keys at a time: their product begins beside the others' weights
-                        uint32_t w[32];
-#pragma unroll
-                        for (int i = 0; i < 32; ++i) {
-                            const int k = 64 * c + 2 * i;
-                            float2 e = cm_fma2(float2{v[k], v[k + 1]}, lam2, ref2);
-                            e.x = ex2(e.x);
-                            e.y = ex2(e.y);
-                            sum[i & 1] = cm_add2(sum[i & 1], e);
-                            w[i] = pack_f32<T>(e.x, e.y);
-                        }
-                        cm_st32(ts + 32 * c, w);
-                        if (c == 0) {
-                            cm_wait_st();
-                            cm_before();
-                            __syncwarp();
-                            if (lane == 0 && left >= CM_KEYS) mbar_arrive(&B.p_half[t]);
-                            __syncwarp();
-                        }
+                    for (int i = 0; i < CM_KEYS / 2; ++i) {
+                        float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                        e.x = ex2(e.x);
+                        e.y = ex2(e.y);
+                        sum[i & 1] = cm_add2(sum[i & 1], e);
+                        w[i] = pack_f32<T>(e.x, e.y);
                     }
+                    cm_st32(cols, w);
                     const float2 both = cm_add2(sum[0], sum[1]);
                     l += both.x + both.y;
                     if (left < CM_KEYS) {                        // value rows past the end, up to the last step's 16
@@ -391,10 +377,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     cm_wait_st();
                     cm_before();
                     __syncwarp();
-                    if (lane == 0) {
-                        if (left < CM_KEYS) mbar_arrive(&B.p_half[t]);
-                        mbar_arrive(&B.p_ready[t]);
-                    }
+                    if (lane == 0) mbar_arrive(&B.p_ready[t][half]);
                 }
             }
             if (!ok) break;
@@ -406,7 +389,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                 if (has_work(x)) load_q(x);
             }
             if (mine) {
-                if (done.tiles > 0 && !(ok = wait(&B.pv_done[t], sn - 1))) break;            // nothing is written
+                if (done.tiles > 0 && !(ok = wait(&B.pv_done[t][(sn - 1) & 1], (sn - 1) >> 1))) break;     // nothing is written
                 cm_after();
                 const bool whole = done.p.a == 0 && done.p.b == done.p.units;
                 const bool row_ok = t * CM_ROWS + r < done.nrows;
@@ -497,21 +480,24 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     } else if (warp < CM_SOFTMAX + 2) {
         // ---------------- products of tile t ----------------
         const int t = warp - CM_SOFTMAX;
-        const uint32_t lead = lane == 0, ts = tmem + t * 128, to = tmem + 256 + t * 128;
+        const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
         constexpr uint32_t IS = cm_idesc(CM_KEYS, BF16, 0), IO = cm_idesc(D, BF16, 1);
-        const uint64_t dq = cm_desc_k(smem_u32(sq + t * S::TILE)), dk = cm_desc_k(smem_u32(sk)), dv = cm_desc_mn(smem_u32(sv), S::HALF);
-        uint32_t it = 0, sn = 0, items = 0;
+        const uint64_t dq = cm_desc_k(smem_u32(sq + t * S::QTILE)), dk = cm_desc_k(smem_u32(sk)), dv = cm_desc_mn(smem_u32(sv), S::HALF);
+        uint32_t it = 0, sn = 0, items = 0;                      // units of the block, S of this tile, items of this tile
         bool ok = true;
-        auto scores = [&](uint32_t st) {                         // S = Q K^T of the stage's keys
+        // S number n = Q K^T of unit u's keys, once the product two before, which reads the weights in S's columns, is done
+        auto scores = [&](uint32_t n, uint32_t u) {
+            const uint32_t st = u % S::STAGES;
+            if (!wait(&B.k_full[st], u / S::STAGES) || (n >= 2 && !wait(&B.pv_done[t][n & 1], (n >> 1) - 1))) return false;
             cm_after();
             const uint64_t k = dk + uint64_t(st * (S::TILE >> 4));
 #pragma unroll
-            for (int c = 0; c < D / 16; ++c) {                   // descriptors count 16 bytes
-                const uint32_t off = (c >> 2) * (S::HALF >> 4) + (c & 3) * 2;
-                cm_mma_ss(lead, ts, dq + off, k + off, IS, c > 0);
-            }
-            cm_commit(lead, &B.s_full[t]);
-            cm_commit(lead, &B.k_empty[st]);
+            for (int c = 0; c < D / 16; ++c)                     // descriptors count 16 bytes
+                cm_mma_ss(ts + CM_KEYS * (n & 1), dq + uint64_t((c >> 2) * (S::QHALF >> 4) + (c & 3) * 2),
+                          k + uint64_t((c >> 2) * (S::HALF >> 4) + (c & 3) * 2), IS, c > 0);
+            cm_commit(&B.s_full[t][n & 1]);
+            cm_commit(&B.k_empty[st]);
+            return true;
         };
         for (int cur = u0; cur < u1 && ok;) {
             const Item x = item_at(cur);
@@ -526,36 +512,25 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     if (ok && lane == 0) mbar_arrive(&B.v_empty[st]);
                 }
             } else if (tiles > 0) {
-                // the queries have come, and the product before, which reads the weights in S's columns, is done
-                ok = wait(&B.q_full[t], items++) && wait(&B.k_full[it % S::STAGES], it / S::STAGES) && (sn == 0 || wait(&B.pv_done[t], sn - 1));
-                if (ok) scores(it % S::STAGES);
+                ok = wait(&B.q_full[t], items++) && scores(sn, it) && (tiles < 2 || scores(sn + 1, it + 1));
                 for (int j = 0; j < tiles && ok; ++j, ++it, ++sn) {
-                    const uint32_t st = it % S::STAGES, use = it / S::STAGES, nst = (it + 1) % S::STAGES, nuse = (it + 1) / S::STAGES;
+                    const uint32_t st = it % S::STAGES, p = ts + CM_KEYS * (sn & 1);
                     const uint64_t v = dv + uint64_t(st * (S::TILE >> 4));
                     const int steps = min((left - j * CM_KEYS + 15) / 16, CM_KEYS / 16);
-                    if (!(ok = wait(&B.v_full[st], use) && wait(&B.p_half[t], sn))) break;
+                    if (!(ok = wait(&B.v_full[st], it / S::STAGES) && wait(&B.p_ready[t][sn & 1], sn >> 1))) break;
                     cm_after();
 #pragma unroll
-                    for (int c = 0; c < CM_KEYS / 32; ++c)
-                        if (c < steps) cm_mma_ts(lead, to, ts + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, j > 0 || c > 0);
-                    const bool more = j + 1 < tiles;
-                    if (!(ok = (!more || wait(&B.k_full[nst], nuse)) && wait(&B.p_ready[t], sn))) break;
-                    cm_after();
-#pragma unroll
-                    for (int c = CM_KEYS / 32; c < CM_KEYS / 16; ++c)
-                        if (c < steps) cm_mma_ts(lead, to, ts + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, 1);
-                    cm_commit(lead, &B.pv_done[t]);
-                    cm_commit(lead, &B.v_empty[st]);
-                    if (more) {
-                        if (!(ok = wait(&B.pv_done[t], sn))) break;
-                        scores(nst);
-                    }
+                    for (int c = 0; c < CM_KEYS / 16; ++c)
+                        if (c < steps) cm_mma_ts(to, p + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, j > 0 || c > 0);
+                    cm_commit(&B.pv_done[t][sn & 1]);
+                    cm_commit(&B.v_empty[st]);
+                    if (j + 2 < tiles) ok = scores(sn + 2, it + 2);
                 }
             }
             cur += __shfl_sync(0xffffffffu, x.p.b - x.p.a, 0);
         }
         if (!ok) {                                               // products in flight end before tensor memory is freed
-            cm_commit(lead, &B.drained[t]);
+            cm_commit(&B.drained[t]);
             mbar_wait(&B.drained[t], 0, 10000000ull);
         }
         __syncwarp();
