@@ -80,8 +80,8 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
     for (int64_t st : {q_row, q_head, k_row, k_head, v_row, v_head})
         if (st < 0 || st % 8 != 0 || st >= int64_t(1) << 38) return fail(KVB_EINVAL, "cross_attention: row and head strides multiples of 8 elements");
     if (nk > 1 && (k_row == 0 || v_row == 0)) return fail(KVB_EUNSUPPORTED, "cross_attention: key and value rows of their own (row strides above 0)");
-    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 16) || !aligned(lse, 4))
-        return fail(KVB_EINVAL, "cross_attention: q, k, v and out need 16-byte alignment, lse 4-byte");
+    if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 32) || !aligned(lse, 4))
+        return fail(KVB_EINVAL, "cross_attention: q, k and v need 16-byte alignment, out 32-byte, lse 4-byte");
     if (workspace_bytes < kvb_cross_workspace(d) || !aligned(workspace, 256))
         return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
     kvb::CrossParams a{};

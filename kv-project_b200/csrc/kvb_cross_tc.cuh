@@ -10,8 +10,8 @@
 // balanced.  Items that a run's end cuts leave partial sums in the workspace, and the last warp to arrive joins them in the
 // order of the keys.
 //
-// The 256 rows are two tiles of 128, each with a warpgroup for its softmax (a thread a row) and a warp that issues its
-// products, so that one tile's softmax runs beside the other's products; both read the same keys and values, which one warp
+// The 256 rows are two tiles of 128, each with a warpgroup for its softmax (a thread a row) and a warp that issues O += P V;
+// S of both in turn comes from another, so that one tile's softmax runs beside the other's products; both read the same keys and values, which one warp
 // copies with TMA through rings.  Tensor memory: two S of 64 columns for each tile, O (128 columns each); P is rounded to the
 // inputs' type and takes the columns of its S, from where it is the A operand of P V.  While a tile's softmax works on one S,
 // the next is computed into the other columns, once the P V that reads the weights there is done (by barrier: the instruction
@@ -35,8 +35,8 @@ namespace kvb {
 constexpr int CM_ROWS = 128;                  // of a tile
 constexpr int CM_KEYS = 64;                   // of a unit
 constexpr int CM_SOFTMAX = 8;                 // warps
-constexpr int CM_WARPS = CM_SOFTMAX + 3;      // and an issuer per tile, and the copying warp
-constexpr int CM_FIXED = 4;                   // what an item costs beside its units, in units
+constexpr int CM_WARPS = CM_SOFTMAX + 4;      // and one that issues S, one per tile that issues O, and the copying warp
+constexpr int CM_FIXED = 10;                  // what an item costs beside its units, in units
 constexpr int CM_TMEM = 512;
 
 template <int D>
@@ -155,8 +155,15 @@ __device__ __forceinline__ float2 cm_add2(float2 a, float2 b) {
     return d;
 }
 
+// a whole sector
+__device__ __forceinline__ void cm_store32(void* to, const uint32_t (&w)[8]) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
+                 "r"(w[5]), "r"(w[6]), "r"(w[7])
+                 : "memory");
+}
+
 struct CmBars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], drained[2];
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], drained[3];
     uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];         // of a tile, by the half of its columns
 };
 
@@ -180,18 +187,18 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         for (int i = 0; i < 4; ++i) {
             mbar_init(&B.k_full[i], 1);
             mbar_init(&B.v_full[i], 1);
-            mbar_init(&B.k_empty[i], 2);
+            mbar_init(&B.k_empty[i], 1);
             mbar_init(&B.v_empty[i], 2);
         }
         for (int i = 0; i < 2; ++i) {
             mbar_init(&B.q_full[i], 4);
-            mbar_init(&B.drained[i], 1);
             for (int k = 0; k < 2; ++k) {
                 mbar_init(&B.s_full[i][k], 1);
                 mbar_init(&B.p_ready[i][k], 4);
                 mbar_init(&B.pv_done[i][k], 1);
             }
         }
+        for (int i = 0; i < 3; ++i) mbar_init(&B.drained[i], 1);
         fence_mbar_init();
         pre[0] = shares[0] = 0;
     }
@@ -279,16 +286,20 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         const uint32_t lanes = uint32_t(quarter * 32) << 16, ts = tmem + lanes + t * 128, to = tmem + lanes + 256 + t * 128;
         auto load_q = [&](const Item& x) {                       // the warp's 32 rows of the tile, swizzled; zeros past the last
             constexpr int CHUNKS = D / 8, PER = 32 / CHUNKS;     // 16-byte chunks of a row, rows at a time
-#pragma unroll 4
+            const int c = lane % CHUNKS;
+            uint4 v[32 / PER];
+#pragma unroll
             for (int i = 0; i < 32 / PER; ++i) {
-                const int row = quarter * 32 + i * PER + lane / CHUNKS, c = lane % CHUNKS, at = x.row0 + t * CM_ROWS + row;
-                uint4 v{0, 0, 0, 0};
-                if (t * CM_ROWS + row < x.nrows) {
-                    const int tok = pd_div(at, A.by_rep);
-                    v = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (int64_t(x.s.q0) + tok) * A.q_row +
-                                                              int64_t(x.h * A.rep + at - tok * A.rep) * A.q_head + 8 * c));
-                }
-                *reinterpret_cast<uint4*>(sq + t * S::QTILE + (c >> 3) * S::QHALF + row * 128 + (((c ^ row) & 7) * 16)) = v;
+                const int row = t * CM_ROWS + quarter * 32 + i * PER + lane / CHUNKS, at = x.row0 + row, tok = pd_div(at, A.by_rep);
+                v[i] = uint4{0, 0, 0, 0};
+                if (row < x.nrows)
+                    v[i] = __ldg(reinterpret_cast<const uint4*>(static_cast<const T*>(A.q) + (int64_t(x.s.q0) + tok) * A.q_row +
+                                                                 int64_t(x.h * A.rep + at - tok * A.rep) * A.q_head + 8 * c));
+            }
+#pragma unroll
+            for (int i = 0; i < 32 / PER; ++i) {
+                const int row = quarter * 32 + i * PER + lane / CHUNKS;
+                *reinterpret_cast<uint4*>(sq + t * S::QTILE + (c >> 3) * S::QHALF + row * 128 + (((c ^ row) & 7) * 16)) = v[i];
             }
             fence_proxy_async_smem();
             __syncwarp();
@@ -397,11 +408,14 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                 const int64_t row = (int64_t(done.s.q0) + tok) * A.Hq + done.h * A.rep + at - tok * A.rep;
                 auto store = [&](int c, const float (&v)[32], float inv) {       // 32 channels of the row
                     if (!row_ok) return;
-                    uint4* to = reinterpret_cast<uint4*>(static_cast<T*>(A.out) + row * D + 32 * c);
+                    T* to = static_cast<T*>(A.out) + row * D + 32 * c;
 #pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        to[i] = uint4{pack_f32<T>(v[8 * i] * inv, v[8 * i + 1] * inv), pack_f32<T>(v[8 * i + 2] * inv, v[8 * i + 3] * inv),
-                                      pack_f32<T>(v[8 * i + 4] * inv, v[8 * i + 5] * inv), pack_f32<T>(v[8 * i + 6] * inv, v[8 * i + 7] * inv)};
+                    for (int i = 0; i < 2; ++i) {
+                        uint32_t w[8];
+#pragma unroll
+                        for (int k = 0; k < 8; ++k) w[k] = pack_f32<T>(v[16 * i + 2 * k] * inv, v[16 * i + 2 * k + 1] * inv);
+                        cm_store32(to + 16 * i, w);
+                    }
                 };
                 auto finish = [&](float top, float sum) {
                     if (A.lse && row_ok) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
@@ -477,61 +491,68 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             cur = next;
             first = 0;
         }
-    } else if (warp < CM_SOFTMAX + 2) {
-        // ---------------- products of tile t ----------------
-        const int t = warp - CM_SOFTMAX;
-        const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
+    } else if (warp < CM_SOFTMAX + 3) {
+        // ---------------- products: S = Q K^T of both tiles in turn from one warp, O += P V of each from another ----------------
+        const int role = warp - CM_SOFTMAX;
         constexpr uint32_t IS = cm_idesc(CM_KEYS, BF16, 0), IO = cm_idesc(D, BF16, 1);
-        const uint64_t dq = cm_desc_k(smem_u32(sq + t * S::QTILE)), dk = cm_desc_k(smem_u32(sk)), dv = cm_desc_mn(smem_u32(sv), S::HALF);
-        uint32_t it = 0, sn = 0, items = 0;                      // units of the block, S of this tile, items of this tile
+        uint32_t it = 0, sn[2] = {0, 0}, items[2] = {0, 0};      // units of the block; S and items of the tiles
         bool ok = true;
-        // S number n = Q K^T of unit u's keys, once the product two before, which reads the weights in S's columns, is done
-        auto scores = [&](uint32_t n, uint32_t u) {
-            const uint32_t st = u % S::STAGES;
-            if (!wait(&B.k_full[st], u / S::STAGES) || (n >= 2 && !wait(&B.pv_done[t][n & 1], (n >> 1) - 1))) return false;
-            cm_after();
-            const uint64_t k = dk + uint64_t(st * (S::TILE >> 4));
-#pragma unroll
-            for (int c = 0; c < D / 16; ++c)                     // descriptors count 16 bytes
-                cm_mma_ss(ts + CM_KEYS * (n & 1), dq + uint64_t((c >> 2) * (S::QHALF >> 4) + (c & 3) * 2),
-                          k + uint64_t((c >> 2) * (S::HALF >> 4) + (c & 3) * 2), IS, c > 0);
-            cm_commit(&B.s_full[t][n & 1]);
-            cm_commit(&B.k_empty[st]);
-            return true;
-        };
         for (int cur = u0; cur < u1 && ok;) {
             const Item x = item_at(cur);
             const int tiles = __shfl_sync(0xffffffffu, x.tiles, 0), left = __shfl_sync(0xffffffffu, x.s.kl - x.p.a * CM_KEYS, 0);
-            if (__shfl_sync(0xffffffffu, x.nrows, 0) <= t * CM_ROWS) {
-                // nothing to multiply: the stages are free for this tile
+            const bool both = __shfl_sync(0xffffffffu, x.nrows, 0) > CM_ROWS;
+            if (role == 0) {
+                const uint64_t dq = cm_desc_k(smem_u32(sq)), dk = cm_desc_k(smem_u32(sk));
+                if (tiles > 0) ok = wait(&B.q_full[0], items[0]++) && (!both || wait(&B.q_full[1], items[1]++));
                 for (int j = 0; j < tiles && ok; ++j, ++it) {
-                    const uint32_t st = it % S::STAGES, use = it / S::STAGES;
-                    ok = wait(&B.k_full[st], use);
-                    if (ok && lane == 0) mbar_arrive(&B.k_empty[st]);
-                    ok = ok && wait(&B.v_full[st], use);
-                    if (ok && lane == 0) mbar_arrive(&B.v_empty[st]);
+                    const uint32_t st = it % S::STAGES;
+                    const uint64_t k = dk + uint64_t(st * (S::TILE >> 4));
+                    ok = wait(&B.k_full[st], it / S::STAGES);
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        if (!ok || (t == 1 && !both)) break;
+                        const uint32_t half = sn[t] & 1;
+                        // the product two before, which reads the weights in these columns, is done
+                        if (sn[t] >= 2 && !(ok = wait(&B.pv_done[t][half], (sn[t] >> 1) - 1))) break;
+                        cm_after();
+#pragma unroll
+                        for (int c = 0; c < D / 16; ++c)         // descriptors count 16 bytes
+                            cm_mma_ss(tmem + t * 128 + CM_KEYS * half, dq + uint64_t(t * (S::QTILE >> 4) + (c >> 2) * (S::QHALF >> 4) + (c & 3) * 2),
+                                      k + uint64_t((c >> 2) * (S::HALF >> 4) + (c & 3) * 2), IS, c > 0);
+                        cm_commit(&B.s_full[t][half]);
+                        ++sn[t];
+                    }
+                    if (ok) cm_commit(&B.k_empty[st]);
                 }
-            } else if (tiles > 0) {
-                ok = wait(&B.q_full[t], items++) && scores(sn, it) && (tiles < 2 || scores(sn + 1, it + 1));
-                for (int j = 0; j < tiles && ok; ++j, ++it, ++sn) {
-                    const uint32_t st = it % S::STAGES, p = ts + CM_KEYS * (sn & 1);
+            } else {
+                const int t = role - 1;
+                const uint32_t ts = tmem + t * 128, to = tmem + 256 + t * 128;
+                const uint64_t dv = cm_desc_mn(smem_u32(sv), S::HALF);
+                for (int j = 0; j < tiles && ok; ++j, ++it) {
+                    const uint32_t st = it % S::STAGES, half = sn[0] & 1, p = ts + CM_KEYS * half;
                     const uint64_t v = dv + uint64_t(st * (S::TILE >> 4));
-                    const int steps = min((left - j * CM_KEYS + 15) / 16, CM_KEYS / 16);
-                    if (!(ok = wait(&B.v_full[st], it / S::STAGES) && wait(&B.p_ready[t][sn & 1], sn >> 1))) break;
+                    if (!(ok = wait(&B.v_full[st], it / S::STAGES))) break;
+                    if (t == 1 && !both) {                       // nothing to multiply: the stage is free for this tile
+                        if (lane == 0) mbar_arrive(&B.v_empty[st]);
+                        __syncwarp();
+                        continue;
+                    }
+                    if (!(ok = wait(&B.p_ready[t][half], sn[0] >> 1))) break;
                     cm_after();
+                    const int steps = min((left - j * CM_KEYS + 15) / 16, CM_KEYS / 16);
 #pragma unroll
                     for (int c = 0; c < CM_KEYS / 16; ++c)
                         if (c < steps) cm_mma_ts(to, p + 8 * c, v + uint64_t(c * (2048 >> 4)), IO, j > 0 || c > 0);
-                    cm_commit(&B.pv_done[t][sn & 1]);
+                    cm_commit(&B.pv_done[t][half]);
                     cm_commit(&B.v_empty[st]);
-                    if (j + 2 < tiles) ok = scores(sn + 2, it + 2);
+                    ++sn[0];
                 }
             }
             cur += __shfl_sync(0xffffffffu, x.p.b - x.p.a, 0);
         }
         if (!ok) {                                               // products in flight end before tensor memory is freed
-            cm_commit(&B.drained[t]);
-            mbar_wait(&B.drained[t], 0, 10000000ull);
+            cm_commit(&B.drained[role]);
+            mbar_wait(&B.drained[role], 0, 10000000ull);
         }
         __syncwarp();
     } else {
