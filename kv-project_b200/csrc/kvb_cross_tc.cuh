@@ -36,8 +36,9 @@ constexpr int CM_ROWS = 128;                  // of a tile
 constexpr int CM_KEYS = 64;                   // of a unit
 constexpr int CM_SOFTMAX = 8;                 // warps
 constexpr int CM_WARPS = CM_SOFTMAX + 4;      // and one that issues S, one per tile that issues O, and the copying warp
-constexpr int CM_FIXED = 10;                  // what an item costs beside its units, in units
+constexpr int CM_FIXED = 6;                   // what an item costs beside its units, in units
 constexpr int CM_TMEM = 512;
+constexpr int CM_FMA = 1;                     // pairs of keys of four whose weights take the FMA pipe
 
 template <int D>
 struct CmShape {
@@ -160,6 +161,34 @@ __device__ __forceinline__ void cm_store32(void* to, const uint32_t (&w)[8]) {
     asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]),
                  "r"(w[5]), "r"(w[6]), "r"(w[7])
                  : "memory");
+}
+
+// the greatest of three, NaN if one is
+__device__ __forceinline__ float cm_max3(float a, float b, float c) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+// 2^x of two values up to 2^22 on the FMA pipe: x = n + r, |r| <= 1/2, by rounding to integers (adding 1.5 2^23), a minimax
+// polynomial of 2^r with value 1 at 0, n added to the exponent.  -127 and less give 0.  Relative error 1.01e-4 (third degree,
+// beside bfloat16's 2^-8) or 2.8e-6 (fourth, beside float16's 2^-11).
+template <typename T>
+__device__ __forceinline__ float2 cm_ex2(float2 x) {
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
+    const float2 t = cm_add2(x, float2{12582912.f, 12582912.f});
+    const float2 r = cm_fma2(cm_add2(t, float2{-12582912.f, -12582912.f}), float2{-1.f, -1.f}, x);
+    float2 p;
+    if constexpr (std::is_same<T, __half>::value) {
+        p = cm_fma2(float2{0.009582576341927052f, 0.009582576341927052f}, r, float2{0.05590682849287987f, 0.05590682849287987f});
+        p = cm_fma2(p, r, float2{0.24024106562137604f, 0.24024106562137604f});
+        p = cm_fma2(p, r, float2{0.6931241154670715f, 0.6931241154670715f});
+    } else {
+        p = cm_fma2(float2{0.055009059607982635f, 0.055009059607982635f}, r, float2{0.2422109693288803f, 0.2422109693288803f});
+        p = cm_fma2(p, r, float2{0.6932829022407532f, 0.6932829022407532f});
+    }
+    p = cm_fma2(p, r, float2{1.f, 1.f});
+    return float2{__int_as_float(__float_as_int(p.x) + (__float_as_int(t.x) << 23)), __int_as_float(__float_as_int(p.y) + (__float_as_int(t.y) << 23))};
 }
 
 struct CmBars {
@@ -346,8 +375,12 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     }
                     float top[4] = {v[0], v[1], v[2], v[3]};
 #pragma unroll
-                    for (int i = 4; i < CM_KEYS; ++i) top[i & 3] = fmaxf(top[i & 3], v[i]);
-                    const float y = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * A.lam;
+                    for (int i = 4; i < CM_KEYS - 4; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[i + k], v[i + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[CM_KEYS - 4 + k], -INFINITY);
+                    const float y = cm_max3(cm_max3(top[0], top[1], top[2]), top[3], -INFINITY) * A.lam;
                     const bool grow = y > m + PF_LAZY;
                     if (__any_sync(0xffffffffu, grow)) {
                         const float f = grow ? ex2(m - y) : 1.f;
@@ -363,14 +396,25 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     const float2 lam2{A.lam, A.lam}, ref2{-ref, -ref};
                     float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                     uint32_t w[CM_KEYS / 2];
+                    // of four pairs of keys CM_FMA on the FMA pipe: with all on the special-function unit, which the two
+                    // warpgroups share, it is what bounds the step
+                    auto weights = [&](auto plain) {
 #pragma unroll
-                    for (int i = 0; i < CM_KEYS / 2; ++i) {
-                        float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
-                        e.x = ex2(e.x);
-                        e.y = ex2(e.y);
-                        sum[i & 1] = cm_add2(sum[i & 1], e);
-                        w[i] = pack_f32<T>(e.x, e.y);
-                    }
+                        for (int i = 0; i < CM_KEYS / 2; ++i) {
+                            float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                            if (plain && i % 4 < CM_FMA) {
+                                e = cm_ex2<T>(e);
+                            } else {
+                                e.x = ex2(e.x);
+                                e.y = ex2(e.y);
+                            }
+                            sum[i & 1] = cm_add2(sum[i & 1], e);
+                            w[i] = pack_f32<T>(e.x, e.y);
+                        }
+                    };
+                    // NaN and infinities, masked keys and rows that have seen nothing want the exact limits
+                    if (__all_sync(0xffffffffu, fabsf(y) < INFINITY) && left >= CM_KEYS) weights(std::true_type{});
+                    else weights(std::false_type{});
                     cm_st32(cols, w);
                     const float2 both = cm_add2(sum[0], sum[1]);
                     l += both.x + both.y;
