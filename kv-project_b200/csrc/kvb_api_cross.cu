@@ -6,7 +6,7 @@
 namespace {
 
 // Query rows (tokens x heads of a KV head) of a sequence, on average, up to which cross_few_kernel is taken.
-constexpr int kFewRows = 64;
+constexpr int kFewRows = 16;
 
 constexpr size_t kCrossCounts = size_t(kvb::PD_MAX_CTAS) * kvb::CR_WARPS * 4;
 
@@ -29,7 +29,7 @@ int cross_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
 
 template <typename T, int D, bool MANY>
 kvb_status launch(kvb::CrossParams a, cudaStream_t s) {
-    constexpr int SM = MANY ? kvb::CmShape<D>::SMEM : kvb::CrShape<D>::SMEM, THREADS = 32 * (MANY ? kvb::CM_WARPS : kvb::CR_WARPS);
+    constexpr int SM = MANY ? kvb::CrossTcShape<D>::SMEM : kvb::CrShape<D>::SMEM, THREADS = 32 * (MANY ? kvb::CM_WARPS : kvb::CR_WARPS);
     const auto kern = MANY ? kvb::cross_many_kernel<T, D> : kvb::cross_few_kernel<T, D>;
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = kvbh::allow_smem("cross_attention", reinterpret_cast<const void*>(kern), SM, done)) return st;
@@ -56,7 +56,7 @@ extern "C" {
 
 size_t kvb_cross_workspace(int d) {
     // two partials a CTA: of 2 x 128 rows (cross_many_kernel), of 16 (cross_few_kernel)
-    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * cross_ctas() * 2 * kvb::CM_ROWS * (d + 2) * 4 : 0;
+    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * cross_ctas() * 2 * kvb::CM_ROWS * (d + 3) * 4 : 0;
 }
 
 kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
