@@ -38,6 +38,8 @@ kvb_status launch(kvb::CrossParams a, cudaStream_t s) {
     for (int i = 0; i < n; i += kvb::CR_MAX_SEQS) {
         a.n = std::min(n - i, kvb::CR_MAX_SEQS);
         if (kvb_status st = launch_chained("cross_attention", kern, grid, THREADS, SM, s, a)) return st;
+        if (MANY)
+            if (kvb_status st = launch_chained("cross_attention join", kvb::cross_join_kernel<T, D>, 2 * grid, 32 * kvb::CJ_WARPS, 0, s, a)) return st;
         a.cu_q += kvb::CR_MAX_SEQS;
         a.cu_k += kvb::CR_MAX_SEQS;
     }
@@ -86,6 +88,7 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
         return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
     kvb::CrossParams a{};
     a.rep = Hq / Hkv;
+    a.ctas = cross_ctas();
     const bool many = nq * a.rep > int64_t(kFewRows) * n;
     const int keys = many ? kvb::CM_KEYS : 2048 / d, rows = many ? 2 * kvb::CM_ROWS : kvb::CR_ROWS;
     // units of a sequence times row groups of all fit 32 bits

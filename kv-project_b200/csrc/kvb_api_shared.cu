@@ -2,13 +2,28 @@
 // shared pages (kvb_share.cuh) and of the attention that computes them once for all their sequences (kvb_paged_decode.cuh).
 #include "kvb_paged_host.cuh"
 #include "kvb_share.cuh"
+#include "kvb_shared_tc.cuh"
 
 namespace {
 
 // Segments cover a sequence at most this often: each has two or more parts below it.
 int levels_of(int n) { return std::min(kvb::PS_LEVELS, std::max(n - 1, 0)); }
 
-int64_t level_offset(int d) { return (int64_t(kvbh::paged_part_bytes(d)) + 255) / 256 * 256; }
+int shared_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
+
+// The workspace: counters and partials of the sequences' own tokens, partials of cut items of the segments, the rows' parts by level.
+int64_t part_offset(int d) { return (int64_t(kvbh::paged_part_bytes(d)) + 255) / 256 * 256; }
+int64_t level_offset(int d) { return part_offset(d) + int64_t(2) * shared_ctas() * 2 * kvb::CM_ROWS * (d + 3) * 4; }
+
+template <typename T, int D>
+kvb_status launch_segments(const kvb::SharedTcParams& a, cudaStream_t s) {
+    constexpr int SM = kvb::StShape<D>::SMEM;
+    const auto kern = kvb::shared_pages_kernel<T, D>;
+    static std::atomic<uint64_t> done{0};
+    if (kvb_status st = kvbh::allow_smem("page_attend_shared", reinterpret_cast<const void*>(kern), SM, done)) return st;
+    if (kvb_status st = launch_chained("page_attend_shared", kern, unsigned(a.ctas), 32 * kvb::ST_WARPS, SM, s, a)) return st;
+    return launch_chained("page_attend_shared join", kvb::shared_join_kernel<D>, unsigned(2 * a.ctas), 32 * kvb::CJ_WARPS, 0, s, a);
+}
 
 }  // namespace
 
@@ -51,10 +66,33 @@ kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, 
     a.rows = int64_t(n) * Tq * Hq;
     a.level_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + level_offset(p->d));
     a.level_ml = a.level_o + levels_of(n) * a.rows * p->d;
-    a.by_rows = kvbh::reciprocal(a.rep * Tq);
     cudaStream_t s = static_cast<cudaStream_t>(stream);
-    if (n > 1)
-        if (kvb_status st = kvbh::paged_launch_any<kvb::PD_SEGMENTS>("page_attend_shared", a, dtype, int64_t(n) * a.rep * Tq, s)) return st;
+    if (n > 1) {
+        kvb::SharedTcParams b{};
+        if (kvb_status st = kvbh::make_map("page_attend_shared", &b.tm_k, p, p->kc, kvb::CM_KEYS, false)) return st;
+        if (kvb_status st = kvbh::make_map("page_attend_shared", &b.tm_v, p, p->vc, kvb::CM_KEYS, false)) return st;
+        b.P = a.P;
+        b.shared = a.shared;
+        b.q = q;
+        b.Hq = Hq;
+        b.Tq = Tq;
+        b.rep = a.rep;
+        b.by_rep = a.by_rep;
+        b.by_rows = kvbh::reciprocal(a.rep * Tq);
+        b.page_log2 = a.page_log2;
+        // a scaling of zero becomes one too small to matter, so that -inf stays -inf
+        b.lam = std::max(std::fabs(a.lam), 1e-37f);
+        b.negate = scaling < 0;
+        b.rows = a.rows;
+        b.level_o = a.level_o;
+        b.level_ml = a.level_ml;
+        b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_offset(p->d));
+        b.ctas = shared_ctas();
+        kvb_status st = dtype == KVB_F16 ? p->d == 128 ? launch_segments<__half, 128>(b, s) : launch_segments<__half, 64>(b, s)
+                        : p->d == 128    ? launch_segments<__nv_bfloat16, 128>(b, s)
+                                         : launch_segments<__nv_bfloat16, 64>(b, s);
+        if (st) return st;
+    }
     return kvbh::paged_launch_any<kvb::PD_OWN>("page_attend_shared", a, dtype, int64_t(a.rep) * Tq, s);
 }
 

@@ -41,7 +41,8 @@ struct CrossParams {
     void* out;                                // (nq, Hq, d)
     float* lse;                               // (nq, Hq) or null
     float* part;                              // two a CTA: O, maximum, sum
-    uint32_t* count;                          // [grid][8 warps]
+    uint32_t* count;                          // cross_few_kernel: [grid][8 warps]
+    int ctas;                                 // cross_many_kernel: that take part
 };
 
 template <int D>
@@ -133,7 +134,7 @@ __global__ void __launch_bounds__(32 * CR_WARPS, 1) cross_few_kernel(const __gri
     }
     const int work = shares[A.n];
     if (work == 0) return;
-    PdPlan<PD_SEGMENTS> W;
+    PdPlan<true> W;
     W.pre = pre;
     W.shares = shares;
     W.n = A.n;

@@ -22,6 +22,22 @@ struct CrossTcShape {
     static constexpr int SMEM = 1024 + 2 * S::QTILE + 2 * CM_STAGES * S::TILE + S::XBYTES;
 };
 
+// The work of a call dealt to `ctas` CTAs; false when there is none.  Whole block.
+template <int WARPS>
+__device__ __forceinline__ bool cross_plan(const CrossParams& A, int ctas, int* pre, int* shares, int (*warp_sum)[WARPS], PdPlan<true, CM_FIXED>& W) {
+    if (!cm_scan<WARPS>(A.n, pre, shares, warp_sum, [&](int i, int& u, int& p) {
+            const CrSeq x = cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, i);
+            const int hg = int((int64_t(x.ql) * A.rep + 2 * CM_ROWS - 1) / (2 * CM_ROWS)) * A.Hkv;
+            u = max(1, (x.kl + CM_KEYS - 1) / CM_KEYS) * hg;     // without keys one empty unit: its rows are written
+            p = u + CM_FIXED * hg;
+        })) {
+        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        return false;
+    }
+    cm_deal(W, A.n, pre, shares, ctas);
+    return shares[A.n] > 0;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __grid_constant__ CrossParams A) {
     using S = CmShape<D>;
@@ -31,7 +47,6 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     __shared__ CmBars B;
     __shared__ int warp_sum[2][CM_WARPS];
     __shared__ uint32_t s_tmem;
-    __shared__ int s_last;
     uint8_t* base = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(cm_raw) + 1023) & ~uintptr_t(1023));
     uint8_t* const sq = base;                                    // [2 tiles], then keys and values [stage]
     uint8_t* const sk = sq + 2 * S::QTILE;
@@ -45,25 +60,8 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     }
     chain_kernels();
     auto seq_at = [&](int i) { return cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, i); };
-    if (!cm_scan<CM_WARPS>(A.n, pre, shares, warp_sum, [&](int i, int& u, int& p) {
-            const CrSeq x = seq_at(i);
-            const int hg = int((int64_t(x.ql) * A.rep + 2 * CM_ROWS - 1) / (2 * CM_ROWS)) * A.Hkv;
-            u = max(1, (x.kl + CM_KEYS - 1) / CM_KEYS) * hg;     // without keys one empty unit: its rows are written
-            p = u + CM_FIXED * hg;
-        })) {
-        if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
-        return;
-    }
-    const int work = shares[A.n];
-    if (work == 0) return;
-    PdPlan<PD_SEGMENTS, CM_FIXED> W;
-    W.pre = pre;
-    W.shares = shares;
-    W.n = A.n;
-    W.hg = 0;
-    W.ctas = max(1, min(int(gridDim.x), work / PD_LEAST));
-    W.quota = work / W.ctas;
-    W.extra = work - W.quota * W.ctas;
+    PdPlan<true, CM_FIXED> W;
+    if (!cross_plan<CM_WARPS>(A, A.ctas, pre, shares, warp_sum, W)) return;
     const int cta = blockIdx.x;
     if (cta >= W.ctas) return;
     const int u0 = W.units_before(W.share(cta)), u1 = W.units_before(W.share(cta + 1));
@@ -130,7 +128,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             x = item_at(u0);
             if (cm_units(x.split(), x.tiles, t) > 0) load_q(x);
         }
-        uint32_t sn = 0, it = 0, xn = 0, cuts = 0;               // S of this tile so far; units of the block; parts passed on; items cut
+        uint32_t sn = 0, it = 0, xn = 0;                         // S of this tile so far; units of the block; parts passed on
         int first = 1;
         bool ok = true;
         for (int cur = u0; cur < u1 && ok;) {
@@ -299,23 +297,6 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     }
                 }
             }
-            if (ok && !whole) {
-                // the CTAs c0 .. c1 hold the item's units: the last to arrive joins their partials
-                const int c0 = W.holder(done.p.v0 + CM_FIXED), c1 = W.holder(done.p.v0 + CM_FIXED + done.p.units - 1);
-                const int last = cm_arrive(B, &s_last, A.count + c0, c1 - c0 + 1, cuts++);
-                ok = last >= 0;
-                // the partial of c is its first one, unless the item begins inside c's run
-                if (last > 0)
-                    cm_join<D, false>(A.part, 2 * c0 + (W.share(c0) < done.p.v0 ? 1 : 0), c0, c1, done.nrows,
-                                      [&](int r, int ch, const float (&o)[8], float top, float sum, float) {
-                                          const float inv = cm_inverse(sum);
-                                          const int64_t row = out_row(r);
-                                          *reinterpret_cast<uint4*>(static_cast<T*>(A.out) + row * D + ch) =
-                                              uint4{pack_f32<T>(o[0] * inv, o[1] * inv), pack_f32<T>(o[2] * inv, o[3] * inv),
-                                                    pack_f32<T>(o[4] * inv, o[5] * inv), pack_f32<T>(o[6] * inv, o[7] * inv)};
-                                          if (ch == 0) store_lse(row, top, sum);
-                                      });
-            }
             __syncwarp();
             cm_before();                                         // O is read: the next product into it comes after the next P
             cur = next;
@@ -365,6 +346,36 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     __syncthreads();
     cm_after();
     if (warp == CM_SOFTMAX) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(CM_TMEM));
+}
+
+struct CrossItem {
+    int64_t row;                              // of out: the sequence's first token, the KV head's first query head
+    int row0;
+};
+
+// Joins the items that cross_many_kernel cut.
+template <typename T, int D>
+__global__ void __launch_bounds__(32 * CJ_WARPS) cross_join_kernel(const __grid_constant__ CrossParams A) {
+    __shared__ int pre[CR_MAX_SEQS + 1], shares[CR_MAX_SEQS + 1], warp_sum[2][CJ_WARPS];
+    __shared__ CjSmem<CrossItem> S;
+    PdPlan<true, CM_FIXED> W;
+    if (!cross_plan<CJ_WARPS>(A, A.ctas, pre, shares, warp_sum, W)) return;
+    cm_join<D, false>(W, A.part, S,
+                      [&](const PdPiece& p, CrossItem& x) {
+                          const CrSeq s = cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, p.seq);
+                          const int groups = W.heads(p.seq) / A.Hkv, h = p.vh / groups;
+                          x.row0 = (p.vh - h * groups) * 2 * CM_ROWS;
+                          x.row = int64_t(s.q0) * A.Hq + h * A.rep;
+                          return min(s.ql * A.rep - x.row0, 2 * CM_ROWS);
+                      },
+                      [&](const CrossItem& x, int r, int ch, const float (&o)[4], float top, float sum, float) {
+                          const int at = x.row0 + r, tok = pd_div(at, A.by_rep);
+                          const int64_t row = x.row + int64_t(tok) * A.Hq + at - tok * A.rep;
+                          const float inv = cm_inverse(sum);
+                          *reinterpret_cast<uint2*>(static_cast<T*>(A.out) + row * D + ch) =
+                              uint2{pack_f32<T>(o[0] * inv, o[1] * inv), pack_f32<T>(o[2] * inv, o[3] * inv)};
+                          if (ch == 0 && A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+                      });
 }
 
 }  // namespace kvb

@@ -54,7 +54,6 @@ constexpr float PD_LAZY = 8.f;
 // What a launch attends over.
 constexpr int PD_ALL = 0;                     // every sequence's tokens
 constexpr int PD_OWN = 1;                     // the tokens behind a sequence's shared ones; its segments' parts are joined in
-constexpr int PD_SEGMENTS = 2;                // the tokens that several sequences share, for all of them at once
 
 struct PagedDecodeParams {
     CUtensorMap tm_k, tm_v;                   // codes as (d, page, n_pages * Hkv), box d x min(page, 32) x 1
@@ -70,13 +69,12 @@ struct PagedDecodeParams {
     float* lse;                               // (n, Tq, Hq) or null
     float* part;                              // [2 grid][8 NT x (6 + d)]
     uint32_t* count;                          // [grid][8 warps]
-    // PD_OWN and PD_SEGMENTS
+    // PD_OWN
     SharedView shared;
-    int seq0;                                 // PD_OWN: the launch's first sequence in the plan
+    int seq0;                                 // the launch's first sequence in the plan
     int64_t rows;                             // of the call, all sequences: n Tq Hq
     float* level_o;                           // [PS_LEVELS][rows][d], normalised
     float* level_ml;                          // [PS_LEVELS][rows][2]: maximum, sum
-    uint64_t by_rows;                         // for pd_div by rep Tq
 };
 
 template <int D, int NT>
@@ -95,20 +93,21 @@ struct PdShape {
 
 // The work of a call: per (sequence, KV head, row group) its units, and PD_FIXED more in the shares that the CTAs get
 // (preparing the queries and joining the warps costs about as much time as that many units).
-template <int MODE, int FIXED = PD_FIXED>
+// ANY: sequences with numbers of groups of their own.
+template <bool ANY = false, int FIXED = PD_FIXED>
 struct PdPlan {
-    const int* pre;                           // [n + 1] units before each sequence, for one head and group (segments: for all)
-    const int* shares;                        // segments: [n + 1] places before each
+    const int* pre;                           // [n + 1] units before each sequence, for one head and group (ANY: for all)
+    const int* shares;                        // ANY: [n + 1] places before each
     int n, hg;                                // sequences; KV heads x groups
     int quota, extra, ctas;                   // shares: the first `extra` CTAs get quota + 1
 
-    __device__ __forceinline__ int unit0(int i) const { return MODE == PD_SEGMENTS ? pre[i] : pre[i] * hg; }
-    __device__ __forceinline__ int place0(int i) const { return MODE == PD_SEGMENTS ? shares[i] : (pre[i] + i * FIXED) * hg; }
+    __device__ __forceinline__ int unit0(int i) const { return ANY ? pre[i] : pre[i] * hg; }
+    __device__ __forceinline__ int place0(int i) const { return ANY ? shares[i] : (pre[i] + i * FIXED) * hg; }
     __device__ __forceinline__ int heads(int i) const {          // KV heads x groups of a sequence
-        return MODE == PD_SEGMENTS ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / FIXED : hg;
+        return ANY ? (shares[i + 1] - shares[i] - (pre[i + 1] - pre[i])) / FIXED : hg;
     }
     __device__ __forceinline__ int units(int i) const {
-        return MODE == PD_SEGMENTS ? (pre[i + 1] - pre[i]) / max(heads(i), 1) : pre[i + 1] - pre[i];
+        return ANY ? (pre[i + 1] - pre[i]) / max(heads(i), 1) : pre[i + 1] - pre[i];
     }
     __device__ __forceinline__ int share(int c) const { return c * quota + min(c, extra); }
     __device__ __forceinline__ int holder(int v) const {
@@ -134,8 +133,8 @@ struct PdPiece {
 };
 
 // The piece that begins at unit `cur` of all work.
-template <int MODE, int FIXED>
-__device__ __forceinline__ PdPiece pd_piece(const PdPlan<MODE, FIXED>& W, int cur, int end) {
+template <bool ANY, int FIXED>
+__device__ __forceinline__ PdPiece pd_piece(const PdPlan<ANY, FIXED>& W, int cur, int end) {
     int lo = 0, hi = W.n;
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;
@@ -200,10 +199,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     using S = PdShape<D, NT>;
     constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
     extern __shared__ uint8_t pd_raw[];
-    // of the sequences (or segments): units before them, slot, tokens up to which they go and from which on; of segments the
-    // places before them, the others stay in global memory
-    constexpr int MAX = MODE == PD_SEGMENTS ? PS_MAX_SEQS : PD_MAX_SEQS, HELD = MODE == PD_SEGMENTS ? 1 : PD_MAX_SEQS;
-    __shared__ int pre[MAX + 1], s_shares[MODE == PD_SEGMENTS ? MAX + 1 : 1], s_slot[HELD], s_len[HELD], s_first[MODE == PD_OWN ? HELD : 1];
+    __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS], s_first[MODE == PD_OWN ? PD_MAX_SEQS : 1];
     __shared__ uint64_t full[S::WARPS][S::STAGES];
     __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS], s_w[S::WARPS][S::ROWS];
     __shared__ int warp_sum[S::WARPS];
@@ -219,32 +215,17 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         s_abort = 0;
         fence_mbar_init();
         pre[0] = 0;
-        if (MODE == PD_SEGMENTS) s_shares[0] = 0;
     }
     chain_kernels();
     const SharedView& V = A.shared;
-    const int n_seqs = MODE == PD_SEGMENTS ? V.segment_count() : A.n;
-    auto first_of = [&](int i) { return MODE == PD_OWN ? s_first[i] : MODE == PD_SEGMENTS ? V.segment(i).start : 0; };
-    auto end_of = [&](int i) { return MODE == PD_SEGMENTS ? V.segment(i).end : s_len[i]; };
-    auto slot_of_seq = [&](int i) { return MODE == PD_SEGMENTS ? V.slot_of(V.segment(i), P.n_slots) : s_slot[i]; };
-    // query rows of a sequence (or segment) for one KV head, and their groups
-    auto rows_of = [&](int i) { return MODE == PD_SEGMENTS ? V.segment(i).members * A.rep * A.Tq : A.rep * A.Tq; };
+    auto first_of = [&](int i) { return MODE == PD_OWN ? s_first[i] : 0; };
     // units before each sequence: an inclusive scan, S::THREADS sequences at a time; an empty sequence is one unit
     // without keys, whose rows still have to be written
     int before = 0;
-    int before_places = 0;
-    for (int i0 = 0; i0 < n_seqs; i0 += S::THREADS) {
+    for (int i0 = 0; i0 < A.n; i0 += S::THREADS) {
         const int i = i0 + threadIdx.x;
-        int u = 0, places = 0;
-        if constexpr (MODE == PD_SEGMENTS) {
-            if (i < n_seqs) {
-                const SharedSegment g = V.segment(i);
-                const int hg = (g.members * A.rep * A.Tq + S::ROWS - 1) / S::ROWS * P.Hkv, units = (g.end - g.start + PD_UNIT - 1) / PD_UNIT;
-                // a plan's segments fit 32 bits together (the host has seen to it); what is no plan may not
-                u = units <= INT_MAX / hg - PD_FIXED ? units * hg : 0;
-                places = u + PD_FIXED * hg;
-            }
-        } else if (i < A.n) {
+        int u = 0;
+        if (i < A.n) {
             const int slot = A.slots[i];
             int len = 0;
             if (slot >= 0 && slot < P.n_slots) len = min(max(P.lens[slot], 0), P.max_blocks * P.page);
@@ -257,24 +238,6 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 len -= own;
             }
             u = max(1, (len + PD_UNIT - 1) / PD_UNIT);
-        }
-        if constexpr (MODE == PD_SEGMENTS) {                     // the places the same way
-            int y = places;
-#pragma unroll
-            for (int o = 1; o < 32; o <<= 1) {
-                const int z = __shfl_up_sync(0xffffffffu, y, o);
-                if (lane >= o) y += z;
-            }
-            __syncthreads();
-            if (lane == 31) warp_sum[warp] = y;
-            __syncthreads();
-            int sum = 0;
-            for (int w = 0; w < S::WARPS; ++w) {
-                if (w == warp) y += sum;
-                sum += warp_sum[w];
-            }
-            if (i < n_seqs) s_shares[i + 1] = before_places + y;
-            before_places += sum;
         }
         int x = u;
 #pragma unroll
@@ -290,26 +253,16 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             if (w == warp) x += sum;
             sum += warp_sum[w];
         }
-        if (i < n_seqs) pre[i + 1] = before + x;
+        if (i < A.n) pre[i + 1] = before + x;
         before += sum;
     }
-    if constexpr (MODE == PD_SEGMENTS) {
-        __syncthreads();
-        bool fits = true;                                        // a sum that passed 32 bits shows as one that falls
-        for (int i = threadIdx.x; i < n_seqs; i += S::THREADS) fits &= s_shares[i + 1] >= s_shares[i] && pre[i + 1] >= pre[i];
-        if (!__syncthreads_and(fits)) {
-            if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
-            return;
-        }
-        if (n_seqs == 0) return;
-    }
     __syncthreads();
-    PdPlan<MODE> W;
+    PdPlan<> W;
     W.pre = pre;
-    W.shares = s_shares;
-    W.n = n_seqs;
+    W.shares = nullptr;
+    W.n = A.n;
     W.hg = P.Hkv * A.groups;
-    const int64_t work = MODE == PD_SEGMENTS ? int64_t(s_shares[n_seqs]) : (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
+    const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
     if (work > INT_MAX) {                                        // the host's launches hold less, but for one group of 2^31 units
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return;
@@ -328,29 +281,9 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         return false;
     };
 
-    // KV head and first row of a piece
-    auto head_of = [&](const PdPiece& p, int& row0) {
-        const int groups = MODE == PD_SEGMENTS ? W.heads(p.seq) / P.Hkv : A.groups;
-        const int h = MODE == PD_SEGMENTS ? p.vh / groups : pd_div(p.vh, A.by_groups);
-        row0 = A.row0 + (p.vh - h * groups) * S::ROWS;
-        return h;
-    };
-    // sequence, token and query head in its group of row r (segments: the rows of a member behind one another)
-    auto row_parts = [&](int seq, int r, int& tok, int& head) {
-        int of = seq;
-        if constexpr (MODE == PD_SEGMENTS) {
-            const int member = pd_div(r, A.by_rows);
-            r -= member * A.rep * A.Tq;
-            of = V.member(V.segment(seq), member);
-        }
-        tok = pd_div(r, A.by_rep);
-        head = r - tok * A.rep;
-        return of;
-    };
     auto row_at = [&](int seq, int h, int r) {
-        int tok, head;
-        const int of = row_parts(seq, r, tok, head);
-        return (int64_t(of) * A.Tq + tok) * A.Hq + h * A.rep + head;
+        const int tok = pd_div(r, A.by_rep);
+        return (int64_t(seq) * A.Tq + tok) * A.Hq + h * A.rep + r - tok * A.rep;
     };
     auto finite_ref = [](float m) { return m == -INFINITY ? 0.f : m; };
     // Where a finished row goes: maximum `top`, sum, O and its factor `inv`, which becomes that of the whole row.  PD_OWN: the
@@ -388,10 +321,8 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     };
     // 2^(mw - m) / l; rows that see nothing give 0, NaN stays
     auto scale_of = [&](float m, float mw, float sum) { return sum > 0.f ? ex2(mw - finite_ref(m)) / sum : (sum == sum ? 0.f : sum); };
-    auto store_pair = [&](int seq, int64_t row, int ch, float a, float b, float inv) {
-        if constexpr (MODE == PD_SEGMENTS) {
-            *reinterpret_cast<float2*>(A.level_o + (V.segment(seq).level * A.rows + row) * D + ch) = float2{a * inv, b * inv};
-        } else if constexpr (MODE == PD_OWN) {
+    auto store_pair = [&](int64_t row, int ch, float a, float b, float inv) {
+        if constexpr (MODE == PD_OWN) {
             const float* from = A.level_o + (row + int64_t(A.seq0) * A.Tq * A.Hq) * D + ch;
             a *= inv, b *= inv;
 #pragma unroll
@@ -406,27 +337,22 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             *reinterpret_cast<uint32_t*>(static_cast<T*>(A.out) + row * D + ch) = pack_f32<T>(a * inv, b * inv);
         }
     };
-    auto store_lse = [&](int seq, int64_t row, float top, float sum) {
-        if constexpr (MODE == PD_SEGMENTS)
-            *reinterpret_cast<float2*>(A.level_ml + 2 * (V.segment(seq).level * A.rows + row)) = float2{top, sum};
-        else if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
+    auto store_lse = [&](int64_t row, float top, float sum) {
+        if (A.lse) A.lse[row] = sum == 0.f ? -INFINITY : top * 0.693147180559945309f + logf(sum);
     };
 
     // the query rows of a piece: lane (g, t) holds row g of 8, channels (D / 4) t ..
     const int g = lane >> 2, t = lane & 3;
     uint4 raw[NT][KS / 2];
     auto load_q = [&](const PdPiece& p) {
-        int row0;
-        const int h = head_of(p, row0), rows = rows_of(p.seq);
+        const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS;
 #pragma unroll
         for (int x = 0; x < NT; ++x) {
-            const int r = row0 + 8 * x + g;
+            const int r = row0 + 8 * x + g, tok = pd_div(r, A.by_rep);
 #pragma unroll
             for (int i = 0; i < KS / 2; ++i) raw[x][i] = uint4{0, 0, 0, 0};
-            if (r < rows) {
-                int tok, head;
-                const int of = row_parts(p.seq, r, tok, head);
-                const T* q = static_cast<const T*>(A.q) + ((int64_t(of) * A.Hq + h * A.rep + head) * A.Tq + tok) * D + (D / 4) * t;
+            if (r < A.rep * A.Tq) {
+                const T* q = static_cast<const T*>(A.q) + ((int64_t(p.seq) * A.Hq + h * A.rep + r - tok * A.rep) * A.Tq + tok) * D + (D / 4) * t;
 #pragma unroll
                 for (int i = 0; i < KS / 2; ++i) raw[x][i] = __ldg(reinterpret_cast<const uint4*>(q + 8 * i));
             }
@@ -448,13 +374,12 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
         const PdPiece p = pd_piece(W, u0 + warp + k * S::WARPS, u1);
-        int row0;
-        const int h = head_of(p, row0), t0 = first_of(p.seq) + p.a * PD_UNIT, len = end_of(p.seq), slot = slot_of_seq(p.seq);
+        const int h = pd_div(p.vh, A.by_groups), t0 = first_of(p.seq) + p.a * PD_UNIT, len = s_len[p.seq];
         x.off = t0 & (P.page - 1);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             if (i * box >= PD_UNIT || t0 + i * box >= len) continue;
-            const int id = MODE == PD_SEGMENTS && slot < 0 ? -1 : P.table[int64_t(slot) * P.max_blocks + ((t0 + i * box) >> A.page_log2)];
+            const int id = P.table[int64_t(s_slot[p.seq]) * P.max_blocks + ((t0 + i * box) >> A.page_log2)];
             if (id >= 0 && id < P.n_pages) x.row[i] = id * P.Hkv + h;
             else raise_status(KVB_DEV_BOUNDS);
         }
@@ -498,9 +423,8 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     {
         int first = 1, unit = 0;
         for (int cur = u0; cur < u1;) {
-            int row0;
-            const int h = head_of(p, row0), len = end_of(p.seq), start = first_of(p.seq);
-            const int nrows = min(rows_of(p.seq) - row0, S::ROWS);
+            const int h = pd_div(p.vh, A.by_groups), row0 = A.row0 + (p.vh - h * A.groups) * S::ROWS, len = s_len[p.seq], start = first_of(p.seq);
+            const int nrows = min(A.rep * A.Tq - row0, S::ROWS);
             // ---- the group's query rows as B operands
             uint32_t qf[NT][KS][2];
             float lam[NT][2], bias[NT][2];                       // bias: -1152 sum q, what the codes' pattern adds
@@ -615,12 +539,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
                         for (int k = 0; k < 2; ++k) {
                             // keys from this unit on that the row 2t + k sees
-                            int lim = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1 - t0;
-                            if constexpr (MODE == PD_SEGMENTS) { // by the member's own length; rows past the last see nothing new
-                                int tok, head;
-                                const int r = min(row0 + 8 * x + 2 * t + k, rows_of(p.seq) - 1), of = row_parts(p.seq, r, tok, head);
-                                lim = min(len, V.length_of(of, P) - A.Tq + tok + 1) - t0;
-                            }
+                            const int lim = len - A.Tq + pd_div(row0 + 8 * x + 2 * t + k, A.by_rep) + 1 - t0;
 #pragma unroll
                             for (int half = 0; half < 2; ++half)
 #pragma unroll
@@ -761,7 +680,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
                 const int r = row_of(x);
-                const int64_t row = whole && (MODE != PD_SEGMENTS || r < nrows) ? row_at(p.seq, h, row0 + r) : 0;
+                const int64_t row = whole ? row_at(p.seq, h, row0 + r) : 0;
                 float top = -INFINITY, topw = -INFINITY, sum = 0.f, inv = 0.f, f[S::WARPS];
 #pragma unroll
                 for (int y = 0; y < D / 64; ++y) {
@@ -792,14 +711,14 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
                     if (whole) {
-                        if (r < nrows) store_pair(p.seq, row, channel_of(y), acc.x, acc.y, inv);
+                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, inv);
                     } else if (r < nrows) {
                         *reinterpret_cast<float2*>(part + 6 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
                 }
                 if (lane == 0 && r < nrows) {
                     if (whole) {
-                        if (ml == 0) store_lse(p.seq, row, top, sum);
+                        if (ml == 0) store_lse(row, top, sum);
                     } else {
                         part[3 * ml * S::ROWS + r] = top;
                         part[(3 * ml + 1) * S::ROWS + r] = sum;
@@ -892,8 +811,8 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         weigh(p.seq, row, top[x], sum[x], inv);
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y)
-                            if (!(few && y > 0)) store_pair(p.seq, row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
-                        if (lane == 0 && ml == 0) store_lse(p.seq, row, top[x], sum[x]);
+                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
+                        if (lane == 0 && ml == 0) store_lse(row, top[x], sum[x]);
                     }
                 }
             }

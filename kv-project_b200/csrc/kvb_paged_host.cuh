@@ -21,16 +21,16 @@ inline int64_t part_floats(int d) { return 16 * (int64_t(d) + 6); }
 // ceil(2^64 / d) for kvb::pd_div; 0 for 1
 inline uint64_t reciprocal(int d) { return d == 1 ? 0 : UINT64_MAX / uint64_t(d) + 1; }
 
-// Codes as (d, page, n_pages * Hkv) bytes: box d x min(page, 32) x 1, swizzled over the d bytes of a row.
-inline kvb_status make_map(const char* who, CUtensorMap* m, const kvb_pages* p, const void* codes) {
+// Codes as (d, page, n_pages * Hkv) bytes: box d x min(page, tokens) x 1, swizzled over the d bytes of a row or not at all.
+inline kvb_status make_map(const char* who, CUtensorMap* m, const kvb_pages* p, const void* codes, int tokens, bool swizzled) {
     EncodeTiledFn fn = encode_tiled();
     if (!fn) return fail(KVB_ECUDA, "%s: cuTensorMapEncodeTiled unavailable", who);
     const cuuint64_t dims[3] = {cuuint64_t(p->d), cuuint64_t(p->page), cuuint64_t(p->n_pages * p->Hkv)};
     const cuuint64_t strides[2] = {cuuint64_t(p->d), cuuint64_t(p->d) * p->page};
-    const cuuint32_t box[3] = {cuuint32_t(p->d), cuuint32_t(std::min(p->page, kvb::PD_UNIT)), 1};
+    const cuuint32_t box[3] = {cuuint32_t(p->d), cuuint32_t(std::min(p->page, tokens)), 1};
     const cuuint32_t estr[3] = {1, 1, 1};
     const CUresult r = fn(m, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(codes), dims, strides, box, estr,
-                          CU_TENSOR_MAP_INTERLEAVE_NONE, p->d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
+                          CU_TENSOR_MAP_INTERLEAVE_NONE, !swizzled ? CU_TENSOR_MAP_SWIZZLE_NONE : p->d == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B,
                           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     return r == CUDA_SUCCESS ? KVB_OK : fail(KVB_ECUDA, "%s: no tensor map for the codes", who);
 }
@@ -42,7 +42,6 @@ kvb_status paged_launch(const char* who, kvb::PagedDecodeParams a, cudaStream_t 
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = allow_smem(who, reinterpret_cast<const void*>(kern), SM, done)) return st;
     const unsigned grid = unsigned(std::min(resolve_ctas(0), kvb::PD_MAX_CTAS));
-    if (MODE == kvb::PD_SEGMENTS) return launch_chained(who, kern, grid, kvb::PdShape<D, NT>::THREADS, SM, s, a);
     // A launch's work has to fit 32 bits whatever the lengths are: fewer sequences, and where one alone can be too much, fewer
     // row groups a launch.
     const int rows = a.rep * a.Tq, groups = (rows + 8 * NT - 1) / (8 * NT);
@@ -113,8 +112,8 @@ inline kvb_status paged_params(const char* who, const kvb_pages* p, const void* 
 }
 
 inline kvb_status paged_maps(const char* who, const kvb_pages* p, kvb::PagedDecodeParams& a) {
-    if (kvb_status st = make_map(who, &a.tm_k, p, p->kc)) return st;
-    return make_map(who, &a.tm_v, p, p->vc);
+    if (kvb_status st = make_map(who, &a.tm_k, p, p->kc, kvb::PD_UNIT, true)) return st;
+    return make_map(who, &a.tm_v, p, p->vc, kvb::PD_UNIT, true);
 }
 
 inline void paged_workspace(void* workspace, kvb::PagedDecodeParams& a) {

@@ -4,7 +4,7 @@
 //   S = Q K^T,  x = scaling log2(e) S,  m = running row maximum of x,  P = 2^(x - m),  l = sum P,  O = P V,  out = O / l.
 //
 // One persistent CTA per SM takes an equal run of units (PdPlan), so that any mixture of lengths is balanced; items that a
-// run's end cuts leave partial sums in the workspace, and the last warp to arrive joins them in the order of the keys.
+// run's end cuts leave partial sums in the workspace, which a second kernel joins in the order of the keys.
 //
 // Two tiles of 128 rows, each with a warpgroup for its softmax (a thread a row) and a warp that issues O += P V; S of both in
 // turn comes from another warp, so that one tile's softmax runs beside the other's products.  An item of more than 128 rows is two tiles
@@ -194,7 +194,7 @@ __device__ __forceinline__ float2 cm_ex2(float2 x) {
 }
 
 struct CmBars {
-    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], drained[3], x_full[4], x_empty[4], written, verdict;
+    uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4], q_full[2], drained[3], x_full[4], x_empty[4];
     uint64_t s_full[2][2], p_ready[2][2], pv_done[2][2];         // of a tile, by the half of its columns
 
     // `loads`: arrivals that fill a stage of keys or values
@@ -216,8 +216,6 @@ struct CmBars {
             }
         }
         for (int i = 0; i < 3; ++i) mbar_init(&drained[i], 1);
-        mbar_init(&written, CM_SOFTMAX);
-        mbar_init(&verdict, 1);
     }
 };
 
@@ -255,6 +253,19 @@ __device__ __forceinline__ bool cm_scan(int n, int* pre, int* shares, int (*warp
     bool fits = true;                                            // a sum that passed 32 bits shows as one that falls
     for (int i = threadIdx.x; i < n; i += 32 * WARPS) fits &= shares[i + 1] >= shares[i] && pre[i + 1] >= pre[i];
     return __syncthreads_and(fits);
+}
+
+// The work of pre and shares in equal runs for `ctas` CTAs at most.
+template <int FIXED>
+__device__ __forceinline__ void cm_deal(PdPlan<true, FIXED>& W, int n, const int* pre, const int* shares, int ctas) {
+    const int work = shares[n];
+    W.pre = pre;
+    W.shares = shares;
+    W.n = n;
+    W.hg = 0;
+    W.ctas = max(1, min(ctas, work / PD_LEAST));
+    W.quota = work / W.ctas;
+    W.extra = work - W.quota * W.ctas;
 }
 
 // What the issuing warps know of a piece of an item: the units that pass, those with keys, the keys from its first unit on,
@@ -368,8 +379,8 @@ __device__ __forceinline__ void cm_rescale(uint32_t to, float f) {
     }
 }
 
-// A cut item's partial in the workspace: O (256 rows, D), then the rows' maxima, sums and, where the values have a reference of
-// their own (WREF), that.
+// A cut item's partial in the workspace, two a CTA (of its first item, of its last): O (256 rows, D), then the rows' maxima, sums
+// and, where the values have a reference of their own (WREF), that.
 template <int D>
 constexpr int CM_PART = 2 * CM_ROWS * (D + 3);
 
@@ -384,78 +395,122 @@ __device__ __forceinline__ void cm_put(float* to, const float (&v)[32]) {
     }
 }
 
-// The block's partial of a cut item is written, n the count of cut items before; all softmax warps.  Whether it was the last of
-// the item's `parts`, whose blocks count in *count (set back to zero); -1: a wait ran out.
-__device__ __forceinline__ int cm_arrive(CmBars& B, volatile int* s_last, uint32_t* count, int parts, uint32_t n) {
-    const int lane = threadIdx.x & 31;
-    __syncwarp();
-    if (lane == 0) mbar_arrive(&B.written);
-    if (threadIdx.x < 32) {
-        if (!cm_wait(&B.written, n)) return -1;
-        if (lane == 0) {
-            const uint32_t seen = atomic_add_acq_rel(count, 1u);
-            if (seen >= uint32_t(parts)) raise_status(KVB_DEV_WORKSPACE);
-            if (seen + 1 == uint32_t(parts)) *count = 0;
-            *s_last = seen + 1 == uint32_t(parts);
-            mbar_arrive(&B.verdict);
-        }
-        __syncwarp();
+// Joining, in a kernel of its own after the first (a row's parts may be a hundred, and joined by the block that finishes an item
+// they were most of its time): a row of a cut item a warp (two of 64 channels).
+constexpr int CJ_WARPS = 8;                   // a thread for each CTA of the first kernel at least
+
+struct CmCut {
+    PdPiece p;                                // of the item, from where it is cut first; p.a == 0: none
+    int slot0, c0, c1;                        // its parts: slot0, then slots 2 c of the CTAs up to c1
+};
+// The item that the run of CTA b - 1 begins and its end cuts.
+template <int FIXED>
+__device__ __forceinline__ CmCut cm_cut(const PdPlan<true, FIXED>& W, int b) {
+    CmCut x;
+    x.p.a = 0;
+    x.slot0 = x.c0 = x.c1 = 0;
+    const int u = W.units_before(W.share(b));
+    if (u <= 0 || u >= W.pre[W.n]) return x;
+    x.p = pd_piece(W, u, u + 1);
+    if (x.p.a == 0 || u - x.p.a < W.units_before(W.share(b - 1))) {
+        x.p.a = 0;
+        return x;
     }
-    if (!cm_wait(&B.verdict, n)) return -1;
-    return *s_last;
+    x.c0 = W.holder(x.p.v0 + FIXED);
+    x.c1 = W.holder(x.p.v0 + FIXED + x.p.units - 1);
+    // the partial of c0 is its first one, unless the item begins inside its run
+    x.slot0 = 2 * x.c0 + (W.share(x.c0) < x.p.v0 ? 1 : 0);
+    return x;
 }
 
-// Joins the partials of the blocks c0 .. c1 (the first one's in slot slot0, the others' in 2 c) in the order of the keys; all softmax
-// warps, a thread 8 channels of a row at a time.  finish(row, channel, o, top, sum, topw): O over its own reference topw.
-template <int D, bool WREF, typename F>
-__device__ __forceinline__ void cm_join(const float* part, int slot0, int c0, int c1, int rows, F finish) {
-    constexpr int B = 4;                                         // partials whose loads are in flight together
-    for (int e = threadIdx.x; e < rows * (D / 8); e += 32 * CM_SOFTMAX) {
-        const int r = e / (D / 8), ch = e % (D / 8) * 8;
-        float top = -INFINITY, topw = -INFINITY, sum = 0.f, acc[8];
+// Row r of a cut item, 4 channels from ch: the parts in the order of the keys, O over its own reference topw.
+template <int D, bool WREF>
+__device__ __forceinline__ void cm_join_row(const float* part, const CmCut& x, int r, int ch, float (&acc)[4], float& top, float& sum, float& topw) {
+    constexpr int B = 8;                                         // partials whose loads are in flight together
+    top = topw = -INFINITY;
+    sum = 0.f;
 #pragma unroll
-        for (int i = 0; i < 8; ++i) acc[i] = 0.f;
+    for (int i = 0; i < 4; ++i) acc[i] = 0.f;
 #pragma unroll 1
-        for (int c = c0; c <= c1; c += B) {
-            float m[B], l[B], w[B];
-            float4 o[B][2];
+    for (int c = x.c0; c <= x.c1; c += B) {
+        float m[B], l[B], w[B];
+        float4 o[B];
 #pragma unroll
-            for (int k = 0; k < B; ++k) {
-                const float* from = part + int64_t(c + k == c0 ? slot0 : 2 * (c + k)) * CM_PART<D>;
-                const bool ok = c + k <= c1;
-                const float* st = from + 2 * CM_ROWS * D + r;
-                m[k] = ok ? __ldcg(st) : -INFINITY;
-                l[k] = ok ? __ldcg(st + 2 * CM_ROWS) : 0.f;
-                w[k] = !WREF ? m[k] : ok ? __ldcg(st + 4 * CM_ROWS) : -INFINITY;
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-                    o[k][i] = ok ? __ldcg(reinterpret_cast<const float4*>(from + r * D + ch) + i) : float4{0.f, 0.f, 0.f, 0.f};
-            }
-            float most = top, mostw = topw;
-#pragma unroll
-            for (int k = 0; k < B; ++k) most = fmaxf(most, m[k]), mostw = fmaxf(mostw, w[k]);
-            const float ref = most == -INFINITY ? 0.f : most, refw = mostw == -INFINITY ? 0.f : mostw;
-            sum *= ex2(top - ref);
-            const float old = ex2(topw - refw);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) acc[i] *= old;
-#pragma unroll
-            for (int k = 0; k < B; ++k) {
-                sum = __fmaf_rn(l[k], ex2(m[k] - ref), sum);
-                const float f = ex2(w[k] - refw);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    acc[4 * i] = __fmaf_rn(o[k][i].x, f, acc[4 * i]);
-                    acc[4 * i + 1] = __fmaf_rn(o[k][i].y, f, acc[4 * i + 1]);
-                    acc[4 * i + 2] = __fmaf_rn(o[k][i].z, f, acc[4 * i + 2]);
-                    acc[4 * i + 3] = __fmaf_rn(o[k][i].w, f, acc[4 * i + 3]);
-                }
-            }
-            top = most, topw = mostw;
+        for (int k = 0; k < B; ++k) {
+            const float* from = part + int64_t(c + k == x.c0 ? x.slot0 : 2 * (c + k)) * CM_PART<D>;
+            const bool ok = c + k <= x.c1;
+            const float* st = from + 2 * CM_ROWS * D + r;
+            m[k] = ok ? __ldcg(st) : -INFINITY;
+            l[k] = ok ? __ldcg(st + 2 * CM_ROWS) : 0.f;
+            w[k] = !WREF ? m[k] : ok ? __ldcg(st + 4 * CM_ROWS) : -INFINITY;
+            o[k] = ok ? __ldcg(reinterpret_cast<const float4*>(from + r * D + ch)) : float4{0.f, 0.f, 0.f, 0.f};
         }
-        finish(r, ch, acc, top, sum, topw);
+        float most = top, mostw = topw;
+#pragma unroll
+        for (int k = 0; k < B; ++k) most = fmaxf(most, m[k]), mostw = fmaxf(mostw, w[k]);
+        const float ref = most == -INFINITY ? 0.f : most, refw = mostw == -INFINITY ? 0.f : mostw;
+        sum *= ex2(top - ref);
+        const float old = ex2(topw - refw);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[i] *= old;
+#pragma unroll
+        for (int k = 0; k < B; ++k) {
+            sum = __fmaf_rn(l[k], ex2(m[k] - ref), sum);
+            const float f = ex2(w[k] - refw);
+            acc[0] = __fmaf_rn(o[k].x, f, acc[0]);
+            acc[1] = __fmaf_rn(o[k].y, f, acc[1]);
+            acc[2] = __fmaf_rn(o[k].z, f, acc[2]);
+            acc[3] = __fmaf_rn(o[k].w, f, acc[3]);
+        }
+        top = most, topw = mostw;
     }
-    __syncwarp();
+}
+
+// I: what finish() needs of an item
+template <typename I>
+struct CjSmem {
+    CmCut cut[256];                           // by the CTA whose end cuts
+    I item[256];
+    int rows[256], before[257];               // rows of each; warps' tasks before each
+    int warp_sum[CJ_WARPS];
+};
+
+// All cut items: rows_of(piece, item) rows of one, finish(item, row, channel, o, top, sum, topw).  What is cut is found before the parts
+// are waited for: the plan is older than the kernel that writes them, which waited for it before it let this one in.
+template <int D, bool WREF, int FIXED, typename I, typename R, typename F>
+__device__ __forceinline__ void cm_join(const PdPlan<true, FIXED>& W, const float* part, CjSmem<I>& S, R rows_of, F finish) {
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, id = threadIdx.x;
+    constexpr int LANES = D / 4, PER = 32 / LANES;               // of a row; rows of a warp
+    CmCut mine;
+    mine.p.a = 0;
+    if (id + 1 < W.ctas) mine = cm_cut(W, id + 1);
+    const int rows = mine.p.a > 0 ? rows_of(mine.p, S.item[id]) : 0, tasks = (rows + PER - 1) / PER;
+    S.cut[id] = mine;
+    S.rows[id] = rows;
+    int x = tasks;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) S.warp_sum[warp] = x;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) x += S.warp_sum[w];
+    S.before[id + 1] = x;
+    if (id == 0) S.before[0] = 0;
+    __syncthreads();
+    chain_kernels();
+    for (int task = blockIdx.x * CJ_WARPS + warp; task < S.before[256]; task += gridDim.x * CJ_WARPS) {
+        int lo = 0;
+#pragma unroll
+        for (int step = 128; step > 0; step >>= 1)
+            if (S.before[lo + step] <= task) lo += step;
+        const int r = (task - S.before[lo]) * PER + lane / LANES, ch = lane % LANES * 4;
+        if (r >= S.rows[lo]) continue;
+        float o[4], top, sum, topw;
+        cm_join_row<D, WREF>(part, S.cut[lo], r, ch, o, top, sum, topw);
+        finish(S.item[lo], r, ch, o, top, sum, topw);
+    }
 }
 
 __device__ __forceinline__ float cm_inverse(float sum) { return sum > 0.f ? 1.f / sum : (sum == sum ? 0.f : sum); }
