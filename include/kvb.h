@@ -561,9 +561,8 @@ kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32
 /* kvb_page_attend for the slots of a plan: the same results up to rounding, each segment's codes read once for all its
  * members.  The plan stays good while the sequences only grow (extend, write); after fork, free, compact or copy it has to be
  * made anew (what it says is checked, so that a stale plan reads no wrong address; segments that do not fit raise status bit 1
- * and the results of their members are not defined).  workspace: 256-byte aligned, its first
- * kvb_page_attend_workspace(p, n, Hq, Tq) bytes zero-filled once before its first use and then reused (every call leaves its
- * counters at zero), one per stream that runs calls concurrently. */
+ * and the results of their members are not defined).  workspace: 256-byte aligned, its first 8192 bytes zero-filled once before
+ * its first use and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently. */
 size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq);
 kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
                                   const int32_t* plan, float scaling, void* out, float* lse, void* workspace,

@@ -9,11 +9,16 @@ namespace {
 // Segments cover a sequence at most this often: each has two or more parts below it.
 int levels_of(int n) { return std::min(kvb::PS_LEVELS, std::max(n - 1, 0)); }
 
+constexpr int64_t kTogether = 220;          // see PD_LONE
+
 int shared_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
 
-// The workspace: counters and partials of the sequences' own tokens, partials of cut items of the segments, the rows' parts by level.
-int64_t part_offset(int d) { return (int64_t(kvbh::paged_part_bytes(d)) + 255) / 256 * 256; }
-int64_t level_offset(int d) { return part_offset(d) + int64_t(2) * shared_ctas() * 2 * kvb::CM_ROWS * (d + 3) * 4; }
+// The workspace: counters; partials of cut items, first of the segments, then of the sequences' own tokens (the former are
+// joined by then); the rows' parts by level.
+int64_t level_offset(int d) {
+    const int64_t segments = int64_t(2) * shared_ctas() * 2 * kvb::CM_ROWS * (d + 3), own = int64_t(2) * shared_ctas() * 8 * 16 * (d + 4);
+    return kvbh::kCountBytes + (std::max(segments, own) * 4 + 255) / 256 * 256;
+}
 
 template <typename T, int D>
 kvb_status launch_segments(const kvb::SharedTcParams& a, cudaStream_t s) {
@@ -62,6 +67,8 @@ kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, 
         return fail(KVB_EINVAL, "page_attend_shared: workspace of %zu bytes, 256-byte aligned", kvb_page_attend_shared_workspace(p, n, Hq, Tq));
     if (kvb_status st = kvbh::paged_maps("page_attend_shared", p, a)) return st;
     kvbh::paged_workspace(workspace, a);
+    a.whole_words = aligned(out, 16);
+    a.early = n > 1;
     a.shared = kvb::SharedView{plan, slots, n, p->page, p->max_blocks * p->page, levels_of(n)};
     a.rows = int64_t(n) * Tq * Hq;
     a.level_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + level_offset(p->d));
@@ -86,14 +93,17 @@ kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, 
         b.rows = a.rows;
         b.level_o = a.level_o;
         b.level_ml = a.level_ml;
-        b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + part_offset(p->d));
+        b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kvbh::kCountBytes);
         b.ctas = shared_ctas();
         kvb_status st = dtype == KVB_F16 ? p->d == 128 ? launch_segments<__half, 128>(b, s) : launch_segments<__half, 64>(b, s)
                         : p->d == 128    ? launch_segments<__nv_bfloat16, 128>(b, s)
                                          : launch_segments<__nv_bfloat16, 64>(b, s);
         if (st) return st;
     }
-    return kvbh::paged_launch_any<kvb::PD_OWN>("page_attend_shared", a, dtype, int64_t(a.rep) * Tq, s);
+    // items of the sequences' own tokens: up to kTogether the eight warps of a CTA work on one together, above each on its own
+    const int64_t rows = int64_t(a.rep) * Tq, items = (rows <= 8 ? 1 : (rows + 15) / 16) * n * p->Hkv;
+    return items <= kTogether ? kvbh::paged_launch_any<kvb::PD_OWN>("page_attend_shared", a, dtype, rows, s)
+                              : kvbh::paged_launch_any<kvb::PD_LONE>("page_attend_shared", a, dtype, rows, s);
 }
 
 }  // extern "C"

@@ -48,12 +48,18 @@ constexpr int PD_MAX_CTAS = 256;
 // what a (sequence, head, group) costs beside its units, in units: 48 ragged sequences take 123 us with 6, 88 with 12, 70
 // with 16 to 32
 constexpr int PD_FIXED = 16;
-constexpr int PD_LEAST = 4;                   // a CTA's least share
+// The same where warps work alone (PD_LONE), which join nothing in shared memory.
+constexpr int PD_FIXED_LONE = 6;
+constexpr int PD_LEAST = 4;                   // a CTA's (a lone warp's) least share
 constexpr float PD_LAZY = 8.f;
 
 // What a launch attends over.
 constexpr int PD_ALL = 0;                     // every sequence's tokens
 constexpr int PD_OWN = 1;                     // the tokens behind a sequence's shared ones; its segments' parts are joined in
+// The same, a warp for itself: it takes a run of its own units, keeps its results in registers to the end and stores them from
+// there.  For many short items, of which the eight warps of a CTA together spend most of the time on joining (512 items of 20 to
+// 700 tokens: 34 us together, 25 alone; 200 of up to 260, 15 and 21; 16 of 60, 10 and 14).
+constexpr int PD_LONE = 2;
 
 struct PagedDecodeParams {
     CUtensorMap tm_k, tm_v;                   // codes as (d, page, n_pages * Hkv), box d x min(page, 32) x 1
@@ -69,8 +75,10 @@ struct PagedDecodeParams {
     float* lse;                               // (n, Tq, Hq) or null
     float* part;                              // [2 grid][8 NT x (6 + d)]
     uint32_t* count;                          // [grid][8 warps]
-    // PD_OWN
+    // PD_OWN, PD_LONE
     SharedView shared;
+    int early;                                // the kernels of the segments come directly before
+    int whole_words;                          // out is 16-byte aligned
     int seq0;                                 // the launch's first sequence in the plan
     int64_t rows;                             // of the call, all sequences: n Tq Hq
     float* level_o;                           // [PS_LEVELS][rows][d], normalised
@@ -88,6 +96,7 @@ struct PdShape {
     static constexpr int JOIN = WARPS * 8 * (64 + 4) * 4;    // the warps' O rows, 8 query rows and 64 channels at a time
     static constexpr int PAIRS = NT * (D / 64);              // (row, 64 channels) that a warp joins
     static constexpr int PART = ROWS * (D + 6);              // m, l, mw of the rows, twice (see the joining), then O
+    static constexpr int LONE_PART = ROWS * (D + 4);         // O of the rows, then m, l, mw
     static constexpr int SMEM = 1024 + WARPS * STAGES * STAGE + JOIN;
 };
 
@@ -199,7 +208,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     using S = PdShape<D, NT>;
     constexpr int KS = D / 16;                                   // MMA steps over the channels, and channel tiles
     extern __shared__ uint8_t pd_raw[];
-    __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS], s_first[MODE == PD_OWN ? PD_MAX_SEQS : 1];
+    __shared__ int pre[PD_MAX_SEQS + 1], s_slot[PD_MAX_SEQS], s_len[PD_MAX_SEQS], s_first[MODE != PD_ALL ? PD_MAX_SEQS : 1];
     __shared__ uint64_t full[S::WARPS][S::STAGES];
     __shared__ float s_m[S::WARPS][S::ROWS], s_l[S::WARPS][S::ROWS], s_w[S::WARPS][S::ROWS];
     __shared__ int warp_sum[S::WARPS];
@@ -216,9 +225,13 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         fence_mbar_init();
         pre[0] = 0;
     }
-    chain_kernels();
+    constexpr bool LONE = MODE == PD_LONE, OWN = MODE != PD_ALL;
+    // After the kernels of the segments only their parts are younger than those kernels, which waited for all else: that wait
+    // then comes before the first result.
+    bool waited = !OWN || !A.early;
+    if (waited) chain_kernels();
     const SharedView& V = A.shared;
-    auto first_of = [&](int i) { return MODE == PD_OWN ? s_first[i] : 0; };
+    auto first_of = [&](int i) { return OWN ? s_first[i] : 0; };
     // units before each sequence: an inclusive scan, S::THREADS sequences at a time; an empty sequence is one unit
     // without keys, whose rows still have to be written
     int before = 0;
@@ -232,7 +245,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             else raise_status(KVB_DEV_BOUNDS);
             s_slot[i] = slot;
             s_len[i] = len;
-            if constexpr (MODE == PD_OWN) {
+            if constexpr (OWN) {
                 const int own = V.own_of(A.seq0 + i, len);
                 s_first[i] = own;
                 len -= own;
@@ -257,22 +270,24 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         before += sum;
     }
     __syncthreads();
-    PdPlan<> W;
+    constexpr int FIXED = LONE ? PD_FIXED_LONE : PD_FIXED;
+    PdPlan<false, FIXED> W;
     W.pre = pre;
     W.shares = nullptr;
     W.n = A.n;
     W.hg = P.Hkv * A.groups;
-    const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * PD_FIXED) * W.hg;
+    const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * FIXED) * W.hg;
     if (work > INT_MAX) {                                        // the host's launches hold less, but for one group of 2^31 units
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return;
     }
-    W.ctas = max(1, min(int(gridDim.x), int(work) / PD_LEAST));
+    W.ctas = max(1, min(int(gridDim.x) * (LONE ? S::WARPS : 1), int(work) / PD_LEAST));
     W.quota = int(work) / W.ctas;
     W.extra = int(work) - W.quota * W.ctas;
-    const int cta = blockIdx.x;
-    if (cta >= W.ctas) return;
-    const int u0 = W.units_before(W.share(cta)), u1 = W.units_before(W.share(cta + 1));
+    // lone warps: those of a small work on all SMs
+    const int cta = LONE ? blockIdx.x + warp * gridDim.x : blockIdx.x;
+    if (!LONE && cta >= W.ctas) return;
+    const int u0 = cta < W.ctas ? W.units_before(W.share(cta)) : 0, u1 = cta < W.ctas ? W.units_before(W.share(cta + 1)) : 0;
     volatile int* abort = &s_abort;
     auto wait = [&](uint64_t* bar, uint32_t count) {
         if (*abort) return false;
@@ -286,13 +301,11 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         return (int64_t(seq) * A.Tq + tok) * A.Hq + h * A.rep + r - tok * A.rep;
     };
     auto finite_ref = [](float m) { return m == -INFINITY ? 0.f : m; };
-    // Where a finished row goes: maximum `top`, sum, O and its factor `inv`, which becomes that of the whole row.  PD_OWN: the
-    // row's parts of its sequence's segments are joined in, weights sum 2^(top - the largest).
+    // PD_OWN: maximum, sum and factor of a finished row become those of the whole row, the weights of its segments' parts
+    // sum 2^(top - the largest)
     float wl[MODE == PD_OWN ? PS_LEVELS : 1];
-    int levels = 0;
-    auto weigh = [&](int seq, int64_t row, float& top, float& sum, float& inv) {
+    auto weigh = [&](int levels, int64_t row, float& top, float& sum, float& inv) {
         if constexpr (MODE == PD_OWN) {
-            levels = V.depth_of(A.seq0 + seq);
             const int64_t at = row + int64_t(A.seq0) * A.Tq * A.Hq;
             float m[PS_LEVELS], most = top;
 #pragma unroll
@@ -321,7 +334,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     };
     // 2^(mw - m) / l; rows that see nothing give 0, NaN stays
     auto scale_of = [&](float m, float mw, float sum) { return sum > 0.f ? ex2(mw - finite_ref(m)) / sum : (sum == sum ? 0.f : sum); };
-    auto store_pair = [&](int64_t row, int ch, float a, float b, float inv) {
+    auto store_pair = [&](int levels, int64_t row, int ch, float a, float b, float inv) {
         if constexpr (MODE == PD_OWN) {
             const float* from = A.level_o + (row + int64_t(A.seq0) * A.Tq * A.Hq) * D + ch;
             a *= inv, b *= inv;
@@ -369,11 +382,11 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
         int row[2], off;                                         // rows of the tensor maps (< 0: nothing there), token in the page
     };
     const int box = min(P.page, PD_UNIT);
-    const int mine = max(0, (u1 - u0 - warp + S::WARPS - 1) / S::WARPS);                 // units of this warp
+    const int mine = LONE ? u1 - u0 : max(0, (u1 - u0 - warp + S::WARPS - 1) / S::WARPS);                // units of this warp
     auto place = [&](int k) {
         Place x{{-1, -1}, 0};
         if (k >= mine) return x;
-        const PdPiece p = pd_piece(W, u0 + warp + k * S::WARPS, u1);
+        const PdPiece p = pd_piece(W, LONE ? u0 + k : u0 + warp + k * S::WARPS, u1);
         const int h = pd_div(p.vh, A.by_groups), t0 = first_of(p.seq) + p.a * PD_UNIT, len = s_len[p.seq];
         x.off = t0 & (P.page - 1);
 #pragma unroll
@@ -466,6 +479,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                     bias[x][k] = -1152.f * __shfl_sync(0xffffffffu, sum, 4 * (2 * t + k));
                 }
             }
+            const int levels = OWN ? V.depth_of(A.seq0 + p.seq) : 0;
             float o[NT][KS][4], m[NT][2], mw[NT][2], l[NT][2];
 #pragma unroll
             for (int x = 0; x < NT; ++x) {
@@ -476,7 +490,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
             }
             // the first unit of the piece that is this warp's (units go to the warps in turn over the CTA's whole run)
             const int lead = (cur - u0) % S::WARPS;
-            for (int k = warp < lead ? warp - lead + S::WARPS : warp - lead; k < p.b - p.a; k += S::WARPS, ++unit) {
+            for (int k = LONE ? 0 : warp < lead ? warp - lead + S::WARPS : warp - lead; k < p.b - p.a; k += LONE ? 1 : S::WARPS, ++unit) {
                 const int st = unit % S::STAGES;
                 if (!__all_sync(0xffffffffu, wait(&full[warp][st], unit / S::STAGES))) continue;
                 if ((unit & 31) == 0) sc_now = float4{sc_next.x, sc_next.y, log_scale(sc_next.z), log_scale(sc_next.w)};
@@ -642,13 +656,184 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                 pn = pd_piece(W, next, u1);
                 load_q(pn);
             }
+            if (OWN && !waited) {
+                chain_kernels();
+                waited = true;
+            }
+            if constexpr (LONE) {
+                // ---- the warp's rows 8 x + 2 t + k: lane (g, t) has the channels (D / 8) g .. of two of them
+                constexpr int CH = D / 8;
+                const bool whole = p.a == 0 && p.b == p.units;
+                const int c0 = whole ? 0 : W.holder(p.v0 + FIXED), c1 = whole ? 0 : W.holder(p.v0 + FIXED + p.units - 1);
+#pragma unroll
+                for (int x = 0; x < NT; ++x)
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        l[x][k] += __shfl_xor_sync(0xffffffffu, l[x][k], 4);
+                        l[x][k] += __shfl_xor_sync(0xffffffffu, l[x][k], 8);
+                        l[x][k] += __shfl_xor_sync(0xffffffffu, l[x][k], 16);
+                    }
+                // the rows 8 x + 2 t and the next: O over its references, joined with their parts of the sequence's segments, weights
+                // sum 2^(top - the largest)
+                auto finish = [&](int x, float (&v)[2][CH], float (&top)[2], float (&sum)[2], const float (&topw)[2]) {
+                    int64_t row[2];
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        row[k] = row_at(p.seq, h, row0 + min(8 * x + 2 * t + k, nrows - 1));
+                        // over the maximum from here on: sum times the normalised O
+                        const float f = sum[k] > 0.f ? ex2(topw[k] - finite_ref(top[k])) : (sum[k] == sum[k] ? 0.f : sum[k]);
+#pragma unroll
+                        for (int i = 0; i < CH; ++i) v[k][i] *= f;
+                    }
+#pragma unroll 1
+                    for (int level = 0; level < levels; ++level) {
+                        float2 ml[2];
+                        float4 o4[2][CH / 4];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int64_t at = level * A.rows + row[k] + int64_t(A.seq0) * A.Tq * A.Hq;
+                            ml[k] = __ldcg(reinterpret_cast<const float2*>(A.level_ml) + at);
+#pragma unroll
+                            for (int i = 0; i < CH / 4; ++i) o4[k][i] = __ldcg(reinterpret_cast<const float4*>(A.level_o + at * D + CH * g) + i);
+                        }
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const float most = fmaxf(top[k], ml[k].x), ref = finite_ref(most), old = ex2(top[k] - ref), now = ml[k].y * ex2(ml[k].x - ref);
+                            top[k] = most;
+                            sum[k] = sum[k] * old + now;
+#pragma unroll
+                            for (int i = 0; i < CH / 4; ++i) {
+                                v[k][4 * i] = __fmaf_rn(o4[k][i].x, now, v[k][4 * i] * old);
+                                v[k][4 * i + 1] = __fmaf_rn(o4[k][i].y, now, v[k][4 * i + 1] * old);
+                                v[k][4 * i + 2] = __fmaf_rn(o4[k][i].z, now, v[k][4 * i + 2] * old);
+                                v[k][4 * i + 3] = __fmaf_rn(o4[k][i].w, now, v[k][4 * i + 3] * old);
+                            }
+                        }
+                    }
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        if (8 * x + 2 * t + k >= nrows) continue;
+                        const float inv = sum[k] > 0.f ? 1.f / sum[k] : (sum[k] == sum[k] ? 0.f : sum[k]);
+                        uint32_t y[CH / 2];
+#pragma unroll
+                        for (int i = 0; i < CH / 2; ++i) y[i] = pack_f32<T>(v[k][2 * i] * inv, v[k][2 * i + 1] * inv);
+                        T* to = static_cast<T*>(A.out) + row[k] * D + CH * g;
+#pragma unroll
+                        for (int i = 0; i < CH / 8; ++i) {
+                            if (A.whole_words) {
+                                reinterpret_cast<uint4*>(to)[i] = uint4{y[4 * i], y[4 * i + 1], y[4 * i + 2], y[4 * i + 3]};
+                            } else {
+#pragma unroll
+                                for (int j = 0; j < 4; ++j) reinterpret_cast<uint32_t*>(to)[4 * i + j] = y[4 * i + j];
+                            }
+                        }
+                        if (g == 0) store_lse(row[k], top[k], sum[k]);
+                    }
+                };
+                if (whole) {
+#pragma unroll
+                    for (int x = 0; x < NT; ++x) {
+                        if (8 * x >= nrows) break;
+                        float v[2][CH];
+#pragma unroll
+                        for (int k = 0; k < 2; ++k)
+#pragma unroll
+                            for (int c = 0; c < KS; ++c) v[k][2 * c] = o[x][c][k], v[k][2 * c + 1] = o[x][c][2 + k];
+                        finish(x, v, m[x], l[x], mw[x]);
+                    }
+                } else {
+                    float* part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * S::LONE_PART;
+#pragma unroll
+                    for (int x = 0; x < NT; ++x)
+#pragma unroll
+                        for (int k = 0; k < 2; ++k) {
+                            const int r = 8 * x + 2 * t + k;
+                            if (r >= nrows) continue;
+#pragma unroll
+                            for (int c = 0; c < KS; c += 2)
+                                __stcg(reinterpret_cast<float4*>(part + r * D + CH * g + 2 * c), float4{o[x][c][k], o[x][c][2 + k], o[x][c + 1][k], o[x][c + 1][2 + k]});
+                            if (g == 0) {
+                                __stcg(part + S::ROWS * D + r, m[x][k]);
+                                __stcg(part + S::ROWS * (D + 1) + r, l[x][k]);
+                                __stcg(part + S::ROWS * (D + 2) + r, mw[x][k]);
+                            }
+                        }
+                    // the last warp to arrive joins the warps' partials in the order of the tokens
+                    uint32_t seen = 0;
+                    __syncwarp();
+                    if (lane == 0) seen = atomic_add_acq_rel(A.count + c0, 1u);
+                    seen = __shfl_sync(0xffffffffu, seen, 0);
+                    if (seen > uint32_t(c1 - c0)) {
+                        if (lane == 0) raise_status(KVB_DEV_WORKSPACE);
+                    } else if (seen == uint32_t(c1 - c0)) {
+                        if (lane == 0) A.count[c0] = 0;
+                        // the partial of c is its first one, unless the (sequence, head, group) begins inside c's run
+                        const int slot0 = 2 * c0 + (W.share(c0) < p.v0 ? 1 : 0);
+#pragma unroll 1
+                        for (int x = 0; x < NT; ++x) {
+                            if (8 * x >= nrows) break;
+                            float acc[2][CH], top[2], topw[2], sum[2];
+#pragma unroll
+                            for (int k = 0; k < 2; ++k) {
+                                top[k] = topw[k] = -INFINITY;
+                                sum[k] = 0.f;
+#pragma unroll
+                                for (int i = 0; i < CH; ++i) acc[k][i] = 0.f;
+                            }
+#pragma unroll 1
+                            for (int c = c0; c <= c1; c += 2) {  // two partials' loads in flight
+                                float ms[2][2], ls[2][2], ws[2][2];
+                                float4 v[2][2][CH / 4];
+#pragma unroll
+                                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k) {
+                                        const int r = 8 * x + 2 * t + k;
+                                        const bool ok = c + y <= c1 && r < nrows;
+                                        const float* from = A.part + int64_t(c + y == c0 ? slot0 : 2 * (c + y)) * S::LONE_PART;
+                                        ms[y][k] = ok ? __ldcg(from + S::ROWS * D + r) : -INFINITY;
+                                        ls[y][k] = ok ? __ldcg(from + S::ROWS * (D + 1) + r) : 0.f;
+                                        ws[y][k] = ok ? __ldcg(from + S::ROWS * (D + 2) + r) : -INFINITY;
+#pragma unroll
+                                        for (int i = 0; i < CH / 4; ++i)
+                                            v[y][k][i] = ok ? __ldcg(reinterpret_cast<const float4*>(from + r * D + CH * g) + i) : float4{0.f, 0.f, 0.f, 0.f};
+                                    }
+#pragma unroll
+                                for (int y = 0; y < 2; ++y)
+#pragma unroll
+                                    for (int k = 0; k < 2; ++k) {
+                                        const float most = fmaxf(top[k], ms[y][k]), ref = finite_ref(most);
+                                        sum[k] = sum[k] * ex2(top[k] - ref) + ls[y][k] * ex2(ms[y][k] - ref);
+                                        top[k] = most;
+                                        const float mostw = fmaxf(topw[k], ws[y][k]), refw = finite_ref(mostw);
+                                        const float old = ex2(topw[k] - refw), now = ex2(ws[y][k] - refw);
+                                        topw[k] = mostw;
+#pragma unroll
+                                        for (int i = 0; i < CH / 4; ++i) {
+                                            acc[k][4 * i] = __fmaf_rn(v[y][k][i].x, now, acc[k][4 * i] * old);
+                                            acc[k][4 * i + 1] = __fmaf_rn(v[y][k][i].y, now, acc[k][4 * i + 1] * old);
+                                            acc[k][4 * i + 2] = __fmaf_rn(v[y][k][i].z, now, acc[k][4 * i + 2] * old);
+                                            acc[k][4 * i + 3] = __fmaf_rn(v[y][k][i].w, now, acc[k][4 * i + 3] * old);
+                                        }
+                                    }
+                            }
+                            finish(x, acc, top, sum, topw);
+                        }
+                    }
+                }
+                __syncwarp();
+                cur = next;
+                p = pn;
+                first = 0;
+                continue;
+            }
             // ---- join the warps.  Warp w joins the rows w and 8 + w, 64 channels at a time; where there are at most four
             // rows of 128 channels, row w % 4 and the half w / 4 of its channels, all at once.  Column c of the buffer is
             // channel (D / 8) (c / 8) + 8 y + c % 8 of the half y.
             const bool few = D == 128 && NT == 1 && nrows <= 4;
             const bool whole = p.a == 0 && p.b == p.units;
             // the CTAs c0 .. c1 hold its units
-            const int c0 = whole ? 0 : W.holder(p.v0 + PD_FIXED), c1 = whole ? 0 : W.holder(p.v0 + PD_FIXED + p.units - 1);
+            const int c0 = whole ? 0 : W.holder(p.v0 + FIXED), c1 = whole ? 0 : W.holder(p.v0 + FIXED + p.units - 1);
             if (!first) asm volatile("bar.sync 1, %0;" ::"n"(32 * S::WARPS) : "memory");       // the last join's reads are done
 #pragma unroll
             for (int x = 0; x < NT; ++x)
@@ -701,7 +886,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                             sum = __fmaf_rn(s_l[w][r], ex2(s_m[w][r] - ref), sum);
                         }
                         inv = scale_of(top, topw, sum);
-                        if (whole && r < nrows) weigh(p.seq, row, top, sum, inv);
+                        if (whole && r < nrows) weigh(levels, row, top, sum, inv);
                     }
                     float2 acc{0.f, 0.f};
 #pragma unroll
@@ -711,7 +896,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         acc.y = __fmaf_rn(v.y, f[w], acc.y);
                     }
                     if (whole) {
-                        if (r < nrows) store_pair(row, channel_of(y), acc.x, acc.y, inv);
+                        if (r < nrows) store_pair(levels, row, channel_of(y), acc.x, acc.y, inv);
                     } else if (r < nrows) {
                         *reinterpret_cast<float2*>(part + 6 * S::ROWS + r * D + channel_of(y)) = acc;
                     }
@@ -808,10 +993,10 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
                         if (row_of(x) >= nrows) continue;
                         const int64_t row = row_at(p.seq, h, row0 + row_of(x));
                         float inv = scale_of(top[x], topw[x], sum[x]);
-                        weigh(p.seq, row, top[x], sum[x], inv);
+                        weigh(levels, row, top[x], sum[x], inv);
 #pragma unroll
                         for (int y = 0; y < D / 64; ++y)
-                            if (!(few && y > 0)) store_pair(row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
+                            if (!(few && y > 0)) store_pair(levels, row, channel_of(y), acc[x][y].x, acc[x][y].y, inv);
                         if (lane == 0 && ml == 0) store_lse(row, top[x], sum[x]);
                     }
                 }

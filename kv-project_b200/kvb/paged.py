@@ -60,6 +60,9 @@ def _not_capturing(who: str):
         raise NotImplementedError(f"{who}: the first call on a stream makes a workspace, which a stream capture cannot")
 
 
+_COUNTS = 8192                                                  # bytes at such a workspace's start that are counters
+
+
 def _fresh_workspace(size: int, zeroed: int, device) -> torch.Tensor:
     """A workspace with its counters zeroed.  Inside a stream capture it comes from the graph's own memory: two graphs never
     share one, and each replay zeroes the counters."""
@@ -129,16 +132,15 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
 
 
 _CROSS_WS = {}
-_CROSS_COUNTS = 8192             # bytes at a workspace's start that are counters
 
 
 def _cross_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
     """The workspace of one stream (40 MB at d 128), its counters zeroed."""
     if torch._C._cuda_isCurrentStreamCapturing():
-        return _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _CROSS_COUNTS, device)
+        return _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device)
     ws = _CROSS_WS.get((device.index, stream, d))
     if ws is None:
-        ws = _CROSS_WS[(device.index, stream, d)] = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _CROSS_COUNTS, device)
+        ws = _CROSS_WS[(device.index, stream, d)] = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device)
     return ws
 
 
@@ -399,7 +401,7 @@ class PagePool:
         lib, stream = L.lib(), _raw_stream(self._index)
         size = lib.kvb_page_attend_shared_workspace(self._p, n, hq, tq)
         if torch._C._cuda_isCurrentStreamCapturing():
-            ws = _fresh_workspace(max(size, 256), self._attend_bytes, self.device)
+            ws = _fresh_workspace(max(size, _COUNTS), _COUNTS, self.device)
         else:
             ws = self._workspace("attend_shared", stream, size)
         st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, shared.slots.data_ptr(), n,
