@@ -5,12 +5,14 @@
 // block that all of its members hold in full.  A class's number is its first member, so the result does not depend on timing.
 //
 // One block: the classes of a round come from a hash table in shared memory (class and page, the least index and the count by
-// atomics), the common blocks of a member and its class's first by a warp that compares their rows of the table, the order at
+// atomics), the common blocks of a member and its class's first by eight lanes that compare their rows of the table, the order at
 // the end from one sort of (class numbers of all rounds, index), 10 bits each.
 //
 // The floor is the rows of the table read once, n blocks 4 bytes; the time is a chain of latencies (a round: insert, look
 // up, compare, minimum), because everything after a round depends on it.
 #pragma once
+
+#include <climits>
 
 #include "kvb_share_view.cuh"
 
@@ -18,7 +20,7 @@ namespace kvb {
 
 constexpr int PS_THREADS = 1024;
 constexpr int PS_HASH = 2 * PS_MAX_SEQS;      // entries: at most half of them are taken
-constexpr int PS_UNROLL = 4;                  // entries of a row that a lane has in flight
+constexpr int PS_UNROLL = 8;                  // entries of either row that a lane has in flight
 
 struct ShareSmem {
     unsigned long long key[PS_HASH];          // class << 32 | page
@@ -85,32 +87,38 @@ __global__ void __launch_bounds__(PS_THREADS, 1) page_share_kernel(const __grid_
             more = __syncthreads_or(size > 1);
         }
         if (more) {
-            // blocks that a member and its class's first have in common, a warp a member
-            for (int m = warp; m < n; m += PS_THREADS / 32) {
-                const int first = S.leader[m];
-                if (S.size[m] < 2 || first == m) continue;
-                const int stop = min(S.full[m], S.full[first]);
-                const int32_t* a = P.table + int64_t(S.slot[m]) * P.max_blocks;
-                const int32_t* b = P.table + int64_t(S.slot[first]) * P.max_blocks;
-                int same = stop;
-                for (int b0 = S.end[m] + 1; b0 < stop && same == stop; b0 += 32 * PS_UNROLL) {
-                    bool ok[PS_UNROLL];
+            // blocks that a member and its class's first have in common: eight lanes a member, four members a warp, so that the loads
+            // of all 480 members of a call are on their way in four rounds (a warp a member: 41 us a call, 15 rounds of latency)
+            for (int m0 = warp * 4; m0 < n; m0 += PS_THREADS / 8) {
+                const int mb = min(m0 + (lane >> 3), n - 1), first = S.leader[mb], stop = min(S.full[mb], S.full[first]);
+                const bool compares = m0 + (lane >> 3) < n && S.size[mb] > 1 && first != mb;
+                const int32_t* a = P.table + int64_t(compares ? S.slot[mb] : 0) * P.max_blocks;
+                const int32_t* b = P.table + int64_t(compares ? S.slot[first] : 0) * P.max_blocks;
+                int same = stop, b0 = S.end[mb] + 1;
+                bool active = compares && b0 < stop;
+                while (__any_sync(0xffffffffu, active)) {
+                    int ids[PS_UNROLL], others[PS_UNROLL];
 #pragma unroll
                     for (int u = 0; u < PS_UNROLL; ++u) {
-                        const int x = b0 + 32 * u + lane;
-                        ok[u] = true;
-                        if (x < stop) {
-                            const int id = a[x];
-                            ok[u] = id == b[x] && id >= 0 && id < P.n_pages;
-                        }
+                        const int x = b0 + 8 * u + (lane & 7);
+                        const bool in = active && x < stop;
+                        ids[u] = in ? a[x] : 0;
+                        others[u] = in ? b[x] : 0;
                     }
+                    int differ = INT_MAX;
 #pragma unroll
-                    for (int u = PS_UNROLL - 1; u >= 0; --u) {
-                        const uint32_t differ = ~__ballot_sync(0xffffffffu, ok[u]);
-                        if (differ) same = b0 + 32 * u + __ffs(int(differ)) - 1;
+                    for (int u = PS_UNROLL - 1; u >= 0; --u)
+                        if (ids[u] != others[u] || ids[u] < 0 || ids[u] >= P.n_pages) differ = b0 + 8 * u + (lane & 7);
+                    differ = min(differ, __shfl_xor_sync(0xffffffffu, differ, 1));
+                    differ = min(differ, __shfl_xor_sync(0xffffffffu, differ, 2));
+                    differ = min(differ, __shfl_xor_sync(0xffffffffu, differ, 4));
+                    if (active) {
+                        same = min(same, differ);
+                        b0 += 8 * PS_UNROLL;
+                        active = differ == INT_MAX && b0 < stop;
                     }
                 }
-                if (lane == 0) atomicMin(&S.common[first], same);
+                if (compares && (lane & 7) == 0) atomicMin(&S.common[first], same);
             }
             __syncthreads();
             alive = size > 1;
