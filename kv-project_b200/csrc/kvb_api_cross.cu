@@ -39,7 +39,7 @@ kvb_status launch(kvb::CrossParams a, cudaStream_t s) {
         a.n = std::min(n - i, kvb::CR_MAX_SEQS);
         if (kvb_status st = launch_chained("cross_attention", kern, grid, THREADS, SM, s, a)) return st;
         if (MANY)
-            if (kvb_status st = launch_chained("cross_attention join", kvb::cross_join_kernel<T, D>, 2 * grid, 32 * kvb::CJ_WARPS, 0, s, a)) return st;
+            if (kvb_status st = launch_chained("cross_attention join", kvb::cross_join_kernel<T, D>, 4 * grid, 32 * kvb::CJ_WARPS, 0, s, a)) return st;
         a.cu_q += kvb::CR_MAX_SEQS;
         a.cu_k += kvb::CR_MAX_SEQS;
     }

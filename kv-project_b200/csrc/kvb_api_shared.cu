@@ -27,7 +27,7 @@ kvb_status launch_segments(const kvb::SharedTcParams& a, cudaStream_t s) {
     static std::atomic<uint64_t> done{0};
     if (kvb_status st = kvbh::allow_smem("page_attend_shared", reinterpret_cast<const void*>(kern), SM, done)) return st;
     if (kvb_status st = launch_chained("page_attend_shared", kern, unsigned(a.ctas), 32 * kvb::ST_WARPS, SM, s, a)) return st;
-    return launch_chained("page_attend_shared join", kvb::shared_join_kernel<D>, unsigned(2 * a.ctas), 32 * kvb::CJ_WARPS, 0, s, a);
+    return launch_chained("page_attend_shared join", kvb::shared_join_kernel<D>, unsigned(4 * a.ctas), 32 * kvb::CJ_WARPS, 0, s, a);
 }
 
 }  // namespace

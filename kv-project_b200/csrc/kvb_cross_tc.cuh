@@ -355,7 +355,7 @@ struct CrossItem {
 
 // Joins the items that cross_many_kernel cut.
 template <typename T, int D>
-__global__ void __launch_bounds__(32 * CJ_WARPS) cross_join_kernel(const __grid_constant__ CrossParams A) {
+__global__ void __launch_bounds__(32 * CJ_WARPS, 4) cross_join_kernel(const __grid_constant__ CrossParams A) {
     __shared__ int pre[CR_MAX_SEQS + 1], shares[CR_MAX_SEQS + 1], warp_sum[2][CJ_WARPS];
     __shared__ CjSmem<CrossItem> S;
     PdPlan<true, CM_FIXED> W;

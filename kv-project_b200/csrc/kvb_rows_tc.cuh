@@ -426,7 +426,7 @@ __device__ __forceinline__ CmCut cm_cut(const PdPlan<true, FIXED>& W, int b) {
 // Row r of a cut item, 4 channels from ch: the parts in the order of the keys, O over its own reference topw.
 template <int D, bool WREF>
 __device__ __forceinline__ void cm_join_row(const float* part, const CmCut& x, int r, int ch, float (&acc)[4], float& top, float& sum, float& topw) {
-    constexpr int B = 8;                                         // partials whose loads are in flight together
+    constexpr int B = 4;                                         // partials whose loads are in flight together
     top = topw = -INFINITY;
     sum = 0.f;
 #pragma unroll

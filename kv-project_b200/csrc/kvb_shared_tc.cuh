@@ -527,7 +527,7 @@ struct SharedItem {
 
 // Joins the items that shared_pages_kernel cut.
 template <int D>
-__global__ void __launch_bounds__(32 * CJ_WARPS) shared_join_kernel(const __grid_constant__ SharedTcParams A) {
+__global__ void __launch_bounds__(32 * CJ_WARPS, 4) shared_join_kernel(const __grid_constant__ SharedTcParams A) {
     __shared__ int pre[PS_MAX_SEQS + 1], shares[PS_MAX_SEQS + 1], warp_sum[2][CJ_WARPS];
     __shared__ CjSmem<SharedItem> S;
     PdPlan<true, CM_FIXED> W;
