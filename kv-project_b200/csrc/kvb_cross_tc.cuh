@@ -175,24 +175,26 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                 float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 uint32_t w[CM_KEYS / 2];
                 // of four pairs of keys CM_FMA on the FMA pipe: with all on the special-function unit, which the two
-                // warpgroups share, it is what bounds the step
-                auto weights = [&](auto plain) {
+                // warpgroups share, it is what bounds the step.  Rows with NaN or infinities, or that have seen nothing, want the exact
+                // limits (masked keys, -inf, give 0 on either); what their neighbours get does not depend on them.
+                const bool plain = fabsf(y) < INFINITY;
+                auto weights = [&](auto all) {
 #pragma unroll
                     for (int i = 0; i < CM_KEYS / 2; ++i) {
-                        float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
-                        if (plain && i % 4 < CM_FMA) {
-                            e = cm_ex2<T>(e);
-                        } else {
-                            e.x = ex2(e.x);
-                            e.y = ex2(e.y);
+                        const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                        float2 e = x;
+                        if (i % 4 < CM_FMA) e = cm_ex2<T>(x);
+                        if (i % 4 >= CM_FMA || (!all && !plain)) {
+                            e.x = ex2(x.x);
+                            e.y = ex2(x.y);
                         }
                         sum[i & 1] = cm_add2(sum[i & 1], e);
                         w[i] = pack_f32<T>(e.x, e.y);
                     }
                 };
-                // NaN and infinities, masked keys and rows that have seen nothing want the exact limits
-                if (__all_sync(0xffffffffu, fabsf(y) < INFINITY) && left >= CM_KEYS) weights(std::true_type{});
+                if (__all_sync(0xffffffffu, plain)) weights(std::true_type{});
                 else weights(std::false_type{});
+                __syncwarp();
                 cm_st32(cols, w);
                 const float2 both = cm_add2(sum[0], sum[1]);
                 l += both.x + both.y;

@@ -286,37 +286,38 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                 float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 uint32_t w[CM_KEYS / 2];
                 const float2 ref2{-ref, -ref};
-                // NaN and infinities, masked tokens, rows that have seen nothing and value scales that lie very far apart want every
-                // weight from its own exponent
-                plain = plain && fabsf(y) < INFINITY && fmaxf(fmaxf(lv[0], lv[1]), fmaxf(lv[2], lv[3])) + dr < 100.f;
-                if (__all_sync(0xffffffffu, plain)) {
+                // Rows with NaN or infinities, that have seen nothing, or whose value scales lie very far apart want every weight from
+                // its own exponent (masked tokens, -inf, give 0 on either way); what their neighbours get does not depend on them.
+                plain = fabsf(y) < INFINITY && fmaxf(fmaxf(lv[0], lv[1]), fmaxf(lv[2], lv[3])) + dr < 100.f;
+                auto weights = [&](auto all) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
                         const float f = ex2(lv[g] + dr);
-                        const float2 lam2{lamk[g], lamk[g]}, f2{f, f};
+                        const float2 lam2{fabsf(lamk[g]), fabsf(lamk[g])}, f2{f, f};
 #pragma unroll
                         for (int k = 0; k < 8; ++k) {
                             const int i = 8 * g + k;
-                            float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                            const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                            float2 e = x;
                             if (i % 4 < CM_FMA) {
-                                e = cm_ex2<__half>(e);
+                                e = cm_ex2<__half>(x);
                             } else {
-                                e.x = ex2(e.x);
-                                e.y = ex2(e.y);
+                                e.x = ex2(x.x);
+                                e.y = ex2(x.y);
+                            }
+                            float2 y = cm_mul2(e, f2);
+                            if (!all && !plain) {
+                                e = float2{ex2(x.x), ex2(x.y)};
+                                y = float2{ex2(x.x + (lv[g] + dr)), ex2(x.y + (lv[g] + dr))};
                             }
                             sum[i & 1] = cm_add2(sum[i & 1], e);
-                            e = cm_mul2(e, f2);
-                            w[i] = pack_half2(e.x, e.y);
+                            w[i] = pack_half2(y.x, y.y);
                         }
                     }
-                } else {
-#pragma unroll
-                    for (int i = 0; i < CM_KEYS / 2; ++i) {
-                        const float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, float2{fabsf(lamk[i / 8]), fabsf(lamk[i / 8])}, ref2);
-                        sum[i & 1] = cm_add2(sum[i & 1], float2{ex2(e.x), ex2(e.y)});
-                        w[i] = pack_half2(ex2(e.x + (lv[i / 8] + dr)), ex2(e.y + (lv[i / 8] + dr)));
-                    }
-                }
+                };
+                if (__all_sync(0xffffffffu, plain)) weights(std::true_type{});
+                else weights(std::false_type{});
+                __syncwarp();
                 cm_st32(cols, w);
                 const float2 both = cm_add2(sum[0], sum[1]);
                 l += both.x + both.y;

@@ -108,3 +108,211 @@ def test_cross(cuda_dev, dtype, d, hkv, rep, queries, keys):
     q = rand(g, sum(queries), hkv * rep, d, dtype=dtype)
     check(q, k, v, cu_of(queries), cu_of(keys))
     check(3 * q, k, v, cu_of(queries), cu_of(keys), -0.11)
+
+
+# ------------------------------------------------------------------------------------------------
+# layouts and edges, few rows (single tokens) and many (prompts)
+# ------------------------------------------------------------------------------------------------
+FORMS = [([1, 2, 1], [130, 70, 515]), ([150, 1, 300], [130, 70, 515])]
+
+
+@pytest.mark.parametrize("queries,keys", FORMS)
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+def test_layouts(cuda_dev, dtype, d, queries, keys):
+    """Head-major storage, rows of a wider tensor, one head expanded to all, strides of extents of one."""
+    g = torch.Generator(device="cuda").manual_seed(5)
+    nq, nk, hkv, rep = sum(queries), sum(keys), 4, 2
+    cq, ck = cu_of(queries), cu_of(keys)
+    q, (k, v) = rand(g, nq, hkv * rep, d, dtype=dtype), states(g, nk, hkv, d, dtype)
+    want = check(q, k.contiguous(), v.contiguous(), cq, ck)
+    major = [x.transpose(0, 1).contiguous().transpose(0, 1) for x in (q, k, v)]
+    assert torch.equal(check(*major, cq, ck), want)
+    wide = torch.zeros(nk, 3, hkv, d + 8, dtype=dtype, device="cuda")
+    wide[:, 1, :, :d], wide[:, 2, :, :d] = k, v
+    assert torch.equal(check(q, wide[:, 1, :, :d], wide[:, 2, :, :d], cq, ck), want)
+    one, two = k[:, :1].contiguous(), v[:, 1:2].contiguous()
+    want = check(q, one.repeat(1, hkv, 1), two.repeat(1, hkv, 1), cq, ck)
+    assert torch.equal(check(q, one.expand(-1, hkv, -1), two.expand(-1, hkv, -1), cq, ck), want)
+    check(q[:, :1], one.as_strided((nk, 1, d), (one.stride(0), 3, 1)), two, cq, ck)            # a stride of an extent of one
+    check(q[:1], k, v, cu_of([1]), cu_of([nk]))
+
+
+@pytest.mark.parametrize("queries,keys", FORMS)
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 64), (torch.float16, 128)])
+def test_what_is_not_the_sequences_does_not_matter(cuda_dev, dtype, d, queries, keys):
+    """NaN and infinities in the rows behind a sequence's last key (the next sequence's first), rows of no sequence, outputs
+    of no sequence."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(6)
+    gap = [0] + [x for n in keys for x in (n, 5)]              # five rows of nobody after each
+    edges = np.cumsum(gap)
+    nk, nq, hkv, rep = int(edges[-1]), sum(queries) + 7, 2, 4
+    k, v = rand(g, nk, hkv, d, dtype=dtype), rand(g, nk, hkv, d, dtype=dtype)
+    q = rand(g, nq, hkv * rep, d, dtype=dtype)
+    cq = cu_of(queries)
+    for a in range(len(keys)):                                  # one sequence at a time has keys; the others are empty
+        lo, hi = int(edges[2 * a]), int(edges[2 * a + 1])
+        ck = torch.tensor([lo] * (a + 1) + [hi] * (len(keys) - a), dtype=torch.int32, device="cuda")
+        kk, vv = k.clone(), v.clone()
+        for x, bad in ((kk, float("inf")), (vv, float("nan"))):
+            x[:lo], x[hi:] = bad, bad
+        kk[hi:hi + 2] = float("nan")
+        out = torch.full((nq, hkv * rep, d), 7.0, dtype=dtype, device="cuda")
+        got = kvb.cross_attention(q, kk, vv, cq, ck, out=out)
+        assert got is out and (out[sum(queries):] == 7).all()
+        want = kvb.cross_attention(q, torch.where(torch.isfinite(kk), kk, 0), torch.where(torch.isfinite(vv), vv, 0), cq, ck)
+        assert torch.equal(out[:sum(queries)], want[:sum(queries)]) and torch.isfinite(out).all()
+        for b in range(len(keys)):
+            rows = out[int(cq[b]):int(cq[b + 1])]
+            assert (rows == 0).all() if b != a else (rows != 0).any()
+
+
+@pytest.mark.parametrize("queries,keys", FORMS)
+def test_a_row_that_is_not_finite_stays_alone(cuda_dev, queries, keys):
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(7)
+    q, (k, v) = rand(g, sum(queries), 8, 128, dtype=torch.bfloat16), states(g, sum(keys), 2, 128, torch.bfloat16)
+    cq, ck = cu_of(queries), cu_of(keys)
+    clean = kvb.cross_attention(q, k, v, cq, ck)
+    for at, value in (((0, 3, 5), float("nan")), ((sum(queries) - 1, 0, 0), float("inf"))):
+        p = q.clone()
+        p[at] = value
+        got, lse = kvb.cross_attention(p, k, v, cq, ck, return_lse=True)
+        hurt = torch.zeros(got.shape[:2], dtype=torch.bool, device="cuda")
+        hurt[at[:2]] = True
+        assert torch.equal(got[~hurt], clean[~hurt]) and torch.isnan(got[hurt]).all() and torch.isnan(lse[hurt]).all()
+
+
+@pytest.mark.parametrize("queries", [[1, 1], [300, 200]])
+@pytest.mark.parametrize("scaling", [0.0, 1e-30, -1.0, 2.5])
+def test_any_scaling(cuda_dev, scaling, queries):
+    g = torch.Generator(device="cuda").manual_seed(8)
+    q, (k, v) = rand(g, sum(queries), 4, 64, dtype=torch.float16), states(g, 700, 2, 64, torch.float16)
+    check(q, k, v, cu_of(queries), cu_of([333, 367]), scaling)
+
+
+@pytest.mark.parametrize("dtype,d", [(torch.bfloat16, 128), (torch.float16, 64)])
+@pytest.mark.parametrize("queries", [2, 200])
+def test_maxima_that_keep_growing(cuda_dev, dtype, d, queries):
+    """Logits that rise by more than 2^8 from unit to unit, fall again, and one key far above all."""
+    g = torch.Generator(device="cuda").manual_seed(9)
+    n = 1500
+    v = rand(g, n, 1, d, dtype=dtype)
+    way = torch.randn(d, generator=g, device="cuda")
+    way /= way.norm()
+    rise = torch.cat([torch.linspace(-60, 60, 1000, device="cuda"), torch.linspace(60, -60, 500, device="cuda")])
+    for spike in (None, 777):
+        x = rise.clone()
+        if spike:
+            x[spike] = 90
+        k = (x[:, None] * way).to(dtype)[:, None]
+        q = (way * (1 + 0.3 * torch.randn(queries, 1, 1, generator=g, device="cuda"))).to(dtype).expand(-1, 4, -1).contiguous()
+        check(q, k, v, cu_of([queries]), cu_of([n]), 1.0)
+
+
+@pytest.mark.parametrize("per", [1, 40])
+def test_more_sequences_than_one_launch_takes(cuda_dev, per):
+    g = torch.Generator(device="cuda").manual_seed(10)
+    n = 1100
+    keys = [(i * 7) % 40 for i in range(n)]
+    q, (k, v) = rand(g, n * per, 4, 64, dtype=torch.float16), states(g, sum(keys), 1, 64, torch.float16)
+    check(q, k, v, cu_of([per] * n), cu_of(keys))
+
+
+def test_long_states(cuda_dev):
+    """Items cut over many blocks: single rows, a tile's, two tiles' over 40000 keys."""
+    g = torch.Generator(device="cuda").manual_seed(11)
+    k, v = states(g, 40000, 1, 128, torch.bfloat16)
+    for rows in (1, 20, 90):
+        q = rand(g, rows, 4, 128, dtype=torch.bfloat16)
+        check(q, k, v, cu_of([rows]), cu_of([40000]))
+
+
+def test_empty_calls_and_refusals(cuda_dev):
+    import kvb
+    q, k = torch.randn(5, 4, 64, device="cuda").half(), torch.randn(9, 2, 64, device="cuda").half()
+    cq, ck = cu_of([5]), cu_of([9])
+    assert kvb.cross_attention(q[:0], k, k, cu_of([0]), ck).shape == (0, 4, 64)
+    assert kvb.cross_attention(q, k, k, cu_of([]), cu_of([])).shape == q.shape
+    out, lse = kvb.cross_attention(q, k[:0], k[:0], cq, cu_of([0]), return_lse=True)
+    assert (out == 0).all() and torch.isneginf(lse).all()
+    for bad in (dict(q=q.float()), dict(q=q.bfloat16()), dict(v=k[:8]), dict(q=q[:, :, :32]), dict(q=q[:, :3]), dict(cu_q=cq.long()), dict(cu_k=cq.cpu()),
+                dict(cu_k=cu_of([4, 5])), dict(k=k.cpu()), dict(q=q.transpose(1, 2)), dict(out=q[:4]), dict(out=q.float()), dict(scaling=float("nan")),
+                dict(out=torch.empty(5 * 256 + 4, device="cuda", dtype=torch.float16)[4:].view(5, 4, 64)),
+                dict(k=torch.empty(9 * 128 + 3, device="cuda", dtype=torch.float16)[3:].view(9, 2, 64))):
+        a = dict(q=q, k=k, v=k, cu_q=cq, cu_k=ck)
+        a.update(bad)
+        with pytest.raises((ValueError, NotImplementedError)):
+            kvb.cross_attention(**a)
+    with pytest.raises(NotImplementedError):
+        kvb.cross_attention(q.float(), k.float(), k.float(), cq, ck)
+    with pytest.raises(NotImplementedError):
+        kvb.cross_attention(q, k[:1].expand(9, -1, -1), k, cq, ck)                 # rows that are one
+
+
+@pytest.mark.parametrize("rows", [1, 100])
+def test_offsets_that_do_not_fit(cuda_dev, rows):
+    """The sequence is left out, the others are not."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(12)
+    q, (k, v) = rand(g, 3 * rows, 4, 64, dtype=torch.float16), states(g, 300, 2, 64, torch.float16)
+    good = cu_of([rows] * 3), cu_of([100] * 3)
+    want = kvb.cross_attention(q, k, v, *good)
+    ints = lambda x: torch.tensor(x, dtype=torch.int32, device="cuda")            # noqa: E731
+    for cq, ck, whole in ((good[0], ints([0, 100, 200, 301]), [0, 1]), (good[0], ints([0, 100, 90, 190]), [0]), (ints([0, rows, 2 * rows, 3 * rows + 1]), good[1], [0, 1]),
+                          (ints([-1, rows, 2 * rows, 3 * rows]), good[1], [1, 2]), (ints([0, rows, 2 * rows, -2 ** 31]), good[1], [0, 1]),
+                          (good[0], ints([0, 100, 200, 2 ** 31 - 1]), [0, 1])):
+        out = torch.full_like(q, 3)
+        kvb.cross_attention(q, k, v, cq, ck, out=out)
+        assert status() == 2
+        for s in whole:
+            assert torch.equal(out[s * rows:(s + 1) * rows], want[s * rows:(s + 1) * rows])
+
+
+@pytest.mark.parametrize("queries", [1, 130])
+def test_streams_and_graphs(cuda_dev, queries):
+    """Calls on two streams at once; a captured call replayed over other lengths and other contents; two graphs replayed at
+    once share nothing."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(13)
+    keys = [3000, 77]
+    q, (k, v) = rand(g, 2 * queries, 8, 128, dtype=torch.bfloat16), states(g, sum(keys), 2, 128, torch.bfloat16)
+    cq, ck = cu_of([queries] * 2), cu_of(keys)
+    want = check(q, k, v, cq, ck)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        there = [kvb.cross_attention(q, k, v, cq, ck) for _ in range(50)]
+    here = [kvb.cross_attention(q, k, v, cq, ck) for _ in range(50)]
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for x in there + here)
+    graphs, outs = [], []
+    for _ in range(2):
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append([kvb.cross_attention(q, k, v, cq, ck) for _ in range(3)])
+        graphs.append(graph)
+    for lens in ([3000, 77], [1, 3076], [3077, 0], [1500, 1577]):
+        ck.copy_(cu_of(lens))
+        q.copy_(rand(g, *q.shape, dtype=q.dtype))
+        want = kvb.cross_attention(q, k, v, cq, ck)
+        torch.cuda.synchronize()
+        for _ in range(20):
+            for graph, stream in zip(graphs, (torch.cuda.current_stream(), side)):
+                with torch.cuda.stream(stream):
+                    graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, want) for out in outs for x in out)
+
+
+@pytest.mark.parametrize("queries", [1, 130])
+def test_many_calls_give_the_same_bits(cuda_dev, queries):
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(14)
+    keys = [700, 0, 64, 1999]
+    q, (k, v) = rand(g, 4 * queries, 8, 128, dtype=torch.float16), states(g, sum(keys), 2, 128, torch.float16)
+    cq, ck = cu_of([queries] * 4), cu_of(keys)
+    want, same = kvb.cross_attention(q, k, v, cq, ck), torch.ones((), dtype=torch.bool, device="cuda")
+    for _ in range(2000):
+        same &= (kvb.cross_attention(q, k, v, cq, ck) == want).all()
+    assert bool(same)

@@ -67,3 +67,25 @@ def test_oracle_finds_what_forks_share():
     assert s["segments"] == [[1, 4, 0, 32, 0], [1, 2, 32, 48, 1]]
     assert s["own"] == [0, 48, 32, 32, 48] and s["depth"] == [0, 2, 1, 1, 2]
     assert O.share(pool, [2])["own"] == [0]
+
+
+@pytest.mark.parametrize("change,status,word", [
+    (dict(q=None), 1, "null"), (dict(cu_k=None), 1, "null"), (dict(workspace=None), 1, "null"), (dict(nq=-1), 1, "n >= 0"),
+    (dict(nk=1 << 31), 1, "row counts"), (dict(Hq=5), 1, "Hq"), (dict(Hkv=0), 1, "Hq"), (dict(dtype=0), 4, "float16"), (dict(d=32), 4, "d 64"),
+    (dict(q_row=516), 1, "strides"), (dict(v_head=-128), 1, "strides"), (dict(k_row=0), 4, "rows of their own"), (dict(q=A + 8), 1, "alignment"),
+    (dict(out=A + 16), 1, "alignment"), (dict(scaling=float("nan")), 1, "finite"), (dict(workspace=A + 8), 1, "workspace"),
+    (dict(workspace_bytes=64), 1, "workspace"), (dict(nq=1 << 30, Hq=64, Hkv=1, k_head=0), 4, "too many"),
+    (dict(nq=1 << 24, nk=1 << 30, n=1), 4, "too many")])
+def test_cross(change, status, word):
+    a = dict(q=A, k=A, v=A, dtype=2, nq=10, nk=10, Hq=4, Hkv=2, d=128, q_row=512, q_head=128, k_row=256, k_head=128, v_row=256,
+             v_head=128, cu_q=A, cu_k=A, n=1, scaling=0.1, out=A, lse=None, workspace=A, workspace_bytes=B, stream=None)
+    a.update(change)
+    st, msg = call("kvb_cross_attention", *a.values())
+    assert st == status and word in msg and "cross_attention" in msg, (st, msg)
+
+
+def test_cross_sizes():
+    from kvb import _lib
+    f = _lib.lib().kvb_cross_workspace
+    assert f(32) == f(0) == 0 and 8192 < f(64) < f(128)
+    assert call("kvb_cross_attention", *[None] * 3, 2, 0, 0, 4, 2, 128, *[0] * 6, None, None, 0, 0.1, None, None, None, 0, None)[0] == 0
