@@ -183,7 +183,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     for (int i = 0; i < CM_KEYS / 2; ++i) {
                         const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
                         float2 e = x;
-                        if (i % 4 < CM_FMA) e = cm_ex2<T>(x);
+                        if (i % 4 < CM_FMA) e = cm_ex2(x);
                         if (i % 4 >= CM_FMA || (!all && !plain)) {
                             e.x = ex2(x.x);
                             e.y = ex2(x.y);

@@ -300,7 +300,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                             const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
                             float2 e = x;
                             if (i % 4 < CM_FMA) {
-                                e = cm_ex2<__half>(x);
+                                e = cm_ex2(x);
                             } else {
                                 e.x = ex2(x.x);
                                 e.y = ex2(x.y);
