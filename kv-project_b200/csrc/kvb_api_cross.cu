@@ -9,6 +9,8 @@ namespace {
 constexpr int kFewRows = 16;
 
 constexpr size_t kCrossCounts = size_t(kvb::PD_MAX_CTAS) * kvb::CR_WARPS * 4;
+constexpr size_t kCrossCuts = kvb::PD_MAX_CTAS * sizeof(kvb::CmCut<kvb::CrossItem>);
+static_assert(kCrossCuts % 256 == 0, "the partials begin on a 256-byte boundary");
 
 // Rows (nk, heads, d) with their strides as (d, heads, rows), box 64 channels x 1 x `rows`, 128-byte swizzle.  A head stride of
 // zero (one head for all) is a map of one head.
@@ -58,7 +60,7 @@ extern "C" {
 
 size_t kvb_cross_workspace(int d) {
     // two partials a CTA: of 2 x 128 rows (cross_many_kernel), of 16 (cross_few_kernel)
-    return d == 64 || d == 128 ? kCrossCounts + size_t(2) * cross_ctas() * 2 * kvb::CM_ROWS * (d + 3) * 4 : 0;
+    return d == 64 || d == 128 ? kCrossCounts + kCrossCuts + size_t(2) * cross_ctas() * 2 * kvb::CM_ROWS * (d + 3) * 4 : 0;
 }
 
 kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
@@ -117,7 +119,8 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
     a.out = out;
     a.lse = lse;
     a.count = static_cast<uint32_t*>(workspace);
-    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCrossCounts);
+    a.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kCrossCounts + kCrossCuts);
+    a.cuts = static_cast<char*>(workspace) + kCrossCounts;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     return many ? launch_any<true>(a, dtype, d, s) : launch_any<false>(a, dtype, d, s);
 }

@@ -13,11 +13,13 @@ constexpr int64_t kTogether = 220;          // see PD_LONE
 
 int shared_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
 
-// The workspace: counters; partials of cut items, first of the segments, then of the sequences' own tokens (the former are
+constexpr int64_t kCuts = (kvb::PD_MAX_CTAS * sizeof(kvb::CmCut<kvb::SharedItem>) + 255) / 256 * 256;
+
+// The workspace: counters; what is cut; partials of cut items, first of the segments, then of the sequences' own tokens (the former are
 // joined by then); the rows' parts by level.
 int64_t level_offset(int d) {
     const int64_t segments = int64_t(2) * shared_ctas() * 2 * kvb::CM_ROWS * (d + 3), own = int64_t(2) * shared_ctas() * 8 * 16 * (d + 4);
-    return kvbh::kCountBytes + (std::max(segments, own) * 4 + 255) / 256 * 256;
+    return kvbh::kCountBytes + kCuts + (std::max(segments, own) * 4 + 255) / 256 * 256;
 }
 
 template <typename T, int D>
@@ -93,7 +95,8 @@ kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, 
         b.rows = a.rows;
         b.level_o = a.level_o;
         b.level_ml = a.level_ml;
-        b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kvbh::kCountBytes);
+        b.cuts = static_cast<char*>(workspace) + kvbh::kCountBytes;
+        b.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + kvbh::kCountBytes + kCuts);
         b.ctas = shared_ctas();
         kvb_status st = dtype == KVB_F16 ? p->d == 128 ? launch_segments<__half, 128>(b, s) : launch_segments<__half, 64>(b, s)
                         : p->d == 128    ? launch_segments<__nv_bfloat16, 128>(b, s)

@@ -42,7 +42,8 @@ struct CrossParams {
     float* lse;                               // (nq, Hq) or null
     float* part;                              // two a CTA: O, maximum, sum
     uint32_t* count;                          // cross_few_kernel: [grid][8 warps]
-    int ctas;                                 // cross_many_kernel: that take part
+    void* cuts;                               // cross_many_kernel: CmCut<CrossItem> a CTA
+    int ctas;                                 // that take part
 };
 
 template <int D>

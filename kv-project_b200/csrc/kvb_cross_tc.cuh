@@ -22,6 +22,11 @@ struct CrossTcShape {
     static constexpr int SMEM = 1024 + 2 * S::QTILE + 2 * CM_STAGES * S::TILE + S::XBYTES;
 };
 
+struct CrossItem {
+    int64_t row;                              // of out: the sequence's first token, the KV head's first query head
+    int row0;
+};
+
 // The work of a call dealt to `ctas` CTAs; false when there is none.  Whole block.
 template <int WARPS>
 __device__ __forceinline__ bool cross_plan(const CrossParams& A, int ctas, int* pre, int* shares, int (*warp_sum)[WARPS], PdPlan<true, CM_FIXED>& W) {
@@ -61,9 +66,13 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     chain_kernels();
     auto seq_at = [&](int i) { return cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, i); };
     PdPlan<true, CM_FIXED> W;
-    if (!cross_plan<CM_WARPS>(A, A.ctas, pre, shares, warp_sum, W)) return;
     const int cta = blockIdx.x;
-    if (cta >= W.ctas) return;
+    const bool any = cross_plan<CM_WARPS>(A, A.ctas, pre, shares, warp_sum, W);
+    CmCut<CrossItem>* const cuts = static_cast<CmCut<CrossItem>*>(A.cuts);
+    if (!any || cta >= W.ctas) {
+        if (threadIdx.x == 0) cuts[cta] = CmCut<CrossItem>{};
+        return;
+    }
     const int u0 = W.units_before(W.share(cta)), u1 = W.units_before(W.share(cta + 1));
 
     if (warp == CM_SOFTMAX) {
@@ -175,25 +184,23 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                 float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 uint32_t w[CM_KEYS / 2];
                 // of four pairs of keys CM_FMA on the FMA pipe: with all on the special-function unit, which the two
-                // warpgroups share, it is what bounds the step.  Rows with NaN or infinities, or that have seen nothing, want the exact
-                // limits (masked keys, -inf, give 0 on either); what their neighbours get does not depend on them.
-                const bool plain = fabsf(y) < INFINITY;
-                auto weights = [&](auto all) {
+                // warpgroups share, it is what bounds the step.  -inf gives 0 on either.
 #pragma unroll
-                    for (int i = 0; i < CM_KEYS / 2; ++i) {
-                        const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
-                        float2 e = x;
-                        if (i % 4 < CM_FMA) e = cm_ex2(x);
-                        if (i % 4 >= CM_FMA || (!all && !plain)) {
-                            e.x = ex2(x.x);
-                            e.y = ex2(x.y);
-                        }
-                        sum[i & 1] = cm_add2(sum[i & 1], e);
-                        w[i] = pack_f32<T>(e.x, e.y);
+                for (int i = 0; i < CM_KEYS / 2; ++i) {
+                    float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                    if (i % 4 < CM_FMA) {
+                        e = cm_ex2(e);
+                    } else {
+                        e.x = ex2(e.x);
+                        e.y = ex2(e.y);
                     }
-                };
-                if (__all_sync(0xffffffffu, plain)) weights(std::true_type{});
-                else weights(std::false_type{});
+                    sum[i & 1] = cm_add2(sum[i & 1], e);
+                    w[i] = pack_f32<T>(e.x, e.y);
+                }
+                if (!(y < INFINITY)) {                           // NaN or +inf among the logits: the row is NaN
+                    sum[0].x = NAN;
+                    w[0] = 0x7fff7fffu;
+                }
                 __syncwarp();
                 cm_st32(cols, w);
                 const float2 both = cm_add2(sum[0], sum[1]);
@@ -226,7 +233,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             cm_after();
             const bool whole = done.p.a == 0 && done.p.b == done.p.units, two = split && done.tiles > 1;
             const int tile0 = split ? 0 : t * CM_ROWS;
-            float* const part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * CM_PART<D> + int64_t(tile0 + r) * D;
+            float* const part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * CM_PART<D>;
             auto out_row = [&](int r) {                          // row r of the item in out and lse
                 const int at = done.row0 + r, tok = pd_div(at, A.by_rep);
                 return (int64_t(done.s.q0) + tok) * A.Hq + done.h * A.rep + at - tok * A.rep;
@@ -284,7 +291,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                                 cm_store32(static_cast<T*>(A.out) + row * D + 32 * c + 16 * i, w);
                             }
                         } else {
-                            cm_put(part + 32 * c, v);
+                            cm_put(part + (tile0 + r) * D + 32 * c, v);
                         }
                     }
                     __syncwarp();
@@ -293,9 +300,8 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                     if (whole) {
                         store_lse(row, m, l);
                     } else {
-                        float* st = part - int64_t(tile0 + r) * D + 2 * CM_ROWS * D + tile0 + r;
-                        __stcg(st, m);
-                        __stcg(st + 2 * CM_ROWS, l);
+                        __stcg(part + 2 * CM_ROWS * D + tile0 + r, m);
+                        __stcg(part + 2 * CM_ROWS * (D + 1) + tile0 + r, l);
                     }
                 }
             }
@@ -307,6 +313,16 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     } else if (warp == CM_SOFTMAX) {
         cm_issue_scores<D, BF16, CM_STAGES>(B, tmem, smem_u32(sq), smem_u32(sk), u0, u1, step_at);
     } else if (warp < CM_SOFTMAX + 3) {
+        // the second of these has the time: the joining kernel is told what this CTA's end cuts
+        if (warp == CM_SOFTMAX + 2 && lane == 0)
+            cm_note_cut(W, cta, cuts, [&](const PdPiece& p, CrossItem& x) {
+                const CrSeq s = seq_at(p.seq);
+                const int groups = W.heads(p.seq) / A.Hkv, h = p.vh / groups;
+                x.row0 = (p.vh - h * groups) * 2 * CM_ROWS;
+                x.row = int64_t(s.q0) * A.Hq + h * A.rep;
+                return min(s.ql * A.rep - x.row0, 2 * CM_ROWS);
+            });
+        __syncwarp();
         cm_issue_values<D, BF16, CM_STAGES>(B, tmem, smem_u32(sv), warp - CM_SOFTMAX - 1, u0, u1, step_at);
     } else {
         // ---------------- copies ----------------
@@ -350,27 +366,11 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
     if (warp == CM_SOFTMAX) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(CM_TMEM));
 }
 
-struct CrossItem {
-    int64_t row;                              // of out: the sequence's first token, the KV head's first query head
-    int row0;
-};
-
 // Joins the items that cross_many_kernel cut.
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * CJ_WARPS, 4) cross_join_kernel(const __grid_constant__ CrossParams A) {
-    __shared__ int pre[CR_MAX_SEQS + 1], shares[CR_MAX_SEQS + 1], warp_sum[2][CJ_WARPS];
-    __shared__ CjSmem<CrossItem> S;
-    PdPlan<true, CM_FIXED> W;
-    if (!cross_plan<CJ_WARPS>(A, A.ctas, pre, shares, warp_sum, W)) return;
-    cm_join<D, false>(W, A.part, S,
-                      [&](const PdPiece& p, CrossItem& x) {
-                          const CrSeq s = cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, p.seq);
-                          const int groups = W.heads(p.seq) / A.Hkv, h = p.vh / groups;
-                          x.row0 = (p.vh - h * groups) * 2 * CM_ROWS;
-                          x.row = int64_t(s.q0) * A.Hq + h * A.rep;
-                          return min(s.ql * A.rep - x.row0, 2 * CM_ROWS);
-                      },
-                      [&](const CrossItem& x, int r, int ch, const float (&o)[4], float top, float sum, float) {
+    cm_join<D, false>(static_cast<const CmCut<CrossItem>*>(A.cuts), A.ctas, A.part,
+                      [&](const CrossItem& x, int r, int ch, const float (&o)[CJ_CH], float top, float sum, float) {
                           const int at = x.row0 + r, tok = pd_div(at, A.by_rep);
                           const int64_t row = x.row + int64_t(tok) * A.Hq + at - tok * A.rep;
                           const float inv = cm_inverse(sum);

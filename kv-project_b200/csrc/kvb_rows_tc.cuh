@@ -377,7 +377,110 @@ __device__ __forceinline__ void cm_rescale(uint32_t to, float f) {
 template <int D>
 constexpr int CM_PART = 2 * CM_ROWS * (D + 3);
 
-// 32 channels of a row of a partial
+// What the joining kernel is told of an item that a CTA's run begins and its end cuts: rows, parts (slot0, then slots 2 c of the
+// CTAs up to c1), and I, which it hands to the function that stores the rows.
+template <typename I>
+struct CmCut {
+    int rows, slot0, c0, c1;
+    I item;
+};
+
+// Of CTA `cta`, by one thread: item_of(piece, item) gives the rows.
+template <int FIXED, typename I, typename F>
+__device__ __forceinline__ void cm_note_cut(const PdPlan<true, FIXED>& W, int cta, CmCut<I>* cuts, F item_of) {
+    CmCut<I> x{};
+    const int u = cta + 1 < W.ctas ? W.units_before(W.share(cta + 1)) : 0;
+    if (u > 0 && u < W.pre[W.n]) {
+        const PdPiece p = pd_piece(W, u, u + 1);
+        if (p.a > 0 && u - p.a >= W.units_before(W.share(cta))) {
+            x.rows = item_of(p, x.item);
+            x.c0 = W.holder(p.v0 + FIXED);
+            x.c1 = W.holder(p.v0 + FIXED + p.units - 1);
+            // the partial of c0 is its first one, unless the item begins inside its run
+            x.slot0 = 2 * x.c0 + (W.share(x.c0) < p.v0 ? 1 : 0);
+        }
+    }
+    cuts[cta] = x;
+}
+
+// Joining, in a kernel of its own after the first (a row's parts may be a hundred, and joined by the block that finishes an item
+// they were most of its time): a warp takes a row of a cut item (two of 64 channels), the parts in the order of the keys.
+constexpr int CJ_WARPS = 8;                   // a thread for each CTA of the first kernel at least
+constexpr int CJ_CH = 4;                      // channels of a lane
+
+template <int D, bool WREF, typename I, typename F>
+__device__ __forceinline__ void cm_join(const CmCut<I>* cuts, int ctas, const float* part, F finish) {
+    __shared__ CmCut<I> cut[32 * CJ_WARPS];
+    __shared__ int before[32 * CJ_WARPS + 1], warp_sum[CJ_WARPS];
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, id = threadIdx.x;
+    chain_kernels();
+    CmCut<I> mine{};
+    if (id < ctas) mine = cuts[id];
+    cut[id] = mine;
+    constexpr int LANES = D / CJ_CH, PER = 32 / LANES;           // of a row; rows of a warp
+    int x = (mine.rows + PER - 1) / PER;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_sum[warp] = x;
+    __syncthreads();
+    for (int w = 0; w < warp; ++w) x += warp_sum[w];
+    before[id + 1] = x;
+    if (id == 0) before[0] = 0;
+    __syncthreads();
+    for (int task = blockIdx.x * CJ_WARPS + warp; task < before[32 * CJ_WARPS]; task += gridDim.x * CJ_WARPS) {
+        int lo = 0;
+#pragma unroll
+        for (int step = 16 * CJ_WARPS; step > 0; step >>= 1)
+            if (before[lo + step] <= task) lo += step;
+        const CmCut<I>& c = cut[lo];
+        const int row = (task - before[lo]) * PER + lane / LANES, ch = lane % LANES * CJ_CH;
+        if (row >= c.rows) continue;
+        constexpr int B = 4;                                     // parts whose loads are in flight together
+        float top = -INFINITY, topw = -INFINITY, sum = 0.f, acc[CJ_CH];
+#pragma unroll
+        for (int i = 0; i < CJ_CH; ++i) acc[i] = 0.f;
+#pragma unroll 1
+        for (int k0 = c.c0; k0 <= c.c1; k0 += B) {
+            float m[B], l[B], w[B];
+            float4 o[B];
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                const float* from = part + int64_t(k0 + k == c.c0 ? c.slot0 : 2 * (k0 + k)) * CM_PART<D>;
+                const bool ok = k0 + k <= c.c1;
+                const float* st = from + 2 * CM_ROWS * D + row;
+                m[k] = ok ? __ldcg(st) : -INFINITY;
+                l[k] = ok ? __ldcg(st + 2 * CM_ROWS) : 0.f;
+                w[k] = !WREF ? m[k] : ok ? __ldcg(st + 4 * CM_ROWS) : -INFINITY;
+                o[k] = ok ? __ldcg(reinterpret_cast<const float4*>(from + row * D + ch)) : float4{0.f, 0.f, 0.f, 0.f};
+            }
+            float most = top, mostw = topw;
+#pragma unroll
+            for (int k = 0; k < B; ++k) most = fmaxf(most, m[k]), mostw = fmaxf(mostw, w[k]);
+            const float ref = most == -INFINITY ? 0.f : most, refw = mostw == -INFINITY ? 0.f : mostw;
+            sum *= ex2(top - ref);
+            const float old = ex2(topw - refw);
+#pragma unroll
+            for (int i = 0; i < CJ_CH; ++i) acc[i] *= old;
+#pragma unroll
+            for (int k = 0; k < B; ++k) {
+                if (k0 + k > c.c1) break;
+                sum = __fmaf_rn(l[k], ex2(m[k] - ref), sum);
+                const float f = ex2(w[k] - refw);
+                acc[0] = __fmaf_rn(o[k].x, f, acc[0]);
+                acc[1] = __fmaf_rn(o[k].y, f, acc[1]);
+                acc[2] = __fmaf_rn(o[k].z, f, acc[2]);
+                acc[3] = __fmaf_rn(o[k].w, f, acc[3]);
+            }
+            top = most, topw = mostw;
+        }
+        finish(c.item, row, ch, acc, top, sum, topw);
+    }
+}
+
+// 32 channels of a row of 32-bit values
 __device__ __forceinline__ void cm_put(float* to, const float (&v)[32]) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -385,124 +488,6 @@ __device__ __forceinline__ void cm_put(float* to, const float (&v)[32]) {
 #pragma unroll
         for (int k = 0; k < 8; ++k) w[k] = __float_as_uint(v[8 * i + k]);
         cm_store32(to + 8 * i, w);
-    }
-}
-
-// Joining, in a kernel of its own after the first (a row's parts may be a hundred, and joined by the block that finishes an item
-// they were most of its time): a row of a cut item a warp (two of 64 channels).
-constexpr int CJ_WARPS = 8;                   // a thread for each CTA of the first kernel at least
-
-struct CmCut {
-    PdPiece p;                                // of the item, from where it is cut first; p.a == 0: none
-    int slot0, c0, c1;                        // its parts: slot0, then slots 2 c of the CTAs up to c1
-};
-// The item that the run of CTA b - 1 begins and its end cuts.
-template <int FIXED>
-__device__ __forceinline__ CmCut cm_cut(const PdPlan<true, FIXED>& W, int b) {
-    CmCut x;
-    x.p.a = 0;
-    x.slot0 = x.c0 = x.c1 = 0;
-    const int u = W.units_before(W.share(b));
-    if (u <= 0 || u >= W.pre[W.n]) return x;
-    x.p = pd_piece(W, u, u + 1);
-    if (x.p.a == 0 || u - x.p.a < W.units_before(W.share(b - 1))) {
-        x.p.a = 0;
-        return x;
-    }
-    x.c0 = W.holder(x.p.v0 + FIXED);
-    x.c1 = W.holder(x.p.v0 + FIXED + x.p.units - 1);
-    // the partial of c0 is its first one, unless the item begins inside its run
-    x.slot0 = 2 * x.c0 + (W.share(x.c0) < x.p.v0 ? 1 : 0);
-    return x;
-}
-
-// Row r of a cut item, 4 channels from ch: the parts in the order of the keys, O over its own reference topw.
-template <int D, bool WREF>
-__device__ __forceinline__ void cm_join_row(const float* part, const CmCut& x, int r, int ch, float (&acc)[4], float& top, float& sum, float& topw) {
-    constexpr int B = 4;                                         // partials whose loads are in flight together
-    top = topw = -INFINITY;
-    sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) acc[i] = 0.f;
-#pragma unroll 1
-    for (int c = x.c0; c <= x.c1; c += B) {
-        float m[B], l[B], w[B];
-        float4 o[B];
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            const float* from = part + int64_t(c + k == x.c0 ? x.slot0 : 2 * (c + k)) * CM_PART<D>;
-            const bool ok = c + k <= x.c1;
-            const float* st = from + 2 * CM_ROWS * D + r;
-            m[k] = ok ? __ldcg(st) : -INFINITY;
-            l[k] = ok ? __ldcg(st + 2 * CM_ROWS) : 0.f;
-            w[k] = !WREF ? m[k] : ok ? __ldcg(st + 4 * CM_ROWS) : -INFINITY;
-            o[k] = ok ? __ldcg(reinterpret_cast<const float4*>(from + r * D + ch)) : float4{0.f, 0.f, 0.f, 0.f};
-        }
-        float most = top, mostw = topw;
-#pragma unroll
-        for (int k = 0; k < B; ++k) most = fmaxf(most, m[k]), mostw = fmaxf(mostw, w[k]);
-        const float ref = most == -INFINITY ? 0.f : most, refw = mostw == -INFINITY ? 0.f : mostw;
-        sum *= ex2(top - ref);
-        const float old = ex2(topw - refw);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) acc[i] *= old;
-#pragma unroll
-        for (int k = 0; k < B; ++k) {
-            sum = __fmaf_rn(l[k], ex2(m[k] - ref), sum);
-            const float f = ex2(w[k] - refw);
-            acc[0] = __fmaf_rn(o[k].x, f, acc[0]);
-            acc[1] = __fmaf_rn(o[k].y, f, acc[1]);
-            acc[2] = __fmaf_rn(o[k].z, f, acc[2]);
-            acc[3] = __fmaf_rn(o[k].w, f, acc[3]);
-        }
-        top = most, topw = mostw;
-    }
-}
-
-// I: what finish() needs of an item
-template <typename I>
-struct CjSmem {
-    CmCut cut[256];                           // by the CTA whose end cuts
-    I item[256];
-    int rows[256], before[257];               // rows of each; warps' tasks before each
-    int warp_sum[CJ_WARPS];
-};
-
-// All cut items: rows_of(piece, item) rows of one, finish(item, row, channel, o, top, sum, topw).  What is cut is found before the parts
-// are waited for: the plan is older than the kernel that writes them, which waited for it before it let this one in.
-template <int D, bool WREF, int FIXED, typename I, typename R, typename F>
-__device__ __forceinline__ void cm_join(const PdPlan<true, FIXED>& W, const float* part, CjSmem<I>& S, R rows_of, F finish) {
-    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, id = threadIdx.x;
-    constexpr int LANES = D / 4, PER = 32 / LANES;               // of a row; rows of a warp
-    CmCut mine;
-    mine.p.a = 0;
-    if (id + 1 < W.ctas) mine = cm_cut(W, id + 1);
-    const int rows = mine.p.a > 0 ? rows_of(mine.p, S.item[id]) : 0, tasks = (rows + PER - 1) / PER;
-    S.cut[id] = mine;
-    S.rows[id] = rows;
-    int x = tasks;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-    }
-    if (lane == 31) S.warp_sum[warp] = x;
-    __syncthreads();
-    for (int w = 0; w < warp; ++w) x += S.warp_sum[w];
-    S.before[id + 1] = x;
-    if (id == 0) S.before[0] = 0;
-    __syncthreads();
-    chain_kernels();
-    for (int task = blockIdx.x * CJ_WARPS + warp; task < S.before[256]; task += gridDim.x * CJ_WARPS) {
-        int lo = 0;
-#pragma unroll
-        for (int step = 128; step > 0; step >>= 1)
-            if (S.before[lo + step] <= task) lo += step;
-        const int r = (task - S.before[lo]) * PER + lane / LANES, ch = lane % LANES * 4;
-        if (r >= S.rows[lo]) continue;
-        float o[4], top, sum, topw;
-        cm_join_row<D, WREF>(part, S.cut[lo], r, ch, o, top, sum, topw);
-        finish(S.item[lo], r, ch, o, top, sum, topw);
     }
 }
 

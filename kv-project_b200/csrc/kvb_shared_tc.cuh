@@ -35,6 +35,7 @@ struct SharedTcParams {
     float* level_o;                           // [levels][rows][d], normalised
     float* level_ml;                          // [levels][rows][2]: maximum, sum
     float* part;                              // two a CTA
+    void* cuts;                               // CmCut<SharedItem> a CTA
     int ctas;                                 // that take part
 };
 
@@ -68,6 +69,11 @@ __device__ __forceinline__ void st_convert(const uint4& w, uint4 (&to)[2]) {
     to[0] = uint4{r[0], r[1], r[2], r[3]};
     to[1] = uint4{r[4], r[5], r[6], r[7]};
 }
+
+struct SharedItem {
+    SharedSegment g;
+    int h, row0;
+};
 
 // The work of a call; false when there is none.  Whole block.
 template <int WARPS>
@@ -152,9 +158,13 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
     }
     chain_kernels();
     PdPlan<true, CM_FIXED> W;
-    if (!shared_plan<ST_WARPS>(A, pre, shares, warp_sum, W)) return;
     const int cta = blockIdx.x;
-    if (cta >= W.ctas) return;
+    const bool any = shared_plan<ST_WARPS>(A, pre, shares, warp_sum, W);
+    CmCut<SharedItem>* const cuts = static_cast<CmCut<SharedItem>*>(A.cuts);
+    if (!any || cta >= W.ctas) {
+        if (threadIdx.x == 0) cuts[cta] = CmCut<SharedItem>{};
+        return;
+    }
     const int u0 = W.units_before(W.share(cta)), u1 = W.units_before(W.share(cta + 1));
 
     if (warp == CM_SOFTMAX) {
@@ -248,12 +258,12 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                 const float lamk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, lv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
                 float v[CM_KEYS];
                 cm_ld64(cols, v);
-                bool plain = left >= CM_KEYS && fminf(fminf(lamk[0], lamk[1]), fminf(lamk[2], lamk[3])) > 0.f;
                 if (A.negate) {
 #pragma unroll
                     for (int i = 0; i < CM_KEYS; ++i) v[i] = -v[i];
                 }
-                if (!__all_sync(0xffffffffu, plain)) {           // tokens that the row does not see, or that have no page
+                // tokens that the row does not see, or that have no page
+                if (__any_sync(0xffffffffu, left < CM_KEYS || fminf(fminf(lamk[0], lamk[1]), fminf(lamk[2], lamk[3])) < 0.f)) {
 #pragma unroll
                     for (int i = 0; i < CM_KEYS; ++i) v[i] = i < left && lamk[i / 16] > 0.f ? v[i] : -INFINITY;
                 }
@@ -283,44 +293,47 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                     }
                 }
                 const float ref = m == -INFINITY ? 0.f : m, dr = ref - (mw == -INFINITY ? 0.f : mw);
-                float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
                 uint32_t w[CM_KEYS / 2];
-                const float2 ref2{-ref, -ref};
-                // Rows with NaN or infinities, that have seen nothing, or whose value scales lie very far apart want every weight from
-                // its own exponent (masked tokens, -inf, give 0 on either way); what their neighbours get does not depend on them.
-                plain = fabsf(y) < INFINITY && fmaxf(fmaxf(lv[0], lv[1]), fmaxf(lv[2], lv[3])) + dr < 100.f;
-                auto weights = [&](auto all) {
+                // w = p 2^e, e = lv + dr.  A weight that float32 has to hold as p 2^e with a large e has a p that it cannot: where
+                // e passes 100, p is taken 2^(e - 100) times as large and its sum is scaled back.
+                float up[4] = {0.f, 0.f, 0.f, 0.f}, back[4] = {1.f, 1.f, 1.f, 1.f};
+                if (__any_sync(0xffffffffu, fmaxf(fmaxf(lv[0], lv[1]), fmaxf(lv[2], lv[3])) + dr > 100.f)) {
 #pragma unroll
                     for (int g = 0; g < 4; ++g) {
-                        const float f = ex2(lv[g] + dr);
-                        const float2 lam2{fabsf(lamk[g]), fabsf(lamk[g])}, f2{f, f};
-#pragma unroll
-                        for (int k = 0; k < 8; ++k) {
-                            const int i = 8 * g + k;
-                            const float2 x = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
-                            float2 e = x;
-                            if (i % 4 < CM_FMA) {
-                                e = cm_ex2(x);
-                            } else {
-                                e.x = ex2(x.x);
-                                e.y = ex2(x.y);
-                            }
-                            float2 y = cm_mul2(e, f2);
-                            if (!all && !plain) {
-                                e = float2{ex2(x.x), ex2(x.y)};
-                                y = float2{ex2(x.x + (lv[g] + dr)), ex2(x.y + (lv[g] + dr))};
-                            }
-                            sum[i & 1] = cm_add2(sum[i & 1], e);
-                            w[i] = pack_half2(y.x, y.y);
-                        }
+                        up[g] = fmaxf(lv[g] + dr - 100.f, 0.f);
+                        back[g] = ex2(-up[g]);
                     }
-                };
-                if (__all_sync(0xffffffffu, plain)) weights(std::true_type{});
-                else weights(std::false_type{});
+                }
+                float both = 0.f;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {
+                    const float f = ex2(lv[g] + dr - up[g]);
+                    const float2 lam2{fabsf(lamk[g]), fabsf(lamk[g])}, f2{f, f}, ref2{up[g] - ref, up[g] - ref};
+                    float2 sum[2];
+#pragma unroll
+                    for (int k = 0; k < 8; ++k) {
+                        const int i = 8 * g + k;
+                        float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                        if (i % 4 < CM_FMA) {
+                            e = cm_ex2(e);
+                        } else {
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                        }
+                        sum[k & 1] = k < 2 ? e : cm_add2(sum[k & 1], e);
+                        e = cm_mul2(e, f2);
+                        w[i] = pack_half2(e.x, e.y);
+                    }
+                    sum[0] = cm_add2(sum[0], sum[1]);
+                    both = __fmaf_rn(sum[0].x + sum[0].y, back[g], both);
+                }
+                if (!(y < INFINITY)) {                           // NaN or +inf among the logits: the row is NaN
+                    both = NAN;
+                    w[0] = 0x7fff7fffu;
+                }
                 __syncwarp();
                 cm_st32(cols, w);
-                const float2 both = cm_add2(sum[0], sum[1]);
-                l += both.x + both.y;
+                l += both;
                 cm_wait_st();
                 cm_before();
                 __syncwarp();
@@ -338,7 +351,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
             cm_after();
             const bool whole = done.p.a == 0 && done.p.b == done.p.units, two = split && done.tiles() > 1;
             const int tile0 = split ? 0 : t * CM_ROWS;
-            float* const part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * CM_PART<D> + int64_t(tile0 + r) * D;
+            float* const part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * CM_PART<D>;
             if (split && t == 1) {                               // the second tile passes its part on to the first
                 for (int c = 0; c < D / 32 && two; ++c, ++xn) {
                     if (xn > 0 && !(ok = cm_wait(&B.x_empty[quarter], xn - 1))) break;
@@ -386,7 +399,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                             for (int i = 0; i < 32; ++i) v[i] *= inv;
                             cm_put(A.level_o + row * D + 32 * c, v);
                         } else {
-                            cm_put(part + 32 * c, v);
+                            cm_put(part + (tile0 + r) * D + 32 * c, v);
                         }
                     }
                     __syncwarp();
@@ -395,10 +408,9 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                     if (whole) {
                         *reinterpret_cast<float2*>(A.level_ml + 2 * row) = float2{m, l};
                     } else {
-                        float* st = part - int64_t(tile0 + r) * D + 2 * CM_ROWS * D + tile0 + r;
-                        __stcg(st, m);
-                        __stcg(st + 2 * CM_ROWS, l);
-                        __stcg(st + 4 * CM_ROWS, mw);
+                        __stcg(part + 2 * CM_ROWS * D + tile0 + r, m);
+                        __stcg(part + 2 * CM_ROWS * (D + 1) + tile0 + r, l);
+                        __stcg(part + 2 * CM_ROWS * (D + 2) + tile0 + r, mw);
                     }
                 }
             }
@@ -410,6 +422,16 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
     } else if (warp == CM_SOFTMAX) {
         cm_issue_scores<D, BF16, ST_K>(B, tmem, smem_u32(sq), smem_u32(sk), u0, u1, step_at);
     } else if (warp < CM_SOFTMAX + 3) {
+        // the second of these has the time: the joining kernel is told what this CTA's end cuts
+        if (warp == CM_SOFTMAX + 2 && lane == 0)
+            cm_note_cut(W, cta, cuts, [&](const PdPiece& p, SharedItem& x) {
+                x.g = V.segment(p.seq);
+                const int groups = W.heads(p.seq) / P.Hkv;
+                x.h = p.vh / groups;
+                x.row0 = (p.vh - x.h * groups) * 2 * CM_ROWS;
+                return min(x.g.members * A.rep * A.Tq - x.row0, 2 * CM_ROWS);
+            });
+        __syncwarp();
         cm_issue_values<D, 0, ST_V>(B, tmem, smem_u32(sv), warp - CM_SOFTMAX - 1, u0, u1, step_at);
     } else if (warp == CM_SOFTMAX + 3) {
         // ---------------- copies of codes: lane i looks after the units i mod 32 of the block ----------------
@@ -521,27 +543,11 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
     if (warp == CM_SOFTMAX) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(CM_TMEM));
 }
 
-struct SharedItem {
-    SharedSegment g;
-    int h, row0;
-};
-
 // Joins the items that shared_pages_kernel cut.
 template <int D>
 __global__ void __launch_bounds__(32 * CJ_WARPS, 4) shared_join_kernel(const __grid_constant__ SharedTcParams A) {
-    __shared__ int pre[PS_MAX_SEQS + 1], shares[PS_MAX_SEQS + 1], warp_sum[2][CJ_WARPS];
-    __shared__ CjSmem<SharedItem> S;
-    PdPlan<true, CM_FIXED> W;
-    if (!shared_plan<CJ_WARPS>(A, pre, shares, warp_sum, W)) return;
-    cm_join<D, true>(W, A.part, S,
-                     [&](const PdPiece& p, SharedItem& x) {
-                         x.g = A.shared.segment(p.seq);
-                         const int groups = W.heads(p.seq) / A.P.Hkv;
-                         x.h = p.vh / groups;
-                         x.row0 = (p.vh - x.h * groups) * 2 * CM_ROWS;
-                         return min(x.g.members * A.rep * A.Tq - x.row0, 2 * CM_ROWS);
-                     },
-                     [&](const SharedItem& x, int r, int ch, const float (&o)[4], float top, float sum, float topw) {
+    cm_join<D, true>(static_cast<const CmCut<SharedItem>*>(A.cuts), A.ctas, A.part,
+                     [&](const SharedItem& x, int r, int ch, const float (&o)[CJ_CH], float top, float sum, float topw) {
                          const int64_t row = shared_out(A, x.g, x.h, x.row0 + r);
                          const float inv = shared_inverse(top, topw, sum);
                          *reinterpret_cast<float4*>(A.level_o + row * D + ch) = float4{o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv};
