@@ -111,16 +111,23 @@ __device__ __forceinline__ float shared_inverse(float m, float mw, float sum) {
     return sum > 0.f ? ex2(mw - (m == -INFINITY ? 0.f : m)) / sum : (sum == sum ? 0.f : sum);
 }
 
-// ROUNDS times 16 codes as operands, STEP bytes apart, and to the asynchronous proxy; whole warp.
+// ROUNDS times 16 codes, 2048 bytes apart, as operands STEP bytes apart, and to the asynchronous proxy; whole warp.  In a short loop,
+// the next codes read before these are stored: unrolled, it and the softmax beside it did not fit the instruction cache, and half
+// of the time was waiting for code.
 template <typename T, int ROUNDS, int STEP>
-__device__ __forceinline__ void st_store(const uint4 (&from)[ROUNDS], uint8_t* to, uint32_t first, bool swap) {
-#pragma unroll
+__device__ __forceinline__ void st_store(const uint8_t* from, uint8_t* to, uint32_t first, bool swap) {
+    uint4 next = *reinterpret_cast<const uint4*>(from);
+#pragma unroll 1
     for (int i = 0; i < ROUNDS; ++i) {
+        const uint4 codes = next;
+        from += 2048;
+        if (i + 1 < ROUNDS) next = *reinterpret_cast<const uint4*>(from);
         uint4 x[2];
-        st_convert<T>(from[i], x);
+        st_convert<T>(codes, x);
         // the two halves of the channels in opposite order: their chunks then meet different banks
-        *reinterpret_cast<uint4*>(to + i * STEP + first) = swap ? x[1] : x[0];
-        *reinterpret_cast<uint4*>(to + i * STEP + (first ^ 16)) = swap ? x[0] : x[1];
+        *reinterpret_cast<uint4*>(to + first) = swap ? x[1] : x[0];
+        *reinterpret_cast<uint4*>(to + (first ^ 16)) = swap ? x[0] : x[1];
+        to += STEP;
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -518,21 +525,16 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
         for (int k = 0; k < total && ok; ++k) {
             const uint32_t st = k % ST_CODES, kst = k % ST_K, vst = k % ST_V;
             if (!(ok = cm_wait(&codes_full[st], k / ST_CODES))) break;
-            uint4 keys[ROUNDS], values[ROUNDS];                  // read before anything is written, which might lie in the same place for all the compiler knows
             const uint8_t* from = sc + st * StShape<D>::CODES + 16 * id;
-#pragma unroll
-            for (int i = 0; i < ROUNDS; ++i) {
-                keys[i] = *reinterpret_cast<const uint4*>(from + 2048 * i);
-                values[i] = *reinterpret_cast<const uint4*>(from + CM_KEYS * D + 2048 * i);
-            }
-            __syncwarp();
-            if (lane == 0) mbar_arrive(&codes_empty[st]);
             if (k >= ST_K && !(ok = cm_wait(&B.k_empty[kst], k / ST_K - 1))) break;
-            st_store<T, ROUNDS, ROW_STEP>(keys, sk + kst * S::TILE + at, first, swap);
+            st_store<T, ROUNDS, ROW_STEP>(from, sk + kst * S::TILE + at, first, swap);
             if (lane == 0) mbar_arrive(&B.k_full[kst]);
             if (k >= ST_V && !(ok = cm_wait(&B.v_empty[vst], k / ST_V - 1))) break;
-            st_store<__half, ROUNDS, ROW_STEP>(values, sv + vst * S::TILE + at, first, swap);
-            if (lane == 0) mbar_arrive(&B.v_full[vst]);
+            st_store<__half, ROUNDS, ROW_STEP>(from + CM_KEYS * D, sv + vst * S::TILE + at, first, swap);
+            if (lane == 0) {
+                mbar_arrive(&B.v_full[vst]);
+                mbar_arrive(&codes_empty[st]);
+            }
             __syncwarp();
         }
         __syncwarp();
