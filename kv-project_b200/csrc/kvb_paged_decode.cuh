@@ -57,8 +57,8 @@ constexpr float PD_LAZY = 8.f;
 constexpr int PD_ALL = 0;                     // every sequence's tokens
 constexpr int PD_OWN = 1;                     // the tokens behind a sequence's shared ones; its segments' parts are joined in
 // The same, a warp for itself: it takes a run of its own units, keeps its results in registers to the end and stores them from
-// there.  For many short items, of which the eight warps of a CTA together spend most of the time on joining (512 items of 20 to
-// 700 tokens: 34 us together, 25 alone; 200 of up to 260, 15 and 21; 16 of 60, 10 and 14).
+// there.  For many items, of which the eight warps of a CTA together spend most of the time on joining (512 items of 60 tokens
+// behind 640 shared ones: 43 us together, 32 alone; 64 items of 4000, 40 and 48).
 constexpr int PD_LONE = 2;
 
 struct PagedDecodeParams {
@@ -279,6 +279,7 @@ __global__ void __launch_bounds__(PdShape<D, NT>::THREADS, 1) paged_decode_kerne
     const int64_t work = (int64_t(pre[A.n]) + int64_t(A.n) * FIXED) * W.hg;
     if (work > INT_MAX) {                                        // the host's launches hold less, but for one group of 2^31 units
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
+        if (!waited) chain_kernels();                            // the kernel does not end before those it follows
         return;
     }
     W.ctas = max(1, min(int(gridDim.x) * (LONE ? S::WARPS : 1), int(work) / PD_LEAST));

@@ -281,6 +281,21 @@ def test_a_row_that_is_not_finite_stays_alone(cuda_dev):
         assert torch.equal(got[~hurt], clean[~hurt]) and torch.isnan(got[hurt]).all()
 
 
+@pytest.mark.parametrize("side,value", [("ks", float("nan")), ("vs", float("inf"))])
+def test_a_scale_that_is_not_finite_is_that_of_its_head(cuda_dev, side, value):
+    """No write makes such a scale; where one is, attend_shared is not finite where attend is not, and nowhere else."""
+    rng = np.random.default_rng(18)
+    pool, slots = family(rng, 500, [64, 1], 4, [30] * 8, 2, 128, 64)
+    q = torch.from_numpy(rng.standard_normal((8, 8, 1, 128))).to(torch.bfloat16).cuda()
+    g = on_gpu(pool)
+    clean = g.attend_shared(q, g.share(ints(slots)))
+    pool[side][pool["table"][slots[0], 3], 1] = value
+    g = on_gpu(pool)
+    got = g.attend_shared(q, g.share(ints(slots)))
+    assert torch.isnan(g.attend(q, ints(slots))[:, :, 4:]).all() and torch.isnan(got[:, :, 4:]).all()
+    assert torch.equal(got[:, :, :4], clean[:, :, :4])
+
+
 def test_a_plan_stays_good_while_sequences_grow(cuda_dev):
     rng = np.random.default_rng(11)
     pool, slots = family(rng, 100, [40, 64], 3, [1, 2, 3, 4, 5, 6], 2, 64, 16)
