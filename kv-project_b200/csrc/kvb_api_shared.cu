@@ -9,7 +9,11 @@ namespace {
 // Segments cover a sequence at most this often: each has two or more parts below it.
 int levels_of(int n) { return std::min(kvb::PS_LEVELS, std::max(n - 1, 0)); }
 
-constexpr int64_t kTogether = 220;          // see PD_LONE
+// Items of the sequences' own tokens up to which the eight warps of a CTA work on one together (PD_OWN); above, each on its own
+// (PD_LONE).  attend_shared behind 640 shared tokens with 60, 1200 and 4000 of their own: 32 items 26, 30 and 34 us together,
+// 26, 34 and 50 alone; 128 items 28, 38 and 57, 28, 39 and 58; 192 items 34, 44 and 69, 29, 41 and 68; 512 items 43, 75 and 126,
+// 32, 63 and 121.
+constexpr int64_t kTogether = 160;
 
 int shared_ctas() { return std::min(resolve_ctas(0), kvb::PD_MAX_CTAS); }
 

@@ -11,8 +11,8 @@
 
 Every call enqueues on the current stream of its tensors' device and never synchronises.  Whole numbers (slots, lengths,
 page numbers) are int32 tensors on the device, so a captured graph of a pool's calls serves any lengths (one call of each
-kind on the stream first: workspaces are not made inside a capture); prefill_attention is not captured, it raises
-NotImplementedError.  Ranges that do not fit are left out and raise the device status word (``kvb.device_status``: bit 1 a
+kind on the stream first: workspaces are not made inside a capture; share, attend_shared and cross_attention need none, a
+graph holds workspaces of its own for them); prefill_attention is not captured, it raises NotImplementedError.  Ranges that do not fit are left out and raise the device status word (``kvb.device_status``: bit 1 a
 range, bit 4 a pool without enough free pages); rows that are left out of a result are not written.
 """
 
