@@ -489,7 +489,7 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
  * has the query rows [cu_q[s], cu_q[s + 1]) and sees all of the key rows [cu_k[s], cu_k[s + 1]), which may be none (zeros and -inf).
  * q (nq, Hq, d), k and v (nk, Hkv, d) of one dtype (f16 / bf16) with d in {64, 128} contiguous, 16-byte aligned, the element
  * strides below multiples of 8 (a head stride of 0: one head for all; key rows have to lie apart); cu_q, cu_k (n + 1) int32 on
- * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 16-byte aligned; lse (nq, Hq) float32 (natural log) or
+ * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 32-byte aligned; lse (nq, Hq) float32 (natural log) or
  * null.  Rows of no sequence are not written.  Offsets that do not fit the rows raise status bit 1 and their sequences are left
  * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): its first 8192 bytes zero-filled once before its first use
  * and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently. */
