@@ -228,6 +228,21 @@ def test_long_states(cuda_dev):
         check(q, k, v, cu_of([rows]), cu_of([40000]))
 
 
+@pytest.mark.parametrize("queries,keys", [([1] * 1100, [1] * 1100), ([1100], [1100]), ([3, 1097], [0, 1100])])
+def test_rows_whose_offsets_pass_32_bits(cuda_dev, queries, keys):
+    """Queries, keys and values 2^21 elements apart, 1100 of them: the results of dense ones, bit for bit."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(12)
+    far = torch.empty(1100 << 21, dtype=torch.float16, device="cuda")
+    q, k, v = (far.as_strided((1100, h, 64), (1 << 21, 64, 1), at) for h, at in ((4, 0), (2, 1024), (2, 2048)))
+    for x in (q, k, v):
+        x.copy_(rand(g, *x.shape, dtype=torch.float16))
+    got = kvb.cross_attention(q, k, v, cu_of(queries), cu_of(keys))
+    dense = kvb.cross_attention(q.contiguous(), k.contiguous(), v.contiguous(), cu_of(queries), cu_of(keys))
+    assert torch.equal(got, dense)
+    check(q.contiguous(), k.contiguous(), v.contiguous(), cu_of(queries), cu_of(keys))
+
+
 def test_empty_calls_and_refusals(cuda_dev):
     import kvb
     q, k = torch.randn(5, 4, 64, device="cuda").half(), torch.randn(9, 2, 64, device="cuda").half()

@@ -89,3 +89,37 @@ def test_cross_sizes():
     f = _lib.lib().kvb_cross_workspace
     assert f(32) == f(0) == 0 and 8192 < f(64) < f(128)
     assert call("kvb_cross_attention", *[None] * 3, 2, 0, 0, 4, 2, 128, *[0] * 6, None, None, 0, 0.1, None, None, None, 0, None)[0] == 0
+
+
+def test_calls_run_on_the_device_of_their_tensors(monkeypatch):
+    """With device 0 current, calls on device 1 begin again with that one current, and the first is back afterwards."""
+    import torch
+    from kvb import paged
+    now = [0]
+
+    class device:
+        def __init__(self, index):
+            self.index = index
+
+        def __enter__(self):
+            self.before, now[0] = now[0], self.index
+
+        def __exit__(self, *exc):
+            now[0] = self.before
+
+    class Tensor:
+        def get_device(self):
+            return 1
+
+    monkeypatch.setattr(torch._C, "_cuda_getDevice", lambda: now[0], raising=False)
+    monkeypatch.setattr(torch.cuda, "device", device)
+    names = ("share", "attend_shared")
+    Pool = type("Pool", (paged.PagePool,), {x: (lambda x: lambda self, *args: (x, now[0], args))(x) for x in names})
+    pool = Pool.__new__(Pool)
+    pool._index = 1
+    assert paged.PagePool.share(pool, 5) == ("share", 1, (5,)) and now == [0]
+    assert paged.PagePool.attend_shared(pool, 5, 6, 0.5, 7, True) == ("attend_shared", 1, (5, 6, 0.5, 7, True)) and now == [0]
+    whole = paged.cross_attention
+    monkeypatch.setattr(paged, "cross_attention", lambda *args: (args, now[0]))
+    q = Tensor()
+    assert whole(q, 1, 2, 3, 4, return_lse=True) == ((q, 1, 2, 3, 4, None, None, True), 1) and now == [0]

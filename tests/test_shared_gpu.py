@@ -296,6 +296,27 @@ def test_a_scale_that_is_not_finite_is_that_of_its_head(cuda_dev, side, value):
     assert torch.equal(got[:, :, :4], clean[:, :, :4])
 
 
+@pytest.mark.parametrize("samples", [2, 16])
+def test_pages_whose_offsets_pass_32_bits(cuda_dev, samples):
+    """The last pages of a pool of 4.3 GB a side: the results of a small pool, bit for bit."""
+    import kvb
+    rng = np.random.default_rng(19)
+    pool, slots = family(rng, 700, [64, 1], samples, [30] * (2 * samples), 2, 128, 64)
+    small, pages = on_gpu(pool), len(pool["refs"])
+    before = (1 << 32) // (2 * 64 * 128)
+    far = {x: torch.empty((before + pages, *getattr(small, x).shape[1:]), dtype=getattr(small, x).dtype, device="cuda")
+           for x in ("kc", "vc", "ks", "vs", "refs")}
+    for x, to in far.items():
+        to[before:] = getattr(small, x)
+    table = torch.where(small.table >= 0, small.table + before, small.table)
+    large = kvb.PagePool(far["kc"], far["vc"], far["ks"], far["vs"], table, small.lens.clone(), far["refs"])
+    q = torch.from_numpy(rng.standard_normal((2 * samples, 8, 1, 128))).to(torch.bfloat16).cuda()
+    a, b = small.share(ints(slots)), large.share(ints(slots))
+    assert torch.equal(a.plan, b.plan) and int(a.count) > 0
+    for x, y in zip(small.attend_shared(q, a, return_lse=True), large.attend_shared(q, b, return_lse=True)):
+        assert torch.equal(x, y)
+
+
 def test_a_plan_stays_good_while_sequences_grow(cuda_dev):
     rng = np.random.default_rng(11)
     pool, slots = family(rng, 100, [40, 64], 3, [1, 2, 3, 4, 5, 6], 2, 64, 16)
