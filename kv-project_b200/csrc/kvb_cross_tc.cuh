@@ -12,7 +12,7 @@
 // TFLOP/s, with the power limit active and the SM clock between 1600 and 1710 MHz; of that kernel's time on 2048 queries over
 // 8192 keys the tensor cores are busy 53 %, the special functions 40 %, the issue slots 48 %, and no single one bounds it: a tile's
 // softmax and its products wait for one another where the other tile does not fill in.  Eight packed prompts of 5300 queries
-// over 14860 keys 202 us, 850 TFLOP/s: items start and end (queries, sums, cut items).  37 queries of 6 sequences (67 MB) 28 us,
+// over 14860 keys 197 us, 870 TFLOP/s: items start and end (queries, sums, cut items).  37 queries of 6 sequences (67 MB) 28 us,
 // of which 9 are the joining kernel.
 #pragma once
 #include "kvb_cross.cuh"
@@ -150,6 +150,8 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
         for (int cur = u0; cur < u1 && ok;) {
             const bool split = x.split();
             const int units = cm_units(split, x.tiles, t);
+            // a warp without a row lets its S pass: what its part of O then is, nobody reads
+            const bool live = __any_sync(0xffffffffu, (split ? 0 : t * CM_ROWS) + r < x.nrows);
             float m = -INFINITY, l = 0.f;
             for (int j = 0; j < units; ++j, ++sn) {
                 const uint32_t half = sn & 1, cols = ts + CM_KEYS * half;
@@ -157,61 +159,63 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
                 if (!(ok = cm_wait(&B.s_full[t][half], sn >> 1))) break;
                 cm_after();
                 const int left = x.s.kl - (x.p.a + u) * CM_KEYS; // keys of the sequence from this unit on
-                float v[CM_KEYS];
-                cm_ld64(cols, v);
-                if (A.negate) {
+                if (live) {
+                    float v[CM_KEYS];
+                    cm_ld64(cols, v);
+                    if (A.negate) {
 #pragma unroll
-                    for (int i = 0; i < CM_KEYS; ++i) v[i] = -v[i];
-                }
-                if (left < CM_KEYS) {
-#pragma unroll
-                    for (int i = 0; i < CM_KEYS; ++i) v[i] = i < left ? v[i] : -INFINITY;
-                }
-                float top[4] = {v[0], v[1], v[2], v[3]};
-#pragma unroll
-                for (int i = 4; i < CM_KEYS - 4; i += 8)
-#pragma unroll
-                    for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[i + k], v[i + 4 + k]);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[CM_KEYS - 4 + k], -INFINITY);
-                const float y = cm_max3(cm_max3(top[0], top[1], top[2]), top[3], -INFINITY) * A.lam;
-                const bool grow = y > m + PF_LAZY;
-                if (__any_sync(0xffffffffu, grow)) {
-                    const float f = grow ? ex2(m - y) : 1.f;
-                    if (grow) m = y;
-                    l *= f;
-                    if (j > 0) {                                 // once the product before is done
-                        if (!(ok = cm_wait(&B.pv_done[t][half ^ 1], (sn - 1) >> 1))) break;
-                        cm_after();
-                        cm_rescale<D>(to, f);
+                        for (int i = 0; i < CM_KEYS; ++i) v[i] = -v[i];
                     }
-                }
-                const float ref = m == -INFINITY ? 0.f : m;
-                const float2 lam2{A.lam, A.lam}, ref2{-ref, -ref};
-                float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
-                uint32_t w[CM_KEYS / 2];
-                // of four pairs of keys CM_FMA on the FMA pipe: with all on the special-function unit, which the two
-                // warpgroups share, it is what bounds the step.  -inf gives 0 on either.
+                    if (left < CM_KEYS) {
 #pragma unroll
-                for (int i = 0; i < CM_KEYS / 2; ++i) {
-                    float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
-                    if (i % 4 < CM_FMA) {
-                        e = cm_ex2(e);
-                    } else {
-                        e.x = ex2(e.x);
-                        e.y = ex2(e.y);
+                        for (int i = 0; i < CM_KEYS; ++i) v[i] = i < left ? v[i] : -INFINITY;
                     }
-                    sum[i & 1] = cm_add2(sum[i & 1], e);
-                    w[i] = pack_f32<T>(e.x, e.y);
+                    float top[4] = {v[0], v[1], v[2], v[3]};
+#pragma unroll
+                    for (int i = 4; i < CM_KEYS - 4; i += 8)
+#pragma unroll
+                        for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[i + k], v[i + 4 + k]);
+#pragma unroll
+                    for (int k = 0; k < 4; ++k) top[k] = cm_max3(top[k], v[CM_KEYS - 4 + k], -INFINITY);
+                    const float y = cm_max3(cm_max3(top[0], top[1], top[2]), top[3], -INFINITY) * A.lam;
+                    const bool grow = y > m + PF_LAZY;
+                    if (__any_sync(0xffffffffu, grow)) {
+                        const float f = grow ? ex2(m - y) : 1.f;
+                        if (grow) m = y;
+                        l *= f;
+                        if (j > 0) {                                 // once the product before is done
+                            if (!(ok = cm_wait(&B.pv_done[t][half ^ 1], (sn - 1) >> 1))) break;
+                            cm_after();
+                            cm_rescale<D>(to, f);
+                        }
+                    }
+                    const float ref = m == -INFINITY ? 0.f : m;
+                    const float2 lam2{A.lam, A.lam}, ref2{-ref, -ref};
+                    float2 sum[2] = {{0.f, 0.f}, {0.f, 0.f}};
+                    uint32_t w[CM_KEYS / 2];
+                    // of four pairs of keys CM_FMA on the FMA pipe: with all on the special-function unit, which the two
+                    // warpgroups share, it is what bounds the step.  -inf gives 0 on either.
+#pragma unroll
+                    for (int i = 0; i < CM_KEYS / 2; ++i) {
+                        float2 e = cm_fma2(float2{v[2 * i], v[2 * i + 1]}, lam2, ref2);
+                        if (i % 4 < CM_FMA) {
+                            e = cm_ex2(e);
+                        } else {
+                            e.x = ex2(e.x);
+                            e.y = ex2(e.y);
+                        }
+                        sum[i & 1] = cm_add2(sum[i & 1], e);
+                        w[i] = pack_f32<T>(e.x, e.y);
+                    }
+                    if (!(y < INFINITY)) {                           // NaN or +inf among the logits: the row is NaN
+                        sum[0].x = NAN;
+                        w[0] = 0x7fff7fffu;
+                    }
+                    __syncwarp();
+                    cm_st32(cols, w);
+                    const float2 both = cm_add2(sum[0], sum[1]);
+                    l += both.x + both.y;
                 }
-                if (!(y < INFINITY)) {                           // NaN or +inf among the logits: the row is NaN
-                    sum[0].x = NAN;
-                    w[0] = 0x7fff7fffu;
-                }
-                __syncwarp();
-                cm_st32(cols, w);
-                const float2 both = cm_add2(sum[0], sum[1]);
-                l += both.x + both.y;
                 if (left < CM_KEYS) {                            // value rows past the end, up to the last step's 16
                     const uint32_t st = (it + u) % CM_STAGES;
                     if (!(ok = cm_wait(&B.v_full[st], (it + u) / CM_STAGES))) break;
@@ -238,7 +242,7 @@ __global__ void __launch_bounds__(32 * CM_WARPS, 1) cross_many_kernel(const __gr
             }
             if (units > 0 && !(ok = cm_wait(&B.pv_done[t][(sn - 1) & 1], (sn - 1) >> 1))) break;     // nothing is written
             cm_after();
-            const bool whole = done.p.a == 0 && done.p.b == done.p.units, two = split && done.tiles > 1;
+            const bool whole = done.p.a == 0 && done.p.b == done.p.units, two = live && split && done.tiles > 1;
             const int tile0 = split ? 0 : t * CM_ROWS;
             float* const part = A.part + int64_t(2 * cta + (first ? 0 : 1)) * CM_PART<D>;
             auto out_row = [&](int r) {                          // row r of the item in out and lse
