@@ -15,9 +15,10 @@
 //
 // The conversion is a loop that is not unrolled: with all of it in line, it and the softmax together left the instruction cache
 // at every unit (64 sequences behind 16384 tokens 80 us, 75 with the loop; 32 behind four prompts 61 and 54).  Neither HBM nor the
-// tensor cores bound it (20 % busy in the first case, issue slots 42 %, waits for instructions 1.4 of 9 cycles a warp): a unit is a
-// chain of copy, conversion, S, softmax and P V, of which two or three are under way, and the start (page look-ups, queries,
-// first instructions) is 10 of the about 45 us of this kernel there.
+// tensor cores bound it (20 % busy in the first case, issue slots 42 %, waits for instructions 1.4 of 9 cycles a warp) but the
+// converting warps, of which the registers leave one an SM partition: of a unit's 2750 cycles there (3200 with 256 rows) 1000 are keys, 700
+// values, the rest fences, barriers and the wait for codes; the softmax takes 1400.  The start (page look-ups, queries, first instructions) is
+// 10 of the about 45 us of this kernel in the first case.  Two rounds of the loop at a time: 75.6 us and 56.7.
 #pragma once
 #include "kvb_rows_tc.cuh"
 
@@ -309,19 +310,11 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                 uint32_t w[CM_KEYS / 2];
                 // w = p 2^e, e = lv + dr.  A weight that float32 has to hold as p 2^e with a large e has a p that it cannot: where
                 // e passes 100, p is taken 2^(e - 100) times as large and its sum is scaled back.
-                float up[4] = {0.f, 0.f, 0.f, 0.f}, back[4] = {1.f, 1.f, 1.f, 1.f};
-                if (__any_sync(0xffffffffu, fmaxf(fmaxf(lv[0], lv[1]), fmaxf(lv[2], lv[3])) + dr > 100.f)) {
-#pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        up[g] = fmaxf(lv[g] + dr - 100.f, 0.f);
-                        back[g] = ex2(-up[g]);
-                    }
-                }
                 float both = 0.f;
 #pragma unroll
                 for (int g = 0; g < 4; ++g) {
-                    const float f = ex2(lv[g] + dr - up[g]);
-                    const float2 lam2{fabsf(lamk[g]), fabsf(lamk[g])}, f2{f, f}, ref2{up[g] - ref, up[g] - ref};
+                    const float e2 = lv[g] + dr, up = fmaxf(e2 - 100.f, 0.f), f = ex2(e2 - up);
+                    const float2 lam2{fabsf(lamk[g]), fabsf(lamk[g])}, f2{f, f}, ref2{up - ref, up - ref};
                     float2 sum[2];
 #pragma unroll
                     for (int k = 0; k < 8; ++k) {
@@ -338,7 +331,7 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                         w[i] = pack_half2(e.x, e.y);
                     }
                     sum[0] = cm_add2(sum[0], sum[1]);
-                    both = __fmaf_rn(sum[0].x + sum[0].y, back[g], both);
+                    both = __fmaf_rn(sum[0].x + sum[0].y, ex2(-up), both);
                 }
                 if (!(y < INFINITY)) {                           // NaN or +inf among the logits: the row is NaN
                     both = NAN;
