@@ -492,7 +492,8 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
  * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 32-byte aligned; lse (nq, Hq) float32 (natural log) or
  * null.  Rows of no sequence are not written.  Offsets that do not fit the rows raise status bit 1 and their sequences are left
  * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): its first 8192 bytes zero-filled once before its first use
- * and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently. */
+ * and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently; of host threads that
+ * share one (and its stream) only one at a time may be inside the call, whose launches hand data to one another through it. */
 size_t kvb_cross_workspace(int d);
 kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int dtype, int64_t nq, int64_t nk, int Hq, int Hkv,
                                int d, int64_t q_row, int64_t q_head, int64_t k_row, int64_t k_head, int64_t v_row, int64_t v_head,
@@ -562,7 +563,9 @@ kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32
  * members.  The plan stays good while the sequences only grow (extend, write); after fork, free, compact or copy it has to be
  * made anew (what it says is checked, so that a stale plan reads no wrong address; segments that do not fit raise status bit 1
  * and the results of their members are not defined).  workspace: 256-byte aligned, its first 8192 bytes zero-filled once before
- * its first use and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently. */
+ * its first use and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently; of host
+ * threads that share one (and its stream) only one at a time may be inside the call, whose launches hand data to one another
+ * through it. */
 size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq);
 kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
                                   const int32_t* plan, float scaling, void* out, float* lse, void* workspace,

@@ -13,12 +13,14 @@ Every call enqueues on the current stream of its tensors' device and never synch
 page numbers) are int32 tensors on the device, so a captured graph of a pool's calls serves any lengths (one call of each
 kind on the stream first: workspaces are not made inside a capture; share, attend_shared and cross_attention need none, a
 graph holds workspaces of its own for them); prefill_attention is not captured, it raises NotImplementedError.  Ranges that do not fit are left out and raise the device status word (``kvb.device_status``: bit 1 a
-range, bit 4 a pool without enough free pages); rows that are left out of a result are not written.
+range, bit 4 a pool without enough free pages); rows that are left out of a result are not written.  Several threads may
+call cross_attention and attend_shared on one stream: the launches of a call follow one another.
 """
 
 from __future__ import annotations
 
 import ctypes as C
+import threading
 
 import torch
 
@@ -134,14 +136,15 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: t
 _CROSS_WS = {}
 
 
-def _cross_workspace(lib, device, stream: int, d: int) -> torch.Tensor:
-    """The workspace of one stream (40 MB at d 128), its counters zeroed."""
-    if torch._C._cuda_isCurrentStreamCapturing():
-        return _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device)
-    ws = _CROSS_WS.get((device.index, stream, d))
-    if ws is None:
-        ws = _CROSS_WS[(device.index, stream, d)] = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device)
-    return ws
+def _cross_workspace(lib, device, stream: int, d: int):
+    """The workspace of one stream (40 MB at d 128), its counters zeroed, and the lock of the calls that use it: a call's
+    launches hand partial sums to one another through it, and the library's calls run without the interpreter's lock."""
+    own = None if torch._C._cuda_isCurrentStreamCapturing() else _CROSS_WS.get((device.index, stream, d))
+    if own is None:
+        own = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device), threading.Lock()
+        if not torch._C._cuda_isCurrentStreamCapturing():
+            _CROSS_WS[(device.index, stream, d)] = own
+    return own
 
 
 def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: torch.Tensor, cu_k: torch.Tensor,
@@ -177,11 +180,12 @@ def cross_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_q: tor
         raise ValueError("cross_attention: out must be contiguous (Nq, Hq, d) in q's dtype and on its device")
     lse = _new((nq, hq), (hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
     lib, stream = L.lib(), _raw_stream(index)
-    ws = _cross_workspace(lib, q.device, stream, d)
-    st = lib.kvb_cross_attention(
-        q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
-        vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
-        lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
+    ws, lock = _cross_workspace(lib, q.device, stream, d)
+    with lock:
+        st = lib.kvb_cross_attention(
+            q.data_ptr(), k.data_ptr(), v.data_ptr(), _DT.get(q.dtype, -1), nq, nk, hq, hkv, d, qs[0], qs[1], ks[0], ks[1],
+            vs[0], vs[1], cu_q.data_ptr(), cu_k.data_ptr(), n, d ** -0.5 if scaling is None else scaling, out.data_ptr(),
+            lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
     if st:
         L.check(st, "kvb_cross_attention")
     return (out, lse) if return_lse else out
@@ -250,6 +254,9 @@ class PagePool:
         self._p = C.byref(self._c)
         self._layers, self._n = (L.Pages * 1)(self._c), 1
         self._ws, self._replaced = {}, []
+        # held while a call's launches are enqueued: they hand data to one another through a workspace, which another thread's
+        # launches between them on the same stream would overwrite (the library's calls run without the interpreter's lock)
+        self._lock = threading.Lock()
         self._attend_ws = {}                                            # stream: address and bytes
         self._attend_bytes = L.lib().kvb_page_attend_workspace(self._p, 1, hkv, 1)      # the same for any call
 
@@ -271,6 +278,7 @@ class PagePool:
         other = PagePool(kc, vc, ks, vs, self.table, self.lens, self.refs)
         if (other.n_pages, other.page) != (self.n_pages, self.page):
             raise ValueError("add_layer: as many pages of as many tokens as the first pool has")
+        other._lock = self._lock
         other._ws, other._replaced = self._ws, self._replaced           # one workspace a stream for all layers: their calls take turns
         self._layers = (L.Pages * (self._n + 1))(*self._layers, other._c)
         self._n += 1
@@ -405,13 +413,14 @@ class PagePool:
         lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
         lib, stream = L.lib(), _raw_stream(self._index)
         size = lib.kvb_page_attend_shared_workspace(self._p, n, hq, tq)
-        if torch._C._cuda_isCurrentStreamCapturing():
-            ws = _fresh_workspace(max(size, _COUNTS), _COUNTS, self.device)
-        else:
-            ws = self._workspace("attend_shared", stream, size)
-        st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, shared.slots.data_ptr(), n,
-                                        shared.plan.data_ptr(), d ** -0.5 if scaling is None else scaling, out.data_ptr(),
-                                        lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
+        with self._lock:
+            if torch._C._cuda_isCurrentStreamCapturing():
+                ws = _fresh_workspace(max(size, _COUNTS), _COUNTS, self.device)
+            else:
+                ws = self._workspace("attend_shared", stream, size)
+            st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, shared.slots.data_ptr(), n,
+                                            shared.plan.data_ptr(), d ** -0.5 if scaling is None else scaling, out.data_ptr(),
+                                            lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_attend_shared")
         return (out, lse) if return_lse else out
