@@ -14,7 +14,7 @@ page numbers) are int32 tensors on the device, so a captured graph of a pool's c
 kind on the stream first: workspaces are not made inside a capture; share, attend_shared and cross_attention need none, a
 graph holds workspaces of its own for them); prefill_attention is not captured, it raises NotImplementedError.  Ranges that do not fit are left out and raise the device status word (``kvb.device_status``: bit 1 a
 range, bit 4 a pool without enough free pages); rows that are left out of a result are not written.  Several threads may
-call cross_attention and attend_shared on one stream: the launches of a call follow one another.
+use one stream: the launches of a call follow one another.
 """
 
 from __future__ import annotations
@@ -255,7 +255,9 @@ class PagePool:
         self._layers, self._n = (L.Pages * 1)(self._c), 1
         self._ws, self._replaced = {}, []
         # held while a call's launches are enqueued: they hand data to one another through a workspace, which another thread's
-        # launches between them on the same stream would overwrite (the library's calls run without the interpreter's lock)
+        # launches between them on the same stream would overwrite (the library's calls run without the interpreter's lock); and
+        # what plans with the table, then moves pages and writes it (fork, compact) must not be met halfway by what changes
+        # table or pages
         self._lock = threading.Lock()
         self._attend_ws = {}                                            # stream: address and bytes
         self._attend_bytes = L.lib().kvb_page_attend_workspace(self._p, 1, hkv, 1)      # the same for any call
@@ -297,8 +299,9 @@ class PagePool:
         return ws
 
     def _attend_workspace(self, stream: int):
-        ws = self._workspace("attend", stream, self._attend_bytes)
-        self._attend_ws[stream] = at = (ws.data_ptr(), ws.numel())
+        with self._lock:                                                # the address kept is that of the buffer kept
+            ws = self._workspace("attend", stream, self._attend_bytes)
+            self._attend_ws[stream] = at = (ws.data_ptr(), ws.numel())
         return at
 
     def extend(self, slots: torch.Tensor, add: torch.Tensor) -> torch.Tensor:
@@ -310,7 +313,8 @@ class PagePool:
         n = slots.shape[0]
         _check_ints("extend", n, self._index, slots, add)
         start = torch.empty_like(slots)
-        st = L.lib().kvb_page_extend(self._p, slots.data_ptr(), add.data_ptr(), n, start.data_ptr(), _raw_stream(self._index))
+        with self._lock:
+            st = L.lib().kvb_page_extend(self._p, slots.data_ptr(), add.data_ptr(), n, start.data_ptr(), _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_extend")
         return start
@@ -330,8 +334,9 @@ class PagePool:
         a, b = k.stride(), v.stride()
         if a[2] != 1 or b[2] != 1:
             raise ValueError("write: d must be contiguous")
-        st = L.lib().kvb_page_write(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
-                                    _DT.get(k.dtype, -1), k.shape[0], a[0], a[1], b[0], b[1], _raw_stream(self._index))
+        with self._lock:
+            st = L.lib().kvb_page_write(self._p, slots.data_ptr(), start.data_ptr(), cu.data_ptr(), n, k.data_ptr(), v.data_ptr(),
+                                        _DT.get(k.dtype, -1), k.shape[0], a[0], a[1], b[0], b[1], _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_write")
 
@@ -434,8 +439,9 @@ class PagePool:
         n = src.shape[0]
         _check_ints("fork", n, self._index, src, dst)
         lib, stream = L.lib(), _raw_stream(self._index)
-        ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
-        st = lib.kvb_page_fork(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
+        with self._lock:
+            ws = self._workspace("fork", stream, lib.kvb_page_fork_workspace(self._p, n))
+            st = lib.kvb_page_fork(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_fork")
 
@@ -446,7 +452,8 @@ class PagePool:
                 return self.free(slots)
         n = slots.shape[0]
         _check_ints("free", n, self._index, slots)
-        st = L.lib().kvb_page_free(self._p, slots.data_ptr(), n, _raw_stream(self._index))
+        with self._lock:
+            st = L.lib().kvb_page_free(self._p, slots.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_free")
 
@@ -456,9 +463,10 @@ class PagePool:
             with torch.cuda.device(self._index):
                 return self.compact()
         lib, stream = L.lib(), _raw_stream(self._index)
-        ws = self._workspace("compact", stream, lib.kvb_page_compact_workspace(self._p))
         live = torch.empty((), dtype=_I32, device=self.device)
-        st = lib.kvb_page_compact(self._layers, self._n, live.data_ptr(), ws.data_ptr(), ws.numel(), stream)
+        with self._lock:
+            ws = self._workspace("compact", stream, lib.kvb_page_compact_workspace(self._p))
+            st = lib.kvb_page_compact(self._layers, self._n, live.data_ptr(), ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_compact")
         return live
@@ -470,6 +478,7 @@ class PagePool:
                 return self.copy_pages(src, dst)
         n = src.shape[0]
         _check_ints("copy_pages", n, self._index, src, dst)
-        st = L.lib().kvb_page_copy(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
+        with self._lock:
+            st = L.lib().kvb_page_copy(self._layers, self._n, src.data_ptr(), dst.data_ptr(), n, _raw_stream(self._index))
         if st:
             L.check(st, "kvb_page_copy")

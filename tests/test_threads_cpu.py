@@ -19,7 +19,7 @@ class Tensor:
         return len(self.shape)
 
     def stride(self):
-        return tuple(torch.empty(self.shape, device="meta").stride())
+        return tuple(self.shape[i + 1:].numel() for i in range(len(self.shape)))
 
     def get_device(self):
         return 0
@@ -35,10 +35,10 @@ class Tensor:
 
 
 class Library:
-    """Records which thread took which step of a call on which workspace (the argument before the last two)."""
+    """Records which thread took which step of a call on which workspace (the argument before the last two), or all on one."""
 
     def __init__(self):
-        self.steps = []
+        self.steps, self.one = [], False
 
     def __getattr__(self, name):
         if name.endswith("_workspace"):
@@ -46,7 +46,7 @@ class Library:
 
         def call(*args):
             for step in ("begins", "ends"):
-                self.steps.append((args[-3], step, threading.get_ident()))
+                self.steps.append((0 if self.one else args[-3], step, threading.get_ident()))
                 time.sleep(0.002)
             return 0
         return call
@@ -61,6 +61,8 @@ def paged(monkeypatch):
     monkeypatch.setattr(paged, "_raw_stream", lambda index: 0)
     monkeypatch.setattr(paged, "_new", lambda shape, strides, dtype, device: Tensor(*shape, dtype=dtype))
     monkeypatch.setattr(paged, "_fresh_workspace", lambda size, zeroed, device: Tensor(size, at=next(made)))
+    monkeypatch.setattr(torch, "empty_like", lambda x: Tensor(*x.shape, dtype=x.dtype))
+    monkeypatch.setattr(torch, "empty", lambda shape, dtype, device: Tensor(*shape, dtype=dtype))
     monkeypatch.setattr(torch, "zeros", lambda size, **kw: Tensor(size, at=next(made)))
     monkeypatch.setattr(paged, "_not_capturing", lambda who: None)
     monkeypatch.setattr(paged, "_CROSS_WS", {})
@@ -73,6 +75,7 @@ def pool_of(paged):
     pool = paged.PagePool.__new__(paged.PagePool)
     pool._index, pool.device, pool.d, pool.table, pool._p = 0, Tensor.device, 64, Tensor(8, 8, dtype=torch.int32), C.c_void_p()
     pool._ws, pool._replaced, pool._lock = {}, [], threading.Lock()
+    pool.Hkv, pool._layers, pool._n = 2, None, 1
     return pool
 
 
@@ -120,6 +123,17 @@ def test_attend_shared(paged):
     q = Tensor(3, 4, 1, 64)
     together(library, *[lambda p=p: p.attend_shared(q, shared) for p in (one, two, one, two)])
     assert len({x[0] for x in library.steps}) == 1
+
+
+def test_calls_that_change_table_or_pages(paged):
+    """fork and compact plan with the table before they write it: nothing that changes it or the pages comes in between."""
+    paged, library = paged
+    library.one = True
+    pool, ints = pool_of(paged), lambda n: Tensor(n, dtype=torch.int32)
+    shared, q, k = paged.SharedPages(ints(3), ints(25), pool.table), Tensor(3, 4, 1, 64), Tensor(9, 2, 64)
+    together(library, lambda: pool.fork(ints(3), ints(3)), pool.compact, lambda: pool.extend(ints(3), ints(3)), lambda: pool.free(ints(3)),
+             lambda: pool.write(ints(3), ints(3), ints(4), k, k), lambda: pool.copy_pages(ints(3), ints(3)),
+             lambda: pool.attend_shared(q, shared))
 
 
 def test_layers_share_the_lock(paged, monkeypatch):
