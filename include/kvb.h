@@ -558,14 +558,16 @@ kvb_status kvb_page_attend(const kvb_pages* p, const void* q, int dtype, int Hq,
  * members, first token, end, level, zeros behind the last; plan[8 n]: their number.  Table entries that are no page are
  * nobody's; a slot out of range raises status bit 1 and shares nothing. */
 kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, void* stream);
+/* The same, with a copy of the slots in kept (n): the list may then be filled anew before the plan is used. */
+kvb_status kvb_page_share_kept(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, int32_t* kept, void* stream);
 
 /* kvb_page_attend for the slots of a plan: the same results up to rounding, each segment's codes read once for all its
- * members.  The plan stays good while the sequences only grow (extend, write); after fork, free, compact or copy it has to be
- * made anew (what it says is checked, so that a stale plan reads no wrong address; segments that do not fit raise status bit 1
- * and the results of their members are not defined).  workspace: 256-byte aligned, its first 8192 bytes zero-filled once before
- * its first use and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently; of host
- * threads that share one (and its stream) only one at a time may be inside the call, whose launches hand data to one another
- * through it. */
+ * members.  slots: those the plan was made of, as they were then (kvb_page_share_kept keeps them).  The plan stays good while the
+ * sequences only grow (extend, write); after fork, free, compact or copy, or for other slots, it has to be made anew (what it
+ * says is checked, so that a stale plan reads no wrong address; segments that do not fit raise status bit 1 and the results of
+ * their members are not defined).  workspace: 256-byte aligned, its first 8192 bytes zero-filled once before its first use and
+ * then reused (every call leaves its counters at zero), one per stream that runs calls concurrently; of host threads that share
+ * one (and its stream) only one at a time may be inside the call, whose launches hand data to one another through it. */
 size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq);
 kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, int Hq, int Tq, const int32_t* slots, int n,
                                   const int32_t* plan, float scaling, void* out, float* lse, void* workspace,

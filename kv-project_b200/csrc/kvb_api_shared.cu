@@ -36,11 +36,7 @@ kvb_status launch_segments(const kvb::SharedTcParams& a, cudaStream_t s) {
     return launch_chained("page_attend_shared join", kvb::shared_join_kernel<D>, unsigned(4 * a.ctas), 32 * kvb::CJ_WARPS, 0, s, a);
 }
 
-}  // namespace
-
-extern "C" {
-
-kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, void* stream) {
+kvb_status launch_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, int32_t* kept, void* stream) {
     if (kvb_status st = kvbh::check_pages("page_share", p)) return st;
     if (!plan || (n > 0 && !slots)) return fail(KVB_EINVAL, "page_share: null argument");
     if (n < 0 || n > kvb::PS_MAX_SEQS) return fail(KVB_EINVAL, "page_share: 0 <= n <= %d sequences a call", kvb::PS_MAX_SEQS);
@@ -48,7 +44,20 @@ kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32
     if (kvb_status st = kvbh::allow_smem("page_share", reinterpret_cast<const void*>(kvb::page_share_kernel), int(sizeof(kvb::ShareSmem)), done))
         return st;
     return launch_chained("page_share", kvb::page_share_kernel, 1, kvb::PS_THREADS, sizeof(kvb::ShareSmem), static_cast<cudaStream_t>(stream),
-                          kvbh::view_of(p), slots, n, plan);
+                          kvbh::view_of(p), slots, n, plan, kept);
+}
+
+}  // namespace
+
+extern "C" {
+
+kvb_status kvb_page_share(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, void* stream) {
+    return launch_share(p, slots, n, plan, nullptr, stream);
+}
+
+kvb_status kvb_page_share_kept(const kvb_pages* p, const int32_t* slots, int n, int32_t* plan, int32_t* kept, void* stream) {
+    if (n > 0 && !kept) return fail(KVB_EINVAL, "page_share: null argument");
+    return launch_share(p, slots, n, plan, kept, stream);
 }
 
 size_t kvb_page_attend_shared_workspace(const kvb_pages* p, int n, int Hq, int Tq) {

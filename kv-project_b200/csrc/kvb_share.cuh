@@ -34,7 +34,7 @@ struct ShareSmem {
 };
 
 __global__ void __launch_bounds__(PS_THREADS, 1) page_share_kernel(const __grid_constant__ PagesView P, const int32_t* slots, int n,
-                                                                   int32_t* plan) {
+                                                                   int32_t* plan, int32_t* kept) {
     extern __shared__ __align__(16) uint8_t ps_raw[];
     ShareSmem& S = *reinterpret_cast<ShareSmem*>(ps_raw);
     constexpr unsigned long long EMPTY = ~0ull;
@@ -45,6 +45,7 @@ __global__ void __launch_bounds__(PS_THREADS, 1) page_share_kernel(const __grid_
     unsigned long long path = 0;
     if (i < n) {
         slot = slots[i];
+        if (kept) kept[i] = slot;
         if (unsigned(slot) < unsigned(P.n_slots)) full = min(max(P.lens[slot], 0) >> page_shift(P.page), P.max_blocks);
         else raise_status(KVB_DEV_BOUNDS);
     }

@@ -116,6 +116,7 @@ SIGNATURES = {
     "kvb_page_attend_workspace": (C.c_size_t, [_p, _i32, _i32, _i32]),
     "kvb_page_attend": (_i32, [_p, _p, _i32, _i32, _i32, _p, _i32, _f32, _p, _p, _p, C.c_size_t, _p]),
     "kvb_page_share": (_i32, [_p, _p, _i32, _p, _p]),
+    "kvb_page_share_kept": (_i32, [_p, _p, _i32, _p, _p, _p]),
     "kvb_page_attend_shared_workspace": (C.c_size_t, [_p, _i32, _i32, _i32]),
     "kvb_page_attend_shared": (_i32, [_p, _p, _i32, _i32, _i32, _p, _i32, _p, _f32, _p, _p, _p, C.c_size_t, _p]),
     "kvb_page_fork_workspace": (C.c_size_t, [_p, _i32]),

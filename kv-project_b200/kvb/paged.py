@@ -195,12 +195,41 @@ class SharedPages:
     """What PagePool.share found for n sequences, int32 tensors on the device (views of one): order (n), the sequences'
     places in the list, those of a segment together; own (n), the first token of each that no segment covers; depth (n), how
     many segments cover it; segments (n, 5): first place in order, members, first token, end, level; count (1) of them.
-    It stays good while the sequences only grow; fork, free, compact and copy_pages make it stale."""
+    slots (n) are the sequences as they were listed then: a copy, so that the list may be filled anew.  It stays good while the
+    sequences only grow; fork, free, compact and copy_pages make it stale."""
 
-    __slots__ = ("slots", "plan", "n", "table", "_views")
+    __slots__ = ("n", "table", "_whole", "_slots", "_plan", "_views")
 
     def __init__(self, slots, plan, table):
-        self.slots, self.plan, self.n, self.table, self._views = slots, plan, slots.shape[0], table, None
+        self._whole, self._slots, self._plan, self.n, self.table, self._views = None, slots, plan, slots.shape[0], table, None
+
+    @classmethod
+    def _of(cls, whole, n, table):
+        """Of one tensor, the plan and the slots behind it; views of it are made when they are asked for."""
+        self = cls.__new__(cls)
+        self._whole, self._slots, self._plan, self.n, self.table, self._views = whole, None, None, n, table, None
+        return self
+
+    @property
+    def plan(self):
+        if self._plan is None:
+            self._plan, self._slots = self._whole.split_with_sizes((8 * self.n + 1, self.n))
+        return self._plan
+
+    @property
+    def slots(self):
+        if self._slots is None:
+            self._plan, self._slots = self._whole.split_with_sizes((8 * self.n + 1, self.n))
+        return self._slots
+
+    def _addresses(self, index: int):
+        """Of plan and slots, on CUDA device `index`."""
+        if self._whole is None:
+            _check_on("attend_shared", index, self._plan, self._slots)
+            return self._plan.data_ptr(), self._slots.data_ptr()
+        _check_on("attend_shared", index, self._whole)
+        at = self._whole.data_ptr()
+        return at, at + 4 * (8 * self.n + 1)
 
     def _part(self, i):
         if self._views is None:                                                 # in one call: 3 us where five take 6
@@ -391,11 +420,12 @@ class PagePool:
                 return self.share(slots)
         n = slots.shape[0]
         _check_ints("share", n, self._index, slots)
-        plan = _new((8 * n + 1,), (1,), dtype=_I32, device=self.device)
-        st = L.lib().kvb_page_share(self._p, slots.data_ptr(), n, plan.data_ptr(), _raw_stream(self._index))
+        whole = _new((9 * n + 1,), (1,), dtype=_I32, device=self.device)
+        at = whole.data_ptr()
+        st = L.lib().kvb_page_share_kept(self._p, slots.data_ptr(), n, at, at + 4 * (8 * n + 1), _raw_stream(self._index))
         if st:
-            L.check(st, "kvb_page_share")
-        return SharedPages(slots, plan, self.table)
+            L.check(st, "kvb_page_share_kept")
+        return SharedPages._of(whole, n, self.table)
 
     def attend_shared(self, q, shared: SharedPages, scaling: float = None, out=None, return_lse: bool = False):
         """attend for the sequences of `shared`: the same results up to rounding, the pages that several of them hold read
@@ -407,7 +437,8 @@ class PagePool:
             raise ValueError("attend_shared: q (n, Hq, Tq, d) on the pool's device, n the sequences of `shared`")
         if shared.table.data_ptr() != self.table.data_ptr() or shared.table.shape != self.table.shape:
             raise ValueError("attend_shared: `shared` is of another table")
-        _check_on("attend_shared", self._index, q, shared.plan, shared.slots)
+        _check_on("attend_shared", self._index, q)
+        plan, slots = shared._addresses(self._index)
         n, hq, tq, d = q.shape
         if not q.is_contiguous():
             q = q.contiguous()
@@ -423,8 +454,8 @@ class PagePool:
                 ws = _fresh_workspace(max(size, _COUNTS), _COUNTS, self.device)
             else:
                 ws = self._workspace("attend_shared", stream, size)
-            st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, shared.slots.data_ptr(), n,
-                                            shared.plan.data_ptr(), d ** -0.5 if scaling is None else scaling, out.data_ptr(),
+            st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, slots, n, plan,
+                                            d ** -0.5 if scaling is None else scaling, out.data_ptr(),
                                             lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_attend_shared")
