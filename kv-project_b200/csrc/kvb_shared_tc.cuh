@@ -269,17 +269,21 @@ __global__ void __launch_bounds__(32 * ST_WARPS, 1) shared_pages_kernel(const __
                 cm_after();
                 const int left = limit - (x.p.a + u) * CM_KEYS;  // tokens from this unit on that the row sees
                 const float4 sk4 = scales[2 * ((it + u) % ST_SCALES)], sv4 = scales[2 * ((it + u) % ST_SCALES) + 1];
-                const float lamk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, lv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
+                float lamk[4] = {sk4.x, sk4.y, sk4.z, sk4.w}, lv[4] = {sv4.x, sv4.y, sv4.z, sv4.w};
                 float v[CM_KEYS];
                 cm_ld64(cols, v);
                 if (A.negate) {
 #pragma unroll
                     for (int i = 0; i < CM_KEYS; ++i) v[i] = -v[i];
                 }
-                // tokens that the row does not see, or that have no page
+                // tokens that the row does not see, or that have no page.  What it sees nothing of (16 tokens are of one page) gives it
+                // nothing whatever its scales are: -inf times NaN and -inf + inf would be NaN.
                 if (__any_sync(0xffffffffu, left < CM_KEYS || fminf(fminf(lamk[0], lamk[1]), fminf(lamk[2], lamk[3])) < 0.f)) {
 #pragma unroll
                     for (int i = 0; i < CM_KEYS; ++i) v[i] = i < left && lamk[i / 16] > 0.f ? v[i] : -INFINITY;
+#pragma unroll
+                    for (int g = 0; g < 4; ++g)
+                        if (16 * g >= left) lamk[g] = 1.f, lv[g] = -INFINITY;
                 }
                 float y = -INFINITY, yw = -INFINITY;
 #pragma unroll
