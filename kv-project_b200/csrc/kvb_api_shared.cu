@@ -74,9 +74,12 @@ kvb_status kvb_page_attend_shared(const kvb_pages* p, const void* q, int dtype, 
     kvb::PagedDecodeParams a{};
     if (kvb_status st = kvbh::paged_params("page_attend_shared", p, q, dtype, Hq, Tq, slots, n, scaling, out, lse, workspace, a)) return st;
     if (n == 0) return KVB_OK;
-    // units x row groups of all segments fit 32 bits: on a level they are those of disjoint sequences
-    const int64_t units = int64_t(p->max_blocks) * p->page / kvb::PD_UNIT + kvb::PS_LEVELS * (1 + kvb::PD_FIXED), groups = int64_t(n) * a.rep * Tq / 8 + n;
-    if (units > INT32_MAX / p->Hkv / groups)
+    // The segments' places fit 32 bits (launches of own tokens are divided until theirs do).  One of m >= 2 members has at most
+    // m (rep Tq / 256 + 1 / 2) groups of rows, so that each member counts with its segments' places, at most those of a table row cut
+    // in PS_LEVELS, times rep Tq / 256 + 1 / 2.
+    const int64_t rows_of_kv = int64_t(n) * a.rep * Tq, groups = (rows_of_kv + int64_t(n) * kvb::CM_ROWS + 2 * kvb::CM_ROWS - 1) / (2 * kvb::CM_ROWS);
+    const int64_t places = int64_t(p->max_blocks) * p->page / kvb::CM_KEYS + kvb::PS_LEVELS * (1 + kvb::CM_FIXED);
+    if (rows_of_kv > INT32_MAX - 65536 || places > INT32_MAX / p->Hkv / groups)
         return fail(KVB_EUNSUPPORTED, "page_attend_shared: tokens of a table row times query rows too many for one call");
     if (workspace_bytes < kvb_page_attend_shared_workspace(p, n, Hq, Tq) || !aligned(workspace, 256))
         return fail(KVB_EINVAL, "page_attend_shared: workspace of %zu bytes, 256-byte aligned", kvb_page_attend_shared_workspace(p, n, Hq, Tq));

@@ -14,3 +14,13 @@ def test_share_kept(change, word):
     a.update(change)
     st, msg = call("kvb_page_share_kept", C.byref(pages()), *a.values())
     assert st == 1 and word in msg and "page_share" in msg, (st, msg)
+
+
+@pytest.mark.parametrize("pool,n,Hq,Tq,fits", [
+    (dict(max_blocks=65536, Hkv=8), 512, 64, 4, True), (dict(max_blocks=1 << 20, Hkv=1, page=16), 1024, 128, 1, True),
+    (dict(max_blocks=1 << 24, Hkv=1), 100, 1, 1, True), (dict(max_blocks=1 << 24, Hkv=8), 100, 8, 1, False),
+    (dict(max_blocks=8), 1000, 2 * 32767, 1000, False), (dict(max_blocks=65536, Hkv=8), 1024, 64, 64, True)])
+def test_width_of_a_table(pool, n, Hq, Tq, fits):
+    """What is refused goes by the segments' own work, 64 tokens by 256 rows: the next check is that of the workspace."""
+    st, msg = call("kvb_page_attend_shared", C.byref(pages(**pool)), A, 1, Hq, Tq, A, n, A, 0.1, A, None, A, 64, None)
+    assert (st, "workspace" in msg) == (1, True) if fits else (st, "too many" in msg) == (4, True), (st, msg)

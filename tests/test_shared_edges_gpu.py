@@ -106,3 +106,16 @@ def test_four_levels(cuda_dev, d, page, tq, many):
     s = g.share(ints(order))
     assert s.depth.tolist() == [4] * n and s.count.tolist() == [15 * many]
     check(g, pool, torch.from_numpy(rng.standard_normal((n, 4, tq, d))).to(torch.bfloat16).cuda(), order, shared=s)
+
+
+def test_a_wide_table_of_short_sequences(cuda_dev):
+    """Rows for 65536 pages: the results of a narrow table, bit for bit."""
+    rng = np.random.default_rng(5)
+    pool, slots = family(rng, 64, [70] * 75, 8, [20] * 600, 2, 64, 64)
+    g = on_gpu(pool)
+    q = torch.from_numpy(rng.standard_normal((600, 16, 16, 64), np.float32)).to(torch.float16).cuda()
+    want = g.attend_shared(q, g.share(ints(slots)))
+    pool["table"] = np.pad(pool["table"], ((0, 0), (0, 65536 - pool["table"].shape[1])), constant_values=-1)
+    g = on_gpu(pool)
+    assert torch.equal(g.attend_shared(q, g.share(ints(slots))), want)
+    check(g, pool, q[:4, :, :2].contiguous(), slots[:4])
