@@ -257,46 +257,6 @@ class SharedPages:
         return self._part(4)
 
 
-def _capture_workspace(size: int, zeroed: int, device) -> torch.Tensor:
-    """A workspace inside a stream capture, from the graph's own memory: two graphs never share one, and its counters are
-    zeroed by each replay."""
-    ws = torch.empty(size, dtype=torch.uint8, device=device)
-    ws[:zeroed].zero_()
-    return ws
-
-
-class SharedPages:
-    """What PagePool.share found for n sequences, int32 tensors on the device (views of one): order (n), the sequences'
-    places in the list, those of a segment together; own (n), the first token of each that no segment covers; depth (n), how
-    many segments cover it; segments (n, 5): first place in order, members, first token, end, level; count (1) of them.
-    It stays good while the sequences only grow; fork, free, compact and copy_pages make it stale."""
-
-    __slots__ = ("slots", "plan", "n", "table")
-
-    def __init__(self, slots, plan, table):
-        self.slots, self.plan, self.n, self.table = slots, plan, slots.shape[0], table
-
-    @property
-    def order(self):
-        return self.plan[:self.n]
-
-    @property
-    def own(self):
-        return self.plan[self.n:2 * self.n]
-
-    @property
-    def depth(self):
-        return self.plan[2 * self.n:3 * self.n]
-
-    @property
-    def segments(self):
-        return self.plan[3 * self.n:8 * self.n].view(self.n, 5)
-
-    @property
-    def count(self):
-        return self.plan[8 * self.n:]
-
-
 class PagePool:
     """Pages of ``page`` tokens for Hkv KV heads: codes kc, vc (n_pages, Hkv, page, d) uint8 and scales ks, vs (n_pages,
     Hkv) float32 (a stored value is (code - 128) * scale), table (n_slots, max_blocks) int32 with each sequence's pages,
@@ -497,52 +457,6 @@ class PagePool:
             st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, slots, n, plan,
                                             d ** -0.5 if scaling is None else scaling, out.data_ptr(),
                                             lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
-        if st:
-            L.check(st, "kvb_page_attend_shared")
-        return (out, lse) if return_lse else out
-
-    def share(self, slots) -> SharedPages:
-        """Which leading full pages the sequences hold in common (at most 1024; forked ones share their parents'), in up to
-        four levels: once a step, for the attend_shared of all layers."""
-        if _elsewhere(self._index):
-            with torch.cuda.device(self._index):
-                return self.share(slots)
-        n = slots.shape[0]
-        _check_ints("share", n, self._index, slots)
-        plan = _new((8 * n + 1,), (1,), dtype=_I32, device=self.device)
-        st = L.lib().kvb_page_share(self._p, slots.data_ptr(), n, plan.data_ptr(), _raw_stream(self._index))
-        if st:
-            L.check(st, "kvb_page_share")
-        return SharedPages(slots, plan, self.table)
-
-    def attend_shared(self, q, shared: SharedPages, scaling: float = None, out=None, return_lse: bool = False):
-        """attend for the sequences of `shared`: the same results up to rounding, the pages that several of them hold read
-        and multiplied once for all.  q (n, Hq, Tq, d) -> (n, Tq, Hq, d), with return_lse also (n, Tq, Hq) float32."""
-        if _elsewhere(self._index):
-            with torch.cuda.device(self._index):
-                return self.attend_shared(q, shared, scaling, out, return_lse)
-        if q.dim() != 4 or q.shape[3] != self.d or q.shape[0] != shared.n:
-            raise ValueError("attend_shared: q (n, Hq, Tq, d) on the pool's device, n the sequences of `shared`")
-        if shared.table.data_ptr() != self.table.data_ptr() or shared.table.shape != self.table.shape:
-            raise ValueError("attend_shared: `shared` is of another table")
-        _check_on("attend_shared", self._index, q, shared.plan, shared.slots)
-        n, hq, tq, d = q.shape
-        if not q.is_contiguous():
-            q = q.contiguous()
-        if out is None:
-            out = _new((n, tq, hq, d), (tq * hq * d, hq * d, d, 1), dtype=q.dtype, device=q.device)
-        elif out.shape != (n, tq, hq, d) or out.dtype != q.dtype or out.get_device() != self._index or not out.is_contiguous():
-            raise ValueError("attend_shared: out must be contiguous (n, Tq, Hq, d) in q's dtype on the pool's device")
-        lse = _new((n, tq, hq), (tq * hq, hq, 1), dtype=torch.float32, device=q.device) if return_lse else None
-        lib, stream = L.lib(), _raw_stream(self._index)
-        size = lib.kvb_page_attend_shared_workspace(self._p, n, hq, tq)
-        if torch._C._cuda_isCurrentStreamCapturing():
-            ws = _capture_workspace(max(size, 256), self._attend_bytes, self.device)
-        else:
-            ws = self._workspace("attend_shared", stream, size)
-        st = lib.kvb_page_attend_shared(self._p, q.data_ptr(), _DT.get(q.dtype, -1), hq, tq, shared.slots.data_ptr(), n,
-                                        shared.plan.data_ptr(), d ** -0.5 if scaling is None else scaling, out.data_ptr(),
-                                        lse.data_ptr() if return_lse else None, ws.data_ptr(), ws.numel(), stream)
         if st:
             L.check(st, "kvb_page_attend_shared")
         return (out, lse) if return_lse else out
