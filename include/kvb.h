@@ -491,7 +491,9 @@ kvb_status kvb_prefill_attention(const void* q, const void* k, const void* v, in
  * strides below multiples of 8 (a head stride of 0: one head for all; key rows have to lie apart); cu_q, cu_k (n + 1) int32 on
  * the device, ascending from 0.  out (nq, Hq, d) dense in the same dtype, 32-byte aligned; lse (nq, Hq) float32 (natural log) or
  * null.  Rows of no sequence are not written.  Offsets that do not fit the rows raise status bit 1 and their sequences are left
- * out.  workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): its first 8192 bytes zero-filled once before its first use
+ * out, and so does work beyond 2^31 steps (64 keys for 256 query rows of a KV head; 4 KB of keys for 16 where a sequence has
+ * no more on average) in one sequence, or in 512 that follow one another; of one sequence that may have it the call is refused.
+ * workspace (kvb_cross_workspace(d) bytes, 256-byte aligned): its first 8192 bytes zero-filled once before its first use
  * and then reused (every call leaves its counters at zero), one per stream that runs calls concurrently; of host threads that
  * share one (and its stream) only one at a time may be inside the call, whose launches hand data to one another through it. */
 size_t kvb_cross_workspace(int d);

@@ -88,17 +88,18 @@ kvb_status kvb_cross_attention(const void* q, const void* k, const void* v, int 
     if (nk > 1 && (k_row == 0 || v_row == 0)) return fail(KVB_EUNSUPPORTED, "cross_attention: key and value rows of their own (row strides above 0)");
     if (!aligned(q, 16) || !aligned(k, 16) || !aligned(v, 16) || !aligned(out, 32) || !aligned(lse, 4))
         return fail(KVB_EINVAL, "cross_attention: q, k and v need 16-byte alignment, out 32-byte, lse 4-byte");
-    if (workspace_bytes < kvb_cross_workspace(d) || !aligned(workspace, 256))
-        return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
     kvb::CrossParams a{};
     a.rep = Hq / Hkv;
     a.ctas = cross_ctas();
     const bool many = nq * a.rep > int64_t(kFewRows) * n;
     const int keys = many ? kvb::CM_KEYS : 2048 / d, rows = many ? 2 * kvb::CM_ROWS : kvb::CR_ROWS;
-    // units of a sequence times row groups of all fit 32 bits
-    const int64_t units = nk / keys + 2 + kvb::PD_FIXED, groups = (nq * a.rep + rows - 1) / rows + n;
-    if (nq * a.rep > INT32_MAX - 65536 || units > INT32_MAX / Hkv / groups)
+    // One sequence alone has work of 32 bits.  How the rows of several are dealt to them only the kernels see: they leave out a
+    // sequence, or the up to CR_MAX_SEQS of a launch, whose work is more.
+    const int64_t units = nk / keys + 2 + kvb::PD_FIXED, groups = (nq * a.rep + rows - 1) / rows;
+    if (nq * a.rep > INT32_MAX - 65536 || (n == 1 && units > INT32_MAX / Hkv / groups))
         return fail(KVB_EUNSUPPORTED, "cross_attention: query rows times keys too many for one call");
+    if (workspace_bytes < kvb_cross_workspace(d) || !aligned(workspace, 256))
+        return fail(KVB_EINVAL, "cross_attention: workspace of %zu bytes, 256-byte aligned", kvb_cross_workspace(d));
     if (kvb_status st = cross_map(&a.tm_k, k, q, dtype, d, nk, Hkv, k_row, k_head, keys)) return st;
     if (kvb_status st = cross_map(&a.tm_v, v, q, dtype, d, nk, Hkv, v_row, v_head, keys)) return st;
     a.q = q;

@@ -80,6 +80,18 @@ __device__ __forceinline__ CrSeq cr_seq(const int32_t* cu_q, const int32_t* cu_k
     return x;
 }
 
+// Units and places of a sequence: groups of ROWS query rows of the KV heads, units of KEYS keys.  None where they do not fit 32
+// bits: it is left out.
+template <int ROWS, int KEYS, int FIXED>
+__device__ __forceinline__ void cr_work(const CrSeq& x, int rep, int Hkv, int& u, int& p) {
+    const int64_t hg = (int64_t(x.ql) * rep + ROWS - 1) / ROWS * Hkv;
+    const int units = max(1, (x.kl + KEYS - 1) / KEYS);          // without keys one empty unit: its rows are written
+    const bool fits = (int64_t(units) + FIXED) * hg <= INT_MAX;
+    if (!fits) raise_status(KVB_DEV_BOUNDS);
+    u = fits ? int(units * hg) : 0;
+    p = fits ? int((units + FIXED) * hg) : 0;
+}
+
 template <typename T, int D>
 __global__ void __launch_bounds__(32 * CR_WARPS, 1) cross_few_kernel(const __grid_constant__ CrossParams A) {
     using S = CrShape<D>;
@@ -108,12 +120,7 @@ __global__ void __launch_bounds__(32 * CR_WARPS, 1) cross_few_kernel(const __gri
     for (int i0 = 0; i0 < A.n; i0 += 32 * CR_WARPS) {
         const int i = i0 + threadIdx.x;
         int u = 0, p = 0;
-        if (i < A.n) {
-            const CrSeq x = seq_at(i);
-            const int hg = int((int64_t(x.ql) * A.rep + CR_ROWS - 1) / CR_ROWS) * A.Hkv;
-            u = max(1, (x.kl + S::KEYS - 1) / S::KEYS) * hg;     // without keys one empty unit: its rows are written
-            p = u + PD_FIXED * hg;
-        }
+        if (i < A.n) cr_work<CR_ROWS, S::KEYS, PD_FIXED>(seq_at(i), A.rep, A.Hkv, u, p);
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
             const int a = __shfl_up_sync(0xffffffffu, u, o), b = __shfl_up_sync(0xffffffffu, p, o);
@@ -131,7 +138,7 @@ __global__ void __launch_bounds__(32 * CR_WARPS, 1) cross_few_kernel(const __gri
         before_u += sum_u, before_p += sum_p;
     }
     __syncthreads();
-    bool fits = true;                                            // offsets that do not ascend may hold more work than 32 bits do
+    bool fits = true;                                            // a sum that passed 32 bits shows as one that falls
     for (int i = threadIdx.x; i < A.n; i += 32 * CR_WARPS) fits &= shares[i + 1] >= shares[i] && pre[i + 1] >= pre[i];
     if (!__syncthreads_and(fits)) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);

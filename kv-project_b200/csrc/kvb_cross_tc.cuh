@@ -38,10 +38,7 @@ struct CrossItem {
 template <int WARPS>
 __device__ __forceinline__ bool cross_plan(const CrossParams& A, int ctas, int* pre, int* shares, int (*warp_sum)[WARPS], PdPlan<true, CM_FIXED>& W) {
     if (!cm_scan<WARPS>(A.n, pre, shares, warp_sum, [&](int i, int& u, int& p) {
-            const CrSeq x = cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, i);
-            const int hg = int((int64_t(x.ql) * A.rep + 2 * CM_ROWS - 1) / (2 * CM_ROWS)) * A.Hkv;
-            u = max(1, (x.kl + CM_KEYS - 1) / CM_KEYS) * hg;     // without keys one empty unit: its rows are written
-            p = u + CM_FIXED * hg;
+            cr_work<2 * CM_ROWS, CM_KEYS, CM_FIXED>(cr_seq(A.cu_q, A.cu_k, A.nq, A.nk, i), A.rep, A.Hkv, u, p);
         })) {
         if (threadIdx.x == 0) raise_status(KVB_DEV_BOUNDS);
         return false;
