@@ -5,9 +5,11 @@
 A small random-weight decoder (attention only; no weights are shipped with this repository) runs as a server
 would run it: the prompts are packed without padding and attend causally in one call per layer
 (kvb.prefill_attention), their keys and values go into 8-bit pages (PagePool.write), each prompt is forked into
-several samples that share its full pages (PagePool.fork), the samples decode token by token (extend, share once a step, then
-write and attend_shared in every layer, which reads the shared pages once for all samples), one of them ends (free), the pool closes the holes (compact), and a follow-up question continues a finished sample
-by a chunk after its prefix (read, then prefill_attention with more keys than queries).
+several samples that share its full pages (PagePool.fork), the samples decode token by token (extend, then write and attend in
+every layer), one of them ends (free), the pool closes the holes (compact), and a follow-up question continues a finished
+sample by a chunk after its prefix (read, then prefill_attention with more keys than queries).  Behind longer prompts, or with
+more samples, a step would call PagePool.share once and attend_shared in every layer; for these few and short ones attend is
+the faster of the two.
 """
 
 import argparse
@@ -66,12 +68,11 @@ def prompt(model, pools, slots, tokens, lens):
 def step(model, pools, slots, tokens, cu, one):
     """One decode step: every sequence's next token."""
     start = pools[0].extend(slots, one)
-    shared = pools[0].share(slots)
     x = model.embed[tokens]
     for i, pool in enumerate(pools):
         q, k, v = model.split(x, i)
         pool.write(slots, start, cu, k, v)
-        x = x + pool.attend_shared(q[:, :, None], shared).view(len(slots), -1) @ model.out[i]
+        x = x + pool.attend(q[:, :, None], slots).view(len(slots), -1) @ model.out[i]
     return model.next_token(x)
 
 

@@ -431,7 +431,8 @@ class PagePool:
         and multiplied once for all.  q (n, Hq, Tq, d) -> (n, Tq, Hq, d), with return_lse also (n, Tq, Hq) float32.
         Its three launches take 25 us where attend takes 8 for two short sequences: it is for batches whose sequences hold much in
         common.  With 8 KV heads of 128 channels it is the faster one from about 100 000 tokens on, counted once per sequence, in groups
-        of 8 sequences and more (16 behind one prompt of 4096 tokens 32 us and 31, 64 of them 37 and 94, 64 behind 16384 55 and 310)."""
+        of 8 sequences and more (attend_shared and attend: 16 behind one prompt of 4096 tokens 32 us and 31, 64 of them 37 and 94, 64
+        behind 16384 55 and 310)."""
         if _elsewhere(self._index):
             with torch.cuda.device(self._index):
                 return self.attend_shared(q, shared, scaling, out, return_lse)
