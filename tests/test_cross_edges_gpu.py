@@ -46,3 +46,53 @@ def test_a_sequence_of_too_much_work_is_left_out(cuda_dev, rows):
     top = float(k[:100, 0].float().abs().max())
     e = 64 * 2.0 ** -24 * float(k[:100, 0].float().abs().sum(-1).max()) * float(q[0].float().abs().max()) / 8
     assert ((out[:2].float() - want.float()).abs() <= 2 * (2.0 ** -10 + 2.0 ** -13 + 2 * e + 100 * 2.0 ** -24) * top).all()
+
+
+def rows_of_digits(units, dtype):
+    """256 queries whose logits are 0 for the first key of every 64 and -x for the others, x from 0 to 1.5 in steps that either
+    type holds: (x, the exact log-sum-exp over `units` such 64 keys, the bound of its error).  Of the weights 2^(-x log2 e) a
+    quarter comes from the polynomial (2.8e-6), the rest from ex2.approx (2^-22), each from an argument that was rounded twice
+    (2 2^-24 x relatively); a unit's sum has at most 32 roundings in a row, the sum over units one each; the logarithm and its product
+    with the maximum 2^-22 |lse|."""
+    x = torch.arange(256, dtype=torch.float64, device="cuda") * (2.0 ** -7 if dtype == torch.bfloat16 else 1.5 / 256)
+    if dtype == torch.bfloat16:                                 # eight digits: from 1 on every second one
+        x = torch.where(x < 1, x, 1 + (x - 1).mul(64).floor() / 64).clamp(max=1.5)
+    lse = torch.log(units * (1 + 63 * torch.exp(-x)))
+    argument = 2 * 2.0 ** -24 * x
+    tol = (2.8e-6 + argument) / 4 + (2.0 ** -22 + argument) * 3 / 4 + (32 + units) * 2.0 ** -24 + 2.0 ** -22 * lse.abs()
+    return x, lse, tol
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("d,units", [(64, 16), (128, 3)])
+def test_the_log_sum_exp_keeps_the_digits_of_float32(cuda_dev, dtype, d, units):
+    import kvb
+    x, lse, tol = rows_of_digits(units, dtype)
+    q = torch.zeros(256, 1, d, dtype=dtype, device="cuda")
+    q[:, 0, 0] = -x
+    assert torch.equal(q[:, 0, 0].double(), -x) and float(tol.max()) < 1e-5
+    k = torch.zeros(64 * units, 1, d, dtype=dtype, device="cuda")
+    k[torch.arange(64 * units, device="cuda") % 64 > 0, 0, 0] = 1
+    _, got = kvb.cross_attention(q, k, k, cu_of([256]), cu_of([64 * units]), 1.0, return_lse=True)
+    bad = (got[:, 0].double() - lse).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((got[:, 0].double() - lse).abs() / tol).max()))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.bfloat16])
+def test_the_log_sum_exp_of_shared_pages_keeps_the_digits_of_float32(cuda_dev, dtype):
+    import kvb
+    x, lse, tol = rows_of_digits(16, dtype)
+    pool = kvb.PagePool.create(20, 1, 64, 64, n_slots=32, max_blocks=16)
+    pool.table[:] = torch.arange(16, dtype=torch.int32, device="cuda")
+    pool.lens.fill_(1024)
+    pool.refs[:16] = 32
+    pool.kc[:, :, 1:, 0] = 129
+    pool.ks.fill_(1)
+    pool.vs.fill_(0.01)
+    q = torch.zeros(256, 64, dtype=dtype, device="cuda")
+    q[:, 0] = -x
+    s = pool.share(torch.arange(32, dtype=torch.int32, device="cuda"))
+    assert s.segments[0].tolist() == [0, 32, 0, 1024, 0]
+    _, got = pool.attend_shared(q.view(32, 8, 1, 64), s, 1.0, return_lse=True)
+    bad = (got.view(256).double() - lse).abs() > tol
+    assert not bad.any(), (int(bad.sum()), float(((got.view(256).double() - lse).abs() / tol).max()))

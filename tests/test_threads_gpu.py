@@ -71,3 +71,47 @@ def test_attend_shared(cuda_dev):
         jobs.append((call, call()))
     torch.cuda.synchronize()
     together(jobs, 300)
+
+
+def test_a_pool_that_two_threads_change(cuda_dev):
+    """One thread grows and frees its sequences, the other forks, frees and compacts: what is held is told by the table, and the
+    sequences that stay keep their rows."""
+    import kvb
+    g = torch.Generator(device="cuda").manual_seed(3)
+    pool = kvb.PagePool.create(400, 2, 64, 16, n_slots=40, max_blocks=40)
+    layer = pool.add_layer()
+    stay, mine, forks = ints(range(8)), ints(range(8, 16)), ints(range(16, 24))
+    lens = [100 + 7 * i for i in range(8)]
+    cu = ints(np.concatenate([[0], np.cumsum(lens)]))
+    start = pool.extend(stay, ints(lens))
+    for p in (pool, layer):
+        p.write(stay, start, cu, *(torch.randn(sum(lens), 2, 64, generator=g, device="cuda").half() for _ in "kv"))
+    zero, before = ints([0] * 8), []
+    for p in (pool, layer):
+        before += p.read(stay, zero, cu, sum(lens))
+    add, ca = ints([21] * 8), ints(np.arange(9) * 21)
+    k, v = (torch.randn(8 * 21, 2, 64, generator=g, device="cuda").half() for _ in "kv")
+
+    def grow():
+        at = pool.extend(mine, add)
+        for p in (pool, layer):
+            p.write(mine, at, ca, k, v)
+        pool.free(mine)
+        return ()
+
+    def move():
+        pool.fork(stay, forks)
+        pool.free(stay[:4])
+        pool.fork(forks[:4], stay[:4])
+        pool.free(forks)
+        pool.compact()
+        return ()
+
+    torch.cuda.synchronize()
+    together([(grow, ()), (move, ())], 200)
+    after = []
+    for p in (pool, layer):
+        after += p.read(stay, zero, cu, sum(lens))
+    assert all(torch.equal(x, y) for x, y in zip(before, after))
+    held = torch.bincount(pool.table[pool.table >= 0].long(), minlength=400)
+    assert torch.equal(held, pool.refs.long()) and pool.lens.tolist() == lens + [0] * 32
