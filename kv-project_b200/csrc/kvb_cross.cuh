@@ -15,7 +15,7 @@
 // the sequence has those rows zeroed in shared memory first.
 //
 // Bound by HBM where there is enough to read: 48 single queries over 257 to 7258 keys (665 MB, 8 KV heads of 128 channels,
-// bfloat16) take 113 us, 5.9 TB/s, 0.90 of the rate of a copy; tensor cores 19 % busy, issue slots 22 %.  One query over 1500
+// bfloat16) take 115 us, 5.8 TB/s, 0.88 of the rate of a copy; tensor cores 19 % busy, issue slots 22 %.  One query over 1500
 // keys takes 10 us: the offsets, the first copies and the joining, one after the other.
 #pragma once
 #include <cuda.h>
