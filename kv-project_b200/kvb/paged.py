@@ -141,7 +141,7 @@ def _cross_workspace(lib, device, stream: int, d: int):
     launches hand partial sums to one another through it, and the library's calls run without the interpreter's lock."""
     own = None if torch._C._cuda_isCurrentStreamCapturing() else _CROSS_WS.get((device.index, stream, d))
     if own is None:
-        own = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device), threading.Lock()
+        own = _fresh_workspace(max(lib.kvb_cross_workspace(d), 256), _COUNTS, device), threading.RLock()
         if not torch._C._cuda_isCurrentStreamCapturing():
             _CROSS_WS[(device.index, stream, d)] = own
     return own
@@ -285,8 +285,9 @@ class PagePool:
         # held while a call's launches are enqueued: they hand data to one another through a workspace, which another thread's
         # launches between them on the same stream would overwrite (the library's calls run without the interpreter's lock); and
         # what plans with the table, then moves pages and writes it (fork, compact) must not be met halfway by what changes
-        # table or pages
-        self._lock = threading.Lock()
+        # table or pages.  Reentrant: a finalizer that frees a sequence may run inside (never between a call's launches, which are
+        # one call of the library)
+        self._lock = threading.RLock()
         self._attend_ws = {}                                            # stream: address and bytes
         self._attend_bytes = L.lib().kvb_page_attend_workspace(self._p, 1, hkv, 1)      # the same for any call
 

@@ -136,6 +136,37 @@ def test_calls_that_change_table_or_pages(paged):
              lambda: pool.attend_shared(q, shared))
 
 
+def test_a_finalizer_may_call_the_pool_inside_a_call(paged):
+    """As the collection of garbage would have it: the object whose end frees a sequence goes while a call holds the lock."""
+    paged, library = paged
+    library.one = True
+    pool, ints = pool_of(paged), lambda n: Tensor(n, dtype=torch.int32)
+    pool._lock, whole = paged.threading.RLock(), pool._workspace
+
+    class Handle:
+        def __del__(self):
+            pool.free(ints(3))
+
+    def workspace(*args):
+        Handle()
+        return whole(*args)
+
+    pool._workspace = workspace
+    t = threading.Thread(target=lambda: pool.fork(ints(3), ints(3)), daemon=True)
+    t.start()
+    t.join(10)
+    assert not t.is_alive()
+    assert [x[1] for x in library.steps] == ["begins", "ends"] * 2
+
+
+def test_locks_are_reentrant(paged):
+    paged, _ = paged
+    cu = Tensor(2, dtype=torch.int32)
+    paged.cross_attention(Tensor(5, 4, 64), Tensor(9, 2, 64), Tensor(9, 2, 64), cu, cu)
+    (_, lock), = paged._CROSS_WS.values()
+    assert type(lock) is type(threading.RLock())
+
+
 def test_layers_share_the_lock(paged, monkeypatch):
     paged, _ = paged
     monkeypatch.setattr(paged.PagePool, "__init__", lambda self, *ts: vars(self).update(vars(pool_of(paged)), n_pages=1, page=16, _c=paged.L.Pages(), _n=1, _layers=(paged.L.Pages * 1)()))
