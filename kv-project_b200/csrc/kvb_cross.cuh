@@ -86,7 +86,7 @@ template <int ROWS, int KEYS, int FIXED>
 __device__ __forceinline__ void cr_work(const CrSeq& x, int rep, int Hkv, int& u, int& p) {
     const int64_t hg = (int64_t(x.ql) * rep + ROWS - 1) / ROWS * Hkv;
     const int units = max(1, (x.kl + KEYS - 1) / KEYS);          // without keys one empty unit: its rows are written
-    const bool fits = (int64_t(units) + FIXED) * hg <= INT_MAX;
+    const bool fits = hg <= INT_MAX && (int64_t(units) + FIXED) * hg <= INT_MAX;       // the product itself within 64 bits
     if (!fits) raise_status(KVB_DEV_BOUNDS);
     u = fits ? int(units * hg) : 0;
     p = fits ? int((units + FIXED) * hg) : 0;
